@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define MOSAIC_BSA_ABI_VERSION 11
+#define MOSAIC_BSA_ABI_VERSION 12
 
 #if defined(__GNUC__) || defined(__clang__)
 #define MOSAIC_API __attribute__((visibility("default")))
@@ -432,6 +432,57 @@ MOSAIC_API int mosaic_swiglu_linear_fwd(const void* x, int64_t rows, int32_t dim
 MOSAIC_API int mosaic_swiglu_linear_w13_fwd(const void* x, int64_t rows, int32_t dim, int64_t x_row_stride,
                                             const void* w13, int32_t hidden, const void* noise,
                                             int32_t noise_rows, void* out, void* stream);
+
+/* Element types of positions. */
+typedef enum {
+    MOSAIC_POS_F32 = 0,
+    MOSAIC_POS_F64 = 1,
+    MOSAIC_POS_I32 = 2,
+    MOSAIC_POS_I64 = 3
+} mosaic_position_type;
+
+#define MOSAIC_MAX_AXES 8
+
+/* How the pairs of a head are turned: by tables (cos and sin, fp32 [seq_len, head_dim / 2]
+   contiguous, one row for each token of every batch member), or, where those are NULL, by
+   positions: token n of member b has the num_axes values at positions + b stride_b + n stride_n
+   (elements of position_type, contiguous).  Axis a turns sections[a] pairs, in order; pair j of
+   its n turns by position * theta[a]^(-j / n) radians; pairs past the last section stay.  A head's
+   pair i is (2i, 2i + 1) if interleaved, else (i, i + head_dim / 2). */
+typedef struct {
+    const float* cos;
+    const float* sin;
+    const void* positions;
+    int64_t stride_b, stride_n;
+    int32_t position_type, num_axes, interleaved;
+    int32_t sections[MOSAIC_MAX_AXES];
+    double theta[MOSAIC_MAX_AXES];
+} mosaic_rotation;
+
+/* Rotary positions of q and k in one launch, after the RMS norm of each head where norm is set:
+     out = R (x * rsqrt(mean(x^2) + eps) * weight)     fp32, rounded once to dtype
+   (without norm: out = R x; weights, eps unused).  The RoPE module (primitives.py:108-135) with
+   tables, and its form for several axes.  backward = 1 turns back instead: the gradient of the
+   rotation alone (not with norm).  rotation NULL: the norm alone.  q, k: dtype [B, N, H, head_dim]
+   by strides; num_k_heads 0: q alone.  weights: optional fp32 [head_dim].  Outputs contiguous.
+   head_dim 32, 64 or 128; batch * seq_len < 2^31.  The norm has no counterpart in the reference. */
+MOSAIC_API int mosaic_qk_rotate_fwd(mosaic_bnhd q, mosaic_bnhd k, int32_t dtype, int32_t batch, int32_t seq_len,
+                                    int32_t num_q_heads, int32_t num_k_heads, int32_t head_dim,
+                                    const mosaic_rotation* rotation, int32_t backward, int32_t norm,
+                                    const float* q_weight, const float* k_weight, float eps, void* q_out,
+                                    void* k_out, void* stream);
+
+/* Gradients of mosaic_qk_rotate_fwd with norm: grad_q / grad_k are the outputs' gradients, q / k
+   the forward's inputs (all dtype, by strides); dq / dk contiguous.  q_weight_grad /
+   k_weight_grad: optional fp32 [head_dim] (written, not added to), summed in a fixed order; with
+   either, workspace of mosaic_qk_norm_bwd_workspace_size() bytes, 16-byte aligned. */
+MOSAIC_API size_t mosaic_qk_norm_bwd_workspace_size(int32_t batch, int32_t seq_len, int32_t head_dim);
+MOSAIC_API int mosaic_qk_norm_rotate_bwd(mosaic_bnhd grad_q, mosaic_bnhd grad_k, mosaic_bnhd q, mosaic_bnhd k,
+                                         int32_t dtype, int32_t batch, int32_t seq_len, int32_t num_q_heads,
+                                         int32_t num_k_heads, int32_t head_dim, const mosaic_rotation* rotation,
+                                         const float* q_weight, const float* k_weight, float eps, void* dq,
+                                         void* dk, float* q_weight_grad, float* k_weight_grad, void* workspace,
+                                         size_t workspace_bytes, void* stream);
 
 /* Name of a status code (static storage). */
 MOSAIC_API const char* mosaic_bsa_strerror(int status);

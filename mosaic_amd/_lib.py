@@ -12,7 +12,7 @@ import threading
 
 LIB_NAME = "libmosaic_bsa.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 # mosaic_bsa_mode
 MODE_FULL = 0
@@ -37,6 +37,13 @@ NOALLOC_SCRATCH_BYTES = 128 << 20
 # mosaic_dtype
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+
+# mosaic_position_type, MOSAIC_MAX_AXES
+POS_F32 = 0
+POS_F64 = 1
+POS_I32 = 2
+POS_I64 = 3
+MAX_AXES = 8
 
 EXPORTED_SYMBOLS = (
     "mosaic_bsa_workspace_size",
@@ -66,6 +73,9 @@ EXPORTED_SYMBOLS = (
     "mosaic_pool_mean_fwd",
     "mosaic_attn_topk_workspace_size",
     "mosaic_attn_topk_fwd",
+    "mosaic_qk_rotate_fwd",
+    "mosaic_qk_norm_bwd_workspace_size",
+    "mosaic_qk_norm_rotate_bwd",
     "mosaic_bsa_strerror",
     "mosaic_bsa_abi_version",
 )
@@ -108,6 +118,15 @@ class ProjArgs(ctypes.Structure):
         ("dim", ctypes.c_int32), ("weight_rows", ctypes.c_int32), ("weight", ctypes.c_void_p),
         ("rope_cos", ctypes.c_void_p), ("rope_sin", ctypes.c_void_p),
         ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+    ]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [
+        ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64), ("stride_n", ctypes.c_int64),
+        ("position_type", ctypes.c_int32), ("num_axes", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * MAX_AXES), ("theta", ctypes.c_double * MAX_AXES),
     ]
 
 
@@ -182,6 +201,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mosaic_attn_topk_fwd.argtypes = [Bnhd, Bnhd, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp,
                                          c_size, c_vp]
     lib.mosaic_attn_topk_fwd.restype = c_int
+    lib.mosaic_qk_rotate_fwd.argtypes = [Bnhd, Bnhd, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, P(Rotation), c_i32,
+                                         c_i32, c_vp, c_vp, c_f, c_vp, c_vp, c_vp]
+    lib.mosaic_qk_rotate_fwd.restype = c_int
+    lib.mosaic_qk_norm_bwd_workspace_size.argtypes = [c_i32, c_i32, c_i32]
+    lib.mosaic_qk_norm_bwd_workspace_size.restype = c_size
+    lib.mosaic_qk_norm_rotate_bwd.argtypes = [Bnhd, Bnhd, Bnhd, Bnhd, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
+                                              P(Rotation), c_vp, c_vp, c_f, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]
+    lib.mosaic_qk_norm_rotate_bwd.restype = c_int
     lib.mosaic_bsa_strerror.argtypes = [c_int]
     lib.mosaic_bsa_strerror.restype = ctypes.c_char_p
     lib.mosaic_bsa_abi_version.argtypes = []

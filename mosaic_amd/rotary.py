@@ -1,0 +1,280 @@
+"""Rotary positions with several axes, and the norm of query and key heads with their rotation.
+
+* ``rope_axes(q, k, positions, sections, theta)``: each head's pairs of dimensions turned by angles
+  from a position of several axes (time, longitude, latitude; frame, row, column), where the
+  reference's ``RoPE`` (primitives.py:108-135) has two axes in precomputed tables.
+* ``qk_norm_rope(q, k, q_weight, k_weight, ...)``: the RMS norm of every query and key head and its
+  rotation, by tables or by positions, in the same pass over q and k.  ``MosaicAttention`` calls it
+  where its config sets ``head_norm``.
+
+q is [B, N, Hq, d] and k [B, N, Hk, d] (or None), both bfloat16 or both float32, d 32, 64 or 128,
+any strides with contiguous rows; outputs are new contiguous tensors of q's type.  Both ops are
+differentiable once: in q, k and the weights, not in positions or tables.  They enqueue on the
+current stream of q's device and never synchronise the host.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from . import _lib
+from .ops import stream_of
+
+__all__ = ["rope_axes", "qk_norm_rope"]
+
+_DT = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+_POS = {torch.float32: _lib.POS_F32, torch.float64: _lib.POS_F64, torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
+_WIDER = {torch.float16: torch.float32, torch.bfloat16: torch.float32, torch.int16: torch.int32,
+          torch.int8: torch.int32, torch.uint8: torch.int32}
+
+
+def _heads(what: str, q: torch.Tensor, k: torch.Tensor | None):
+    """The checks of q and k that need no device."""
+    for name, t in (("q", q), ("k", k)):
+        if t is None and name == "k":
+            continue
+        if t.dim() != 4:
+            raise ValueError(f"{what}: {name} must be [B, N, H, d], got shape {tuple(t.shape)}")
+        if t.dtype not in _DT:
+            raise TypeError(f"{what}: {name} is {t.dtype}; bfloat16 and float32 are computed")
+    if q.shape[3] not in (32, 64, 128):
+        raise ValueError(f"{what}: head_dim must be 32, 64 or 128, got {q.shape[3]}")
+    if q.shape[2] == 0 or (k is not None and k.shape[2] == 0):
+        raise ValueError(f"{what}: q and k need a head")
+    if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype):
+        raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} disagree")
+    if q.shape[0] * q.shape[1] >= 1 << 31:
+        raise ValueError(f"{what}: B * N must be below 2^31")
+
+
+def _no_grad_through(what: str, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no gradient in {name}: pass it detached")
+
+
+def _same_device(what: str, q: torch.Tensor, **tensors) -> None:
+    if q.device.type != "cuda":
+        raise ValueError(f"{what}: q must be on a ROCm device, got {q.device}")
+    for name, t in tensors.items():
+        if t is not None and t.device != q.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, q on {q.device}")
+
+
+def _strides(t: torch.Tensor) -> list[int]:
+    """Strides with those of single-element dimensions, which address nothing, as 0."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous, 16-byte aligned rows (copied only where they are not)."""
+    unit = 4 if t.dtype == torch.float32 else 8
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % unit for s in _strides(t)[:3]):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _bnhd(t: torch.Tensor | None) -> _lib.Bnhd:
+    return _lib.Bnhd() if t is None else _lib.Bnhd(t.data_ptr(), *_strides(t)[:3])
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=64)
+def _axes(sections: tuple, theta: tuple):
+    n = len(sections)
+    pad = (0,) * (_lib.MAX_AXES - n)
+    return (ctypes.c_int32 * _lib.MAX_AXES)(*(sections + pad)), (ctypes.c_double * _lib.MAX_AXES)(*(theta + pad))
+
+
+def _positions(what: str, q: torch.Tensor, positions: torch.Tensor, sections, theta):
+    """(positions as the kernel takes them, sections, theta for each axis), checked."""
+    sections = tuple(int(n) for n in sections)
+    B, N, d = q.shape[0], q.shape[1], q.shape[3]
+    if not 1 <= len(sections) <= _lib.MAX_AXES or min(sections) < 0 or sum(sections) > d // 2:
+        raise ValueError(f"{what}: sections {sections} must be 1 to {_lib.MAX_AXES} counts of pairs, at most {d // 2} together")
+    theta = tuple(float(x) for x in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(sections)
+    if len(theta) != len(sections) or not all(0 < x < math.inf for x in theta):
+        raise ValueError(f"{what}: theta must be a positive number, or one for each of the {len(sections)} axes")
+    if tuple(positions.shape) not in ((N, len(sections)), (B, N, len(sections)), (1, N, len(sections))):
+        raise ValueError(f"{what}: positions {tuple(positions.shape)} must be [N, axes] or [B, N, axes] = "
+                         f"{(B, N, len(sections))}")
+    if positions.dtype in _WIDER:
+        positions = positions.to(_WIDER[positions.dtype])
+    if positions.dtype not in _POS:
+        raise TypeError(f"{what}: positions are {positions.dtype}; floating and integer types are taken")
+    if positions.shape[-1] > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    return positions, sections, theta
+
+
+def _tables(what: str, q: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
+    want = (q.shape[1], q.shape[3] // 2)
+    if tuple(cos.shape) != want or tuple(sin.shape) != want:
+        raise ValueError(f"{what}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [N, d/2] = {want}")
+    made = []
+    for t in (cos, sin):
+        t = t.to(torch.float32).contiguous()
+        made.append(t.clone() if t.data_ptr() % 16 else t)
+    return made
+
+
+def _rotation(cos, sin, positions, sections, theta, interleaved: bool) -> _lib.Rotation | None:
+    r = _lib.Rotation()
+    r.interleaved = 1 if interleaved else 0
+    if cos is not None:
+        r.cos, r.sin = cos.data_ptr(), sin.data_ptr()
+        return r
+    if positions is None:
+        return None
+    st = _strides(positions)
+    r.positions, r.position_type, r.num_axes = positions.data_ptr(), _POS[positions.dtype], len(sections)
+    r.stride_b, r.stride_n = (0 if positions.dim() == 2 else st[0]), st[-2]
+    r.sections, r.theta = _axes(sections, theta)
+    return r
+
+
+def _rotate(q, k, rotation, backward: bool, norm: bool, wq=None, wk=None, eps: float = 0.0):
+    """mosaic_qk_rotate_fwd on q and k (k may be None)."""
+    B, N, Hq, d = q.shape
+    Hk = 0 if k is None else k.shape[2]
+    q_out = torch.empty(B, N, Hq, d, dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(B, N, Hk, d, dtype=q.dtype, device=q.device)
+    if B * N == 0:
+        return q_out, k_out
+    q, k = _rows(q), None if k is None else _rows(k)
+    with torch.cuda.device(q.device):
+        st = _lib.lib().mosaic_qk_rotate_fwd(
+            _bnhd(q), _bnhd(k), _DT[q.dtype], B, N, Hq, Hk, d, None if rotation is None else ctypes.byref(rotation),
+            int(backward), int(norm), _ptr(wq), _ptr(wk), eps, q_out.data_ptr(), _ptr(k_out), stream_of(q))
+    _lib.check(st, "mosaic_qk_rotate_fwd")
+    return q_out, k_out
+
+
+class _RopeAxes(torch.autograd.Function):
+    """The rotation; its gradient is the rotation back."""
+
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, q, k, positions, sections, theta, interleaved):
+        ctx.save_for_backward(positions)
+        ctx.rest = (sections, theta, interleaved)
+        return _rotate(q, k, _rotation(None, None, positions, *ctx.rest), False, False)
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        (positions,) = ctx.saved_tensors
+        dq, dk = _rotate(gq, gk, _rotation(None, None, positions, *ctx.rest), True, False)
+        return dq, dk, None, None, None, None
+
+
+def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, sections, theta=10000.0, *,
+              interleaved: bool = True):
+    """q and k with each pair of dimensions turned by its axis of the position: ``(q', k')``.
+
+    ``positions`` [N, axes] or [B, N, axes], floating or integer, on q's device.  ``sections``: the
+    pairs of each axis, in order; pair j of an axis with n pairs turns by ``position *
+    theta ** (-j / n)`` radians (``theta`` a number, or one for each axis), and pairs past the last
+    section stay as they are.  The angle is formed in 64 bits and reduced there, so far positions
+    keep it.  ``interleaved``: pair i is dimensions (2i, 2i + 1), else (i, i + d/2).
+
+    ``rope_axes(q, k, deg2rad(grid), (d/4, d/4))`` is the reference's RoPE on that (longitude,
+    latitude) grid (primitives.py:115-135), up to the rounding of its fp32 tables.
+    """
+    _heads("rope_axes", q, k)
+    _no_grad_through("rope_axes", positions=positions)
+    positions, sections, theta = _positions("rope_axes", q, positions, sections, theta)
+    _same_device("rope_axes", q, k=k, positions=positions)
+    return _RopeAxes.apply(q, k, positions, sections, theta, bool(interleaved))
+
+
+class _QkNormRope(torch.autograd.Function):
+    """The norm and rotation; the backward reads q and k again and forms the norms anew."""
+
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, q, k, q_weight, k_weight, eps, cos, sin, positions, sections, theta, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.rest = (sections, theta, interleaved)
+        ctx.eps = eps
+        wq, wk = (None if w is None else w.to(torch.float32).contiguous() for w in (q_weight, k_weight))
+        return _rotate(q, k, _rotation(cos, sin, positions, *ctx.rest), False, True, wq, wk, eps)
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        B, N, Hq, d = q.shape
+        Hk = 0 if k is None else k.shape[2]
+        dev = q.device
+        dq = torch.empty(B, N, Hq, d, dtype=q.dtype, device=dev)
+        dk = None if k is None else torch.empty(B, N, Hk, d, dtype=q.dtype, device=dev)
+        weights = (q_weight, k_weight)
+        dw = [torch.zeros(d, dtype=torch.float32, device=dev) if B * N == 0 else
+              torch.empty(d, dtype=torch.float32, device=dev) if w is not None and need else None
+              for w, need in zip(weights, ctx.needs_input_grad[2:4])]
+        if B * N:
+            wq, wk = (None if w is None else w.to(torch.float32).contiguous() for w in weights)
+            gq, q = _rows(gq.to(q.dtype)), _rows(q)
+            gk, k = (None, None) if k is None else (_rows(gk.to(k.dtype)), _rows(k))
+            rotation = _rotation(cos, sin, positions, *ctx.rest)
+            L = _lib.lib()
+            nbytes = L.mosaic_qk_norm_bwd_workspace_size(B, N, d)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if any(w is not None for w in dw) else None
+            with torch.cuda.device(dev):
+                st = L.mosaic_qk_norm_rotate_bwd(
+                    _bnhd(gq), _bnhd(gk), _bnhd(q), _bnhd(k), _DT[q.dtype], B, N, Hq, Hk, d,
+                    None if rotation is None else ctypes.byref(rotation), _ptr(wq), _ptr(wk), ctx.eps, dq.data_ptr(),
+                    _ptr(dk), _ptr(dw[0]), _ptr(dw[1]), _ptr(ws), nbytes if ws is not None else 0, stream_of(q))
+            _lib.check(st, "mosaic_qk_norm_rotate_bwd")
+        dw = [None if g is None or w is None else g.to(w.dtype) for g, w in zip(dw, weights)]
+        return (dq, dk, *dw) + (None,) * 7
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None = None,
+                 k_weight: torch.Tensor | None = None, *, eps: float | None = None, cos: torch.Tensor | None = None,
+                 sin: torch.Tensor | None = None, positions: torch.Tensor | None = None, sections=None,
+                 theta=10000.0, interleaved: bool = True):
+    """The RMS norm of every head of q and k over its d dimensions, then its rotation: ``(q', k')``.
+
+    ``y = R (w * x * rsqrt(mean(x^2) + eps))`` with the statistics in fp32 and one rounding, of y.
+    ``q_weight`` / ``k_weight`` [d] are shared by all heads (None: ones); ``eps`` None is torch's
+    RMSNorm default, the epsilon of fp32.  The rotation comes from ``cos`` / ``sin`` (the RoPE
+    module's tables, [N, d/2]), or from ``positions`` and ``sections`` as in ``rope_axes``, or is
+    left out where neither is given.
+    """
+    what = "qk_norm_rope"
+    _heads(what, q, k)
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{what}: cos and sin go together")
+    if (positions is None) != (sections is None):
+        raise ValueError(f"{what}: positions and sections go together")
+    if cos is not None and positions is not None:
+        raise ValueError(f"{what}: tables or positions, not both")
+    if k is None and k_weight is not None:
+        raise ValueError(f"{what}: k_weight without k")
+    eps = torch.finfo(torch.float32).eps if eps is None else float(eps)
+    if not 0 <= eps < math.inf:
+        raise ValueError(f"{what}: eps must not be negative, got {eps}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and tuple(w.shape) != (q.shape[3],):
+            raise ValueError(f"{what}: {name} {tuple(w.shape)} must be [d] = ({q.shape[3]},)")
+        if w is not None and not w.dtype.is_floating_point:
+            raise TypeError(f"{what}: {name} is {w.dtype}")
+    _no_grad_through(what, cos=cos, sin=sin, positions=positions)
+    if cos is not None:
+        cos, sin = _tables(what, q, cos, sin)
+        theta = ()
+    elif positions is not None:
+        positions, sections, theta = _positions(what, q, positions, sections, theta)
+    _same_device(what, q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
+    return _QkNormRope.apply(q, k, q_weight, k_weight, eps, cos, sin, positions, sections, theta, bool(interleaved))
