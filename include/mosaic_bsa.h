@@ -484,6 +484,18 @@ MOSAIC_API int mosaic_qk_norm_rotate_bwd(mosaic_bnhd grad_q, mosaic_bnhd grad_k,
                                          void* dk, float* q_weight_grad, float* k_weight_grad, void* workspace,
                                          size_t workspace_bytes, void* stream);
 
+/* The key blocks of each query token.  Row (b, n, h): score[u] = sum over the query heads g of kv
+   head h's group of q[b, n, g] . k_cmp[b, u, h]; indices_out[b, n, h, :] = the block_count blocks
+   of the largest (exact) scores, ties to the lower block, in ascending order, -1 past the last.
+   block_mask: optional [batch, num_blocks] bytes, 0 for blocks that are never taken.  q: bf16
+   [B, Nq, Hq, 64]; k_cmp: bf16 [B, nb, Hk, 64]; indices_out: int64 [B, Nq, Hk, K] contiguous.
+   block_count at most 64, at most 16 query heads per kv head.  Scores that are NaN are not
+   taken.  attn_topk (primitives.py:35-51) is the counterpart for query blocks. */
+MOSAIC_API int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uint8_t* block_mask, int32_t batch,
+                                     int32_t num_queries, int32_t num_blocks, int32_t num_q_heads,
+                                     int32_t num_kv_heads, int32_t head_dim, int32_t block_count,
+                                     int64_t* indices_out, void* stream);
+
 /* Name of a status code (static storage). */
 MOSAIC_API const char* mosaic_bsa_strerror(int status);
 

@@ -76,6 +76,7 @@ EXPORTED_SYMBOLS = (
     "mosaic_qk_rotate_fwd",
     "mosaic_qk_norm_bwd_workspace_size",
     "mosaic_qk_norm_rotate_bwd",
+    "mosaic_query_topk_fwd",
     "mosaic_bsa_strerror",
     "mosaic_bsa_abi_version",
 )
@@ -209,6 +210,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mosaic_qk_norm_rotate_bwd.argtypes = [Bnhd, Bnhd, Bnhd, Bnhd, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                               P(Rotation), c_vp, c_vp, c_f, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]
     lib.mosaic_qk_norm_rotate_bwd.restype = c_int
+    lib.mosaic_query_topk_fwd.argtypes = [Bnhd, Bnhd, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]
+    lib.mosaic_query_topk_fwd.restype = c_int
     lib.mosaic_bsa_strerror.argtypes = [c_int]
     lib.mosaic_bsa_strerror.restype = ctypes.c_char_p
     lib.mosaic_bsa_abi_version.argtypes = []
