@@ -496,6 +496,38 @@ MOSAIC_API int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uin
                                      int32_t num_kv_heads, int32_t head_dim, int32_t block_count,
                                      int64_t* indices_out, void* stream);
 
+/* Attention of each query token over its own key blocks.  Row (b, n, h): the softmax over the keys
+   of the blocks named in block_indices[b, n, h, :] -- a set: repeated entries count once, entries
+   outside [0, ceil(num_keys / block_size)) not at all -- below the sequence's length kv_lens[b]
+   (optional, clamped to [0, num_keys]; NULL: num_keys); a row without a key is zeros, its lse -inf.
+   What a row has not chosen does not reach it, whatever it holds.  q: bf16 [B, Nq, Hq, 64]; k, v:
+   bf16 [B, Nk, Hk, 64]; block_indices: int64 [B, Nq, Hk, K] contiguous; out: bf16 [B, Nq, Hq, 64]
+   contiguous; lse: optional fp32 [B, Nq, Hq], base 2 of the scaled logits.  block_size a multiple
+   of 64 (the last block may be short), at most 16 query heads per kv head, K at most 1024.
+   workspace: mosaic_query_attn_fwd_workspace_size() bytes (0 for many queries), 256-byte aligned.
+   softmax_scale <= 0 selects 64^-0.5.  mosaic_sparse_attn (ops.py:557-566) is the counterpart for
+   query blocks. */
+MOSAIC_API size_t mosaic_query_attn_fwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_q_heads,
+                                                       int32_t num_kv_heads, int32_t block_count);
+MOSAIC_API int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int64_t* block_indices,
+                                     const int32_t* kv_lens, int32_t batch, int32_t num_queries, int32_t num_keys,
+                                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                     int32_t block_count, float softmax_scale, void* out, float* lse,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of mosaic_query_attn_fwd from its out and lse: grad_q [B, Nq, Hq, 64], grad_k, grad_v
+   [B, Nk, Hk, 64], bf16 contiguous, every row written (zeros for keys nobody chose or past a
+   sequence's end), sums in a fixed order.  workspace: mosaic_query_attn_bwd_workspace_size()
+   bytes, 256-byte aligned. */
+MOSAIC_API size_t mosaic_query_attn_bwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_keys,
+                                                       int32_t num_q_heads, int32_t num_kv_heads, int32_t block_size);
+MOSAIC_API int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const void* out, const float* lse,
+                                     mosaic_bnhd grad_out, const int64_t* block_indices, const int32_t* kv_lens,
+                                     int32_t batch, int32_t num_queries, int32_t num_keys, int32_t num_q_heads,
+                                     int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t block_count,
+                                     float softmax_scale, void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 /* Name of a status code (static storage). */
 MOSAIC_API const char* mosaic_bsa_strerror(int status);
 

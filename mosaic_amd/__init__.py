@@ -20,7 +20,7 @@ from .primitives import (
     pool_mean,
     stack_projection_weight,
 )
-from .query import query_topk
+from .query import mosaic_query_attn, query_sparse_attn, query_topk
 from .rotary import qk_norm_rope, rope_axes
 from .healpix import get_healpix_grid, pix2ang_nest
 
@@ -28,6 +28,6 @@ __all__ = [
     "MosaicAttnFunction", "mosaic_attn_bwd", "mosaic_attn_fwd", "mosaic_sparse_attn", "MosaicAttention", "RoPE",
     "attn_topk", "block_attention", "dense_attention", "mosaic_attn_func", "mosaic_attn_func_rope", "mosaic_attn_proj",
     "stack_projection_weight", "pool_mean",
-    "query_topk", "rope_axes", "qk_norm_rope",
+    "query_topk", "query_sparse_attn", "mosaic_query_attn", "rope_axes", "qk_norm_rope",
     "get_healpix_grid", "pix2ang_nest",
 ]

@@ -77,6 +77,10 @@ EXPORTED_SYMBOLS = (
     "mosaic_qk_norm_bwd_workspace_size",
     "mosaic_qk_norm_rotate_bwd",
     "mosaic_query_topk_fwd",
+    "mosaic_query_attn_fwd_workspace_size",
+    "mosaic_query_attn_fwd",
+    "mosaic_query_attn_bwd_workspace_size",
+    "mosaic_query_attn_bwd",
     "mosaic_bsa_strerror",
     "mosaic_bsa_abi_version",
 )
@@ -212,6 +216,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mosaic_qk_norm_rotate_bwd.restype = c_int
     lib.mosaic_query_topk_fwd.argtypes = [Bnhd, Bnhd, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]
     lib.mosaic_query_topk_fwd.restype = c_int
+    lib.mosaic_query_attn_fwd_workspace_size.argtypes = [c_i32] * 5
+    lib.mosaic_query_attn_fwd_workspace_size.restype = c_size
+    lib.mosaic_query_attn_fwd.argtypes = [Bnhd, Bnhd, Bnhd, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
+                                          c_i32, c_f, c_vp, c_vp, c_vp, c_size, c_vp]
+    lib.mosaic_query_attn_fwd.restype = c_int
+    lib.mosaic_query_attn_bwd_workspace_size.argtypes = [c_i32] * 6
+    lib.mosaic_query_attn_bwd_workspace_size.restype = c_size
+    lib.mosaic_query_attn_bwd.argtypes = [Bnhd, Bnhd, Bnhd, c_vp, c_vp, Bnhd, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32,
+                                          c_i32, c_i32, c_i32, c_i32, c_f, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]
+    lib.mosaic_query_attn_bwd.restype = c_int
     lib.mosaic_bsa_strerror.argtypes = [c_int]
     lib.mosaic_bsa_strerror.restype = ctypes.c_char_p
     lib.mosaic_bsa_abi_version.argtypes = []

@@ -32,6 +32,7 @@
 #include <cstdint>
 
 #include "bsa_common.h"
+#include "lds_dma.h"
 #include "mosaic_bsa.h"
 
 namespace mosaic {
@@ -75,14 +76,6 @@ typedef short v4i16 __attribute__((ext_vector_type(4)));
 constexpr int kTileElems = 64 * 64;
 typedef __attribute__((address_space(3))) void lds_void;
 
-__device__ __forceinline__ void wait_vmem() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-// Workgroup barrier for LDS data whose direct-to-LDS loads each wave has already waited for
-// itself: __syncthreads() would also wait for every load still in flight (its release fence
-// covers the loads' LDS writes), which takes the prefetch of the next step out of the overlap.
-// The memory clobber keeps the compiler from moving LDS accesses across it; lgkmcnt(0) retires
-// this wave's LDS reads of the slot that is refilled after the barrier.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
 // LDS layout of the backward's 64-row tiles: 128-byte rows, chunk c of row r at position
 // c ^ bwd_swz(r).  The tiles are read both along rows (ds_read_b128 of one chunk of 16
 // consecutive rows) and transposed (ds_read_b64_tr_b16 of two chunks of 4 consecutive rows,
@@ -104,27 +97,6 @@ __device__ __forceinline__ void tile_dma_init(uint32_t* dk, uint32_t* dv, int wa
     }
 }
 
-// Direct-to-LDS loads issued as inline assembly, address = base (uniform) + voff (per lane),
-// LDS destination M0 + 16 l (dwordx4) or M0 + 4 l (dword) for lane l.  The compiler's wait
-// insertion does not see them: across the joins of a ring loop its tracking of which LDS
-// object a direct-to-LDS load writes becomes conservative, and it waited for the loads just
-// requested for a later step before the current step's LDS reads.  The caller waits for these
-// loads (s_waitcnt vmcnt) and synchronises the workgroup itself.  M0 is declared clobbered;
-// the compiler sets M0 again before each of its own uses, so nothing it holds is lost.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ uint32_t lds_addr(const void* ptr) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)ptr;
-}
-__device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds)
-                 : "memory", "m0");
-}
-__device__ __forceinline__ void dma4(const void* base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
 // One 64-row tile's direct-to-LDS loads (offsets from tile_dma_init), issued as dma16
 template <int NW>
 __device__ __forceinline__ void tile_dma(const uint32_t* dk, const uint32_t* dv, const bf16_t* kb, const bf16_t* vb,

@@ -6,6 +6,9 @@ need not lie on the mesh: stations, points of another grid, one token.
 
 * ``query_topk(q, k_cmp, block_count, block_mask=None)``: the blocks of the largest scores of each
   query token and kv head against pooled keys.
+* ``query_sparse_attn(q, k, v, block_indices, block_size, softmax_scale=None, kv_lens=None)``:
+  attention of each query token over its blocks, differentiable in q, k and v.
+* ``mosaic_query_attn(q, k, v, block_size, block_count, ...)``: both, on keys it pools itself.
 
 q is [B, Nq, Hq, 64], keys [B, Nk, Hk, 64], Hq a multiple of Hk with at most 16 query heads per kv
 head.  The computation is bf16 with fp32 statistics; fp32 inputs are converted and fp16 is refused,
@@ -15,13 +18,16 @@ synchronise the host.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
 from .ops import stream_of
-from .rotary import _bnhd, _rows, _same_device
+from .primitives import _workspace, pool_mean
+from .rotary import _bnhd, _ptr, _rows, _same_device
 
-__all__ = ["query_topk"]
+__all__ = ["query_topk", "query_sparse_attn", "mosaic_query_attn"]
 
 
 def _bf16_heads(what: str, **tensors) -> None:
@@ -81,3 +87,127 @@ def query_topk(q: torch.Tensor, k_cmp: torch.Tensor, block_count: int, block_mas
                                               Hq, Hk, d, block_count, idx.data_ptr(), stream_of(q))
     _lib.check(st, "mosaic_query_topk_fwd")
     return idx
+
+
+def _attn_fwd(q, k, v, idx, block_size, scale, lens, want_lse):
+    """(output bf16 [B, Nq, Hq, 64], lse fp32 [B, Nq, Hq] or None) of bf16 rows."""
+    B, Nq, Hq, d = q.shape
+    Nk, Hk = k.shape[1:3]
+    K = idx.shape[-1]
+    out = torch.empty(B, Nq, Hq, d, dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty(B, Nq, Hq, dtype=torch.float32, device=q.device) if want_lse else None
+    L = _lib.lib()
+    nbytes = L.mosaic_query_attn_fwd_workspace_size(B, Nq, Hq, Hk, K)
+    ws = _workspace(nbytes, q.device) if nbytes else None
+    with torch.cuda.device(q.device):
+        st = L.mosaic_query_attn_fwd(_bnhd(q), _bnhd(k), _bnhd(v), idx.data_ptr(), _ptr(lens), B, Nq, Nk, Hq, Hk, d, block_size,
+                                     K, scale, out.data_ptr(), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel(), stream_of(q))
+    _lib.check(st, "mosaic_query_attn_fwd")
+    return out, lse
+
+
+class _QueryAttn(torch.autograd.Function):
+    """Saves the bf16 rows the kernels read, the output and its log-sum-exp."""
+
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, q, k, v, idx, block_size, scale, lens):
+        ctx.dtypes = (q.dtype, k.dtype, v.dtype)
+        ctx.rest = (block_size, scale)
+        grad = any(ctx.needs_input_grad[:3])
+        if 0 in q.shape or 0 in k.shape or idx.shape[-1] == 0:     # no row, or no key for any
+            ctx.save_for_backward(q, k, v)
+            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        qb, kb, vb = (_as_bf16(t) for t in (q, k, v))
+        out, lse = _attn_fwd(qb, kb, vb, idx, block_size, scale, lens, grad)
+        if grad:
+            ctx.save_for_backward(qb, kb, vb, out, lse, idx, lens)
+        return out.to(q.dtype)
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        if len(ctx.saved_tensors) == 3:
+            return tuple(torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * 4
+        q, k, v, out, lse, idx, lens = ctx.saved_tensors
+        block_size, scale = ctx.rest
+        B, Nq, Hq, d = q.shape
+        Nk, Hk = k.shape[1:3]
+        go = _as_bf16(go)
+        gq = torch.empty(B, Nq, Hq, d, dtype=torch.bfloat16, device=q.device)
+        gk, gv = (torch.empty(B, Nk, Hk, d, dtype=torch.bfloat16, device=q.device) for _ in range(2))
+        L = _lib.lib()
+        ws = _workspace(L.mosaic_query_attn_bwd_workspace_size(B, Nq, Nk, Hq, Hk, block_size), q.device)
+        with torch.cuda.device(q.device):
+            st = L.mosaic_query_attn_bwd(_bnhd(q), _bnhd(k), _bnhd(v), out.data_ptr(), lse.data_ptr(), _bnhd(go), idx.data_ptr(),
+                                         _ptr(lens), B, Nq, Nk, Hq, Hk, d, block_size, idx.shape[-1], scale, gq.data_ptr(),
+                                         gk.data_ptr(), gv.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(q))
+        _lib.check(st, "mosaic_query_attn_bwd")
+        return tuple(g.to(t) for g, t in zip((gq, gk, gv), ctx.dtypes)) + (None,) * 4
+
+
+def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_indices: torch.Tensor, block_size: int,
+                      softmax_scale: float | None = None, kv_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each query token over its own key blocks: [B, Nq, Hq, 64] in q's type.
+
+    ``block_indices`` (int64 or int32 [B, Nq, Hk, K], on q's device, K at most 1024) names, for each
+    query token and kv head, blocks of ``block_size`` keys (a multiple of 64; the last block of k may
+    be short).  It is a set: an index counts once however often it stands there, and one outside the
+    blocks (such as -1) not at all.  ``kv_lens`` (integers [B]): keys from ``kv_lens[b]`` on are not
+    attended; what they hold does not matter.  A token without a key gets zeros.  ``softmax_scale``
+    defaults to 1/8.  Differentiable in q, k and v, once.
+    """
+    what = "query_sparse_attn"
+    _bf16_heads(what, q=q, k=k, v=v)
+    _groups(what, q, k)
+    if k.shape != v.shape:
+        raise ValueError(f"{what}: k and v shapes differ: {tuple(k.shape)} vs {tuple(v.shape)}")
+    B, Nq, Hk = q.shape[0], q.shape[1], k.shape[2]
+    if block_size <= 0 or block_size % 64:
+        raise ValueError(f"{what}: block_size must be a positive multiple of 64, got {block_size}")
+    if block_indices.dim() != 4 or tuple(block_indices.shape[:3]) != (B, Nq, Hk) or block_indices.shape[3] > 1024:
+        raise ValueError(f"{what}: block_indices {tuple(block_indices.shape)} must be [B, Nq, Hk, K] = {(B, Nq, Hk, '*')}, "
+                         "K at most 1024")
+    if block_indices.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: block_indices are {block_indices.dtype}, not int64 or int32")
+    scale = 0.125 if softmax_scale is None else float(softmax_scale)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"{what}: softmax_scale must be positive, got {softmax_scale}")
+    if kv_lens is not None:
+        if tuple(kv_lens.shape) != (B,):
+            raise ValueError(f"{what}: kv_lens {tuple(kv_lens.shape)} must be [B] = ({B},)")
+        if kv_lens.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"{what}: kv_lens are {kv_lens.dtype}, not int64 or int32")
+    _same_device(what, q, k=k, v=v, block_indices=block_indices, kv_lens=kv_lens)
+    if kv_lens is not None:   # clamped before the conversion: a far length stays one
+        kv_lens = (kv_lens if kv_lens.dtype == torch.int32 else kv_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
+    idx = block_indices.to(torch.int64).contiguous()
+    return _QueryAttn.apply(q, k, v, idx, int(block_size), scale, kv_lens)
+
+
+def mosaic_query_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_size: int, block_count: int, *,
+                      softmax_scale: float | None = None, block_mask: torch.Tensor | None = None,
+                      k_cmp: torch.Tensor | None = None, return_block_indices: bool = False):
+    """Each query token chooses ``block_count`` blocks of k and attends to them: [B, Nq, Hq, 64].
+
+    The keys' blocks are pooled by their mean (``pool_mean``), or ``k_cmp`` [B, Nk / block_size, Hk,
+    64] holds what a program pooled once for many calls; ``query_topk`` chooses (``block_mask`` bool
+    [B, nb]), ``query_sparse_attn`` attends.  Nk must be a multiple of ``block_size``.  Gradients pass
+    through the attention, not through the choice.  With ``return_block_indices`` the choice (int64
+    [B, Nq, Hk, block_count]) is returned too.
+    """
+    what = "mosaic_query_attn"
+    _bf16_heads(what, q=q, k=k, v=v)
+    if block_size <= 0 or block_size % 64 or k.shape[1] % block_size:
+        raise ValueError(f"{what}: block_size must be a multiple of 64 that divides {k.shape[1]} keys, got {block_size}")
+    nb = k.shape[1] // block_size
+    if k_cmp is None:
+        _same_device(what, q, k=k)
+        with torch.no_grad():
+            k_cmp = pool_mean(k.detach(), block_size)
+    elif k_cmp.dim() != 4 or tuple(k_cmp.shape) != (k.shape[0], nb, k.shape[2], 64):
+        raise ValueError(f"{what}: k_cmp {tuple(k_cmp.shape)} must be {(k.shape[0], nb, k.shape[2], 64)}")
+    idx = query_topk(q.detach(), k_cmp.detach(), block_count, block_mask)
+    out = query_sparse_attn(q, k, v, idx, block_size, softmax_scale)
+    return (out, idx) if return_block_indices else out
