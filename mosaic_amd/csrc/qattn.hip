@@ -7,21 +7,27 @@
 // key is zeros (lse -inf).  fp32 scores, maxima, sums and accumulators; P is rounded to bf16 for
 // the PV product (an error of half a step of bf16 per term, as the output's own rounding).
 //
-// A workgroup takes 4 waves x QW = 16 / G neighbouring tokens of one kv head, a wave the 16 rows
-// (token, head) of its tokens.  Its tokens' sets are united in LDS (one 16-bit token mask per wave
-// and block), and the union's blocks are staged once, 64 keys at a time, for all four waves; a
-// wave skips the blocks none of its tokens has.  Neighbouring tokens of a mesh mostly choose the
-// same blocks, so the union is little longer than one set, and where they do not, a wave computes
-// no more 16-row tiles than its tokens would one by one.
+// A workgroup takes 4 waves x QW = 32 / G tokens of one kv head, a wave the 32 rows (token, head) of
+// its tokens.  The tokens' sets are united in LDS (one 32-bit token mask per wave and block), and
+// the union's blocks are staged once, 64 keys at a time, for all four waves; a wave skips the blocks
+// none of its tokens has.  Neighbouring tokens of a mesh mostly choose the same blocks, so the union
+// is little longer than one set (17.4 blocks for 32 tokens with 16 each on nside 64's field).  Tokens
+// in no such order are taken in the order of a block of theirs (query_order_kernel): 10007 scattered
+// points then unite 22 blocks instead of 313.  A row's result does not depend on the tokens beside
+// it: its own blocks come in ascending order in any union.
 //
-// Per tile of 64 keys, transposed so that a lane's 16 scores are one row's
-// (v_mfma_f32_16x16x32_bf16):
+// Per tile of 64 keys, transposed so that a lane's 32 scores are one row's
+// (v_mfma_f32_32x32x16_bf16, a row in lanes r and r + 32):
 //   S^T = K Q^T    A = K rows (16-byte LDS reads),  B = q (registers)
 //   O^T = V^T P^T  A = V^T (transposing LDS reads), B = P, which S^T's accumulators already hold in
-//                  operand order (contraction index (g, i) <-> keys 4 g + i, 16 + 4 g + i - 4)
-// Rows that are no members of a block keep their state: the tile's product goes to accumulators of
-// its own and is added under the row's predicate, so nothing a row did not choose -- infinities and
-// NaN among it -- reaches it.
+//                  operand order
+// 32 rows rather than 16 per wave (v_mfma_f32_16x16x32_bf16) halve the LDS reads per score, which
+// bound that variant.  The reference m of a row moves only when a score exceeds it by 2^8; l sums
+// the rounded P, so numerator and denominator share their roundings (the
+// log-sum-exp, where one is asked for, sums P unrounded).  The tile's product goes to
+// accumulators of its own and is added under the row's predicate: rows that are no members of the
+// block keep their state, nothing a row did not choose -- infinities and NaN among it -- reaches it,
+// and its sums are the same bits whoever shares its wave.
 //
 // Few queries: the union is split over workgroups and the partial (m, l, O) joined by a second
 // kernel.
@@ -38,9 +44,12 @@ namespace mosaic {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kRowsPerWave = 32;
 constexpr int kTileElems = 64 * 64;
 constexpr int kUnion = 1024;       // blocks whose members are marked at a time
 constexpr int kMaxSplit = 32;
+constexpr int kBuckets = 4096;     // of the order of tokens
+constexpr float kTau = 8.f;        // a row's reference moves when a score exceeds it by 2^kTau
 
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 
@@ -55,21 +64,27 @@ struct QueryAttnParams {
     bf16_t* out;               // [B, Nq, Hq, 64]: the output, or grad q
     float* lse;                // [B, Nq, Hq], or null (forward: written, backward: read)
     float* part_o;             // [splits, rows, 64] (splits > 1)
-    float2* part_ml;           // [splits, rows]
+    float4* part_ml;           // [splits, rows] (m, l, l of the unrounded P, -)
     float* nlse;               // backward: -lse / c and -sum(o do) of each row
     float* ndelta;
     uint32_t* marks;           // backward: [B, Hk, nb, words] bit n: token n has the block
     bf16_t* dk; bf16_t* dv;    // [B, Nk, Hk, 64]
+    uint16_t* keys;            // [B, Hk, Nq] bucket of each token (null: tokens in their own order)
+    int32_t* order;            // [B, Hk, Nq] tokens in the order they are taken in,
+    int32_t* ordered;          // [B, Hk] where this is not 0
+    int32_t* far;              // [B, Hk, chunks of 256 tokens]
     int B, Nq, Nk, Hq, Hk, G, QW, bs, K, nb, words;
     int qtiles, splits;
+    int qw_inverse;            // t / QW = t qw_inverse >> 16 for t < 128
+    int short_rows;            // 64 rows of k and of v span less than 2^31 bytes
     float scale, c;
 };
 
-// 16-byte chunk c of row r of a 64-row tile lies at c ^ swz16(r).  Row reads take one chunk of 16
-// consecutive rows at a time: over the rows of one parity (256 bytes of banks hold two rows) it is a
-// permutation.  Transposing reads take two neighbouring chunks of 8 consecutive rows: over the four
-// of one parity its upper bits differ.
-__device__ __forceinline__ int swz16(int r) { return (((r >> 1) & 3) << 1) | ((r >> 3) & 1); }
+// LDS layout of 64-row tiles: 128-byte rows, 16-byte chunk c of row r at c ^ swz32(r).  Row reads
+// (one chunk of 16 consecutive rows at a time) and transposing reads (four chunks of 4 rows) are
+// both free of bank conflicts: over rows of one parity in 16 consecutive ones swz32 is a
+// permutation of 0..7, and rows r and r + 2 of an aligned four differ in bit 2.
+__device__ __forceinline__ int swz32(int row) { return (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
 
 __device__ __forceinline__ bf16x8 tr_pair(const bf16_t* lo, const bf16_t* hi) {
     const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -83,35 +98,156 @@ __device__ __forceinline__ int seq_keys(const QueryAttnParams& p, int b) {
     return p.lens == nullptr ? p.Nk : min(max(p.lens[b], 0), p.Nk);
 }
 
+// ------------------------------------------------------------------ the order of tokens
+// Tokens of one kv head by a block of theirs: the middle entry of the row or, where that is no
+// block, the next one that is (query_topk's rows ascend, so it is their median).
+
+__device__ __forceinline__ int bucket_of(const QueryAttnParams& p, int64_t blk) {
+    return p.nb <= kBuckets ? (int)blk : (int)(blk * kBuckets / p.nb);
+}
+
+// A workgroup takes 256 tokens of one (b, h) and counts those that lie more than a 32nd of the blocks
+// from the token before.
+__global__ __launch_bounds__(kThreads) void query_keys_kernel(QueryAttnParams p, int chunks) {
+    __shared__ int far[kWaves];
+    const int bh = blockIdx.x / chunks, chunk = blockIdx.x - bh * chunks, h = bh % p.Hk, b = bh / p.Hk;
+    const int n = chunk * kThreads + threadIdx.x, lane = threadIdx.x & 63;
+    int key = kBuckets;
+    if (n < p.Nq) {
+        const int64_t* e = p.idx + (((int64_t)b * p.Nq + n) * p.Hk + h) * p.K;
+        for (int i = 0, at = p.K / 2; i < p.K; ++i) {
+            const int64_t blk = e[at];
+            if (blk >= 0 && blk < p.nb) {
+                key = bucket_of(p, blk);
+                break;
+            }
+            at = at + 1 == p.K ? 0 : at + 1;
+        }
+        p.keys[(int64_t)bh * p.Nq + n] = (uint16_t)key;
+    }
+    const int before = __shfl_up(key, 1);
+    const uint64_t jumps = __builtin_amdgcn_ballot_w64(lane > 0 && n < p.Nq && abs(key - before) * 32 > min(p.nb, kBuckets));
+    if (lane == 0) far[threadIdx.x >> 6] = (int)__builtin_popcountll(jumps);
+    __syncthreads();
+    if (threadIdx.x == 0) p.far[blockIdx.x] = far[0] + far[1] + far[2] + far[3];
+}
+
+// One workgroup = one (b, h): a counting sort by bucket.  Where the tokens' own order is already one
+// of neighbours -- three in four lie near the token before -- it is left as it is.
+// The order within a bucket is that of the LDS atomics; nothing depends on it.
+constexpr int kOrderThreads = 1024, kOrderRun = 8;   // keys a thread has in flight
+__global__ __launch_bounds__(kOrderThreads) void query_order_kernel(QueryAttnParams p, int chunks) {
+    __shared__ int start[kBuckets + 1];
+    __shared__ int waves[kOrderThreads / 64];
+    const int tid = threadIdx.x;
+    int far = 0;
+    for (int i = tid; i < chunks; i += kOrderThreads) far += p.far[blockIdx.x * chunks + i];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) far += __shfl_xor(far, d);
+    if ((tid & 63) == 0) waves[tid >> 6] = far;
+    for (int i = tid; i <= kBuckets; i += kOrderThreads) start[i] = 0;
+    __syncthreads();
+    far = 0;
+    for (int w = 0; w < kOrderThreads / 64; ++w) far += waves[w];
+    const bool sort = far > p.Nq / 4;
+    if (tid == 0) p.ordered[blockIdx.x] = sort;
+    if (!sort) return;
+    const uint16_t* key = p.keys + (int64_t)blockIdx.x * p.Nq;
+    int32_t* out = p.order + (int64_t)blockIdx.x * p.Nq;
+    auto each = [&](auto use) {   // use(token, its key)
+        for (int i0 = tid; i0 < p.Nq; i0 += kOrderThreads * kOrderRun) {
+            int k[kOrderRun];
+#pragma unroll
+            for (int j = 0; j < kOrderRun; ++j) k[j] = key[min(i0 + j * kOrderThreads, p.Nq - 1)];
+#pragma unroll
+            for (int j = 0; j < kOrderRun; ++j)
+                if (i0 + j * kOrderThreads < p.Nq) use(i0 + j * kOrderThreads, k[j]);
+        }
+    };
+    each([&](int, int k) { atomicAdd(&start[k], 1); });
+    __syncthreads();
+    // exclusive prefix sums of the counts, 4 per thread; the last bucket is that of tokens without a block
+    int c[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        c[i] = start[4 * tid + i];
+        sum += c[i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(upto, d);
+        upto += (tid & 63) >= d ? x : 0;
+    }
+    if ((tid & 63) == 63) waves[tid >> 6] = upto;
+    __syncthreads();
+    int at = upto - sum;
+    for (int w = 0; w < tid >> 6; ++w) at += waves[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        start[4 * tid + i] = at;
+        at += c[i];
+    }
+    if (tid == kOrderThreads - 1) start[kBuckets] = at;
+    __syncthreads();
+    each([&](int n, int k) { out[atomicAdd(&start[k], 1)] = n; });
+}
+
+// ------------------------------------------------------------------ tiles of a union
+
 // LDS of the forward and grad-q kernels
 struct RowsLds {
     __attribute__((aligned(1024))) bf16_t K[2][kTileElems];
     __attribute__((aligned(1024))) bf16_t V[2][kTileElems];
-    uint32_t members[kUnion][2];   // wave w: 16 bits at 16 (w % 2) of word w / 2
+    __attribute__((aligned(16))) uint32_t members[kUnion][kWaves];   // bit t: the wave's token t has the block
     uint16_t list[kUnion];
+    int tokens[kWaves * kRowsPerWave];
     int found[kWaves];
 };
 
-// Marks the members of blocks [c0, c0 + nc) among the workgroup's tokens n0 .. and lists the
-// blocks that have any, ascending; returns their number.  Ends with a barrier.
-__device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int end, int c0, int nc) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < nc; i += kThreads) L.members[i][0] = L.members[i][1] = 0;
+// The workgroup's tokens (positions n0 .. of the order) into LDS; ends with a barrier.
+__device__ __forceinline__ void load_tokens(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0) {
+    const int64_t bh = (int64_t)b * p.Hk + h;
+    const bool ordered = p.keys != nullptr && p.ordered[bh] != 0;
+    for (int i = threadIdx.x; i < kWaves * p.QW; i += kThreads) {
+        const int at = min(n0 + i, p.Nq - 1);
+        L.tokens[i] = ordered ? p.order[bh * p.Nq + at] : at;
+    }
     __syncthreads();
+}
+
+// Marks the members of blocks [c0, c0 + nc) among the workgroup's tokens and lists the blocks that
+// have any, ascending; returns their number.  of_split < splits leaves other splits' blocks out
+// (blocks u with u % splits == of_split remain).  Ends with a barrier.
+__device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int end, int c0, int nc,
+                                     int of_split, int splits) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int i = tid; i < nc; i += kThreads) *reinterpret_cast<uint4*>(L.members[i]) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    // eight lanes a token
     const int tokens = min(kWaves * p.QW, p.Nq - n0);
-    for (int e = tid; e < tokens * p.K; e += kThreads) {
-        const int t = e / p.K, kk = e - t * p.K;
-        const int64_t blk = p.idx[(((int64_t)b * p.Nq + n0 + t) * p.Hk + h) * p.K + kk] - c0;
-        if (blk >= 0 && blk < nc && (c0 + blk) * p.bs < end) {
-            const int w = t / p.QW;
-            atomicOr(&L.members[blk][w >> 1], 1u << (16 * (w & 1) + t - w * p.QW));
+    for (int t = tid >> 3; t < tokens; t += kThreads / 8) {
+        const int64_t* e = p.idx + (((int64_t)b * p.Nq + L.tokens[t]) * p.Hk + h) * p.K;
+        const int w = (t * p.qw_inverse) >> 16;
+        const uint32_t bit = 1u << (t - w * p.QW);
+        for (int kk = tid & 7; kk < p.K; kk += 8) {
+            const int64_t blk = e[kk] - c0;
+            if (blk < 0 || blk >= nc) continue;
+            const int u = c0 + (int)blk;
+            if ((int64_t)u * p.bs < end && (splits == 1 || (uint32_t)u % (uint32_t)splits == (uint32_t)of_split))
+                atomicOr(&L.members[blk][w], bit);
         }
     }
     __syncthreads();
+    auto any = [&](int i) {
+        if (i >= nc) return false;
+        const uint4 m = *reinterpret_cast<const uint4*>(L.members[i]);
+        return (m.x | m.y | m.z | m.w) != 0;
+    };
     const int per = (nc + kThreads - 1) / kThreads * 64;   // blocks a wave lists
     int n = 0;
     for (int i = wave * per + lane; i - lane < (wave + 1) * per; i += 64)
-        n += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < nc && (L.members[i][0] | L.members[i][1])));
+        n += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(any(i)));
     if (lane == 0) L.found[wave] = n;
     __syncthreads();
     int at = 0, total = 0;
@@ -121,7 +257,7 @@ __device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds& L, int b
         total += L.found[w];
     }
     for (int i = wave * per + lane; i - lane < (wave + 1) * per; i += 64) {
-        const bool on = i < nc && (L.members[i][0] | L.members[i][1]);
+        const bool on = any(i);
         const uint64_t m = __builtin_amdgcn_ballot_w64(on);
         if (on) L.list[at + (int)__builtin_popcountll(m & ((1ull << lane) - 1ull))] = (uint16_t)i;
         at += (int)__builtin_popcountll(m);
@@ -130,205 +266,264 @@ __device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds& L, int b
     return total;
 }
 
-// Requests keys key0 .. key0 + 63 into one buffer; rows past the sequence's end repeat its last
-// one.  Each wave loads 16 rows of K and V; addresses are 64-bit throughout.
-__device__ __forceinline__ void stage(const QueryAttnParams& p, const bf16_t* kb, const bf16_t* vb, int key0, int end,
-                                      bf16_t* Kd, bf16_t* Vd, int wave, int lane) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row0 = 16 * wave + 8 * i, row = row0 + (lane >> 3);
-        const int64_t key = min(key0 + row, end - 1);
-        const int chunk = 8 * ((lane & 7) ^ swz16(row));
-        dma16_at(kb + key * p.k_sn + chunk, lds_addr(Kd + row0 * 64));
-        dma16_at(vb + key * p.v_sn + chunk, lds_addr(Vd + row0 * 64));
-    }
-}
-
-// Per-lane LDS element offsets of the operand reads
-struct RowReads {
-    int row[2];   // row c16, chunk 4 ks + g; + 16 kt * 64
-    int tr[4];    // transposing read of dims 16 dt ..: row 4 g + s / 4, + (32 c + 16 half) * 64
-    __device__ __forceinline__ void init(int lane) {
-        const int s = lane & 15, g = lane >> 4, r = 4 * g + (s >> 2);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) row[ks] = s * 64 + 8 * ((4 * ks + g) ^ swz16(s));
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) tr[dt] = r * 64 + 8 * ((2 * dt + ((s & 3) >> 1)) ^ swz16(r)) + 4 * (s & 1);
-    }
-};
-
-// acc^T[key tile] = T rows . B^T over 64 dims, from `start`
-__device__ __forceinline__ void row_products(const bf16_t* T, const RowReads& rr, const bf16x8 (&b)[2], float start, f32x4 (&acc)[4]) {
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[kt][e] = start;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-            acc[kt] = mfma16(as_bf16x8(*reinterpret_cast<const uint4*>(T + 16 * kt * 64 + rr.row[ks])), b[ks], acc[kt]);
-    }
-}
-
-// acc^T[dim tile] += T^T . B^T over 64 keys, B in the accumulator order of row_products
-__device__ __forceinline__ void col_products(const bf16_t* T, const RowReads& rr, const bf16x8 (&b)[2], f32x4 (&acc)[4]) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-            acc[dt] = mfma16(tr_pair(T + 32 * c * 64 + rr.tr[dt], T + (32 * c + 16) * 64 + rr.tr[dt]), b[c], acc[dt]);
-}
-
-__device__ __forceinline__ float row_add(float x) {   // over the four lanes of a row
-    x += __shfl_xor(x, 16);
-    return xor32_add(x);
-}
-__device__ __forceinline__ float row_max(float x) { return xor32_max(fmaxf(x, __shfl_xor(x, 16))); }
-
-// The rows of a wave, one per column c16 = lane % 16: token and query head, and its place in [B, Nq, Hq]
-struct Row {
-    int token, head;   // token within the wave
-    bool live;
-    int64_t n, at;
-    __device__ __forceinline__ void init(const QueryAttnParams& p, int b, int h, int wave_n0, int lane) {
-        const int r = lane & 15;
-        token = r / p.G;
-        live = token < p.QW && wave_n0 + token < p.Nq;
-        head = h * p.G + (live ? r - token * p.G : 0);
-        n = live ? wave_n0 + token : min(wave_n0, p.Nq - 1);
-        at = ((int64_t)b * p.Nq + n) * p.Hq + head;
-    }
-};
-
-__device__ __forceinline__ void load_row(const bf16_t* x, int64_t sb, int64_t sn, int64_t sh, int b, const Row& r, int lane, bf16x8 (&f)[2]) {
-    const bf16_t* at = x + b * sb + r.n * sn + r.head * sh + 8 * (lane >> 4);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) f[ks] = as_bf16x8(ld16(at + 32 * ks));
-}
-
-__device__ __forceinline__ void store_row(bf16_t* out, int64_t at, int lane, const f32x4 (&o)[4], float f) {
-    bf16_t* d = out + at * 64 + 4 * (lane >> 4);
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-        *reinterpret_cast<uint2*>(d + 16 * dt) =
-            make_uint2(pack_bf16x2(o[dt][0] * f, o[dt][1] * f), pack_bf16x2(o[dt][2] * f, o[dt][3] * f));
-}
-
 // Runs `tile(K, V, members of this wave, valid keys)` over the tiles of this workgroup's share of
-// the union, staged in two buffers with one barrier each.
+// the union, staged in two buffers with one barrier each.  Each wave loads 16 rows of K and V per
+// tile: from a uniform base with per-lane offsets that do not change (64 rows within 2^31 bytes), or
+// from 64-bit addresses, as the tile with the sequence's last key does, where the rows behind it
+// repeat it (V's are zeroed: what P = 0 multiplies there).
 template <typename Tile>
 __device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int split, int splits, Tile tile) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int end = seq_keys(p, b), sub = p.bs / 64;
     const bf16_t* kb = p.k + b * p.k_sb + h * p.k_sh;
     const bf16_t* vb = p.v + b * p.v_sb + h * p.v_sh;
-    const int live = (int)min((int64_t)p.nb, ((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
-    for (int c0 = 0; c0 < live; c0 += kUnion) {
-        const int found = unite(p, L, b, h, n0, end, c0, min(kUnion, live - c0));
-        const int first = (int)((int64_t)found * split / splits), past = (int)((int64_t)found * (split + 1) / splits);
-        const int tiles = (past - first) * sub;
-        auto key_of = [&](int t) { return (c0 + __builtin_amdgcn_readfirstlane((int)L.list[first + t / sub])) * p.bs + t % sub * 64; };
-        // tiles past the end are only in the union's last block
-        if (tiles > 0) stage(p, kb, vb, key_of(0), end, L.K[0], L.V[0], wave, lane);
-        for (int t = 0; t < tiles; ++t) {
-            const int key0 = key_of(t), valid = min(64, end - key0);
-            wait_vmem();
-            lds_barrier();
-            if (t + 1 < tiles && key_of(t + 1) < end) stage(p, kb, vb, key_of(t + 1), end, L.K[(t + 1) & 1], L.V[(t + 1) & 1], wave, lane);
-            if (valid <= 0) break;
-            if (valid < 64) {   // zeros behind the last key: what P = 0 multiplies there
-                for (int i = threadIdx.x; i < (64 - valid) * 8; i += kThreads)
-                    *reinterpret_cast<uint4*>(L.V[t & 1] + (valid + i / 8) * 64 + i % 8 * 8) = make_uint4(0, 0, 0, 0);
-                lds_barrier();
+    uint32_t ko[2], vo[2];
+    int row[2], chunk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        row[i] = 16 * wave + 8 * i + (lane >> 3);
+        chunk[i] = 8 * ((lane & 7) ^ swz32(row[i]));
+        ko[i] = 2u * (uint32_t)(row[i] * p.k_sn + chunk[i]);
+        vo[i] = 2u * (uint32_t)(row[i] * p.v_sn + chunk[i]);
+    }
+    auto stage = [&](int key0, int buf) {
+        if (p.short_rows && key0 + 64 <= end) {
+            const bf16_t* kt = kb + (int64_t)key0 * p.k_sn;
+            const bf16_t* vt = vb + (int64_t)key0 * p.v_sn;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                dma16(kt, ko[i], lds_addr(L.K[buf] + (16 * wave + 8 * i) * 64));
+                dma16(vt, vo[i], lds_addr(L.V[buf] + (16 * wave + 8 * i) * 64));
             }
-            const int u = L.list[first + t / sub];
-            const uint32_t mine = (L.members[u][wave >> 1] >> (16 * (wave & 1))) & 0xffffu;
-            const uint32_t m = __builtin_amdgcn_readfirstlane(mine);
-            if (m != 0) tile(L.K[t & 1], L.V[t & 1], m, valid);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t key = min(key0 + row[i], end - 1);
+                dma16_at(kb + key * p.k_sn + chunk[i], lds_addr(L.K[buf] + (16 * wave + 8 * i) * 64));
+                dma16_at(vb + key * p.v_sn + chunk[i], lds_addr(L.V[buf] + (16 * wave + 8 * i) * 64));
+            }
         }
-        wait_vmem();
-        __syncthreads();   // the lists and buffers are free for the next blocks
+    };
+    // one token's worth of tiles: shares by position in the list; more: by block (see unite), so
+    // that a row's share does not depend on the tokens beside it
+    const bool by_block = p.keys != nullptr;
+    const int live = min(p.nb, (int)((uint32_t)(end + p.bs - 1) / (uint32_t)p.bs));   // blocks with a key
+    for (int c0 = 0; c0 < live; c0 += kUnion) {
+        const int found = unite(p, L, b, h, n0, end, c0, min(kUnion, live - c0), split, by_block ? splits : 1);
+        const int first = by_block ? 0 : (int)((uint32_t)(found * split) / (uint32_t)splits);
+        const int past = by_block ? found : (int)((uint32_t)(found * (split + 1)) / (uint32_t)splits);
+        for (int e0 = first; e0 < past; e0 += 64) {
+            // up to 64 blocks of the list and this wave's members in registers: lane i holds block i
+            const int count = min(64, past - e0);
+            const int uv = L.list[e0 + min(lane, count - 1)];
+            const int mv = (int)L.members[uv][wave];
+            int key0 = (c0 + __builtin_amdgcn_readlane(uv, 0)) * p.bs, buf = 0;
+            stage(key0, 0);
+            for (int i = 0; i < count; ++i) {
+                const uint32_t members = (uint32_t)__builtin_amdgcn_readlane(mv, i);
+                for (int st = 0; st < sub; ++st) {
+                    const bool more = st + 1 < sub ? key0 + 64 < end : i + 1 < count;
+                    const int next = st + 1 < sub ? key0 + 64 : (c0 + __builtin_amdgcn_readlane(uv, min(i + 1, 63))) * p.bs;
+                    wait_vmem();
+                    lds_barrier();
+                    if (more) stage(next, buf ^ 1);
+                    const int valid = min(64, end - key0);
+                    if (valid < 64) {
+                        for (int z = threadIdx.x; z < (64 - valid) * 8; z += kThreads)
+                            *reinterpret_cast<uint4*>(L.V[buf] + (valid + z / 8) * 64 + z % 8 * 8) = make_uint4(0, 0, 0, 0);
+                        lds_barrier();
+                    }
+                    if (members != 0) tile(L.K[buf], L.V[buf], members, valid);
+                    if (!more) break;   // past the last key, or past the list
+                    key0 = next;
+                    buf ^= 1;
+                }
+            }
+            lds_barrier();   // the buffers are free for the next blocks
+        }
+        __syncthreads();     // and the lists
     }
 }
 
-__global__ __launch_bounds__(kThreads) void query_attn_kernel(QueryAttnParams p, int total) {
+// Per-lane LDS element offsets of the operand reads: row r, chunk 2 ds + hh, + 32 kt * 64; and the
+// transposing reads of dims 32 dt + lane % 32, rows 4 hh + 0..3 and 8 more, + 16 rows * 64
+struct TileReads {
+    int row[4], tr[2][2];
+    __device__ __forceinline__ void init(int lane) {
+        const int r = lane & 31, hh = lane >> 5, s4 = lane & 15, half = (lane >> 4) & 1;
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) row[ds] = r * 64 + 8 * ((2 * ds + hh) ^ swz32(r));
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+            for (int sec = 0; sec < 2; ++sec) {
+                const int rr = 4 * hh + (s4 >> 2) + 8 * sec;
+                tr[dt][sec] = rr * 64 + 8 * ((4 * dt + 2 * half + ((s4 & 3) >> 1)) ^ swz32(rr)) + 4 * (s4 & 1);
+            }
+    }
+    __device__ __forceinline__ bf16x8 rows(const bf16_t* T, int r0, int ds) const {
+        return as_bf16x8(*reinterpret_cast<const uint4*>(T + r0 * 64 + row[ds]));
+    }
+    __device__ __forceinline__ bf16x8 cols(const bf16_t* T, int r0, int dt) const {
+        return tr_pair(T + r0 * 64 + tr[dt][0], T + r0 * 64 + tr[dt][1]);
+    }
+};
+
+__device__ __forceinline__ f32x16 splat(float x) {
+    f32x16 y;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = x;
+    return y;
+}
+
+// acc + the 8 rounded values of one operand, two per instruction.  (A product with ones on the
+// matrix pipe would do it too, but a 16-column one mixes rows r and r + 16, and zeros do not keep
+// another row's NaN out.)
+__device__ __forceinline__ float operand_sum(const bf16x8& x, float acc) {
+    const uint4 u = __builtin_bit_cast(uint4, x);
+    const bf16x2 ones = __builtin_bit_cast(bf16x2, 0x3f803f80u);
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u.x), ones, acc, false);
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u.y), ones, acc, false);
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u.z), ones, acc, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u.w), ones, acc, false);
+}
+
+// The rows of a wave, one per column r = lane % 32: token (position in the wave), query head, and
+// its place in [B, Nq, Hq]
+struct Row {
+    int token, head;
+    bool live;
+    int64_t n, at;
+    __device__ __forceinline__ void init(const QueryAttnParams& p, const RowsLds& L, int b, int h, int n0, int wave, int lane) {
+        const int r = lane & 31;
+        token = r / p.G;
+        live = token < p.QW && n0 + wave * p.QW + token < p.Nq;
+        head = h * p.G + (live ? r - token * p.G : 0);
+        n = L.tokens[wave * p.QW + (live ? token : 0)];
+        at = ((int64_t)b * p.Nq + n) * p.Hq + head;
+    }
+};
+
+__device__ __forceinline__ void load_row(const bf16_t* x, int64_t sb, int64_t sn, int64_t sh, int b, const Row& r, int lane, bf16x8 (&f)[4]) {
+    const bf16_t* at = x + b * sb + r.n * sn + r.head * sh + 8 * (lane >> 5);
+#pragma unroll
+    for (int ds = 0; ds < 4; ++ds) f[ds] = as_bf16x8(ld16(at + 16 * ds));
+}
+
+__device__ __forceinline__ void store_row(bf16_t* out, int64_t at, int lane, const f32x16 (&o)[2], float f) {
+    bf16_t* d = out + at * 64 + 4 * (lane >> 5);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+            *reinterpret_cast<uint2*>(d + 32 * dt + 8 * g4) = make_uint2(pack_bf16x2(o[dt][4 * g4] * f, o[dt][4 * g4 + 1] * f),
+                                                                         pack_bf16x2(o[dt][4 * g4 + 2] * f, o[dt][4 * g4 + 3] * f));
+}
+
+// In a branch that is rarely taken: keeps the compiler from computing it always and selecting.
+__device__ __forceinline__ void seldom() { asm volatile(""); }
+
+// Scores of keys at or past `valid` become `fill` (accumulator element e of key half kt: key 32 kt + 8 (e / 4) + 4 hh + e % 4)
+__device__ __forceinline__ void mask_keys(f32x16& s, int kt, int hh, int valid, float fill) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3) < valid ? s[e] : fill;
+}
+
+template <bool LSE>
+__global__ __launch_bounds__(kThreads, 3) void query_attn_kernel(QueryAttnParams p, int total) {
     __shared__ RowsLds L;
-    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = xcd_remap(blockIdx.x, total);
     const int split = id % p.splits, tile_id = id / p.splits % p.qtiles, rest = id / p.splits / p.qtiles;
     const int h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
+    load_tokens(p, L, b, h, n0);
     Row row;
-    row.init(p, b, h, n0 + wave * p.QW, lane);
-    bf16x8 qf[2];
+    row.init(p, L, b, h, n0, wave, lane);
+    bf16x8 qf[4];
     load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
-    RowReads rr;
-    rr.init(lane);
-    f32x4 o[4];
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[dt][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    TileReads tr;
+    tr.init(lane);
+    f32x16 o[2] = {splat(0.f), splat(0.f)};
+    float m = -INFINITY, l = 0.f, lx = 0.f;    // l, lx: this lane's part of the sums of the rounded and unrounded P
     for_tiles(p, L, b, h, n0, split, p.splits, [&](const bf16_t* Kt, const bf16_t* Vt, uint32_t members, int valid) {
-        f32x4 s[4];
-        row_products(Kt, rr, qf, 0.f, s);
+        f32x16 s[2] = {splat(0.f), splat(0.f)};
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) s[kt] = mfma32(tr.rows(Kt, 32 * kt, ds), qf[ds], s[kt]);
         if (valid < 64) {
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[kt][e] = 16 * kt + 4 * g + e < valid ? s[kt][e] : -INFINITY;
+            seldom();
+            mask_keys(s[0], 0, hh, valid, -INFINITY);
+            mask_keys(s[1], 1, hh, valid, -INFINITY);
         }
+        // (the maximum that NaN wins takes three operands and no canonicalising instruction)
         float mt = s[0][0];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mt = fmaxf(mt, s[kt][e]);
-        const float mnew = fmaxf(m, row_max(mt) * p.c);
-        bf16x8 pb[2];
-        float lt = 0.f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4& x = s[2 * c + i / 2];
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1)], p.c, -mnew));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1) + 1], p.c, -mnew));
-                lt += p0 + p1;
-                w[i] = pack_bf16x2(p0, p1);
-            }
-            pb[c] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+            for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
+        mt = xor32_max(mt) * p.c;
+        const bool member = row.live && (members >> row.token & 1);
+        const bool move = member && mt > m + kTau;
+        if (__builtin_amdgcn_ballot_w64(move)) {   // rare after a row's first tile
+            const float alpha = move ? __builtin_amdgcn_exp2f(m - mt) : 1.f;
+            m = move ? mt : m;
+            o[0] *= alpha;
+            o[1] *= alpha;
+            l *= alpha;
+            lx *= alpha;
         }
-        f32x4 add[4];
+        bf16x8 pb[2][2];
+        float lt[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) add[dt][e] = 0.f;
-        col_products(Vt, rr, pb, add);
-        if (row.live && (members >> row.token & 1)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-            m = mnew;
-            l = fmaf(l, alpha, lt);
+            for (int s2 = 0; s2 < 2; ++s2) {
+                uint32_t w[4];
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
+                for (int i = 0; i < 4; ++i) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i], p.c, -m));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i + 1], p.c, -m));
+                    if constexpr (LSE) sum[kt] += p0 + p1;
+                    w[i] = pack_bf16x2(p0, p1);
+                }
+                pb[kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+                lt[kt] = operand_sum(pb[kt][s2], lt[kt]);
+            }
+        if (member) {
+            l += lt[0] + lt[1];
+            if constexpr (LSE) lx += sum[0] + sum[1];
+        }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[dt][e] = fmaf(o[dt][e], alpha, add[dt][e]);
+        for (int dt = 0; dt < 2; ++dt) {
+            f32x16 add = splat(0.f);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) add = mfma32(tr.cols(Vt, 32 * kt + 16 * s2, dt), pb[kt][s2], add);
+            if (member) o[dt] += add;
         }
     });
-    l = row_add(l);
+    l = xor32_add(l);
+    if constexpr (LSE) lx = xor32_add(lx);
     if (!row.live) return;
     if (p.splits > 1) {
         const int64_t rows = (int64_t)p.B * p.Nq * p.Hq;
-        float* d = p.part_o + (split * rows + row.at) * 64 + 4 * g;
+        float* d = p.part_o + (split * rows + row.at) * 64 + 4 * hh;
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<float4*>(d + 16 * dt) = make_float4(o[dt][0], o[dt][1], o[dt][2], o[dt][3]);
-        if (g == 0) p.part_ml[split * rows + row.at] = make_float2(m, l);
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4)
+                *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) = make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+        if (hh == 0) p.part_ml[split * rows + row.at] = make_float4(m, l, lx, 0.f);
         return;
     }
-    // a row without a key has l = 0 (any other at least the largest score's 1, or NaN)
+    // a row without a key has l = 0 (any other at least 2^-8, or NaN)
     store_row(p.out, row.at, lane, o, l == 0.f ? 0.f : 1.f / l);
-    if (p.lse != nullptr && g == 0) p.lse[row.at] = m + __builtin_amdgcn_logf(l);
+    if constexpr (LSE)
+        if (hh == 0) p.lse[row.at] = m + __builtin_amdgcn_logf(lx);
 }
 
 // Joins the splits' partials: 16 lanes a row, 4 dims each.
@@ -338,19 +533,20 @@ __global__ __launch_bounds__(kThreads) void query_attn_join_kernel(QueryAttnPara
     const int d = threadIdx.x % 16 * 4;
     float m = -INFINITY;
     for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[s * rows + row].x);
-    float l = 0.f;
+    float l = 0.f, lx = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s = 0; s < p.splits; ++s) {
-        const float2 ml = p.part_ml[s * rows + row];
+        const float4 ml = p.part_ml[s * rows + row];
         if (ml.y == 0.f) continue;          // no key in this share
         const float a = __builtin_amdgcn_exp2f(ml.x - m);
         const float4 x = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * 64 + d);
         l = fmaf(a, ml.y, l);
+        lx = fmaf(a, ml.z, lx);
         o.x = fmaf(a, x.x, o.x); o.y = fmaf(a, x.y, o.y); o.z = fmaf(a, x.z, o.z); o.w = fmaf(a, x.w, o.w);
     }
     const float f = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<uint2*>(p.out + row * 64 + d) = make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
-    if (p.lse != nullptr && d == 0) p.lse[row] = m + __builtin_amdgcn_logf(l);
+    if (p.lse != nullptr && d == 0) p.lse[row] = m + __builtin_amdgcn_logf(lx);
 }
 
 // ------------------------------------------------------------------ backward
@@ -368,102 +564,96 @@ __global__ __launch_bounds__(kThreads) void query_attn_join_kernel(QueryAttnPara
 // here, and the exact one, delta + sum P (do.v - delta), goes to grad k / v.  One product more per
 // tile on operands at hand; without it grad q at 12288 tokens of nside 32 (12 blocks of 64) is
 // 5.1e-3 off (2-norm), with it 2.4e-3 (the output's own rounding alone: 1.7e-3).
-__global__ __launch_bounds__(kThreads) void query_attn_dq_kernel(QueryAttnParams p, int total) {
+__global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnParams p, int total) {
     __shared__ RowsLds L;
-    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = xcd_remap(blockIdx.x, total);
     const int tile_id = id % p.qtiles, rest = id / p.qtiles;
     const int h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
+    load_tokens(p, L, b, h, n0);
     Row row;
-    row.init(p, b, h, n0 + wave * p.QW, lane);
-    bf16x8 qf[2], gf[2];
+    row.init(p, L, b, h, n0, wave, lane);
+    bf16x8 qf[4], gf[4];
     load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
     load_row(p.go, p.go_sb, p.go_sn, p.go_sh, b, row, lane, gf);
     float delta = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-        const uint4 ov = ld16(p.o + row.at * 64 + 32 * ks + 8 * g), gv = __builtin_bit_cast(uint4, gf[ks]);
+    for (int ds = 0; ds < 4; ++ds) {
+        const uint4 ov = ld16(p.o + row.at * 64 + 16 * ds + 8 * hh), gv = __builtin_bit_cast(uint4, gf[ds]);
         const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) delta = fmaf(bf_lo(ow[i]), bf_lo(gw[i]), fmaf(bf_hi(ow[i]), bf_hi(gw[i]), delta));
     }
-    delta = row_add(delta);
+    delta = xor32_add(delta);
     const float nlse = -p.lse[row.at] / p.c;
-    RowReads rr;
-    rr.init(lane);
-    const bf16x8 ones = as_bf16x8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
-    f32x4 dq[4], kbar[4], sum = {0.f, 0.f, 0.f, 0.f};   // sum dS' k, sum P k, sum dS'
-    float rest_d = 0.f;                                  // this lane's part of sum P (do.v - delta)
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dq[dt][e] = kbar[dt][e] = 0.f;
+    TileReads tr;
+    tr.init(lane);
+    f32x16 dq[2] = {splat(0.f), splat(0.f)}, kbar[2] = {splat(0.f), splat(0.f)};   // sum dS' k, sum P k
+    float sum = 0.f, rest_d = 0.f;   // this lane's parts of sum dS' and of sum P (do.v - delta)
     for_tiles(p, L, b, h, n0, 0, 1, [&](const bf16_t* Kt, const bf16_t* Vt, uint32_t members, int valid) {
-        f32x4 s[4], dp[4];
-        row_products(Kt, rr, qf, nlse, s);
-        row_products(Vt, rr, gf, -delta, dp);
-        if (valid < 64) {
+        const bool member = row.live && (members >> row.token & 1);
+#pragma unroll 1
+        for (int kt = 0; kt < 2; ++kt) {
+            f32x16 s = splat(nlse), dp = splat(-delta);
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
+            for (int ds = 0; ds < 4; ++ds) {
+                s = mfma32(tr.rows(Kt, 32 * kt, ds), qf[ds], s);
+                dp = mfma32(tr.rows(Vt, 32 * kt, ds), gf[ds], dp);
+            }
+            if (valid < 64) {
+                seldom();
+                mask_keys(s, kt, hh, valid, -INFINITY);
+                mask_keys(dp, kt, hh, valid, 0.f);
+            }
+            bf16x8 pb[2], db[2];
+            float dsum = 0.f, rsum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool on = 16 * kt + 4 * g + e < valid;
-                    s[kt][e] = on ? s[kt][e] : -INFINITY;
-                    dp[kt][e] = on ? dp[kt][e] : 0.f;
+            for (int s2 = 0; s2 < 2; ++s2) {
+                uint32_t w[4], x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 8 * s2 + 2 * i;
+                    const float p0 = __builtin_amdgcn_exp2f(s[e] * p.c), p1 = __builtin_amdgcn_exp2f(s[e + 1] * p.c);
+                    const float d0 = p0 * dp[e], d1 = p1 * dp[e + 1];
+                    dsum += d0 + d1;
+                    w[i] = pack_bf16x2(p0, p1);
+                    x[i] = pack_bf16x2(d0, d1);
                 }
-        }
-        bf16x8 pb[2], db[2];
-        float dsum = 0.f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            uint32_t w[4], x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int kt = 2 * c + i / 2, e = 2 * (i & 1);
-                const float p0 = __builtin_amdgcn_exp2f(s[kt][e] * p.c), p1 = __builtin_amdgcn_exp2f(s[kt][e + 1] * p.c);
-                const float d0 = p0 * dp[kt][e], d1 = p1 * dp[kt][e + 1];
-                dsum += d0 + d1;
-                w[i] = pack_bf16x2(p0, p1);
-                x[i] = pack_bf16x2(d0, d1);
+                pb[s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+                db[s2] = as_bf16x8(make_uint4(x[0], x[1], x[2], x[3]));
+                rsum = operand_sum(db[s2], rsum);
             }
-            pb[c] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-            db[c] = as_bf16x8(make_uint4(x[0], x[1], x[2], x[3]));
-        }
-        f32x4 dqt[4], kt_[4], st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+            for (int dt = 0; dt < 2; ++dt) {
+                f32x16 da = splat(0.f), ka = splat(0.f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dqt[dt][e] = kt_[dt][e] = 0.f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            st = mfma16(ones, db[c], st);
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt) {
-                const bf16x8 kT = tr_pair(Kt + 32 * c * 64 + rr.tr[dt], Kt + (32 * c + 16) * 64 + rr.tr[dt]);
-                dqt[dt] = mfma16(kT, db[c], dqt[dt]);
-                kt_[dt] = mfma16(kT, pb[c], kt_[dt]);
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const bf16x8 kT = tr.cols(Kt, 32 * kt + 16 * s2, dt);
+                    da = mfma32(kT, db[s2], da);
+                    ka = mfma32(kT, pb[s2], ka);
+                }
+                if (member) {
+                    dq[dt] += da;
+                    kbar[dt] += ka;
+                }
             }
-        }
-        if (row.live && (members >> row.token & 1)) {
-            rest_d += dsum;
-            sum += st;
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt) {
-                dq[dt] += dqt[dt];
-                kbar[dt] += kt_[dt];
+            if (member) {
+                sum += rsum;
+                rest_d += dsum;
             }
         }
     });
-    rest_d = row_add(rest_d);
+    rest_d = xor32_add(rest_d);
+    sum = xor32_add(sum);
     if (!row.live) return;
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+    for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dq[dt][e] = fmaf(-sum[0], kbar[dt][e], dq[dt][e]);
+        for (int e = 0; e < 16; ++e) dq[dt][e] = fmaf(-sum, kbar[dt][e], dq[dt][e]);
     store_row(p.out, row.at, lane, dq, p.scale);
-    if (g == 0) {
+    if (hh == 0) {
         p.nlse[row.at] = nlse;
         p.ndelta[row.at] = -(delta + rest_d);
     }
@@ -501,8 +691,6 @@ __global__ __launch_bounds__(kThreads) void query_marks_kernel(QueryAttnParams p
 // dK^T += q^T dS, whose A operands are transposing LDS reads.  The row halves are added at the end.
 constexpr int kSegWords = 128;                 // words of marks listed at a time: 4096 tokens
 constexpr int kListed = 32 * kSegWords + 64;   // and what was left of the last ones
-
-__device__ __forceinline__ int swz32(int row) { return (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
 
 struct KeysLds {
     __attribute__((aligned(1024))) bf16_t q[2][kTileElems];
@@ -595,14 +783,18 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
                 dp = mfma32(as_bf16x8(*reinterpret_cast<const uint4*>(Gc + 32 * qh * 64 + rd[kk])), vf[kk], dp);
             }
             bf16x8 pb[2], db[2];
+            if (rows < 64) {   // rows past the list, or past QS G: P = 0 and dS = 0
+                seldom();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool on = 32 * qh + 8 * (e >> 2) + 4 * hh + (e & 3) < rows;
+                    s[e] = on ? s[e] : -INFINITY;
+                    dp[e] = on ? dp[e] : 0.f;
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                float pr = __builtin_amdgcn_exp2f(s[e] * p.c), ds = pr * dp[e];
-                if (rows < 64) {   // rows past the list, or past QS G
-                    const bool on = 32 * qh + 8 * (e >> 2) + 4 * hh + (e & 3) < rows;
-                    pr = on ? pr : 0.f;
-                    ds = on ? ds : 0.f;
-                }
+                const float pr = __builtin_amdgcn_exp2f(s[e] * p.c), ds = pr * dp[e];
                 pb[e >> 3][e & 7] = (__bf16)pr;
                 db[e >> 3][e & 7] = (__bf16)ds;
             }
@@ -714,19 +906,38 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
     if (K > kMaxSelected) return MOSAIC_ERR_UNSUPPORTED;
     // ids of workgroups and keys stay in 31 bits
     if (nk > 0x7fffffff - bs || nq > 0x7fffffff - kMarkTokens) return MOSAIC_ERR_SHAPE;
-    const int64_t qw = 16 / (hq / hk), tiles = ((int64_t)nq + 4 * qw - 1) / (4 * qw);
+    const int64_t per = kWaves * (kRowsPerWave / (hq / hk)), tiles = ((int64_t)nq + per - 1) / per;
     if ((double)tiles * hk * batch * kMaxSplit > 2147483647.0) return MOSAIC_ERR_SHAPE;
     if ((double)((nk + 63) / 64) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
+    if (((double)nq / kThreads + 1) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
     return MOSAIC_OK;
 }
 
 // Workgroups of one share: below one per CU the union is split, up to two per CU together.
 int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
-    const int64_t per = 4 * (16 / (hq / hk));
+    const int64_t per = kWaves * (kRowsPerWave / (hq / hk));
     const int64_t wgs = (nq + per - 1) / per * hk * batch;
     if (wgs >= 256) return 1;
     const int64_t s = 512 / wgs;
     return (int)(s < K ? (s < kMaxSplit ? s : kMaxSplit) : (K < kMaxSplit ? K : kMaxSplit));
+}
+
+// Whether tokens may be taken in another order: with more than two workgroups of them.
+bool may_order(int32_t nq, int32_t hq, int32_t hk) { return nq > 2 * kWaves * (kRowsPerWave / (hq / hk)); }
+int key_chunks(int32_t nq) { return (nq + kThreads - 1) / kThreads; }
+size_t order_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
+    if (!may_order(nq, hq, hk)) return 0;
+    const size_t rows = (size_t)batch * hk * nq;
+    return up(rows * sizeof(uint16_t)) + up(rows * sizeof(int32_t)) + up((size_t)batch * hk * sizeof(int32_t)) +
+           up((size_t)batch * hk * key_chunks(nq) * sizeof(int32_t));
+}
+void place_order(QueryAttnParams& p, char* ws) {
+    if (!may_order(p.Nq, p.Hq, p.Hk)) return;
+    const size_t rows = (size_t)p.B * p.Hk * p.Nq;
+    p.keys = reinterpret_cast<uint16_t*>(ws);
+    p.order = reinterpret_cast<int32_t*>(ws + up(rows * sizeof(uint16_t)));
+    p.ordered = reinterpret_cast<int32_t*>(ws + up(rows * sizeof(uint16_t)) + up(rows * sizeof(int32_t)));
+    p.far = p.ordered + up((size_t)p.B * p.Hk * sizeof(int32_t)) / sizeof(int32_t);
 }
 
 void fill(QueryAttnParams& p, const mosaic_bnhd& q, const mosaic_bnhd& k, const mosaic_bnhd& v, const int64_t* idx,
@@ -735,17 +946,30 @@ void fill(QueryAttnParams& p, const mosaic_bnhd& q, const mosaic_bnhd& k, const 
     p.k = static_cast<const bf16_t*>(k.ptr); p.k_sb = k.stride_b; p.k_sn = k.stride_n; p.k_sh = k.stride_h;
     p.v = static_cast<const bf16_t*>(v.ptr); p.v_sb = v.stride_b; p.v_sn = v.stride_n; p.v_sh = v.stride_h;
     p.idx = idx; p.lens = lens;
-    p.B = batch; p.Nq = nq; p.Nk = nk; p.Hq = hq; p.Hk = hk; p.G = hq / hk; p.QW = 16 / p.G; p.bs = bs; p.K = K;
+    p.B = batch; p.Nq = nq; p.Nk = nk; p.Hq = hq; p.Hk = hk; p.G = hq / hk; p.QW = kRowsPerWave / p.G; p.bs = bs; p.K = K;
     p.nb = (nk + bs - 1) / bs;
     p.qtiles = (nq + kWaves * p.QW - 1) / (kWaves * p.QW);
     p.splits = 1;
+    p.qw_inverse = (65536 + p.QW - 1) / p.QW;
+    const int64_t most = (int64_t)1 << 23;   // 64 rows of 2^23 bf16 are 2^30 bytes
+    p.short_rows = k.stride_n >= 0 && k.stride_n <= most && v.stride_n >= 0 && v.stride_n <= most;
     p.scale = scale > 0.f ? scale : 0.125f;   // head_dim^-0.5
     p.c = p.scale * kLog2e;
 }
 
 int words_of(int32_t nq) { return (nq + kMarkTokens - 1) / kMarkTokens * kMarkWords; }
 
-hipError_t launch(const void* fn, dim3 grid, void** args, hipStream_t s) { return hipLaunchKernel(fn, grid, dim3(kThreads), args, 0, s); }
+hipError_t launch(const void* fn, dim3 grid, void** args, hipStream_t s, int threads = kThreads) {
+    return hipLaunchKernel(fn, grid, dim3(threads), args, 0, s);
+}
+
+int launch_order(QueryAttnParams& p, hipStream_t s) {
+    if (p.keys == nullptr) return MOSAIC_OK;
+    int chunks = key_chunks(p.Nq);
+    void* args[] = {&p, &chunks};
+    if (launch((const void*)&query_keys_kernel, dim3(p.B * p.Hk * chunks), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    return launch((const void*)&query_order_kernel, dim3(p.B * p.Hk), args, s, kOrderThreads) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+}
 
 }  // namespace
 }  // namespace mosaic
@@ -758,9 +982,9 @@ size_t mosaic_query_attn_fwd_workspace_size(int32_t batch, int32_t num_queries, 
                                             int32_t block_count) {
     if (check_shape(batch, num_queries, 1, num_q_heads, num_kv_heads, kHeadDim, 64, block_count) != MOSAIC_OK) return 0;
     const int s = choose_split(batch, num_queries, num_q_heads, num_kv_heads, block_count);
-    if (s == 1) return 0;
-    const size_t rows = (size_t)batch * num_queries * num_q_heads;
-    return up(s * rows * kHeadDim * sizeof(float)) + up(s * rows * sizeof(float2));
+    const size_t rows = s == 1 ? 0 : (size_t)batch * num_queries * num_q_heads;
+    return up(s * rows * kHeadDim * sizeof(float)) + up(s * rows * sizeof(float4)) +
+           order_bytes(batch, num_queries, num_q_heads, num_kv_heads);
 }
 
 int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int64_t* block_indices, const int32_t* kv_lens,
@@ -778,16 +1002,22 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
     p.lse = lse;
     p.splits = choose_split(batch, num_queries, num_q_heads, num_kv_heads, block_count);
     int64_t rows = (int64_t)batch * num_queries * num_q_heads;
+    const size_t need = mosaic_query_attn_fwd_workspace_size(batch, num_queries, num_q_heads, num_kv_heads, block_count);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256))) return MOSAIC_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
     if (p.splits > 1) {
-        const size_t need = mosaic_query_attn_fwd_workspace_size(batch, num_queries, num_q_heads, num_kv_heads, block_count);
-        if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)) return MOSAIC_ERR_WORKSPACE;
-        p.part_o = static_cast<float*>(workspace);
-        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + up(p.splits * rows * kHeadDim * sizeof(float)));
+        p.part_o = reinterpret_cast<float*>(ws);
+        ws += up(p.splits * rows * kHeadDim * sizeof(float));
+        p.part_ml = reinterpret_cast<float4*>(ws);
+        ws += up(p.splits * rows * sizeof(float4));
     }
+    place_order(p, ws);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (int e = launch_order(p, s)) return e;
     int total = p.qtiles * num_kv_heads * batch * p.splits;
     void* args[] = {&p, &total};
-    if (launch((const void*)&query_attn_kernel, dim3(total), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    const void* fn = lse != nullptr ? (const void*)&query_attn_kernel<true> : (const void*)&query_attn_kernel<false>;
+    if (launch(fn, dim3(total), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
     void* jargs[] = {&p, &rows};
     return launch((const void*)&query_attn_join_kernel, dim3((unsigned)((rows + 15) / 16)), jargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
@@ -797,7 +1027,8 @@ size_t mosaic_query_attn_bwd_workspace_size(int32_t batch, int32_t num_queries, 
                                             int32_t num_kv_heads, int32_t block_size) {
     if (check_shape(batch, num_queries, num_keys, num_q_heads, num_kv_heads, kHeadDim, block_size, 1) != MOSAIC_OK) return 0;
     const size_t rows = (size_t)batch * num_queries * num_q_heads, nb = ((size_t)num_keys + block_size - 1) / block_size;
-    return 2 * up(rows * sizeof(float)) + up((size_t)batch * num_kv_heads * nb * words_of(num_queries) * sizeof(uint32_t));
+    return 2 * up(rows * sizeof(float)) + up((size_t)batch * num_kv_heads * nb * words_of(num_queries) * sizeof(uint32_t)) +
+           order_bytes(batch, num_queries, num_q_heads, num_kv_heads);
 }
 
 int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const void* out, const float* lse, mosaic_bnhd grad_out,
@@ -825,6 +1056,8 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     p.ndelta = reinterpret_cast<float*>(static_cast<char*>(workspace) + row_bytes);
     p.marks = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + 2 * row_bytes);
     p.words = words_of(num_queries);
+    place_order(p, static_cast<char*>(workspace) + 2 * row_bytes +
+                       up((size_t)batch * num_kv_heads * p.nb * p.words * sizeof(uint32_t)));
     p.out = static_cast<bf16_t*>(grad_q);
     p.dk = static_cast<bf16_t*>(grad_k);
     p.dv = static_cast<bf16_t*>(grad_v);
@@ -832,6 +1065,7 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     int groups = p.words / kMarkWords;
     if (chunks > 65535 || (double)groups * num_kv_heads * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (int e = launch_order(p, s)) return e;
     int total = p.qtiles * num_kv_heads * batch;
     void* args[] = {&p, &total};
     if (launch((const void*)&query_attn_dq_kernel, dim3(total), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
