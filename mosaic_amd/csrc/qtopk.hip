@@ -17,10 +17,12 @@
 //
 // One workgroup = 16 query tokens of one kv head.  Its waves form the scores S^T = K Q^T of up to
 // 64 PL blocks with v_mfma_f32_16x16x32_bf16 into LDS (16 rows of fp32), then each wave takes
-// rows: PL scores per lane in registers, T by bisection between the row's largest score and the
-// smallest of the lanes' largest ones (64 scores at least lie above it, and K <= 64), each step a
-// compare and a population count per register, and the indices by their prefix counts.  More
-// blocks than 64 PL go in chunks: the rows' best K so far join the next chunk's scores.
+// rows, PL scores per lane in registers.  The K-th largest of the lanes' largest scores bounds T
+// from below, so the scores from there on hold all K; there are seldom more than a few of them, and
+// up to 64 go one to a lane, where T is found by bisection, a compare and a population count per
+// step.  (Bisection over all PL registers, the first form of this kernel: 1105 vector instructions a
+// row at 768 blocks, 432 us for the tokens of nside 64.)  More blocks than 64 PL go in chunks: the
+// rows' best K so far join the next chunk's scores.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -44,20 +46,97 @@ struct QueryTopkParams {
     int qtiles;
 };
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
-    return x;
+// max (or min) over the wave, in every lane: DPP steps within 16 lanes, then the swaps of 16- and
+// 32-lane halves
+template <bool MAX>
+__device__ __forceinline__ float either(float a, float b) { return MAX ? fmaxf(a, b) : fminf(a, b); }
+template <bool MAX, int CTRL>
+__device__ __forceinline__ float dpp_either(float x) {
+    return either<MAX>(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false)));
 }
-__device__ __forceinline__ float wave_min(float x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x = fminf(x, __shfl_xor(x, m));
-    return x;
+template <bool MAX>
+__device__ __forceinline__ float wave_either(float x) {
+    x = dpp_either<MAX, 0xb1>(x);    // quad_perm [1,0,3,2]
+    x = dpp_either<MAX, 0x4e>(x);    // quad_perm [2,3,0,1]
+    x = dpp_either<MAX, 0x141>(x);   // row_half_mirror
+    x = dpp_either<MAX, 0x140>(x);   // row_mirror
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = either<MAX>(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return either<MAX>(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+__device__ __forceinline__ float wave_max(float x) { return wave_either<true>(x); }
+__device__ __forceinline__ float wave_min(float x) { return wave_either<false>(x); }
+
+// The K-th largest of the lanes' values (-inf among them; none is NaN), by bisection: a compare and a
+// population count per step.  -inf where fewer than K are above it.
+__device__ __forceinline__ float wave_kth(float x, int K, int lane) {
+    auto count = [&](float t) { return (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= t)); };
+    if (count(-__FLT_MAX__) < K) return -INFINITY;
+    float hi = wave_max(x), lo = wave_min(x == -INFINITY ? INFINITY : x);
+    if (count(hi) >= K) return hi;
+    for (;;) {   // count(lo) >= K > count(hi)
+        const float mid = 0.5f * lo + 0.5f * hi;
+        if (!(mid > lo && mid < hi)) return lo;   // neighbours
+        const int n = count(mid);
+        if (n == K) return wave_min(x >= mid ? x : INFINITY);
+        if (n > K) lo = mid; else hi = mid;
+    }
 }
 
+// Lane of the n-th set bit of m (anything past the last)
+__device__ __forceinline__ int nth_bit(uint64_t m, int n) {
+    for (int i = 0; i < n; ++i) m &= m - 1;
+    return m == 0 ? 0 : (int)__builtin_ctzll(m);
+}
+
+// The exact summed query of a row, a dim per lane, to LDS
+__device__ __forceinline__ void summed_query(const QueryTopkParams& p, int b, int n, int h, int lane, double* qs) {
+    const bf16_t* qb = p.q + b * p.q_sb + (int64_t)n * p.q_sn + (int64_t)h * p.G * p.q_sh + lane;
+    double sum = 0.0;
+    for (int g = 0; g < p.G; ++g) sum += (double)bf2f(qb[g * p.q_sh]);
+    qs[lane] = sum;
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ double exact_score(const bf16_t* kr, const double* qs) {
+    double s = 0.0;
+    for (int d = 0; d < 64; d += 8) {
+        const uint4 w4 = ld16(kr + d);
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s = fma(qs[d + 2 * j], (double)bf_lo(w[j]), s);
+            s = fma(qs[d + 2 * j + 1], (double)bf_hi(w[j]), s);
+        }
+    }
+    return s;
+}
+// How many of the lanes in `of` come before this one: a larger score, or the same and a lower lane.
+__device__ __forceinline__ int exact_rank(double x, bool of, int lane) {
+    int rank = 0;
+    for (uint64_t m = __builtin_amdgcn_ballot_w64(of); m != 0; m &= m - 1) {
+        const int j = (int)__builtin_ctzll(m);
+        const double y = __shfl(x, j);
+        rank += y > x || (y == x && j < lane);
+    }
+    return rank;
+}
+
+// How many values of the lanes in `of` are above y, or equal where `ties`.
+__device__ __forceinline__ int exact_above(double x, bool of, double y, bool ties) {
+    int n = 0;
+    for (uint64_t m = __builtin_amdgcn_ballot_w64(of); m != 0; m &= m - 1) {
+        const double z = __shfl(x, (int)__builtin_ctzll(m));
+        n += z > y || (ties && z == y);
+    }
+    return n;
+}
+
+// Waves per SIMD: what the LDS of two workgroups (one from 768 blocks on) allows, at most 4
 template <int PL, int NW>
-__global__ __launch_bounds__(NW * 64) void query_topk_kernel(QueryTopkParams p) {
+__global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams p) {
     constexpr int kChunk = 64 * PL, kStride = kChunk + 4;
+    static_assert(4 * 64 + 2 * 64 * (PL + 1) <= 4 * kStride, "64 scores and a row's codes fit its scores' place");
     __shared__ __attribute__((aligned(16))) float sc[kRows * kStride];
     __shared__ float carry_v[kRows][kMaxTopk];   // best K of the chunks so far, ascending blocks
     __shared__ int carry_u[kRows][kMaxTopk];
@@ -82,6 +161,7 @@ __global__ __launch_bounds__(NW * 64) void query_topk_kernel(QueryTopkParams p) 
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[ks][i] = tot[ks][i] = 0.f;
+#pragma unroll 4
         for (int g = 0; g < p.G; ++g)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
@@ -111,40 +191,62 @@ __global__ __launch_bounds__(NW * 64) void query_topk_kernel(QueryTopkParams p) 
     const int rows = min(kRows, p.Nq - n0);
     float kn = 0.f;   // largest squared norm of this lane's dims over the blocks it has loaded
     for (int u0 = 0; u0 < p.nb; u0 += kChunk) {
-        const int nc = min(kChunk, p.nb - u0);
-        for (int t = wave; t < (nc + 15) / 16; t += NW) {
-            const int u = u0 + 16 * t + c16;
-            const bf16_t* kr = kb + (int64_t)min(u, p.nb - 1) * p.k_sn + 8 * g4;
-            const uint4 a0 = ld16(kr), a1 = ld16(kr + 32);
-            const bool on = u < p.nb && (mask == nullptr || mask[u]);
-            float nn = 0.f;
-            const uint32_t aw[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+        const int nc = min(kChunk, p.nb - u0), tiles = (nc + 15) / 16;
+        // kTiles tiles' keys are requested together
+        constexpr int kTiles = 4;
+        for (int t0 = wave; t0 < tiles; t0 += kTiles * NW) {
+            uint4 a[kTiles][2];
+            bool on[kTiles];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bf16x2 e = __builtin_bit_cast(bf16x2, aw[i]);
-                nn = __builtin_amdgcn_fdot2_f32_bf16(e, e, nn, false);
+            for (int j = 0; j < kTiles; ++j) {
+                const int u = u0 + 16 * (t0 + j * NW) + c16, at = min(u, p.nb - 1);
+                const bf16_t* kr = kb + (int64_t)at * p.k_sn + 8 * g4;
+                a[j][0] = ld16(kr);
+                a[j][1] = ld16(kr + 32);
+                on[j] = u < p.nb;
+                if (mask != nullptr) on[j] = on[j] && mask[at];
             }
-            kn = on ? fmaxf(kn, nn) : kn;
-            f32x4 s = {0.f, 0.f, 0.f, 0.f};
-            s = mfma16(as_bf16x8(a0), hi[0], s);
-            s = mfma16(as_bf16x8(a1), hi[1], s);
-            if (p.G > 1) {
-                s = mfma16(as_bf16x8(a0), lo[0], s);
-                s = mfma16(as_bf16x8(a1), lo[1], s);
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+                const int t = t0 + j * NW;
+                if (t >= tiles) break;
+                float nn = 0.f;
+                const uint32_t aw[8] = {a[j][0].x, a[j][0].y, a[j][0].z, a[j][0].w, a[j][1].x, a[j][1].y, a[j][1].z, a[j][1].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bf16x2 e = __builtin_bit_cast(bf16x2, aw[i]);
+                    nn = __builtin_amdgcn_fdot2_f32_bf16(e, e, nn, false);
+                }
+                kn = on[j] ? fmaxf(kn, nn) : kn;
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                s = mfma16(as_bf16x8(a[j][0]), hi[0], s);
+                s = mfma16(as_bf16x8(a[j][1]), hi[1], s);
+                if (p.G > 1) {
+                    s = mfma16(as_bf16x8(a[j][0]), lo[0], s);
+                    s = mfma16(as_bf16x8(a[j][1]), lo[1], s);
+                }
+                // lane: blocks 16 t + 4 g4 + e of query c16 (a maximum with -inf takes NaN out); the flag
+                // of block c is lane c's
+                float4 v = make_float4(fmaxf(s[0], -INFINITY), fmaxf(s[1], -INFINITY), fmaxf(s[2], -INFINITY), fmaxf(s[3], -INFINITY));
+                const uint32_t ons = (uint32_t)__builtin_amdgcn_ballot_w64(on[j]);
+                if (ons != ~0u) {
+                    const uint32_t four = ons >> (4 * g4);
+                    v.x = (four & 1) ? v.x : -INFINITY;
+                    v.y = (four & 2) ? v.y : -INFINITY;
+                    v.z = (four & 4) ? v.z : -INFINITY;
+                    v.w = (four & 8) ? v.w : -INFINITY;
+                }
+                *reinterpret_cast<float4*>(sc + c16 * kStride + 16 * t + 4 * g4) = v;
             }
-            // lane: blocks 16 t + 4 g4 + e of query c16; the flag of block c is lane c's
-            const uint32_t ons = (uint32_t)__builtin_amdgcn_ballot_w64(on) >> (4 * g4);
-            float4 v;
-            v.x = (ons & 1) && s[0] == s[0] ? s[0] : -INFINITY;
-            v.y = (ons & 2) && s[1] == s[1] ? s[1] : -INFINITY;
-            v.z = (ons & 4) && s[2] == s[2] ? s[2] : -INFINITY;
-            v.w = (ons & 8) && s[3] == s[3] ? s[3] : -INFINITY;
-            *reinterpret_cast<float4*>(sc + c16 * kStride + 16 * t + 4 * g4) = v;
         }
+        for (int i = 16 * tiles + threadIdx.x % 64; i < kChunk; i += 64)   // no blocks behind the last tile
+            for (int r = threadIdx.x / 64; r < kRows; r += NW) sc[r * kStride + i] = -INFINITY;
         {   // |k|^2 <= the sum over the four dim groups of their largest
             float m = kn;
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+            m = dpp_either<true, 0xb1>(m);
+            m = dpp_either<true, 0x4e>(m);
+            m = dpp_either<true, 0x141>(m);
+            m = dpp_either<true, 0x140>(m);
             m += __shfl_xor(m, 16);
             m += __shfl_xor(m, 32);
             if (lane == 0) knorm[wave] = m;
@@ -156,152 +258,103 @@ __global__ __launch_bounds__(NW * 64) void query_topk_kernel(QueryTopkParams p) 
         kmax = sqrtf(kmax);
         const bool last = u0 + kChunk >= p.nb;
         for (int r = wave; r < rows; r += NW) {
-            // element 0: the carried best, element 1 + i: block u0 + lane + 64 i; -inf past the end
+            // element 0: the carried best, element 1 + i: block u0 + lane + 64 i; -inf where there is none
             float v[PL + 1];
-            int cu = 0;
-            v[0] = -INFINITY;
-            if (u0 > 0 && lane < carry_n[r]) {
-                v[0] = carry_v[r][lane];
-                cu = carry_u[r][lane];
-            }
+            v[0] = u0 > 0 && lane < carry_n[r] ? carry_v[r][lane] : -INFINITY;
 #pragma unroll
-            for (int i = 0; i < PL; ++i) v[1 + i] = lane + 64 * i < nc ? sc[r * kStride + lane + 64 * i] : -INFINITY;
-            auto count = [&](float x) {   // scores >= x
-                int n = 0;
+            for (int i = 0; i < PL; ++i) v[1 + i] = sc[r * kStride + lane + 64 * i];
+            float top = v[0];
 #pragma unroll
-                for (int i = 0; i <= PL; ++i) n += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= x));
-                return n;
-            };
-            float top = v[0], low = v[0] == -INFINITY ? INFINITY : v[0];
-#pragma unroll
-            for (int i = 1; i <= PL; ++i) {
-                top = fmaxf(top, v[i]);
-                low = fminf(low, v[i] == -INFINITY ? INFINITY : v[i]);
-            }
-            const float inner = wave_min(top);     // -inf where a lane has no block
-            const int valid = count(-__FLT_MAX__);
-            float from, to;                        // taken: certainly above `to`, perhaps in [from, to]
-            int sure = 0, maybe = valid;
-            if (valid <= p.K) {
-                from = -__FLT_MAX__;
-                to = INFINITY;
-            } else {
-                float hi_s = wave_max(top), lo_s = inner > -INFINITY ? inner : wave_min(low);
-                // count(lo_s) >= K and fewer than K lie above hi_s; T in [lo_s, hi_s]
-                float T = hi_s;
-                if (count(hi_s) < p.K) {
-                    for (;;) {
-                        const float mid = 0.5f * lo_s + 0.5f * hi_s;
-                        if (!(mid > lo_s && mid < hi_s)) {   // neighbours: ties
-                            T = lo_s;
-                            break;
-                        }
-                        const int n = count(mid);
-                        if (n == p.K) {
-                            float least = INFINITY;
-#pragma unroll
-                            for (int i = 0; i <= PL; ++i) least = fminf(least, v[i] >= mid ? v[i] : INFINITY);
-                            T = wave_min(least);
-                            break;
-                        }
-                        if (n > p.K) lo_s = mid; else hi_s = mid;
-                    }
-                }
-                float e2 = 0x1p-14f * qnorm[r] * kmax;       // 2 eps
-                if (!(e2 < INFINITY)) e2 = 0.f;
-                from = T - e2;
-                to = T + e2;
-                maybe = count(from);
-#pragma unroll
-                for (int i = 0; i <= PL; ++i) sure += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] > to));
-                maybe -= sure;
-            }
-            uint32_t taken = 0;    // bit i: element i
-#pragma unroll
-            for (int i = 0; i <= PL; ++i) taken |= (v[i] >= from) ? 1u << i : 0u;
-            if (sure + maybe > p.K) {
-                // exact scores of the blocks between, one per lane at a time
-                double* qs = qd[wave];
-                {
-                    const bf16_t* qb = p.q + b * p.q_sb + (int64_t)(n0 + r) * p.q_sn + (int64_t)h * p.G * p.q_sh + lane;
-                    double sum = 0.0;
-                    for (int g = 0; g < p.G; ++g) sum += (double)bf2f(qb[g * p.q_sh]);
-                    qs[lane] = sum;
-                }
-                double s[PL + 1];
-                uint32_t open = 0;
-#pragma unroll
-                for (int i = 0; i <= PL; ++i) {
-                    s[i] = 0.0;
-                    if (v[i] >= from && v[i] <= to) {
-                        open |= 1u << i;
-                        const bf16_t* kr = kb + (int64_t)(i == 0 ? cu : u0 + lane + 64 * (i - 1)) * p.k_sn;
-                        double a = 0.0;
-                        for (int d = 0; d < 64; d += 8) {
-                            const uint4 w4 = ld16(kr + d);
-                            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                a = fma(qs[d + 2 * j], (double)bf_lo(w[j]), a);
-                                a = fma(qs[d + 2 * j + 1], (double)bf_hi(w[j]), a);
-                            }
-                        }
-                        s[i] = a;
-                    }
-                }
-                taken &= ~open;
-                for (int left = p.K - sure; left > 0; --left) {   // the best of the open ones, the lower block first
-                    double best = -INFINITY;
-                    int bu = 0x7fffffff, bi = 0;
-#pragma unroll
-                    for (int i = 0; i <= PL; ++i) {
-                        const int u = i == 0 ? cu : u0 + lane + 64 * (i - 1);
-                        if ((open >> i & 1) && (s[i] > best || (s[i] == best && u < bu))) {
-                            best = s[i];
-                            bu = u;
-                            bi = i;
-                        }
-                    }
-                    double wb = best;
-                    int wu = bu;
-#pragma unroll
-                    for (int m = 1; m < 64; m <<= 1) {
-                        const double ob = __shfl_xor(wb, m);
-                        const int ou = __shfl_xor(wu, m);
-                        if (ob > wb || (ob == wb && ou < wu)) {
-                            wb = ob;
-                            wu = ou;
-                        }
-                    }
-                    if (wu == bu && bu != 0x7fffffff) {
-                        taken |= 1u << bi;
-                        open &= ~(1u << bi);
-                    }
-                }
-            }
-            // taken blocks in ascending order: the carried ones, then the chunk's by register and lane
-            int at = 0;
-            int64_t* row = p.out + (((int64_t)b * p.Nq + n0 + r) * p.Hk + h) * p.K;
+            for (int i = 1; i <= PL; ++i) top = __builtin_elementwise_maximum(top, v[i]);   // no score is NaN
+            float e2 = 0x1p-14f * qnorm[r] * kmax;       // 2 eps
+            if (!(e2 < INFINITY)) e2 = 0.f;
+            // The K-th largest of the lanes' largest scores has K scores at least at or above it: T is
+            // no smaller. Where no more than 64 come within 2 eps of it, as they nearly always do (K
+            // good blocks are spread over the lanes), they go one to a lane, ascending by block.
+            const float least = wave_kth(top, p.K, lane);
+            const float keep = fmaxf(least - e2, -__FLT_MAX__);
+            float* scores = sc + r * kStride;                            // of the first 64, and all codes
+            uint16_t* codes = reinterpret_cast<uint16_t*>(scores + 64);   // (64 i + l: element i of lane l)
+            asm volatile("" ::: "memory");     // the row's scores are read before these take their place
+            int n = 0;
 #pragma unroll
             for (int i = 0; i <= PL; ++i) {
-                const bool on = taken >> i & 1;
-                const uint64_t m = __builtin_amdgcn_ballot_w64(on);
-                const int pos = at + (int)__builtin_popcountll(m & ((1ull << lane) - 1ull));
-                const int u = i == 0 ? cu : u0 + lane + 64 * (i - 1);
-                if (on) {
-                    if (last) {
-                        row[pos] = u;
-                    } else {
-                        carry_v[r][pos] = v[i];
-                        carry_u[r][pos] = u;
+                const uint64_t m = __builtin_amdgcn_ballot_w64(v[i] >= keep);
+                if (m == 0) continue;
+                const int pos = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+                n += (int)__builtin_popcountll(m);
+                if (v[i] >= keep) {
+                    codes[pos] = (uint16_t)(64 * i + lane);
+                    if (pos < 64) scores[pos] = v[i];
+                }
+            }
+            asm volatile("" ::: "memory");     // (LDS is in order within a wave)
+            auto block = [&](int code) { return code < 64 ? carry_u[r][code] : u0 + code - 64; };
+            bool take;
+            float mine = -INFINITY;
+            int u = 0;
+            if (n <= 64) {
+                take = lane < n;
+                if (take) {
+                    u = block(codes[lane]);
+                    mine = scores[lane];
+                }
+                if (n > p.K) {
+                    const float T = wave_kth(mine, p.K, lane);
+                    const uint64_t in = __builtin_amdgcn_ballot_w64(mine >= T - e2 && lane < n);
+                    take = in >> lane & 1;
+                    if ((int)__builtin_popcountll(in) > p.K) {
+                        // more within 2 eps of T than slots are left: exact scores decide
+                        const bool open = take && mine <= T + e2;
+                        take = take && !open;
+                        const int sure = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(take));
+                        summed_query(p, b, n0 + r, h, lane, qd[wave]);
+                        const double x = open ? exact_score(kb + (int64_t)u * p.k_sn, qd[wave]) : -INFINITY;
+                        const int rank = exact_rank(x, open, lane);
+                        take = take || (open && rank < p.K - sure);
                     }
                 }
-                at += (int)__builtin_popcountll(m);
+            } else {
+                // ties: every candidate's exact score is formed, 64 at a time, and the best K held, one a
+                // lane and ascending; all held ones have lower blocks than the new ones
+                summed_query(p, b, n0 + r, h, lane, qd[wave]);
+                double held = -INFINITY;
+                int held_u = 0, holds = 0;
+                for (int at = 0; at < n; at += 64) {
+                    const bool fresh = at + lane < n, old = lane < holds;
+                    const int fu = fresh ? block(codes[at + lane]) : 0;
+                    const double x = fresh ? exact_score(kb + (int64_t)fu * p.k_sn, qd[wave]) : -INFINITY;
+                    const int rank_x = exact_rank(x, fresh, lane) + exact_above(held, old, x, true);
+                    const int rank_h = exact_rank(held, old, lane) + exact_above(x, fresh, held, false);
+                    const uint64_t mh = __builtin_amdgcn_ballot_w64(old && rank_h < p.K);
+                    const uint64_t mx = __builtin_amdgcn_ballot_w64(fresh && rank_x < p.K);
+                    const int nh = (int)__builtin_popcountll(mh);
+                    const int jh = nth_bit(mh, min(lane, 63)), jx = nth_bit(mx, max(lane - nh, 0));
+                    const double h1 = __shfl(held, jh), x1 = __shfl(x, jx);
+                    const int u1 = __shfl(held_u, jh), u2 = __shfl(fu, jx);
+                    held = lane < nh ? h1 : x1;
+                    held_u = lane < nh ? u1 : u2;
+                    holds = nh + (int)__builtin_popcountll(mx);
+                }
+                take = lane < holds;
+                u = held_u;
+                mine = (float)held;
             }
+            // taken blocks, ascending by lane
+            const uint64_t m = __builtin_amdgcn_ballot_w64(take);
+            const int count = (int)__builtin_popcountll(m);
+            const int pos = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+            asm volatile("" ::: "memory");         // the carried blocks are read before they are written
             if (last) {
-                if (lane >= at && lane < p.K) row[lane] = -1;
-            } else if (lane == 0) {
-                carry_n[r] = at;
+                int64_t* row = p.out + (((int64_t)b * p.Nq + n0 + r) * p.Hk + h) * p.K;
+                if (take) row[pos] = u;
+                if (lane >= count && lane < p.K) row[lane] = -1;
+            } else {
+                if (take) {
+                    carry_v[r][pos] = mine;
+                    carry_u[r][pos] = u;
+                }
+                if (lane == 0) carry_n[r] = count;
             }
         }
         if (!last) __syncthreads();   // the rows' scores are read before the next chunk's are written
@@ -310,7 +363,7 @@ __global__ __launch_bounds__(NW * 64) void query_topk_kernel(QueryTopkParams p) 
 
 template <int PL>
 const void* topk_fn(bool wide) {
-    return wide ? (const void*)&query_topk_kernel<PL, 16> : (const void*)&query_topk_kernel<PL, 4>;
+    return wide ? (const void*)&query_topk_kernel<PL, 16> : (const void*)&query_topk_kernel<PL, 8>;
 }
 
 bool rows_ok(const mosaic_bnhd& t) {
@@ -347,6 +400,6 @@ extern "C" int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uin
     const void* fn = num_blocks <= 256 ? topk_fn<4>(wide) : num_blocks <= 512 ? topk_fn<8>(wide)
                    : num_blocks <= 768 ? topk_fn<12>(wide) : topk_fn<16>(wide);
     void* args[] = {&p};
-    return hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(wide ? 1024 : 256), args, 0, static_cast<hipStream_t>(stream)) == hipSuccess
+    return hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(wide ? 1024 : 512), args, 0, static_cast<hipStream_t>(stream)) == hipSuccess
                ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
