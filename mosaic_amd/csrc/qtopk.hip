@@ -132,7 +132,7 @@ __device__ __forceinline__ int exact_above(double x, bool of, double y, bool tie
     return n;
 }
 
-// Waves per SIMD: what the LDS of two workgroups (one from 768 blocks on) allows, at most 4
+// PL = 12 at most: two workgroups of 8 waves then share a CU's LDS and fill its 4 waves per SIMD.
 template <int PL, int NW>
 __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams p) {
     constexpr int kChunk = 64 * PL, kStride = kChunk + 4;
@@ -142,6 +142,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
     __shared__ int carry_u[kRows][kMaxTopk];
     __shared__ int carry_n[kRows];
     __shared__ float qnorm[kRows], knorm[NW];
+    __shared__ __attribute__((aligned(16))) bf16_t qpart[2][kRows][72];   // (rows 144 bytes apart: distinct banks)
     __shared__ double qd[NW][64];                // a wave's exact summed query (rows that need it)
 
     const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
@@ -152,48 +153,54 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
     const bf16_t* kb = p.k + b * p.k_sb + h * p.k_sh;
     const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (int64_t)b * p.nb;
 
-    // the summed query of column c16 (dims 32 ks + 8 g4 .. + 7), as hi + lo operands
-    bf16x8 hi[2], lo[2];
+    // the summed queries, each thread a run of dims of one, as hi + lo parts by way of LDS
     {
-        const bf16_t* qb = p.q + b * p.q_sb + (int64_t)min(n0 + c16, p.Nq - 1) * p.q_sn + (int64_t)h * p.G * p.q_sh;
-        float sum[2][8], mag = 0.f, tot[2][8];
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[ks][i] = tot[ks][i] = 0.f;
+        constexpr int kDims = kRows * 64 / (NW * 64), kLanes = 64 / kDims;   // dims a thread, threads a query
+        static_assert(kDims == 2 || kDims == 1, "one or two dims a thread");
+        const int r = threadIdx.x / kLanes, d = threadIdx.x % kLanes * kDims;
+        const bf16_t* qb = p.q + b * p.q_sb + (int64_t)min(n0 + r, p.Nq - 1) * p.q_sn + (int64_t)h * p.G * p.q_sh + d;
+        float sum[kDims] = {}, tot[kDims] = {};
 #pragma unroll 4
-        for (int g = 0; g < p.G; ++g)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const uint4 u = ld16(qb + g * p.q_sh + 32 * ks + 8 * g4);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sum[ks][2 * i] += bf_lo(w[i]);
-                    sum[ks][2 * i + 1] += bf_hi(w[i]);
-                    tot[ks][2 * i] += fabsf(bf_lo(w[i]));
-                    tot[ks][2 * i + 1] += fabsf(bf_hi(w[i]));
-                }
+        for (int g = 0; g < p.G; ++g) {
+            float x[kDims];
+            if constexpr (kDims == 2) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(qb + g * p.q_sh);
+                x[0] = bf_lo(w);
+                x[1] = bf_hi(w);
+            } else {
+                x[0] = bf2f(qb[g * p.q_sh]);
             }
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float a = round_bf16(sum[ks][i]);
-                hi[ks][i] = (__bf16)a;
-                lo[ks][i] = (__bf16)(sum[ks][i] - a);
-                mag = fmaf(tot[ks][i], tot[ks][i], mag);
+            for (int i = 0; i < kDims; ++i) {
+                sum[i] += x[i];
+                tot[i] += fabsf(x[i]);
             }
-        mag += __shfl_xor(mag, 16);
-        mag += __shfl_xor(mag, 32);
-        if (wave == 0 && lane < 16) qnorm[lane] = sqrtf(mag);
+        }
+        float mag = 0.f;
+#pragma unroll
+        for (int i = 0; i < kDims; ++i) {
+            const float a = round_bf16(sum[i]);
+            qpart[0][r][d + i] = (bf16_t)(__float_as_uint(a) >> 16);
+            qpart[1][r][d + i] = (bf16_t)(pack_bf16x2(sum[i] - a, 0.f) & 0xffffu);
+            mag = fmaf(tot[i], tot[i], mag);
+        }
+#pragma unroll
+        for (int m = 1; m < kLanes; m <<= 1) mag += __shfl_xor(mag, m);
+        if (threadIdx.x % kLanes == 0) qnorm[r] = sqrtf(mag);
+    }
+    __syncthreads();
+    bf16x8 hi[2], lo[2];   // of column c16, dims 32 ks + 8 g4 .. + 7
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+        hi[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[0][c16][32 * ks + 8 * g4]));
+        lo[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[1][c16][32 * ks + 8 * g4]));
     }
     const int rows = min(kRows, p.Nq - n0);
     float kn = 0.f;   // largest squared norm of this lane's dims over the blocks it has loaded
     for (int u0 = 0; u0 < p.nb; u0 += kChunk) {
         const int nc = min(kChunk, p.nb - u0), tiles = (nc + 15) / 16;
-        // kTiles tiles' keys are requested together
-        constexpr int kTiles = 4;
+        // a wave's tiles of a whole chunk are requested together
+        constexpr int kTiles = 4 * PL > NW ? 4 * PL / NW : 1;
         for (int t0 = wave; t0 < tiles; t0 += kTiles * NW) {
             uint4 a[kTiles][2];
             bool on[kTiles];
@@ -397,8 +404,7 @@ extern "C" int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uin
     const int64_t wgs = (int64_t)p.qtiles * num_kv_heads * batch;
     if (wgs > 0x7fffffff) return MOSAIC_ERR_SHAPE;
     const bool wide = wgs < 256;
-    const void* fn = num_blocks <= 256 ? topk_fn<4>(wide) : num_blocks <= 512 ? topk_fn<8>(wide)
-                   : num_blocks <= 768 ? topk_fn<12>(wide) : topk_fn<16>(wide);
+    const void* fn = num_blocks <= 256 ? topk_fn<4>(wide) : num_blocks <= 512 ? topk_fn<8>(wide) : topk_fn<12>(wide);
     void* args[] = {&p};
     return hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(wide ? 1024 : 512), args, 0, static_cast<hipStream_t>(stream)) == hipSuccess
                ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
