@@ -526,24 +526,46 @@ __global__ __launch_bounds__(kThreads, 3) void query_attn_kernel(QueryAttnParams
         if (hh == 0) p.lse[row.at] = m + __builtin_amdgcn_logf(lx);
 }
 
-// Joins the splits' partials: 16 lanes a row, 4 dims each.
+// Joins the splits' partials: 16 lanes a row, 4 dims each.  Lane j holds the weights of splits j and
+// j + 16, so that no load waits for another.
 __global__ __launch_bounds__(kThreads) void query_attn_join_kernel(QueryAttnParams p, int64_t rows) {
-    const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    if (row >= rows) return;
-    const int d = threadIdx.x % 16 * 4;
-    float m = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[s * rows + row].x);
-    float l = 0.f, lx = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-        const float4 ml = p.part_ml[s * rows + row];
-        if (ml.y == 0.f) continue;          // no key in this share
-        const float a = __builtin_amdgcn_exp2f(ml.x - m);
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * 64 + d);
-        l = fmaf(a, ml.y, l);
-        lx = fmaf(a, ml.z, lx);
-        o.x = fmaf(a, x.x, o.x); o.y = fmaf(a, x.y, o.y); o.z = fmaf(a, x.z, o.z); o.w = fmaf(a, x.w, o.w);
+    static_assert(kMaxSplit == 32, "two splits a lane");
+    const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, row = at < rows ? at : rows - 1;
+    const int j = threadIdx.x % 16, d = 4 * j;
+    float4 ml[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int s = j + 16 * i;
+        ml[i] = s < p.splits ? p.part_ml[s * rows + row] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
     }
+    float m = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    // l = 0: no key in that share (its m is -inf, as is that of one with nothing but NaN)
+    float a[2], l = 0.f, lx = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        a[i] = ml[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - m);
+        l = fmaf(a[i], ml[i].y, l);
+        lx = fmaf(a[i], ml[i].z, lx);
+    }
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) {
+        l += __shfl_xor(l, x);
+        lx += __shfl_xor(lx, x);
+    }
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int n = min(16, p.splits - 16 * i);
+#pragma unroll 8
+        for (int s = 0; s < n; ++s) {
+            const float4 x = *reinterpret_cast<const float4*>(p.part_o + ((s + 16 * i) * rows + row) * 64 + d);
+            const float w = __shfl(a[i], (threadIdx.x & 48) + s);
+            o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+        }
+    }
+    if (at >= rows) return;
     const float f = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<uint2*>(p.out + row * 64 + d) = make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
     if (p.lse != nullptr && d == 0) p.lse[row] = m + __builtin_amdgcn_logf(lx);

@@ -23,9 +23,8 @@ import math
 import torch
 
 from . import _lib
-from .ops import stream_of
-from .primitives import _workspace, pool_mean
-from .rotary import _bnhd, _ptr, _rows, _same_device
+from .primitives import pool_mean
+from .rotary import _on, _ptr, _rows, _same_device, _stream, _wants_grad
 
 __all__ = ["query_topk", "query_sparse_attn", "mosaic_query_attn"]
 
@@ -52,7 +51,8 @@ def _groups(what: str, q: torch.Tensor, k: torch.Tensor) -> None:
         raise ValueError(f"{what}: {Hq} query heads must be a multiple of {Hk} kv heads, at most 16 times as many")
 
 
-def _as_bf16(t: torch.Tensor) -> torch.Tensor:
+def _as_bf16(t: torch.Tensor):
+    """bf16 rows as the kernels read them: (tensor, its pointer and strides)."""
     return _rows(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16))
 
 
@@ -80,28 +80,33 @@ def query_topk(q: torch.Tensor, k_cmp: torch.Tensor, block_count: int, block_mas
     idx = torch.empty(B, Nq, Hk, block_count, dtype=torch.int64, device=q.device)
     if idx.numel() == 0:
         return idx
-    q, k_cmp = _as_bf16(q), _as_bf16(k_cmp)
+    (q, qb), (k_cmp, kb) = _as_bf16(q), _as_bf16(k_cmp)
     mask = None if block_mask is None else block_mask.contiguous()
-    with torch.cuda.device(q.device):
-        st = _lib.lib().mosaic_query_topk_fwd(_bnhd(q), _bnhd(k_cmp), None if mask is None else mask.data_ptr(), B, Nq, nb,
-                                              Hq, Hk, d, block_count, idx.data_ptr(), stream_of(q))
+    with _on(q.device):
+        st = _lib.lib().mosaic_query_topk_fwd(qb, kb, _ptr(mask), B, Nq, nb, Hq, Hk, d, block_count, idx.data_ptr(), _stream(q.device))
     _lib.check(st, "mosaic_query_topk_fwd")
     return idx
 
 
+def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    """Workspace (torch's allocator aligns to 512 bytes; the library checks the 256 it needs)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _attn_fwd(q, k, v, idx, block_size, scale, lens, want_lse):
-    """(output bf16 [B, Nq, Hq, 64], lse fp32 [B, Nq, Hq] or None) of bf16 rows."""
+    """(output bf16 [B, Nq, Hq, 64], lse fp32 [B, Nq, Hq] or None); q, k, v as (rows, their Bnhd)."""
+    (q, qb), (k, kb), (v, vb) = q, k, v
     B, Nq, Hq, d = q.shape
     Nk, Hk = k.shape[1:3]
-    K = idx.shape[-1]
-    out = torch.empty(B, Nq, Hq, d, dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty(B, Nq, Hq, dtype=torch.float32, device=q.device) if want_lse else None
+    K, device = idx.shape[-1], q.device
+    out = torch.empty((B, Nq, Hq, d), dtype=torch.bfloat16, device=device)
+    lse = torch.empty((B, Nq, Hq), dtype=torch.float32, device=device) if want_lse else None
     L = _lib.lib()
     nbytes = L.mosaic_query_attn_fwd_workspace_size(B, Nq, Hq, Hk, K)
-    ws = _workspace(nbytes, q.device) if nbytes else None
-    with torch.cuda.device(q.device):
-        st = L.mosaic_query_attn_fwd(_bnhd(q), _bnhd(k), _bnhd(v), idx.data_ptr(), _ptr(lens), B, Nq, Nk, Hq, Hk, d, block_size,
-                                     K, scale, out.data_ptr(), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel(), stream_of(q))
+    ws = _scratch(nbytes, device)
+    with _on(device):
+        st = L.mosaic_query_attn_fwd(qb, kb, vb, idx.data_ptr(), _ptr(lens), B, Nq, Nk, Hq, Hk, d, block_size, K, scale,
+                                     out.data_ptr(), _ptr(lse), _ptr(ws), nbytes, _stream(device))
     _lib.check(st, "mosaic_query_attn_fwd")
     return out, lse
 
@@ -110,39 +115,32 @@ class _QueryAttn(torch.autograd.Function):
     """Saves the bf16 rows the kernels read, the output and its log-sum-exp."""
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, q, k, v, idx, block_size, scale, lens):
         ctx.dtypes = (q.dtype, k.dtype, v.dtype)
         ctx.rest = (block_size, scale)
-        grad = any(ctx.needs_input_grad[:3])
-        if 0 in q.shape or 0 in k.shape or idx.shape[-1] == 0:     # no row, or no key for any
-            ctx.save_for_backward(q, k, v)
-            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        qb, kb, vb = (_as_bf16(t) for t in (q, k, v))
-        out, lse = _attn_fwd(qb, kb, vb, idx, block_size, scale, lens, grad)
-        if grad:
-            ctx.save_for_backward(qb, kb, vb, out, lse, idx, lens)
+        rows = [_as_bf16(t) for t in (q, k, v)]
+        out, lse = _attn_fwd(*rows, idx, block_size, scale, lens, True)
+        ctx.save_for_backward(*(t for t, _ in rows), out, lse, idx, lens)
         return out.to(q.dtype)
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        if len(ctx.saved_tensors) == 3:
-            return tuple(torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * 4
         q, k, v, out, lse, idx, lens = ctx.saved_tensors
         block_size, scale = ctx.rest
         B, Nq, Hq, d = q.shape
         Nk, Hk = k.shape[1:3]
-        go = _as_bf16(go)
-        gq = torch.empty(B, Nq, Hq, d, dtype=torch.bfloat16, device=q.device)
-        gk, gv = (torch.empty(B, Nk, Hk, d, dtype=torch.bfloat16, device=q.device) for _ in range(2))
+        device = q.device
+        (q, qb), (k, kb), (v, vb), (go, gb) = (_as_bf16(t) for t in (q, k, v, go))
+        gq = torch.empty((B, Nq, Hq, d), dtype=torch.bfloat16, device=device)
+        gk, gv = (torch.empty((B, Nk, Hk, d), dtype=torch.bfloat16, device=device) for _ in range(2))
         L = _lib.lib()
-        ws = _workspace(L.mosaic_query_attn_bwd_workspace_size(B, Nq, Nk, Hq, Hk, block_size), q.device)
-        with torch.cuda.device(q.device):
-            st = L.mosaic_query_attn_bwd(_bnhd(q), _bnhd(k), _bnhd(v), out.data_ptr(), lse.data_ptr(), _bnhd(go), idx.data_ptr(),
-                                         _ptr(lens), B, Nq, Nk, Hq, Hk, d, block_size, idx.shape[-1], scale, gq.data_ptr(),
-                                         gk.data_ptr(), gv.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(q))
+        nbytes = L.mosaic_query_attn_bwd_workspace_size(B, Nq, Nk, Hq, Hk, block_size)
+        ws = _scratch(nbytes, device)
+        with _on(device):
+            st = L.mosaic_query_attn_bwd(qb, kb, vb, out.data_ptr(), lse.data_ptr(), gb, idx.data_ptr(), _ptr(lens), B, Nq, Nk,
+                                         Hq, Hk, d, block_size, idx.shape[-1], scale, gq.data_ptr(), gk.data_ptr(),
+                                         gv.data_ptr(), ws.data_ptr(), nbytes, _stream(device))
         _lib.check(st, "mosaic_query_attn_bwd")
         return tuple(g.to(t) for g, t in zip((gq, gk, gv), ctx.dtypes)) + (None,) * 4
 
@@ -182,8 +180,14 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
     _same_device(what, q, k=k, v=v, block_indices=block_indices, kv_lens=kv_lens)
     if kv_lens is not None:   # clamped before the conversion: a far length stays one
         kv_lens = (kv_lens if kv_lens.dtype == torch.int32 else kv_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
+    block_size = int(block_size)
+    if q.numel() == 0 or k.numel() == 0 or block_indices.numel() == 0:   # no row, or no key for any
+        # (a product with nothing, so that gradients of the inputs are zeros)
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device) + 0 * (q[:0].sum() + k[:0].sum() + v[:0].sum()).to(q.dtype)
     idx = block_indices.to(torch.int64).contiguous()
-    return _QueryAttn.apply(q, k, v, idx, int(block_size), scale, kv_lens)
+    if _wants_grad(q, k, v):
+        return _QueryAttn.apply(q, k, v, idx, block_size, scale, kv_lens)
+    return _attn_fwd(_as_bf16(q), _as_bf16(k), _as_bf16(v), idx, block_size, scale, kv_lens, False)[0].to(q.dtype)
 
 
 def mosaic_query_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_size: int, block_count: int, *,

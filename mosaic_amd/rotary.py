@@ -15,6 +15,7 @@ current stream of q's device and never synchronise the host.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -22,7 +23,6 @@ import math
 import torch
 
 from . import _lib
-from .ops import stream_of
 
 __all__ = ["rope_axes", "qk_norm_rope"]
 
@@ -32,7 +32,7 @@ _WIDER = {torch.float16: torch.float32, torch.bfloat16: torch.float32, torch.int
           torch.int8: torch.int32, torch.uint8: torch.int32}
 
 
-def _heads(what: str, q: torch.Tensor, k: torch.Tensor | None):
+def _heads(what: str, q: torch.Tensor, k: torch.Tensor | None) -> None:
     """The checks of q and k that need no device."""
     for name, t in (("q", q), ("k", k)):
         if t is None and name == "k":
@@ -41,13 +41,14 @@ def _heads(what: str, q: torch.Tensor, k: torch.Tensor | None):
             raise ValueError(f"{what}: {name} must be [B, N, H, d], got shape {tuple(t.shape)}")
         if t.dtype not in _DT:
             raise TypeError(f"{what}: {name} is {t.dtype}; bfloat16 and float32 are computed")
-    if q.shape[3] not in (32, 64, 128):
-        raise ValueError(f"{what}: head_dim must be 32, 64 or 128, got {q.shape[3]}")
-    if q.shape[2] == 0 or (k is not None and k.shape[2] == 0):
+    B, N, H, d = q.shape
+    if d not in (32, 64, 128):
+        raise ValueError(f"{what}: head_dim must be 32, 64 or 128, got {d}")
+    if H == 0 or (k is not None and k.shape[2] == 0):
         raise ValueError(f"{what}: q and k need a head")
-    if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype):
+    if k is not None and (k.shape[0] != B or k.shape[1] != N or k.shape[3] != d or k.dtype != q.dtype):
         raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} disagree")
-    if q.shape[0] * q.shape[1] >= 1 << 31:
+    if B * N >= 1 << 31:
         raise ValueError(f"{what}: B * N must be below 2^31")
 
 
@@ -58,11 +59,26 @@ def _no_grad_through(what: str, **tensors) -> None:
 
 
 def _same_device(what: str, q: torch.Tensor, **tensors) -> None:
-    if q.device.type != "cuda":
-        raise ValueError(f"{what}: q must be on a ROCm device, got {q.device}")
+    device = q.device
+    if device.type != "cuda":
+        raise ValueError(f"{what}: q must be on a ROCm device, got {device}")
     for name, t in tensors.items():
-        if t is not None and t.device != q.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, q on {q.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, q on {device}")
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device's context, entered only where another device is current (a call's host time counts
+    where it has one row: the context takes longer than the comparison)."""
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    """The handle of torch.cuda.current_stream(device), without making the stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _strides(t: torch.Tensor) -> list[int]:
@@ -70,89 +86,108 @@ def _strides(t: torch.Tensor) -> list[int]:
     return [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with contiguous, 16-byte aligned rows (copied only where they are not)."""
-    unit = 4 if t.dtype == torch.float32 else 8
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % unit for s in _strides(t)[:3]):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, _lib.Bnhd]:
+    """t with contiguous, 16-byte aligned rows (copied only where they are not), and as the kernels take it."""
+    sb, sn, sh, sd = t.stride()
+    unit = 3 if t.dtype == torch.float32 else 7
+    ptr = t.data_ptr()
+    if sd != 1 or ptr & 15 or (sb | sn | sh) & unit:
+        sb, sn, sh, _ = _strides(t)
+        if (sd != 1 and t.shape[3] > 1) or ptr & 15 or (sb | sn | sh) & unit:
+            t = t.clone(memory_format=torch.contiguous_format)
+            sb, sn, sh, _ = t.stride()
+            ptr = t.data_ptr()
+    return t, _lib.Bnhd(ptr, sb, sn, sh)
 
 
-def _bnhd(t: torch.Tensor | None) -> _lib.Bnhd:
-    return _lib.Bnhd() if t is None else _lib.Bnhd(t.data_ptr(), *_strides(t)[:3])
+_NONE = _lib.Bnhd()
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-@functools.lru_cache(maxsize=64)
-def _axes(sections: tuple, theta: tuple):
+@functools.lru_cache(maxsize=256)
+def _axes(what: str, sections: tuple, theta, half: int):
+    """(counts of pairs, their thetas) as the kernels take them, checked."""
     n = len(sections)
+    if not 1 <= n <= _lib.MAX_AXES or min(sections) < 0 or sum(sections) > half:
+        raise ValueError(f"{what}: sections {sections} must be 1 to {_lib.MAX_AXES} counts of pairs, at most {half} together")
+    theta = tuple(float(x) for x in theta) if isinstance(theta, tuple) else (float(theta),) * n
+    if len(theta) != n or not all(0 < x < math.inf for x in theta):
+        raise ValueError(f"{what}: theta must be a positive number, or one for each of the {n} axes")
     pad = (0,) * (_lib.MAX_AXES - n)
     return (ctypes.c_int32 * _lib.MAX_AXES)(*(sections + pad)), (ctypes.c_double * _lib.MAX_AXES)(*(theta + pad))
 
 
 def _positions(what: str, q: torch.Tensor, positions: torch.Tensor, sections, theta):
-    """(positions as the kernel takes them, sections, theta for each axis), checked."""
-    sections = tuple(int(n) for n in sections)
-    B, N, d = q.shape[0], q.shape[1], q.shape[3]
-    if not 1 <= len(sections) <= _lib.MAX_AXES or min(sections) < 0 or sum(sections) > d // 2:
-        raise ValueError(f"{what}: sections {sections} must be 1 to {_lib.MAX_AXES} counts of pairs, at most {d // 2} together")
-    theta = tuple(float(x) for x in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(sections)
-    if len(theta) != len(sections) or not all(0 < x < math.inf for x in theta):
-        raise ValueError(f"{what}: theta must be a positive number, or one for each of the {len(sections)} axes")
-    if tuple(positions.shape) not in ((N, len(sections)), (B, N, len(sections)), (1, N, len(sections))):
-        raise ValueError(f"{what}: positions {tuple(positions.shape)} must be [N, axes] or [B, N, axes] = "
-                         f"{(B, N, len(sections))}")
+    """(positions as the kernels take them, counts and thetas), checked."""
+    sections = tuple(map(int, sections))
+    axes = _axes(what, sections, tuple(theta) if isinstance(theta, list) else theta, q.shape[3] // 2)
+    B, N, n, shape = q.shape[0], q.shape[1], len(sections), positions.shape
+    if shape[-2:] != (N, n) or not (len(shape) == 2 or (len(shape) == 3 and shape[0] in (1, B))):
+        raise ValueError(f"{what}: positions {tuple(shape)} must be [N, axes] or [B, N, axes] = {(B, N, n)}")
     if positions.dtype in _WIDER:
         positions = positions.to(_WIDER[positions.dtype])
     if positions.dtype not in _POS:
         raise TypeError(f"{what}: positions are {positions.dtype}; floating and integer types are taken")
-    if positions.shape[-1] > 1 and positions.stride(-1) != 1:
+    if n > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    return positions, sections, theta
+    return positions, axes
 
 
 def _tables(what: str, q: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
     want = (q.shape[1], q.shape[3] // 2)
-    if tuple(cos.shape) != want or tuple(sin.shape) != want:
+    if cos.shape != want or sin.shape != want:
         raise ValueError(f"{what}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [N, d/2] = {want}")
     made = []
     for t in (cos, sin):
-        t = t.to(torch.float32).contiguous()
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            t = t.to(torch.float32).contiguous()
         made.append(t.clone() if t.data_ptr() % 16 else t)
     return made
 
 
-def _rotation(cos, sin, positions, sections, theta, interleaved: bool) -> _lib.Rotation | None:
+def _rotation(cos, sin, positions, axes, interleaved: bool) -> _lib.Rotation | None:
     r = _lib.Rotation()
-    r.interleaved = 1 if interleaved else 0
+    r.interleaved = interleaved
     if cos is not None:
         r.cos, r.sin = cos.data_ptr(), sin.data_ptr()
         return r
     if positions is None:
         return None
-    st = _strides(positions)
-    r.positions, r.position_type, r.num_axes = positions.data_ptr(), _POS[positions.dtype], len(sections)
-    r.stride_b, r.stride_n = (0 if positions.dim() == 2 else st[0]), st[-2]
-    r.sections, r.theta = _axes(sections, theta)
+    shape, stride = positions.shape, positions.stride()
+    r.positions, r.position_type, r.num_axes = positions.data_ptr(), _POS[positions.dtype], shape[-1]
+    r.stride_n = stride[-2]
+    if len(shape) == 3 and shape[0] > 1:
+        r.stride_b = stride[0]
+    r.sections, r.theta = axes
     return r
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _rotate(q, k, rotation, backward: bool, norm: bool, wq=None, wk=None, eps: float = 0.0):
     """mosaic_qk_rotate_fwd on q and k (k may be None)."""
     B, N, Hq, d = q.shape
-    Hk = 0 if k is None else k.shape[2]
-    q_out = torch.empty(B, N, Hq, d, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(B, N, Hk, d, dtype=q.dtype, device=q.device)
+    dtype, device = q.dtype, q.device
+    q_out = torch.empty((B, N, Hq, d), dtype=dtype, device=device)
+    Hk, k_out, kb, k_ptr = 0, None, _NONE, None
+    if k is not None:
+        Hk = k.shape[2]
+        k_out = torch.empty((B, N, Hk, d), dtype=dtype, device=device)
+        k_ptr = k_out.data_ptr()
     if B * N == 0:
         return q_out, k_out
-    q, k = _rows(q), None if k is None else _rows(k)
-    with torch.cuda.device(q.device):
+    q, qb = _rows(q)
+    if k is not None:
+        k, kb = _rows(k)
+    with _on(device):
         st = _lib.lib().mosaic_qk_rotate_fwd(
-            _bnhd(q), _bnhd(k), _DT[q.dtype], B, N, Hq, Hk, d, None if rotation is None else ctypes.byref(rotation),
-            int(backward), int(norm), _ptr(wq), _ptr(wk), eps, q_out.data_ptr(), _ptr(k_out), stream_of(q))
+            qb, kb, _DT[dtype], B, N, Hq, Hk, d, None if rotation is None else ctypes.byref(rotation), backward, norm,
+            _ptr(wq), _ptr(wk), eps, q_out.data_ptr(), k_ptr, _stream(device))
     _lib.check(st, "mosaic_qk_rotate_fwd")
     return q_out, k_out
 
@@ -161,19 +196,17 @@ class _RopeAxes(torch.autograd.Function):
     """The rotation; its gradient is the rotation back."""
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
-    def forward(ctx, q, k, positions, sections, theta, interleaved):
+    def forward(ctx, q, k, positions, axes, interleaved):
         ctx.save_for_backward(positions)
-        ctx.rest = (sections, theta, interleaved)
+        ctx.rest = (axes, interleaved)
         return _rotate(q, k, _rotation(None, None, positions, *ctx.rest), False, False)
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         (positions,) = ctx.saved_tensors
         dq, dk = _rotate(gq, gk, _rotation(None, None, positions, *ctx.rest), True, False)
-        return dq, dk, None, None, None, None
+        return dq, dk, None, None, None
 
 
 def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, sections, theta=10000.0, *,
@@ -191,53 +224,61 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, 
     """
     _heads("rope_axes", q, k)
     _no_grad_through("rope_axes", positions=positions)
-    positions, sections, theta = _positions("rope_axes", q, positions, sections, theta)
+    positions, axes = _positions("rope_axes", q, positions, sections, theta)
     _same_device("rope_axes", q, k=k, positions=positions)
-    return _RopeAxes.apply(q, k, positions, sections, theta, bool(interleaved))
+    if _wants_grad(q, k):
+        return _RopeAxes.apply(q, k, positions, axes, bool(interleaved))
+    return _rotate(q, k, _rotation(None, None, positions, axes, bool(interleaved)), False, False)
+
+
+def _fp32(w: torch.Tensor | None) -> torch.Tensor | None:
+    return w if w is None or (w.dtype == torch.float32 and w.is_contiguous()) else w.to(torch.float32).contiguous()
 
 
 class _QkNormRope(torch.autograd.Function):
     """The norm and rotation; the backward reads q and k again and forms the norms anew."""
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
-    def forward(ctx, q, k, q_weight, k_weight, eps, cos, sin, positions, sections, theta, interleaved):
+    def forward(ctx, q, k, q_weight, k_weight, eps, cos, sin, positions, axes, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.rest = (sections, theta, interleaved)
+        ctx.rest = (axes, interleaved)
         ctx.eps = eps
-        wq, wk = (None if w is None else w.to(torch.float32).contiguous() for w in (q_weight, k_weight))
-        return _rotate(q, k, _rotation(cos, sin, positions, *ctx.rest), False, True, wq, wk, eps)
+        return _rotate(q, k, _rotation(cos, sin, positions, *ctx.rest), False, True, _fp32(q_weight), _fp32(k_weight), eps)
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         B, N, Hq, d = q.shape
-        Hk = 0 if k is None else k.shape[2]
-        dev = q.device
-        dq = torch.empty(B, N, Hq, d, dtype=q.dtype, device=dev)
-        dk = None if k is None else torch.empty(B, N, Hk, d, dtype=q.dtype, device=dev)
+        dtype, device = q.dtype, q.device
+        dq = torch.empty((B, N, Hq, d), dtype=dtype, device=device)
+        Hk, dk, kb, gkb = 0, None, _NONE, _NONE
+        if k is not None:
+            Hk = k.shape[2]
+            dk = torch.empty((B, N, Hk, d), dtype=dtype, device=device)
         weights = (q_weight, k_weight)
-        dw = [torch.zeros(d, dtype=torch.float32, device=dev) if B * N == 0 else
-              torch.empty(d, dtype=torch.float32, device=dev) if w is not None and need else None
+        dw = [(torch.empty if B * N else torch.zeros)(d, dtype=torch.float32, device=device) if w is not None and need else None
               for w, need in zip(weights, ctx.needs_input_grad[2:4])]
         if B * N:
-            wq, wk = (None if w is None else w.to(torch.float32).contiguous() for w in weights)
-            gq, q = _rows(gq.to(q.dtype)), _rows(q)
-            gk, k = (None, None) if k is None else (_rows(gk.to(k.dtype)), _rows(k))
+            gq, gqb = _rows(gq)
+            q, qb = _rows(q)
+            if k is not None:
+                gk, gkb = _rows(gk)
+                k, kb = _rows(k)
+            wq, wk = map(_fp32, weights)
             rotation = _rotation(cos, sin, positions, *ctx.rest)
             L = _lib.lib()
-            nbytes = L.mosaic_qk_norm_bwd_workspace_size(B, N, d)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if any(w is not None for w in dw) else None
-            with torch.cuda.device(dev):
+            ws, nbytes = None, 0
+            if dw[0] is not None or dw[1] is not None:
+                nbytes = L.mosaic_qk_norm_bwd_workspace_size(B, N, d)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            with _on(device):
                 st = L.mosaic_qk_norm_rotate_bwd(
-                    _bnhd(gq), _bnhd(gk), _bnhd(q), _bnhd(k), _DT[q.dtype], B, N, Hq, Hk, d,
-                    None if rotation is None else ctypes.byref(rotation), _ptr(wq), _ptr(wk), ctx.eps, dq.data_ptr(),
-                    _ptr(dk), _ptr(dw[0]), _ptr(dw[1]), _ptr(ws), nbytes if ws is not None else 0, stream_of(q))
+                    gqb, gkb, qb, kb, _DT[dtype], B, N, Hq, Hk, d, None if rotation is None else ctypes.byref(rotation), _ptr(wq),
+                    _ptr(wk), ctx.eps, dq.data_ptr(), _ptr(dk), _ptr(dw[0]), _ptr(dw[1]), _ptr(ws), nbytes, _stream(device))
             _lib.check(st, "mosaic_qk_norm_rotate_bwd")
-        dw = [None if g is None or w is None else g.to(w.dtype) for g, w in zip(dw, weights)]
-        return (dq, dk, *dw) + (None,) * 7
+        dw = [None if g is None else g.to(w.dtype) for g, w in zip(dw, weights)]
+        return (dq, dk, *dw) + (None,) * 6
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None = None,
@@ -271,10 +312,13 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
         if w is not None and not w.dtype.is_floating_point:
             raise TypeError(f"{what}: {name} is {w.dtype}")
     _no_grad_through(what, cos=cos, sin=sin, positions=positions)
+    axes = None
     if cos is not None:
         cos, sin = _tables(what, q, cos, sin)
-        theta = ()
     elif positions is not None:
-        positions, sections, theta = _positions(what, q, positions, sections, theta)
+        positions, axes = _positions(what, q, positions, sections, theta)
     _same_device(what, q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
-    return _QkNormRope.apply(q, k, q_weight, k_weight, eps, cos, sin, positions, sections, theta, bool(interleaved))
+    interleaved = bool(interleaved)
+    if _wants_grad(q, k, q_weight, k_weight):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, eps, cos, sin, positions, axes, interleaved)
+    return _rotate(q, k, _rotation(cos, sin, positions, axes, interleaved), False, True, _fp32(q_weight), _fp32(k_weight), eps)

@@ -88,7 +88,9 @@ def test_abi_validation(fn, change, status):
 @HAVE_LIB
 def test_workspace_sizes():
     L = _lib.lib()
-    assert L.mosaic_query_attn_fwd_workspace_size(1, 49152, 12, 3, 16) == 0
+    # many tokens: their order alone (2 + 4 bytes each and kv head); one block each of one token: nothing
+    assert 6 * 3 * 49152 <= L.mosaic_query_attn_fwd_workspace_size(1, 49152, 12, 3, 16) < 7 * 3 * 49152
+    assert L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 3, 1) == 0
     one = L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 3, 16)
     assert one >= 16 * 12 * (64 * 4 + 8) and one % 256 == 0
     assert L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 5, 16) == 0       # refused shapes
