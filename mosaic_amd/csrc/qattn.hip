@@ -7,27 +7,29 @@
 // key is zeros (lse -inf).  fp32 scores, maxima, sums and accumulators; P is rounded to bf16 for
 // the PV product (an error of half a step of bf16 per term, as the output's own rounding).
 //
-// A workgroup takes 4 waves x QW = 32 / G tokens of one kv head, a wave the 32 rows (token, head) of
-// its tokens.  The tokens' sets are united in LDS (one 32-bit token mask per wave and block), and
+// A workgroup takes 4 waves x QW = 64 / G tokens of one kv head, a wave the 64 rows (token, head) of
+// its tokens (grad q: 32).  The tokens' sets are united in LDS (a token mask per wave and block), and
 // the union's blocks are staged once, 64 keys at a time, for all four waves; a wave skips the blocks
 // none of its tokens has.  Neighbouring tokens of a mesh mostly choose the same blocks, so the union
-// is little longer than one set (17.4 blocks for 32 tokens with 16 each on nside 64's field).  Tokens
-// in no such order are taken in the order of a block of theirs (query_order_kernel): 10007 scattered
-// points then unite 22 blocks instead of 313.  A row's result does not depend on the tokens beside
-// it: its own blocks come in ascending order in any union.
+// is little longer than one set (18 blocks for 64 tokens with 16 each on nside 64's field).  Tokens in
+// no such order are taken in the order of a block of theirs (query_order_kernel): 10007 scattered
+// points then unite 24 blocks instead of 460.
 //
-// Per tile of 64 keys, transposed so that a lane's 32 scores are one row's
+// Per tile of 64 keys, transposed so that a lane's scores are those of two rows
 // (v_mfma_f32_32x32x16_bf16, a row in lanes r and r + 32):
 //   S^T = K Q^T    A = K rows (16-byte LDS reads),  B = q (registers)
 //   O^T = V^T P^T  A = V^T (transposing LDS reads), B = P, which S^T's accumulators already hold in
 //                  operand order
-// 32 rows rather than 16 per wave (v_mfma_f32_16x16x32_bf16) halve the LDS reads per score, which
-// bound that variant.  The reference m of a row moves only when a score exceeds it by 2^8; l sums
-// the rounded P, so numerator and denominator share their roundings (the
-// log-sum-exp, where one is asked for, sums P unrounded).  The tile's product goes to
-// accumulators of its own and is added under the row's predicate: rows that are no members of the
-// block keep their state, nothing a row did not choose -- infinities and NaN among it -- reaches it,
-// and its sums are the same bits whoever shares its wave.
+// The reference m of a row moves only when a score exceeds it by 2^8; l sums the rounded P, so
+// numerator and denominator share their roundings (the log-sum-exp, where one is asked for, sums P
+// unrounded).  Rows that are no members of a block take P = 0, which leaves their accumulators' bits
+// as they are: a row's result does not depend on who shares its wave.  Only 0 * NaN would, so where a
+// workgroup ends with a value that is not finite it runs again, each product's accumulators restored
+// for the rows that are no members, and what a row did not choose does not reach it then either.
+//
+// 64 rows a wave rather than 32 (two waves a SIMD instead of three) halve LDS reads and barriers per
+// score and give a wave four independent chains of products: XXX us instead of 260 for the tokens
+// of nside 64; 16 rows (v_mfma_f32_16x16x32_bf16): 345.
 //
 // Few queries: the union is split over workgroups and the partial (m, l, O) joined by a second
 // kernel.
@@ -44,7 +46,7 @@ namespace mosaic {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kRowsPerWave = 32;
+constexpr int kFwdRows = 32, kDqRows = 32;   // rows (token, head) of a wave
 constexpr int kTileElems = 64 * 64;
 constexpr int kUnion = 1024;       // blocks whose members are marked at a time
 constexpr int kMaxSplit = 32;
@@ -75,7 +77,7 @@ struct QueryAttnParams {
     int32_t* far;              // [B, Hk, chunks of 256 tokens]
     int B, Nq, Nk, Hq, Hk, G, QW, bs, K, nb, words;
     int qtiles, splits;
-    int qw_inverse;            // t / QW = t qw_inverse >> 16 for t < 128
+    int qw_inverse;            // t / QW = t qw_inverse >> 16 for t < 256
     int short_rows;            // 64 rows of k and of v span less than 2^31 bytes
     float scale, c;
 };
@@ -92,6 +94,15 @@ __device__ __forceinline__ bf16x8 tr_pair(const bf16_t* lo, const bf16_t* hi) {
     const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                   (__attribute__((address_space(3))) v4i16*)(hi)));
     return as_bf16x8(make_uint4(a.x, a.y, b.x, b.y));
+}
+
+// Uses x, so that its load is waited for here.  A loop that counts direct-to-LDS loads itself has to
+// begin without loads of the compiler's in flight: it would wait for them in every round, by a count
+// that by then is that of the round's own loads, and the prefetch would overlap nothing.
+__device__ __forceinline__ void arrived(bf16x8& x) {
+    uint4 u = __builtin_bit_cast(uint4, x);
+    asm volatile("" : "+v"(u.x), "+v"(u.y), "+v"(u.z), "+v"(u.w));
+    x = as_bf16x8(u);
 }
 
 __device__ __forceinline__ int seq_keys(const QueryAttnParams& p, int b) {
@@ -195,18 +206,21 @@ __global__ __launch_bounds__(kOrderThreads) void query_order_kernel(QueryAttnPar
 
 // ------------------------------------------------------------------ tiles of a union
 
-// LDS of the forward and grad-q kernels
+// LDS of the forward (64 rows a wave) and grad-q (32) kernels
+template <int ROWS>
 struct RowsLds {
+    static constexpr int kWords = ROWS / 32;   // of a wave's token mask: bit t, its token t has the block
     __attribute__((aligned(1024))) bf16_t K[2][kTileElems];
     __attribute__((aligned(1024))) bf16_t V[2][kTileElems];
-    __attribute__((aligned(16))) uint32_t members[kUnion][kWaves];   // bit t: the wave's token t has the block
+    __attribute__((aligned(16))) uint32_t members[kUnion][kWaves * kWords];
     uint16_t list[kUnion];
-    int tokens[kWaves * kRowsPerWave];
+    int tokens[kWaves * ROWS];
     int found[kWaves];
 };
 
 // The workgroup's tokens (positions n0 .. of the order) into LDS; ends with a barrier.
-__device__ __forceinline__ void load_tokens(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0) {
+template <int ROWS>
+__device__ __forceinline__ void load_tokens(const QueryAttnParams& p, RowsLds<ROWS>& L, int b, int h, int n0) {
     const int64_t bh = (int64_t)b * p.Hk + h;
     const bool ordered = p.keys != nullptr && p.ordered[bh] != 0;
     for (int i = threadIdx.x; i < kWaves * p.QW; i += kThreads) {
@@ -219,30 +233,38 @@ __device__ __forceinline__ void load_tokens(const QueryAttnParams& p, RowsLds& L
 // Marks the members of blocks [c0, c0 + nc) among the workgroup's tokens and lists the blocks that
 // have any, ascending; returns their number.  of_split < splits leaves other splits' blocks out
 // (blocks u with u % splits == of_split remain).  Ends with a barrier.
-__device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int end, int c0, int nc,
+template <int ROWS>
+__device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds<ROWS>& L, int b, int h, int n0, int end, int c0, int nc,
                                      int of_split, int splits) {
+    constexpr int kWords = RowsLds<ROWS>::kWords;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < nc; i += kThreads) *reinterpret_cast<uint4*>(L.members[i]) = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < nc * kWords; i += kThreads) reinterpret_cast<uint4*>(L.members)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     // eight lanes a token
     const int tokens = min(kWaves * p.QW, p.Nq - n0);
     for (int t = tid >> 3; t < tokens; t += kThreads / 8) {
         const int64_t* e = p.idx + (((int64_t)b * p.Nq + L.tokens[t]) * p.Hk + h) * p.K;
-        const int w = (t * p.qw_inverse) >> 16;
-        const uint32_t bit = 1u << (t - w * p.QW);
+        const int w = (t * p.qw_inverse) >> 16, of_wave = t - w * p.QW;
+        const int word = w * kWords + (of_wave >> 5);
+        const uint32_t bit = 1u << (of_wave & 31);
         for (int kk = tid & 7; kk < p.K; kk += 8) {
             const int64_t blk = e[kk] - c0;
             if (blk < 0 || blk >= nc) continue;
             const int u = c0 + (int)blk;
             if ((int64_t)u * p.bs < end && (splits == 1 || (uint32_t)u % (uint32_t)splits == (uint32_t)of_split))
-                atomicOr(&L.members[blk][w], bit);
+                atomicOr(&L.members[blk][word], bit);
         }
     }
     __syncthreads();
     auto any = [&](int i) {
         if (i >= nc) return false;
-        const uint4 m = *reinterpret_cast<const uint4*>(L.members[i]);
-        return (m.x | m.y | m.z | m.w) != 0;
+        uint32_t m = 0;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+            const uint4 x = *reinterpret_cast<const uint4*>(&L.members[i][4 * w]);
+            m |= x.x | x.y | x.z | x.w;
+        }
+        return m != 0;
     };
     const int per = (nc + kThreads - 1) / kThreads * 64;   // blocks a wave lists
     int n = 0;
@@ -271,20 +293,19 @@ __device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds& L, int b
 // tile: from a uniform base with per-lane offsets that do not change (64 rows within 2^31 bytes), or
 // from 64-bit addresses, as the tile with the sequence's last key does, where the rows behind it
 // repeat it (V's are zeroed: what P = 0 multiplies there).
-template <typename Tile>
-__device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int split, int splits, Tile tile) {
+template <int ROWS, typename Tile>
+__device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds<ROWS>& L, int b, int h, int n0, int split, int splits, Tile tile) {
+    constexpr int kWords = RowsLds<ROWS>::kWords;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int end = seq_keys(p, b), sub = p.bs / 64;
     const bf16_t* kb = p.k + b * p.k_sb + h * p.k_sh;
     const bf16_t* vb = p.v + b * p.v_sb + h * p.v_sh;
     uint32_t ko[2], vo[2];
-    int row[2], chunk[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        row[i] = 16 * wave + 8 * i + (lane >> 3);
-        chunk[i] = 8 * ((lane & 7) ^ swz32(row[i]));
-        ko[i] = 2u * (uint32_t)(row[i] * p.k_sn + chunk[i]);
-        vo[i] = 2u * (uint32_t)(row[i] * p.v_sn + chunk[i]);
+        const int row = 16 * wave + 8 * i + (lane >> 3), chunk = 8 * ((lane & 7) ^ swz32(row));
+        ko[i] = 2u * (uint32_t)(row * p.k_sn + chunk);
+        vo[i] = 2u * (uint32_t)(row * p.v_sn + chunk);
     }
     auto stage = [&](int key0, int buf) {
         if (p.short_rows && key0 + 64 <= end) {
@@ -298,14 +319,15 @@ __device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds& L, 
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int64_t key = min(key0 + row[i], end - 1);
-                dma16_at(kb + key * p.k_sn + chunk[i], lds_addr(L.K[buf] + (16 * wave + 8 * i) * 64));
-                dma16_at(vb + key * p.v_sn + chunk[i], lds_addr(L.V[buf] + (16 * wave + 8 * i) * 64));
+                const int row = 16 * wave + 8 * i + (lane >> 3), chunk = 8 * ((lane & 7) ^ swz32(row));
+                const int64_t key = min(key0 + row, end - 1);
+                dma16_at(kb + key * p.k_sn + chunk, lds_addr(L.K[buf] + (16 * wave + 8 * i) * 64));
+                dma16_at(vb + key * p.v_sn + chunk, lds_addr(L.V[buf] + (16 * wave + 8 * i) * 64));
             }
         }
     };
-    // one token's worth of tiles: shares by position in the list; more: by block (see unite), so
-    // that a row's share does not depend on the tokens beside it
+    // without an order of tokens (few of them): shares by position in the list; else by block (see
+    // unite), so that a row's share does not depend on the tokens beside it
     const bool by_block = p.keys != nullptr;
     const int live = min(p.nb, (int)((uint32_t)(end + p.bs - 1) / (uint32_t)p.bs));   // blocks with a key
     for (int c0 = 0; c0 < live; c0 += kUnion) {
@@ -316,11 +338,12 @@ __device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds& L, 
             // up to 64 blocks of the list and this wave's members in registers: lane i holds block i
             const int count = min(64, past - e0);
             const int uv = L.list[e0 + min(lane, count - 1)];
-            const int mv = (int)L.members[uv][wave];
+            const int m0 = (int)L.members[uv][wave * kWords], m1 = kWords > 1 ? (int)L.members[uv][wave * kWords + kWords - 1] : 0;
             int key0 = (c0 + __builtin_amdgcn_readlane(uv, 0)) * p.bs, buf = 0;
             stage(key0, 0);
             for (int i = 0; i < count; ++i) {
-                const uint32_t members = (uint32_t)__builtin_amdgcn_readlane(mv, i);
+                uint64_t members = (uint32_t)__builtin_amdgcn_readlane(m0, i);
+                if (kWords > 1) members |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane(m1, i) << 32;
                 for (int st = 0; st < sub; ++st) {
                     const bool more = st + 1 < sub ? key0 + 64 < end : i + 1 < count;
                     const int next = st + 1 < sub ? key0 + 64 : (c0 + __builtin_amdgcn_readlane(uv, min(i + 1, 63))) * p.bs;
@@ -388,26 +411,31 @@ __device__ __forceinline__ float operand_sum(const bf16x8& x, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u.w), ones, acc, false);
 }
 
-// The rows of a wave, one per column r = lane % 32: token (position in the wave), query head, and
-// its place in [B, Nq, Hq]
+// Row r of a wave (column r % 32 of its row tile r / 32): token (position in the wave), query head,
+// and its place in [B, Nq, Hq]
 struct Row {
     int token, head;
     bool live;
     int64_t n, at;
-    __device__ __forceinline__ void init(const QueryAttnParams& p, const RowsLds& L, int b, int h, int n0, int wave, int lane) {
-        const int r = lane & 31;
+    template <int ROWS>
+    __device__ __forceinline__ void init(const QueryAttnParams& p, const RowsLds<ROWS>& L, int b, int h, int n0, int wave, int r) {
         token = r / p.G;
         live = token < p.QW && n0 + wave * p.QW + token < p.Nq;
         head = h * p.G + (live ? r - token * p.G : 0);
         n = L.tokens[wave * p.QW + (live ? token : 0)];
         at = ((int64_t)b * p.Nq + n) * p.Hq + head;
     }
+    __device__ __forceinline__ bool in(uint64_t members) const { return live && (members >> token & 1); }
 };
 
 __device__ __forceinline__ void load_row(const bf16_t* x, int64_t sb, int64_t sn, int64_t sh, int b, const Row& r, int lane, bf16x8 (&f)[4]) {
     const bf16_t* at = x + b * sb + r.n * sn + r.head * sh + 8 * (lane >> 5);
 #pragma unroll
     for (int ds = 0; ds < 4; ++ds) f[ds] = as_bf16x8(ld16(at + 16 * ds));
+}
+__device__ __forceinline__ void arrived(bf16x8 (&f)[4]) {
+#pragma unroll
+    for (int ds = 0; ds < 4; ++ds) arrived(f[ds]);
 }
 
 __device__ __forceinline__ void store_row(bf16_t* out, int64_t at, int lane, const f32x16 (&o)[2], float f) {
@@ -423,15 +451,169 @@ __device__ __forceinline__ void store_row(bf16_t* out, int64_t at, int lane, con
 // In a branch that is rarely taken: keeps the compiler from computing it always and selecting.
 __device__ __forceinline__ void seldom() { asm volatile(""); }
 
-// Scores of keys at or past `valid` become `fill` (accumulator element e of key half kt: key 32 kt + 8 (e / 4) + 4 hh + e % 4)
+// Scores of keys at or past `valid` become `fill` (accumulator element e of key half kt: key
+// 32 kt + 8 (e / 4) + 4 hh + e % 4).  `valid` is opaque to the compiler, which would otherwise keep
+// the comparisons of all calls in scalar registers at once.
 __device__ __forceinline__ void mask_keys(f32x16& s, int kt, int hh, int valid, float fill) {
+    int left = valid - 32 * kt - 4 * hh;
+    asm volatile("" : "+v"(left));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3) < valid ? s[e] : fill;
+    for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < left ? s[e] : fill;
+}
+
+constexpr int kRowTiles = kFwdRows / 32;   // of a wave
+struct FwdState {
+    f32x16 o[2][kRowTiles];   // O^T [dim tile][row tile]
+    float m[kRowTiles], l[kRowTiles], lx[kRowTiles];   // reference, and this lane's parts of the sums of the rounded and unrounded P
+};
+
+// SAFE: the rows that are no members of a tile get their accumulators back after its products
+template <bool LSE, bool SAFE>
+__device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds<kFwdRows>& L, int b, int h, int n0, int split,
+                                       const Row (&row)[kRowTiles], const bf16x8 (&qf)[kRowTiles][4], FwdState& a) {
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
+    TileReads tr;
+    tr.init(lane);
+#pragma unroll
+    for (int qt = 0; qt < kRowTiles; ++qt) {
+        a.o[0][qt] = splat(0.f);
+        a.o[1][qt] = splat(0.f);
+        a.m[qt] = -INFINITY;
+        a.l[qt] = a.lx[qt] = 0.f;
+    }
+    for_tiles(p, L, b, h, n0, split, p.splits, [&](const bf16_t* Kt, const bf16_t* Vt, uint64_t members, int valid) {
+        f32x16 s[2][kRowTiles];   // [key half][row tile]
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int qt = 0; qt < kRowTiles; ++qt) s[kt][qt] = splat(0.f);
+        // operands are read two steps ahead (at this register count the compiler would otherwise read
+        // each where it is used, and wait for it)
+        bf16x8 k[4][2];
+#pragma unroll
+        for (int ds = 0; ds < 2; ++ds)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) k[ds][kt] = tr.rows(Kt, 32 * kt, ds);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int qt = 0; qt < kRowTiles; ++qt) s[kt][qt] = mfma32(k[ds][kt], qf[qt][ds], s[kt][qt]);
+            if (ds < 2) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) k[ds + 2][kt] = tr.rows(Kt, 32 * kt, ds + 2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (valid < 64) {
+            seldom();
+#pragma unroll
+            for (int qt = 0; qt < kRowTiles; ++qt) {
+                mask_keys(s[0][qt], 0, hh, valid, -INFINITY);
+                mask_keys(s[1][qt], 1, hh, valid, -INFINITY);
+            }
+        }
+        // (the maximum that NaN wins takes three operands and no canonicalising instruction)
+        float mt[kRowTiles];
+        bool member[kRowTiles], move[kRowTiles], any = false;
+#pragma unroll
+        for (int qt = 0; qt < kRowTiles; ++qt) {
+            mt[qt] = s[0][qt][0];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mt[qt] = __builtin_elementwise_maximum(mt[qt], s[kt][qt][e]);
+            mt[qt] = xor32_max(mt[qt]) * p.c;
+            member[qt] = row[qt].in(members);
+            move[qt] = member[qt] && mt[qt] > a.m[qt] + kTau;
+            any |= move[qt];
+        }
+        if (__builtin_amdgcn_ballot_w64(any)) {   // rare after a row's first tile
+#pragma unroll
+            for (int qt = 0; qt < kRowTiles; ++qt) {
+                const float alpha = move[qt] ? __builtin_amdgcn_exp2f(a.m[qt] - mt[qt]) : 1.f;
+                a.m[qt] = move[qt] ? mt[qt] : a.m[qt];
+                a.o[0][qt] *= alpha;
+                a.o[1][qt] *= alpha;
+                a.l[qt] *= alpha;
+                if constexpr (LSE) a.lx[qt] *= alpha;
+            }
+        }
+        bf16x8 v[2];          // V^T of the first 16 keys: read before the exponentials
+        if constexpr (!SAFE) {
+            v[0] = tr.cols(Vt, 0, 0);
+            v[1] = tr.cols(Vt, 0, 1);
+        }
+        bf16x8 pb[kRowTiles][2][2];   // [row tile][key half][16-key step]
+#pragma unroll
+        for (int qt = 0; qt < kRowTiles; ++qt) {
+            const float ref = member[qt] ? a.m[qt] : INFINITY;   // P = 0 for the others
+            float lt[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][qt][8 * s2 + 2 * i], p.c, -ref));
+                        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][qt][8 * s2 + 2 * i + 1], p.c, -ref));
+                        if constexpr (LSE) sum[kt] += p0 + p1;
+                        w[i] = pack_bf16x2(p0, p1);
+                    }
+                    pb[qt][kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+                    lt[kt] = operand_sum(pb[qt][kt][s2], lt[kt]);
+                }
+            if (!SAFE || member[qt]) {
+                a.l[qt] += lt[0] + lt[1];
+                if constexpr (LSE) a.lx[qt] += sum[0] + sum[1];
+            }
+        }
+        if constexpr (SAFE) {
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+                for (int qt = 0; qt < kRowTiles; ++qt) {
+                    f32x16 y = a.o[dt][qt];
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int s2 = 0; s2 < 2; ++s2) y = mfma32(tr.cols(Vt, 32 * kt + 16 * s2, dt), pb[qt][kt][s2], y);
+                    if (member[qt]) a.o[dt][qt] = y;
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                bf16x8 next[2];
+                if (j < 3)
+#pragma unroll
+                    for (int dt = 0; dt < 2; ++dt) next[dt] = tr.cols(Vt, 16 * (j + 1), dt);
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+                    for (int qt = 0; qt < kRowTiles; ++qt) a.o[dt][qt] = mfma32(v[dt], pb[qt][j >> 1][j & 1], a.o[dt][qt]);
+                if (j < 3) {
+                    v[0] = next[0];
+                    v[1] = next[1];
+                }
+            }
+        }
+    });
+}
+
+// Whether every element of x is finite (their difference with themselves is 0)
+__device__ __forceinline__ bool finite(const f32x16& x) {
+    float d = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) d = fmaf(0.f, x[e], d);
+    return d == 0.f;
 }
 
 template <bool LSE>
-__global__ __launch_bounds__(kThreads, 3) void query_attn_kernel(QueryAttnParams p, int total) {
-    __shared__ RowsLds L;
+__global__ __launch_bounds__(kThreads, kFwdRows == 32 ? 3 : 2) void query_attn_kernel(QueryAttnParams p, int total) {
+    __shared__ RowsLds<kFwdRows> L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = xcd_remap(blockIdx.x, total);
@@ -439,91 +621,42 @@ __global__ __launch_bounds__(kThreads, 3) void query_attn_kernel(QueryAttnParams
     const int h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
     load_tokens(p, L, b, h, n0);
-    Row row;
-    row.init(p, L, b, h, n0, wave, lane);
-    bf16x8 qf[4];
-    load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
-    TileReads tr;
-    tr.init(lane);
-    f32x16 o[2] = {splat(0.f), splat(0.f)};
-    float m = -INFINITY, l = 0.f, lx = 0.f;    // l, lx: this lane's part of the sums of the rounded and unrounded P
-    for_tiles(p, L, b, h, n0, split, p.splits, [&](const bf16_t* Kt, const bf16_t* Vt, uint32_t members, int valid) {
-        f32x16 s[2] = {splat(0.f), splat(0.f)};
+    Row row[kRowTiles];
+    bf16x8 qf[kRowTiles][4];
 #pragma unroll
-        for (int ds = 0; ds < 4; ++ds)
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) s[kt] = mfma32(tr.rows(Kt, 32 * kt, ds), qf[ds], s[kt]);
-        if (valid < 64) {
-            seldom();
-            mask_keys(s[0], 0, hh, valid, -INFINITY);
-            mask_keys(s[1], 1, hh, valid, -INFINITY);
-        }
-        // (the maximum that NaN wins takes three operands and no canonicalising instruction)
-        float mt = s[0][0];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
-        mt = xor32_max(mt) * p.c;
-        const bool member = row.live && (members >> row.token & 1);
-        const bool move = member && mt > m + kTau;
-        if (__builtin_amdgcn_ballot_w64(move)) {   // rare after a row's first tile
-            const float alpha = move ? __builtin_amdgcn_exp2f(m - mt) : 1.f;
-            m = move ? mt : m;
-            o[0] *= alpha;
-            o[1] *= alpha;
-            l *= alpha;
-            lx *= alpha;
-        }
-        bf16x8 pb[2][2];
-        float lt[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i], p.c, -m));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i + 1], p.c, -m));
-                    if constexpr (LSE) sum[kt] += p0 + p1;
-                    w[i] = pack_bf16x2(p0, p1);
-                }
-                pb[kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-                lt[kt] = operand_sum(pb[kt][s2], lt[kt]);
-            }
-        if (member) {
-            l += lt[0] + lt[1];
-            if constexpr (LSE) lx += sum[0] + sum[1];
-        }
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt) {
-            f32x16 add = splat(0.f);
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) add = mfma32(tr.cols(Vt, 32 * kt + 16 * s2, dt), pb[kt][s2], add);
-            if (member) o[dt] += add;
-        }
-    });
-    l = xor32_add(l);
-    if constexpr (LSE) lx = xor32_add(lx);
-    if (!row.live) return;
-    if (p.splits > 1) {
-        const int64_t rows = (int64_t)p.B * p.Nq * p.Hq;
-        float* d = p.part_o + (split * rows + row.at) * 64 + 4 * hh;
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4)
-                *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) = make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
-        if (hh == 0) p.part_ml[split * rows + row.at] = make_float4(m, l, lx, 0.f);
-        return;
+    for (int qt = 0; qt < kRowTiles; ++qt) {
+        row[qt].init(p, L, b, h, n0, wave, 32 * qt + (lane & 31));
+        load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row[qt], lane, qf[qt]);
     }
-    // a row without a key has l = 0 (any other at least 2^-8, or NaN)
-    store_row(p.out, row.at, lane, o, l == 0.f ? 0.f : 1.f / l);
-    if constexpr (LSE)
-        if (hh == 0) p.lse[row.at] = m + __builtin_amdgcn_logf(lx);
+#pragma unroll
+    for (int qt = 0; qt < kRowTiles; ++qt) arrived(qf[qt]);
+    FwdState a;
+    attend<LSE, false>(p, L, b, h, n0, split, row, qf, a);
+    bool ok = true;
+#pragma unroll
+    for (int qt = 0; qt < kRowTiles; ++qt) ok = ok && finite(a.o[0][qt]) && finite(a.o[1][qt]) && a.l[qt] - a.l[qt] == 0.f;
+    if (__syncthreads_or(!ok)) attend<LSE, true>(p, L, b, h, n0, split, row, qf, a);
+#pragma unroll
+    for (int qt = 0; qt < kRowTiles; ++qt) {
+        const float l = xor32_add(a.l[qt]), lx = LSE ? xor32_add(a.lx[qt]) : 0.f;
+        if (!row[qt].live) continue;
+        const f32x16 o[2] = {a.o[0][qt], a.o[1][qt]};
+        if (p.splits > 1) {
+            const int64_t rows = (int64_t)p.B * p.Nq * p.Hq;
+            float* d = p.part_o + (split * rows + row[qt].at) * 64 + 4 * hh;
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4)
+                    *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) = make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+            if (hh == 0) p.part_ml[split * rows + row[qt].at] = make_float4(a.m[qt], l, lx, 0.f);
+            continue;
+        }
+        // a row without a key has l = 0 (any other at least 2^-8, or NaN)
+        store_row(p.out, row[qt].at, lane, o, l == 0.f ? 0.f : 1.f / l);
+        if constexpr (LSE)
+            if (hh == 0) p.lse[row[qt].at] = a.m[qt] + __builtin_amdgcn_logf(lx);
+    }
 }
 
 // Joins the splits' partials: 16 lanes a row, 4 dims each.  Lane j holds the weights of splits j and
@@ -587,7 +720,7 @@ __global__ __launch_bounds__(kThreads) void query_attn_join_kernel(QueryAttnPara
 // tile on operands at hand; without it grad q at 12288 tokens of nside 32 (12 blocks of 64) is
 // 5.1e-3 off (2-norm), with it 2.4e-3 (the output's own rounding alone: 1.7e-3).
 __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnParams p, int total) {
-    __shared__ RowsLds L;
+    __shared__ RowsLds<kDqRows> L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = xcd_remap(blockIdx.x, total);
@@ -596,7 +729,7 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
     const int n0 = tile_id * kWaves * p.QW;
     load_tokens(p, L, b, h, n0);
     Row row;
-    row.init(p, L, b, h, n0, wave, lane);
+    row.init(p, L, b, h, n0, wave, lane & 31);
     bf16x8 qf[4], gf[4];
     load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
     load_row(p.go, p.go_sb, p.go_sn, p.go_sh, b, row, lane, gf);
@@ -609,13 +742,16 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
         for (int i = 0; i < 4; ++i) delta = fmaf(bf_lo(ow[i]), bf_lo(gw[i]), fmaf(bf_hi(ow[i]), bf_hi(gw[i]), delta));
     }
     delta = xor32_add(delta);
-    const float nlse = -p.lse[row.at] / p.c;
+    float nlse = -p.lse[row.at] / p.c;
+    asm volatile("" : "+v"(nlse));
+    arrived(qf);
+    arrived(gf);
     TileReads tr;
     tr.init(lane);
     f32x16 dq[2] = {splat(0.f), splat(0.f)}, kbar[2] = {splat(0.f), splat(0.f)};   // sum dS' k, sum P k
     float sum = 0.f, rest_d = 0.f;   // this lane's parts of sum dS' and of sum P (do.v - delta)
-    for_tiles(p, L, b, h, n0, 0, 1, [&](const bf16_t* Kt, const bf16_t* Vt, uint32_t members, int valid) {
-        const bool member = row.live && (members >> row.token & 1);
+    for_tiles(p, L, b, h, n0, 0, 1, [&](const bf16_t* Kt, const bf16_t* Vt, uint64_t members, int valid) {
+        const bool member = row.in(members);
 #pragma unroll 1
         for (int kt = 0; kt < 2; ++kt) {
             f32x16 s = splat(nlse), dp = splat(-delta);
@@ -767,6 +903,8 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
                 kf[kk] = as_bf16x8(ld16(kr + 16 * kk));
                 vf[kk] = as_bf16x8(ld16(vr + 16 * kk));
             }
+            arrived(kf);
+            arrived(vf);
         }
         const bf16_t* qb = p.q + b * p.q_sb;
         const bf16_t* gb = p.go + b * p.go_sb;
@@ -928,7 +1066,7 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
     if (K > kMaxSelected) return MOSAIC_ERR_UNSUPPORTED;
     // ids of workgroups and keys stay in 31 bits
     if (nk > 0x7fffffff - bs || nq > 0x7fffffff - kMarkTokens) return MOSAIC_ERR_SHAPE;
-    const int64_t per = kWaves * (kRowsPerWave / (hq / hk)), tiles = ((int64_t)nq + per - 1) / per;
+    const int64_t per = kWaves * (kDqRows / (hq / hk)), tiles = ((int64_t)nq + per - 1) / per;
     if ((double)tiles * hk * batch * kMaxSplit > 2147483647.0) return MOSAIC_ERR_SHAPE;
     if ((double)((nk + 63) / 64) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
     if (((double)nq / kThreads + 1) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
@@ -937,15 +1075,15 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
 
 // Workgroups of one share: below one per CU the union is split, up to two per CU together.
 int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
-    const int64_t per = kWaves * (kRowsPerWave / (hq / hk));
+    const int64_t per = kWaves * (kFwdRows / (hq / hk));
     const int64_t wgs = (nq + per - 1) / per * hk * batch;
     if (wgs >= 256) return 1;
     const int64_t s = 512 / wgs;
     return (int)(s < K ? (s < kMaxSplit ? s : kMaxSplit) : (K < kMaxSplit ? K : kMaxSplit));
 }
 
-// Whether tokens may be taken in another order: with more than two workgroups of them.
-bool may_order(int32_t nq, int32_t hq, int32_t hk) { return nq > 2 * kWaves * (kRowsPerWave / (hq / hk)); }
+// Whether tokens may be taken in another order: with more than one workgroup of them.
+bool may_order(int32_t nq, int32_t hq, int32_t hk) { return nq > kWaves * (kFwdRows / (hq / hk)); }
 int key_chunks(int32_t nq) { return (nq + kThreads - 1) / kThreads; }
 size_t order_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
     if (!may_order(nq, hq, hk)) return 0;
@@ -963,12 +1101,12 @@ void place_order(QueryAttnParams& p, char* ws) {
 }
 
 void fill(QueryAttnParams& p, const mosaic_bnhd& q, const mosaic_bnhd& k, const mosaic_bnhd& v, const int64_t* idx,
-          const int32_t* lens, int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, int32_t bs, int32_t K, float scale) {
+          const int32_t* lens, int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, int32_t bs, int32_t K, float scale, int rows) {
     p.q = static_cast<const bf16_t*>(q.ptr); p.q_sb = q.stride_b; p.q_sn = q.stride_n; p.q_sh = q.stride_h;
     p.k = static_cast<const bf16_t*>(k.ptr); p.k_sb = k.stride_b; p.k_sn = k.stride_n; p.k_sh = k.stride_h;
     p.v = static_cast<const bf16_t*>(v.ptr); p.v_sb = v.stride_b; p.v_sn = v.stride_n; p.v_sh = v.stride_h;
     p.idx = idx; p.lens = lens;
-    p.B = batch; p.Nq = nq; p.Nk = nk; p.Hq = hq; p.Hk = hk; p.G = hq / hk; p.QW = kRowsPerWave / p.G; p.bs = bs; p.K = K;
+    p.B = batch; p.Nq = nq; p.Nk = nk; p.Hq = hq; p.Hk = hk; p.G = hq / hk; p.QW = rows / p.G; p.bs = bs; p.K = K;
     p.nb = (nk + bs - 1) / bs;
     p.qtiles = (nq + kWaves * p.QW - 1) / (kWaves * p.QW);
     p.splits = 1;
@@ -1019,7 +1157,7 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
     if (block_indices == nullptr || out == nullptr) return MOSAIC_ERR_NULL_POINTER;
     if (!aligned(block_indices, 8) || !aligned(out, 16) || !aligned(lse, 4) || !aligned(kv_lens, 4)) return MOSAIC_ERR_ALIGNMENT;
     QueryAttnParams p{};
-    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale);
+    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kFwdRows);
     p.out = static_cast<bf16_t*>(out);
     p.lse = lse;
     p.splits = choose_split(batch, num_queries, num_q_heads, num_kv_heads, block_count);
@@ -1068,7 +1206,7 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     const size_t need = mosaic_query_attn_bwd_workspace_size(batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size);
     if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)) return MOSAIC_ERR_WORKSPACE;
     QueryAttnParams p{};
-    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale);
+    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kDqRows);
     p.go = static_cast<const bf16_t*>(grad_out.ptr);
     p.go_sb = grad_out.stride_b; p.go_sn = grad_out.stride_n; p.go_sh = grad_out.stride_h;
     p.o = static_cast<const bf16_t*>(out);
