@@ -719,6 +719,89 @@ __global__ __launch_bounds__(kThreads) void query_attn_join_kernel(QueryAttnPara
 // here, and the exact one, delta + sum P (do.v - delta), goes to grad k / v.  One product more per
 // tile on operands at hand; without it grad q at 12288 tokens of nside 32 (12 blocks of 64) is
 // 5.1e-3 off (2-norm), with it 2.4e-3 (the output's own rounding alone: 1.7e-3).
+struct DqState {
+    f32x16 dq[2], kbar[2];   // sum dS' k, sum P k [dim tile]
+    float sum, rest;         // this lane's parts of sum dS' and of sum P (do.v - delta)
+};
+
+// SAFE as in the forward
+template <bool SAFE>
+__device__ __forceinline__ void differentiate(const QueryAttnParams& p, RowsLds<kDqRows>& L, int b, int h, int n0, const Row& row,
+                                              const bf16x8 (&qf)[4], const bf16x8 (&gf)[4], float nlse, float delta, DqState& a) {
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
+    TileReads tr;
+    tr.init(lane);
+    a.dq[0] = a.dq[1] = a.kbar[0] = a.kbar[1] = splat(0.f);
+    a.sum = a.rest = 0.f;
+    for_tiles(p, L, b, h, n0, 0, 1, [&](const bf16_t* Kt, const bf16_t* Vt, uint64_t members, int valid) {
+        const bool member = row.in(members);
+        const float off = member ? 0.f : -INFINITY;   // P = 0 and dS = 0 for the others
+#pragma unroll 1
+        for (int kt = 0; kt < 2; ++kt) {
+            f32x16 s = splat(nlse), dp = splat(-delta);
+            bf16x8 k[4], v[4];
+#pragma unroll
+            for (int ds = 0; ds < 2; ++ds) {
+                k[ds] = tr.rows(Kt, 32 * kt, ds);
+                v[ds] = tr.rows(Vt, 32 * kt, ds);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ds = 0; ds < 4; ++ds) {
+                s = mfma32(k[ds], qf[ds], s);
+                dp = mfma32(v[ds], gf[ds], dp);
+                if (ds < 2) {
+                    k[ds + 2] = tr.rows(Kt, 32 * kt, ds + 2);
+                    v[ds + 2] = tr.rows(Vt, 32 * kt, ds + 2);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (valid < 64) {
+                seldom();
+                mask_keys(s, kt, hh, valid, -INFINITY);
+                mask_keys(dp, kt, hh, valid, 0.f);
+            }
+            bf16x8 pb[2], db[2];
+            float dsum = 0.f, rsum = 0.f;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                uint32_t w[4], x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 8 * s2 + 2 * i;
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, off)), p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], p.c, off));
+                    const float d0 = p0 * dp[e], d1 = p1 * dp[e + 1];
+                    dsum += d0 + d1;
+                    w[i] = pack_bf16x2(p0, p1);
+                    x[i] = pack_bf16x2(d0, d1);
+                }
+                pb[s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+                db[s2] = as_bf16x8(make_uint4(x[0], x[1], x[2], x[3]));
+                rsum = operand_sum(db[s2], rsum);
+            }
+            if (!SAFE || member) {
+                a.sum += rsum;
+                a.rest += dsum;
+            }
+            f32x16 dq[2] = {a.dq[0], a.dq[1]}, kbar[2] = {a.kbar[0], a.kbar[1]};
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt) {
+                    const bf16x8 kT = tr.cols(Kt, 32 * kt + 16 * s2, dt);
+                    dq[dt] = mfma32(kT, db[s2], dq[dt]);
+                    kbar[dt] = mfma32(kT, pb[s2], kbar[dt]);
+                }
+            if (!SAFE || member) {
+                a.dq[0] = dq[0];
+                a.dq[1] = dq[1];
+                a.kbar[0] = kbar[0];
+                a.kbar[1] = kbar[1];
+            }
+        }
+    });
+}
+
 __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnParams p, int total) {
     __shared__ RowsLds<kDqRows> L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
@@ -746,74 +829,20 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
     asm volatile("" : "+v"(nlse));
     arrived(qf);
     arrived(gf);
-    TileReads tr;
-    tr.init(lane);
-    f32x16 dq[2] = {splat(0.f), splat(0.f)}, kbar[2] = {splat(0.f), splat(0.f)};   // sum dS' k, sum P k
-    float sum = 0.f, rest_d = 0.f;   // this lane's parts of sum dS' and of sum P (do.v - delta)
-    for_tiles(p, L, b, h, n0, 0, 1, [&](const bf16_t* Kt, const bf16_t* Vt, uint64_t members, int valid) {
-        const bool member = row.in(members);
-#pragma unroll 1
-        for (int kt = 0; kt < 2; ++kt) {
-            f32x16 s = splat(nlse), dp = splat(-delta);
-#pragma unroll
-            for (int ds = 0; ds < 4; ++ds) {
-                s = mfma32(tr.rows(Kt, 32 * kt, ds), qf[ds], s);
-                dp = mfma32(tr.rows(Vt, 32 * kt, ds), gf[ds], dp);
-            }
-            if (valid < 64) {
-                seldom();
-                mask_keys(s, kt, hh, valid, -INFINITY);
-                mask_keys(dp, kt, hh, valid, 0.f);
-            }
-            bf16x8 pb[2], db[2];
-            float dsum = 0.f, rsum = 0.f;
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                uint32_t w[4], x[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = 8 * s2 + 2 * i;
-                    const float p0 = __builtin_amdgcn_exp2f(s[e] * p.c), p1 = __builtin_amdgcn_exp2f(s[e + 1] * p.c);
-                    const float d0 = p0 * dp[e], d1 = p1 * dp[e + 1];
-                    dsum += d0 + d1;
-                    w[i] = pack_bf16x2(p0, p1);
-                    x[i] = pack_bf16x2(d0, d1);
-                }
-                pb[s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-                db[s2] = as_bf16x8(make_uint4(x[0], x[1], x[2], x[3]));
-                rsum = operand_sum(db[s2], rsum);
-            }
-#pragma unroll
-            for (int dt = 0; dt < 2; ++dt) {
-                f32x16 da = splat(0.f), ka = splat(0.f);
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    const bf16x8 kT = tr.cols(Kt, 32 * kt + 16 * s2, dt);
-                    da = mfma32(kT, db[s2], da);
-                    ka = mfma32(kT, pb[s2], ka);
-                }
-                if (member) {
-                    dq[dt] += da;
-                    kbar[dt] += ka;
-                }
-            }
-            if (member) {
-                sum += rsum;
-                rest_d += dsum;
-            }
-        }
-    });
-    rest_d = xor32_add(rest_d);
-    sum = xor32_add(sum);
+    DqState a;
+    differentiate<false>(p, L, b, h, n0, row, qf, gf, nlse, delta, a);
+    const bool ok = finite(a.dq[0]) && finite(a.dq[1]) && finite(a.kbar[0]) && finite(a.kbar[1]) && a.sum - a.sum == 0.f && a.rest - a.rest == 0.f;
+    if (__syncthreads_or(!ok)) differentiate<true>(p, L, b, h, n0, row, qf, gf, nlse, delta, a);
+    const float more = xor32_add(a.rest), sum = xor32_add(a.sum);
     if (!row.live) return;
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dq[dt][e] = fmaf(-sum, kbar[dt][e], dq[dt][e]);
-    store_row(p.out, row.at, lane, dq, p.scale);
+        for (int e = 0; e < 16; ++e) a.dq[dt][e] = fmaf(-sum, a.kbar[dt][e], a.dq[dt][e]);
+    store_row(p.out, row.at, lane, a.dq, p.scale);
     if (hh == 0) {
         p.nlse[row.at] = nlse;
-        p.ndelta[row.at] = -(delta + rest_d);
+        p.ndelta[row.at] = -(delta + more);
     }
 }
 
@@ -851,9 +880,9 @@ constexpr int kSegWords = 128;                 // words of marks listed at a tim
 constexpr int kListed = 32 * kSegWords + 64;   // and what was left of the last ones
 
 struct KeysLds {
-    __attribute__((aligned(1024))) bf16_t q[2][kTileElems];
-    __attribute__((aligned(1024))) bf16_t g[2][kTileElems];
-    float nlse[2][64], ndelta[2][64];
+    __attribute__((aligned(1024))) bf16_t q[3][kTileElems];
+    __attribute__((aligned(1024))) bf16_t g[3][kTileElems];
+    float nlse[3][64], ndelta[3][64];
     int list[kListed];
     int sums[2];
 };
@@ -908,16 +937,22 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
         }
         const bf16_t* qb = p.q + b * p.q_sb;
         const bf16_t* gb = p.go + b * p.go_sb;
-        // step s's rows into buffer s & 1; entries past the list repeat its last one
-        auto request = [&](int s, int count) {
-            const int buf = s & 1;
+        int64_t qoff[2], goff[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int chunk = 8 * ((lane & 7) ^ swz32(16 * w + 8 * i + (lane >> 3)));
+            qoff[i] = lhead[i] * p.q_sh + chunk;
+            goff[i] = lhead[i] * p.go_sh + chunk;
+        }
+        // Step s's rows into slot `buf`; entries past the list repeat its last one.  Six loads a wave,
+        // whatever the step, so that waiting for all but the newest request is one count.
+        auto request = [&](int s, int buf, int count) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int64_t n = L.list[min(s * QS + ltok[i], count - 1)];
-                const int row0 = 16 * w + 8 * i, row = row0 + (lane >> 3);
-                const int chunk = 8 * ((lane & 7) ^ swz32(row));
-                dma16_at(qb + n * p.q_sn + lhead[i] * p.q_sh + chunk, lds_addr(L.q[buf] + row0 * 64));
-                dma16_at(gb + n * p.go_sn + lhead[i] * p.go_sh + chunk, lds_addr(L.g[buf] + row0 * 64));
+                const int row0 = 16 * w + 8 * i;
+                dma16_at(qb + n * p.q_sn + qoff[i], lds_addr(L.q[buf] + row0 * 64));
+                dma16_at(gb + n * p.go_sn + goff[i], lds_addr(L.g[buf] + row0 * 64));
             }
             const int64_t at = ((int64_t)b * p.Nq + L.list[min(s * QS + ltok[2], count - 1)]) * p.Hq + lhead[2];
             if (lane < 16) {
@@ -986,13 +1021,19 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
             __syncthreads();
             const bool last = w0 + kSegWords >= p.words;
             const int steps = last ? (count + QS - 1) / QS : count / QS;
-            if (steps > 0) request(0, count);
-            for (int s = 0; s < steps; ++s) {
-                wait_vmem();
-                lds_barrier();
-                if (s + 1 < steps) request(s + 1, count);
-                step(s & 1, min(QS, count - s * QS) * p.G);
+            // a ring of three slots: a step's rows are requested two steps before it
+            if (steps > 0) {
+                request(0, 0, count);
+                request(1, 1, count);
             }
+            for (int s = 0, buf = 0; s < steps; ++s) {
+                asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+                lds_barrier();
+                request(s + 2, buf == 0 ? 2 : buf - 1, count);
+                step(buf, min(QS, count - s * QS) * p.G);
+                buf = buf == 2 ? 0 : buf + 1;
+            }
+            wait_vmem();
             // the tokens left over go to the list's front
             const int rest_n = count - steps * QS;
             int keep = 0;
