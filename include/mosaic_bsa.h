@@ -520,7 +520,8 @@ MOSAIC_API int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v
    sequence's end), sums in a fixed order.  workspace: mosaic_query_attn_bwd_workspace_size()
    bytes, 256-byte aligned. */
 MOSAIC_API size_t mosaic_query_attn_bwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_keys,
-                                                       int32_t num_q_heads, int32_t num_kv_heads, int32_t block_size);
+                                                       int32_t num_q_heads, int32_t num_kv_heads, int32_t block_size,
+                                                       int32_t block_count);
 MOSAIC_API int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const void* out, const float* lse,
                                      mosaic_bnhd grad_out, const int64_t* block_indices, const int32_t* kv_lens,
                                      int32_t batch, int32_t num_queries, int32_t num_keys, int32_t num_q_heads,

@@ -70,6 +70,12 @@ struct QueryAttnParams {
     float* nlse;               // backward: -lse / c and -sum(o do) of each row
     float* ndelta;
     uint32_t* marks;           // backward: [B, Hk, nb, words] bit n: token n has the block
+    int32_t* counts;           // backward: [B, Hk, nb] tokens of each block
+    int2* items;               // backward: (key tile, share | shares << 16) of each workgroup of grad k / v
+    int32_t* slots;            // backward: [key tiles] first partial of a tile in several shares, else -1;
+                               // then the number of items
+    float* parts;              // backward: [slots, 2, 64 keys, 64] partials of grad k, grad v
+    int share;                 // tokens of one share at most
     bf16_t* dk; bf16_t* dv;    // [B, Nk, Hk, 64]
     uint16_t* keys;            // [B, Hk, Nq] bucket of each token (null: tokens in their own order)
     int32_t* order;            // [B, Hk, Nq] tokens in the order they are taken in,
@@ -810,6 +816,8 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
     const int tile_id = id % p.qtiles, rest = id / p.qtiles;
     const int h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)p.B * p.Hk * p.nb; i += (int64_t)total * kThreads)
+        p.counts[i] = 0;   // for query_marks_kernel
     load_tokens(p, L, b, h, n0);
     Row row;
     row.init(p, L, b, h, n0, wave, lane & 31);
@@ -847,8 +855,8 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
 }
 
 // The tokens of each block, as bits: a workgroup takes 512 tokens (16 words) of one kv head and up
-// to kUnion blocks, marks in LDS and writes every word, so nothing needs clearing and no order of
-// atomics reaches memory.
+// to kUnion blocks, marks in LDS and writes every word, so they need no clearing; the blocks' numbers
+// of tokens are added up beside them (integers: their order does not matter).
 constexpr int kMarkTokens = 512, kMarkWords = kMarkTokens / 32;
 __global__ __launch_bounds__(kThreads) void query_marks_kernel(QueryAttnParams p, int groups) {
     __shared__ __attribute__((aligned(16))) uint32_t bits[kUnion * kMarkWords];
@@ -869,10 +877,82 @@ __global__ __launch_bounds__(kThreads) void query_marks_kernel(QueryAttnParams p
         const int blk = i / (kMarkWords / 4), w = i % (kMarkWords / 4) * 4;
         *reinterpret_cast<uint4*>(out + (int64_t)blk * p.words + w) = *reinterpret_cast<const uint4*>(bits + blk * kMarkWords + w);
     }
+    int32_t* counts = p.counts + ((int64_t)b * p.Hk + h) * p.nb + c0;
+    for (int i = threadIdx.x; i < nc; i += kThreads) {
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < kMarkWords; ++w) n += __builtin_popcount(bits[i * kMarkWords + w]);
+        if (n > 0) atomicAdd(&counts[i], n);
+    }
 }
 
-// grad k, grad v.  One workgroup = 64 keys of one kv head: it walks the tokens that have the block,
-// QS = 64 / G at a time (64 rows of q and do gathered straight into LDS).  Wave w = (key half w / 2,
+// The workgroups of grad k / v: a tile of 64 keys whose block has more than p.share tokens is split
+// into equal shares of them (blocks differ in popularity by factors: the most wanted one would run
+// long after the others are done).  One workgroup; items are in the order of the tiles.
+__global__ __launch_bounds__(1024) void query_plan_kernel(QueryAttnParams p, int tiles, int total) {
+    __shared__ int sums[16][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int items = 0, slots = 0;
+    for (int i0 = 0; i0 < total; i0 += 1024) {
+        const int i = i0 + tid;
+        int shares = 0;
+        if (i < total) {
+            const int kt = i % tiles, bh = i / tiles;
+            const int count = p.counts[(int64_t)bh * p.nb + (int64_t)kt * 64 / p.bs];
+            shares = max(1, (count + p.share - 1) / p.share);
+        }
+        const int held = shares > 1 ? shares : 0;
+        int a = shares, c = held;   // prefix sums over the wave, then over the waves
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(a, d), y = __shfl_up(c, d);
+            a += lane >= d ? x : 0;
+            c += lane >= d ? y : 0;
+        }
+        if (lane == 63) {
+            sums[wave][0] = a;
+            sums[wave][1] = c;
+        }
+        __syncthreads();
+        int at = items + a - shares, slot = slots + c - held;
+        for (int w = 0; w < 16; ++w) {
+            at += w < wave ? sums[w][0] : 0;
+            slot += w < wave ? sums[w][1] : 0;
+            items += sums[w][0];
+            slots += sums[w][1];
+        }
+        for (int j = 0; j < shares; ++j) p.items[at + j] = make_int2(i, j | shares << 16);
+        if (i < total) p.slots[i] = shares > 1 ? slot : -1;
+        __syncthreads();
+    }
+    if (tid == 0) p.slots[total] = items;
+}
+
+// Sums of a split tile's partials, in the order of the shares.
+__global__ __launch_bounds__(kThreads) void query_sum_kernel(QueryAttnParams p, int tiles) {
+    const int i = blockIdx.x, slot = p.slots[i];
+    if (slot < 0) return;
+    const int kt = i % tiles, bh = i / tiles, h = bh % p.Hk, b = bh / p.Hk;
+    const int count = p.counts[(int64_t)bh * p.nb + (int64_t)kt * 64 / p.bs];
+    const int shares = (count + p.share - 1) / p.share;
+    // a thread: 4 dims of 8 rows of the 2 x 64
+    const int d = threadIdx.x % 16 * 4;
+    for (int r = threadIdx.x / 16; r < 128; r += kThreads / 16) {
+        const int key = kt * 64 + r % 64;
+        if (key >= p.Nk) continue;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int j = 0; j < shares; ++j) {
+            const float4 x = *reinterpret_cast<const float4*>(p.parts + ((int64_t)(slot + j) * 128 + r) * 64 + d);
+            y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+        }
+        bf16_t* out = (r < 64 ? p.dk : p.dv) + (((int64_t)b * p.Nk + key) * p.Hk + h) * 64 + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+    }
+}
+
+// grad k, grad v.  One workgroup = 64 keys of one kv head and its share of the tokens that have the
+// block: it walks them QS = 64 / G at a time (64 rows of q and do gathered straight into LDS).  Wave w = (key half w / 2,
 // row half w % 2) forms S = q k^T and dP = do v^T of its 32 rows x 32 keys
 // (v_mfma_f32_32x32x16_bf16); P and dS stay in registers as the B operands of dV^T += do^T P and
 // dK^T += q^T dS, whose A operands are transposing LDS reads.  The row halves are added at the end.
@@ -891,9 +971,14 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
     __shared__ KeysLds L;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), kh = w >> 1, qh = w & 1;
-    const int id = xcd_remap(blockIdx.x, total);
-    const int kt = id % tiles, rest = id / tiles, h = rest % p.Hk, b = rest / p.Hk;
+    const int items = p.slots[total];
+    if ((int)blockIdx.x >= items) return;
+    const int2 item = p.items[xcd_remap(blockIdx.x, items)];
+    const int kt = item.x % tiles, rest = item.x / tiles, h = rest % p.Hk, b = rest / p.Hk;
+    const int share = item.y & 0xffff, shares = item.y >> 16;
     const int key0 = kt * 64, end = seq_keys(p, b);
+    const int64_t all = p.counts[((int64_t)b * p.Hk + h) * p.nb + key0 / p.bs];
+    const int from = (int)(all * share / shares), past = (int)(all * (share + 1) / shares);   // this share's tokens, by rank
     const uint32_t* marks = p.marks + (((int64_t)b * p.Hk + h) * p.nb + key0 / p.bs) * p.words;
     const int QS = 64 / p.G;
 
@@ -1001,9 +1086,9 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
                     dkT[dt] = mfma32(tr_read(Qc, 32 * qh + 16 * ch, dt), db[ch], dkT[dt]);
                 }
         };
-        int count = 0;   // tokens listed
-        for (int w0 = 0; w0 < p.words; w0 += kSegWords) {
-            // list the tokens of words w0 .. behind the ones left over: waves 0 and 1, a word per lane
+        int count = 0, seen = 0;   // tokens listed, and passed in the marks
+        for (int w0 = 0; w0 < p.words && seen < past; w0 += kSegWords) {
+            // list this share's tokens of words w0 .. behind the ones left over: waves 0 and 1, a word per lane
             const uint32_t word = w < 2 && w0 + tid < p.words ? marks[w0 + tid] : 0;
             int before = __builtin_popcount(word);
 #pragma unroll
@@ -1013,13 +1098,16 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
             }
             if (w < 2 && lane == 63) L.sums[w] = before;
             __syncthreads();
+            const int first = max(from, seen);
             if (w < 2) {
-                int at = count + before - __builtin_popcount(word) + (w == 1 ? L.sums[0] : 0);
-                for (uint32_t m = word; m != 0; m &= m - 1) L.list[at++] = 32 * (w0 + tid) + __builtin_ctz(m);
+                int rank = seen + before - __builtin_popcount(word) + (w == 1 ? L.sums[0] : 0);
+                for (uint32_t m = word; m != 0; m &= m - 1, ++rank)
+                    if (rank >= first && rank < past) L.list[count + rank - first] = 32 * (w0 + tid) + __builtin_ctz(m);
             }
-            count += L.sums[0] + L.sums[1];
+            seen += L.sums[0] + L.sums[1];
+            count += max(0, min(seen, past) - first);
             __syncthreads();
-            const bool last = w0 + kSegWords >= p.words;
+            const bool last = w0 + kSegWords >= p.words || seen >= past;
             const int steps = last ? (count + QS - 1) / QS : count / QS;
             // a ring of three slots: a step's rows are requested two steps before it
             if (steps > 0) {
@@ -1066,6 +1154,23 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
         }
     }
     const int key = key0 + 32 * kh + r;
+    if (shares > 1) {
+        if (qh == 0) {   // rows past the sequence's end too: zeros
+            float* d = p.parts + ((int64_t)(p.slots[item.x] + share) * 128 + 32 * kh + r) * 64 + 4 * hh;
+            const bool on = key < end;
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const f32x16 &x = dkT[dt], &y = dvT[dt];
+                    *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) =
+                        on ? make_float4(x[4 * g4] * p.scale, x[4 * g4 + 1] * p.scale, x[4 * g4 + 2] * p.scale, x[4 * g4 + 3] * p.scale) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    *reinterpret_cast<float4*>(d + 64 * 64 + 32 * dt + 8 * g4) =
+                        on ? make_float4(y[4 * g4], y[4 * g4 + 1], y[4 * g4 + 2], y[4 * g4 + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+        }
+        return;
+    }
     if (qh == 0 && key < p.Nk) {   // zeros for keys past the sequence's end
         const int64_t base = (((int64_t)b * p.Nk + key) * p.Hk + h) * 64;
         const bool on = key < end;
@@ -1164,6 +1269,38 @@ hipError_t launch(const void* fn, dim3 grid, void** args, hipStream_t s, int thr
     return hipLaunchKernel(fn, grid, dim3(threads), args, 0, s);
 }
 
+// Workspace of the backward, and the tokens of one share of a key tile: half as many again as a block
+// has on average, fewer where the tiles alone do not fill the chip twice.
+struct BwdLayout {
+    size_t nlse, ndelta, marks, counts, plan, slots, parts, order, bytes;
+    int64_t items;   // workgroups of grad k / v at most
+    int share;
+};
+BwdLayout bwd_layout(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, int32_t bs, int32_t K) {
+    BwdLayout a{};
+    const int64_t nb = ((int64_t)nk + bs - 1) / bs, tiles = ((int64_t)nk + 63) / 64 * hk * batch;
+    const int64_t chosen = (int64_t)nq * (K < nb ? K : nb);                // (token, block) pairs of a kv head at most
+    const int64_t pairs = chosen * hk * batch * (bs / 64);                 // (token, key tile)
+    int64_t share = chosen / nb * 3 / 2;
+    if (tiles < 512 && share > pairs / 512) share = pairs / 512;
+    if (share < 64) share = 64;
+    if (share < (nq + 4095) / 4096) share = (nq + 4095) / 4096;            // a tile's shares are counted in 16 bits
+    a.share = (int)(share < 0x7fffffff ? share : 0x7fffffff);
+    // a tile with c tokens has at most 1 + c / share shares, of one with several there are 2 c / share at most
+    a.items = tiles + pairs / a.share;
+    const int64_t slots = 2 * (pairs / a.share) + 2;
+    const size_t rows = up((size_t)batch * nq * hq * sizeof(float));
+    a.ndelta = a.nlse + rows;
+    a.marks = a.ndelta + rows;
+    a.counts = a.marks + up((size_t)batch * hk * nb * words_of(nq) * sizeof(uint32_t));
+    a.plan = a.counts + up((size_t)batch * hk * nb * sizeof(int32_t));
+    a.slots = a.plan + up((size_t)a.items * sizeof(int2));
+    a.parts = a.slots + up((size_t)(tiles + 1) * sizeof(int32_t));
+    a.order = a.parts + up((size_t)slots * 128 * kHeadDim * sizeof(float));
+    a.bytes = a.order + order_bytes(batch, nq, hq, hk);
+    return a;
+}
+
 int launch_order(QueryAttnParams& p, hipStream_t s) {
     if (p.keys == nullptr) return MOSAIC_OK;
     int chunks = key_chunks(p.Nq);
@@ -1225,11 +1362,9 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
 }
 
 size_t mosaic_query_attn_bwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_keys, int32_t num_q_heads,
-                                            int32_t num_kv_heads, int32_t block_size) {
-    if (check_shape(batch, num_queries, num_keys, num_q_heads, num_kv_heads, kHeadDim, block_size, 1) != MOSAIC_OK) return 0;
-    const size_t rows = (size_t)batch * num_queries * num_q_heads, nb = ((size_t)num_keys + block_size - 1) / block_size;
-    return 2 * up(rows * sizeof(float)) + up((size_t)batch * num_kv_heads * nb * words_of(num_queries) * sizeof(uint32_t)) +
-           order_bytes(batch, num_queries, num_q_heads, num_kv_heads);
+                                            int32_t num_kv_heads, int32_t block_size, int32_t block_count) {
+    if (check_shape(batch, num_queries, num_keys, num_q_heads, num_kv_heads, kHeadDim, block_size, block_count) != MOSAIC_OK) return 0;
+    return bwd_layout(batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count).bytes;
 }
 
 int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const void* out, const float* lse, mosaic_bnhd grad_out,
@@ -1244,21 +1379,26 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     for (const void* t : {out, (const void*)grad_q, (const void*)grad_k, (const void*)grad_v})
         if (!aligned(t, 16)) return MOSAIC_ERR_ALIGNMENT;
     if (!aligned(block_indices, 8) || !aligned(lse, 4) || !aligned(kv_lens, 4)) return MOSAIC_ERR_ALIGNMENT;
-    const size_t need = mosaic_query_attn_bwd_workspace_size(batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size);
-    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)) return MOSAIC_ERR_WORKSPACE;
+    const BwdLayout at = bwd_layout(batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count);
+    if (workspace == nullptr || workspace_bytes < at.bytes || !aligned(workspace, 256)) return MOSAIC_ERR_WORKSPACE;
+    if (at.items > 0x7fffffff) return MOSAIC_ERR_SHAPE;
     QueryAttnParams p{};
     fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kDqRows);
     p.go = static_cast<const bf16_t*>(grad_out.ptr);
     p.go_sb = grad_out.stride_b; p.go_sn = grad_out.stride_n; p.go_sh = grad_out.stride_h;
     p.o = static_cast<const bf16_t*>(out);
     p.lse = const_cast<float*>(lse);
-    const size_t row_bytes = up((size_t)batch * num_queries * num_q_heads * sizeof(float));
-    p.nlse = static_cast<float*>(workspace);
-    p.ndelta = reinterpret_cast<float*>(static_cast<char*>(workspace) + row_bytes);
-    p.marks = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + 2 * row_bytes);
+    char* ws = static_cast<char*>(workspace);
+    p.nlse = reinterpret_cast<float*>(ws + at.nlse);
+    p.ndelta = reinterpret_cast<float*>(ws + at.ndelta);
+    p.marks = reinterpret_cast<uint32_t*>(ws + at.marks);
+    p.counts = reinterpret_cast<int32_t*>(ws + at.counts);
+    p.items = reinterpret_cast<int2*>(ws + at.plan);
+    p.slots = reinterpret_cast<int32_t*>(ws + at.slots);
+    p.parts = reinterpret_cast<float*>(ws + at.parts);
+    p.share = at.share;
     p.words = words_of(num_queries);
-    place_order(p, static_cast<char*>(workspace) + 2 * row_bytes +
-                       up((size_t)batch * num_kv_heads * p.nb * p.words * sizeof(uint32_t)));
+    place_order(p, ws + at.order);
     p.out = static_cast<bf16_t*>(grad_q);
     p.dk = static_cast<bf16_t*>(grad_k);
     p.dv = static_cast<bf16_t*>(grad_v);
@@ -1273,9 +1413,11 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     void* margs[] = {&p, &groups};
     if (launch((const void*)&query_marks_kernel, dim3(groups * num_kv_heads * batch, (unsigned)chunks), margs, s) != hipSuccess)
         return MOSAIC_ERR_LAUNCH;
-    int tiles = (num_keys + 63) / 64, dkv_total = tiles * num_kv_heads * batch;
-    void* kargs[] = {&p, &tiles, &dkv_total};
-    return launch((const void*)&query_attn_dkv_kernel, dim3(dkv_total), kargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+    int tiles = (num_keys + 63) / 64, key_tiles = tiles * num_kv_heads * batch;
+    void* kargs[] = {&p, &tiles, &key_tiles};
+    if (launch((const void*)&query_plan_kernel, dim3(1), kargs, s, 1024) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    if (launch((const void*)&query_attn_dkv_kernel, dim3((unsigned)at.items), kargs, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    return launch((const void*)&query_sum_kernel, dim3(key_tiles), kargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
 
 }  // extern "C"

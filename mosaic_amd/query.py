@@ -135,7 +135,7 @@ class _QueryAttn(torch.autograd.Function):
         gq = torch.empty((B, Nq, Hq, d), dtype=torch.bfloat16, device=device)
         gk, gv = (torch.empty((B, Nk, Hk, d), dtype=torch.bfloat16, device=device) for _ in range(2))
         L = _lib.lib()
-        nbytes = L.mosaic_query_attn_bwd_workspace_size(B, Nq, Nk, Hq, Hk, block_size)
+        nbytes = L.mosaic_query_attn_bwd_workspace_size(B, Nq, Nk, Hq, Hk, block_size, idx.shape[-1])
         ws = _scratch(nbytes, device)
         with _on(device):
             st = L.mosaic_query_attn_bwd(qb, kb, vb, out.data_ptr(), lse.data_ptr(), gb, idx.data_ptr(), _ptr(lens), B, Nq, Nk,

@@ -94,7 +94,7 @@ def test_workspace_sizes():
     one = L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 3, 16)
     assert one >= 16 * 12 * (64 * 4 + 8) and one % 256 == 0
     assert L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 5, 16) == 0       # refused shapes
-    assert L.mosaic_query_attn_bwd_workspace_size(1, 100, 1000, 12, 3, 64) >= 2 * 4 * 1200 + 3 * 16 * 16 * 4
+    assert L.mosaic_query_attn_bwd_workspace_size(1, 100, 1000, 12, 3, 64, 5) >= 2 * 4 * 1200 + 3 * 16 * 16 * 4
 
 
 # ------------------------------------------------------------------------------- GPU
