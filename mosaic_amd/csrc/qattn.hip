@@ -70,7 +70,9 @@ struct QueryAttnParams {
     float* nlse;               // backward: -lse / c and -sum(o do) of each row
     float* ndelta;
     uint32_t* marks;           // backward: [B, Hk, nb, words] bit n: token n has the block
-    int32_t* counts;           // backward: [B, Hk, nb] tokens of each block
+    int32_t* counts;           // backward: [B, Hk, nb] number of tokens of each block
+    int32_t* starts;           // backward: [B, Hk, nb] where they begin in
+    int32_t* takers;           // the tokens of each block, ascending
     int2* items;               // backward: (key tile, share | shares << 16) of each workgroup of grad k / v
     int32_t* slots;            // backward: [key tiles] first partial of a tile in several shares, else -1;
                                // then the number of items
@@ -84,7 +86,8 @@ struct QueryAttnParams {
     int B, Nq, Nk, Hq, Hk, G, QW, bs, K, nb, words;
     int qtiles, splits;
     int qw_inverse;            // t / QW = t qw_inverse >> 16 for t < 256
-    int short_rows;            // 64 rows of k and of v span less than 2^31 bytes
+    int short_rows;            // 64 rows of k and of v span less than 2^31 bytes (backward: and a sequence of q
+                               // and of the output's gradient less than 2^32)
     float scale, c;
 };
 
@@ -886,13 +889,44 @@ __global__ __launch_bounds__(kThreads) void query_marks_kernel(QueryAttnParams p
     }
 }
 
-// The workgroups of grad k / v: a tile of 64 keys whose block has more than p.share tokens is split
-// into equal shares of them (blocks differ in popularity by factors: the most wanted one would run
-// long after the others are done).  One workgroup; items are in the order of the tiles.
+// Exclusive prefix sums over 1024 threads of a pair of counts, on top of `base`, which becomes the
+// whole's.
+__device__ __forceinline__ int2 prefix_1024(int2 x, int2& base, int2 (&sums)[16]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int2 y = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(y.x, d), v = __shfl_up(y.y, d);
+        y.x += lane >= d ? u : 0;
+        y.y += lane >= d ? v : 0;
+    }
+    if (lane == 63) sums[wave] = y;
+    __syncthreads();
+    int2 at = make_int2(base.x + y.x - x.x, base.y + y.y - x.y);
+    for (int w = 0; w < 16; ++w) {
+        at.x += w < wave ? sums[w].x : 0;
+        at.y += w < wave ? sums[w].y : 0;
+        base.x += sums[w].x;
+        base.y += sums[w].y;
+    }
+    __syncthreads();
+    return at;
+}
+
+// Where each block's tokens begin, and the workgroups of grad k / v: a tile of 64 keys whose block has
+// more than p.share tokens is split into equal shares of them (blocks differ in popularity by
+// factors: the most wanted one would run long after the others are done).  One workgroup; items are
+// in the order of the tiles.
 __global__ __launch_bounds__(1024) void query_plan_kernel(QueryAttnParams p, int tiles, int total) {
-    __shared__ int sums[16][2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int items = 0, slots = 0;
+    __shared__ int2 sums[16];
+    const int tid = threadIdx.x, blocks = p.B * p.Hk * p.nb;
+    int2 base = make_int2(0, 0);
+    for (int i0 = 0; i0 < blocks; i0 += 1024) {
+        const int n = i0 + tid < blocks ? p.counts[i0 + tid] : 0;
+        const int2 at = prefix_1024(make_int2(n, 0), base, sums);
+        if (i0 + tid < blocks) p.starts[i0 + tid] = at.x;
+    }
+    base = make_int2(0, 0);
     for (int i0 = 0; i0 < total; i0 += 1024) {
         const int i = i0 + tid;
         int shares = 0;
@@ -901,31 +935,41 @@ __global__ __launch_bounds__(1024) void query_plan_kernel(QueryAttnParams p, int
             const int count = p.counts[(int64_t)bh * p.nb + (int64_t)kt * 64 / p.bs];
             shares = max(1, (count + p.share - 1) / p.share);
         }
-        const int held = shares > 1 ? shares : 0;
-        int a = shares, c = held;   // prefix sums over the wave, then over the waves
+        const int2 at = prefix_1024(make_int2(shares, shares > 1 ? shares : 0), base, sums);   // items, partials
+        for (int j = 0; j < shares; ++j) p.items[at.x + j] = make_int2(i, j | shares << 16);
+        if (i < total) p.slots[i] = shares > 1 ? at.y : -1;
+    }
+    if (tid == 0) p.slots[total] = base.x;
+}
+
+// The tokens of each block, ascending, from its marks: one workgroup a block.
+__global__ __launch_bounds__(kThreads) void query_takers_kernel(QueryAttnParams p) {
+    __shared__ int sums[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int left = p.counts[blockIdx.x];
+    if (left == 0) return;
+    const uint32_t* marks = p.marks + (int64_t)blockIdx.x * p.words;
+    int32_t* out = p.takers + p.starts[blockIdx.x];
+    int seen = 0;
+    for (int w0 = 0; w0 < p.words && seen < left; w0 += kThreads) {
+        const uint32_t word = w0 + tid < p.words ? marks[w0 + tid] : 0;
+        int upto = __builtin_popcount(word);
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(a, d), y = __shfl_up(c, d);
-            a += lane >= d ? x : 0;
-            c += lane >= d ? y : 0;
+            const int x = __shfl_up(upto, d);
+            upto += lane >= d ? x : 0;
         }
-        if (lane == 63) {
-            sums[wave][0] = a;
-            sums[wave][1] = c;
-        }
+        if (lane == 63) sums[wave] = upto;
         __syncthreads();
-        int at = items + a - shares, slot = slots + c - held;
-        for (int w = 0; w < 16; ++w) {
-            at += w < wave ? sums[w][0] : 0;
-            slot += w < wave ? sums[w][1] : 0;
-            items += sums[w][0];
-            slots += sums[w][1];
+        int at = seen + upto - __builtin_popcount(word);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            at += w < wave ? sums[w] : 0;
+            seen += sums[w];
         }
-        for (int j = 0; j < shares; ++j) p.items[at + j] = make_int2(i, j | shares << 16);
-        if (i < total) p.slots[i] = shares > 1 ? slot : -1;
+        for (uint32_t m = word; m != 0; m &= m - 1) out[at++] = 32 * (w0 + tid) + __builtin_ctz(m);
         __syncthreads();
     }
-    if (tid == 0) p.slots[total] = items;
 }
 
 // Sums of a split tile's partials, in the order of the shares.
@@ -956,15 +1000,13 @@ __global__ __launch_bounds__(kThreads) void query_sum_kernel(QueryAttnParams p, 
 // row half w % 2) forms S = q k^T and dP = do v^T of its 32 rows x 32 keys
 // (v_mfma_f32_32x32x16_bf16); P and dS stay in registers as the B operands of dV^T += do^T P and
 // dK^T += q^T dS, whose A operands are transposing LDS reads.  The row halves are added at the end.
-constexpr int kSegWords = 128;                 // words of marks listed at a time: 4096 tokens
-constexpr int kListed = 32 * kSegWords + 64;   // and what was left of the last ones
+constexpr int kListed = 2048;   // tokens listed at a time
 
 struct KeysLds {
     __attribute__((aligned(1024))) bf16_t q[3][kTileElems];
     __attribute__((aligned(1024))) bf16_t g[3][kTileElems];
     float nlse[3][64], ndelta[3][64];
     int list[kListed];
-    int sums[2];
 };
 
 __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnParams p, int tiles, int total) {
@@ -979,7 +1021,7 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
     const int key0 = kt * 64, end = seq_keys(p, b);
     const int64_t all = p.counts[((int64_t)b * p.Hk + h) * p.nb + key0 / p.bs];
     const int from = (int)(all * share / shares), past = (int)(all * (share + 1) / shares);   // this share's tokens, by rank
-    const uint32_t* marks = p.marks + (((int64_t)b * p.Hk + h) * p.nb + key0 / p.bs) * p.words;
+    const int64_t block = ((int64_t)b * p.Hk + h) * p.nb + key0 / p.bs;
     const int QS = 64 / p.G;
 
     f32x16 dkT[2], dvT[2];
@@ -1022,6 +1064,8 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
         }
         const bf16_t* qb = p.q + b * p.q_sb;
         const bf16_t* gb = p.go + b * p.go_sb;
+        const float* nlse = p.nlse + (int64_t)b * p.Nq * p.Hq;
+        const float* ndelta = p.ndelta + (int64_t)b * p.Nq * p.Hq;
         int64_t qoff[2], goff[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -1030,26 +1074,54 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
             goff[i] = lhead[i] * p.go_sh + chunk;
         }
         // Step s's rows into slot `buf`; entries past the list repeat its last one.  Six loads a wave,
-        // whatever the step, so that waiting for all but the newest request is one count.
-        auto request = [&](int s, int buf, int count) {
+        // whatever the step, so that waiting for all but the newest request is one count.  The tokens
+        // of the step after it are read from the list meanwhile.
+        int tok[3];
+        auto look = [&](int s, int count) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t n = L.list[min(s * QS + ltok[i], count - 1)];
-                const int row0 = 16 * w + 8 * i;
-                dma16_at(qb + n * p.q_sn + qoff[i], lds_addr(L.q[buf] + row0 * 64));
-                dma16_at(gb + n * p.go_sn + goff[i], lds_addr(L.g[buf] + row0 * 64));
+            for (int i = 0; i < 3; ++i) tok[i] = L.list[min(s * QS + ltok[i], count - 1)];
+        };
+        auto request = [&](int s, int buf, int count) {
+            if (p.short_rows) {   // offsets from the tensors' starts fit 32 bits
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int row0 = 16 * w + 8 * i;
+                    dma16(qb, 2u * ((uint32_t)tok[i] * (uint32_t)p.q_sn + (uint32_t)qoff[i]), lds_addr(L.q[buf] + row0 * 64));
+                    dma16(gb, 2u * ((uint32_t)tok[i] * (uint32_t)p.go_sn + (uint32_t)goff[i]), lds_addr(L.g[buf] + row0 * 64));
+                }
+                const uint32_t at = 4u * ((uint32_t)tok[2] * (uint32_t)p.Hq + (uint32_t)lhead[2]);
+                if (lane < 16) {
+                    dma4(nlse, at, lds_addr(L.nlse[buf] + 16 * w));
+                    dma4(ndelta, at, lds_addr(L.ndelta[buf] + 16 * w));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int row0 = 16 * w + 8 * i;
+                    dma16_at(qb + (int64_t)tok[i] * p.q_sn + qoff[i], lds_addr(L.q[buf] + row0 * 64));
+                    dma16_at(gb + (int64_t)tok[i] * p.go_sn + goff[i], lds_addr(L.g[buf] + row0 * 64));
+                }
+                const int64_t at = (int64_t)tok[2] * p.Hq + lhead[2];
+                if (lane < 16) {
+                    dma4_at(nlse + at, lds_addr(L.nlse[buf] + 16 * w));
+                    dma4_at(ndelta + at, lds_addr(L.ndelta[buf] + 16 * w));
+                }
             }
-            const int64_t at = ((int64_t)b * p.Nq + L.list[min(s * QS + ltok[2], count - 1)]) * p.Hq + lhead[2];
-            if (lane < 16) {
-                dma4_at(p.nlse + at, lds_addr(L.nlse[buf] + 16 * w));
-                dma4_at(p.ndelta + at, lds_addr(L.ndelta[buf] + 16 * w));
-            }
+            look(s + 1, count);
         };
         auto tr_read = [&](const bf16_t* T, int q0, int dt) { return tr_pair(T + q0 * 64 + tr[dt][0], T + q0 * 64 + tr[dt][1]); };
         auto step = [&](int buf, int rows) {
             const bf16_t* Qc = L.q[buf];
             const bf16_t* Gc = L.g[buf];
+            // reads are ahead of their products and exponentials throughout (the compiler left to itself
+            // waits for each)
             f32x16 s, dp;
+            bf16x8 qa[4], ga[4];
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                qa[kk] = as_bf16x8(*reinterpret_cast<const uint4*>(Qc + 32 * qh * 64 + rd[kk]));
+                ga[kk] = as_bf16x8(*reinterpret_cast<const uint4*>(Gc + 32 * qh * 64 + rd[kk]));
+            }
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
                 const float4 l4 = *reinterpret_cast<const float4*>(L.nlse[buf] + 32 * qh + 8 * g4 + 4 * hh);
@@ -1057,12 +1129,17 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
                 s[4 * g4] = l4.x; s[4 * g4 + 1] = l4.y; s[4 * g4 + 2] = l4.z; s[4 * g4 + 3] = l4.w;
                 dp[4 * g4] = d4.x; dp[4 * g4 + 1] = d4.y; dp[4 * g4 + 2] = d4.z; dp[4 * g4 + 3] = d4.w;
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
-                s = mfma32(as_bf16x8(*reinterpret_cast<const uint4*>(Qc + 32 * qh * 64 + rd[kk])), kf[kk], s);
-                dp = mfma32(as_bf16x8(*reinterpret_cast<const uint4*>(Gc + 32 * qh * 64 + rd[kk])), vf[kk], dp);
+                s = mfma32(qa[kk], kf[kk], s);
+                dp = mfma32(ga[kk], vf[kk], dp);
+                if (kk < 2) {
+                    qa[kk + 2] = as_bf16x8(*reinterpret_cast<const uint4*>(Qc + 32 * qh * 64 + rd[kk + 2]));
+                    ga[kk + 2] = as_bf16x8(*reinterpret_cast<const uint4*>(Gc + 32 * qh * 64 + rd[kk + 2]));
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            bf16x8 pb[2], db[2];
             if (rows < 64) {   // rows past the list, or past QS G: P = 0 and dS = 0
                 seldom();
 #pragma unroll
@@ -1072,6 +1149,13 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
                     dp[e] = on ? dp[e] : 0.f;
                 }
             }
+            bf16x8 gT[2][2], qT[2][2];   // [dim tile][16 rows]
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+                for (int ch = 0; ch < 2; ++ch) gT[dt][ch] = tr_read(Gc, 32 * qh + 16 * ch, dt);
+            __builtin_amdgcn_sched_barrier(0);
+            bf16x8 pb[2], db[2];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float pr = __builtin_amdgcn_exp2f(s[e] * p.c), ds = pr * dp[e];
@@ -1081,39 +1165,26 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
 #pragma unroll
             for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-                for (int ch = 0; ch < 2; ++ch) {
-                    dvT[dt] = mfma32(tr_read(Gc, 32 * qh + 16 * ch, dt), pb[ch], dvT[dt]);
-                    dkT[dt] = mfma32(tr_read(Qc, 32 * qh + 16 * ch, dt), db[ch], dkT[dt]);
-                }
-        };
-        int count = 0, seen = 0;   // tokens listed, and passed in the marks
-        for (int w0 = 0; w0 < p.words && seen < past; w0 += kSegWords) {
-            // list this share's tokens of words w0 .. behind the ones left over: waves 0 and 1, a word per lane
-            const uint32_t word = w < 2 && w0 + tid < p.words ? marks[w0 + tid] : 0;
-            int before = __builtin_popcount(word);
+                for (int ch = 0; ch < 2; ++ch) qT[dt][ch] = tr_read(Qc, 32 * qh + 16 * ch, dt);
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int x = __shfl_up(before, d);
-                before += lane >= d ? x : 0;
-            }
-            if (w < 2 && lane == 63) L.sums[w] = before;
+            for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt) dvT[dt] = mfma32(gT[dt][ch], pb[ch], dvT[dt]);
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt) dkT[dt] = mfma32(qT[dt][ch], db[ch], dkT[dt]);
+        };
+        const int32_t* takers = p.takers + p.starts[block];
+        const int run = kListed / QS * QS;   // tokens listed at a time
+        for (int c0 = from; c0 < past; c0 += run) {
+            const int count = min(run, past - c0), steps = (count + QS - 1) / QS;
+            for (int i = tid; i < count; i += kThreads) L.list[i] = takers[c0 + i];
             __syncthreads();
-            const int first = max(from, seen);
-            if (w < 2) {
-                int rank = seen + before - __builtin_popcount(word) + (w == 1 ? L.sums[0] : 0);
-                for (uint32_t m = word; m != 0; m &= m - 1, ++rank)
-                    if (rank >= first && rank < past) L.list[count + rank - first] = 32 * (w0 + tid) + __builtin_ctz(m);
-            }
-            seen += L.sums[0] + L.sums[1];
-            count += max(0, min(seen, past) - first);
-            __syncthreads();
-            const bool last = w0 + kSegWords >= p.words || seen >= past;
-            const int steps = last ? (count + QS - 1) / QS : count / QS;
             // a ring of three slots: a step's rows are requested two steps before it
-            if (steps > 0) {
-                request(0, 0, count);
-                request(1, 1, count);
-            }
+            look(0, count);
+            request(0, 0, count);
+            request(1, 1, count);
             for (int s = 0, buf = 0; s < steps; ++s) {
                 asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
                 lds_barrier();
@@ -1122,15 +1193,8 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
                 buf = buf == 2 ? 0 : buf + 1;
             }
             wait_vmem();
-            // the tokens left over go to the list's front
-            const int rest_n = count - steps * QS;
-            int keep = 0;
-            if (tid < rest_n) keep = L.list[steps * QS + tid];
             __syncthreads();
-            if (tid < rest_n) L.list[tid] = keep;
-            count = rest_n > 0 ? rest_n : 0;
         }
-        __syncthreads();
         // the row halves' sums: qh = 1 parks its accumulators in the buffers
         float* red = reinterpret_cast<float*>((kh == 0 ? L.q[0] : L.g[0]) + hh * kTileElems) + r;
         if (qh == 1) {
@@ -1272,8 +1336,9 @@ hipError_t launch(const void* fn, dim3 grid, void** args, hipStream_t s, int thr
 // Workspace of the backward, and the tokens of one share of a key tile: half as many again as a block
 // has on average, fewer where the tiles alone do not fill the chip twice.
 struct BwdLayout {
-    size_t nlse, ndelta, marks, counts, plan, slots, parts, order, bytes;
+    size_t nlse, ndelta, marks, counts, starts, takers, plan, slots, parts, order, bytes;
     int64_t items;   // workgroups of grad k / v at most
+    int64_t pairs;   // (token, block) pairs at most
     int share;
 };
 BwdLayout bwd_layout(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, int32_t bs, int32_t K) {
@@ -1288,12 +1353,15 @@ BwdLayout bwd_layout(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t 
     a.share = (int)(share < 0x7fffffff ? share : 0x7fffffff);
     // a tile with c tokens has at most 1 + c / share shares, of one with several there are 2 c / share at most
     a.items = tiles + pairs / a.share;
+    a.pairs = chosen * hk * batch;
     const int64_t slots = 2 * (pairs / a.share) + 2;
     const size_t rows = up((size_t)batch * nq * hq * sizeof(float));
     a.ndelta = a.nlse + rows;
     a.marks = a.ndelta + rows;
     a.counts = a.marks + up((size_t)batch * hk * nb * words_of(nq) * sizeof(uint32_t));
-    a.plan = a.counts + up((size_t)batch * hk * nb * sizeof(int32_t));
+    a.starts = a.counts + up((size_t)batch * hk * nb * sizeof(int32_t));
+    a.takers = a.starts + up((size_t)batch * hk * nb * sizeof(int32_t));
+    a.plan = a.takers + up((size_t)batch * hk * chosen * sizeof(int32_t));
     a.slots = a.plan + up((size_t)a.items * sizeof(int2));
     a.parts = a.slots + up((size_t)(tiles + 1) * sizeof(int32_t));
     a.order = a.parts + up((size_t)slots * 128 * kHeadDim * sizeof(float));
@@ -1381,11 +1449,17 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     if (!aligned(block_indices, 8) || !aligned(lse, 4) || !aligned(kv_lens, 4)) return MOSAIC_ERR_ALIGNMENT;
     const BwdLayout at = bwd_layout(batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count);
     if (workspace == nullptr || workspace_bytes < at.bytes || !aligned(workspace, 256)) return MOSAIC_ERR_WORKSPACE;
-    if (at.items > 0x7fffffff) return MOSAIC_ERR_SHAPE;
+    // token lists are indexed in 31 bits
+    if (at.items > 0x7fffffff || at.pairs > 0x7fffffff) return MOSAIC_ERR_SHAPE;
     QueryAttnParams p{};
     fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kDqRows);
     p.go = static_cast<const bf16_t*>(grad_out.ptr);
     p.go_sb = grad_out.stride_b; p.go_sn = grad_out.stride_n; p.go_sh = grad_out.stride_h;
+    auto spans = [&](const mosaic_bnhd& t) {   // a sequence's rows lie within 2^32 bytes of its first
+        return t.stride_n >= 0 && t.stride_h >= 0 &&
+               (double)(num_queries - 1) * t.stride_n + (double)(num_q_heads - 1) * t.stride_h + 64 < 2147483648.0;
+    };
+    p.short_rows = p.short_rows && spans(q) && spans(grad_out) && (double)num_queries * num_q_heads < 1073741824.0;
     p.o = static_cast<const bf16_t*>(out);
     p.lse = const_cast<float*>(lse);
     char* ws = static_cast<char*>(workspace);
@@ -1393,6 +1467,8 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     p.ndelta = reinterpret_cast<float*>(ws + at.ndelta);
     p.marks = reinterpret_cast<uint32_t*>(ws + at.marks);
     p.counts = reinterpret_cast<int32_t*>(ws + at.counts);
+    p.starts = reinterpret_cast<int32_t*>(ws + at.starts);
+    p.takers = reinterpret_cast<int32_t*>(ws + at.takers);
     p.items = reinterpret_cast<int2*>(ws + at.plan);
     p.slots = reinterpret_cast<int32_t*>(ws + at.slots);
     p.parts = reinterpret_cast<float*>(ws + at.parts);
@@ -1416,6 +1492,9 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     int tiles = (num_keys + 63) / 64, key_tiles = tiles * num_kv_heads * batch;
     void* kargs[] = {&p, &tiles, &key_tiles};
     if (launch((const void*)&query_plan_kernel, dim3(1), kargs, s, 1024) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    void* targs[] = {&p};
+    if (launch((const void*)&query_takers_kernel, dim3((unsigned)(p.nb * num_kv_heads * batch)), targs, s) != hipSuccess)
+        return MOSAIC_ERR_LAUNCH;
     if (launch((const void*)&query_attn_dkv_kernel, dim3((unsigned)at.items), kargs, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     return launch((const void*)&query_sum_kernel, dim3(key_tiles), kargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
