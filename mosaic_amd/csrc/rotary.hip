@@ -34,7 +34,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kHeadRun = 4;        // heads whose loads are in flight together
 constexpr int kMaxPairs = 64;      // D <= 128
-constexpr int kMaxBwdGroups = 1024;  // workgroups (rows of weight-gradient partials) of the norm's backward
+constexpr int kMaxBwdGroups = 2048;  // workgroups (rows of weight-gradient partials) of the norm's backward
 
 struct RotTensor {
     const void* x; int64_t sb, sn, sh;   // forward input (the norm's backward: x)
@@ -293,9 +293,15 @@ __global__ __launch_bounds__(kThreads) void wgrad_kernel(const float* partial, i
     __shared__ float part[32][9];
     const int c = threadIdx.x & 7, r0 = threadIdx.x >> 3;
     const int col = 8 * blockIdx.x + c;
-    float s = 0.f;
-    for (int r = r0; r < rows; r += 32) s += partial[(int64_t)r * 2 * D + col];
-    part[r0][c] = s;
+    float s[8] = {};   // eight loads in flight
+    for (int r = r0; r < rows; r += 256)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = r + 32 * i;
+            const float x = partial[(int64_t)min(at, rows - 1) * 2 * D + col];
+            s[i] += at < rows ? x : 0.f;
+        }
+    part[r0][c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (r0 == 0) {
         float sum = 0.f;
