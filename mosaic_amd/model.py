@@ -89,6 +89,7 @@ class ModelConfig:
     ortho_init: bool = False
     rmsnorm_elementwise_affine: bool = True
     no_compression: bool = False
+    head_norm: bool = False     # RMS norm of every query and key head (``qk_norm``, the reference's flag, is read by nothing)
 
 
 @dataclass
@@ -106,6 +107,7 @@ class _MergedStageConfig:
     mlp_ratio: float
     noise_dim: int
     rmsnorm_elementwise_affine: bool
+    head_norm: bool = False
 
 
 def _merge_configs(config: ModelConfig, stage_cfg) -> _MergedStageConfig:
@@ -114,7 +116,7 @@ def _merge_configs(config: ModelConfig, stage_cfg) -> _MergedStageConfig:
         sparse_block_size=stage_cfg.sparse_block_size, sparse_block_count=stage_cfg.sparse_block_count,
         gqa_ratio=stage_cfg.gqa_ratio, qkv_compress_ratio=config.qkv_compress_ratio, rope=config.rope,
         rope_theta=config.rope_theta, mlp_ratio=stage_cfg.mlp_ratio, noise_dim=config.noise_dim,
-        rmsnorm_elementwise_affine=config.rmsnorm_elementwise_affine)
+        rmsnorm_elementwise_affine=config.rmsnorm_elementwise_affine, head_norm=config.head_norm)
 
 
 def era5_config(num_variables: int = 82, num_static: int = 3) -> ModelConfig:

@@ -24,6 +24,7 @@ import torch.nn as nn
 from . import _lib, fused
 from .healpix import rope_tables
 from .ops import _as_bf16_bnhd, _check_gqa, bnhd, forward_only, mosaic_sparse_attn, stream_of
+from .rotary import qk_norm_rope
 
 __all__ = [
     "block_attention", "dense_attention", "pool_mean", "attn_topk", "mosaic_attn_func",
@@ -400,6 +401,11 @@ class MosaicAttention(nn.Module):
 
     ``config`` needs: block_attn_size, sparse_block_size, sparse_block_count, num_heads,
     gqa_ratio, dim, qkv_compress_ratio, rope, rope_theta.  x is sequence-first [S, B, dim].
+
+    ``config.head_norm`` (absent: False, the reference's module) adds an RMS norm of every query
+    and key head before their rotation, ``q_norm`` and ``k_norm``, each with one weight of head_dim
+    where ``rmsnorm_elementwise_affine`` (absent: True): logits stay bounded by the weights however
+    the projections grow.  Norm and rotation are then one pass over q and k (``qk_norm_rope``).
     """
 
     def __init__(self, config, block_attn_only: bool, no_compression: bool = False):
@@ -419,6 +425,11 @@ class MosaicAttention(nn.Module):
         self.to_o = nn.Linear(q_heads * head_dim, config.dim, bias=False)
         self.q_rope = RoPE(head_dim, config.rope_theta) if config.rope else None
         self.k_rope = RoPE(head_dim, config.rope_theta) if config.rope else None
+        self.head_norm = bool(getattr(config, "head_norm", False))
+        if self.head_norm:
+            affine = getattr(config, "rmsnorm_elementwise_affine", True)
+            self.q_norm = fused.RMSNorm(head_dim, elementwise_affine=affine)
+            self.k_norm = fused.RMSNorm(head_dim, elementwise_affine=affine)
         self.to_strategy_combine_mlp = None if block_attn_only else nn.Linear(config.dim, 3 * q_heads, bias=False)
         # a list to append each call's selected block indices to (int64 [B, N/bs, Hk, K], None
         # without selection), or None; tests use it to evaluate a checker on the same selection
@@ -498,7 +509,7 @@ class MosaicAttention(nn.Module):
     def _fused_input_side(self, x):
         """Whether mosaic_attn_proj can run this call: bf16 arithmetic (bf16 autocast, or bf16
         input and weights), q and k rotated by equal tables (or no RoPE), and its shape limits."""
-        if not self.fused_input_side:
+        if not self.fused_input_side or self.head_norm:
             return False
         if x.device.type != "cuda" or x.dim() != 3 or self.to_q.out_features != 64 * self.q_heads:
             return False
@@ -510,6 +521,19 @@ class MosaicAttention(nn.Module):
         if not self.block_attn_only and (self.sparse_block_size not in (64, 128) or 3 * self.q_heads > 64):
             return False
         return self.q_rope is None or self._shared_rope_tables()
+
+    def _norm_and_rotate(self, q, k):
+        """q and k normalised per head and rotated: one pass over both, or one over each where the
+        two RoPE modules hold different tables."""
+        norms = dict(eps=self.q_norm.eps)
+        if self.q_rope is None:
+            return qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, **norms)
+        if self._shared_rope_tables():
+            return qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, **norms,
+                                cos=self.q_rope.cos_freqs, sin=self.q_rope.sin_freqs)
+        q, _ = qk_norm_rope(q, None, self.q_norm.weight, **norms, cos=self.q_rope.cos_freqs, sin=self.q_rope.sin_freqs)
+        k, _ = qk_norm_rope(k, None, self.k_norm.weight, **norms, cos=self.k_rope.cos_freqs, sin=self.k_rope.sin_freqs)
+        return q, k
 
     def forward(self, x):
         S_, B_ = x.shape[:2]
@@ -546,7 +570,11 @@ class MosaicAttention(nn.Module):
         o = torch.empty(S_, B_, self.q_heads * q.shape[-1], dtype=torch.bfloat16, device=x.device)
         o_view = o.view(S_, B_, self.q_heads, -1).transpose(0, 1)
         record = self.record_block_indices is not None
-        if self.q_rope is not None and self._shared_rope_tables():
+        if self.head_norm:
+            q, k = self._norm_and_rotate(q, k)
+            res = mosaic_attn_func(q=q, k=k, v=v, weight_ba_cmp_slc=w, **args, out=o_view,
+                                   return_block_indices=record)
+        elif self.q_rope is not None and self._shared_rope_tables():
             # the rotation runs inside the op's pooling pass (one read of q and k)
             res = mosaic_attn_func_rope(q, k, v, w, self.q_rope.cos_freqs, self.q_rope.sin_freqs, **args,
                                         out=o_view, return_block_indices=record)
