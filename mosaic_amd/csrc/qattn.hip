@@ -7,13 +7,13 @@
 // key is zeros (lse -inf).  fp32 scores, maxima, sums and accumulators; P is rounded to bf16 for
 // the PV product (an error of half a step of bf16 per term, as the output's own rounding).
 //
-// A workgroup takes 4 waves x QW = 64 / G tokens of one kv head, a wave the 64 rows (token, head) of
-// its tokens (grad q: 32).  The tokens' sets are united in LDS (a token mask per wave and block), and
-// the union's blocks are staged once, 64 keys at a time, for all four waves; a wave skips the blocks
-// none of its tokens has.  Neighbouring tokens of a mesh mostly choose the same blocks, so the union
-// is little longer than one set (18 blocks for 64 tokens with 16 each on nside 64's field).  Tokens in
-// no such order are taken in the order of a block of theirs (query_order_kernel): 10007 scattered
-// points then unite 24 blocks instead of 460.
+// A workgroup takes 4 waves x QW = 32 / G tokens of one kv head, a wave the 32 rows (token, head) of
+// its tokens.  The tokens' sets are united in LDS (a token mask per wave and block), and the union's
+// blocks are staged once, 64 keys at a time, for all four waves; a wave skips the blocks none of its
+// tokens has.  Neighbouring tokens of a mesh mostly choose the same blocks, so the union is little
+// longer than one set (17.4 blocks for 32 tokens with 16 each on nside 64's field).  Tokens in no such
+// order are taken in the order of a block of theirs (query_order_kernel): 10007 scattered points then
+// unite 22 blocks instead of 313.
 //
 // Per tile of 64 keys, transposed so that a lane's scores are those of two rows
 // (v_mfma_f32_32x32x16_bf16, a row in lanes r and r + 32):
@@ -27,14 +27,18 @@
 // workgroup ends with a value that is not finite it runs again, each product's accumulators restored
 // for the rows that are no members, and what a row did not choose does not reach it then either.
 //
-// 64 rows a wave rather than 32 (two waves a SIMD instead of three) halve LDS reads and barriers per
-// score and give a wave four independent chains of products: XXX us instead of 260 for the tokens
-// of nside 64; 16 rows (v_mfma_f32_16x16x32_bf16): 345.
+// Bound by the vector ALU's exponentials and packing beside the products, at three waves a SIMD: 231 us
+// for 49152 tokens of 16 blocks of 64 keys in one kv head of four query heads (nside 64), 206 Gflop and
+// 51 MB at least; two passes of 2 x 64 x 64 flops a score make that 0.89 Pflop/s.  Each further block
+// costs 11.4 us, and 57 us are spent before the first.  64 rows a wave (two waves a SIMD, half the LDS
+// reads a score) measured 253 us there, 262 instead of 205 for two members' 10007 stations and 11.6
+// instead of 9.4 for one token; 16 rows (v_mfma_f32_16x16x32_bf16) 345.
 //
 // Few queries: the union is split over workgroups and the partial (m, l, O) joined by a second
 // kernel.
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -46,7 +50,7 @@ namespace mosaic {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kFwdRows = 32, kDqRows = 32;   // rows (token, head) of a wave
+constexpr int kRows = 32;          // rows (token, head) of a wave
 constexpr int kTileElems = 64 * 64;
 constexpr int kUnion = 1024;       // blocks whose members are marked at a time
 constexpr int kMaxSplit = 32;
@@ -215,21 +219,18 @@ __global__ __launch_bounds__(kOrderThreads) void query_order_kernel(QueryAttnPar
 
 // ------------------------------------------------------------------ tiles of a union
 
-// LDS of the forward (64 rows a wave) and grad-q (32) kernels
-template <int ROWS>
+// LDS of the forward and grad-q kernels
 struct RowsLds {
-    static constexpr int kWords = ROWS / 32;   // of a wave's token mask: bit t, its token t has the block
     __attribute__((aligned(1024))) bf16_t K[2][kTileElems];
     __attribute__((aligned(1024))) bf16_t V[2][kTileElems];
-    __attribute__((aligned(16))) uint32_t members[kUnion][kWaves * kWords];
+    __attribute__((aligned(16))) uint32_t members[kUnion][kWaves];   // bit t: token t of the wave has the block
     uint16_t list[kUnion];
-    int tokens[kWaves * ROWS];
+    int tokens[kWaves * kRows];
     int found[kWaves];
 };
 
 // The workgroup's tokens (positions n0 .. of the order) into LDS; ends with a barrier.
-template <int ROWS>
-__device__ __forceinline__ void load_tokens(const QueryAttnParams& p, RowsLds<ROWS>& L, int b, int h, int n0) {
+__device__ __forceinline__ void load_tokens(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0) {
     const int64_t bh = (int64_t)b * p.Hk + h;
     const bool ordered = p.keys != nullptr && p.ordered[bh] != 0;
     for (int i = threadIdx.x; i < kWaves * p.QW; i += kThreads) {
@@ -242,38 +243,30 @@ __device__ __forceinline__ void load_tokens(const QueryAttnParams& p, RowsLds<RO
 // Marks the members of blocks [c0, c0 + nc) among the workgroup's tokens and lists the blocks that
 // have any, ascending; returns their number.  of_split < splits leaves other splits' blocks out
 // (blocks u with u % splits == of_split remain).  Ends with a barrier.
-template <int ROWS>
-__device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds<ROWS>& L, int b, int h, int n0, int end, int c0, int nc,
+__device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int end, int c0, int nc,
                                      int of_split, int splits) {
-    constexpr int kWords = RowsLds<ROWS>::kWords;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < nc * kWords; i += kThreads) reinterpret_cast<uint4*>(L.members)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < nc; i += kThreads) reinterpret_cast<uint4*>(L.members)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     // eight lanes a token
     const int tokens = min(kWaves * p.QW, p.Nq - n0);
     for (int t = tid >> 3; t < tokens; t += kThreads / 8) {
         const int64_t* e = p.idx + (((int64_t)b * p.Nq + L.tokens[t]) * p.Hk + h) * p.K;
         const int w = (t * p.qw_inverse) >> 16, of_wave = t - w * p.QW;
-        const int word = w * kWords + (of_wave >> 5);
-        const uint32_t bit = 1u << (of_wave & 31);
+        const uint32_t bit = 1u << of_wave;
         for (int kk = tid & 7; kk < p.K; kk += 8) {
             const int64_t blk = e[kk] - c0;
             if (blk < 0 || blk >= nc) continue;
             const int u = c0 + (int)blk;
             if ((int64_t)u * p.bs < end && (splits == 1 || (uint32_t)u % (uint32_t)splits == (uint32_t)of_split))
-                atomicOr(&L.members[blk][word], bit);
+                atomicOr(&L.members[blk][w], bit);
         }
     }
     __syncthreads();
     auto any = [&](int i) {
         if (i >= nc) return false;
-        uint32_t m = 0;
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-            const uint4 x = *reinterpret_cast<const uint4*>(&L.members[i][4 * w]);
-            m |= x.x | x.y | x.z | x.w;
-        }
-        return m != 0;
+        const uint4 x = *reinterpret_cast<const uint4*>(L.members[i]);
+        return (x.x | x.y | x.z | x.w) != 0;
     };
     const int per = (nc + kThreads - 1) / kThreads * 64;   // blocks a wave lists
     int n = 0;
@@ -302,9 +295,8 @@ __device__ __forceinline__ int unite(const QueryAttnParams& p, RowsLds<ROWS>& L,
 // tile: from a uniform base with per-lane offsets that do not change (64 rows within 2^31 bytes), or
 // from 64-bit addresses, as the tile with the sequence's last key does, where the rows behind it
 // repeat it (V's are zeroed: what P = 0 multiplies there).
-template <int ROWS, typename Tile>
-__device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds<ROWS>& L, int b, int h, int n0, int split, int splits, Tile tile) {
-    constexpr int kWords = RowsLds<ROWS>::kWords;
+template <typename Tile>
+__device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int split, int splits, Tile tile) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int end = seq_keys(p, b), sub = p.bs / 64;
     const bf16_t* kb = p.k + b * p.k_sb + h * p.k_sh;
@@ -347,12 +339,11 @@ __device__ __forceinline__ void for_tiles(const QueryAttnParams& p, RowsLds<ROWS
             // up to 64 blocks of the list and this wave's members in registers: lane i holds block i
             const int count = min(64, past - e0);
             const int uv = L.list[e0 + min(lane, count - 1)];
-            const int m0 = (int)L.members[uv][wave * kWords], m1 = kWords > 1 ? (int)L.members[uv][wave * kWords + kWords - 1] : 0;
+            const int mv = (int)L.members[uv][wave];
             int key0 = (c0 + __builtin_amdgcn_readlane(uv, 0)) * p.bs, buf = 0;
             stage(key0, 0);
             for (int i = 0; i < count; ++i) {
-                uint64_t members = (uint32_t)__builtin_amdgcn_readlane(m0, i);
-                if (kWords > 1) members |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane(m1, i) << 32;
+                const uint32_t members = (uint32_t)__builtin_amdgcn_readlane(mv, i);
                 for (int st = 0; st < sub; ++st) {
                     const bool more = st + 1 < sub ? key0 + 64 < end : i + 1 < count;
                     const int next = st + 1 < sub ? key0 + 64 : (c0 + __builtin_amdgcn_readlane(uv, min(i + 1, 63))) * p.bs;
@@ -420,21 +411,20 @@ __device__ __forceinline__ float operand_sum(const bf16x8& x, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u.w), ones, acc, false);
 }
 
-// Row r of a wave (column r % 32 of its row tile r / 32): token (position in the wave), query head,
+// Row r of a wave: token (position in the wave), query head,
 // and its place in [B, Nq, Hq]
 struct Row {
     int token, head;
     bool live;
     int64_t n, at;
-    template <int ROWS>
-    __device__ __forceinline__ void init(const QueryAttnParams& p, const RowsLds<ROWS>& L, int b, int h, int n0, int wave, int r) {
+        __device__ __forceinline__ void init(const QueryAttnParams& p, const RowsLds& L, int b, int h, int n0, int wave, int r) {
         token = r / p.G;
         live = token < p.QW && n0 + wave * p.QW + token < p.Nq;
         head = h * p.G + (live ? r - token * p.G : 0);
         n = L.tokens[wave * p.QW + (live ? token : 0)];
         at = ((int64_t)b * p.Nq + n) * p.Hq + head;
     }
-    __device__ __forceinline__ bool in(uint64_t members) const { return live && (members >> token & 1); }
+    __device__ __forceinline__ bool in(uint32_t members) const { return live && (members >> token & 1); }
 };
 
 __device__ __forceinline__ void load_row(const bf16_t* x, int64_t sb, int64_t sn, int64_t sh, int b, const Row& r, int lane, bf16x8 (&f)[4]) {
@@ -470,32 +460,23 @@ __device__ __forceinline__ void mask_keys(f32x16& s, int kt, int hh, int valid, 
     for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < left ? s[e] : fill;
 }
 
-constexpr int kRowTiles = kFwdRows / 32;   // of a wave
 struct FwdState {
-    f32x16 o[2][kRowTiles];   // O^T [dim tile][row tile]
-    float m[kRowTiles], l[kRowTiles], lx[kRowTiles];   // reference, and this lane's parts of the sums of the rounded and unrounded P
+    f32x16 o[2];      // O^T [dim tile]
+    float m, l, lx;   // reference, and this lane's parts of the sums of the rounded and unrounded P
 };
 
 // SAFE: the rows that are no members of a tile get their accumulators back after its products
 template <bool LSE, bool SAFE>
-__device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds<kFwdRows>& L, int b, int h, int n0, int split,
-                                       const Row (&row)[kRowTiles], const bf16x8 (&qf)[kRowTiles][4], FwdState& a) {
+__device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int split, const Row& row,
+                                       const bf16x8 (&qf)[4], FwdState& a) {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     TileReads tr;
     tr.init(lane);
-#pragma unroll
-    for (int qt = 0; qt < kRowTiles; ++qt) {
-        a.o[0][qt] = splat(0.f);
-        a.o[1][qt] = splat(0.f);
-        a.m[qt] = -INFINITY;
-        a.l[qt] = a.lx[qt] = 0.f;
-    }
-    for_tiles(p, L, b, h, n0, split, p.splits, [&](const bf16_t* Kt, const bf16_t* Vt, uint64_t members, int valid) {
-        f32x16 s[2][kRowTiles];   // [key half][row tile]
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int qt = 0; qt < kRowTiles; ++qt) s[kt][qt] = splat(0.f);
+    a.o[0] = a.o[1] = splat(0.f);
+    a.m = -FLT_MAX;   // finite, so that keys whose score is -inf are exp2(-inf) = 0 also before any other
+    a.l = a.lx = 0.f;
+    for_tiles(p, L, b, h, n0, split, p.splits, [&](const bf16_t* Kt, const bf16_t* Vt, uint32_t members, int valid) {
+        f32x16 s[2] = {splat(0.f), splat(0.f)};   // [key half]
         // operands are read two steps ahead (at this register count the compiler would otherwise read
         // each where it is used, and wait for it)
         bf16x8 k[4][2];
@@ -507,9 +488,7 @@ __device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds<kFwdRow
 #pragma unroll
         for (int ds = 0; ds < 4; ++ds) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int qt = 0; qt < kRowTiles; ++qt) s[kt][qt] = mfma32(k[ds][kt], qf[qt][ds], s[kt][qt]);
+            for (int kt = 0; kt < 2; ++kt) s[kt] = mfma32(k[ds][kt], qf[ds], s[kt]);
             if (ds < 2) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) k[ds + 2][kt] = tr.rows(Kt, 32 * kt, ds + 2);
@@ -518,80 +497,62 @@ __device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds<kFwdRow
         }
         if (valid < 64) {
             seldom();
-#pragma unroll
-            for (int qt = 0; qt < kRowTiles; ++qt) {
-                mask_keys(s[0][qt], 0, hh, valid, -INFINITY);
-                mask_keys(s[1][qt], 1, hh, valid, -INFINITY);
-            }
+            mask_keys(s[0], 0, hh, valid, -INFINITY);
+            mask_keys(s[1], 1, hh, valid, -INFINITY);
         }
         // (the maximum that NaN wins takes three operands and no canonicalising instruction)
-        float mt[kRowTiles];
-        bool member[kRowTiles], move[kRowTiles], any = false;
+        float mt = s[0][0];
 #pragma unroll
-        for (int qt = 0; qt < kRowTiles; ++qt) {
-            mt[qt] = s[0][qt][0];
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mt[qt] = __builtin_elementwise_maximum(mt[qt], s[kt][qt][e]);
-            mt[qt] = xor32_max(mt[qt]) * p.c;
-            member[qt] = row[qt].in(members);
-            move[qt] = member[qt] && mt[qt] > a.m[qt] + kTau;
-            any |= move[qt];
-        }
-        if (__builtin_amdgcn_ballot_w64(any)) {   // rare after a row's first tile
-#pragma unroll
-            for (int qt = 0; qt < kRowTiles; ++qt) {
-                const float alpha = move[qt] ? __builtin_amdgcn_exp2f(a.m[qt] - mt[qt]) : 1.f;
-                a.m[qt] = move[qt] ? mt[qt] : a.m[qt];
-                a.o[0][qt] *= alpha;
-                a.o[1][qt] *= alpha;
-                a.l[qt] *= alpha;
-                if constexpr (LSE) a.lx[qt] *= alpha;
-            }
+            for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
+        mt = xor32_max(mt) * p.c;
+        const bool member = row.in(members), move = member && mt > a.m + kTau;
+        if (__builtin_amdgcn_ballot_w64(move)) {   // rare after a row's first tile
+            const float alpha = move ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
+            a.m = move ? mt : a.m;
+            a.o[0] *= alpha;
+            a.o[1] *= alpha;
+            a.l *= alpha;
+            if constexpr (LSE) a.lx *= alpha;
         }
         bf16x8 v[2];          // V^T of the first 16 keys: read before the exponentials
         if constexpr (!SAFE) {
             v[0] = tr.cols(Vt, 0, 0);
             v[1] = tr.cols(Vt, 0, 1);
         }
-        bf16x8 pb[kRowTiles][2][2];   // [row tile][key half][16-key step]
+        const float ref = member ? a.m : INFINITY;   // P = 0 for the others
+        bf16x8 pb[2][2];                             // [key half][16-key step]
+        float lt[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int qt = 0; qt < kRowTiles; ++qt) {
-            const float ref = member[qt] ? a.m[qt] : INFINITY;   // P = 0 for the others
-            float lt[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int s2 = 0; s2 < 2; ++s2) {
+                uint32_t w[4];
 #pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][qt][8 * s2 + 2 * i], p.c, -ref));
-                        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][qt][8 * s2 + 2 * i + 1], p.c, -ref));
-                        if constexpr (LSE) sum[kt] += p0 + p1;
-                        w[i] = pack_bf16x2(p0, p1);
-                    }
-                    pb[qt][kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-                    lt[kt] = operand_sum(pb[qt][kt][s2], lt[kt]);
+                for (int i = 0; i < 4; ++i) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i], p.c, -ref));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i + 1], p.c, -ref));
+                    if constexpr (LSE) sum[kt] += p0 + p1;
+                    w[i] = pack_bf16x2(p0, p1);
                 }
-            if (!SAFE || member[qt]) {
-                a.l[qt] += lt[0] + lt[1];
-                if constexpr (LSE) a.lx[qt] += sum[0] + sum[1];
+                pb[kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+                lt[kt] = operand_sum(pb[kt][s2], lt[kt]);
             }
+        if (!SAFE || member) {
+            a.l += lt[0] + lt[1];
+            if constexpr (LSE) a.lx += sum[0] + sum[1];
         }
         if constexpr (SAFE) {
 #pragma unroll
-            for (int dt = 0; dt < 2; ++dt)
+            for (int dt = 0; dt < 2; ++dt) {
+                f32x16 y = a.o[dt];
 #pragma unroll
-                for (int qt = 0; qt < kRowTiles; ++qt) {
-                    f32x16 y = a.o[dt][qt];
+                for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                        for (int s2 = 0; s2 < 2; ++s2) y = mfma32(tr.cols(Vt, 32 * kt + 16 * s2, dt), pb[qt][kt][s2], y);
-                    if (member[qt]) a.o[dt][qt] = y;
-                }
+                    for (int s2 = 0; s2 < 2; ++s2) y = mfma32(tr.cols(Vt, 32 * kt + 16 * s2, dt), pb[kt][s2], y);
+                if (member) a.o[dt] = y;
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -600,9 +561,7 @@ __device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds<kFwdRow
 #pragma unroll
                     for (int dt = 0; dt < 2; ++dt) next[dt] = tr.cols(Vt, 16 * (j + 1), dt);
 #pragma unroll
-                for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-                    for (int qt = 0; qt < kRowTiles; ++qt) a.o[dt][qt] = mfma32(v[dt], pb[qt][j >> 1][j & 1], a.o[dt][qt]);
+                for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(v[dt], pb[j >> 1][j & 1], a.o[dt]);
                 if (j < 3) {
                     v[0] = next[0];
                     v[1] = next[1];
@@ -621,8 +580,8 @@ __device__ __forceinline__ bool finite(const f32x16& x) {
 }
 
 template <bool LSE>
-__global__ __launch_bounds__(kThreads, kFwdRows == 32 ? 3 : 2) void query_attn_kernel(QueryAttnParams p, int total) {
-    __shared__ RowsLds<kFwdRows> L;
+__global__ __launch_bounds__(kThreads, 3) void query_attn_kernel(QueryAttnParams p, int total) {
+    __shared__ RowsLds L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = xcd_remap(blockIdx.x, total);
@@ -630,42 +589,33 @@ __global__ __launch_bounds__(kThreads, kFwdRows == 32 ? 3 : 2) void query_attn_k
     const int h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
     load_tokens(p, L, b, h, n0);
-    Row row[kRowTiles];
-    bf16x8 qf[kRowTiles][4];
-#pragma unroll
-    for (int qt = 0; qt < kRowTiles; ++qt) {
-        row[qt].init(p, L, b, h, n0, wave, 32 * qt + (lane & 31));
-        load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row[qt], lane, qf[qt]);
-    }
-#pragma unroll
-    for (int qt = 0; qt < kRowTiles; ++qt) arrived(qf[qt]);
+    Row row;
+    row.init(p, L, b, h, n0, wave, lane & 31);
+    bf16x8 qf[4];
+    load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
+    arrived(qf);
     FwdState a;
     attend<LSE, false>(p, L, b, h, n0, split, row, qf, a);
-    bool ok = true;
-#pragma unroll
-    for (int qt = 0; qt < kRowTiles; ++qt) ok = ok && finite(a.o[0][qt]) && finite(a.o[1][qt]) && a.l[qt] - a.l[qt] == 0.f;
+    const bool ok = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f;
     if (__syncthreads_or(!ok)) attend<LSE, true>(p, L, b, h, n0, split, row, qf, a);
+    const float l = xor32_add(a.l), lx = LSE ? xor32_add(a.lx) : 0.f;
+    if (!row.live) return;
+    if (p.splits > 1) {
+        const int64_t rows = (int64_t)p.B * p.Nq * p.Hq;
+        float* d = p.part_o + (split * rows + row.at) * 64 + 4 * hh;
 #pragma unroll
-    for (int qt = 0; qt < kRowTiles; ++qt) {
-        const float l = xor32_add(a.l[qt]), lx = LSE ? xor32_add(a.lx[qt]) : 0.f;
-        if (!row[qt].live) continue;
-        const f32x16 o[2] = {a.o[0][qt], a.o[1][qt]};
-        if (p.splits > 1) {
-            const int64_t rows = (int64_t)p.B * p.Nq * p.Hq;
-            float* d = p.part_o + (split * rows + row[qt].at) * 64 + 4 * hh;
+        for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4)
-                    *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) = make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
-            if (hh == 0) p.part_ml[split * rows + row[qt].at] = make_float4(a.m[qt], l, lx, 0.f);
-            continue;
-        }
-        // a row without a key has l = 0 (any other at least 2^-8, or NaN)
-        store_row(p.out, row[qt].at, lane, o, l == 0.f ? 0.f : 1.f / l);
-        if constexpr (LSE)
-            if (hh == 0) p.lse[row[qt].at] = a.m[qt] + __builtin_amdgcn_logf(lx);
+            for (int g4 = 0; g4 < 4; ++g4)
+                *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) =
+                    make_float4(a.o[dt][4 * g4], a.o[dt][4 * g4 + 1], a.o[dt][4 * g4 + 2], a.o[dt][4 * g4 + 3]);
+        if (hh == 0) p.part_ml[split * rows + row.at] = make_float4(a.m, l, lx, 0.f);
+        return;
     }
+    // a row without a key, or with none whose score is above -inf, has l = 0 (any other at least 2^-8, or NaN)
+    store_row(p.out, row.at, lane, a.o, l == 0.f ? 0.f : 1.f / l);
+    if constexpr (LSE)
+        if (hh == 0) p.lse[row.at] = a.m + __builtin_amdgcn_logf(lx);
 }
 
 // Joins the splits' partials: 16 lanes a row, 4 dims each.  Lane j holds the weights of splits j and
@@ -683,7 +633,7 @@ __global__ __launch_bounds__(kThreads) void query_attn_join_kernel(QueryAttnPara
     float m = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-    // l = 0: no key in that share (its m is -inf, as is that of one with nothing but NaN)
+    // l = 0: no key in that share (its m is the lowest value, as is that of one with nothing but NaN)
     float a[2], l = 0.f, lx = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -735,14 +685,14 @@ struct DqState {
 
 // SAFE as in the forward
 template <bool SAFE>
-__device__ __forceinline__ void differentiate(const QueryAttnParams& p, RowsLds<kDqRows>& L, int b, int h, int n0, const Row& row,
+__device__ __forceinline__ void differentiate(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, const Row& row,
                                               const bf16x8 (&qf)[4], const bf16x8 (&gf)[4], float nlse, float delta, DqState& a) {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     TileReads tr;
     tr.init(lane);
     a.dq[0] = a.dq[1] = a.kbar[0] = a.kbar[1] = splat(0.f);
     a.sum = a.rest = 0.f;
-    for_tiles(p, L, b, h, n0, 0, 1, [&](const bf16_t* Kt, const bf16_t* Vt, uint64_t members, int valid) {
+    for_tiles(p, L, b, h, n0, 0, 1, [&](const bf16_t* Kt, const bf16_t* Vt, uint32_t members, int valid) {
         const bool member = row.in(members);
         const float off = member ? 0.f : -INFINITY;   // P = 0 and dS = 0 for the others
 #pragma unroll 1
@@ -812,7 +762,7 @@ __device__ __forceinline__ void differentiate(const QueryAttnParams& p, RowsLds<
 }
 
 __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnParams p, int total) {
-    __shared__ RowsLds<kDqRows> L;
+    __shared__ RowsLds L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = xcd_remap(blockIdx.x, total);
@@ -836,7 +786,8 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
         for (int i = 0; i < 4; ++i) delta = fmaf(bf_lo(ow[i]), bf_lo(gw[i]), fmaf(bf_hi(ow[i]), bf_hi(gw[i]), delta));
     }
     delta = xor32_add(delta);
-    float nlse = -p.lse[row.at] / p.c;
+    const float lse = p.lse[row.at];
+    float nlse = lse == -INFINITY ? 0.f : -lse / p.c;   // (nothing to add up for a row without a key)
     asm volatile("" : "+v"(nlse));
     arrived(qf);
     arrived(gf);
@@ -1276,7 +1227,7 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
     if (K > kMaxSelected) return MOSAIC_ERR_UNSUPPORTED;
     // ids of workgroups and keys stay in 31 bits
     if (nk > 0x7fffffff - bs || nq > 0x7fffffff - kMarkTokens) return MOSAIC_ERR_SHAPE;
-    const int64_t per = kWaves * (kDqRows / (hq / hk)), tiles = ((int64_t)nq + per - 1) / per;
+    const int64_t per = kWaves * (kRows / (hq / hk)), tiles = ((int64_t)nq + per - 1) / per;
     if ((double)tiles * hk * batch * kMaxSplit > 2147483647.0) return MOSAIC_ERR_SHAPE;
     if ((double)((nk + 63) / 64) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
     if (((double)nq / kThreads + 1) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
@@ -1285,7 +1236,7 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
 
 // Workgroups of one share: below one per CU the union is split, up to two per CU together.
 int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
-    const int64_t per = kWaves * (kFwdRows / (hq / hk));
+    const int64_t per = kWaves * (kRows / (hq / hk));
     const int64_t wgs = (nq + per - 1) / per * hk * batch;
     if (wgs >= 256) return 1;
     const int64_t s = 512 / wgs;
@@ -1293,7 +1244,7 @@ int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
 }
 
 // Whether tokens may be taken in another order: with more than one workgroup of them.
-bool may_order(int32_t nq, int32_t hq, int32_t hk) { return nq > kWaves * (kFwdRows / (hq / hk)); }
+bool may_order(int32_t nq, int32_t hq, int32_t hk) { return nq > kWaves * (kRows / (hq / hk)); }
 int key_chunks(int32_t nq) { return (nq + kThreads - 1) / kThreads; }
 size_t order_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
     if (!may_order(nq, hq, hk)) return 0;
@@ -1404,7 +1355,7 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
     if (block_indices == nullptr || out == nullptr) return MOSAIC_ERR_NULL_POINTER;
     if (!aligned(block_indices, 8) || !aligned(out, 16) || !aligned(lse, 4) || !aligned(kv_lens, 4)) return MOSAIC_ERR_ALIGNMENT;
     QueryAttnParams p{};
-    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kFwdRows);
+    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kRows);
     p.out = static_cast<bf16_t*>(out);
     p.lse = lse;
     p.splits = choose_split(batch, num_queries, num_q_heads, num_kv_heads, block_count);
@@ -1453,7 +1404,7 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     // token lists are indexed in 31 bits
     if (at.items > 0x7fffffff || at.pairs > 0x7fffffff) return MOSAIC_ERR_SHAPE;
     QueryAttnParams p{};
-    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kDqRows);
+    fill(p, q, k, v, block_indices, kv_lens, batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count, softmax_scale, kRows);
     p.go = static_cast<const bf16_t*>(grad_out.ptr);
     p.go_sb = grad_out.stride_b; p.go_sn = grad_out.stride_n; p.go_sh = grad_out.stride_h;
     auto spans = [&](const mosaic_bnhd& t) {   // a sequence's rows lie within 2^32 bytes of its first

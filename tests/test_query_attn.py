@@ -397,3 +397,121 @@ def test_the_run_of_operators_as_they_are_used():
     mask[0, 3] = True
     out, idx = M.mosaic_query_attn(q, k, v, bs, K, block_mask=mask, return_block_indices=True)
     assert bool((idx[0, ..., 0] == 3).all()) and bool((idx[0, ..., 1:] == -1).all()) and not out[1].any()
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hk,K", [(4, 1, 3), (6, 2, 5)])
+def test_a_block_that_every_token_wants(Hq, Hk, K):
+    """Its keys' gradients are shared out over workgroups and summed; twice the same bits."""
+    gen = torch.Generator(device=DEV).manual_seed(10)
+    B, Nq, Nk, bs = 1, 2000, 1250, 64
+    q, k, v, go = randn(gen, B, Nq, Hq, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nq, Hq, 64)
+    idx = choose(gen, B, Nq, Hk, 20, K, "far")
+    idx[..., 0], idx[:, 1000:, :, 1] = 3, 19                       # one of them the ragged last block
+    lens = torch.tensor([1230], device=DEV)
+    want = oracle(q, k, v, idx, bs, lens=lens, go=go)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = M.query_sparse_attn(*leaves, idx, bs, kv_lens=lens)
+    got = torch.autograd.grad(out, leaves, go, retain_graph=True)
+    for name, g in zip(("o", "dq", "dk", "dv"), (out.detach(), *got)):
+        near(g, want[name], name)
+    assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(out, leaves, go)))
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hk,Nq,K", [(2, 2, 1500, 40), (16, 1, 300, 70), (3, 1, 1000, 1)])
+def test_scattered_tokens(Hq, Hk, Nq, K):
+    """Tokens that share little with the ones beside them, in unions of more than 64 blocks.  A
+    token's result does not depend on the order of the tokens (workgroups as many either way)."""
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    B, Nk, bs = 2, 130 * 64, 64
+    q, k, v, go = randn(gen, B, Nq, Hq, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nq, Hq, 64)
+    idx = choose(gen, B, Nq, Hk, 130, K, "far")
+    want = oracle(q, k, v, idx, bs, go=go)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = M.query_sparse_attn(*leaves, idx, bs)
+    for name, g in zip(("o", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, go))):
+        near(g, want[name], name)
+    perm = torch.randperm(Nq, generator=gen, device=DEV)
+    assert torch.equal(M.query_sparse_attn(q[:, perm], k, v, idx[:, perm], bs), out.detach()[:, perm])
+
+
+@gpu
+def test_more_blocks_than_are_united_at_a_time():
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    B, Nq, nb, Hq, Hk, bs = 1, 37, 2100, 4, 1, 64
+    Nk = nb * bs - 17
+    q, k, v, go = randn(gen, B, Nq, Hq, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nq, Hq, 64)
+    idx = choose(gen, B, Nq, Hk, nb, 6, "far")
+    idx[..., :3] = torch.tensor([1023, 1024, nb - 1], device=DEV)
+    idx[:, ::2, :, 0] = 2048
+    want = oracle(q, k, v, idx, bs, go=go)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = M.query_sparse_attn(*leaves, idx, bs)
+    for name, g in zip(("o", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, go))):
+        near(g, want[name], name)
+
+
+@gpu
+def test_keys_whose_scores_are_minus_infinity():
+    """They have no weight, wherever they stand among a row's keys; with nothing else a row is zeros."""
+    gen = torch.Generator(device=DEV).manual_seed(13)
+    for Nq in (3, 400):                                                     # with a share of the blocks each, and without
+        q, k, v = randn(gen, 1, Nq, 4, 64), randn(gen, 1, 640, 1, 64), randn(gen, 1, 640, 1, 64)
+        q[..., 0] = 1
+        k[:, :128, :, 0] = -float("inf")                                    # blocks 0 and 1
+        k[:, 300:310, :, 0] = -float("inf")                                 # and keys of block 4
+        idx = torch.tensor([0, 4, 1, 7], device=DEV).expand(1, Nq, 1, 4).clone()
+        idx[:, 2] = torch.tensor([0, 1, 1, -1], device=DEV)
+        out = M.query_sparse_attn(q, k, v, idx, 64)
+        assert torch.isfinite(out).all() and not out[:, 2].any()
+        kf = k.clone()
+        kf[:, 300:310, :, 0] = -1e30
+        rows = torch.arange(Nq, device=DEV) != 2
+        near(out[:, rows], tuple(x[:, rows] for x in oracle(q, kf, v, idx.clamp(4, 9), 64)["o"]), "output")
+
+
+@gpu
+def test_query_and_gradient_offsets_past_32_bits():
+    # rows of q and of the gradient 2^25 elements apart: the last begin past 2^32 bytes and elements
+    apart, Nq = 1 << 25, 140
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    small = randn(gen, 1, Nq, 2, 64), randn(gen, 1, Nq, 2, 64)
+    wide = [torch.empty((Nq - 1) * apart + 128, device=DEV, dtype=BF16).as_strided((1, Nq, 2, 64), (0, apart, 64, 1)) for _ in small]
+    for w, s in zip(wide, small):
+        w.copy_(s)
+    k, v = randn(gen, 1, 256, 1, 64), randn(gen, 1, 256, 1, 64)
+    idx = torch.tensor([0, 2], device=DEV).view(1, 1, 1, 2).expand(1, Nq, 1, 2)
+
+    def run(q, go):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = M.query_sparse_attn(*leaves, idx, 64)
+        return (out.detach(), *torch.autograd.grad(out, leaves, go))
+    assert all(torch.equal(a, b) for a, b in zip(run(*wide), run(*small)))
+
+
+@gpu
+def test_calls_on_two_streams_at_once():
+    gen = torch.Generator(device=DEV).manual_seed(15)
+    sets = []
+    for Nq in (2, 900):
+        q, k, v, go = randn(gen, 1, Nq, 4, 64), randn(gen, 1, 2560, 1, 64), randn(gen, 1, 2560, 1, 64), randn(gen, 1, Nq, 4, 64)
+        sets.append((q, k, v, go, choose(gen, 1, Nq, 1, 40, 8, "far")))
+
+    def step(q, k, v, go, idx):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = M.query_sparse_attn(*leaves, idx, 64)
+        return (out.detach(), *torch.autograd.grad(out, leaves, go))
+    want = [step(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(5):
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(step(*s))
+    for st in streams:
+        torch.cuda.current_stream().wait_stream(st)
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2])), i
