@@ -27,10 +27,10 @@
 // workgroup ends with a value that is not finite it runs again, each product's accumulators restored
 // for the rows that are no members, and what a row did not choose does not reach it then either.
 //
-// Bound by the vector ALU's exponentials and packing beside the products, at three waves a SIMD: 231 us
-// for 49152 tokens of 16 blocks of 64 keys in one kv head of four query heads (nside 64), 206 Gflop and
-// 51 MB at least; two passes of 2 x 64 x 64 flops a score make that 0.89 Pflop/s.  Each further block
-// costs 11.4 us, and 57 us are spent before the first.  64 rows a wave (two waves a SIMD, half the LDS
+// Bound by the vector ALU (exponentials, maxima, packing) beside the products, at three waves a SIMD:
+// 49152 tokens with 12 query and 3 kv heads and 16 blocks of 64 keys (nside 64), 155 Gflop and 207 MB,
+// take 231 us, 0.67 Pflop/s (a large matrix product reaches 1.2).  Each further block costs
+// 11.4 us, and 57 us are spent before the first.  64 rows a wave (two waves a SIMD, half the LDS
 // reads a score) measured 253 us there, 262 instead of 205 for two members' 10007 stations and 11.6
 // instead of 9.4 for one token; 16 rows (v_mfma_f32_16x16x32_bf16) 345.
 //
