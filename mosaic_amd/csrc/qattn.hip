@@ -86,7 +86,7 @@ struct QueryAttnParams {
     uint16_t* keys;            // [B, Hk, Nq] bucket of each token (null: tokens in their own order)
     int32_t* order;            // [B, Hk, Nq] tokens in the order they are taken in,
     int32_t* ordered;          // [B, Hk] where this is not 0
-    int32_t* far;              // [B, Hk, chunks of 256 tokens]
+    int32_t* far;              // [B, Hk, chunks of 32 tokens] of them far from the one before
     int B, Nq, Nk, Hq, Hk, G, QW, bs, K, nb, words;
     int qtiles, splits;
     int qw_inverse;            // t / QW = t qw_inverse >> 16 for t < 256
@@ -118,42 +118,77 @@ __device__ __forceinline__ void arrived(bf16x8& x) {
     x = as_bf16x8(u);
 }
 
+// The logical workgroup of a launched one: an XCD (workgroups go to the eight in turn) takes runs of
+// 32 neighbours, which share key blocks in its L2, from all over the call, because sequences of a
+// padded batch differ in work.  (One range of all the neighbours each, two sequences of 46209 and
+// 44969 keys: 206 us instead of 183; runs of 8, 16, 64 and 128 are within 3 % of these there, and of
+// each other where the work is even.)  The last, incomplete round keeps its order.
+__device__ __forceinline__ int xcd_runs(int id, int total) {
+    constexpr int kRun = 32;
+    const int in = id & (8 * kRun - 1), first = id - in;
+    return first + 8 * kRun > total ? id : first + (in & 7) * kRun + (in >> 3);
+}
+
 __device__ __forceinline__ int seq_keys(const QueryAttnParams& p, int b) {
     return p.lens == nullptr ? p.Nk : min(max(p.lens[b], 0), p.Nk);
 }
 
 // ------------------------------------------------------------------ the order of tokens
-// Tokens of one kv head by a block of theirs: the middle entry of the row or, where that is no
-// block, the next one that is (query_topk's rows ascend, so it is their median).
+// Tokens of one kv head by a block of theirs: the one nearest the mean of them, in whatever order
+// the row has them.  (10007 stations whose rows are in the order of scores: 22.0 blocks in a
+// workgroup's union, as by the median; by the row's middle entry 31.7, by the mean itself 24.1.)
 
-__device__ __forceinline__ int bucket_of(const QueryAttnParams& p, int64_t blk) {
-    return p.nb <= kBuckets ? (int)blk : (int)(blk * kBuckets / p.nb);
+__device__ __forceinline__ int bucket_of(const QueryAttnParams& p, int blk) {
+    return p.nb <= kBuckets ? blk : (int)((int64_t)blk * kBuckets / p.nb);
 }
 
-// A workgroup takes 256 tokens of one (b, h) and counts those that lie more than a 32nd of the blocks
-// from the token before.
+// A workgroup takes 32 tokens of one (b, h), eight lanes a token, and counts those that lie more
+// than a 32nd of the blocks from the token before.
+constexpr int kKeyTokens = kThreads / 8;
 __global__ __launch_bounds__(kThreads) void query_keys_kernel(QueryAttnParams p, int chunks) {
-    __shared__ int far[kWaves];
+    __shared__ int keys[kKeyTokens];
     const int bh = blockIdx.x / chunks, chunk = blockIdx.x - bh * chunks, h = bh % p.Hk, b = bh / p.Hk;
-    const int n = chunk * kThreads + threadIdx.x, lane = threadIdx.x & 63;
-    int key = kBuckets;
-    if (n < p.Nq) {
-        const int64_t* e = p.idx + (((int64_t)b * p.Nq + n) * p.Hk + h) * p.K;
-        for (int i = 0, at = p.K / 2; i < p.K; ++i) {
-            const int64_t blk = e[at];
-            if (blk >= 0 && blk < p.nb) {
-                key = bucket_of(p, blk);
-                break;
-            }
-            at = at + 1 == p.K ? 0 : at + 1;
-        }
-        p.keys[(int64_t)bh * p.Nq + n] = (uint16_t)key;
+    const int tid = threadIdx.x, n0 = chunk * kKeyTokens, tokens = min(kKeyTokens, p.Nq - n0);
+    const int64_t* e = p.idx + (((int64_t)b * p.Nq + n0 + min(tid >> 3, tokens - 1)) * p.Hk + h) * p.K;
+    auto entry = [&](int i) {   // -1: none
+        const int64_t blk = e[i];
+        return blk >= 0 && blk < p.nb ? (int)blk : -1;
+    };
+    float sum = 0.f, count = 0.f;
+    for (int i = tid & 7; i < p.K; i += 8) {
+        const int blk = entry(i);
+        sum += blk >= 0 ? (float)blk : 0.f;
+        count += blk >= 0 ? 1.f : 0.f;
     }
-    const int before = __shfl_up(key, 1);
-    const uint64_t jumps = __builtin_amdgcn_ballot_w64(lane > 0 && n < p.Nq && abs(key - before) * 32 > min(p.nb, kBuckets));
-    if (lane == 0) far[threadIdx.x >> 6] = (int)__builtin_popcountll(jumps);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+        sum += __shfl_xor(sum, d);
+        count += __shfl_xor(count, d);
+    }
+    const float mean = sum / count;
+    float off = INFINITY;
+    int nearest = -1;
+    auto take = [&](float d, int blk) {
+        const bool better = blk >= 0 && (d < off || (d == off && blk < nearest));
+        off = better ? d : off;
+        nearest = better ? blk : nearest;
+    };
+    for (int i = tid & 7; i < p.K; i += 8) {
+        const int blk = entry(i);
+        take(fabsf((float)blk - mean), blk);
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+        const float u = __shfl_xor(off, d);
+        take(u, __shfl_xor(nearest, d));
+    }
+    if ((tid & 7) == 0) keys[tid >> 3] = nearest < 0 ? kBuckets : bucket_of(p, nearest);
     __syncthreads();
-    if (threadIdx.x == 0) p.far[blockIdx.x] = far[0] + far[1] + far[2] + far[3];
+    if (tid >= 64) return;
+    const bool jump = tid > 0 && tid < tokens && abs(keys[tid] - keys[tid - 1]) * 32 > min(p.nb, kBuckets);
+    if (tid < tokens) p.keys[(int64_t)bh * p.Nq + n0 + tid] = (uint16_t)keys[tid];
+    const uint64_t jumps = __builtin_amdgcn_ballot_w64(jump);
+    if (tid == 0) p.far[blockIdx.x] = (int)__builtin_popcountll(jumps);
 }
 
 // One workgroup = one (b, h): a counting sort by bucket.  Where the tokens' own order is already one
@@ -584,7 +619,7 @@ __global__ __launch_bounds__(kThreads, 3) void query_attn_kernel(QueryAttnParams
     __shared__ RowsLds L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_remap(blockIdx.x, total);
+    const int id = xcd_runs(blockIdx.x, total);
     const int split = id % p.splits, tile_id = id / p.splits % p.qtiles, rest = id / p.splits / p.qtiles;
     const int h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
@@ -765,7 +800,7 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
     __shared__ RowsLds L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_remap(blockIdx.x, total);
+    const int id = xcd_runs(blockIdx.x, total);
     const int tile_id = id % p.qtiles, rest = id / p.qtiles;
     const int h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
@@ -966,7 +1001,7 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), kh = w >> 1, qh = w & 1;
     const int items = p.slots[total];
     if ((int)blockIdx.x >= items) return;
-    const int2 item = p.items[xcd_remap(blockIdx.x, items)];
+    const int2 item = p.items[xcd_runs(blockIdx.x, items)];
     const int kt = item.x % tiles, rest = item.x / tiles, h = rest % p.Hk, b = rest / p.Hk;
     const int share = item.y & 0xffff, shares = item.y >> 16;
     const int key0 = kt * 64, end = seq_keys(p, b);
@@ -1230,7 +1265,7 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
     const int64_t per = kWaves * (kRows / (hq / hk)), tiles = ((int64_t)nq + per - 1) / per;
     if ((double)tiles * hk * batch * kMaxSplit > 2147483647.0) return MOSAIC_ERR_SHAPE;
     if ((double)((nk + 63) / 64) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
-    if (((double)nq / kThreads + 1) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
+    if (((double)nq / kKeyTokens + 1) * hk * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
     return MOSAIC_OK;
 }
 
@@ -1245,7 +1280,7 @@ int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
 
 // Whether tokens may be taken in another order: with more than one workgroup of them.
 bool may_order(int32_t nq, int32_t hq, int32_t hk) { return nq > kWaves * (kRows / (hq / hk)); }
-int key_chunks(int32_t nq) { return (nq + kThreads - 1) / kThreads; }
+int key_chunks(int32_t nq) { return (nq + kKeyTokens - 1) / kKeyTokens; }
 size_t order_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
     if (!may_order(nq, hq, hk)) return 0;
     const size_t rows = (size_t)batch * hk * nq;
