@@ -855,10 +855,17 @@ __global__ __launch_bounds__(kThreads) void query_marks_kernel(QueryAttnParams p
     for (int i = threadIdx.x; i < nc * kMarkWords; i += kThreads) bits[i] = 0;
     __syncthreads();
     const int n0 = grp * kMarkTokens, tokens = min(kMarkTokens, p.Nq - n0);
-    for (int e = threadIdx.x; e < tokens * p.K; e += kThreads) {
-        const int t = e / p.K, kk = e - t * p.K;
-        const int64_t blk = p.idx[(((int64_t)b * p.Nq + n0 + t) * p.Hk + h) * p.K + kk] - c0;
-        if (blk >= 0 && blk < nc) atomicOr(&bits[blk * kMarkWords + t / 32], 1u << (t % 32));
+    // two lanes a token, eight entries of theirs at once (one seen twice does no harm)
+    for (int t = threadIdx.x / 2; t < tokens; t += kThreads / 2) {
+        const int64_t* e = p.idx + (((int64_t)b * p.Nq + n0 + t) * p.Hk + h) * p.K;
+        for (int k0 = threadIdx.x % 2; k0 < p.K; k0 += 16) {
+            int64_t blk[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) blk[j] = e[min(k0 + 2 * j, p.K - 1)] - c0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (blk[j] >= 0 && blk[j] < nc) atomicOr(&bits[blk[j] * kMarkWords + t / 32], 1u << (t % 32));
+        }
     }
     __syncthreads();
     uint32_t* out = p.marks + (((int64_t)b * p.Hk + h) * p.nb + c0) * p.words + grp * kMarkWords;
@@ -1001,7 +1008,7 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), kh = w >> 1, qh = w & 1;
     const int items = p.slots[total];
     if ((int)blockIdx.x >= items) return;
-    const int2 item = p.items[xcd_runs(blockIdx.x, items)];
+    const int2 item = p.items[xcd_remap(blockIdx.x, items)];   // (their work is even)
     const int kt = item.x % tiles, rest = item.x / tiles, h = rest % p.Hk, b = rest / p.Hk;
     const int share = item.y & 0xffff, shares = item.y >> 16;
     const int key0 = kt * 64, end = seq_keys(p, b);
