@@ -46,42 +46,62 @@ struct QueryTopkParams {
     int qtiles;
 };
 
-// max (or min) over the wave, in every lane: DPP steps within 16 lanes, then the swaps of 16- and
-// 32-lane halves
-template <bool MAX>
-__device__ __forceinline__ float either(float a, float b) { return MAX ? fmaxf(a, b) : fminf(a, b); }
-template <bool MAX, int CTRL>
-__device__ __forceinline__ float dpp_either(float x) {
-    return either<MAX>(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false)));
+// Signed integers in the order of the floats (none is NaN), and back
+__device__ __forceinline__ int order_key(float x) {
+    const int i = __float_as_int(x);
+    return i ^ ((i >> 31) & 0x7fffffff);
 }
+__device__ __forceinline__ float key_value(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+
+// max (or min) over the wave, in every lane: DPP steps within 16 lanes, then the swaps of 16- and
+// 32-lane halves (of integers: a float's maximum is two instructions and takes no DPP operand)
 template <bool MAX>
-__device__ __forceinline__ float wave_either(float x) {
+__device__ __forceinline__ int either(int a, int b) { return MAX ? max(a, b) : min(a, b); }
+template <bool MAX, int CTRL>
+__device__ __forceinline__ int dpp_either(int x) { return either<MAX>(x, __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true)); }
+template <bool MAX>
+__device__ __forceinline__ float wave_either(float y) {
+    int x = order_key(y);
     x = dpp_either<MAX, 0xb1>(x);    // quad_perm [1,0,3,2]
     x = dpp_either<MAX, 0x4e>(x);    // quad_perm [2,3,0,1]
     x = dpp_either<MAX, 0x141>(x);   // row_half_mirror
     x = dpp_either<MAX, 0x140>(x);   // row_mirror
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = either<MAX>(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return either<MAX>(__uint_as_float(c[0]), __uint_as_float(c[1]));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = either<MAX>((int)a[0], (int)a[1]);
+    const auto c = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return key_value(__builtin_amdgcn_readfirstlane(either<MAX>((int)c[0], (int)c[1])));
 }
 __device__ __forceinline__ float wave_max(float x) { return wave_either<true>(x); }
 __device__ __forceinline__ float wave_min(float x) { return wave_either<false>(x); }
 
-// The K-th largest of the lanes' values (-inf among them; none is NaN), by bisection: a compare and a
-// population count per step.  -inf where fewer than K are above it.
-__device__ __forceinline__ float wave_kth(float x, int K, int lane) {
-    auto count = [&](float t) { return (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= t)); };
-    if (count(-__FLT_MAX__) < K) return -INFINITY;
+__device__ __forceinline__ int lanes_from(float x, float t) { return (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= t)); }
+
+// A value that at least K, and where it can be found so soon no more than `most`, of the lanes' values
+// (-inf among them; none is NaN) reach, by bisection: a compare and a population count per step.
+// -inf where fewer than K are above it.
+__device__ __forceinline__ float reached_by(float x, int K, int most) {
+    if (lanes_from(x, -__FLT_MAX__) < K) return -INFINITY;
     float hi = wave_max(x), lo = wave_min(x == -INFINITY ? INFINITY : x);
-    if (count(hi) >= K) return hi;
-    for (;;) {   // count(lo) >= K > count(hi)
+    if (lanes_from(x, hi) >= K) return hi;
+    for (;;) {   // lo is reached by K or more, hi by fewer
         const float mid = 0.5f * lo + 0.5f * hi;
         if (!(mid > lo && mid < hi)) return lo;   // neighbours
-        const int n = count(mid);
-        if (n == K) return wave_min(x >= mid ? x : INFINITY);
-        if (n > K) lo = mid; else hi = mid;
+        const int n = lanes_from(x, mid);
+        if (n >= K) {
+            lo = mid;
+            if (n <= most) return lo;
+        } else {
+            hi = mid;
+        }
     }
+}
+
+// The larger of three; a NaN among them does not count (v_max3_f32 alone: the compiler would put a
+// canonicalising instruction before each operand)
+__device__ __forceinline__ float larger(float a, float b, float c) {
+    float y;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+    return y;
 }
 
 // Lane of the n-th set bit of m (anything past the last)
@@ -232,9 +252,8 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
                     s = mfma16(as_bf16x8(a[j][0]), lo[0], s);
                     s = mfma16(as_bf16x8(a[j][1]), lo[1], s);
                 }
-                // lane: blocks 16 t + 4 g4 + e of query c16 (a maximum with -inf takes NaN out); the flag
-                // of block c is lane c's
-                float4 v = make_float4(fmaxf(s[0], -INFINITY), fmaxf(s[1], -INFINITY), fmaxf(s[2], -INFINITY), fmaxf(s[3], -INFINITY));
+                // lane: blocks 16 t + 4 g4 + e of query c16; the flag of block c is lane c's
+                float4 v = make_float4(s[0], s[1], s[2], s[3]);
                 const uint32_t ons = (uint32_t)__builtin_amdgcn_ballot_w64(on[j]);
                 if (ons != ~0u) {
                     const uint32_t four = ons >> (4 * g4);
@@ -250,10 +269,11 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             for (int r = threadIdx.x / 64; r < kRows; r += NW) sc[r * kStride + i] = -INFINITY;
         {   // |k|^2 <= the sum over the four dim groups of their largest
             float m = kn;
-            m = dpp_either<true, 0xb1>(m);
-            m = dpp_either<true, 0x4e>(m);
-            m = dpp_either<true, 0x141>(m);
-            m = dpp_either<true, 0x140>(m);
+            int key = __float_as_int(m);   // (of no negative ones: in order as they are)
+            key = dpp_either<true, 0xb1>(key);
+            key = dpp_either<true, 0x4e>(key);
+            key = dpp_either<true, 0x141>(key);
+            m = __int_as_float(dpp_either<true, 0x140>(key));
             m += __shfl_xor(m, 16);
             m += __shfl_xor(m, 32);
             if (lane == 0) knorm[wave] = m;
@@ -270,19 +290,41 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             v[0] = u0 > 0 && lane < carry_n[r] ? carry_v[r][lane] : -INFINITY;
 #pragma unroll
             for (int i = 0; i < PL; ++i) v[1 + i] = sc[r * kStride + lane + 64 * i];
-            float top = v[0];
+            static_assert(PL % 2 == 0, "pairs of scores");
+            float top = larger(v[0], v[1], v[2]);
 #pragma unroll
-            for (int i = 1; i <= PL; ++i) top = __builtin_elementwise_maximum(top, v[i]);   // no score is NaN
+            for (int i = 3; i < PL; i += 2) top = larger(top, v[i], v[i + 1]);
+            top = larger(top, v[PL], -INFINITY);         // (where all of them are NaN)
             float e2 = 0x1p-14f * qnorm[r] * kmax;       // 2 eps
             if (!(e2 < INFINITY)) e2 = 0.f;
-            // The K-th largest of the lanes' largest scores has K scores at least at or above it: T is
-            // no smaller. Where no more than 64 come within 2 eps of it, as they nearly always do (K
-            // good blocks are spread over the lanes), they go one to a lane, ascending by block.
-            const float least = wave_kth(top, p.K, lane);
+            // Where K of the lanes' largest scores reach a value, T is no smaller.  Scores within 2 eps of
+            // it go one to a lane, ascending by block, where they are no more than 64: nearly always where
+            // K is no more than half the lanes; else the value is raised first.
+            float least = reached_by(top, p.K, max(p.K, min(p.K + 8, 32)));
+            auto all_from = [&](float t) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i <= PL; ++i) n += lanes_from(v[i], t);
+                return n;
+            };
+            if (p.K > 24 && all_from(fmaxf(least - e2, -__FLT_MAX__)) > 64) {
+                float lo = least == -INFINITY ? wave_min(top == -INFINITY ? INFINITY : top) : least, hi = wave_max(top);
+                for (;;) {
+                    const float mid = 0.5f * lo + 0.5f * hi;
+                    if (!(mid > lo && mid < hi)) break;
+                    if (all_from(mid) < p.K) {
+                        hi = mid;
+                        continue;
+                    }
+                    lo = least = mid;
+                    if (all_from(mid - e2) <= 64) break;
+                }
+            }
             const float keep = fmaxf(least - e2, -__FLT_MAX__);
             float* scores = sc + r * kStride;                            // of the first 64, and all codes
             uint16_t* codes = reinterpret_cast<uint16_t*>(scores + 64);   // (64 i + l: element i of lane l)
             asm volatile("" ::: "memory");     // the row's scores are read before these take their place
+            scores[lane] = -INFINITY;
             int n = 0;
 #pragma unroll
             for (int i = 0; i <= PL; ++i) {
@@ -307,7 +349,16 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
                     mine = scores[lane];
                 }
                 if (n > p.K) {
-                    const float T = wave_kth(mine, p.K, lane);
+                    // T is the smallest that has fewer than K above it
+                    int above = 0;
+                    for (int i = 0; i < n; i += 8) {
+                        const float4 x = *reinterpret_cast<const float4*>(scores + i), y = *reinterpret_cast<const float4*>(scores + i + 4);
+                        above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+                        above += (y.x > mine) + (y.y > mine) + (y.z > mine) + (y.w > mine);
+                    }
+                    uint64_t at = 0;
+                    for (int i = p.K - 1; at == 0; --i) at = __builtin_amdgcn_ballot_w64(take && above == i);   // (equal ones: fewer)
+                    const float T = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), (int)__builtin_ctzll(at)));
                     const uint64_t in = __builtin_amdgcn_ballot_w64(mine >= T - e2 && lane < n);
                     take = in >> lane & 1;
                     if ((int)__builtin_popcountll(in) > p.K) {
