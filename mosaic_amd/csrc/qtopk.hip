@@ -15,14 +15,20 @@
 // between than slots are left -- about 1 row in 50 on fields, every row on constant keys -- their
 // scores are formed again in fp64, one block per lane, and compared there.
 //
-// One workgroup = 16 query tokens of one kv head.  Its waves form the scores S^T = K Q^T of up to
-// 64 PL blocks with v_mfma_f32_16x16x32_bf16 into LDS (16 rows of fp32), then each wave takes
-// rows, PL scores per lane in registers.  The K-th largest of the lanes' largest scores bounds T
-// from below, so the scores from there on hold all K; there are seldom more than a few of them, and
-// up to 64 go one to a lane, where T is found by bisection, a compare and a population count per
-// step.  (Bisection over all PL registers, the first form of this kernel: 1105 vector instructions a
-// row at 768 blocks, 432 us for the tokens of nside 64.)  More blocks than 64 PL go in chunks: the
-// rows' best K so far join the next chunk's scores.
+// One workgroup = row tiles of 16 query tokens of one kv head.  Its waves form a tile's scores
+// S^T = K Q^T of up to 64 PL blocks with v_mfma_f32_16x16x32_bf16 into LDS (16 rows of fp32), then
+// each wave takes rows, PL scores per lane in registers.  A value that K of the lanes' largest scores
+// reach, found by a few steps of bisection (a compare and a population count each), bounds T from
+// below, so the scores from there on hold all K; there are seldom more than a few of them, and up to
+// 64 go one to a lane, where each lane counts the larger ones.
+//
+// Bound by the selection's vector instructions and its waits for one another: 49152 tokens with 3 kv
+// heads of 4 query heads and 768 blocks (nside 64), 14.5 Gflop of scores and 94 MB, take 136 us, 49 of
+// them for the scores.  The keys of a chunk stay in registers for as many row tiles as fill the chip
+// once and the next tile's queries are loaded during a selection: with one row tile per workgroup,
+// keys from L2 for each, the scores alone took 133 us, all of it 196.  Exact bisections in both places
+// were 213 us, and bisection over all PL registers, the first form of this kernel, 432.
+// More blocks than 64 PL go in chunks: the rows' best K so far join the next chunk's scores.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -44,6 +50,7 @@ struct QueryTopkParams {
     int64_t* out;               // [B, Nq, Hk, K]
     int B, Nq, nb, Hk, G, K;
     int qtiles;
+    int per, groups;            // row tiles a workgroup takes, workgroups of a (batch, kv head)
 };
 
 // Signed integers in the order of the floats (none is NaN), and back
@@ -153,60 +160,120 @@ __device__ __forceinline__ int exact_above(double x, bool of, double y, bool tie
 }
 
 // PL = 12 at most: two workgroups of 8 waves then share a CU's LDS and fill its 4 waves per SIMD.
-template <int PL, int NW>
+// WHOLE: nb <= 64 PL, one chunk, whose keys stay in registers for all of a workgroup's tiles.
+template <int PL, int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams p) {
     constexpr int kChunk = 64 * PL, kStride = kChunk + 4;
     static_assert(4 * 64 + 2 * 64 * (PL + 1) <= 4 * kStride, "64 scores and a row's codes fit its scores' place");
     __shared__ __attribute__((aligned(16))) float sc[kRows * kStride];
-    __shared__ float carry_v[kRows][kMaxTopk];   // best K of the chunks so far, ascending blocks
-    __shared__ int carry_u[kRows][kMaxTopk];
-    __shared__ int carry_n[kRows];
-    __shared__ float qnorm[kRows], knorm[NW];
+    constexpr int kCarry = WHOLE ? 1 : kRows;
+    __shared__ float carry_v[kCarry][kMaxTopk];   // best K of the chunks so far, ascending blocks
+    __shared__ int carry_u[kCarry][kMaxTopk];
+    __shared__ int carry_n[kCarry];
+    __shared__ float qnorms[2][kRows], knorm[NW];
     __shared__ __attribute__((aligned(16))) bf16_t qpart[2][kRows][72];   // (rows 144 bytes apart: distinct banks)
     __shared__ double qd[NW][64];                // a wave's exact summed query (rows that need it)
 
     const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x % p.qtiles, rest = blockIdx.x / p.qtiles;
+    const int grp = blockIdx.x % p.groups, rest = blockIdx.x / p.groups;
     const int h = rest % p.Hk, b = rest / p.Hk;
-    const int n0 = tile * kRows;
     const bf16_t* kb = p.k + b * p.k_sb + h * p.k_sh;
     const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (int64_t)b * p.nb;
 
-    // the summed queries, each thread a run of dims of one, as hi + lo parts by way of LDS
-    {
-        constexpr int kDims = kRows * 64 / (NW * 64), kLanes = 64 / kDims;   // dims a thread, threads a query
-        static_assert(kDims == 2 || kDims == 1, "one or two dims a thread");
-        const int r = threadIdx.x / kLanes, d = threadIdx.x % kLanes * kDims;
-        const bf16_t* qb = p.q + b * p.q_sb + (int64_t)min(n0 + r, p.Nq - 1) * p.q_sn + (int64_t)h * p.G * p.q_sh + d;
-        float sum[kDims] = {}, tot[kDims] = {};
-#pragma unroll 4
-        for (int g = 0; g < p.G; ++g) {
-            float x[kDims];
-            if constexpr (kDims == 2) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(qb + g * p.q_sh);
-                x[0] = bf_lo(w);
-                x[1] = bf_hi(w);
-            } else {
-                x[0] = bf2f(qb[g * p.q_sh]);
+    // a wave's tiles of 16 blocks of a chunk, every NW-th
+    constexpr int kTiles = 4 * PL / NW;
+    static_assert(kTiles * NW == 4 * PL, "the waves share a chunk's tiles evenly");
+    uint4 a[kTiles][2];
+    uint32_t ons[kTiles];   // the flag of block c of a tile is bit c
+    float kn = 0.f;         // largest squared norm of this lane's dims over the blocks it has loaded
+    auto load_keys = [&](int u0) {
+        bool on[kTiles];
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+            const int u = u0 + 16 * (wave + j * NW) + c16, at = min(u, p.nb - 1);
+            const bf16_t* kr = kb + (int64_t)at * p.k_sn + 8 * g4;
+            a[j][0] = ld16(kr);
+            a[j][1] = ld16(kr + 32);
+            on[j] = u < p.nb;
+            if (mask != nullptr) on[j] = on[j] && mask[at];
+        }
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+            float nn = 0.f;
+            const uint32_t aw[8] = {a[j][0].x, a[j][0].y, a[j][0].z, a[j][0].w, a[j][1].x, a[j][1].y, a[j][1].z, a[j][1].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bf16x2 e = __builtin_bit_cast(bf16x2, aw[i]);
+                nn = __builtin_amdgcn_fdot2_f32_bf16(e, e, nn, false);
             }
+            kn = on[j] ? fmaxf(kn, nn) : kn;
+            ons[j] = (uint32_t)__builtin_amdgcn_ballot_w64(on[j]);
+        }
+        // |k|^2 <= the sum over the four dim groups of their largest
+        float m = kn;
+        int key = __float_as_int(m);   // (of no negative ones: in order as they are)
+        key = dpp_either<true, 0xb1>(key);
+        key = dpp_either<true, 0x4e>(key);
+        key = dpp_either<true, 0x141>(key);
+        m = __int_as_float(dpp_either<true, 0x140>(key));
+        m += __shfl_xor(m, 16);
+        m += __shfl_xor(m, 32);
+        if (lane == 0) knorm[wave] = m;
+    };
+
+    // the summed queries of a row tile, each thread a run of dims of one; the first heads' dims are
+    // loaded a tile ahead
+    constexpr int kDims = kRows * 64 / (NW * 64), kLanes = 64 / kDims;   // dims a thread, threads a query
+    static_assert(kDims == 2 || kDims == 1, "one or two dims a thread");
+    const int qr = threadIdx.x / kLanes, qdim = threadIdx.x % kLanes * kDims;
+    auto query = [&](int tile) {
+        return p.q + b * p.q_sb + (int64_t)min(tile * kRows + qr, p.Nq - 1) * p.q_sn + (int64_t)h * p.G * p.q_sh + qdim;
+    };
+    auto dims = [&](const bf16_t* x) { return kDims == 2 ? *reinterpret_cast<const uint32_t*>(x) : (uint32_t)*x; };
+    constexpr int kAhead = 4;
+    uint32_t ahead[kAhead];
+    auto load_queries = [&](int tile) {
+        const bf16_t* qb = query(tile);
+#pragma unroll
+        for (int g = 0; g < kAhead; ++g) ahead[g] = dims(qb + min(g, p.G - 1) * p.q_sh);
+    };
+
+    const int first = grp * p.per, past = min(first + p.per, p.qtiles);
+    load_queries(first);
+    if constexpr (WHOLE) load_keys(0);
+    for (int tile = first; tile < past; ++tile) {
+    const int n0 = tile * kRows, rows = min(kRows, p.Nq - n0);
+    float* qnorm = qnorms[tile & 1];   // (waves still selecting read the last tile's)
+    {   // as hi + lo parts by way of LDS
+        float sum[kDims] = {}, tot[kDims] = {};
+        auto add = [&](uint32_t w) {
+            const float x[2] = {bf_lo(w), bf_hi(w)};
 #pragma unroll
             for (int i = 0; i < kDims; ++i) {
                 sum[i] += x[i];
                 tot[i] += fabsf(x[i]);
             }
+        };
+#pragma unroll
+        for (int g = 0; g < kAhead; ++g)
+            if (g < p.G) add(ahead[g]);
+        if (p.G > kAhead) {
+            const bf16_t* qb = query(tile);
+#pragma unroll 4
+            for (int g = kAhead; g < p.G; ++g) add(dims(qb + g * p.q_sh));
         }
         float mag = 0.f;
 #pragma unroll
         for (int i = 0; i < kDims; ++i) {
-            const float a = round_bf16(sum[i]);
-            qpart[0][r][d + i] = (bf16_t)(__float_as_uint(a) >> 16);
-            qpart[1][r][d + i] = (bf16_t)(pack_bf16x2(sum[i] - a, 0.f) & 0xffffu);
+            const float hi = round_bf16(sum[i]);
+            qpart[0][qr][qdim + i] = (bf16_t)(__float_as_uint(hi) >> 16);
+            qpart[1][qr][qdim + i] = (bf16_t)(pack_bf16x2(sum[i] - hi, 0.f) & 0xffffu);
             mag = fmaf(tot[i], tot[i], mag);
         }
 #pragma unroll
         for (int m = 1; m < kLanes; m <<= 1) mag += __shfl_xor(mag, m);
-        if (threadIdx.x % kLanes == 0) qnorm[r] = sqrtf(mag);
+        if (threadIdx.x % kLanes == 0) qnorm[qr] = sqrtf(mag);
     }
     __syncthreads();
     bf16x8 hi[2], lo[2];   // of column c16, dims 32 ks + 8 g4 .. + 7
@@ -215,79 +282,41 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
         hi[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[0][c16][32 * ks + 8 * g4]));
         lo[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[1][c16][32 * ks + 8 * g4]));
     }
-    const int rows = min(kRows, p.Nq - n0);
-    float kn = 0.f;   // largest squared norm of this lane's dims over the blocks it has loaded
-    for (int u0 = 0; u0 < p.nb; u0 += kChunk) {
-        const int nc = min(kChunk, p.nb - u0), tiles = (nc + 15) / 16;
-        // a wave's tiles of a whole chunk are requested together
-        constexpr int kTiles = 4 * PL > NW ? 4 * PL / NW : 1;
-        for (int t0 = wave; t0 < tiles; t0 += kTiles * NW) {
-            uint4 a[kTiles][2];
-            bool on[kTiles];
+    for (int u0 = 0; u0 < (WHOLE ? 1 : p.nb); u0 += kChunk) {
+        if constexpr (!WHOLE) load_keys(u0);
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-                const int u = u0 + 16 * (t0 + j * NW) + c16, at = min(u, p.nb - 1);
-                const bf16_t* kr = kb + (int64_t)at * p.k_sn + 8 * g4;
-                a[j][0] = ld16(kr);
-                a[j][1] = ld16(kr + 32);
-                on[j] = u < p.nb;
-                if (mask != nullptr) on[j] = on[j] && mask[at];
+        for (int j = 0; j < kTiles; ++j) {
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+            s = mfma16(as_bf16x8(a[j][0]), hi[0], s);
+            s = mfma16(as_bf16x8(a[j][1]), hi[1], s);
+            if (p.G > 1) {
+                s = mfma16(as_bf16x8(a[j][0]), lo[0], s);
+                s = mfma16(as_bf16x8(a[j][1]), lo[1], s);
             }
-#pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-                const int t = t0 + j * NW;
-                if (t >= tiles) break;
-                float nn = 0.f;
-                const uint32_t aw[8] = {a[j][0].x, a[j][0].y, a[j][0].z, a[j][0].w, a[j][1].x, a[j][1].y, a[j][1].z, a[j][1].w};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bf16x2 e = __builtin_bit_cast(bf16x2, aw[i]);
-                    nn = __builtin_amdgcn_fdot2_f32_bf16(e, e, nn, false);
-                }
-                kn = on[j] ? fmaxf(kn, nn) : kn;
-                f32x4 s = {0.f, 0.f, 0.f, 0.f};
-                s = mfma16(as_bf16x8(a[j][0]), hi[0], s);
-                s = mfma16(as_bf16x8(a[j][1]), hi[1], s);
-                if (p.G > 1) {
-                    s = mfma16(as_bf16x8(a[j][0]), lo[0], s);
-                    s = mfma16(as_bf16x8(a[j][1]), lo[1], s);
-                }
-                // lane: blocks 16 t + 4 g4 + e of query c16; the flag of block c is lane c's
-                float4 v = make_float4(s[0], s[1], s[2], s[3]);
-                const uint32_t ons = (uint32_t)__builtin_amdgcn_ballot_w64(on[j]);
-                if (ons != ~0u) {
-                    const uint32_t four = ons >> (4 * g4);
-                    v.x = (four & 1) ? v.x : -INFINITY;
-                    v.y = (four & 2) ? v.y : -INFINITY;
-                    v.z = (four & 4) ? v.z : -INFINITY;
-                    v.w = (four & 8) ? v.w : -INFINITY;
-                }
-                *reinterpret_cast<float4*>(sc + c16 * kStride + 16 * t + 4 * g4) = v;
+            // lane: blocks 16 t + 4 g4 + e of query c16; -inf where there is none or the mask leaves it out
+            float4 v = make_float4(s[0], s[1], s[2], s[3]);
+            uint32_t bits = ons[j];
+            asm volatile("" : "+s"(bits));   // (the tests of all tiles would be held in registers otherwise)
+            if (bits != ~0u) {
+                const uint32_t four = bits >> (4 * g4);
+                v.x = (four & 1) ? v.x : -INFINITY;
+                v.y = (four & 2) ? v.y : -INFINITY;
+                v.z = (four & 4) ? v.z : -INFINITY;
+                v.w = (four & 8) ? v.w : -INFINITY;
             }
-        }
-        for (int i = 16 * tiles + threadIdx.x % 64; i < kChunk; i += 64)   // no blocks behind the last tile
-            for (int r = threadIdx.x / 64; r < kRows; r += NW) sc[r * kStride + i] = -INFINITY;
-        {   // |k|^2 <= the sum over the four dim groups of their largest
-            float m = kn;
-            int key = __float_as_int(m);   // (of no negative ones: in order as they are)
-            key = dpp_either<true, 0xb1>(key);
-            key = dpp_either<true, 0x4e>(key);
-            key = dpp_either<true, 0x141>(key);
-            m = __int_as_float(dpp_either<true, 0x140>(key));
-            m += __shfl_xor(m, 16);
-            m += __shfl_xor(m, 32);
-            if (lane == 0) knorm[wave] = m;
+            *reinterpret_cast<float4*>(sc + c16 * kStride + 16 * (wave + j * NW) + 4 * g4) = v;
         }
         __syncthreads();
+        const bool last = WHOLE || u0 + kChunk >= p.nb;
+        if (last && tile + 1 < past) load_queries(tile + 1);
         float kmax = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) kmax = fmaxf(kmax, knorm[i]);
         kmax = sqrtf(kmax);
-        const bool last = u0 + kChunk >= p.nb;
         for (int r = wave; r < rows; r += NW) {
             // element 0: the carried best, element 1 + i: block u0 + lane + 64 i; -inf where there is none
             float v[PL + 1];
-            v[0] = u0 > 0 && lane < carry_n[r] ? carry_v[r][lane] : -INFINITY;
+            v[0] = !WHOLE && u0 > 0 && lane < carry_n[r] ? carry_v[r][lane] : -INFINITY;
 #pragma unroll
             for (int i = 0; i < PL; ++i) v[1 + i] = sc[r * kStride + lane + 64 * i];
             static_assert(PL % 2 == 0, "pairs of scores");
@@ -304,7 +333,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             auto all_from = [&](float t) {
                 int n = 0;
 #pragma unroll
-                for (int i = 0; i <= PL; ++i) n += lanes_from(v[i], t);
+                for (int i = WHOLE; i <= PL; ++i) n += lanes_from(v[i], t);
                 return n;
             };
             if (p.K > 24 && all_from(fmaxf(least - e2, -__FLT_MAX__)) > 64) {
@@ -312,12 +341,13 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
                 for (;;) {
                     const float mid = 0.5f * lo + 0.5f * hi;
                     if (!(mid > lo && mid < hi)) break;
-                    if (all_from(mid) < p.K) {
+                    const int n = all_from(mid);
+                    if (n < p.K) {
                         hi = mid;
                         continue;
                     }
                     lo = least = mid;
-                    if (all_from(mid - e2) <= 64) break;
+                    if (n <= 64 && all_from(mid - e2) <= 64) break;
                 }
             }
             const float keep = fmaxf(least - e2, -__FLT_MAX__);
@@ -327,7 +357,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             scores[lane] = -INFINITY;
             int n = 0;
 #pragma unroll
-            for (int i = 0; i <= PL; ++i) {
+            for (int i = WHOLE; i <= PL; ++i) {
                 const uint64_t m = __builtin_amdgcn_ballot_w64(v[i] >= keep);
                 if (m == 0) continue;
                 const int pos = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
@@ -338,7 +368,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
                 }
             }
             asm volatile("" ::: "memory");     // (LDS is in order within a wave)
-            auto block = [&](int code) { return code < 64 ? carry_u[r][code] : u0 + code - 64; };
+            auto block = [&](int code) { return !WHOLE && code < 64 ? carry_u[r][code] : u0 + code - 64; };
             bool take;
             float mine = -INFINITY;
             int u = 0;
@@ -403,7 +433,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             const int count = (int)__builtin_popcountll(m);
             const int pos = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
             asm volatile("" ::: "memory");         // the carried blocks are read before they are written
-            if (last) {
+            if (WHOLE || last) {
                 int64_t* row = p.out + (((int64_t)b * p.Nq + n0 + r) * p.Hk + h) * p.K;
                 if (take) row[pos] = u;
                 if (lane >= count && lane < p.K) row[lane] = -1;
@@ -417,11 +447,12 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
         }
         if (!last) __syncthreads();   // the rows' scores are read before the next chunk's are written
     }
+    }
 }
 
-template <int PL>
+template <int PL, bool WHOLE>
 const void* topk_fn(bool wide) {
-    return wide ? (const void*)&query_topk_kernel<PL, 16> : (const void*)&query_topk_kernel<PL, 8>;
+    return wide ? (const void*)&query_topk_kernel<PL, 16, WHOLE> : (const void*)&query_topk_kernel<PL, 8, WHOLE>;
 }
 
 bool rows_ok(const mosaic_bnhd& t) {
@@ -455,8 +486,16 @@ extern "C" int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uin
     const int64_t wgs = (int64_t)p.qtiles * num_kv_heads * batch;
     if (wgs > 0x7fffffff) return MOSAIC_ERR_SHAPE;
     const bool wide = wgs < 256;
-    const void* fn = num_blocks <= 256 ? topk_fn<4>(wide) : num_blocks <= 512 ? topk_fn<8>(wide) : topk_fn<12>(wide);
+    const void* fn = num_blocks <= 256   ? topk_fn<4, true>(wide)
+                     : num_blocks <= 512 ? topk_fn<8, true>(wide)
+                     : num_blocks <= 768 ? topk_fn<12, true>(wide)
+                                         : topk_fn<12, false>(wide);
+    // Two workgroups are resident on a CU.  Each takes as many row tiles of its kv head as fill the chip
+    // once, so that keys (of one chunk) are loaded once; about four times where kv heads are many.
+    const int64_t heads = (int64_t)num_kv_heads * batch, want = (heads <= 64 ? 512 : 2048) / heads;
+    p.per = (int)(want < 1 ? p.qtiles : ((int64_t)p.qtiles + want - 1) / want);
+    p.groups = (p.qtiles + p.per - 1) / p.per;
     void* args[] = {&p};
-    return hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(wide ? 1024 : 512), args, 0, static_cast<hipStream_t>(stream)) == hipSuccess
+    return hipLaunchKernel(fn, dim3((unsigned)(p.groups * heads)), dim3(wide ? 1024 : 512), args, 0, static_cast<hipStream_t>(stream)) == hipSuccess
                ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
