@@ -504,7 +504,8 @@ MOSAIC_API int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uin
    bf16 [B, Nk, Hk, 64]; block_indices: int64 [B, Nq, Hk, K] contiguous; out: bf16 [B, Nq, Hq, 64]
    contiguous; lse: optional fp32 [B, Nq, Hq], base 2 of the scaled logits.  block_size a multiple
    of 64 (the last block may be short), at most 16 query heads per kv head, K at most 1024.
-   workspace: mosaic_query_attn_fwd_workspace_size() bytes (0 for many queries), 256-byte aligned.
+   workspace: mosaic_query_attn_fwd_workspace_size() bytes (partials of few queries, the order of
+   many; 0 where there is neither), 256-byte aligned.
    softmax_scale <= 0 selects 64^-0.5.  mosaic_sparse_attn (ops.py:557-566) is the counterpart for
    query blocks. */
 MOSAIC_API size_t mosaic_query_attn_fwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_q_heads,

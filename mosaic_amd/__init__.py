@@ -3,7 +3,10 @@
 Drop-in Python surface of the reference op (primitives.py / ops.py):
 ``mosaic_attn_func``, ``block_attention``, ``attn_topk``, ``mosaic_sparse_attn``,
 ``MosaicAttnFunction``, ``RoPE``, ``MosaicAttention``; ``mosaic_attn_func_rope`` runs the op
-with the input side's RoPE fused into its pooling pass.  All compute runs in libmosaic_bsa.so
+with the input side's RoPE fused into its pooling pass.  For query tokens that are not the mesh
+itself: ``query_topk`` and ``query_sparse_attn`` (together ``mosaic_query_attn``), each token's own key
+blocks and the attention over them; ``rope_axes`` and ``qk_norm_rope``, rotary positions with several
+axes and the norm of query and key heads.  All compute runs in libmosaic_bsa.so
 (built with ``python -m mosaic_amd.build``) through its C ABI (include/mosaic_bsa.h).
 """
 

@@ -19,7 +19,9 @@
 // Bound by HBM: q and k are read once and written once (the norm's backward reads x and g).  A
 // group of D/8 lanes owns one token: a lane holds the same 8 dimensions of every head, so its
 // cosines and sines are formed once and used by all heads, and the norm is a sum over the group.
-// Four heads' loads are in flight per lane.
+// Four heads' loads are in flight per lane.  196608 tokens of 12 + 3 heads of 64 in bf16 (757 MB) take
+// 149 us, 5.1 TB/s, and as many with the norm (sequence-first) 151, where a copy of 1 GiB reaches
+// 5.2; the norm's backward on 49152 tokens of 16 + 4 heads (378 MB) 72 us and 5 for the weights'.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(RotParams p) {
 }
 
 // Column sums of the partials [rows, 2 D] -> q's [D] and k's [D] (either may be null): a workgroup
-// takes 8 columns, 32 rows at a time.
+// takes 8 columns, 32 rows at a time, eight loads a thread in flight (2048 rows: 5.5 us; one at a time 10.8).
 __global__ __launch_bounds__(kThreads) void wgrad_kernel(const float* partial, int rows, int D, float* dwq, float* dwk) {
     __shared__ float part[32][9];
     const int c = threadIdx.x & 7, r0 = threadIdx.x >> 3;

@@ -168,3 +168,17 @@ def test_captured_and_on_another_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(idx, oracle(q, kc, 8))
+
+
+@gpu
+@pytest.mark.parametrize("B,Nq,nb,Hq,Hk,K,masked", [
+    (1, 20011, 700, 4, 1, 16, True),        # forty row tiles a workgroup, the last one short
+    (40, 49, 130, 4, 2, 9, False),          # more kv heads than a round of workgroups has for one
+    (3, 2500, 1000, 6, 3, 5, True),         # two chunks for each of several row tiles
+    (1, 3000, 768, 12, 2, 40, False),       # more than four query heads, more blocks than half the lanes
+])
+def test_several_row_tiles_a_workgroup(B, Nq, nb, Hq, Hk, K, masked):
+    gen = torch.Generator(device=DEV).manual_seed(Nq)
+    q, kc = randn(gen, B, Nq, Hq, 64), randn(gen, B, nb, Hk, 64)
+    mask = torch.rand(B, nb, generator=gen, device=DEV) < 0.5 if masked else None
+    assert torch.equal(M.query_topk(q, kc, K, mask), oracle(q, kc, K, mask))
