@@ -509,7 +509,7 @@ MOSAIC_API int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uin
    softmax_scale <= 0 selects 64^-0.5.  mosaic_sparse_attn (ops.py:557-566) is the counterpart for
    query blocks. */
 MOSAIC_API size_t mosaic_query_attn_fwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_q_heads,
-                                                       int32_t num_kv_heads, int32_t block_count);
+                                                       int32_t num_kv_heads, int32_t block_size, int32_t block_count);
 MOSAIC_API int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int64_t* block_indices,
                                      const int32_t* kv_lens, int32_t batch, int32_t num_queries, int32_t num_keys,
                                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,

@@ -216,7 +216,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mosaic_qk_norm_rotate_bwd.restype = c_int
     lib.mosaic_query_topk_fwd.argtypes = [Bnhd, Bnhd, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp]
     lib.mosaic_query_topk_fwd.restype = c_int
-    lib.mosaic_query_attn_fwd_workspace_size.argtypes = [c_i32] * 5
+    lib.mosaic_query_attn_fwd_workspace_size.argtypes = [c_i32] * 6
     lib.mosaic_query_attn_fwd_workspace_size.restype = c_size
     lib.mosaic_query_attn_fwd.argtypes = [Bnhd, Bnhd, Bnhd, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                           c_i32, c_f, c_vp, c_vp, c_vp, c_size, c_vp]

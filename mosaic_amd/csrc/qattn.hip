@@ -35,12 +35,13 @@
 // instead of 9.4 for one token; 16 rows (v_mfma_f32_16x16x32_bf16) 345.
 //
 // Few queries: the union is split over workgroups and the partial (m, l, O) joined by a second
-// kernel.
+// kernel, or, where they have few keys too, a workgroup's waves share them (query_attn_few_kernel).
 #include <hip/hip_runtime.h>
 
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "bsa_common.h"
 #include "lds_dma.h"
@@ -453,11 +454,13 @@ struct Row {
     int token, head;
     bool live;
     int64_t n, at;
-        __device__ __forceinline__ void init(const QueryAttnParams& p, const RowsLds& L, int b, int h, int n0, int wave, int r) {
+        // tokens(i): the token at position n0 + i of the order
+    template <typename Tokens>
+    __device__ __forceinline__ void init(const QueryAttnParams& p, const Tokens& tokens, int b, int h, int n0, int wave, int r) {
         token = r / p.G;
         live = token < p.QW && n0 + wave * p.QW + token < p.Nq;
         head = h * p.G + (live ? r - token * p.G : 0);
-        n = L.tokens[wave * p.QW + (live ? token : 0)];
+        n = tokens(wave * p.QW + (live ? token : 0));
         at = ((int64_t)b * p.Nq + n) * p.Hq + head;
     }
     __device__ __forceinline__ bool in(uint32_t members) const { return live && (members >> token & 1); }
@@ -501,109 +504,120 @@ struct FwdState {
     float m, l, lx;   // reference, and this lane's parts of the sums of the rounded and unrounded P
 };
 
-// SAFE: the rows that are no members of a tile get their accumulators back after its products
-template <bool LSE, bool SAFE>
-__device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int split, const Row& row,
-                                       const bf16x8 (&qf)[4], FwdState& a) {
-    const int lane = threadIdx.x & 63, hh = lane >> 5;
-    TileReads tr;
-    tr.init(lane);
+// One tile of 64 keys, keys(half, step) its A operands.  SAFE: the rows that are no members of it get
+// their accumulators back after its products.
+template <bool LSE, bool SAFE, typename Keys>
+__device__ __forceinline__ void attend_tile(float c, const TileReads& tr, const Keys& keys, const bf16_t* Vt, const bf16x8 (&qf)[4],
+                                            bool member, int valid, FwdState& a) {
+    const int hh = (threadIdx.x & 63) >> 5;
+    f32x16 s[2] = {splat(0.f), splat(0.f)};   // [key half]
+    // operands are read two steps ahead (at this register count the compiler would otherwise read
+    // each where it is used, and wait for it)
+    bf16x8 k[4][2];
+#pragma unroll
+    for (int ds = 0; ds < 2; ++ds)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) k[ds][kt] = keys(kt, ds);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ds = 0; ds < 4; ++ds) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma32(k[ds][kt], qf[ds], s[kt]);
+        if (ds < 2) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) k[ds + 2][kt] = keys(kt, ds + 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (valid < 64) {
+        seldom();
+        mask_keys(s[0], 0, hh, valid, -INFINITY);
+        mask_keys(s[1], 1, hh, valid, -INFINITY);
+    }
+    // (the maximum that NaN wins takes three operands and no canonicalising instruction)
+    float mt = s[0][0];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
+    mt = xor32_max(mt) * c;
+    const bool move = member && mt > a.m + kTau;
+    if (__builtin_amdgcn_ballot_w64(move)) {   // rare after a row's first tile
+        const float alpha = move ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
+        a.m = move ? mt : a.m;
+        a.o[0] *= alpha;
+        a.o[1] *= alpha;
+        a.l *= alpha;
+        if constexpr (LSE) a.lx *= alpha;
+    }
+    bf16x8 v[2];          // V^T of the first 16 keys: read before the exponentials
+    if constexpr (!SAFE) {
+        v[0] = tr.cols(Vt, 0, 0);
+        v[1] = tr.cols(Vt, 0, 1);
+    }
+    const float ref = member ? a.m : INFINITY;   // P = 0 for the others
+    bf16x8 pb[2][2];                             // [key half][16-key step]
+    float lt[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i], c, -ref));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i + 1], c, -ref));
+                if constexpr (LSE) sum[kt] += p0 + p1;
+                w[i] = pack_bf16x2(p0, p1);
+            }
+            pb[kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+            lt[kt] = operand_sum(pb[kt][s2], lt[kt]);
+        }
+    if (!SAFE || member) {
+        a.l += lt[0] + lt[1];
+        if constexpr (LSE) a.lx += sum[0] + sum[1];
+    }
+    if constexpr (SAFE) {
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+            f32x16 y = a.o[dt];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) y = mfma32(tr.cols(Vt, 32 * kt + 16 * s2, dt), pb[kt][s2], y);
+            if (member) a.o[dt] = y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bf16x8 next[2];
+            if (j < 3)
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt) next[dt] = tr.cols(Vt, 16 * (j + 1), dt);
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(v[dt], pb[j >> 1][j & 1], a.o[dt]);
+            if (j < 3) {
+                v[0] = next[0];
+                v[1] = next[1];
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void clear(FwdState& a) {
     a.o[0] = a.o[1] = splat(0.f);
     a.m = -FLT_MAX;   // finite, so that keys whose score is -inf are exp2(-inf) = 0 also before any other
     a.l = a.lx = 0.f;
+}
+
+template <bool LSE, bool SAFE>
+__device__ __forceinline__ void attend(const QueryAttnParams& p, RowsLds& L, int b, int h, int n0, int split, const Row& row,
+                                       const bf16x8 (&qf)[4], FwdState& a) {
+    TileReads tr;
+    tr.init(threadIdx.x & 63);
+    clear(a);
     for_tiles(p, L, b, h, n0, split, p.splits, [&](const bf16_t* Kt, const bf16_t* Vt, uint32_t members, int valid) {
-        f32x16 s[2] = {splat(0.f), splat(0.f)};   // [key half]
-        // operands are read two steps ahead (at this register count the compiler would otherwise read
-        // each where it is used, and wait for it)
-        bf16x8 k[4][2];
-#pragma unroll
-        for (int ds = 0; ds < 2; ++ds)
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) k[ds][kt] = tr.rows(Kt, 32 * kt, ds);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int ds = 0; ds < 4; ++ds) {
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) s[kt] = mfma32(k[ds][kt], qf[ds], s[kt]);
-            if (ds < 2) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt) k[ds + 2][kt] = tr.rows(Kt, 32 * kt, ds + 2);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (valid < 64) {
-            seldom();
-            mask_keys(s[0], 0, hh, valid, -INFINITY);
-            mask_keys(s[1], 1, hh, valid, -INFINITY);
-        }
-        // (the maximum that NaN wins takes three operands and no canonicalising instruction)
-        float mt = s[0][0];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
-        mt = xor32_max(mt) * p.c;
-        const bool member = row.in(members), move = member && mt > a.m + kTau;
-        if (__builtin_amdgcn_ballot_w64(move)) {   // rare after a row's first tile
-            const float alpha = move ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
-            a.m = move ? mt : a.m;
-            a.o[0] *= alpha;
-            a.o[1] *= alpha;
-            a.l *= alpha;
-            if constexpr (LSE) a.lx *= alpha;
-        }
-        bf16x8 v[2];          // V^T of the first 16 keys: read before the exponentials
-        if constexpr (!SAFE) {
-            v[0] = tr.cols(Vt, 0, 0);
-            v[1] = tr.cols(Vt, 0, 1);
-        }
-        const float ref = member ? a.m : INFINITY;   // P = 0 for the others
-        bf16x8 pb[2][2];                             // [key half][16-key step]
-        float lt[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i], p.c, -ref));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][8 * s2 + 2 * i + 1], p.c, -ref));
-                    if constexpr (LSE) sum[kt] += p0 + p1;
-                    w[i] = pack_bf16x2(p0, p1);
-                }
-                pb[kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-                lt[kt] = operand_sum(pb[kt][s2], lt[kt]);
-            }
-        if (!SAFE || member) {
-            a.l += lt[0] + lt[1];
-            if constexpr (LSE) a.lx += sum[0] + sum[1];
-        }
-        if constexpr (SAFE) {
-#pragma unroll
-            for (int dt = 0; dt < 2; ++dt) {
-                f32x16 y = a.o[dt];
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int s2 = 0; s2 < 2; ++s2) y = mfma32(tr.cols(Vt, 32 * kt + 16 * s2, dt), pb[kt][s2], y);
-                if (member) a.o[dt] = y;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                bf16x8 next[2];
-                if (j < 3)
-#pragma unroll
-                    for (int dt = 0; dt < 2; ++dt) next[dt] = tr.cols(Vt, 16 * (j + 1), dt);
-#pragma unroll
-                for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(v[dt], pb[j >> 1][j & 1], a.o[dt]);
-                if (j < 3) {
-                    v[0] = next[0];
-                    v[1] = next[1];
-                }
-            }
-        }
+        attend_tile<LSE, SAFE>(p.c, tr, [&](int kt, int ds) { return tr.rows(Kt, 32 * kt, ds); }, Vt, qf, row.in(members), valid, a);
     });
 }
 
@@ -626,7 +640,7 @@ __global__ __launch_bounds__(kThreads, 3) void query_attn_kernel(QueryAttnParams
     const int n0 = tile_id * kWaves * p.QW;
     load_tokens(p, L, b, h, n0);
     Row row;
-    row.init(p, L, b, h, n0, wave, lane & 31);
+    row.init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
     bf16x8 qf[4];
     load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
     arrived(qf);
@@ -697,6 +711,121 @@ __global__ __launch_bounds__(kThreads) void query_attn_join_kernel(QueryAttnPara
     const float f = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<uint2*>(p.out + row * 64 + d) = make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
     if (p.lse != nullptr && d == 0) p.lse[row] = m + __builtin_amdgcn_logf(lx);
+}
+
+// Few tokens with few keys, one token above all: one launch and no union in LDS.  A workgroup takes 32
+// rows (32 / G tokens) and its waves the tiles of 64 keys in turn, each with its own accumulators; they
+// are joined in LDS.  The tokens' entries, no more than 64, lie one in a lane of every wave.
+//
+// Bound by what one CU reads: 2048 keys (512 KB of k and v) take 14 us and half of them 9.4, where the
+// union split over workgroups and its join take 16 and 11.5, and a launch more of the host (one token of
+// 12 query and 3 kv heads, a call at a time: 15 and 19 us).  At 4096 keys it is 24 to 28 for 15 to 17, so
+// kFewKeys is 2048.  100 tokens with 16 blocks of 64 and 16 heads to one: 15.5 for 34.  12 waves
+// measured 5 % more, 16 spill (24 us), and tiles requested one ahead of their use the same.
+constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves, kFewKeys = 2048;
+
+template <bool LSE>
+__global__ __launch_bounds__(kFewThreads) void query_attn_few_kernel(QueryAttnParams p) {
+    __shared__ __attribute__((aligned(1024))) bf16_t V[kFewWaves][kTileElems];   // a wave's tile, then its O
+    __shared__ float4 ml[kFewWaves][kRows];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tile_id = blockIdx.x % p.qtiles, rest = blockIdx.x / p.qtiles, h = rest % p.Hk, b = rest / p.Hk;
+    const int n0 = tile_id * p.QW, entries = min(p.QW, p.Nq - n0) * p.K, end = seq_keys(p, b), sub = p.bs / 64;
+    const bf16_t* kb = p.k + b * p.k_sb + h * p.k_sh;
+    const bf16_t* vb = p.v + b * p.v_sb + h * p.v_sh;
+    int blk = -1;
+    if (lane < entries) {
+        const int t = lane / p.K;
+        const int64_t u = p.idx[(((int64_t)b * p.Nq + n0 + t) * p.Hk + h) * p.K + lane - t * p.K];
+        blk = u >= 0 && u < p.nb && u * p.bs < end ? (int)u : -1;
+    }
+    Row row;
+    row.init(p, [&](int i) { return n0 + i; }, b, h, n0, 0, r);
+    bf16x8 qf[4];
+    load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
+    // an entry's lane: the tokens with its block, and whether it is the first that names it
+    uint32_t tokens = 0;
+    bool first = blk >= 0;
+    for (int j = 0, t = 0, of = 0; j < entries; ++j) {
+        const bool same = __builtin_amdgcn_readlane(blk, j) == blk;
+        tokens |= same ? 1u << t : 0u;
+        first = first && !(same && j < lane);
+        if (++of == p.K) {
+            of = 0;
+            ++t;
+        }
+    }
+    const uint64_t firsts = __builtin_amdgcn_ballot_w64(first);
+    const int rank = (int)__builtin_popcountll(firsts & ((1ull << lane) - 1ull)), units = (int)__builtin_popcountll(firsts) * sub;
+    TileReads tr;
+    tr.init(lane);
+    FwdState a;
+    auto walk = [&](auto safe) {
+        clear(a);
+        for (int u = wave; u < units; u += kFewWaves) {
+            const int which = (int)((uint32_t)u / (uint32_t)sub);
+            const int src = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(first && rank == which));
+            const int key0 = __builtin_amdgcn_readlane(blk, src) * p.bs + (u - which * sub) * 64;
+            if (key0 >= end) continue;
+            const int valid = min(64, end - key0);
+            bf16x8 k[2][4];   // rows past the end repeat the last one
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const bf16_t* kr = kb + (int64_t)min(key0 + 32 * kt + r, end - 1) * p.k_sn + 8 * hh;
+#pragma unroll
+                for (int ds = 0; ds < 4; ++ds) k[kt][ds] = as_bf16x8(ld16(kr + 16 * ds));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int vr = 8 * i + (lane >> 3), chunk = 8 * ((lane & 7) ^ swz32(vr));
+                dma16_at(vb + (int64_t)min(key0 + vr, end - 1) * p.v_sn + chunk, lds_addr(V[wave] + 8 * i * 64));
+            }
+            wait_vmem();
+            if (valid < 64)
+                for (int z = lane; z < (64 - valid) * 8; z += 64)
+                    *reinterpret_cast<uint4*>(V[wave] + (valid + z / 8) * 64 + z % 8 * 8) = make_uint4(0, 0, 0, 0);
+            asm volatile("" ::: "memory");
+            attend_tile<LSE, decltype(safe)::value>(p.c, tr, [&](int kt, int ds) { return k[kt][ds]; }, V[wave], qf,
+                                                    row.in((uint32_t)__builtin_amdgcn_readlane((int)tokens, src)), valid, a);
+            asm volatile("" ::: "memory");   // the tile is read before the next one, or O, takes its place
+        }
+    };
+    walk(std::false_type{});
+    const bool ok = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f;
+    if (__builtin_amdgcn_ballot_w64(!ok)) walk(std::true_type{});   // (a wave by itself)
+    float4* O = reinterpret_cast<float4*>(V[wave]);   // row r's dims 4 c .. at chunk c ^ (r % 16)
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+            O[r * 16 + ((8 * dt + 2 * g4 + hh) ^ (r & 15))] = make_float4(a.o[dt][4 * g4], a.o[dt][4 * g4 + 1], a.o[dt][4 * g4 + 2], a.o[dt][4 * g4 + 3]);
+    const float l = xor32_add(a.l), lx = LSE ? xor32_add(a.lx) : 0.f;
+    if (hh == 0) ml[wave][r] = make_float4(a.m, l, lx, 0.f);
+    __syncthreads();
+    if (tid >= kRows * 16) return;
+    // 16 threads a row
+    Row to;
+    to.init(p, [&](int i) { return n0 + i; }, b, h, n0, 0, tid / 16);
+    if (!to.live) return;
+    const int tr16 = tid / 16, c = tid % 16;
+    float m = -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) m = fmaxf(m, ml[w][tr16].x);
+    float sum = 0.f, sumx = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+        const float4 part = ml[w][tr16], x = reinterpret_cast<const float4*>(V[w])[tr16 * 16 + (c ^ (tr16 & 15))];
+        const float f = part.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(part.x - m);   // no key: its m is the lowest value
+        sum = fmaf(f, part.y, sum);
+        sumx = fmaf(f, part.z, sumx);
+        o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint2*>(p.out + to.at * 64 + 4 * c) = make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
+    if constexpr (LSE)
+        if (c == 0) p.lse[to.at] = m + __builtin_amdgcn_logf(sumx);
 }
 
 // ------------------------------------------------------------------ backward
@@ -812,7 +941,7 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
         p.counts[i] = 0;   // for query_marks_kernel
     load_tokens(p, L, b, h, n0);
     Row row;
-    row.init(p, L, b, h, n0, wave, lane & 31);
+    row.init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
     bf16x8 qf[4], gf[4];
     load_row(p.q, p.q_sb, p.q_sn, p.q_sh, b, row, lane, qf);
     load_row(p.go, p.go_sb, p.go_sn, p.go_sh, b, row, lane, gf);
@@ -1294,6 +1423,12 @@ int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
     return (int)(s < K ? (s < kMaxSplit ? s : kMaxSplit) : (K < kMaxSplit ? K : kMaxSplit));
 }
 
+// Whether the call is one of query_attn_few_kernel: few workgroups, whose tokens name few keys each.
+bool few(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t bs, int32_t K) {
+    const int64_t tokens = nq < kRows / (hq / hk) ? nq : kRows / (hq / hk), entries = tokens * K;
+    return choose_split(batch, nq, hq, hk, K) > 1 && entries <= 64 && entries * bs <= kFewKeys;
+}
+
 // Whether tokens may be taken in another order: with more than one workgroup of them.
 bool may_order(int32_t nq, int32_t hq, int32_t hk) { return nq > kWaves * (kRows / (hq / hk)); }
 int key_chunks(int32_t nq) { return (nq + kKeyTokens - 1) / kKeyTokens; }
@@ -1388,8 +1523,9 @@ using namespace mosaic;
 extern "C" {
 
 size_t mosaic_query_attn_fwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_q_heads, int32_t num_kv_heads,
-                                            int32_t block_count) {
-    if (check_shape(batch, num_queries, 1, num_q_heads, num_kv_heads, kHeadDim, 64, block_count) != MOSAIC_OK) return 0;
+                                            int32_t block_size, int32_t block_count) {
+    if (check_shape(batch, num_queries, 1, num_q_heads, num_kv_heads, kHeadDim, block_size, block_count) != MOSAIC_OK) return 0;
+    if (few(batch, num_queries, num_q_heads, num_kv_heads, block_size, block_count)) return 0;
     const int s = choose_split(batch, num_queries, num_q_heads, num_kv_heads, block_count);
     const size_t rows = s == 1 ? 0 : (size_t)batch * num_queries * num_q_heads;
     return up(s * rows * kHeadDim * sizeof(float)) + up(s * rows * sizeof(float4)) +
@@ -1411,8 +1547,15 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
     p.lse = lse;
     p.splits = choose_split(batch, num_queries, num_q_heads, num_kv_heads, block_count);
     int64_t rows = (int64_t)batch * num_queries * num_q_heads;
-    const size_t need = mosaic_query_attn_fwd_workspace_size(batch, num_queries, num_q_heads, num_kv_heads, block_count);
+    const size_t need = mosaic_query_attn_fwd_workspace_size(batch, num_queries, num_q_heads, num_kv_heads, block_size, block_count);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256))) return MOSAIC_ERR_WORKSPACE;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (few(batch, num_queries, num_q_heads, num_kv_heads, block_size, block_count)) {
+        p.qtiles = (num_queries + p.QW - 1) / p.QW;
+        void* args[] = {&p};
+        const void* fn = lse != nullptr ? (const void*)&query_attn_few_kernel<true> : (const void*)&query_attn_few_kernel<false>;
+        return launch(fn, dim3((unsigned)(p.qtiles * num_kv_heads * batch)), args, s, kFewThreads) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+    }
     char* ws = static_cast<char*>(workspace);
     if (p.splits > 1) {
         p.part_o = reinterpret_cast<float*>(ws);
@@ -1421,7 +1564,6 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
         ws += up(p.splits * rows * sizeof(float4));
     }
     place_order(p, ws);
-    hipStream_t s = static_cast<hipStream_t>(stream);
     if (int e = launch_order(p, s)) return e;
     int total = p.qtiles * num_kv_heads * batch * p.splits;
     void* args[] = {&p, &total};

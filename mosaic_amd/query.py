@@ -102,7 +102,7 @@ def _attn_fwd(q, k, v, idx, block_size, scale, lens, want_lse):
     out = torch.empty((B, Nq, Hq, d), dtype=torch.bfloat16, device=device)
     lse = torch.empty((B, Nq, Hq), dtype=torch.float32, device=device) if want_lse else None
     L = _lib.lib()
-    nbytes = L.mosaic_query_attn_fwd_workspace_size(B, Nq, Hq, Hk, K)
+    nbytes = L.mosaic_query_attn_fwd_workspace_size(B, Nq, Hq, Hk, block_size, K)
     ws = _scratch(nbytes, device)
     with _on(device):
         st = L.mosaic_query_attn_fwd(qb, kb, vb, idx.data_ptr(), _ptr(lens), B, Nq, Nk, Hq, Hk, d, block_size, K, scale,

@@ -80,7 +80,7 @@ def _call(fn, c):
 ])
 def test_abi_validation(fn, change, status):
     c = dict(q=_lib.Bnhd(FAKE, 0, 256, 64), k=_lib.Bnhd(FAKE, 0, 128, 64), idx=FAKE, B=1, nq=7, nk=200, hq=4, hk=2, d=64, bs=64,
-             K=3, out=FAKE, lse=FAKE, ws=FAKE, n=1 << 40)
+             K=12, out=FAKE, lse=FAKE, ws=FAKE, n=1 << 40)
     c.update(change)
     assert _call(fn, c) == status
 
@@ -88,12 +88,14 @@ def test_abi_validation(fn, change, status):
 @HAVE_LIB
 def test_workspace_sizes():
     L = _lib.lib()
-    # many tokens: their order alone (2 + 4 bytes each and kv head); one block each of one token: nothing
-    assert 6 * 3 * 49152 <= L.mosaic_query_attn_fwd_workspace_size(1, 49152, 12, 3, 16) < 7 * 3 * 49152
-    assert L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 3, 1) == 0
-    one = L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 3, 16)
-    assert one >= 16 * 12 * (64 * 4 + 8) and one % 256 == 0
-    assert L.mosaic_query_attn_fwd_workspace_size(1, 1, 12, 5, 16) == 0       # refused shapes
+    # many tokens: their order alone (2 + 4 bytes each and kv head); few entries of few keys: nothing
+    size = L.mosaic_query_attn_fwd_workspace_size
+    assert 6 * 3 * 49152 <= size(1, 49152, 12, 3, 64, 16) < 7 * 3 * 49152
+    assert size(1, 1, 12, 3, 64, 16) == size(1, 1, 12, 3, 64, 32) == 0
+    one = size(1, 1, 12, 3, 64, 33)
+    assert one >= 32 * 12 * (64 * 4 + 8) and one % 256 == 0
+    assert size(1, 1, 12, 3, 128, 17) > 0
+    assert size(1, 1, 12, 5, 64, 16) == size(1, 1, 12, 3, 96, 16) == 0       # refused shapes
     assert L.mosaic_query_attn_bwd_workspace_size(1, 100, 1000, 12, 3, 64, 5) >= 2 * 4 * 1200 + 3 * 16 * 16 * 4
 
 
@@ -322,10 +324,11 @@ def test_layouts_types_and_empty_calls():
 
 
 @gpu
-def test_captured_replayed_and_on_another_stream():
+@pytest.mark.parametrize("K", [4, 9])          # few keys a workgroup, and a union in shares
+def test_captured_replayed_and_on_another_stream(K):
     gen = torch.Generator(device=DEV).manual_seed(7)
     q, k, v, go = randn(gen, 1, 60, 4, 64), randn(gen, 1, 640, 1, 64), randn(gen, 1, 640, 1, 64), randn(gen, 1, 60, 4, 64)
-    idx = choose(gen, 1, 60, 1, 10, 4, "far")
+    idx = choose(gen, 1, 60, 1, 10, K, "far")
 
     def step():
         leaves = [t.detach().requires_grad_() for t in (q, k, v)]
@@ -345,7 +348,7 @@ def test_captured_replayed_and_on_another_stream():
         held2 = step()
     for i in range(3):
         q.copy_(randn(gen, 1, 60, 4, 64))
-        idx.copy_(choose(gen, 1, 60, 1, 10, 4, "ragged"))
+        idx.copy_(choose(gen, 1, 60, 1, 10, K, "ragged"))
         graph.replay()
         other.replay()
         torch.cuda.synchronize()
@@ -515,3 +518,48 @@ def test_calls_on_two_streams_at_once():
         torch.cuda.current_stream().wait_stream(st)
     for i, g in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2])), i
+
+
+@gpu
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hk,bs,K,how,lens", [
+    (1, 1, 196608, 12, 3, 128, 16, "far", None),          # 16 blocks of two tiles
+    (2, 1, 5000, 4, 1, 256, 8, "far", (4999, 700)),       # the last blocks end inside a tile, and before
+    (3, 5, 900, 8, 1, 64, 7, "ragged", (900, 1, 64)),     # four tokens a workgroup, then one
+    (1, 9, 640, 4, 4, 64, 1, "ragged", None),             # one query head to a kv head
+    (1, 2, 640, 32, 2, 64, 10, "near", (0,)),             # no key at all
+    (2, 40, 2000, 14, 2, 64, 8, "far", (1999, 2000)),     # 28 rows of 32
+])
+def test_few_tokens_with_few_keys(B, Nq, Nk, Hq, Hk, bs, K, how, lens):
+    gen = torch.Generator(device=DEV).manual_seed(Nk + K)
+    q, k, v, go = randn(gen, B, Nq, Hq, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nq, Hq, 64)
+    idx = choose(gen, B, Nq, Hk, -(-Nk // bs), K, how)
+    lens = None if lens is None else torch.tensor(lens, device=DEV)
+    assert _lib.lib().mosaic_query_attn_fwd_workspace_size(B, Nq, Hq, Hk, bs, K) == 0
+    want = oracle(q, k, v, idx, bs, lens=lens, go=go)
+    near(M.query_sparse_attn(q, k, v, idx, bs, kv_lens=lens), want["o"], "output")
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = M.query_sparse_attn(*leaves, idx, bs, kv_lens=lens)
+    for name, g in zip(("o", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, go))):
+        near(g, want[name], name)
+
+
+@gpu
+def test_few_tokens_and_values_that_are_not_finite():
+    """NaN and infinities of one token's block reach that token alone, and none behind the sequence's end."""
+    gen = torch.Generator(device=DEV).manual_seed(16)
+    q, k, v = randn(gen, 1, 8, 4, 64), randn(gen, 1, 640, 1, 64), randn(gen, 1, 640, 1, 64)
+    idx = torch.randint(0, 8, (1, 8, 1, 4), generator=gen, device=DEV)
+    idx[:, 3, :, 0] = 8                                                 # only this token has block 8; nobody has 9
+    lens = torch.tensor([630], device=DEV)
+    value, bound = oracle(q, k, v, idx, 64, lens=lens)["o"]
+    k[:, 512:], v[:, 512:] = float("inf"), float("nan")
+    out = M.query_sparse_attn(q, k, v, idx, 64, kv_lens=lens)
+    rows = torch.arange(8, device=DEV) != 3
+    near(out[:, rows], (value[:, rows], bound[:, rows]), "output")
+    assert not torch.isfinite(out[:, 3]).any()
+    idx[:, 3, :, 0] = 7
+    lens = torch.tensor([460], device=DEV)                              # ends inside block 7
+    k, v = randn(gen, 1, 640, 1, 64), randn(gen, 1, 640, 1, 64)
+    want = oracle(q, k, v, idx, 64, lens=lens)["o"]
+    k[:, 460:], v[:, 460:] = float("nan"), float("inf")
+    near(M.query_sparse_attn(q, k, v, idx, 64, kv_lens=lens), want, "output")
