@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .primitives import pool_mean
-from .rotary import _on, _ptr, _rows, _same_device, _stream, _wants_grad
+from .rotary import _like, _on, _ptr, _rows, _same_device, _stream, _wants_grad
 
 __all__ = ["query_topk", "query_sparse_attn", "mosaic_query_attn"]
 
@@ -32,6 +32,8 @@ __all__ = ["query_topk", "query_sparse_attn", "mosaic_query_attn"]
 def _bf16_heads(what: str, **tensors) -> None:
     """The checks of [B, N, H, 64] tensors that need no device."""
     for name, t in tensors.items():
+        if t.dtype is torch.bfloat16 and t.dim() == 4 and t.shape[3] == 64:
+            continue
         if t.dim() != 4:
             raise ValueError(f"{what}: {name} must be [B, N, H, 64], got shape {tuple(t.shape)}")
         if t.dtype == torch.float16:
@@ -44,8 +46,8 @@ def _bf16_heads(what: str, **tensors) -> None:
 
 
 def _groups(what: str, q: torch.Tensor, k: torch.Tensor) -> None:
-    Hq, Hk = q.shape[2], k.shape[2]
-    if q.shape[0] != k.shape[0]:
+    (B, _, Hq, _), (Bk, _, Hk, _) = q.shape, k.shape
+    if B != Bk:
         raise ValueError(f"{what}: q {tuple(q.shape)} and keys {tuple(k.shape)} disagree on the batch")
     if Hk == 0 or Hq == 0 or Hq % Hk or Hq // Hk > 16:
         raise ValueError(f"{what}: {Hq} query heads must be a multiple of {Hk} kv heads, at most 16 times as many")
@@ -56,7 +58,6 @@ def _as_bf16(t: torch.Tensor):
     return _rows(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16))
 
 
-@torch.no_grad()
 def query_topk(q: torch.Tensor, k_cmp: torch.Tensor, block_count: int, block_mask: torch.Tensor | None = None) -> torch.Tensor:
     """The ``block_count`` key blocks of each query token and kv head: int64 [B, Nq, Hk, K].
 
@@ -80,7 +81,7 @@ def query_topk(q: torch.Tensor, k_cmp: torch.Tensor, block_count: int, block_mas
     idx = torch.empty(B, Nq, Hk, block_count, dtype=torch.int64, device=q.device)
     if idx.numel() == 0:
         return idx
-    (q, qb), (k_cmp, kb) = _as_bf16(q), _as_bf16(k_cmp)
+    (q, qb), (k_cmp, kb) = _as_bf16(q.detach()), _as_bf16(k_cmp.detach())
     mask = None if block_mask is None else block_mask.contiguous()
     with _on(q.device):
         st = _lib.lib().mosaic_query_topk_fwd(qb, kb, _ptr(mask), B, Nq, nb, Hq, Hk, d, block_count, idx.data_ptr(), _stream(q.device))
@@ -99,7 +100,7 @@ def _attn_fwd(q, k, v, idx, block_size, scale, lens, want_lse):
     B, Nq, Hq, d = q.shape
     Nk, Hk = k.shape[1:3]
     K, device = idx.shape[-1], q.device
-    out = torch.empty((B, Nq, Hq, d), dtype=torch.bfloat16, device=device)
+    out = _like(q)
     lse = torch.empty((B, Nq, Hq), dtype=torch.float32, device=device) if want_lse else None
     L = _lib.lib()
     nbytes = L.mosaic_query_attn_fwd_workspace_size(B, Nq, Hq, Hk, block_size, K)
@@ -132,8 +133,7 @@ class _QueryAttn(torch.autograd.Function):
         Nk, Hk = k.shape[1:3]
         device = q.device
         (q, qb), (k, kb), (v, vb), (go, gb) = (_as_bf16(t) for t in (q, k, v, go))
-        gq = torch.empty((B, Nq, Hq, d), dtype=torch.bfloat16, device=device)
-        gk, gv = (torch.empty((B, Nk, Hk, d), dtype=torch.bfloat16, device=device) for _ in range(2))
+        gq, gk, gv = _like(q), _like(k), _like(v)
         L = _lib.lib()
         nbytes = L.mosaic_query_attn_bwd_workspace_size(B, Nq, Nk, Hq, Hk, block_size, idx.shape[-1])
         ws = _scratch(nbytes, device)
@@ -184,10 +184,13 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
     if q.numel() == 0 or k.numel() == 0 or block_indices.numel() == 0:   # no row, or no key for any
         # (a product with nothing, so that gradients of the inputs are zeros)
         return torch.zeros(q.shape, dtype=q.dtype, device=q.device) + 0 * (q[:0].sum() + k[:0].sum() + v[:0].sum()).to(q.dtype)
-    idx = block_indices.to(torch.int64).contiguous()
+    idx = block_indices
+    if idx.dtype is not torch.int64 or not idx.is_contiguous():
+        idx = idx.to(torch.int64).contiguous()
     if _wants_grad(q, k, v):
         return _QueryAttn.apply(q, k, v, idx, block_size, scale, kv_lens)
-    return _attn_fwd(_as_bf16(q), _as_bf16(k), _as_bf16(v), idx, block_size, scale, kv_lens, False)[0].to(q.dtype)
+    out, _ = _attn_fwd(_as_bf16(q), _as_bf16(k), _as_bf16(v), idx, block_size, scale, kv_lens, False)
+    return out if q.dtype is torch.bfloat16 else out.to(q.dtype)
 
 
 def mosaic_query_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_size: int, block_count: int, *,

@@ -44,9 +44,10 @@ def _heads(what: str, q: torch.Tensor, k: torch.Tensor | None) -> None:
     B, N, H, d = q.shape
     if d not in (32, 64, 128):
         raise ValueError(f"{what}: head_dim must be 32, 64 or 128, got {d}")
-    if H == 0 or (k is not None and k.shape[2] == 0):
+    Bk, Nk, Hk, dk = (B, N, 1, d) if k is None else k.shape
+    if H == 0 or Hk == 0:
         raise ValueError(f"{what}: q and k need a head")
-    if k is not None and (k.shape[0] != B or k.shape[1] != N or k.shape[3] != d or k.dtype != q.dtype):
+    if Bk != B or Nk != N or dk != d or (k is not None and k.dtype != q.dtype):
         raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} disagree")
     if B * N >= 1 << 31:
         raise ValueError(f"{what}: B * N must be below 2^31")
@@ -59,15 +60,20 @@ def _no_grad_through(what: str, **tensors) -> None:
 
 
 def _same_device(what: str, q: torch.Tensor, **tensors) -> None:
-    device = q.device
-    if device.type != "cuda":
-        raise ValueError(f"{what}: q must be on a ROCm device, got {device}")
+    if not q.is_cuda:
+        raise ValueError(f"{what}: q must be on a ROCm device, got {q.device}")
+    index = q.get_device()
     for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: {name} is on {t.device}, q on {device}")
+        if t is not None and (t.get_device() != index or not t.is_cuda):
+            raise ValueError(f"{what}: {name} is on {t.device}, q on {q.device}")
 
 
 _here = contextlib.nullcontext()
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of t's shape and type (sooner made than by torch.empty)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _on(device: torch.device):
@@ -166,18 +172,22 @@ def _rotation(cos, sin, positions, axes, interleaved: bool) -> _lib.Rotation | N
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _rotate(q, k, rotation, backward: bool, norm: bool, wq=None, wk=None, eps: float = 0.0):
     """mosaic_qk_rotate_fwd on q and k (k may be None)."""
     B, N, Hq, d = q.shape
     dtype, device = q.dtype, q.device
-    q_out = torch.empty((B, N, Hq, d), dtype=dtype, device=device)
+    q_out = _like(q)
     Hk, k_out, kb, k_ptr = 0, None, _NONE, None
     if k is not None:
         Hk = k.shape[2]
-        k_out = torch.empty((B, N, Hk, d), dtype=dtype, device=device)
+        k_out = _like(k)
         k_ptr = k_out.data_ptr()
     if B * N == 0:
         return q_out, k_out
@@ -251,11 +261,11 @@ class _QkNormRope(torch.autograd.Function):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         B, N, Hq, d = q.shape
         dtype, device = q.dtype, q.device
-        dq = torch.empty((B, N, Hq, d), dtype=dtype, device=device)
+        dq = _like(q)
         Hk, dk, kb, gkb = 0, None, _NONE, _NONE
         if k is not None:
             Hk = k.shape[2]
-            dk = torch.empty((B, N, Hk, d), dtype=dtype, device=device)
+            dk = _like(k)
         weights = (q_weight, k_weight)
         dw = [(torch.empty if B * N else torch.zeros)(d, dtype=torch.float32, device=device) if w is not None and need else None
               for w, need in zip(weights, ctx.needs_input_grad[2:4])]
