@@ -1414,10 +1414,14 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
     return MOSAIC_OK;
 }
 
-// Workgroups of one share: below one per CU the union is split, up to two per CU together.
-int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
+// Workgroups where the union is in one piece.
+int64_t groups_of(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
     const int64_t per = kWaves * (kRows / (hq / hk));
-    const int64_t wgs = (nq + per - 1) / per * hk * batch;
+    return (nq + per - 1) / per * hk * batch;
+}
+// Shares of the union: below one workgroup per CU it is split, up to two per CU together.
+int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
+    const int64_t wgs = groups_of(batch, nq, hq, hk);
     if (wgs >= 256) return 1;
     const int64_t s = 512 / wgs;
     return (int)(s < K ? (s < kMaxSplit ? s : kMaxSplit) : (K < kMaxSplit ? K : kMaxSplit));
@@ -1426,7 +1430,7 @@ int choose_split(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
 // Whether the call is one of query_attn_few_kernel: few workgroups, whose tokens name few keys each.
 bool few(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t bs, int32_t K) {
     const int64_t tokens = nq < kRows / (hq / hk) ? nq : kRows / (hq / hk), entries = tokens * K;
-    return choose_split(batch, nq, hq, hk, K) > 1 && entries <= 64 && entries * bs <= kFewKeys;
+    return groups_of(batch, nq, hq, hk) < 256 && entries <= 64 && entries * bs <= kFewKeys;
 }
 
 // Whether tokens may be taken in another order: with more than one workgroup of them.

@@ -119,7 +119,7 @@ def _axes(what: str, sections: tuple, theta, half: int):
     n = len(sections)
     if not 1 <= n <= _lib.MAX_AXES or min(sections) < 0 or sum(sections) > half:
         raise ValueError(f"{what}: sections {sections} must be 1 to {_lib.MAX_AXES} counts of pairs, at most {half} together")
-    theta = tuple(float(x) for x in theta) if isinstance(theta, tuple) else (float(theta),) * n
+    theta = theta if isinstance(theta, tuple) else (theta,) * n
     if len(theta) != n or not all(0 < x < math.inf for x in theta):
         raise ValueError(f"{what}: theta must be a positive number, or one for each of the {n} axes")
     pad = (0,) * (_lib.MAX_AXES - n)
@@ -129,7 +129,8 @@ def _axes(what: str, sections: tuple, theta, half: int):
 def _positions(what: str, q: torch.Tensor, positions: torch.Tensor, sections, theta):
     """(positions as the kernels take them, counts and thetas), checked."""
     sections = tuple(map(int, sections))
-    axes = _axes(what, sections, tuple(theta) if isinstance(theta, list) else theta, q.shape[3] // 2)
+    theta = tuple(map(float, theta)) if isinstance(theta, (list, tuple)) else float(theta)
+    axes = _axes(what, sections, theta, q.shape[3] // 2)
     B, N, n, shape = q.shape[0], q.shape[1], len(sections), positions.shape
     if shape[-2:] != (N, n) or not (len(shape) == 2 or (len(shape) == 3 and shape[0] in (1, B))):
         raise ValueError(f"{what}: positions {tuple(shape)} must be [N, axes] or [B, N, axes] = {(B, N, n)}")

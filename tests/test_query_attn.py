@@ -528,6 +528,7 @@ def test_calls_on_two_streams_at_once():
     (1, 9, 640, 4, 4, 64, 1, "ragged", None),             # one query head to a kv head
     (1, 2, 640, 32, 2, 64, 10, "near", (0,)),             # no key at all
     (2, 40, 2000, 14, 2, 64, 8, "far", (1999, 2000)),     # 28 rows of 32
+    (1, 1, 5000, 16, 1, 2048, 1, "far", (4000,)),         # one block of 32 tiles
 ])
 def test_few_tokens_with_few_keys(B, Nq, Nk, Hq, Hk, bs, K, how, lens):
     gen = torch.Generator(device=DEV).manual_seed(Nk + K)

@@ -437,3 +437,18 @@ def test_far_token_offsets_past_32_bits():
     a, _ = M.rope_axes(x, None, pos, (32,))
     b, _ = M.rope_axes(x.contiguous(), None, pos, (32,))
     assert torch.equal(a, b)
+
+
+@gpu
+def test_theta_is_read_at_each_call_and_weights_lie_anywhere():
+    gen = torch.Generator(device=DEV).manual_seed(77)
+    q, pos = torch.randn(1, 33, 2, 64, generator=gen, device=DEV), torch.randn(33, 1, generator=gen, device=DEV) * 50
+    theta = torch.tensor(10000.0)
+    first, _ = M.rope_axes(q, None, pos, (32,), theta)
+    assert torch.equal(first, M.rope_axes(q, None, pos, (32,), 10000.0)[0])
+    theta.fill_(100.0)
+    assert torch.equal(M.rope_axes(q, None, pos, (32,), theta)[0], M.rope_axes(q, None, pos, (32,), 100.0)[0])
+    w = torch.rand(131, generator=gen, device=DEV)
+    for at in (1, 2, 3):                    # slices of a larger parameter
+        got, _ = M.qk_norm_rope(q, None, w[at:at + 64], positions=pos, sections=(32,))
+        assert torch.equal(got, M.qk_norm_rope(q, None, w[at:at + 64].clone(), positions=pos, sections=(32,))[0])
