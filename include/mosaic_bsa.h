@@ -518,8 +518,9 @@ MOSAIC_API int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v
 
 /* Gradients of mosaic_query_attn_fwd from its out and lse: grad_q [B, Nq, Hq, 64], grad_k, grad_v
    [B, Nk, Hk, 64], bf16 contiguous, every row written (zeros for keys nobody chose or past a
-   sequence's end), sums in a fixed order.  workspace: mosaic_query_attn_bwd_workspace_size()
-   bytes, 256-byte aligned. */
+   sequence's end), sums in a fixed order.  fwd_workspace: the forward's workspace as that call left
+   it (the order it took the tokens in is read from it), or NULL.  workspace:
+   mosaic_query_attn_bwd_workspace_size() bytes, 256-byte aligned. */
 MOSAIC_API size_t mosaic_query_attn_bwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_keys,
                                                        int32_t num_q_heads, int32_t num_kv_heads, int32_t block_size,
                                                        int32_t block_count);
@@ -527,8 +528,8 @@ MOSAIC_API int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v
                                      mosaic_bnhd grad_out, const int64_t* block_indices, const int32_t* kv_lens,
                                      int32_t batch, int32_t num_queries, int32_t num_keys, int32_t num_q_heads,
                                      int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t block_count,
-                                     float softmax_scale, void* grad_q, void* grad_k, void* grad_v, void* workspace,
-                                     size_t workspace_bytes, void* stream);
+                                     float softmax_scale, const void* fwd_workspace, void* grad_q, void* grad_k,
+                                     void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Name of a status code (static storage). */
 MOSAIC_API const char* mosaic_bsa_strerror(int status);

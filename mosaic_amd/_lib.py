@@ -224,7 +224,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mosaic_query_attn_bwd_workspace_size.argtypes = [c_i32] * 7
     lib.mosaic_query_attn_bwd_workspace_size.restype = c_size
     lib.mosaic_query_attn_bwd.argtypes = [Bnhd, Bnhd, Bnhd, c_vp, c_vp, Bnhd, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32,
-                                          c_i32, c_i32, c_i32, c_i32, c_f, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]
+                                          c_i32, c_i32, c_i32, c_i32, c_f, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]
     lib.mosaic_query_attn_bwd.restype = c_int
     lib.mosaic_bsa_strerror.argtypes = [c_int]
     lib.mosaic_bsa_strerror.restype = ctypes.c_char_p

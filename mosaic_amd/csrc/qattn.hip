@@ -1442,6 +1442,12 @@ size_t order_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
     return up(rows * sizeof(uint16_t)) + up(rows * sizeof(int32_t)) + up((size_t)batch * hk * sizeof(int32_t)) +
            up((size_t)batch * hk * key_chunks(nq) * sizeof(int32_t));
 }
+// Bytes of the forward's partials, behind which its workspace holds the order.
+size_t part_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
+    const int s = choose_split(batch, nq, hq, hk, K);
+    const size_t rows = s == 1 ? 0 : (size_t)batch * nq * hq;
+    return up(s * rows * kHeadDim * sizeof(float)) + up(s * rows * sizeof(float4));
+}
 void place_order(QueryAttnParams& p, char* ws) {
     if (!may_order(p.Nq, p.Hq, p.Hk)) return;
     const size_t rows = (size_t)p.B * p.Hk * p.Nq;
@@ -1530,9 +1536,7 @@ size_t mosaic_query_attn_fwd_workspace_size(int32_t batch, int32_t num_queries, 
                                             int32_t block_size, int32_t block_count) {
     if (check_shape(batch, num_queries, 1, num_q_heads, num_kv_heads, kHeadDim, block_size, block_count) != MOSAIC_OK) return 0;
     if (few(batch, num_queries, num_q_heads, num_kv_heads, block_size, block_count)) return 0;
-    const int s = choose_split(batch, num_queries, num_q_heads, num_kv_heads, block_count);
-    const size_t rows = s == 1 ? 0 : (size_t)batch * num_queries * num_q_heads;
-    return up(s * rows * kHeadDim * sizeof(float)) + up(s * rows * sizeof(float4)) +
+    return part_bytes(batch, num_queries, num_q_heads, num_kv_heads, block_count) +
            order_bytes(batch, num_queries, num_q_heads, num_kv_heads);
 }
 
@@ -1563,11 +1567,9 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
     char* ws = static_cast<char*>(workspace);
     if (p.splits > 1) {
         p.part_o = reinterpret_cast<float*>(ws);
-        ws += up(p.splits * rows * kHeadDim * sizeof(float));
-        p.part_ml = reinterpret_cast<float4*>(ws);
-        ws += up(p.splits * rows * sizeof(float4));
+        p.part_ml = reinterpret_cast<float4*>(ws + up(p.splits * rows * kHeadDim * sizeof(float)));
     }
-    place_order(p, ws);
+    place_order(p, ws + part_bytes(batch, num_queries, num_q_heads, num_kv_heads, block_count));
     if (int e = launch_order(p, s)) return e;
     int total = p.qtiles * num_kv_heads * batch * p.splits;
     void* args[] = {&p, &total};
@@ -1587,15 +1589,15 @@ size_t mosaic_query_attn_bwd_workspace_size(int32_t batch, int32_t num_queries, 
 int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const void* out, const float* lse, mosaic_bnhd grad_out,
                           const int64_t* block_indices, const int32_t* kv_lens, int32_t batch, int32_t num_queries,
                           int32_t num_keys, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-                          int32_t block_count, float softmax_scale, void* grad_q, void* grad_k, void* grad_v, void* workspace,
-                          size_t workspace_bytes, void* stream) {
+                          int32_t block_count, float softmax_scale, const void* fwd_workspace, void* grad_q, void* grad_k,
+                          void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
     if (int e = check_shape(batch, num_queries, num_keys, num_q_heads, num_kv_heads, head_dim, block_size, block_count)) return e;
     for (const mosaic_bnhd* t : {&q, &k, &v, &grad_out})
         if (int e = check_rows(*t)) return e;
     if (!out || !lse || !block_indices || !grad_q || !grad_k || !grad_v) return MOSAIC_ERR_NULL_POINTER;
     for (const void* t : {out, (const void*)grad_q, (const void*)grad_k, (const void*)grad_v})
         if (!aligned(t, 16)) return MOSAIC_ERR_ALIGNMENT;
-    if (!aligned(block_indices, 8) || !aligned(lse, 4) || !aligned(kv_lens, 4)) return MOSAIC_ERR_ALIGNMENT;
+    if (!aligned(block_indices, 8) || !aligned(lse, 4) || !aligned(kv_lens, 4) || !aligned(fwd_workspace, 256)) return MOSAIC_ERR_ALIGNMENT;
     const BwdLayout at = bwd_layout(batch, num_queries, num_keys, num_q_heads, num_kv_heads, block_size, block_count);
     if (workspace == nullptr || workspace_bytes < at.bytes || !aligned(workspace, 256)) return MOSAIC_ERR_WORKSPACE;
     // token lists are indexed in 31 bits
@@ -1623,7 +1625,11 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     p.parts = reinterpret_cast<float*>(ws + at.parts);
     p.share = at.share;
     p.words = words_of(num_queries);
-    place_order(p, ws + at.order);
+    // the forward's order, where it made one
+    const bool have = fwd_workspace != nullptr && !few(batch, num_queries, num_q_heads, num_kv_heads, block_size, block_count);
+    place_order(p, have ? static_cast<char*>(const_cast<void*>(fwd_workspace)) +
+                              part_bytes(batch, num_queries, num_q_heads, num_kv_heads, block_count)
+                        : ws + at.order);
     p.out = static_cast<bf16_t*>(grad_q);
     p.dk = static_cast<bf16_t*>(grad_k);
     p.dv = static_cast<bf16_t*>(grad_v);
@@ -1631,7 +1637,8 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     int groups = p.words / kMarkWords;
     if (chunks > 65535 || (double)groups * num_kv_heads * batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (int e = launch_order(p, s)) return e;
+    if (!have)
+        if (int e = launch_order(p, s)) return e;
     int total = p.qtiles * num_kv_heads * batch;
     void* args[] = {&p, &total};
     if (launch((const void*)&query_attn_dq_kernel, dim3(total), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;

@@ -95,7 +95,7 @@ def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
 
 
 def _attn_fwd(q, k, v, idx, block_size, scale, lens, want_lse):
-    """(output bf16 [B, Nq, Hq, 64], lse fp32 [B, Nq, Hq] or None); q, k, v as (rows, their Bnhd)."""
+    """(output bf16 [B, Nq, Hq, 64], lse fp32 [B, Nq, Hq] or None, workspace or None); q, k, v as (rows, their Bnhd)."""
     (q, qb), (k, kb), (v, vb) = q, k, v
     B, Nq, Hq, d = q.shape
     Nk, Hk = k.shape[1:3]
@@ -109,18 +109,18 @@ def _attn_fwd(q, k, v, idx, block_size, scale, lens, want_lse):
         st = L.mosaic_query_attn_fwd(qb, kb, vb, idx.data_ptr(), _ptr(lens), B, Nq, Nk, Hq, Hk, d, block_size, K, scale,
                                      out.data_ptr(), _ptr(lse), _ptr(ws), nbytes, _stream(device))
     _lib.check(st, "mosaic_query_attn_fwd")
-    return out, lse
+    return out, lse, ws
 
 
 class _QueryAttn(torch.autograd.Function):
-    """Saves the bf16 rows the kernels read, the output and its log-sum-exp."""
+    """Saves the bf16 rows the kernels read, the output and its log-sum-exp, and the order of the tokens."""
 
     @staticmethod
     def forward(ctx, q, k, v, idx, block_size, scale, lens):
         ctx.dtypes = (q.dtype, k.dtype, v.dtype)
         ctx.rest = (block_size, scale)
         rows = [_as_bf16(t) for t in (q, k, v)]
-        out, lse = _attn_fwd(*rows, idx, block_size, scale, lens, True)
+        out, lse, ctx.order = _attn_fwd(*rows, idx, block_size, scale, lens, True)
         ctx.save_for_backward(*(t for t, _ in rows), out, lse, idx, lens)
         return out.to(q.dtype)
 
@@ -139,8 +139,8 @@ class _QueryAttn(torch.autograd.Function):
         ws = _scratch(nbytes, device)
         with _on(device):
             st = L.mosaic_query_attn_bwd(qb, kb, vb, out.data_ptr(), lse.data_ptr(), gb, idx.data_ptr(), _ptr(lens), B, Nq, Nk,
-                                         Hq, Hk, d, block_size, idx.shape[-1], scale, gq.data_ptr(), gk.data_ptr(),
-                                         gv.data_ptr(), ws.data_ptr(), nbytes, _stream(device))
+                                         Hq, Hk, d, block_size, idx.shape[-1], scale, _ptr(ctx.order), gq.data_ptr(),
+                                         gk.data_ptr(), gv.data_ptr(), ws.data_ptr(), nbytes, _stream(device))
         _lib.check(st, "mosaic_query_attn_bwd")
         return tuple(g.to(t) for g, t in zip((gq, gk, gv), ctx.dtypes)) + (None,) * 4
 
@@ -189,7 +189,7 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
         idx = idx.to(torch.int64).contiguous()
     if _wants_grad(q, k, v):
         return _QueryAttn.apply(q, k, v, idx, block_size, scale, kv_lens)
-    out, _ = _attn_fwd(_as_bf16(q), _as_bf16(k), _as_bf16(v), idx, block_size, scale, kv_lens, False)
+    out, _, _ = _attn_fwd(_as_bf16(q), _as_bf16(k), _as_bf16(v), idx, block_size, scale, kv_lens, False)
     return out if q.dtype is torch.bfloat16 else out.to(q.dtype)
 
 

@@ -66,7 +66,8 @@ def _call(fn, c):
         return L.mosaic_query_attn_fwd(c["q"], c["k"], c["k"], c["idx"], None, c["B"], c["nq"], c["nk"], c["hq"], c["hk"], c["d"],
                                        c["bs"], c["K"], 0.125, c["out"], c["lse"], c["ws"], c["n"], None)
     return L.mosaic_query_attn_bwd(c["q"], c["k"], c["k"], FAKE, c["lse"], c["q"], c["idx"], None, c["B"], c["nq"], c["nk"],
-                                   c["hq"], c["hk"], c["d"], c["bs"], c["K"], 0.125, c["out"], FAKE, FAKE, c["ws"], c["n"], None)
+                                   c["hq"], c["hk"], c["d"], c["bs"], c["K"], 0.125, c.get("order"), c["out"], FAKE, FAKE, c["ws"], c["n"],
+                                   None)
 
 
 @HAVE_LIB
@@ -564,3 +565,26 @@ def test_few_tokens_and_values_that_are_not_finite():
     want = oracle(q, k, v, idx, 64, lens=lens)["o"]
     k[:, 460:], v[:, 460:] = float("nan"), float("inf")
     near(M.query_sparse_attn(q, k, v, idx, 64, kv_lens=lens), want, "output")
+
+
+@HAVE_LIB
+def test_backward_refuses_a_misplaced_order():
+    c = dict(q=_lib.Bnhd(FAKE, 0, 256, 64), k=_lib.Bnhd(FAKE, 0, 128, 64), idx=FAKE, B=1, nq=7, nk=200, hq=4, hk=2, d=64, bs=64,
+             K=12, out=FAKE, lse=FAKE, ws=FAKE, n=1 << 40, order=FAKE + 16)
+    assert _call("bwd", c) == 7
+
+
+@gpu
+@pytest.mark.parametrize("Nq,K", [(60, 3), (500, 8), (4000, 20), (40, 20)])
+def test_backward_with_and_without_the_forward_s_order(Nq, K):
+    gen = torch.Generator(device=DEV).manual_seed(Nq)
+    q, k, v, go = randn(gen, 1, Nq, 4, 64), randn(gen, 1, 3000, 1, 64), randn(gen, 1, 3000, 1, 64), randn(gen, 1, Nq, 4, 64)
+    idx = choose(gen, 1, Nq, 1, 47, K, "far")
+
+    def grads(keep):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = M.query_sparse_attn(*leaves, idx, 64)
+        if not keep:
+            out.grad_fn.order = None
+        return torch.autograd.grad(out, leaves, go)
+    assert all(torch.equal(a, b) for a, b in zip(grads(True), grads(False)))
