@@ -87,7 +87,6 @@ struct QueryAttnParams {
     uint16_t* keys;            // [B, Hk, Nq] bucket of each token (null: tokens in their own order)
     int32_t* order;            // [B, Hk, Nq] tokens in the order they are taken in,
     int32_t* ordered;          // [B, Hk] where this is not 0
-    int32_t* far;              // [B, Hk, chunks of 32 tokens] of them far from the one before
     int B, Nq, Nk, Hq, Hk, G, QW, bs, K, nb, words;
     int qtiles, splits;
     int qw_inverse;            // t / QW = t qw_inverse >> 16 for t < 256
@@ -143,13 +142,30 @@ __device__ __forceinline__ int bucket_of(const QueryAttnParams& p, int blk) {
     return p.nb <= kBuckets ? blk : (int)((int64_t)blk * kBuckets / p.nb);
 }
 
-// A workgroup takes 32 tokens of one (b, h), eight lanes a token, and counts those that lie more
-// than a 32nd of the blocks from the token before.
+// Where the tokens' own order is already one of neighbours it is left as it is: of up to 64 pairs of
+// tokens that follow one another, spread over all of them, one in four at most is further apart than a
+// 32nd of the blocks, by the middle entries of their rows (pairs where that is none aside).  Every workgroup looks at the same pairs and
+// then takes 32 tokens of one (b, h), eight lanes a token.  (49152 tokens that stay: 6 us, and 10 where
+// each is read for it.)
 constexpr int kKeyTokens = kThreads / 8;
 __global__ __launch_bounds__(kThreads) void query_keys_kernel(QueryAttnParams p, int chunks) {
-    __shared__ int keys[kKeyTokens];
     const int bh = blockIdx.x / chunks, chunk = blockIdx.x - bh * chunks, h = bh % p.Hk, b = bh / p.Hk;
     const int tid = threadIdx.x, n0 = chunk * kKeyTokens, tokens = min(kKeyTokens, p.Nq - n0);
+    const int pairs = min(64, p.Nq - 1);
+    auto middle = [&](int n) {   // or, where that is no block, the first; -1: neither
+        const int64_t* e = p.idx + (((int64_t)b * p.Nq + n) * p.Hk + h) * p.K;
+        const int64_t x = e[p.K / 2], y = e[0];
+        return x >= 0 && x < p.nb ? (int)x : y >= 0 && y < p.nb ? (int)y : -1;
+    };
+    bool both = false, apart = false;
+    if (tid < pairs) {
+        const int n = (int)((int64_t)tid * (p.Nq - 1) / pairs), x = middle(n), y = middle(n + 1);
+        both = x >= 0 && y >= 0;
+        apart = both && (int64_t)abs(x - y) * 32 > p.nb;
+    }
+    const bool sort = __syncthreads_count(apart) * 4 > __syncthreads_count(both);
+    if (tid == 0 && chunk == 0) p.ordered[bh] = sort;
+    if (!sort) return;
     const int64_t* e = p.idx + (((int64_t)b * p.Nq + n0 + min(tid >> 3, tokens - 1)) * p.Hk + h) * p.K;
     auto entry = [&](int i) {   // -1: none
         const int64_t blk = e[i];
@@ -183,36 +199,21 @@ __global__ __launch_bounds__(kThreads) void query_keys_kernel(QueryAttnParams p,
         const float u = __shfl_xor(off, d);
         take(u, __shfl_xor(nearest, d));
     }
-    if ((tid & 7) == 0) keys[tid >> 3] = nearest < 0 ? kBuckets : bucket_of(p, nearest);
-    __syncthreads();
-    if (tid >= 64) return;
-    const bool jump = tid > 0 && tid < tokens && abs(keys[tid] - keys[tid - 1]) * 32 > min(p.nb, kBuckets);
-    if (tid < tokens) p.keys[(int64_t)bh * p.Nq + n0 + tid] = (uint16_t)keys[tid];
-    const uint64_t jumps = __builtin_amdgcn_ballot_w64(jump);
-    if (tid == 0) p.far[blockIdx.x] = (int)__builtin_popcountll(jumps);
+    if ((tid & 7) == 0 && tid >> 3 < tokens)
+        p.keys[(int64_t)bh * p.Nq + n0 + (tid >> 3)] = (uint16_t)(nearest < 0 ? kBuckets : bucket_of(p, nearest));
 }
 
-// One workgroup = one (b, h): a counting sort by bucket.  Where the tokens' own order is already one
-// of neighbours -- three in four lie near the token before -- it is left as it is.
+// One workgroup = one (b, h): a counting sort by bucket.
 // The order within a bucket is that of the LDS atomics; nothing depends on it.  (2 us where nothing is
 // sorted, 10 for 10007 tokens: one workgroup's LDS atomics.)
 constexpr int kOrderThreads = 1024, kOrderRun = 8;   // keys a thread has in flight
-__global__ __launch_bounds__(kOrderThreads) void query_order_kernel(QueryAttnParams p, int chunks) {
+__global__ __launch_bounds__(kOrderThreads) void query_order_kernel(QueryAttnParams p) {
+    if (p.ordered[blockIdx.x] == 0) return;
     __shared__ int start[kBuckets + 1];
     __shared__ int waves[kOrderThreads / 64];
     const int tid = threadIdx.x;
-    int far = 0;
-    for (int i = tid; i < chunks; i += kOrderThreads) far += p.far[blockIdx.x * chunks + i];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) far += __shfl_xor(far, d);
-    if ((tid & 63) == 0) waves[tid >> 6] = far;
     for (int i = tid; i <= kBuckets; i += kOrderThreads) start[i] = 0;
     __syncthreads();
-    far = 0;
-    for (int w = 0; w < kOrderThreads / 64; ++w) far += waves[w];
-    const bool sort = far > p.Nq / 4;
-    if (tid == 0) p.ordered[blockIdx.x] = sort;
-    if (!sort) return;
     const uint16_t* key = p.keys + (int64_t)blockIdx.x * p.Nq;
     int32_t* out = p.order + (int64_t)blockIdx.x * p.Nq;
     auto each = [&](auto use) {   // use(token, its key)
@@ -1439,8 +1440,7 @@ int key_chunks(int32_t nq) { return (nq + kKeyTokens - 1) / kKeyTokens; }
 size_t order_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
     if (!may_order(nq, hq, hk)) return 0;
     const size_t rows = (size_t)batch * hk * nq;
-    return up(rows * sizeof(uint16_t)) + up(rows * sizeof(int32_t)) + up((size_t)batch * hk * sizeof(int32_t)) +
-           up((size_t)batch * hk * key_chunks(nq) * sizeof(int32_t));
+    return up(rows * sizeof(uint16_t)) + up(rows * sizeof(int32_t)) + up((size_t)batch * hk * sizeof(int32_t));
 }
 // Bytes of the forward's partials, behind which its workspace holds the order.
 size_t part_bytes(int32_t batch, int32_t nq, int32_t hq, int32_t hk, int32_t K) {
@@ -1454,7 +1454,6 @@ void place_order(QueryAttnParams& p, char* ws) {
     p.keys = reinterpret_cast<uint16_t*>(ws);
     p.order = reinterpret_cast<int32_t*>(ws + up(rows * sizeof(uint16_t)));
     p.ordered = reinterpret_cast<int32_t*>(ws + up(rows * sizeof(uint16_t)) + up(rows * sizeof(int32_t)));
-    p.far = p.ordered + up((size_t)p.B * p.Hk * sizeof(int32_t)) / sizeof(int32_t);
 }
 
 void fill(QueryAttnParams& p, const mosaic_bnhd& q, const mosaic_bnhd& k, const mosaic_bnhd& v, const int64_t* idx,
