@@ -243,210 +243,210 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
     load_queries(first);
     if constexpr (WHOLE) load_keys(0);
     for (int tile = first; tile < past; ++tile) {
-    const int n0 = tile * kRows, rows = min(kRows, p.Nq - n0);
-    float* qnorm = qnorms[tile & 1];   // (waves still selecting read the last tile's)
-    {   // as hi + lo parts by way of LDS
-        float sum[kDims] = {}, tot[kDims] = {};
-        auto add = [&](uint32_t w) {
-            const float x[2] = {bf_lo(w), bf_hi(w)};
+        const int n0 = tile * kRows, rows = min(kRows, p.Nq - n0);
+        float* qnorm = qnorms[tile & 1];   // (waves still selecting read the last tile's)
+        {   // as hi + lo parts by way of LDS
+            float sum[kDims] = {}, tot[kDims] = {};
+            auto add = [&](uint32_t w) {
+                const float x[2] = {bf_lo(w), bf_hi(w)};
+#pragma unroll
+                for (int i = 0; i < kDims; ++i) {
+                    sum[i] += x[i];
+                    tot[i] += fabsf(x[i]);
+                }
+            };
+#pragma unroll
+            for (int g = 0; g < kAhead; ++g)
+                if (g < p.G) add(ahead[g]);
+            if (p.G > kAhead) {
+                const bf16_t* qb = query(tile);
+#pragma unroll 4
+                for (int g = kAhead; g < p.G; ++g) add(dims(qb + g * p.q_sh));
+            }
+            float mag = 0.f;
 #pragma unroll
             for (int i = 0; i < kDims; ++i) {
-                sum[i] += x[i];
-                tot[i] += fabsf(x[i]);
+                const float hi = round_bf16(sum[i]);
+                qpart[0][qr][qdim + i] = (bf16_t)(__float_as_uint(hi) >> 16);
+                qpart[1][qr][qdim + i] = (bf16_t)(pack_bf16x2(sum[i] - hi, 0.f) & 0xffffu);
+                mag = fmaf(tot[i], tot[i], mag);
             }
-        };
 #pragma unroll
-        for (int g = 0; g < kAhead; ++g)
-            if (g < p.G) add(ahead[g]);
-        if (p.G > kAhead) {
-            const bf16_t* qb = query(tile);
-#pragma unroll 4
-            for (int g = kAhead; g < p.G; ++g) add(dims(qb + g * p.q_sh));
-        }
-        float mag = 0.f;
-#pragma unroll
-        for (int i = 0; i < kDims; ++i) {
-            const float hi = round_bf16(sum[i]);
-            qpart[0][qr][qdim + i] = (bf16_t)(__float_as_uint(hi) >> 16);
-            qpart[1][qr][qdim + i] = (bf16_t)(pack_bf16x2(sum[i] - hi, 0.f) & 0xffffu);
-            mag = fmaf(tot[i], tot[i], mag);
-        }
-#pragma unroll
-        for (int m = 1; m < kLanes; m <<= 1) mag += __shfl_xor(mag, m);
-        if (threadIdx.x % kLanes == 0) qnorm[qr] = sqrtf(mag);
-    }
-    __syncthreads();
-    bf16x8 hi[2], lo[2];   // of column c16, dims 32 ks + 8 g4 .. + 7
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-        hi[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[0][c16][32 * ks + 8 * g4]));
-        lo[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[1][c16][32 * ks + 8 * g4]));
-    }
-    for (int u0 = 0; u0 < (WHOLE ? 1 : p.nb); u0 += kChunk) {
-        if constexpr (!WHOLE) load_keys(u0);
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-            f32x4 s = {0.f, 0.f, 0.f, 0.f};
-            s = mfma16(as_bf16x8(a[j][0]), hi[0], s);
-            s = mfma16(as_bf16x8(a[j][1]), hi[1], s);
-            if (p.G > 1) {
-                s = mfma16(as_bf16x8(a[j][0]), lo[0], s);
-                s = mfma16(as_bf16x8(a[j][1]), lo[1], s);
-            }
-            // lane: blocks 16 t + 4 g4 + e of query c16; -inf where there is none or the mask leaves it out
-            float4 v = make_float4(s[0], s[1], s[2], s[3]);
-            uint32_t bits = ons[j];
-            asm volatile("" : "+s"(bits));   // (the tests of all tiles would be held in registers otherwise)
-            if (bits != ~0u) {
-                const uint32_t four = bits >> (4 * g4);
-                v.x = (four & 1) ? v.x : -INFINITY;
-                v.y = (four & 2) ? v.y : -INFINITY;
-                v.z = (four & 4) ? v.z : -INFINITY;
-                v.w = (four & 8) ? v.w : -INFINITY;
-            }
-            *reinterpret_cast<float4*>(sc + c16 * kStride + 16 * (wave + j * NW) + 4 * g4) = v;
+            for (int m = 1; m < kLanes; m <<= 1) mag += __shfl_xor(mag, m);
+            if (threadIdx.x % kLanes == 0) qnorm[qr] = sqrtf(mag);
         }
         __syncthreads();
-        const bool last = WHOLE || u0 + kChunk >= p.nb;
-        if (last && tile + 1 < past) load_queries(tile + 1);
-        float kmax = 0.f;
+        bf16x8 hi[2], lo[2];   // of column c16, dims 32 ks + 8 g4 .. + 7
 #pragma unroll
-        for (int i = 0; i < NW; ++i) kmax = fmaxf(kmax, knorm[i]);
-        kmax = sqrtf(kmax);
-        for (int r = wave; r < rows; r += NW) {
-            // element 0: the carried best, element 1 + i: block u0 + lane + 64 i; -inf where there is none
-            float v[PL + 1];
-            v[0] = !WHOLE && u0 > 0 && lane < carry_n[r] ? carry_v[r][lane] : -INFINITY;
+        for (int ks = 0; ks < 2; ++ks) {
+            hi[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[0][c16][32 * ks + 8 * g4]));
+            lo[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(&qpart[1][c16][32 * ks + 8 * g4]));
+        }
+        for (int u0 = 0; u0 < (WHOLE ? 1 : p.nb); u0 += kChunk) {
+            if constexpr (!WHOLE) load_keys(u0);
 #pragma unroll
-            for (int i = 0; i < PL; ++i) v[1 + i] = sc[r * kStride + lane + 64 * i];
-            static_assert(PL % 2 == 0, "pairs of scores");
-            float top = larger(v[0], v[1], v[2]);
+            for (int j = 0; j < kTiles; ++j) {
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                s = mfma16(as_bf16x8(a[j][0]), hi[0], s);
+                s = mfma16(as_bf16x8(a[j][1]), hi[1], s);
+                if (p.G > 1) {
+                    s = mfma16(as_bf16x8(a[j][0]), lo[0], s);
+                    s = mfma16(as_bf16x8(a[j][1]), lo[1], s);
+                }
+                // lane: blocks 16 t + 4 g4 + e of query c16; -inf where there is none or the mask leaves it out
+                float4 v = make_float4(s[0], s[1], s[2], s[3]);
+                uint32_t bits = ons[j];
+                asm volatile("" : "+s"(bits));   // (the tests of all tiles would be held in registers otherwise)
+                if (bits != ~0u) {
+                    const uint32_t four = bits >> (4 * g4);
+                    v.x = (four & 1) ? v.x : -INFINITY;
+                    v.y = (four & 2) ? v.y : -INFINITY;
+                    v.z = (four & 4) ? v.z : -INFINITY;
+                    v.w = (four & 8) ? v.w : -INFINITY;
+                }
+                *reinterpret_cast<float4*>(sc + c16 * kStride + 16 * (wave + j * NW) + 4 * g4) = v;
+            }
+            __syncthreads();
+            const bool last = WHOLE || u0 + kChunk >= p.nb;
+            if (last && tile + 1 < past) load_queries(tile + 1);
+            float kmax = 0.f;
 #pragma unroll
-            for (int i = 3; i < PL; i += 2) top = larger(top, v[i], v[i + 1]);
-            top = larger(top, v[PL], -INFINITY);         // (where all of them are NaN)
-            float e2 = 0x1p-14f * qnorm[r] * kmax;       // 2 eps
-            if (!(e2 < INFINITY)) e2 = 0.f;
-            // Where K of the lanes' largest scores reach a value, T is no smaller.  Scores within 2 eps of
-            // it go one to a lane, ascending by block, where they are no more than 64: nearly always where
-            // K is no more than half the lanes; else the value is raised first.
-            float least = reached_by(top, p.K, max(p.K, min(p.K + 8, 32)));
-            auto all_from = [&](float t) {
+            for (int i = 0; i < NW; ++i) kmax = fmaxf(kmax, knorm[i]);
+            kmax = sqrtf(kmax);
+            for (int r = wave; r < rows; r += NW) {
+                // element 0: the carried best, element 1 + i: block u0 + lane + 64 i; -inf where there is none
+                float v[PL + 1];
+                v[0] = !WHOLE && u0 > 0 && lane < carry_n[r] ? carry_v[r][lane] : -INFINITY;
+#pragma unroll
+                for (int i = 0; i < PL; ++i) v[1 + i] = sc[r * kStride + lane + 64 * i];
+                static_assert(PL % 2 == 0, "pairs of scores");
+                float top = larger(v[0], v[1], v[2]);
+#pragma unroll
+                for (int i = 3; i < PL; i += 2) top = larger(top, v[i], v[i + 1]);
+                top = larger(top, v[PL], -INFINITY);         // (where all of them are NaN)
+                float e2 = 0x1p-14f * qnorm[r] * kmax;       // 2 eps
+                if (!(e2 < INFINITY)) e2 = 0.f;
+                // Where K of the lanes' largest scores reach a value, T is no smaller.  Scores within 2 eps of
+                // it go one to a lane, ascending by block, where they are no more than 64: nearly always where
+                // K is no more than half the lanes; else the value is raised first.
+                float least = reached_by(top, p.K, max(p.K, min(p.K + 8, 32)));
+                auto all_from = [&](float t) {
+                    int n = 0;
+#pragma unroll
+                    for (int i = WHOLE; i <= PL; ++i) n += lanes_from(v[i], t);
+                    return n;
+                };
+                if (p.K > 24 && all_from(fmaxf(least - e2, -__FLT_MAX__)) > 64) {
+                    float lo = least == -INFINITY ? wave_min(top == -INFINITY ? INFINITY : top) : least, hi = wave_max(top);
+                    for (;;) {
+                        const float mid = 0.5f * lo + 0.5f * hi;
+                        if (!(mid > lo && mid < hi)) break;
+                        const int n = all_from(mid);
+                        if (n < p.K) {
+                            hi = mid;
+                            continue;
+                        }
+                        lo = least = mid;
+                        if (n <= 64 && all_from(mid - e2) <= 64) break;
+                    }
+                }
+                const float keep = fmaxf(least - e2, -__FLT_MAX__);
+                float* scores = sc + r * kStride;                            // of the first 64, and all codes
+                uint16_t* codes = reinterpret_cast<uint16_t*>(scores + 64);   // (64 i + l: element i of lane l)
+                asm volatile("" ::: "memory");     // the row's scores are read before these take their place
+                scores[lane] = -INFINITY;
                 int n = 0;
 #pragma unroll
-                for (int i = WHOLE; i <= PL; ++i) n += lanes_from(v[i], t);
-                return n;
-            };
-            if (p.K > 24 && all_from(fmaxf(least - e2, -__FLT_MAX__)) > 64) {
-                float lo = least == -INFINITY ? wave_min(top == -INFINITY ? INFINITY : top) : least, hi = wave_max(top);
-                for (;;) {
-                    const float mid = 0.5f * lo + 0.5f * hi;
-                    if (!(mid > lo && mid < hi)) break;
-                    const int n = all_from(mid);
-                    if (n < p.K) {
-                        hi = mid;
-                        continue;
-                    }
-                    lo = least = mid;
-                    if (n <= 64 && all_from(mid - e2) <= 64) break;
-                }
-            }
-            const float keep = fmaxf(least - e2, -__FLT_MAX__);
-            float* scores = sc + r * kStride;                            // of the first 64, and all codes
-            uint16_t* codes = reinterpret_cast<uint16_t*>(scores + 64);   // (64 i + l: element i of lane l)
-            asm volatile("" ::: "memory");     // the row's scores are read before these take their place
-            scores[lane] = -INFINITY;
-            int n = 0;
-#pragma unroll
-            for (int i = WHOLE; i <= PL; ++i) {
-                const uint64_t m = __builtin_amdgcn_ballot_w64(v[i] >= keep);
-                if (m == 0) continue;
-                const int pos = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
-                n += (int)__builtin_popcountll(m);
-                if (v[i] >= keep) {
-                    codes[pos] = (uint16_t)(64 * i + lane);
-                    if (pos < 64) scores[pos] = v[i];
-                }
-            }
-            asm volatile("" ::: "memory");     // (LDS is in order within a wave)
-            auto block = [&](int code) { return !WHOLE && code < 64 ? carry_u[r][code] : u0 + code - 64; };
-            bool take;
-            float mine = -INFINITY;
-            int u = 0;
-            if (n <= 64) {
-                take = lane < n;
-                if (take) {
-                    u = block(codes[lane]);
-                    mine = scores[lane];
-                }
-                if (n > p.K) {
-                    // T is the smallest that has fewer than K above it
-                    int above = 0;
-                    for (int i = 0; i < n; i += 8) {
-                        const float4 x = *reinterpret_cast<const float4*>(scores + i), y = *reinterpret_cast<const float4*>(scores + i + 4);
-                        above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
-                        above += (y.x > mine) + (y.y > mine) + (y.z > mine) + (y.w > mine);
-                    }
-                    uint64_t at = 0;
-                    for (int i = p.K - 1; at == 0; --i) at = __builtin_amdgcn_ballot_w64(take && above == i);   // (equal ones: fewer)
-                    const float T = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), (int)__builtin_ctzll(at)));
-                    const uint64_t in = __builtin_amdgcn_ballot_w64(mine >= T - e2 && lane < n);
-                    take = in >> lane & 1;
-                    if ((int)__builtin_popcountll(in) > p.K) {
-                        // more within 2 eps of T than slots are left: exact scores decide
-                        const bool open = take && mine <= T + e2;
-                        take = take && !open;
-                        const int sure = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(take));
-                        summed_query(p, b, n0 + r, h, lane, qd[wave]);
-                        const double x = open ? exact_score(kb + (int64_t)u * p.k_sn, qd[wave]) : -INFINITY;
-                        const int rank = exact_rank(x, open, lane);
-                        take = take || (open && rank < p.K - sure);
+                for (int i = WHOLE; i <= PL; ++i) {
+                    const uint64_t m = __builtin_amdgcn_ballot_w64(v[i] >= keep);
+                    if (m == 0) continue;
+                    const int pos = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+                    n += (int)__builtin_popcountll(m);
+                    if (v[i] >= keep) {
+                        codes[pos] = (uint16_t)(64 * i + lane);
+                        if (pos < 64) scores[pos] = v[i];
                     }
                 }
-            } else {
-                // ties: every candidate's exact score is formed, 64 at a time, and the best K held, one a
-                // lane and ascending; all held ones have lower blocks than the new ones
-                summed_query(p, b, n0 + r, h, lane, qd[wave]);
-                double held = -INFINITY;
-                int held_u = 0, holds = 0;
-                for (int at = 0; at < n; at += 64) {
-                    const bool fresh = at + lane < n, old = lane < holds;
-                    const int fu = fresh ? block(codes[at + lane]) : 0;
-                    const double x = fresh ? exact_score(kb + (int64_t)fu * p.k_sn, qd[wave]) : -INFINITY;
-                    const int rank_x = exact_rank(x, fresh, lane) + exact_above(held, old, x, true);
-                    const int rank_h = exact_rank(held, old, lane) + exact_above(x, fresh, held, false);
-                    const uint64_t mh = __builtin_amdgcn_ballot_w64(old && rank_h < p.K);
-                    const uint64_t mx = __builtin_amdgcn_ballot_w64(fresh && rank_x < p.K);
-                    const int nh = (int)__builtin_popcountll(mh);
-                    const int jh = nth_bit(mh, min(lane, 63)), jx = nth_bit(mx, max(lane - nh, 0));
-                    const double h1 = __shfl(held, jh), x1 = __shfl(x, jx);
-                    const int u1 = __shfl(held_u, jh), u2 = __shfl(fu, jx);
-                    held = lane < nh ? h1 : x1;
-                    held_u = lane < nh ? u1 : u2;
-                    holds = nh + (int)__builtin_popcountll(mx);
+                asm volatile("" ::: "memory");     // (LDS is in order within a wave)
+                auto block = [&](int code) { return !WHOLE && code < 64 ? carry_u[r][code] : u0 + code - 64; };
+                bool take;
+                float mine = -INFINITY;
+                int u = 0;
+                if (n <= 64) {
+                    take = lane < n;
+                    if (take) {
+                        u = block(codes[lane]);
+                        mine = scores[lane];
+                    }
+                    if (n > p.K) {
+                        // T is the smallest that has fewer than K above it
+                        int above = 0;
+                        for (int i = 0; i < n; i += 8) {
+                            const float4 x = *reinterpret_cast<const float4*>(scores + i), y = *reinterpret_cast<const float4*>(scores + i + 4);
+                            above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+                            above += (y.x > mine) + (y.y > mine) + (y.z > mine) + (y.w > mine);
+                        }
+                        uint64_t at = 0;
+                        for (int i = p.K - 1; at == 0; --i) at = __builtin_amdgcn_ballot_w64(take && above == i);   // (equal ones: fewer)
+                        const float T = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), (int)__builtin_ctzll(at)));
+                        const uint64_t in = __builtin_amdgcn_ballot_w64(mine >= T - e2 && lane < n);
+                        take = in >> lane & 1;
+                        if ((int)__builtin_popcountll(in) > p.K) {
+                            // more within 2 eps of T than slots are left: exact scores decide
+                            const bool open = take && mine <= T + e2;
+                            take = take && !open;
+                            const int sure = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(take));
+                            summed_query(p, b, n0 + r, h, lane, qd[wave]);
+                            const double x = open ? exact_score(kb + (int64_t)u * p.k_sn, qd[wave]) : -INFINITY;
+                            const int rank = exact_rank(x, open, lane);
+                            take = take || (open && rank < p.K - sure);
+                        }
+                    }
+                } else {
+                    // ties: every candidate's exact score is formed, 64 at a time, and the best K held, one a
+                    // lane and ascending; all held ones have lower blocks than the new ones
+                    summed_query(p, b, n0 + r, h, lane, qd[wave]);
+                    double held = -INFINITY;
+                    int held_u = 0, holds = 0;
+                    for (int at = 0; at < n; at += 64) {
+                        const bool fresh = at + lane < n, old = lane < holds;
+                        const int fu = fresh ? block(codes[at + lane]) : 0;
+                        const double x = fresh ? exact_score(kb + (int64_t)fu * p.k_sn, qd[wave]) : -INFINITY;
+                        const int rank_x = exact_rank(x, fresh, lane) + exact_above(held, old, x, true);
+                        const int rank_h = exact_rank(held, old, lane) + exact_above(x, fresh, held, false);
+                        const uint64_t mh = __builtin_amdgcn_ballot_w64(old && rank_h < p.K);
+                        const uint64_t mx = __builtin_amdgcn_ballot_w64(fresh && rank_x < p.K);
+                        const int nh = (int)__builtin_popcountll(mh);
+                        const int jh = nth_bit(mh, min(lane, 63)), jx = nth_bit(mx, max(lane - nh, 0));
+                        const double h1 = __shfl(held, jh), x1 = __shfl(x, jx);
+                        const int u1 = __shfl(held_u, jh), u2 = __shfl(fu, jx);
+                        held = lane < nh ? h1 : x1;
+                        held_u = lane < nh ? u1 : u2;
+                        holds = nh + (int)__builtin_popcountll(mx);
+                    }
+                    take = lane < holds;
+                    u = held_u;
+                    mine = (float)held;
                 }
-                take = lane < holds;
-                u = held_u;
-                mine = (float)held;
-            }
-            // taken blocks, ascending by lane
-            const uint64_t m = __builtin_amdgcn_ballot_w64(take);
-            const int count = (int)__builtin_popcountll(m);
-            const int pos = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
-            asm volatile("" ::: "memory");         // the carried blocks are read before they are written
-            if (WHOLE || last) {
-                int64_t* row = p.out + (((int64_t)b * p.Nq + n0 + r) * p.Hk + h) * p.K;
-                if (take) row[pos] = u;
-                if (lane >= count && lane < p.K) row[lane] = -1;
-            } else {
-                if (take) {
-                    carry_v[r][pos] = mine;
-                    carry_u[r][pos] = u;
+                // taken blocks, ascending by lane
+                const uint64_t m = __builtin_amdgcn_ballot_w64(take);
+                const int count = (int)__builtin_popcountll(m);
+                const int pos = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+                asm volatile("" ::: "memory");         // the carried blocks are read before they are written
+                if (WHOLE || last) {
+                    int64_t* row = p.out + (((int64_t)b * p.Nq + n0 + r) * p.Hk + h) * p.K;
+                    if (take) row[pos] = u;
+                    if (lane >= count && lane < p.K) row[lane] = -1;
+                } else {
+                    if (take) {
+                        carry_v[r][pos] = mine;
+                        carry_u[r][pos] = u;
+                    }
+                    if (lane == 0) carry_n[r] = count;
                 }
-                if (lane == 0) carry_n[r] = count;
             }
+            if (!last) __syncthreads();   // the rows' scores are read before the next chunk's are written
         }
-        if (!last) __syncthreads();   // the rows' scores are read before the next chunk's are written
-    }
     }
 }
 
