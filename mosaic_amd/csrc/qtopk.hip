@@ -126,17 +126,18 @@ __device__ __forceinline__ void summed_query(const QueryTopkParams& p, int b, in
     asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ double exact_score(const bf16_t* kr, const double* qs) {
-    double s = 0.0;
+    double s[4] = {};   // (one chain of 64 sums would be waited for)
+#pragma unroll
     for (int d = 0; d < 64; d += 8) {
         const uint4 w4 = ld16(kr + d);
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            s = fma(qs[d + 2 * j], (double)bf_lo(w[j]), s);
-            s = fma(qs[d + 2 * j + 1], (double)bf_hi(w[j]), s);
+            s[j] = fma(qs[d + 2 * j], (double)bf_lo(w[j]), s[j]);
+            s[j] = fma(qs[d + 2 * j + 1], (double)bf_hi(w[j]), s[j]);
         }
     }
-    return s;
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 // How many of the lanes in `of` come before this one: a larger score, or the same and a lower lane.
 __device__ __forceinline__ int exact_rank(double x, bool of, int lane) {
@@ -360,11 +361,11 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
                 for (int i = WHOLE; i <= PL; ++i) {
                     const uint64_t m = __builtin_amdgcn_ballot_w64(v[i] >= keep);
                     if (m == 0) continue;
-                    const int pos = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+                    const int pos = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, (uint32_t)n));
                     n += (int)__builtin_popcountll(m);
                     if (v[i] >= keep) {
                         codes[pos] = (uint16_t)(64 * i + lane);
-                        if (pos < 64) scores[pos] = v[i];
+                        if (n <= 64) scores[pos] = v[i];   // (of more than 64 nobody reads them)
                     }
                 }
                 asm volatile("" ::: "memory");     // (LDS is in order within a wave)
