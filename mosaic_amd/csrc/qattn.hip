@@ -1141,6 +1141,11 @@ struct KeysLds {
     int list[kListed];
 };
 
+//
+// FINE: P and dS in two bf16 parts each, 16 bits, so that grad k and grad v are off by their own
+// rounding alone (1.7e-3 in the 2-norm; with one part 2.3e-3, and 3.0e-3 for two tokens, whose terms
+// may cancel).  Half as many products again (165 us for 120 above): for calls that are short anyway.
+template <bool FINE>
 __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnParams p, int tiles, int total) {
     __shared__ KeysLds L;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
@@ -1287,12 +1292,16 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
 #pragma unroll
                 for (int ch = 0; ch < 2; ++ch) gT[dt][ch] = tr_read(Gc, 32 * qh + 16 * ch, dt);
             __builtin_amdgcn_sched_barrier(0);
-            bf16x8 pb[2], db[2];
+            bf16x8 pb[2], db[2], pl[2], dl[2];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float pr = __builtin_amdgcn_exp2f(s[e] * p.c), ds = pr * dp[e];
                 pb[e >> 3][e & 7] = (__bf16)pr;
                 db[e >> 3][e & 7] = (__bf16)ds;
+                if constexpr (FINE) {
+                    pl[e >> 3][e & 7] = (__bf16)(pr - (float)pb[e >> 3][e & 7]);
+                    dl[e >> 3][e & 7] = (__bf16)(ds - (float)db[e >> 3][e & 7]);
+                }
             }
 #pragma unroll
             for (int dt = 0; dt < 2; ++dt)
@@ -1301,11 +1310,17 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dkv_kernel(QueryAttnPa
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
-                for (int dt = 0; dt < 2; ++dt) dvT[dt] = mfma32(gT[dt][ch], pb[ch], dvT[dt]);
+                for (int dt = 0; dt < 2; ++dt) {
+                    dvT[dt] = mfma32(gT[dt][ch], pb[ch], dvT[dt]);
+                    if constexpr (FINE) dvT[dt] = mfma32(gT[dt][ch], pl[ch], dvT[dt]);
+                }
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
-                for (int dt = 0; dt < 2; ++dt) dkT[dt] = mfma32(qT[dt][ch], db[ch], dkT[dt]);
+                for (int dt = 0; dt < 2; ++dt) {
+                    dkT[dt] = mfma32(qT[dt][ch], db[ch], dkT[dt]);
+                    if constexpr (FINE) dkT[dt] = mfma32(qT[dt][ch], dl[ch], dkT[dt]);
+                }
         };
         const int32_t* takers = p.takers + p.starts[block];
         const int run = kListed / QS * QS;   // tokens listed at a time
@@ -1650,7 +1665,10 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
     void* targs[] = {&p};
     if (launch((const void*)&query_takers_kernel, dim3((unsigned)(p.nb * num_kv_heads * batch)), targs, s) != hipSuccess)
         return MOSAIC_ERR_LAUNCH;
-    if (launch((const void*)&query_attn_dkv_kernel, dim3((unsigned)at.items), kargs, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    // rows of the steps in all; up to 2048 steps (four for each workgroup that is resident) take a few us either way
+    const bool fine = (double)at.pairs * (block_size / 64) * p.G <= 2048.0 * 64;
+    const void* dkv = fine ? (const void*)&query_attn_dkv_kernel<true> : (const void*)&query_attn_dkv_kernel<false>;
+    if (launch(dkv, dim3((unsigned)at.items), kargs, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     return launch((const void*)&query_sum_kernel, dim3(key_tiles), kargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
 

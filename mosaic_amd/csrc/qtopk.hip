@@ -23,7 +23,7 @@
 // 64 go one to a lane, where each lane counts the larger ones.
 //
 // Bound by the selection's vector instructions and its waits for one another: 49152 tokens with 3 kv
-// heads of 4 query heads and 768 blocks (nside 64), 14.5 Gflop of scores and 94 MB, take 136 us, 49 of
+// heads of 4 query heads and 768 blocks (nside 64), 14.5 Gflop of scores and 94 MB, take 135 us, 49 of
 // them for the scores.  The keys of a chunk stay in registers for as many row tiles as fill the chip
 // once and the next tile's queries are loaded during a selection: with one row tile per workgroup,
 // keys from L2 for each, the scores alone took 133 us, all of it 196.  Exact bisections in both places

@@ -588,3 +588,19 @@ def test_backward_with_and_without_the_forward_s_order(Nq, K):
             out.grad_fn.order = None
         return torch.autograd.grad(out, leaves, go)
     assert all(torch.equal(a, b) for a, b in zip(grads(True), grads(False)))
+
+
+@gpu
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hk,bs,K", [(1, 2, 700, 8, 4, 64, 7), (2, 5, 3000, 20, 5, 128, 9), (1, 300, 2000, 2, 1, 64, 6)])
+def test_gradients_of_few_tokens_keep_their_precision(B, Nq, Nk, Hq, Hk, bs, K):
+    """P and dS in two parts are off by 2^-16 and the delta by fp32 sums: what remains beside the
+    gradients' own rounding is the exponent's error, a fifth of the terms' part of the bound at most."""
+    gen = torch.Generator(device=DEV).manual_seed(Nk)
+    q, k, v, go = randn(gen, B, Nq, Hq, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nq, Hq, 64)
+    idx = choose(gen, B, Nq, Hk, -(-Nk // bs), K, "far")
+    want = oracle(q, k, v, idx, bs, go=go)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    _, dk, dv = torch.autograd.grad(M.query_sparse_attn(*leaves, idx, bs), leaves, go)
+    for name, got in (("dk", dk), ("dv", dv)):
+        value, bound = want[name]
+        near(got, (value, H * value.abs() + (bound - H * value.abs()) / 4), name)
