@@ -13,7 +13,9 @@
 // With T the K-th largest computed score, a block above T + 2 eps is certainly taken and one below
 // T - 2 eps certainly not (the K-th largest is off by at most eps too).  Where more blocks lie
 // between than slots are left -- about 1 row in 50 on fields, every row on constant keys -- their
-// scores are formed again in fp64, one block per lane, and compared there.
+// scores are formed again in fp64, one block per lane, and compared there.  Where |Q| or |k| is not
+// within 2^-50 .. 2^60 (infinite keys and rows of zeros among them), squares, products or scores may leave
+// fp32 and eps bounds nothing: all of the row's blocks are then compared in fp64.  A NaN is never taken.
 //
 // One workgroup = row tiles of 16 query tokens of one kv head.  Its waves form a tile's scores
 // S^T = K Q^T of up to 64 PL blocks with v_mfma_f32_16x16x32_bf16 into LDS (16 rows of fp32), then
@@ -110,6 +112,9 @@ __device__ __forceinline__ float larger(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
     return y;
 }
+
+// A norm that eps bounds errors by, or infinity for any other (see above; a NaN is another)
+__device__ __forceinline__ float bounding(float x) { return x >= 0x1p-50f && x <= 0x1p60f ? x : INFINITY; }
 
 // Lane of the n-th set bit of m (anything past the last)
 __device__ __forceinline__ int nth_bit(uint64_t m, int n) {
@@ -274,7 +279,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             }
 #pragma unroll
             for (int m = 1; m < kLanes; m <<= 1) mag += __shfl_xor(mag, m);
-            if (threadIdx.x % kLanes == 0) qnorm[qr] = sqrtf(mag);
+            if (threadIdx.x % kLanes == 0) qnorm[qr] = bounding(sqrtf(mag));
         }
         __syncthreads();
         bf16x8 hi[2], lo[2];   // of column c16, dims 32 ks + 8 g4 .. + 7
@@ -313,8 +318,56 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             float kmax = 0.f;
 #pragma unroll
             for (int i = 0; i < NW; ++i) kmax = fmaxf(kmax, knorm[i]);
-            kmax = sqrtf(kmax);
+            kmax = bounding(sqrtf(kmax));
+            // row r's blocks, ascending by lane
+            auto store = [&](int r, bool take, int u, float mine) {
+                const uint64_t m = __builtin_amdgcn_ballot_w64(take);
+                const int count = (int)__builtin_popcountll(m);
+                const int pos = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+                asm volatile("" ::: "memory");         // the carried blocks are read before they are written
+                if (WHOLE || last) {
+                    int64_t* row = p.out + (((int64_t)b * p.Nq + n0 + r) * p.Hk + h) * p.K;
+                    if (take && pos < p.K) row[pos] = u;
+                    if (lane >= count && lane < p.K) row[lane] = -1;
+                } else {
+                    if (take) {
+                        carry_v[r][pos] = mine;
+                        carry_u[r][pos] = u;
+                    }
+                    if (lane == 0) carry_n[r] = count;
+                }
+            };
+            // A row's best K by exact scores, one a lane and ascending: hold(there, u) adds the lanes' blocks that
+            // are there, all of them above the held ones.  A NaN is not held.
+            double held;
+            int held_u, holds;
+            auto hold_none = [&](int r) {
+                summed_query(p, b, n0 + r, h, lane, qd[wave]);
+                held = -INFINITY;
+                held_u = holds = 0;
+            };
+            auto hold = [&](bool there, int fu) {
+                const double x = there ? exact_score(kb + (int64_t)fu * p.k_sn, qd[wave]) : -INFINITY;
+                const bool fresh = there && x == x, old = lane < holds;
+                const int rank_x = exact_rank(x, fresh, lane) + exact_above(held, old, x, true);
+                const int rank_h = exact_rank(held, old, lane) + exact_above(x, fresh, held, false);
+                const uint64_t mh = __builtin_amdgcn_ballot_w64(old && rank_h < p.K);
+                const uint64_t mx = __builtin_amdgcn_ballot_w64(fresh && rank_x < p.K);
+                const int nh = (int)__builtin_popcountll(mh);
+                const int jh = nth_bit(mh, min(lane, 63)), jx = nth_bit(mx, max(lane - nh, 0));
+                const double h1 = __shfl(held, jh), x1 = __shfl(x, jx);
+                const int u1 = __shfl(held_u, jh), u2 = __shfl(fu, jx);
+                held = lane < nh ? h1 : x1;
+                held_u = lane < nh ? u1 : u2;
+                holds = nh + (int)__builtin_popcountll(mx);
+            };
+            uint32_t open_rows = 0;   // those without a bound
             for (int r = wave; r < rows; r += NW) {
+                const float e2 = 0x1p-14f * qnorm[r] * kmax;   // 2 eps
+                if (__builtin_amdgcn_ballot_w64(e2 < INFINITY) == 0) {
+                    open_rows |= 1u << r;
+                    continue;
+                }
                 // element 0: the carried best, element 1 + i: block u0 + lane + 64 i; -inf where there is none
                 float v[PL + 1];
                 v[0] = !WHOLE && u0 > 0 && lane < carry_n[r] ? carry_v[r][lane] : -INFINITY;
@@ -325,8 +378,6 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
 #pragma unroll
                 for (int i = 3; i < PL; i += 2) top = larger(top, v[i], v[i + 1]);
                 top = larger(top, v[PL], -INFINITY);         // (where all of them are NaN)
-                float e2 = 0x1p-14f * qnorm[r] * kmax;       // 2 eps
-                if (!(e2 < INFINITY)) e2 = 0.f;
                 // Where K of the lanes' largest scores reach a value, T is no smaller.  Scores within 2 eps of
                 // it go one to a lane, ascending by block, where they are no more than 64: nearly always where
                 // K is no more than half the lanes; else the value is raised first.
@@ -404,47 +455,22 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
                         }
                     }
                 } else {
-                    // ties: every candidate's exact score is formed, 64 at a time, and the best K held, one a
-                    // lane and ascending; all held ones have lower blocks than the new ones
-                    summed_query(p, b, n0 + r, h, lane, qd[wave]);
-                    double held = -INFINITY;
-                    int held_u = 0, holds = 0;
-                    for (int at = 0; at < n; at += 64) {
-                        const bool fresh = at + lane < n, old = lane < holds;
-                        const int fu = fresh ? block(codes[at + lane]) : 0;
-                        const double x = fresh ? exact_score(kb + (int64_t)fu * p.k_sn, qd[wave]) : -INFINITY;
-                        const int rank_x = exact_rank(x, fresh, lane) + exact_above(held, old, x, true);
-                        const int rank_h = exact_rank(held, old, lane) + exact_above(x, fresh, held, false);
-                        const uint64_t mh = __builtin_amdgcn_ballot_w64(old && rank_h < p.K);
-                        const uint64_t mx = __builtin_amdgcn_ballot_w64(fresh && rank_x < p.K);
-                        const int nh = (int)__builtin_popcountll(mh);
-                        const int jh = nth_bit(mh, min(lane, 63)), jx = nth_bit(mx, max(lane - nh, 0));
-                        const double h1 = __shfl(held, jh), x1 = __shfl(x, jx);
-                        const int u1 = __shfl(held_u, jh), u2 = __shfl(fu, jx);
-                        held = lane < nh ? h1 : x1;
-                        held_u = lane < nh ? u1 : u2;
-                        holds = nh + (int)__builtin_popcountll(mx);
-                    }
+                    // ties: all candidates, 64 at a time
+                    hold_none(r);
+                    for (int at = 0; at < n; at += 64) hold(at + lane < n, at + lane < n ? block(codes[at + lane]) : 0);
                     take = lane < holds;
                     u = held_u;
                     mine = (float)held;
                 }
-                // taken blocks, ascending by lane
-                const uint64_t m = __builtin_amdgcn_ballot_w64(take);
-                const int count = (int)__builtin_popcountll(m);
-                const int pos = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
-                asm volatile("" ::: "memory");         // the carried blocks are read before they are written
-                if (WHOLE || last) {
-                    int64_t* row = p.out + (((int64_t)b * p.Nq + n0 + r) * p.Hk + h) * p.K;
-                    if (take) row[pos] = u;
-                    if (lane >= count && lane < p.K) row[lane] = -1;
-                } else {
-                    if (take) {
-                        carry_v[r][pos] = mine;
-                        carry_u[r][pos] = u;
-                    }
-                    if (lane == 0) carry_n[r] = count;
-                }
+                store(r, take, u, mine);
+            }
+            for (; open_rows != 0; open_rows &= open_rows - 1) {   // all blocks
+                const int r = (int)__builtin_ctz(open_rows);
+                hold_none(r);
+                if (!WHOLE && u0 > 0) hold(lane < carry_n[r], lane < carry_n[r] ? carry_u[r][lane] : 0);
+                for (int u = u0; u < min(u0 + kChunk, p.nb); u += 64)
+                    hold(u + lane < p.nb && (mask == nullptr || mask[u + lane]), min(u + lane, p.nb - 1));
+                store(r, lane < holds, held_u, (float)held);
             }
             if (!last) __syncthreads();   // the rows' scores are read before the next chunk's are written
         }

@@ -63,9 +63,10 @@ def query_topk(q: torch.Tensor, k_cmp: torch.Tensor, block_count: int, block_mas
 
     q [B, Nq, Hq, 64] against pooled keys ``k_cmp`` [B, nb, Hk, 64] (``pool_mean``, say): the score of
     a block is the sum over the kv head's query heads of their dot products with it, and the largest
-    exact scores are taken, ties to the lower block.  Blocks come in ascending order; slots past the
-    last are -1, where ``block_mask`` (bool [B, nb], False: never taken) leaves fewer than
-    ``block_count``.  ``block_count`` is at most 64.  No gradient passes through the choice.
+    exact scores are taken, whatever their magnitude, ties to the lower block; one that is NaN is not.
+    Blocks come in ascending order; slots past the last are -1, where ``block_mask`` (bool [B, nb],
+    False: never taken) and NaN leave fewer than ``block_count``.  ``block_count`` is at most 64.  No
+    gradient passes through the choice.
     """
     what = "query_topk"
     _bf16_heads(what, q=q, k_cmp=k_cmp)

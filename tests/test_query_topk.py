@@ -182,3 +182,56 @@ def test_several_row_tiles_a_workgroup(B, Nq, nb, Hq, Hk, K, masked):
     q, kc = randn(gen, B, Nq, Hq, 64), randn(gen, B, nb, Hk, 64)
     mask = torch.rand(B, nb, generator=gen, device=DEV) < 0.5 if masked else None
     assert torch.equal(M.query_topk(q, kc, K, mask), oracle(q, kc, K, mask))
+
+
+def choice(q, kc, K, mask=None):
+    """The oracle where scores may lie anywhere: the first K of the unmasked blocks by their scores in
+    float64, a NaN never; products one by one, so that an infinity meets no other row's."""
+    B, Nq, Hq, _ = q.shape
+    nb, Hk = kc.shape[1:3]
+    qs, k = q.cpu().double().view(B, Nq, Hk, Hq // Hk, 64).sum(3), kc.cpu().double()
+    s = torch.stack([(qs[:, n, None] * k).sum(-1).transpose(1, 2) for n in range(Nq)], 1)       # [B, Nq, Hk, nb]
+    ok = ~s.isnan() if mask is None else ~s.isnan() & mask.cpu()[:, None, None, :]
+    # (those that may not be taken behind the -inf of those that may)
+    order = torch.where(s.isnan(), 0.0, s).sort(dim=-1, descending=True, stable=True).indices
+    order = order.gather(-1, (~ok.gather(-1, order)).to(torch.int8).sort(dim=-1, stable=True).indices)[..., :K]
+    order = torch.where(ok.gather(-1, order), order, nb).sort(-1).values
+    return torch.where(order == nb, -1, order).to(q.device)
+
+
+@gpu
+@pytest.mark.parametrize("nb,K", [(60, 9), (700, 16), (700, 40), (1200, 16)])
+@pytest.mark.parametrize("scale_q,scale_k", [(70, 0), (0, 70), (70, 70), (120, -100), (-80, 0), (0, -80), (-70, -70), (-126, 0)])
+def test_scores_whose_norms_leave_fp32(nb, K, scale_q, scale_k):
+    # keys that are one key but for a small part in a dimension of theirs: scores of hundreds that are
+    # closer than fp32 holds them, times powers of two, which change no order
+    print(f"scales 2^{scale_q} 2^{scale_k} nb {nb} K {K}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    q = randn(gen, 1, 33, 4, 64)
+    kc = randn(gen, 1, 1, 1, 64).float().mul(64).expand(1, nb, 1, 64).clone()
+    kc[..., 40:] = 0
+    at = torch.randint(40, 64, (nb,), generator=gen, device=DEV)
+    kc[0, torch.arange(nb, device=DEV), 0, at] = torch.randn(nb, generator=gen, device=DEV) * 2.0 ** -12
+    kc = kc.to(BF16)
+    q, kc = (q.double() * 2.0 ** scale_q).to(BF16), (kc.double() * 2.0 ** scale_k).to(BF16)
+    assert torch.equal(M.query_topk(q, kc, K), choice(q, kc, K))
+    mask = torch.rand(1, nb, generator=gen, device=DEV) < 0.5
+    assert torch.equal(M.query_topk(q, kc, K, mask), choice(q, kc, K, mask))
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hk,nb,K", [(2, 2, 40, 1), (2, 2, 40, 40), (8, 2, 300, 16), (3, 1, 300, 33), (4, 1, 1200, 16), (2, 2, 1200, 64)])
+def test_keys_and_queries_that_are_not_finite(Hq, Hk, nb, K):
+    print(f"not finite {Hq}/{Hk} nb {nb} K {K}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(nb + K)
+    q, kc = randn(gen, 2, 20, Hq, 64), randn(gen, 2, nb, Hk, 64)
+    inf = float("inf")
+    kc[0, nb // 2, 0, 5], kc[0, nb - 1, 0, 6], kc[0, 3, 0, 7] = inf, -inf, float("nan")
+    kc[1, 7] = -inf                       # every product of a sign of its own: NaN, or where q is one-signed an infinity
+    q[1, 11] = q[1, 11].abs()
+    q[:, 4] = 0                           # scores of zero, and NaN beside the infinities
+    q[:, 9, :, 3] = inf
+    q[:, 13, :, 20] = float("nan")
+    assert torch.equal(M.query_topk(q, kc, K), choice(q, kc, K))
+    mask = torch.rand(2, nb, generator=gen, device=DEV) < 0.6
+    assert torch.equal(M.query_topk(q, kc, K, mask), choice(q, kc, K, mask))
