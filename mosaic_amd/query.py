@@ -155,7 +155,7 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
     be short).  It is a set: an index counts once however often it stands there, and one outside the
     blocks (such as -1) not at all.  ``kv_lens`` (integers [B]): keys from ``kv_lens[b]`` on are not
     attended; what they hold does not matter.  A token without a key gets zeros.  ``softmax_scale``
-    defaults to 1/8.  Differentiable in q, k and v, once.
+    defaults to 1/8.  Differentiable in q, k and v, once, in reverse mode.
     """
     what = "query_sparse_attn"
     _bf16_heads(what, q=q, k=k, v=v)

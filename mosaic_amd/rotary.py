@@ -9,7 +9,7 @@
 
 q is [B, N, Hq, d] and k [B, N, Hk, d] (or None), both bfloat16 or both float32, d 32, 64 or 128,
 any strides with contiguous rows; outputs are new contiguous tensors of q's type.  Both ops are
-differentiable once: in q, k and the weights, not in positions or tables.  They enqueue on the
+differentiable once, in reverse mode: in q, k and the weights, not in positions or tables.  They enqueue on the
 current stream of q's device and never synchronise the host.
 """
 
@@ -21,6 +21,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -173,6 +174,10 @@ def _rotation(cos, sin, positions, axes, interleaved: bool) -> _lib.Rotation | N
 
 
 def _wants_grad(*tensors) -> bool:
+    """Whether autograd is to see the call: a tensor requires grad, or a forward-mode level is open, where
+    the function refuses inputs that carry a tangent (it has none for its output)."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
