@@ -506,8 +506,8 @@ MOSAIC_API int mosaic_query_topk_fwd(mosaic_bnhd q, mosaic_bnhd k_cmp, const uin
    of 64 (the last block may be short), at most 16 query heads per kv head, K at most 1024.
    workspace: mosaic_query_attn_fwd_workspace_size() bytes (partials of few queries, the order of
    many; 0 where there is neither), 256-byte aligned.
-   softmax_scale <= 0 selects 64^-0.5.  mosaic_sparse_attn (ops.py:557-566) is the counterpart for
-   query blocks. */
+   softmax_scale <= 0 selects 64^-0.5; others lie within 1e-30 .. 1e30.  mosaic_sparse_attn
+   (ops.py:557-566) is the counterpart for query blocks. */
 MOSAIC_API size_t mosaic_query_attn_fwd_workspace_size(int32_t batch, int32_t num_queries, int32_t num_q_heads,
                                                        int32_t num_kv_heads, int32_t block_size, int32_t block_count);
 MOSAIC_API int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int64_t* block_indices,

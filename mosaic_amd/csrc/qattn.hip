@@ -1435,6 +1435,9 @@ int check_shape(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t hk, i
     return MOSAIC_OK;
 }
 
+// fp32 carries the scale and its reciprocal, times the logarithms that the backward divides by it.
+bool scale_ok(float scale) { return scale <= 0.f || (scale >= 1e-30f && scale <= 1e30f); }
+
 // Workgroups where the union is in one piece.
 int64_t groups_of(int32_t batch, int32_t nq, int32_t hq, int32_t hk) {
     const int64_t per = kWaves * (kRows / (hq / hk));
@@ -1564,6 +1567,7 @@ int mosaic_query_attn_fwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const int
                           int32_t head_dim, int32_t block_size, int32_t block_count, float softmax_scale, void* out, float* lse,
                           void* workspace, size_t workspace_bytes, void* stream) {
     if (int e = check_shape(batch, num_queries, num_keys, num_q_heads, num_kv_heads, head_dim, block_size, block_count)) return e;
+    if (!scale_ok(softmax_scale)) return MOSAIC_ERR_UNSUPPORTED;
     for (const mosaic_bnhd* t : {&q, &k, &v})
         if (int e = check_rows(*t)) return e;
     if (block_indices == nullptr || out == nullptr) return MOSAIC_ERR_NULL_POINTER;
@@ -1611,6 +1615,7 @@ int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v, const voi
                           int32_t block_count, float softmax_scale, const void* fwd_workspace, void* grad_q, void* grad_k,
                           void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
     if (int e = check_shape(batch, num_queries, num_keys, num_q_heads, num_kv_heads, head_dim, block_size, block_count)) return e;
+    if (!scale_ok(softmax_scale)) return MOSAIC_ERR_UNSUPPORTED;
     for (const mosaic_bnhd* t : {&q, &k, &v, &grad_out})
         if (int e = check_rows(*t)) return e;
     if (!out || !lse || !block_indices || !grad_q || !grad_k || !grad_v) return MOSAIC_ERR_NULL_POINTER;

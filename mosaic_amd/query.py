@@ -18,8 +18,6 @@ synchronise the host.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib
@@ -56,6 +54,14 @@ def _groups(what: str, q: torch.Tensor, k: torch.Tensor) -> None:
 def _as_bf16(t: torch.Tensor):
     """bf16 rows as the kernels read them: (tensor, its pointer and strides)."""
     return _rows(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16))
+
+
+def _scale(what: str, softmax_scale) -> float:
+    """The scale as fp32 carries it and its reciprocal, with the logarithms the backward divides by it."""
+    scale = 0.125 if softmax_scale is None else float(softmax_scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"{what}: softmax_scale must be within 1e-30 .. 1e30, got {softmax_scale}")
+    return scale
 
 
 def query_topk(q: torch.Tensor, k_cmp: torch.Tensor, block_count: int, block_mask: torch.Tensor | None = None) -> torch.Tensor:
@@ -155,7 +161,7 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
     be short).  It is a set: an index counts once however often it stands there, and one outside the
     blocks (such as -1) not at all.  ``kv_lens`` (integers [B]): keys from ``kv_lens[b]`` on are not
     attended; what they hold does not matter.  A token without a key gets zeros.  ``softmax_scale``
-    defaults to 1/8.  Differentiable in q, k and v, once, in reverse mode.
+    defaults to 1/8 and lies within 1e-30 .. 1e30.  Differentiable in q, k and v, once, in reverse mode.
     """
     what = "query_sparse_attn"
     _bf16_heads(what, q=q, k=k, v=v)
@@ -170,9 +176,7 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
                          "K at most 1024")
     if block_indices.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{what}: block_indices are {block_indices.dtype}, not int64 or int32")
-    scale = 0.125 if softmax_scale is None else float(softmax_scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"{what}: softmax_scale must be positive, got {softmax_scale}")
+    scale = _scale(what, softmax_scale)
     if kv_lens is not None:
         if tuple(kv_lens.shape) != (B,):
             raise ValueError(f"{what}: kv_lens {tuple(kv_lens.shape)} must be [B] = ({B},)")
@@ -210,6 +214,7 @@ def mosaic_query_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_s
     if block_size <= 0 or block_size % 64 or k.shape[1] % block_size:
         raise ValueError(f"{what}: block_size must be a multiple of 64 that divides {k.shape[1]} keys, got {block_size}")
     nb = k.shape[1] // block_size
+    softmax_scale = _scale(what, softmax_scale)
     if k_cmp is None:
         _same_device(what, q, k=k)
         with torch.no_grad():

@@ -604,3 +604,38 @@ def test_gradients_of_few_tokens_keep_their_precision(B, Nq, Nk, Hq, Hk, bs, K):
     for name, got in (("dk", dk), ("dv", dv)):
         value, bound = want[name]
         near(got, (value, H * value.abs() + (bound - H * value.abs()) / 4), name)
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-31, 1e31, 1e39, float("inf"), float("nan"), -1.0])
+def test_scales_that_fp32_does_not_carry_are_refused(scale):
+    with pytest.raises(ValueError, match="softmax_scale"):
+        M.query_sparse_attn(z(*Q), z(*KV), z(*KV), IDX, 64, softmax_scale=scale)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        M.mosaic_query_attn(z(*Q), z(1, 128, 2, 64), z(1, 128, 2, 64), 64, 2, softmax_scale=scale)
+
+
+@HAVE_LIB
+@pytest.mark.parametrize("scale", [1e-44, 1e-31, 1e31, float("inf"), float("nan")])
+def test_abi_refuses_scales(scale):
+    L, row = _lib.lib(), _lib.Bnhd(FAKE, 0, 256, 64)
+    kv = _lib.Bnhd(FAKE, 0, 128, 64)
+    assert L.mosaic_query_attn_fwd(row, kv, kv, FAKE, None, 1, 7, 500, 4, 2, 64, 64, 3, scale, FAKE, FAKE, FAKE, 1 << 30, None) == 11
+    assert L.mosaic_query_attn_bwd(row, kv, kv, FAKE, FAKE, row, FAKE, None, 1, 7, 500, 4, 2, 64, 64, 3, scale, None, FAKE, FAKE,
+                                   FAKE, FAKE, 1 << 30, None) == 11
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1e-30, 1e-6])
+def test_scales_near_nothing(scale):
+    # every key weighs the same: the output and grad v are those of the mean
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    q, k, v, go = randn(gen, 1, 9, 2, 64), randn(gen, 1, 300, 1, 64), randn(gen, 1, 300, 1, 64), randn(gen, 1, 9, 2, 64)
+    idx = choose(gen, 1, 9, 1, 5, 3, "far")
+    want = oracle(q, k, v, idx, 64, scale=scale, go=go)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = M.query_sparse_attn(*leaves, idx, 64, softmax_scale=scale)
+    grads = torch.autograd.grad(out, leaves, go)
+    near(out.detach(), want["o"], "output")
+    near(grads[2], want["dv"], "grad v")
+    for g, name in zip(grads, ("dq", "dk")):
+        near(g.double() / scale, tuple(t / scale for t in want[name]), name)
