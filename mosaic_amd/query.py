@@ -47,6 +47,8 @@ def _groups(what: str, q: torch.Tensor, k: torch.Tensor) -> None:
     (B, _, Hq, _), (Bk, _, Hk, _) = q.shape, k.shape
     if B != Bk:
         raise ValueError(f"{what}: q {tuple(q.shape)} and keys {tuple(k.shape)} disagree on the batch")
+    if max(B, q.shape[1], k.shape[1]) >= 1 << 31:   # (views of few elements may be that long)
+        raise ValueError(f"{what}: the batch, queries and keys must each be below 2^31, got {tuple(q.shape)}, {tuple(k.shape)}")
     if Hk == 0 or Hq == 0 or Hq % Hk or Hq // Hk > 16:
         raise ValueError(f"{what}: {Hq} query heads must be a multiple of {Hk} kv heads, at most 16 times as many")
 
@@ -54,6 +56,12 @@ def _groups(what: str, q: torch.Tensor, k: torch.Tensor) -> None:
 def _as_bf16(t: torch.Tensor):
     """bf16 rows as the kernels read them: (tensor, its pointer and strides)."""
     return _rows(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16))
+
+
+def _block_size(what: str, block_size) -> int:
+    if not 0 < block_size < 1 << 31 or block_size % 64:
+        raise ValueError(f"{what}: block_size must be a positive multiple of 64 below 2^31, got {block_size}")
+    return int(block_size)
 
 
 def _scale(what: str, softmax_scale) -> float:
@@ -169,8 +177,7 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
     if k.shape != v.shape:
         raise ValueError(f"{what}: k and v shapes differ: {tuple(k.shape)} vs {tuple(v.shape)}")
     B, Nq, Hk = q.shape[0], q.shape[1], k.shape[2]
-    if block_size <= 0 or block_size % 64:
-        raise ValueError(f"{what}: block_size must be a positive multiple of 64, got {block_size}")
+    block_size = _block_size(what, block_size)
     if block_indices.dim() != 4 or tuple(block_indices.shape[:3]) != (B, Nq, Hk) or block_indices.shape[3] > 1024:
         raise ValueError(f"{what}: block_indices {tuple(block_indices.shape)} must be [B, Nq, Hk, K] = {(B, Nq, Hk, '*')}, "
                          "K at most 1024")
@@ -185,7 +192,6 @@ def query_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_i
     _same_device(what, q, k=k, v=v, block_indices=block_indices, kv_lens=kv_lens)
     if kv_lens is not None:   # clamped before the conversion: a far length stays one
         kv_lens = (kv_lens if kv_lens.dtype == torch.int32 else kv_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
-    block_size = int(block_size)
     if q.numel() == 0 or k.numel() == 0 or block_indices.numel() == 0:   # no row, or no key for any
         # (a product with nothing, so that gradients of the inputs are zeros)
         return torch.zeros(q.shape, dtype=q.dtype, device=q.device) + 0 * (q[:0].sum() + k[:0].sum() + v[:0].sum()).to(q.dtype)
@@ -211,7 +217,8 @@ def mosaic_query_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_s
     """
     what = "mosaic_query_attn"
     _bf16_heads(what, q=q, k=k, v=v)
-    if block_size <= 0 or block_size % 64 or k.shape[1] % block_size:
+    block_size = _block_size(what, block_size)
+    if k.shape[1] % block_size:
         raise ValueError(f"{what}: block_size must be a multiple of 64 that divides {k.shape[1]} keys, got {block_size}")
     nb = k.shape[1] // block_size
     softmax_scale = _scale(what, softmax_scale)

@@ -46,8 +46,8 @@ def _heads(what: str, q: torch.Tensor, k: torch.Tensor | None) -> None:
     if d not in (32, 64, 128):
         raise ValueError(f"{what}: head_dim must be 32, 64 or 128, got {d}")
     Bk, Nk, Hk, dk = (B, N, 1, d) if k is None else k.shape
-    if H == 0 or Hk == 0:
-        raise ValueError(f"{what}: q and k need a head")
+    if H == 0 or Hk == 0 or max(H, Hk) > 65535:
+        raise ValueError(f"{what}: q and k need a head, and take 65535 at most")
     if Bk != B or Nk != N or dk != d or (k is not None and k.dtype != q.dtype):
         raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} disagree")
     if B * N >= 1 << 31:
@@ -320,8 +320,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     if k is None and k_weight is not None:
         raise ValueError(f"{what}: k_weight without k")
     eps = torch.finfo(torch.float32).eps if eps is None else float(eps)
-    if not 0 <= eps < math.inf:
-        raise ValueError(f"{what}: eps must not be negative, got {eps}")
+    if not 0 <= eps <= torch.finfo(torch.float32).max:
+        raise ValueError(f"{what}: eps must not be negative or beyond fp32, got {eps}")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and tuple(w.shape) != (q.shape[3],):
             raise ValueError(f"{what}: {name} {tuple(w.shape)} must be [d] = ({q.shape[3]},)")

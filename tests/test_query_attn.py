@@ -639,3 +639,17 @@ def test_scales_near_nothing(scale):
     near(grads[2], want["dv"], "grad v")
     for g, name in zip(grads, ("dq", "dk")):
         near(g.double() / scale, tuple(t / scale for t in want[name]), name)
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda: M.query_sparse_attn(z(*Q), z(*KV), z(*KV), IDX, (1 << 32) + 64), "block_size"),
+    (lambda: M.query_sparse_attn(z(*Q), z(*KV), z(*KV), IDX, 1 << 31), "block_size"),
+    (lambda: M.mosaic_query_attn(z(*Q), z(1, 0, 2, 64), z(1, 0, 2, 64), (1 << 32) + 64, 2), "block_size"),
+    (lambda: M.query_sparse_attn(z(*Q), *[z(1, 1, 2, 64).expand(1, (1 << 32) + 64, 2, 64)] * 2, IDX, 64), "2\\^31"),
+    (lambda: M.query_sparse_attn(z(1, 1, 4, 64).expand(1, 1 << 31, 4, 64), z(*KV), z(*KV), IDX, 64), "2\\^31"),
+    (lambda: M.query_topk(z(*Q), z(1, 1, 2, 64).expand(1, (1 << 32) + 64, 2, 64), 2), "2\\^31"),
+    (lambda: M.query_topk(z(1, 1, 1, 64).expand((1 << 32) + 1, 1, 1, 64), z(1, 2, 1, 64).expand((1 << 32) + 1, 2, 1, 64), 2), "2\\^31"),
+])
+def test_sizes_that_32_bits_do_not_carry_are_refused(call, match):
+    with pytest.raises(ValueError, match=match):
+        call()

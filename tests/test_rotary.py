@@ -452,3 +452,9 @@ def test_theta_is_read_at_each_call_and_weights_lie_anywhere():
     for at in (1, 2, 3):                    # slices of a larger parameter
         got, _ = M.qk_norm_rope(q, None, w[at:at + 64], positions=pos, sections=(32,))
         assert torch.equal(got, M.qk_norm_rope(q, None, w[at:at + 64].clone(), positions=pos, sections=(32,))[0])
+
+
+@pytest.mark.parametrize("eps", [1e39, float("inf"), float("nan")])
+def test_eps_beyond_fp32_is_refused(eps):
+    with pytest.raises(ValueError, match="eps"):
+        M.qk_norm_rope(heads(1, 3, 2, 64), None, eps=eps)
