@@ -1504,7 +1504,12 @@ hipError_t launch(const void* fn, dim3 grid, void** args, hipStream_t s, int thr
 
 // Workspace of the backward, and the tokens of one share of a key tile: three quarters of what a block
 // has on average (grad k / v and the sums at 12288 tokens of nside 32: 133 us, with half as many again
-// 139), fewer where the tiles alone do not fill the chip twice.
+// 139), fewer where the tiles alone do not fill the chip twice.  Where there are many tiles only those that would
+// outlast the others are split: a share is a kShares-th of the call at least (a quarter of what a resident
+// workgroup does), so the partials stay below 2 kShares tiles, 128 MiB, however large the call.  (A training
+// step of four members of nside 64, 16 blocks of 64: 4.14-4.20 ms and 240 MiB, in shares of three quarters of a
+// mean 4.23-4.30 ms and 880 MiB; one of nside 128 4.5 ms either way, 402 MiB for 1042.)
+constexpr int64_t kShares = 2048;
 struct BwdLayout {
     size_t nlse, ndelta, marks, counts, starts, takers, plan, slots, parts, order, bytes;
     int64_t items;   // workgroups of grad k / v at most
@@ -1518,6 +1523,7 @@ BwdLayout bwd_layout(int32_t batch, int32_t nq, int32_t nk, int32_t hq, int32_t 
     const int64_t pairs = chosen * hk * batch * (bs / 64);                 // (token, key tile)
     int64_t share = chosen / nb * 3 / 4;
     if (tiles < 512 && share > pairs / 512) share = pairs / 512;
+    if (share < pairs / kShares) share = pairs / kShares;
     if (share < 64) share = 64;
     if (share < (nq + 4095) / 4096) share = (nq + 4095) / 4096;            // a tile's shares are counted in 16 bits
     a.share = (int)(share < 0x7fffffff ? share : 0x7fffffff);

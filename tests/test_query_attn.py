@@ -653,3 +653,34 @@ def test_scales_near_nothing(scale):
 def test_sizes_that_32_bits_do_not_carry_are_refused(call, match):
     with pytest.raises(ValueError, match=match):
         call()
+
+
+@HAVE_LIB
+def test_partials_do_not_grow_with_the_call():
+    # what a large call keeps in proportion to its tokens, blocks and bits; the partials beside it stay below 160 MiB
+    for B, Nq, Nk, Hq, Hk, bs, K in [(24, 196608, 196608, 12, 3, 64, 16), (4, 49152, 49152, 12, 3, 64, 16), (1, 1000, 1 << 22, 8, 8, 64, 2),
+                                     (1, 12288, 12288, 16, 4, 64, 12), (8, 100000, 512, 4, 4, 256, 2)]:
+        nb, tiles = -(-Nk // bs), -(-Nk // 64) * Hk * B
+        chosen = Nq * min(K, nb) * Hk * B
+        rest = 8 * B * Nq * Hq + B * Hk * nb * (Nq + 511) // 512 * 64 + 8 * B * Hk * nb + 4 * chosen + 12 * tiles + 8 * chosen // 64 + 6 * B * Hk * Nq
+        got = _lib.lib().mosaic_query_attn_bwd_workspace_size(B, Nq, Nk, Hq, Hk, bs, K)
+        assert 0 < got <= rest + (160 << 20), (B, Nq, Nk, got / 2 ** 20, rest / 2 ** 20)
+
+
+@gpu
+def test_many_key_tiles_with_wanted_blocks():
+    # 4096 key tiles, so that only blocks that most tokens want are divided
+    gen = torch.Generator(device=DEV).manual_seed(33)
+    B, Nq, Nk, Hk, K = 16, 500, 2048, 8, 8
+    q, k, v, go = randn(gen, B, Nq, Hk, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nk, Hk, 64), randn(gen, B, Nq, Hk, 64)
+    idx = choose(gen, B, Nq, Hk, Nk // 64, K, "far")
+    idx[:, :, 0, 1] = 5
+    idx[3, 20:, 2, 2:] = -1
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = M.query_sparse_attn(*leaves, idx, 64)
+    grads = torch.autograd.grad(out, leaves, go)
+    for b in range(0, B, 5):                     # (a sequence at a time: the oracle's scores are dense)
+        want = oracle(q[b:b + 1], k[b:b + 1], v[b:b + 1], idx[b:b + 1], 64, go=go[b:b + 1])
+        near(out.detach()[b:b + 1], want["o"], "output")
+        for g, name in zip(grads, ("dq", "dk", "dv")):
+            near(g[b:b + 1], want[name], name)
