@@ -396,6 +396,20 @@ class RoPE(nn.Module):
         return out.to(x.dtype)
 
 
+_NORM_FORWARD = fused.RMSNorm.forward
+
+
+def _plain_norm(norm: nn.Module) -> bool:
+    """Whether calling ``norm`` is ``fused.RMSNorm`` with its weight and nothing else sees or replaces it: no
+    other class, parameter type or hook, and no ``forward`` assigned to the module or its class."""
+    own = norm.__dict__
+    return (type(norm) is fused.RMSNorm and "forward" not in own and "_call_impl" not in own and norm._compiled_call_impl is None
+            and type(own["_parameters"].get("weight")) in (nn.Parameter, type(None))
+            and fused.RMSNorm.forward is _NORM_FORWARD
+            and not (own["_forward_hooks"] or own["_forward_pre_hooks"] or own["_backward_hooks"] or own["_backward_pre_hooks"])
+            and not nn.modules.module._has_any_global_hook())
+
+
 class MosaicAttention(nn.Module):
     """The op's caller (primitives.py:138-209): projections, gates, RoPE, block-sparse attention.
 
@@ -405,7 +419,8 @@ class MosaicAttention(nn.Module):
     ``config.head_norm`` (absent: False, the reference's module) adds an RMS norm of every query
     and key head before their rotation, ``q_norm`` and ``k_norm``, each with one weight of head_dim
     where ``rmsnorm_elementwise_affine`` (absent: True): logits stay bounded by the weights however
-    the projections grow.  Norm and rotation are then one pass over q and k (``qk_norm_rope``).
+    the projections grow.  Norm and rotation are then one pass over q and k (``qk_norm_rope``), unless
+    the norms are more than that (a hook, another module in their place, two epsilons): they are called.
     """
 
     def __init__(self, config, block_attn_only: bool, no_compression: bool = False):
@@ -522,6 +537,11 @@ class MosaicAttention(nn.Module):
             return False
         return self.q_rope is None or self._shared_rope_tables()
 
+    def _fused_head_norm(self):
+        """Whether the norms are what qk_norm_rope computes."""
+        return (self.head_norm and _plain_norm(self.q_norm) and _plain_norm(self.k_norm)
+                and self.q_norm.eps == self.k_norm.eps)
+
     def _norm_and_rotate(self, q, k):
         """q and k normalised per head and rotated: one pass over both, or one over each where the
         two RoPE modules hold different tables."""
@@ -570,7 +590,10 @@ class MosaicAttention(nn.Module):
         o = torch.empty(S_, B_, self.q_heads * q.shape[-1], dtype=torch.bfloat16, device=x.device)
         o_view = o.view(S_, B_, self.q_heads, -1).transpose(0, 1)
         record = self.record_block_indices is not None
-        if self.head_norm:
+        fused_norm = self._fused_head_norm()
+        if self.head_norm and not fused_norm:
+            q, k = self.q_norm(q), self.k_norm(k)
+        if fused_norm:
             q, k = self._norm_and_rotate(q, k)
             res = mosaic_attn_func(q=q, k=k, v=v, weight_ba_cmp_slc=w, **args, out=o_view,
                                    return_block_indices=record)

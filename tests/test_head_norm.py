@@ -161,3 +161,82 @@ def test_unet_runs_with_head_norm():
     with torch.no_grad(), torch.autocast(DEV, dtype=torch.bfloat16):
         out = model(x, dyt, 2)
     assert out.shape == (1, 2, 24, 13, 2) and torch.isfinite(out.float()).all()
+
+
+def _module(**kw):
+    torch.manual_seed(7)
+    m = MosaicAttention(attention_config(head_norm=True, **kw), block_attn_only=False)
+    with torch.no_grad():
+        m.q_norm.weight.uniform_(0.5, 2.0)
+        m.k_norm.weight.uniform_(0.5, 2.0)
+    pos = torch.rand(512, 2, generator=torch.Generator().manual_seed(8)) * 3
+    m.q_rope.initialize_rope(pos)
+    m.k_rope.initialize_rope(pos)
+    return m
+
+
+class _Twice(torch.nn.Module):
+    """A norm of the user's own."""
+
+    def __init__(self, norm):
+        super().__init__()
+        self.norm = norm
+
+    def forward(self, x):
+        return 2 * self.norm(x)
+
+
+CHANGES = {
+    "hook": lambda m: m.q_norm.register_forward_hook(lambda mod, args, out: 2 * out),
+    "pre-hook": lambda m: m.k_norm.register_forward_pre_hook(lambda mod, args: (args[0] * 0,)),
+    "forward": lambda m: setattr(m.q_norm, "forward", lambda x: 2 * type(m.q_norm).forward(m.q_norm, x)),
+    "module": lambda m: setattr(m, "k_norm", _Twice(m.k_norm)),
+    "identity": lambda m: setattr(m, "q_norm", torch.nn.Identity()),
+    "epsilon": lambda m: setattr(m.k_norm, "eps", 3.0),
+}
+
+
+@pytest.mark.parametrize("change", CHANGES)
+def test_norms_that_are_not_plain_are_called(change):
+    m = _module()
+    assert m._fused_head_norm()
+    CHANGES[change](m)
+    assert not m._fused_head_norm()
+
+
+def test_global_hooks_see_the_norms():
+    m, seen = _module(), []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda mod, args, out: seen.append(mod))
+    try:
+        assert not m._fused_head_norm()
+    finally:
+        handle.remove()
+    assert m._fused_head_norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change", [None, *CHANGES])
+def test_norms_that_are_called_against_composition(change):
+    """As the composition above, each norm's output rounded to bfloat16 before its rotation: four roundings
+    of q and k where one was, 2^-9 each on scores that every block takes part in; bar 2^-7."""
+    print(f"head_norm change={change}", flush=True)
+    S, B = 512, 2
+    m = _module().to(DEV)
+    x = torch.randn(S, B, 256, generator=torch.Generator().manual_seed(2)).to(DEV, torch.bfloat16)
+    with torch.no_grad(), torch.autocast(DEV, dtype=torch.bfloat16):
+        before = m(x)
+        if change is not None:
+            CHANGES[change](m)
+        got = m(x)
+        q, k, v, logits = m._projections(x)
+        q, k, v = (t.unflatten(-1, (-1, 64)).transpose(0, 1) for t in (q, k, v))
+        w = torch.softmax(logits.unflatten(-1, (4, 3)).permute(3, 1, 0, 2).float(), 0).to(x.dtype).unsqueeze(-1)
+        q, k = (turned(norm(t).double(), r.cos_freqs, r.sin_freqs).to(torch.bfloat16)
+                for t, norm, r in ((q, m.q_norm, m.q_rope), (k, m.k_norm, m.k_rope)))
+        o = mosaic_attn_func(q, k, v, w, block_attn_size=128, sparse_block_size=64, sparse_block_count=8,
+                             block_attn_only=False, no_compression=False)
+        ref = m.to_o(o.transpose(0, 1).flatten(-2))
+    err = ((got.double() - ref.double()).norm() / ref.double().norm()).item()
+    assert err < 2 ** -7, err
+    if change is not None:
+        assert ((got.double() - before.double()).norm() / before.double().norm()).item() > 2 ** -5
