@@ -116,7 +116,8 @@ def _merge_configs(config: ModelConfig, stage_cfg) -> _MergedStageConfig:
         sparse_block_size=stage_cfg.sparse_block_size, sparse_block_count=stage_cfg.sparse_block_count,
         gqa_ratio=stage_cfg.gqa_ratio, qkv_compress_ratio=config.qkv_compress_ratio, rope=config.rope,
         rope_theta=config.rope_theta, mlp_ratio=stage_cfg.mlp_ratio, noise_dim=config.noise_dim,
-        rmsnorm_elementwise_affine=config.rmsnorm_elementwise_affine, head_norm=config.head_norm)
+        rmsnorm_elementwise_affine=config.rmsnorm_elementwise_affine,
+        head_norm=getattr(config, "head_norm", False))      # (config objects of the reference's fields have none)
 
 
 def era5_config(num_variables: int = 82, num_static: int = 3) -> ModelConfig:

@@ -423,6 +423,8 @@ class MosaicAttention(nn.Module):
     the norms are more than that (a hook, another module in their place, two epsilons): they are called.
     """
 
+    head_norm = False       # of modules pickled without it
+
     def __init__(self, config, block_attn_only: bool, no_compression: bool = False):
         super().__init__()
         self.block_attn_only = block_attn_only

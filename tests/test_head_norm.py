@@ -240,3 +240,16 @@ def test_norms_that_are_called_against_composition(change):
     assert err < 2 ** -7, err
     if change is not None:
         assert ((got.double() - before.double()).norm() / before.double().norm()).item() > 2 ** -5
+
+
+def test_configs_and_modules_from_before_the_flag():
+    config = vars(model_config())
+    del config["head_norm"]
+    model = Transformer(types.SimpleNamespace(**config))
+    assert not any(m.head_norm for m in model.modules() if isinstance(m, MosaicAttention))
+    assert list(model.state_dict()) == list(Transformer(model_config()).state_dict())
+    old = MosaicAttention(attention_config(), block_attn_only=False)     # as a pickled module has it
+    old.__dict__.pop("head_norm", None)
+    old.fused_input_side = True
+    assert not old.head_norm and not old._fused_head_norm()
+    assert not old._fused_input_side(torch.zeros(512, 1, 256, dtype=torch.bfloat16))
