@@ -684,3 +684,35 @@ def test_many_key_tiles_with_wanted_blocks():
         near(out.detach()[b:b + 1], want["o"], "output")
         for g, name in zip(grads, ("dq", "dk", "dv")):
             near(g[b:b + 1], want[name], name)
+
+
+@gpu
+@pytest.mark.parametrize("Nq,Nk,Hq,Hk,K", [(6, 128, 2, 1, 2), (40, 700, 4, 2, 5), (300, 500, 4, 1, 3)])
+def test_gradients_along_themselves_against_differences(Nq, Nk, Hq, Hk, K):
+    """The derivative along a gradient is its norm, in which nothing cancels: a gradient twice as large, or
+    with a part left out, is far outside.  What rounding may do to it is the sum of the elements' bounds
+    along that direction (the output's l sums the rounded P, its log-sum-exp, which the backward reads, the
+    unrounded ones); the difference quotient in float64 is off by step^4, below 1e-6 of it."""
+    gen = torch.Generator(device=DEV).manual_seed(Nq)
+    q, k, v, go = (randn(gen, 1, n, h, 64) for n, h in ((Nq, Hq), (Nk, Hk), (Nk, Hk), (Nq, Hq)))
+    idx = choose(gen, 1, Nq, Hk, -(-Nk // 64), K, "far")
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(M.query_sparse_attn(*leaves, idx, 64), leaves, go)
+    bounds = oracle(q, k, v, idx, 64, go=go)
+    member = torch.zeros(1, Nq, Hk, -(-Nk // 64), dtype=torch.bool, device=DEV).scatter_(-1, idx, True)
+    ok = member.repeat_interleave(64, -1)[..., :Nk].permute(0, 2, 1, 3).repeat_interleave(Hq // Hk, 1)
+
+    def f(i, x):
+        qh, kh, vh = (t.double().permute(0, 2, 1, 3) for t in (x if j == i else t for j, t in enumerate((q, k, v))))
+        kh, vh = kh.repeat_interleave(Hq // Hk, 1), vh.repeat_interleave(Hq // Hk, 1)
+        s = (qh @ kh.transpose(-1, -2).contiguous() / 8).masked_fill(~ok, -torch.inf)
+        return ((torch.softmax(s, -1) @ vh).permute(0, 2, 1, 3) * go.double()).sum()
+
+    for i, (g, x, name) in enumerate(zip(grads, (q, k, v), ("dq", "dk", "dv"))):
+        size = g.double().norm()
+        e, step = g.double() / size, 2.0 ** -5
+        at = [f(i, x.double() + s * step * e) for s in (1, -1, 0.5, -0.5)]
+        diff = (8 * (at[2] - at[3]) - (at[0] - at[1])) / (6 * step)
+        slack = (bounds[name][1] * e.abs()).sum() + 1e-6 * size
+        assert slack < diff / 2, (name, (slack / size).item())     # a gradient of twice or half the size is off by diff / 2 or more
+        assert abs(size - diff) <= slack, (name, ((size - diff) / size).item(), (slack / size).item())
