@@ -113,8 +113,12 @@ __device__ __forceinline__ float larger(float a, float b, float c) {
     return y;
 }
 
-// A norm that eps bounds errors by, or infinity for any other (see above; a NaN is another)
-__device__ __forceinline__ float bounding(float x) { return x >= 0x1p-50f && x <= 0x1p60f ? x : INFINITY; }
+// A norm, from its square, that eps bounds errors by, or infinity for any other (see above; a NaN is another).
+// (The instruction's root is off by one step at most, which eps has room for: the terms above are 1.4 2^-16.)
+__device__ __forceinline__ float norm_bound(float square) {
+    const float x = __builtin_amdgcn_sqrtf(square);
+    return x >= 0x1p-50f && x <= 0x1p60f ? x : INFINITY;
+}
 
 // Lane of the n-th set bit of m (anything past the last)
 __device__ __forceinline__ int nth_bit(uint64_t m, int n) {
@@ -144,12 +148,19 @@ __device__ __forceinline__ double exact_score(const bf16_t* kr, const double* qs
     }
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
+// x of lane j, the same j in all lanes
+__device__ __forceinline__ double lane_value(double x, int j) {
+    const uint2 w = __builtin_bit_cast(uint2, x);
+    const uint2 y = make_uint2(__builtin_amdgcn_readlane(w.x, j), __builtin_amdgcn_readlane(w.y, j));
+    return __builtin_bit_cast(double, y);
+}
+
 // How many of the lanes in `of` come before this one: a larger score, or the same and a lower lane.
 __device__ __forceinline__ int exact_rank(double x, bool of, int lane) {
     int rank = 0;
     for (uint64_t m = __builtin_amdgcn_ballot_w64(of); m != 0; m &= m - 1) {
         const int j = (int)__builtin_ctzll(m);
-        const double y = __shfl(x, j);
+        const double y = lane_value(x, j);
         rank += y > x || (y == x && j < lane);
     }
     return rank;
@@ -159,13 +170,14 @@ __device__ __forceinline__ int exact_rank(double x, bool of, int lane) {
 __device__ __forceinline__ int exact_above(double x, bool of, double y, bool ties) {
     int n = 0;
     for (uint64_t m = __builtin_amdgcn_ballot_w64(of); m != 0; m &= m - 1) {
-        const double z = __shfl(x, (int)__builtin_ctzll(m));
+        const double z = lane_value(x, (int)__builtin_ctzll(m));
         n += z > y || (ties && z == y);
     }
     return n;
 }
 
-// PL = 12 at most: two workgroups of 8 waves then share a CU's LDS and fill its 4 waves per SIMD.
+// PL = 12 at most: two workgroups of 8 waves fill a CU at 4 waves per SIMD, whose 128 registers hold no
+// longer chunk (the whole one of 8 waves spills four, 20 bytes of scratch a lane; LDS would allow 16).
 // WHOLE: nb <= 64 PL, one chunk, whose keys stay in registers for all of a workgroup's tiles.
 template <int PL, int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams p) {
@@ -192,7 +204,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
     static_assert(kTiles * NW == 4 * PL, "the waves share a chunk's tiles evenly");
     uint4 a[kTiles][2];
     uint32_t ons[kTiles];   // the flag of block c of a tile is bit c
-    float kn = 0.f;         // largest squared norm of this lane's dims over the blocks it has loaded
+    float kn = -1.f;        // largest squared norm of this lane's dims over the blocks it has loaded (-1: none)
     auto load_keys = [&](int u0) {
         bool on[kTiles];
 #pragma unroll
@@ -218,7 +230,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
         }
         // |k|^2 <= the sum over the four dim groups of their largest
         float m = kn;
-        int key = __float_as_int(m);   // (of no negative ones: in order as they are)
+        int key = __float_as_int(m);   // (of one negative value: in order as they are)
         key = dpp_either<true, 0xb1>(key);
         key = dpp_either<true, 0x4e>(key);
         key = dpp_either<true, 0x141>(key);
@@ -279,7 +291,7 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             }
 #pragma unroll
             for (int m = 1; m < kLanes; m <<= 1) mag += __shfl_xor(mag, m);
-            if (threadIdx.x % kLanes == 0) qnorm[qr] = bounding(sqrtf(mag));
+            if (threadIdx.x % kLanes == 0) qnorm[qr] = norm_bound(mag);
         }
         __syncthreads();
         bf16x8 hi[2], lo[2];   // of column c16, dims 32 ks + 8 g4 .. + 7
@@ -315,10 +327,10 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             __syncthreads();
             const bool last = WHOLE || u0 + kChunk >= p.nb;
             if (last && tile + 1 < past) load_queries(tile + 1);
-            float kmax = 0.f;
+            float kmax = knorm[0];
 #pragma unroll
-            for (int i = 0; i < NW; ++i) kmax = fmaxf(kmax, knorm[i]);
-            kmax = bounding(sqrtf(kmax));
+            for (int i = 1; i < NW; ++i) kmax = fmaxf(kmax, knorm[i]);
+            kmax = kmax < 0.f ? 1.f : norm_bound(kmax);   // (no block yet, and so no score)
             // row r's blocks, ascending by lane
             auto store = [&](int r, bool take, int u, float mine) {
                 const uint64_t m = __builtin_amdgcn_ballot_w64(take);
@@ -339,27 +351,32 @@ __global__ __launch_bounds__(NW * 64, 4) void query_topk_kernel(QueryTopkParams 
             };
             // A row's best K by exact scores, one a lane and ascending: hold(there, u) adds the lanes' blocks that
             // are there, all of them above the held ones.  A NaN is not held.
-            double held;
+            double held, lowest;   // (lowest: of K held ones, which a further one has to exceed)
             int held_u, holds;
             auto hold_none = [&](int r) {
                 summed_query(p, b, n0 + r, h, lane, qd[wave]);
-                held = -INFINITY;
+                held = lowest = -INFINITY;
                 held_u = holds = 0;
             };
             auto hold = [&](bool there, int fu) {
                 const double x = there ? exact_score(kb + (int64_t)fu * p.k_sn, qd[wave]) : -INFINITY;
-                const bool fresh = there && x == x, old = lane < holds;
+                const bool fresh = there && x == x && (holds < p.K || x > lowest), old = lane < holds;
+                if (__builtin_amdgcn_ballot_w64(fresh) == 0) return;
                 const int rank_x = exact_rank(x, fresh, lane) + exact_above(held, old, x, true);
                 const int rank_h = exact_rank(held, old, lane) + exact_above(x, fresh, held, false);
                 const uint64_t mh = __builtin_amdgcn_ballot_w64(old && rank_h < p.K);
                 const uint64_t mx = __builtin_amdgcn_ballot_w64(fresh && rank_x < p.K);
                 const int nh = (int)__builtin_popcountll(mh);
                 const int jh = nth_bit(mh, min(lane, 63)), jx = nth_bit(mx, max(lane - nh, 0));
-                const double h1 = __shfl(held, jh), x1 = __shfl(x, jx);
+                const double before = held, h1 = __shfl(held, jh), x1 = __shfl(x, jx);
                 const int u1 = __shfl(held_u, jh), u2 = __shfl(fu, jx);
                 held = lane < nh ? h1 : x1;
                 held_u = lane < nh ? u1 : u2;
                 holds = nh + (int)__builtin_popcountll(mx);
+                if (holds == p.K) {
+                    const uint64_t lx = __builtin_amdgcn_ballot_w64(fresh && rank_x == p.K - 1), lh = __builtin_amdgcn_ballot_w64(old && rank_h == p.K - 1);
+                    lowest = lx != 0 ? lane_value(x, (int)__builtin_ctzll(lx)) : lane_value(before, (int)__builtin_ctzll(lh));
+                }
             };
             uint32_t open_rows = 0;   // those without a bound
             for (int r = wave; r < rows; r += NW) {
