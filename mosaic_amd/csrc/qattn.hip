@@ -142,11 +142,10 @@ __device__ __forceinline__ int bucket_of(const QueryAttnParams& p, int blk) {
     return p.nb <= kBuckets ? blk : (int)((int64_t)blk * kBuckets / p.nb);
 }
 
-// Where the tokens' own order is already one of neighbours it is left as it is: of up to 64 pairs of
-// tokens that follow one another, spread over all of them, one in four at most is further apart than a
-// 32nd of the blocks, by the middle entries of their rows (pairs where that is none aside).  Every workgroup looks at the same pairs and
-// then takes 32 tokens of one (b, h), eight lanes a token.  (49152 tokens that stay: 6 us, and 10 where
-// each is read for it.)
+// Where the tokens' own order is already one of neighbours it is left as it is.  It is one if, of up to 64
+// pairs of tokens that follow one another and have entries, at most a quarter have middle entries further apart than a 32nd
+// of the blocks.  Every workgroup looks at the same pairs, then takes 32 tokens of one (b, h), eight lanes a
+// token.  (49152 tokens that stay: 6 us, and 10 where each is read for it.)
 constexpr int kKeyTokens = kThreads / 8;
 __global__ __launch_bounds__(kThreads) void query_keys_kernel(QueryAttnParams p, int chunks) {
     const int bh = blockIdx.x / chunks, chunk = blockIdx.x - bh * chunks, h = bh % p.Hk, b = bh / p.Hk;
@@ -205,7 +204,8 @@ __global__ __launch_bounds__(kThreads) void query_keys_kernel(QueryAttnParams p,
 
 // One workgroup = one (b, h): a counting sort by bucket.
 // The order within a bucket is that of the LDS atomics; nothing depends on it.  (2 us where nothing is
-// sorted, 10 for 10007 tokens: one workgroup's LDS atomics.)
+// sorted; one workgroup's LDS atomics, and so linear in the tokens: 10 us for 10007, 37 for 49152, 130 for
+// 196608, beside 89, 288 and 994 of the attention.)
 constexpr int kOrderThreads = 1024, kOrderRun = 8;   // keys a thread has in flight
 __global__ __launch_bounds__(kOrderThreads) void query_order_kernel(QueryAttnParams p) {
     if (p.ordered[blockIdx.x] == 0) return;
@@ -449,13 +449,12 @@ __device__ __forceinline__ float operand_sum(const bf16x8& x, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u.w), ones, acc, false);
 }
 
-// Row r of a wave: token (position in the wave), query head,
-// and its place in [B, Nq, Hq]
+// Row r of a wave: token (position in the wave), query head, and its place in [B, Nq, Hq]
 struct Row {
     int token, head;
     bool live;
     int64_t n, at;
-        // tokens(i): the token at position n0 + i of the order
+    // tokens(i): the token at position n0 + i of the order
     template <typename Tokens>
     __device__ __forceinline__ void init(const QueryAttnParams& p, const Tokens& tokens, int b, int h, int n0, int wave, int r) {
         token = r / p.G;
@@ -845,8 +844,8 @@ __global__ __launch_bounds__(kFewThreads) void query_attn_few_kernel(QueryAttnPa
 // tile on operands at hand; without it grad q at 12288 tokens of nside 32 (12 blocks of 64) is
 // 5.1e-3 off (2-norm), with it 2.4e-3 (the output's own rounding alone: 1.7e-3).
 //
-// Bound as the forward, at two waves a SIMD (256 registers): 115 us for 12288 tokens of 12 blocks, 16
-// query and 4 kv heads: 77 Gflop, 0.67 Pflop/s.
+// Bound as the forward, at two waves a SIMD (256 registers, nine more spilled, 40 bytes of scratch a lane):
+// 116-121 us for 12288 tokens of 12 blocks, 16 query and 4 kv heads: 77 Gflop, 0.65 Pflop/s.
 struct DqState {
     f32x16 dq[2], kbar[2];   // sum dS' k, sum P k [dim tile]
     float sum, rest;         // this lane's parts of sum dS' and of sum P (do.v - delta)
@@ -980,7 +979,8 @@ __global__ __launch_bounds__(kThreads, 2) void query_attn_dq_kernel(QueryAttnPar
 // The tokens of each block, as bits: a workgroup takes 512 tokens (16 words) of one kv head and up
 // to kUnion blocks, marks in LDS and writes every word, so they need no clearing; the blocks' numbers
 // of tokens are added up beside them (integers: their order does not matter).  7 us for 12288 tokens of
-// 12 blocks in 4 heads (one entry at a time: 12).
+// 12 blocks in 4 heads (one entry at a time: 12).  A bit for every token and block: B Hk nb Nq / 8 bytes,
+// 226 MB for one member of nside 128 with blocks of 64 and 3 kv heads, 16 times that at nside 256.
 constexpr int kMarkTokens = 512, kMarkWords = kMarkTokens / 32;
 __global__ __launch_bounds__(kThreads) void query_marks_kernel(QueryAttnParams p, int groups) {
     __shared__ __attribute__((aligned(16))) uint32_t bits[kUnion * kMarkWords];
@@ -1146,7 +1146,6 @@ struct KeysLds {
     int list[kListed];
 };
 
-//
 // FINE: P and dS in two bf16 parts each, 16 bits, so that grad k and grad v are off by their own
 // rounding alone (1.7e-3 in the 2-norm; with one part 2.3e-3, and 3.0e-3 for two tokens, whose terms
 // may cancel).  Half as many products again (165 us for 120 above): for calls that are short anyway.

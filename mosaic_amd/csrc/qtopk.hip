@@ -15,7 +15,8 @@
 // between than slots are left -- about 1 row in 50 on fields, every row on constant keys -- their
 // scores are formed again in fp64, one block per lane, and compared there.  Where |Q| or |k| is not
 // within 2^-50 .. 2^60 (infinite keys and rows of zeros among them), squares, products or scores may leave
-// fp32 and eps bounds nothing: all of the row's blocks are then compared in fp64.  A NaN is never taken.
+// fp32 and eps bounds nothing: all of the row's blocks are then compared in fp64 (every row so: 1.9 ms for the
+// call below with zeros, 4.7 with an infinite key a head).  A NaN is never taken.
 //
 // One workgroup = row tiles of 16 query tokens of one kv head.  Its waves form a tile's scores
 // S^T = K Q^T of up to 64 PL blocks with v_mfma_f32_16x16x32_bf16 into LDS (16 rows of fp32), then
@@ -24,9 +25,11 @@
 // below, so the scores from there on hold all K; there are seldom more than a few of them, and up to
 // 64 go one to a lane, where each lane counts the larger ones.
 //
-// Bound by the selection's vector instructions and its waits for one another: 49152 tokens with 3 kv
-// heads of 4 query heads and 768 blocks (nside 64), 14.5 Gflop of scores and 94 MB, take 135 us, 49 of
-// them for the scores.  The keys of a chunk stay in registers for as many row tiles as fill the chip
+// Bound by the selection's waits: 49152 tokens with 3 kv heads of 4 query heads and 768 blocks (nside 64),
+// 14.5 Gflop of scores and 94 MB, take 123-127 us (134 in a trace, 49 of them for the scores); a wave waits
+// for 53 % of its cycles, the vector ALU is active for 37 % and the matrix pipe busy for 7.  K costs a step
+// with 64 (one call: 161 us with K 16, 256 with 48, 269 with 56, 965 with 64): a threshold of 64 lane
+// maxima leaves more than 64 candidates.  The keys of a chunk stay in registers for as many row tiles as fill the chip
 // once and the next tile's queries are loaded during a selection: with one row tile per workgroup,
 // keys from L2 for each, the scores alone took 133 us, all of it 196.  Exact bisections in both places
 // were 213 us, and bisection over all PL registers, the first form of this kernel, 432.
