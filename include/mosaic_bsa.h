@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define MOSAIC_BSA_ABI_VERSION 12
+#define MOSAIC_BSA_ABI_VERSION 13
 
 #if defined(__GNUC__) || defined(__clang__)
 #define MOSAIC_API __attribute__((visibility("default")))
@@ -530,6 +530,61 @@ MOSAIC_API int mosaic_query_attn_bwd(mosaic_bnhd q, mosaic_bnhd k, mosaic_bnhd v
                                      int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t block_count,
                                      float softmax_scale, const void* fwd_workspace, void* grad_q, void* grad_k,
                                      void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Codes of a cache. */
+typedef enum {
+    MOSAIC_CODE_INT8 = 0,          /* whole numbers -127 .. 127                           */
+    MOSAIC_CODE_E4M3 = 1           /* OCP e4m3, at most 448                               */
+} mosaic_code_type;
+
+/* A key/value cache held in 8 bits, with a scale for each block of tokens, kv head, and for keys and
+   values: the value of a code is code * scale.  batch sequences of capacity tokens, in num_blocks =
+   ceil(capacity / block_size) blocks of block_size (64, 128 or 256).  k_codes, v_codes: bytes
+   [batch, num_blocks, num_kv_heads, block_size * 64], 16-byte aligned, in the library's own order (zeros
+   stand for zeros); k_scale, v_scale: fp32 [batch, num_blocks, num_kv_heads]; k_mean: bf16
+   [batch, num_blocks, num_kv_heads, 64], 16-byte aligned, the mean of each block's keys.  All zeros is an
+   empty cache.  It has no counterpart in the reference. */
+typedef struct {
+    void* k_codes;
+    void* v_codes;
+    float* k_scale;
+    float* v_scale;
+    void* k_mean;
+    int32_t batch, num_blocks, num_kv_heads, block_size, code_type, capacity;
+} mosaic_kv_cache;
+
+/* Writes num_tokens tokens of each sequence from position start on, or starts[b] (optional [batch], device);
+   of those the first counts[b] (optional [batch], device; clamped to 0 .. num_tokens).  The sequence ends
+   with them: later tokens of the blocks written to become zeros, other blocks stay as they are.  Tokens
+   whose position lies outside the cache are left out (with start itself that is MOSAIC_ERR_SHAPE).  For each
+   block and head, with M the largest code: scale = (the largest magnitude of the new tokens) / M, at least
+   the scale before where earlier tokens of the block are kept; code = value / scale to the nearest code, ties
+   to even, and the kept codes are set to the new scale likewise.  Magnitudes below 2^-100 are a block of zeros
+   (scale 0).  A value that is not finite makes the block's scale, and so all its values, NaN.  k_mean becomes
+   the mean of what the block then holds.  k, v: dtype [B, n, Hk, 64] by strides. */
+MOSAIC_API int mosaic_kv_cache_write(const mosaic_kv_cache* cache, mosaic_bnhd k, mosaic_bnhd v, int32_t dtype,
+                                     int32_t head_dim, int32_t num_tokens, int64_t start, const int32_t* starts,
+                                     const int32_t* counts, void* stream);
+
+/* Reads num_tokens tokens from position start, or starts[b], on: code * scale, rounded once to dtype;
+   k_out, v_out: [B, num_tokens, Hk, 64] contiguous.  Positions outside the cache (with starts) are zeros. */
+MOSAIC_API int mosaic_kv_cache_read(const mosaic_kv_cache* cache, int32_t dtype, int32_t head_dim, int32_t num_tokens,
+                                    int64_t start, const int32_t* starts, void* k_out, void* v_out, void* stream);
+
+/* Attention of q over a cache.  Row (b, n, g): the softmax over the keys of sequence b below its length
+   kv_lens[b] (optional, clamped to [0, capacity]; NULL: capacity), with block_indices only over those of the
+   blocks named in block_indices[b, n, h, :], a set as in mosaic_query_attn_fwd; a row without a key is zeros.
+   What a row has not chosen does not reach it, whatever it holds.  q: bf16 [B, Nq, Hq, 64]; block_indices: int64
+   [B, Nq, Hk, block_count] contiguous, or NULL (block_count 0); out: bf16 [B, Nq, Hq, 64] contiguous.  At most
+   16 query heads per kv head, block_count at most 1024.  workspace: mosaic_cache_attn_fwd_workspace_size()
+   bytes, 256-byte aligned (0: none).  softmax_scale <= 0 selects 64^-0.5; others lie within 1e-30 .. 1e30.  It
+   has no counterpart in the reference. */
+MOSAIC_API size_t mosaic_cache_attn_fwd_workspace_size(const mosaic_kv_cache* cache, int32_t num_queries,
+                                                       int32_t num_q_heads, int32_t block_count);
+MOSAIC_API int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int64_t* block_indices,
+                                     const int32_t* kv_lens, int32_t num_queries, int32_t num_q_heads, int32_t head_dim,
+                                     int32_t block_count, float softmax_scale, void* out, void* workspace,
+                                     size_t workspace_bytes, void* stream);
 
 /* Name of a status code (static storage). */
 MOSAIC_API const char* mosaic_bsa_strerror(int status);

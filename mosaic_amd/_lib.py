@@ -12,7 +12,7 @@ import threading
 
 LIB_NAME = "libmosaic_bsa.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 # mosaic_bsa_mode
 MODE_FULL = 0
@@ -44,6 +44,10 @@ POS_F64 = 1
 POS_I32 = 2
 POS_I64 = 3
 MAX_AXES = 8
+
+# mosaic_code_type
+CODE_INT8 = 0
+CODE_E4M3 = 1
 
 EXPORTED_SYMBOLS = (
     "mosaic_bsa_workspace_size",
@@ -81,6 +85,10 @@ EXPORTED_SYMBOLS = (
     "mosaic_query_attn_fwd",
     "mosaic_query_attn_bwd_workspace_size",
     "mosaic_query_attn_bwd",
+    "mosaic_kv_cache_write",
+    "mosaic_kv_cache_read",
+    "mosaic_cache_attn_fwd_workspace_size",
+    "mosaic_cache_attn_fwd",
     "mosaic_bsa_strerror",
     "mosaic_bsa_abi_version",
 )
@@ -132,6 +140,15 @@ class Rotation(ctypes.Structure):
         ("stride_b", ctypes.c_int64), ("stride_n", ctypes.c_int64),
         ("position_type", ctypes.c_int32), ("num_axes", ctypes.c_int32), ("interleaved", ctypes.c_int32),
         ("sections", ctypes.c_int32 * MAX_AXES), ("theta", ctypes.c_double * MAX_AXES),
+    ]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("k_mean", ctypes.c_void_p),
+        ("batch", ctypes.c_int32), ("num_blocks", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("block_size", ctypes.c_int32), ("code_type", ctypes.c_int32), ("capacity", ctypes.c_int32),
     ]
 
 
@@ -226,6 +243,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mosaic_query_attn_bwd.argtypes = [Bnhd, Bnhd, Bnhd, c_vp, c_vp, Bnhd, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32,
                                           c_i32, c_i32, c_i32, c_i32, c_f, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]
     lib.mosaic_query_attn_bwd.restype = c_int
+    lib.mosaic_kv_cache_write.argtypes = [P(Cache), Bnhd, Bnhd, c_i32, c_i32, c_i32, c_i64, c_vp, c_vp, c_vp]
+    lib.mosaic_kv_cache_write.restype = c_int
+    lib.mosaic_kv_cache_read.argtypes = [P(Cache), c_i32, c_i32, c_i32, c_i64, c_vp, c_vp, c_vp, c_vp]
+    lib.mosaic_kv_cache_read.restype = c_int
+    lib.mosaic_cache_attn_fwd_workspace_size.argtypes = [P(Cache), c_i32, c_i32, c_i32]
+    lib.mosaic_cache_attn_fwd_workspace_size.restype = c_size
+    lib.mosaic_cache_attn_fwd.argtypes = [Bnhd, P(Cache), c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_f, c_vp, c_vp, c_size, c_vp]
+    lib.mosaic_cache_attn_fwd.restype = c_int
     lib.mosaic_bsa_strerror.argtypes = [c_int]
     lib.mosaic_bsa_strerror.restype = ctypes.c_char_p
     lib.mosaic_bsa_abi_version.argtypes = []

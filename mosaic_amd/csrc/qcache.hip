@@ -1,0 +1,448 @@
+// qcache.hip -- quantising a key/value cache as it is written, and reading it back (gfx950).
+//
+// A write puts tokens [start, end) of a member into its blocks; its sequence ends there.  For each block
+// touched, kv head, and for keys and values on their own, with M the largest code (127, or 448 in e4m3):
+//   a     = the largest |x| of the block's new tokens (0 where it is below 2^-100)
+//   scale = a / M, and not below the block's scale before where earlier tokens of it are kept
+//   code  = x / scale rounded to the nearest code, ties to even; of a kept token, code scale_before / scale
+// Tokens of the block behind the end become zeros; other blocks stay as they are.  A value that is not
+// finite makes its block's scale NaN, which everything read from the block then is.  The mean of the
+// block's keys (the sum of the codes times the scale over the number of tokens) goes to k_mean, where
+// query_topk takes it from.
+//
+// The rounding is that of the exact quotient: x * (1 / scale) is corrected by its remainder, and made
+// odd in its last bit where a remainder is left, so that no quotient beside a tie becomes one.
+//
+// Bound by HBM: a workgroup takes a block of one head, reads its rows once into registers and writes
+// both code tiles contiguously, 16 bytes a lane.  The heads of a block are neighbouring workgroups, so
+// that the lines of their tokens' rows are read together.
+#include <hip/hip_runtime.h>
+
+#include "qcache.h"
+
+namespace mosaic {
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr float kLeast = 0x1p-100f;   // below it a block is zeros: 1 / scale stays in fp32
+
+struct CacheParams {
+    mosaic_kv_cache c;
+    const void* k; int64_t k_sb, k_sn, k_sh;
+    const void* v; int64_t v_sb, v_sn, v_sh;
+    void* k_out; void* v_out;      // read: [B, n, Hk, 64]
+    const int32_t* starts;         // [B], or null: start
+    const int32_t* counts;         // [B], or null: n
+    int64_t start;
+    int n, units;                  // tokens; blocks (write) or tiles of 64 (read) of a member at most
+};
+
+template <typename T> struct Row4;   // four values of a row
+template <> struct Row4<bf16_t> {
+    static __device__ __forceinline__ float4 load(const bf16_t* p) {
+        const uint2 u = ld8(p);
+        return make_float4(bf_lo(u.x), bf_hi(u.x), bf_lo(u.y), bf_hi(u.y));
+    }
+    static __device__ __forceinline__ void store(bf16_t* p, float4 x) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+    }
+};
+template <> struct Row4<float> {
+    static __device__ __forceinline__ float4 load(const float* p) { return *reinterpret_cast<const float4*>(p); }
+    static __device__ __forceinline__ void store(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
+};
+// sixteen of one, as 16-byte accesses
+__device__ __forceinline__ void load16(const bf16_t* p, float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint4 u = ld16(p + 8 * i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[8 * i + 2 * j] = bf_lo(w[j]);
+            x[8 * i + 2 * j + 1] = bf_hi(w[j]);
+        }
+    }
+}
+__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 u = Row4<float>::load(p + 4 * i);
+        x[4 * i] = u.x; x[4 * i + 1] = u.y; x[4 * i + 2] = u.z; x[4 * i + 3] = u.w;
+    }
+}
+
+// y next to the quotient that `rest` (of any size, its sign that of the quotient minus y) is left of: odd
+// in its last bit unless exact.  A later rounding to fewer bits is then that of the quotient itself.
+__device__ __forceinline__ float to_odd(float y, float rest) {
+    const uint32_t u = __float_as_uint(y);
+    const bool up = (__float_as_uint(rest) ^ u) >> 31 == 0;   // away from zero
+    const uint32_t moved = up ? u + 1 : u - 1;
+    return rest == 0.f || (u & 1) || (u << 1) == 0 ? y : __uint_as_float(moved);
+}
+
+struct Quant {
+    float scale, inv;   // inv 0 where the block is zeros or NaN
+    __device__ __forceinline__ void init(float s) {
+        scale = s;
+        inv = s > 0.f ? 1.f / s : 0.f;
+    }
+    __device__ __forceinline__ float quotient(float x) const {
+        const float y0 = x * inv, y = fmaf(fmaf(-y0, scale, x), inv, y0);
+        return to_odd(y, fmaf(-y, scale, x));
+    }
+    // of a code under another scale: the product has 32 bits, the quotient no tie that fp64 does not tell
+    __device__ __forceinline__ float requotient(float code, float before) const {
+        if (!(inv > 0.f)) return 0.f;
+        const double z = (double)code * (double)before / (double)scale;
+        const float y = (float)z;
+        return to_odd(y, (float)(z - (double)y));
+    }
+};
+
+template <bool FP8>
+__device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
+    if constexpr (FP8) {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+    } else {
+        auto byte = [](float x) { return (uint32_t)(int)rintf(x) & 0xffu; };
+        return byte(a) | byte(b) << 8 | byte(c) << 16 | byte(d) << 24;
+    }
+}
+
+// words of the four lanes of a quad, transposed: lane i's word j becomes lane j's word i
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4]) {
+    const int q = threadIdx.x & 3;
+    // exchange with lane ^ 1 the words whose low index bit differs, then with lane ^ 2
+    const bool odd = q & 1, high = q & 2;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        const uint32_t give = odd ? w[j] : w[j + 1];
+        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0xb1, 0xf, 0xf, true);   // lane ^ 1
+        w[j] = odd ? got : w[j];
+        w[j + 1] = odd ? w[j + 1] : got;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t give = high ? w[j] : w[j + 2];
+        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0x4e, 0xf, 0xf, true);   // lane ^ 2
+        w[j] = high ? got : w[j];
+        w[j + 2] = high ? w[j + 2] : got;
+    }
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }   // NaN above infinity
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, d));
+    return x;
+}
+
+// The scale of a block from the largest magnitude (its bits) of its new tokens
+template <bool FP8>
+__device__ __forceinline__ float new_scale(uint32_t most, bool keeps, float before) {
+    constexpr float kTop = FP8 ? 448.f : 127.f;
+    const float a = __uint_as_float(most);
+    if (most >= 0x7f800000u || (keeps && !(before < INFINITY))) return NAN;
+    const float s = a < kLeast ? 0.f : a / kTop;
+    return keeps ? fmaxf(s, before) : s;
+}
+
+// What a thread holds of each tile of 64 tokens: of the keys the 16 dims of one token that are its chunk
+// of the layout; of the values four dims of four tokens, whose codes four neighbouring lanes then
+// exchange, so that each has a chunk.
+template <typename T, bool FP8, int SUB>
+__global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p) {
+    __shared__ uint32_t most[2][kWaves];
+    __shared__ float sums[2][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.x % p.c.num_kv_heads, rest = blockIdx.x / p.c.num_kv_heads, unit = rest % p.units, b = rest / p.units;
+    constexpr int kBlock = 64 * SUB;
+    // the run's place among the positions of the sequence, and what of it lies in the cache
+    const int64_t at = p.starts != nullptr ? p.starts[b] : p.start;
+    const int count = p.counts != nullptr ? min(max(p.counts[b], 0), p.n) : p.n;
+    const int64_t first = at < 0 ? 0 : at, last = at + count < p.c.capacity ? at + count : p.c.capacity;
+    const int64_t j64 = first / kBlock + unit;
+    if (last <= first || j64 * kBlock >= last) return;
+    const int j = (int)j64, t0 = j * kBlock, begin = (int)first - t0, end = (int)(last - t0) < kBlock ? (int)(last - t0) : kBlock;
+    // new tokens of the block: [max(begin, 0), end); kept ones: those before
+    const bool keeps = begin > 0;
+    const int64_t blk = block_at(p.c, b, j, h);
+    uint8_t* kc = static_cast<uint8_t*>(p.c.k_codes) + blk * (kBlock * 64);
+    uint8_t* vc = static_cast<uint8_t*>(p.c.v_codes) + blk * (kBlock * 64);
+    const int kkey = 32 * (wave >> 1) + key_of_row(lane & 31), kdim = 32 * (wave & 1) + 16 * (lane >> 5);
+    const int vdim = 4 * (lane >> 2), vkey = 16 * wave + 4 * (lane & 3);
+    // chunk of the values' layout that this lane stores: dim vdim + lane % 4, tokens 16 wave ..
+    const int vd = vdim + (lane & 3), vchunk = (((wave >> 1) * 2 + (vd >> 5)) * 2 + (wave & 1)) * 32 + (vd & 31);
+    const T* kx = static_cast<const T*>(p.k) + b * p.k_sb + h * p.k_sh + kdim;
+    const T* vx = static_cast<const T*>(p.v) + b * p.v_sb + h * p.v_sh + vdim;
+
+    float k[SUB][16], v[SUB][4][4];
+    uint32_t km = 0, vm = 0;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+        const int tk = 64 * s + kkey;
+        if (tk >= begin && tk < end) load16(kx + (t0 + tk - at) * p.k_sn, k[s]);
+        else
+#pragma unroll
+            for (int i = 0; i < 16; ++i) k[s][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int tv = 64 * s + vkey + i;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (tv >= begin && tv < end) x = Row4<T>::load(vx + (t0 + tv - at) * p.v_sn);
+            v[s][i][0] = x.x; v[s][i][1] = x.y; v[s][i][2] = x.z; v[s][i][3] = x.w;
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            km = max(km, magnitude(k[s][i]));
+            vm = max(vm, magnitude(v[s][i >> 2][i & 3]));
+        }
+    km = wave_max(km);
+    vm = wave_max(vm);
+    if (lane == 0) {
+        most[0][wave] = km;
+        most[1][wave] = vm;
+    }
+    const float kold = keeps ? p.c.k_scale[blk] : 0.f, vold = keeps ? p.c.v_scale[blk] : 0.f;
+    __syncthreads();   // (the scales before are read by every thread by now)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        km = max(km, most[0][w]);
+        vm = max(vm, most[1][w]);
+    }
+    Quant kq, vq;
+    kq.init(new_scale<FP8>(km, keeps, kold));
+    vq.init(new_scale<FP8>(vm, keeps, vold));
+
+    float sum[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = kq.inv > 0.f ? kq.quotient(k[s][i]) : 0.f;
+        uint4* chunk = reinterpret_cast<uint4*>(kc + s * kCodeTile) + tid;
+        if (keeps && 64 * s + kkey < begin) {
+            const uint4 u = *chunk;
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 c = codes_f32<FP8>(w[i]);
+                y[4 * i] = kq.requotient(c.x, kold); y[4 * i + 1] = kq.requotient(c.y, kold);
+                y[4 * i + 2] = kq.requotient(c.z, kold); y[4 * i + 3] = kq.requotient(c.w, kold);
+            }
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = pack_codes<FP8>(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            const float4 c = codes_f32<FP8>(w[i]);
+            sum[4 * i] += c.x; sum[4 * i + 1] += c.y; sum[4 * i + 2] += c.z; sum[4 * i + 3] += c.w;
+        }
+        *chunk = make_uint4(w[0], w[1], w[2], w[3]);
+
+        uint32_t x[4];
+        uint32_t was[4] = {0, 0, 0, 0};
+        const bool kept = keeps && 64 * s + vkey < begin;
+        if (kept)   // word d: dim vdim + d of this lane's four tokens
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const int vdd = vdim + d, from = (((wave >> 1) * 2 + (vdd >> 5)) * 2 + (wave & 1)) * 32 + (vdd & 31);
+                was[d] = *reinterpret_cast<const uint32_t*>(vc + s * kCodeTile + 16 * from + 4 * (lane & 3));
+            }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            float z[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = vq.inv > 0.f ? vq.quotient(v[s][i][d]) : 0.f;
+            if (kept) {
+                const float4 c = codes_f32<FP8>(was[d]);
+                const float old[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (64 * s + vkey + i < begin) z[i] = vq.requotient(old[i], vold);
+            }
+            x[d] = pack_codes<FP8>(z[0], z[1], z[2], z[3]);
+        }
+        quad_transpose(x);
+        reinterpret_cast<uint4*>(vc + s * kCodeTile)[vchunk] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+
+    // the keys' mean: the sixteen sums over the 32 rows of a half wave, each exchange halving what a lane holds
+#pragma unroll
+    for (int d = 16, n = 16; d > 1; d >>= 1, n >>= 1) {
+        const bool upper = lane & d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= n / 2) break;
+            const float give = upper ? sum[i] : sum[i + n / 2];
+            sum[i] = (upper ? sum[i + n / 2] : sum[i]) + __shfl_xor(give, d);
+        }
+    }
+    sum[0] += __shfl_xor(sum[0], 1);
+    // lane bits 4..1 chose the dim: bit 4 the upper eight of sixteen, and so on
+    const int dim = kdim + 8 * ((lane >> 4) & 1) + 4 * ((lane >> 3) & 1) + 2 * ((lane >> 2) & 1) + ((lane >> 1) & 1);
+    if ((lane & 1) == 0) sums[wave >> 1][dim] = sum[0];
+    __syncthreads();
+    if (tid < 32) {
+        // (the mean of the codes first: their sum times the scale need not fit)
+        const float a = (sums[0][2 * tid] + sums[1][2 * tid]) / (float)end * kq.scale;
+        const float c = (sums[0][2 * tid + 1] + sums[1][2 * tid + 1]) / (float)end * kq.scale;
+        static_cast<uint32_t*>(p.c.k_mean)[blk * 32 + tid] = pack_bf16x2(a, c);
+    }
+    if (tid == 0) {
+        p.c.k_scale[blk] = kq.scale;
+        p.c.v_scale[blk] = vq.scale;
+    }
+}
+
+// The write's exchange backwards; a workgroup takes a tile of 64 tokens of one head.  Tokens outside
+// the cache are zeros.
+template <typename T, bool FP8>
+__global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(CacheParams p) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.x % p.c.num_kv_heads, rest = blockIdx.x / p.c.num_kv_heads, unit = rest % p.units, b = rest / p.units;
+    const int64_t at = p.starts != nullptr ? p.starts[b] : p.start;
+    const int64_t t0 = ((at >> 6) + unit) * 64;    // (>> rounds down, also before the first token)
+    if (t0 >= at + p.n) return;
+    const bool held = t0 >= 0 && t0 < (int64_t)p.c.num_blocks * p.c.block_size;
+    float ks = 0.f, vs = 0.f;
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
+    const int vdim = 4 * (lane >> 2), vkey = 16 * wave + 4 * (lane & 3);
+    if (held) {
+        const int j = (int)(t0 / p.c.block_size), sub = ((int)t0 - j * p.c.block_size) / 64;
+        const int64_t blk = block_at(p.c, b, j, h), from = blk * p.c.block_size * 64 + sub * kCodeTile;
+        const int vd = vdim + (lane & 3), vchunk = (((wave >> 1) * 2 + (vd >> 5)) * 2 + (wave & 1)) * 32 + (vd & 31);
+        k = ld16(static_cast<const uint8_t*>(p.c.k_codes) + from + 16 * tid);
+        v = ld16(static_cast<const uint8_t*>(p.c.v_codes) + from + 16 * vchunk);
+        ks = p.c.k_scale[blk];
+        vs = p.c.v_scale[blk];
+    }
+    const int64_t end = at + p.n < p.c.capacity ? at + p.n : p.c.capacity;
+    auto row = [&](void* out, int64_t t, int dim) {
+        return static_cast<T*>(out) + (((int64_t)b * p.n + (t - at)) * p.c.num_kv_heads + h) * 64 + dim;
+    };
+    auto times = [](float4 c, float s) { return make_float4(c.x * s, c.y * s, c.z * s, c.w * s); };
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int64_t tk = t0 + 32 * (wave >> 1) + key_of_row(lane & 31);
+    if (tk >= at && tk < at + p.n) {
+        T* out = row(p.k_out, tk, 32 * (wave & 1) + 16 * (lane >> 5));
+        const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = tk >= 0 && tk < end ? times(codes_f32<FP8>(w[i]), ks) : zero;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(pack_bf16x2(x[2 * i].x, x[2 * i].y), pack_bf16x2(x[2 * i].z, x[2 * i].w),
+                                                                    pack_bf16x2(x[2 * i + 1].x, x[2 * i + 1].y), pack_bf16x2(x[2 * i + 1].z, x[2 * i + 1].w));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Row4<T>::store(out + 4 * i, x[i]);
+        }
+    }
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    quad_transpose(w);   // word d: dim vdim + d of tokens vkey ..
+    float4 x[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) x[d] = times(codes_f32<FP8>(w[d]), vs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t t = t0 + vkey + i;
+        if (t < at || t >= at + p.n) continue;
+        auto pick = [&](const float4& y) { return i == 0 ? y.x : i == 1 ? y.y : i == 2 ? y.z : y.w; };
+        const bool in = t >= 0 && t < end;
+        Row4<T>::store(row(p.v_out, t, vdim), in ? make_float4(pick(x[0]), pick(x[1]), pick(x[2]), pick(x[3])) : zero);
+    }
+}
+
+// ------------------------------------------------------------------ host
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int check_rows(const mosaic_bnhd& t, int dtype) {
+    const int64_t unit = dtype == MOSAIC_DTYPE_BF16 ? 8 : 4;
+    if (t.ptr == nullptr) return MOSAIC_ERR_NULL_POINTER;
+    if (!aligned(t.ptr, 16) || t.stride_b % unit || t.stride_n % unit || t.stride_h % unit) return MOSAIC_ERR_ALIGNMENT;
+    return MOSAIC_OK;
+}
+
+// Units of `size` tokens that a run of n touches at most
+int64_t units_of(int64_t n, int64_t size, int64_t start, bool anywhere) {
+    if (anywhere) return (n + size - 2) / size + 1;
+    return (start + n + size - 1) / size - start / size;
+}
+
+template <typename T, bool FP8>
+const void* write_kernel(int bs) {
+    return bs == 64    ? (const void*)&kv_cache_write_kernel<T, FP8, 1>
+           : bs == 128 ? (const void*)&kv_cache_write_kernel<T, FP8, 2>
+                       : (const void*)&kv_cache_write_kernel<T, FP8, 4>;
+}
+
+int check_run(const mosaic_kv_cache* cache, int32_t dtype, int32_t head_dim, int32_t n, int64_t start, const int32_t* starts,
+              const int32_t* counts) {
+    if (int e = check_cache(cache)) return e;
+    if (head_dim != kHeadDim) return MOSAIC_ERR_HEAD_DIM;
+    if (dtype != MOSAIC_DTYPE_BF16 && dtype != MOSAIC_DTYPE_F32) return MOSAIC_ERR_UNSUPPORTED;
+    if (n <= 0) return MOSAIC_ERR_SHAPE;
+    if (starts == nullptr && (start < 0 || start + n > cache->capacity)) return MOSAIC_ERR_SHAPE;
+    if (!aligned(starts, 4) || !aligned(counts, 4)) return MOSAIC_ERR_ALIGNMENT;
+    return MOSAIC_OK;
+}
+
+}  // namespace
+}  // namespace mosaic
+
+using namespace mosaic;
+
+extern "C" {
+
+int mosaic_kv_cache_write(const mosaic_kv_cache* cache, mosaic_bnhd k, mosaic_bnhd v, int32_t dtype, int32_t head_dim,
+                          int32_t num_tokens, int64_t start, const int32_t* starts, const int32_t* counts, void* stream) {
+    if (int e = check_run(cache, dtype, head_dim, num_tokens, start, starts, counts)) return e;
+    for (const mosaic_bnhd* t : {&k, &v})
+        if (int e = check_rows(*t, dtype)) return e;
+    CacheParams p{};
+    p.c = *cache;
+    p.k = k.ptr; p.k_sb = k.stride_b; p.k_sn = k.stride_n; p.k_sh = k.stride_h;
+    p.v = v.ptr; p.v_sb = v.stride_b; p.v_sn = v.stride_n; p.v_sh = v.stride_h;
+    p.starts = starts; p.counts = counts; p.start = start; p.n = num_tokens;
+    int64_t units = units_of(num_tokens, cache->block_size, start, starts != nullptr);
+    if (units > cache->num_blocks) units = cache->num_blocks;
+    p.units = (int)units;
+    const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, half = dtype == MOSAIC_DTYPE_BF16;
+    const void* fn = half ? (fp8 ? write_kernel<bf16_t, true>(cache->block_size) : write_kernel<bf16_t, false>(cache->block_size))
+                          : (fp8 ? write_kernel<float, true>(cache->block_size) : write_kernel<float, false>(cache->block_size));
+    void* args[] = {&p};
+    const unsigned grid = (unsigned)(units * cache->num_kv_heads * cache->batch);
+    return hipLaunchKernel(fn, dim3(grid), dim3(kThreads), args, 0, static_cast<hipStream_t>(stream)) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+}
+
+int mosaic_kv_cache_read(const mosaic_kv_cache* cache, int32_t dtype, int32_t head_dim, int32_t num_tokens, int64_t start,
+                         const int32_t* starts, void* k_out, void* v_out, void* stream) {
+    if (int e = check_run(cache, dtype, head_dim, num_tokens, start, starts, nullptr)) return e;
+    if (k_out == nullptr || v_out == nullptr) return MOSAIC_ERR_NULL_POINTER;
+    if (!aligned(k_out, 16) || !aligned(v_out, 16)) return MOSAIC_ERR_ALIGNMENT;
+    CacheParams p{};
+    p.c = *cache;
+    p.k_out = k_out; p.v_out = v_out;
+    p.starts = starts; p.start = start; p.n = num_tokens;
+    const int64_t units = units_of(num_tokens, 64, start, starts != nullptr);
+    p.units = (int)units;
+    if ((double)units * cache->num_kv_heads * cache->batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
+    const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, half = dtype == MOSAIC_DTYPE_BF16;
+    const void* fn = half ? (fp8 ? (const void*)&kv_cache_read_kernel<bf16_t, true> : (const void*)&kv_cache_read_kernel<bf16_t, false>)
+                          : (fp8 ? (const void*)&kv_cache_read_kernel<float, true> : (const void*)&kv_cache_read_kernel<float, false>);
+    void* args[] = {&p};
+    const unsigned grid = (unsigned)(units * cache->num_kv_heads * cache->batch);
+    return hipLaunchKernel(fn, dim3(grid), dim3(kThreads), args, 0, static_cast<hipStream_t>(stream)) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+}
+
+}  // extern "C"
