@@ -312,38 +312,292 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(CacheAttnParams
     store_row(p.out, row.at, lane, a.o, w);
 }
 
-// Joins the splits' partials: 16 lanes a row, 4 dims each.  Lane j holds the weights of splits j and
-// j + 16, so that no load waits for another.
-__global__ __launch_bounds__(kThreads) void cache_attn_join_kernel(CacheAttnParams p, int64_t rows) {
-    static_assert(kMaxSplit == 32, "two splits a lane");
-    const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, row = at < rows ? at : rows - 1;
-    const int j = threadIdx.x % 16, d = 4 * j;
-    float2 ml[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int s = j + 16 * i;
-        ml[i] = s < p.splits ? p.part_ml[s * rows + row] : make_float2(-INFINITY, 0.f);
+// ------------------------------------------------------------------ few rows
+
+// One token above all: no more than 16 rows (token, head) of a kv head.  A workgroup's waves take the tiles
+// of 64 keys of its share in turn, straight from memory into the operands of v_mfma_f32_16x16x32_bf16
+// (lane group g = lane / 16): in step m the keys' rows 4 g + i are tokens 16 g + 4 m + i, so that a lane
+// ends with the scores of the 16 tokens that its chunk of the values holds.  A tile is requested while
+// the one before is computed.
+constexpr int kFewRows = 16, kFewEntries = 64;
+
+struct FewState {
+    f32x4 o[4];       // O^T [16 dims]: dims 16 dg + 4 g + i
+    float m, l;
+};
+struct Codes { uint4 k[4], v[4]; float ks, vs; };
+
+__device__ __forceinline__ float xor16_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_add(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <bool FP8>
+__device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
+    const uint2 x = codes_bf16<FP8>(a), y = codes_bf16<FP8>(b);
+    return as_bf16x8(make_uint4(x.x, x.y, y.x, y.y));
+}
+
+template <bool FP8, bool SAFE>
+__device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2], bool member, int valid, float c, float& w, bool& narrow, FewState& a) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const float ck = score_factor(c, t.ks);
+    float lv = t.vs, iv = 1.f;
+    if constexpr (!SAFE) {
+        if (w == 0.f && t.vs > 0.f && t.vs < INFINITY) w = t.vs;
+        const float base = w == 0.f ? 1.f : w, of = t.vs == 0.f ? base : t.vs;
+        narrow = narrow && of <= base * kSpread && of >= base * (1.f / kSpread);
+        iv = base / of;
+        lv = __builtin_amdgcn_logf(of / base);
     }
-    float m = fmaxf(ml[0].y == 0.f ? -INFINITY : ml[0].x, ml[1].y == 0.f ? -INFINITY : ml[1].x);
+    f32x4 s[4];
 #pragma unroll
-    for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-    float a[2], l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {   // l = 0: no key in that share
-        a[i] = ml[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - m) * ml[i].y;
-        l += a[i];
+    for (int m = 0; m < 4; ++m) {
+        s[m] = mfma16(codes8<FP8>(t.k[m].x, t.k[m].y), qf[0], f32x4{0.f, 0.f, 0.f, 0.f});
+        s[m] = mfma16(codes8<FP8>(t.k[m].z, t.k[m].w), qf[1], s[m]);
     }
+    if (valid < 64) {
+        seldom();
+        int left = valid - 16 * g;
+        asm volatile("" : "+v"(left));
 #pragma unroll
-    for (int x = 1; x < 16; x <<= 1) l += __shfl_xor(l, x);
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[m][i] = 4 * m + i < left ? s[m][i] : -INFINITY;
+    }
+    float mt = s[0][0];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mt = __builtin_elementwise_maximum(mt, s[m][i]);
+    const float shift = SAFE ? 0.f : lv;
+    mt = fmaf(xor32_max(xor16_max(mt)), ck, shift);
+    const bool move = member && mt > a.m + kTau;
+    if (__builtin_amdgcn_ballot_w64(move)) {
+        const float alpha = move ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
+        a.m = move ? mt : a.m;
+#pragma unroll
+        for (int dg = 0; dg < 4; ++dg) a.o[dg] *= alpha;
+        a.l *= alpha;
+    }
+    const float ref = member ? shift - a.m : -INFINITY;   // P = 0 for the others
+    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(SAFE ? times_plus(x, ck, ref) : fmaf(x, ck, ref)); };
+    bf16x8 pb[2];
+    float lt = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = pack_bf16x2(weight(s[2 * j + (i >> 1)][2 * (i & 1)]), weight(s[2 * j + (i >> 1)][2 * (i & 1) + 1]));
+        pb[j] = as_bf16x8(make_uint4(u[0], u[1], u[2], u[3]));
+        lt = operand_sum(pb[j], lt);
+    }
+    if constexpr (SAFE) {
+        if (member) a.l += lt;
+    } else a.l = fmaf(lt, iv, a.l);
+#pragma unroll
+    for (int dg = 0; dg < 4; ++dg) {
+        const bf16x8 v0 = codes8<FP8>(t.v[dg].x, t.v[dg].y), v1 = codes8<FP8>(t.v[dg].z, t.v[dg].w);
+        if constexpr (SAFE) {
+            const f32x4 y = mfma16(v1, pb[1], mfma16(v0, pb[0], f32x4{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a.o[dg][i] = member ? fmaf(y[i], lv, a.o[dg][i]) : a.o[dg][i];
+        } else a.o[dg] = mfma16(v1, pb[1], mfma16(v0, pb[0], a.o[dg]));
+    }
+}
+
+template <bool FP8, bool DENSE>
+__global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnParams p) {
+    __shared__ __attribute__((aligned(16))) float O[kWaves][kFewRows][64];
+    __shared__ float2 ml[kWaves][kFewRows];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits, h = rest % p.Hk, b = rest / p.Hk;
+    const int end = seq_keys(p, b), sub = p.bs / 64, rows = p.Nq * p.G;
+    const bool row_live = r < rows;
+    const int token = row_live ? r / p.G : 0, head = h * p.G + (row_live ? r - token * p.G : 0);
+    const bf16_t* qr = p.q + b * p.q_sb + token * p.q_sn + head * p.q_sh + 16 * g;
+    bf16x8 qf[2] = {as_bf16x8(ld16(qr)), as_bf16x8(ld16(qr + 8))};
+    // the call's blocks: all of them, or those that the tokens' entries name, one in a lane of every wave
+    int units, blk = -1, rank = 0;
+    uint32_t tokens = 0;
+    bool lead = false;
+    if constexpr (DENSE) units = (int)(((int64_t)end + 63) / 64);
+    else {
+        const int entries = p.Nq * p.K;
+        if (lane < entries) {
+            const int t = lane / p.K;
+            const int64_t u = p.idx[(((int64_t)b * p.Nq + t) * p.Hk + h) * p.K + lane - t * p.K];
+            blk = u >= 0 && u < p.nb && u * p.bs < end ? (int)u : -1;
+        }
+        lead = blk >= 0;
+        for (int j = 0, t = 0, of = 0; j < entries; ++j) {
+            const bool same = __builtin_amdgcn_readlane(blk, j) == blk;
+            tokens |= same ? 1u << t : 0u;
+            lead = lead && !(same && j < lane);
+            if (++of == p.K) {
+                of = 0;
+                ++t;
+            }
+        }
+        const uint64_t leads = __builtin_amdgcn_ballot_w64(lead);
+        rank = (int)__builtin_popcountll(leads & ((1ull << lane) - 1ull));
+        units = (int)__builtin_popcountll(leads) * sub;
+    }
+    const int first = (int)((int64_t)units * split / p.splits), past = (int)((int64_t)units * (split + 1) / p.splits);
+    const int kt = r >> 3, ko = kt * 2048 + (g >> 1) * 1024 + (g & 1) * 512 + (r & 7) * 16;
+    const int vo = (g >> 1) * 2048 + (g & 1) * 512 + r * 16;
+    // unit u: its first key, and the tokens that have it
+    auto where = [&](int u, uint32_t& of) {
+        of = ~0u;
+        if constexpr (DENSE) return u * 64;
+        else {
+            const int which = (int)((uint32_t)u / (uint32_t)sub);
+            const int src = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(lead && rank == which));
+            of = (uint32_t)__builtin_amdgcn_readlane((int)tokens, src);
+            return __builtin_amdgcn_readlane(blk, src) * p.bs + (u - which * sub) * 64;
+        }
+    };
+    auto load = [&](int key0, Codes& t) {
+        const int j = (int)((uint32_t)key0 / (uint32_t)p.bs);
+        const int64_t at = block_at(p.cache, b, j, h), from = at * (p.bs * 64) + (key0 - j * p.bs) * 64;
+        const uint8_t* kc = static_cast<const uint8_t*>(p.cache.k_codes) + from;
+        const uint8_t* vc = static_cast<const uint8_t*>(p.cache.v_codes) + from;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            t.k[i] = ld16(kc + ko + 128 * i);
+            t.v[i] = ld16(vc + vo + (i >> 1) * 1024 + (i & 1) * 256);
+        }
+        t.ks = p.cache.k_scale[at];
+        t.vs = p.cache.v_scale[at];
+    };
+    FewState a;
+    float w;
+    bool narrow;
+    auto walk = [&](auto safe) {
+        w = 0.f;
+        narrow = true;
+#pragma unroll
+        for (int dg = 0; dg < 4; ++dg) a.o[dg] = f32x4{0.f, 0.f, 0.f, 0.f};
+        a.m = -FLT_MAX;
+        a.l = 0.f;
+        if (first + wave >= past) return;
+        Codes next;
+        uint32_t of_next;
+        int key_next = where(first + wave, of_next);
+        load(min(key_next, end - 1), next);   // (a block's later tiles may lie behind the end)
+        for (int u = first + wave; u < past; u += kWaves) {
+            const Codes t = next;
+            const uint32_t of = of_next;
+            const int key0 = key_next;
+            if (u + kWaves < past) {
+                key_next = where(u + kWaves, of_next);
+                load(min(key_next, end - 1), next);
+            }
+            if (key0 < end)
+                attend_few<FP8, decltype(safe)::value>(t, qf, row_live && (DENSE || (of >> token & 1)), min(64, end - key0), p.c, w, narrow, a);
+        }
+        if (decltype(safe)::value || w == 0.f) w = 1.f;
+    };
+    walk(std::false_type{});
+    bool ok = narrow && a.l - a.l == 0.f;
+#pragma unroll
+    for (int dg = 0; dg < 4; ++dg)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ok = ok && a.o[dg][i] - a.o[dg][i] == 0.f;
+    if (__builtin_amdgcn_ballot_w64(!ok)) walk(std::true_type{});   // (a wave by itself)
+    const float l = xor32_add(xor16_add(a.l)), f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int dg = 0; dg < 4; ++dg)
+        *reinterpret_cast<float4*>(&O[wave][r][(16 * dg + 4 * g) ^ (4 * r)]) =
+            make_float4(a.o[dg][0] * f * w, a.o[dg][1] * f * w, a.o[dg][2] * f * w, a.o[dg][3] * f * w);
+    if (g == 0) {
+        int e = 0;
+        const float part = frexpf(l, &e);
+        ml[wave][r] = make_float2(a.m + (float)e, part);
+    }
+    __syncthreads();
+    // 16 threads a row
+    const int row = tid / 16, d = 4 * (tid % 16);
+    if (row >= rows) return;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) m = ml[i][row].y == 0.f ? m : fmaxf(m, ml[i][row].x);
+    float sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int n = min(16, p.splits - 16 * i);
+    for (int i = 0; i < kWaves; ++i) {
+        const float2 part = ml[i][row];
+        const float4 x = *reinterpret_cast<const float4*>(&O[i][row][d ^ (4 * row)]);
+        const float y = part.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(part.x - m) * part.y;   // 0: no key
+        sum += y;
+        o.x = fmaf(y, x.x, o.x); o.y = fmaf(y, x.y, o.y); o.z = fmaf(y, x.z, o.z); o.w = fmaf(y, x.w, o.w);
+    }
+    const float y = sum == 0.f ? 0.f : 1.f / sum;
+    const int t = row / p.G;
+    const int64_t at = ((int64_t)b * p.Nq + t) * p.Hq + h * p.G + row - t * p.G;
+    if (p.splits == 1) {
+        *reinterpret_cast<uint2*>(p.out + at * 64 + d) = make_uint2(pack_bf16x2(o.x * y, o.y * y), pack_bf16x2(o.z * y, o.w * y));
+        return;
+    }
+    const int64_t all = (int64_t)p.B * p.Nq * p.Hq;
+    *reinterpret_cast<float4*>(p.part_o + (split * all + at) * 64 + d) = make_float4(o.x * y, o.y * y, o.z * y, o.w * y);
+    if (d == 0) {
+        int e = 0;
+        const float part = frexpf(sum, &e);
+        p.part_ml[split * all + at] = make_float2(m + (float)e, part);
+    }
+}
+
+// ------------------------------------------------------------------ joins
+
+// Joins the splits' partials: 16 lanes a row, 4 dims each, and TEAM such groups a row that take its splits
+// in turn (of few splits one, of many all 16 of a workgroup).
+template <int TEAM>
+__global__ __launch_bounds__(kThreads) void cache_attn_join_kernel(CacheAttnParams p, int64_t rows) {
+    __shared__ __attribute__((aligned(16))) float4 part[16][16];
+    __shared__ float ml[16], sums[16];
+    const int group = threadIdx.x / 16, j = threadIdx.x % 16, d = 4 * j, of = group % TEAM;
+    const int64_t at = (int64_t)blockIdx.x * (16 / TEAM) + group / TEAM, row = at < rows ? at : rows - 1;
+    float m = -INFINITY;
+    for (int s = of + TEAM * j; s < p.splits; s += 16 * TEAM) {
+        const float2 x = p.part_ml[s * rows + row];
+        m = x.y == 0.f ? m : fmaxf(m, x.x);   // l = 0: no key in that share
+    }
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if constexpr (TEAM > 1) {
+        if (j == 0) ml[group] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TEAM; ++i) m = fmaxf(m, ml[group / TEAM * TEAM + i]);
+    }
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-        for (int s = 0; s < n; ++s) {
-            const float4 x = *reinterpret_cast<const float4*>(p.part_o + ((s + 16 * i) * rows + row) * 64 + d);
-            const float f = __shfl(a[i], (threadIdx.x & 48) + s);
-            o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+    for (int s = of; s < p.splits; s += TEAM) {
+        const float2 x = p.part_ml[s * rows + row];
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * 64 + d);
+        const float f = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - m) * x.y;
+        l += f;
+        o.x = fmaf(f, y.x, o.x); o.y = fmaf(f, y.y, o.y); o.z = fmaf(f, y.z, o.z); o.w = fmaf(f, y.w, o.w);
+    }
+    if constexpr (TEAM > 1) {
+        part[group][j] = o;
+        if (j == 0) sums[group] = l;
+        __syncthreads();
+        if (of != 0) return;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < TEAM; ++i) {
+            const float4 y = part[group + i][j];
+            l += sums[group + i];
+            o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
         }
     }
     if (at >= rows) return;
@@ -368,16 +622,29 @@ int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, 
     return MOSAIC_OK;
 }
 
+constexpr int64_t kFewGroups = 1024, kFewTiles = 2;
+
 int64_t groups_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq) {
     const int64_t per = kWaves * (kRows / (hq / c.num_kv_heads));
     return (nq + per - 1) / per * c.num_kv_heads * c.batch;
 }
-// Shares of the keys: below one workgroup per CU they are split, up to two per CU together.
+// Whether the call is one of cache_attn_few_kernel
+bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
+    const int64_t rows = (int64_t)nq * (hq / c.num_kv_heads);
+    return rows <= kFewRows && (int64_t)nq * K <= kFewEntries;
+}
+// Shares of the keys: below one workgroup per CU they are split.
 int choose_split(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
-    const int64_t wgs = groups_of(c, nq, hq), most = K > 0 ? K : c.num_blocks;
+    const int64_t sub = c.block_size / 64;
+    if (few(c, nq, hq, K)) {
+        const int64_t wgs = (int64_t)c.num_kv_heads * c.batch, tiles = K > 0 ? nq * K * sub : c.num_blocks * sub;
+        const int64_t s = kFewGroups / wgs, most = tiles / (kWaves * kFewTiles);
+        const int64_t n = s < most ? s : most;
+        return (int)(n < 1 ? 1 : n);
+    }
+    const int64_t wgs = groups_of(c, nq, hq), most = K > 0 ? (K < kMaxSplit ? K : kMaxSplit) : c.num_blocks;
     if (wgs >= 256) return 1;
-    int64_t s = 512 / wgs;
-    if (s > kMaxSplit) s = kMaxSplit;
+    const int64_t s = (K > 0 ? 512 : 768) / wgs;
     return (int)(s < most ? s : most);
 }
 size_t part_bytes(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
@@ -396,7 +663,7 @@ extern "C" {
 size_t mosaic_cache_attn_fwd_workspace_size(const mosaic_kv_cache* cache, int32_t num_queries, int32_t num_q_heads, int32_t block_count) {
     if (check_call(cache, num_queries, num_q_heads, kHeadDim, block_count) != MOSAIC_OK) return 0;
     return part_bytes(*cache, num_queries, num_q_heads, block_count) +
-           (block_count > 0 ? order_bytes(cache->batch, num_queries, num_q_heads, cache->num_kv_heads) : 0);
+           (block_count > 0 && !few(*cache, num_queries, num_q_heads, block_count) ? order_bytes(cache->batch, num_queries, num_q_heads, cache->num_kv_heads) : 0);
 }
 
 int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int64_t* block_indices, const int32_t* kv_lens,
@@ -428,19 +695,24 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
         p.part_ml = reinterpret_cast<float2*>(ws + up(p.splits * rows * kHeadDim * sizeof(float)));
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (block_count > 0) {
+    if (block_count > 0 && !few(*cache, num_queries, num_q_heads, block_count)) {
         place_order(p, ws + part_bytes(*cache, num_queries, num_q_heads, block_count));
         if (int e = launch_order(p, s)) return e;
     }
-    int total = p.qtiles * p.Hk * p.B * p.splits;
+    const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, small = few(*cache, num_queries, num_q_heads, block_count);
+    int total = (small ? 1 : p.qtiles) * p.Hk * p.B * p.splits;
     void* args[] = {&p, &total};
-    const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3;
     const void* fn = block_count > 0 ? (fp8 ? (const void*)&cache_attn_kernel<true, false> : (const void*)&cache_attn_kernel<false, false>)
                                      : (fp8 ? (const void*)&cache_attn_kernel<true, true> : (const void*)&cache_attn_kernel<false, true>);
+    if (small)
+        fn = block_count > 0 ? (fp8 ? (const void*)&cache_attn_few_kernel<true, false> : (const void*)&cache_attn_few_kernel<false, false>)
+                             : (fp8 ? (const void*)&cache_attn_few_kernel<true, true> : (const void*)&cache_attn_few_kernel<false, true>);
     if (launch(fn, dim3(total), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
     void* jargs[] = {&p, &rows};
-    return launch((const void*)&cache_attn_join_kernel, dim3((unsigned)((rows + 15) / 16)), jargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+    const bool team = p.splits > 16;
+    const void* join = team ? (const void*)&cache_attn_join_kernel<16> : (const void*)&cache_attn_join_kernel<1>;
+    return launch(join, dim3((unsigned)(team ? rows : (rows + 15) / 16)), jargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
 
 }  // extern "C"
