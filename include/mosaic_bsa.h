@@ -541,14 +541,15 @@ typedef enum {
    values: the value of a code is code * scale.  batch sequences of capacity tokens, in num_blocks =
    ceil(capacity / block_size) blocks of block_size (64, 128 or 256).  k_codes, v_codes: bytes
    [batch, num_blocks, num_kv_heads, block_size * 64], 16-byte aligned, in the library's own order (zeros
-   stand for zeros); k_scale, v_scale: fp32 [batch, num_blocks, num_kv_heads]; k_mean: bf16
-   [batch, num_blocks, num_kv_heads, 64], 16-byte aligned, the mean of each block's keys.  All zeros is an
-   empty cache.  It has no counterpart in the reference. */
+   stand for zeros); k_scale, v_scale, k_norm: fp32 [batch, num_blocks, num_kv_heads], k_norm not below the
+   norm of any key of the block; k_mean: bf16 [batch, num_blocks, num_kv_heads, 64], 16-byte aligned, the mean of
+   each block's keys.  All zeros is an empty cache.  It has no counterpart in the reference. */
 typedef struct {
     void* k_codes;
     void* v_codes;
     float* k_scale;
     float* v_scale;
+    float* k_norm;
     void* k_mean;
     int32_t batch, num_blocks, num_kv_heads, block_size, code_type, capacity;
 } mosaic_kv_cache;
@@ -560,8 +561,8 @@ typedef struct {
    block and head, with M the largest code: scale = (the largest magnitude of the new tokens) / M, at least
    the scale before where earlier tokens of the block are kept; code = value / scale to the nearest code, ties
    to even, and the kept codes are set to the new scale likewise.  Magnitudes below 2^-100 are a block of zeros
-   (scale 0).  A value that is not finite makes the block's scale, and so all its values, NaN.  k_mean becomes
-   the mean of what the block then holds.  k, v: dtype [B, n, Hk, 64] by strides. */
+   (scale 0).  A value that is not finite makes the block's scale, and so all its values, NaN.  k_mean and k_norm
+   become those of what the block then holds.  k, v: dtype [B, n, Hk, 64] by strides. */
 MOSAIC_API int mosaic_kv_cache_write(const mosaic_kv_cache* cache, mosaic_bnhd k, mosaic_bnhd v, int32_t dtype,
                                      int32_t head_dim, int32_t num_tokens, int64_t start, const int32_t* starts,
                                      const int32_t* counts, void* stream);

@@ -146,7 +146,7 @@ class Rotation(ctypes.Structure):
 class Cache(ctypes.Structure):
     _fields_ = [
         ("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
-        ("k_mean", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p), ("k_mean", ctypes.c_void_p),
         ("batch", ctypes.c_int32), ("num_blocks", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
         ("block_size", ctypes.c_int32), ("code_type", ctypes.c_int32), ("capacity", ctypes.c_int32),
     ]

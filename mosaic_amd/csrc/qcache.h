@@ -58,7 +58,8 @@ __device__ __forceinline__ float4 codes_f32(uint32_t w) {
 // Whether a cache's description can be addressed.
 inline int check_cache(const mosaic_kv_cache* c) {
     if (c == nullptr) return MOSAIC_ERR_NULL_POINTER;
-    if (c->k_codes == nullptr || c->v_codes == nullptr || c->k_scale == nullptr || c->v_scale == nullptr || c->k_mean == nullptr)
+    if (c->k_codes == nullptr || c->v_codes == nullptr || c->k_scale == nullptr || c->v_scale == nullptr ||
+        c->k_norm == nullptr || c->k_mean == nullptr)
         return MOSAIC_ERR_NULL_POINTER;
     if (c->batch <= 0 || c->num_blocks <= 0 || c->capacity <= 0) return MOSAIC_ERR_SHAPE;
     if (c->num_kv_heads <= 0) return MOSAIC_ERR_HEADS;
@@ -69,7 +70,8 @@ inline int check_cache(const mosaic_kv_cache* c) {
     if (c->capacity > c->num_blocks * c->block_size) return MOSAIC_ERR_SHAPE;
     if ((double)c->num_blocks * (c->block_size / 64) * c->num_kv_heads * c->batch > 2147483647.0 - 1024) return MOSAIC_ERR_SHAPE;
     auto low = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; };
-    if (low(c->k_codes, 16) || low(c->v_codes, 16) || low(c->k_scale, 4) || low(c->v_scale, 4) || low(c->k_mean, 16)) return MOSAIC_ERR_ALIGNMENT;
+    if (low(c->k_codes, 16) || low(c->v_codes, 16) || low(c->k_scale, 4) || low(c->v_scale, 4) || low(c->k_norm, 4) || low(c->k_mean, 16))
+        return MOSAIC_ERR_ALIGNMENT;
     return MOSAIC_OK;
 }
 

@@ -8,10 +8,11 @@
 // Tokens of the block behind the end become zeros; other blocks stay as they are.  A value that is not
 // finite makes its block's scale NaN, which everything read from the block then is.  The mean of the
 // block's keys (the sum of the codes times the scale over the number of tokens) goes to k_mean, where
-// query_topk takes it from.
+// query_topk takes it from, and a bound of their norms (the norm of the largest parts of 16 dims, at most
+// twice the largest norm) to k_norm, by which the attention knows that it needs no maxima.
 //
-// The rounding is that of the exact quotient: x * (1 / scale) is corrected by its remainder, and made
-// odd in its last bit where a remainder is left, so that no quotient beside a tie becomes one.
+// The rounding is that of the exact quotient: x * (1 / scale), within 1.5 units of its last place, is taken to
+// the nearest number that could be a tie, and moved off it by the sign of the remainder, which an fma gives.
 //
 // Bound by HBM: a workgroup takes a block of one head, reads its rows once into registers and writes
 // both code tiles contiguously, 16 bytes a lane.  The heads of a block are neighbouring workgroups, so
@@ -51,35 +52,67 @@ template <> struct Row4<float> {
     static __device__ __forceinline__ float4 load(const float* p) { return *reinterpret_cast<const float4*>(p); }
     static __device__ __forceinline__ void store(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
 };
-// sixteen of one, as 16-byte accesses
-__device__ __forceinline__ void load16(const bf16_t* p, float (&x)[16]) {
+
+// N values as they lie in memory, and the largest of their magnitudes' bits (NaN above infinity)
+template <typename T, int N> struct Raw;
+template <int N> struct Raw<bf16_t, N> {
+    uint32_t w[N / 2];
+    __device__ __forceinline__ void load(const bf16_t* p) {
+        if constexpr (N == 4) {
+            const uint2 u = ld8(p);
+            w[0] = u.x; w[1] = u.y;
+        } else
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint4 u = ld16(p + 8 * i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            for (int i = 0; i < N / 8; ++i) {
+                const uint4 u = ld16(p + 8 * i);
+                w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+            }
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[8 * i + 2 * j] = bf_lo(w[j]);
-            x[8 * i + 2 * j + 1] = bf_hi(w[j]);
+        for (int i = 0; i < N / 2; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf_hi(w[i / 2]) : bf_lo(w[i / 2]); }
+    // two magnitudes a word until the end
+    __device__ __forceinline__ uint32_t most(uint32_t m) const {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+            m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu)));
+        return m;
+    }
+    static __device__ __forceinline__ uint32_t end(uint32_t m) { return max(m & 0xffff0000u, m << 16); }
+};
+template <int N> struct Raw<float, N> {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 u = ld16(p + 4 * i);
+            w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
         }
     }
-}
-__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float4 u = Row4<float>::load(p + 4 * i);
-        x[4 * i] = u.x; x[4 * i + 1] = u.y; x[4 * i + 2] = u.z; x[4 * i + 3] = u.w;
+        for (int i = 0; i < N; ++i) w[i] = 0;
     }
-}
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(w[i]); }
+    __device__ __forceinline__ uint32_t most(uint32_t m) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = max(m, w[i] & 0x7fffffffu);
+        return m;
+    }
+    static __device__ __forceinline__ uint32_t end(uint32_t m) { return m; }
+};
 
-// y next to the quotient that `rest` (of any size, its sign that of the quotient minus y) is left of: odd
-// in its last bit unless exact.  A later rounding to fewer bits is then that of the quotient itself.
-__device__ __forceinline__ float to_odd(float y, float rest) {
-    const uint32_t u = __float_as_uint(y);
-    const bool up = (__float_as_uint(rest) ^ u) >> 31 == 0;   // away from zero
-    const uint32_t moved = up ? u + 1 : u - 1;
-    return rest == 0.f || (u & 1) || (u << 1) == 0 ? y : __uint_as_float(moved);
+// y, moved by a few units of its last place towards the side on which the quotient lies: the sign of
+// `rest` is that of the quotient minus y, and 0 stays 0.
+__device__ __forceinline__ float beside(float y, float rest) {
+    return rest == 0.f ? y : fmaf(fabsf(y), copysignf(0x1p-22f, rest), y);
 }
+// The nearest number to y with four zeros at its end: among such are all the codes and the middles between
+// them, and no two lie within the error of x * (1 / scale).
+__device__ __forceinline__ float blunt(float y) { return __uint_as_float((__float_as_uint(y) + 8) & ~15u); }
 
 struct Quant {
     float scale, inv;   // inv 0 where the block is zeros or NaN
@@ -88,15 +121,15 @@ struct Quant {
         inv = s > 0.f ? 1.f / s : 0.f;
     }
     __device__ __forceinline__ float quotient(float x) const {
-        const float y0 = x * inv, y = fmaf(fmaf(-y0, scale, x), inv, y0);
-        return to_odd(y, fmaf(-y, scale, x));
+        const float y = blunt(x * inv);
+        return beside(y, fmaf(-y, scale, x));
     }
-    // of a code under another scale: the product has 32 bits, the quotient no tie that fp64 does not tell
+    // of a code under another scale: code * before is high + low exactly
     __device__ __forceinline__ float requotient(float code, float before) const {
-        if (!(inv > 0.f)) return 0.f;
-        const double z = (double)code * (double)before / (double)scale;
-        const float y = (float)z;
-        return to_odd(y, (float)(z - (double)y));
+        if (inv == 0.f) return 0.f;
+        const float high = code * before, low = fmaf(code, before, -high);
+        const float y = blunt(high * inv);
+        return beside(y, fmaf(-y, scale, high) + low);
     }
 };
 
@@ -106,8 +139,10 @@ __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float 
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
         return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
     } else {
-        auto byte = [](float x) { return (uint32_t)(int)rintf(x) & 0xffu; };
-        return byte(a) | byte(b) << 8 | byte(c) << 16 | byte(d) << 24;
+        // rounded to a whole number by the sum, whose last byte it then is
+        auto round = [](float x) { return __float_as_uint(x + 12582912.f); };
+        const uint32_t lo = __builtin_amdgcn_perm(round(b), round(a), 0x0c0c0400), hi = __builtin_amdgcn_perm(round(d), round(c), 0x04000c0c);
+        return lo | hi;
     }
 }
 
@@ -132,11 +167,20 @@ __device__ __forceinline__ void quad_transpose(uint32_t (&w)[4]) {
     }
 }
 
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }   // NaN above infinity
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+// x of lane ^ D of the same half wave
+template <int D>
+__device__ __forceinline__ float lane_xor(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_ds_swizzle((int)__float_as_uint(x), D << 10 | 0x1f));
+}
+
+// Of 2 N sums a lane keeps the upper or the lower N, with those of lane ^ D added
+template <int N, int D>
+__device__ __forceinline__ void halve_sums(float (&sum)[16], bool upper) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, d));
-    return x;
+    for (int i = 0; i < N; ++i) {
+        const float keep = upper ? sum[i + N] : sum[i], give = upper ? sum[i] : sum[i + N];
+        sum[i] = keep + lane_xor<D>(give);
+    }
 }
 
 // The scale of a block from the largest magnitude (its bits) of its new tokens
@@ -155,7 +199,7 @@ __device__ __forceinline__ float new_scale(uint32_t most, bool keeps, float befo
 template <typename T, bool FP8, int SUB>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p) {
     __shared__ uint32_t most[2][kWaves];
-    __shared__ float sums[2][64];
+    __shared__ float sums[2][64], norms[2][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x % p.c.num_kv_heads, rest = blockIdx.x / p.c.num_kv_heads, unit = rest % p.units, b = rest / p.units;
     constexpr int kBlock = 64 * SUB;
@@ -178,38 +222,45 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
     const T* kx = static_cast<const T*>(p.k) + b * p.k_sb + h * p.k_sh + kdim;
     const T* vx = static_cast<const T*>(p.v) + b * p.v_sb + h * p.v_sh + vdim;
 
-    float k[SUB][16], v[SUB][4][4];
+    Raw<T, 16> k[SUB];
+    Raw<T, 4> v[SUB][4];
     uint32_t km = 0, vm = 0;
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
         const int tk = 64 * s + kkey;
-        if (tk >= begin && tk < end) load16(kx + (t0 + tk - at) * p.k_sn, k[s]);
-        else
-#pragma unroll
-            for (int i = 0; i < 16; ++i) k[s][i] = 0.f;
+        if (tk >= begin && tk < end) k[s].load(kx + (t0 + tk - at) * p.k_sn);
+        else k[s].clear();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int tv = 64 * s + vkey + i;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (tv >= begin && tv < end) x = Row4<T>::load(vx + (t0 + tv - at) * p.v_sn);
-            v[s][i][0] = x.x; v[s][i][1] = x.y; v[s][i][2] = x.z; v[s][i][3] = x.w;
+            if (tv >= begin && tv < end) v[s][i].load(vx + (t0 + tv - at) * p.v_sn);
+            else v[s][i].clear();
         }
     }
+    // the codes that are kept, as far as they share this lane's chunks
+    uint4 kwas[SUB], vwas[SUB];
+    const float kold = keeps ? p.c.k_scale[blk] : 0.f, vold = keeps ? p.c.v_scale[blk] : 0.f;
+    if (keeps)
 #pragma unroll
-    for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            km = max(km, magnitude(k[s][i]));
-            vm = max(vm, magnitude(v[s][i >> 2][i & 3]));
+        for (int s = 0; s < SUB; ++s) {
+            kwas[s] = reinterpret_cast<const uint4*>(kc + s * kCodeTile)[tid];
+            vwas[s] = reinterpret_cast<const uint4*>(vc + s * kCodeTile)[vchunk];
         }
-    km = wave_max(km);
-    vm = wave_max(vm);
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+        km = k[s].most(km);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vm = v[s][i].most(vm);
+    }
+    km = Raw<T, 4>::end(km);
+    vm = Raw<T, 4>::end(vm);
+    km = wave_max_all_u32(km);
+    vm = wave_max_all_u32(vm);
     if (lane == 0) {
         most[0][wave] = km;
         most[1][wave] = vm;
     }
-    const float kold = keeps ? p.c.k_scale[blk] : 0.f, vold = keeps ? p.c.v_scale[blk] : 0.f;
-    __syncthreads();   // (the scales before are read by every thread by now)
+    __syncthreads();   // (what the block held is read by every thread by now)
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         km = max(km, most[0][w]);
@@ -219,18 +270,26 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
     kq.init(new_scale<FP8>(km, keeps, kold));
     vq.init(new_scale<FP8>(vm, keeps, vold));
 
-    float sum[16];
+    // a block of zeros or of NaN: codes of zeros
+    if (kq.inv == 0.f)
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) k[s].clear();
+    if (vq.inv == 0.f)
+#pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[s][i].clear();
+
+    float sum[16], norm = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[i] = 0.f;
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
         float y[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = kq.inv > 0.f ? kq.quotient(k[s][i]) : 0.f;
-        uint4* chunk = reinterpret_cast<uint4*>(kc + s * kCodeTile) + tid;
+        for (int i = 0; i < 16; ++i) y[i] = kq.quotient(k[s][i]);
         if (keeps && 64 * s + kkey < begin) {
-            const uint4 u = *chunk;
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const uint32_t w[4] = {kwas[s].x, kwas[s].y, kwas[s].z, kwas[s].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float4 c = codes_f32<FP8>(w[i]);
@@ -239,28 +298,29 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
             }
         }
         uint32_t w[4];
+        float square = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             w[i] = pack_codes<FP8>(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
             const float4 c = codes_f32<FP8>(w[i]);
             sum[4 * i] += c.x; sum[4 * i + 1] += c.y; sum[4 * i + 2] += c.z; sum[4 * i + 3] += c.w;
+            square = fmaf(c.x, c.x, fmaf(c.y, c.y, fmaf(c.z, c.z, fmaf(c.w, c.w, square))));
         }
-        *chunk = make_uint4(w[0], w[1], w[2], w[3]);
+        norm = fmaxf(norm, square);
+        reinterpret_cast<uint4*>(kc + s * kCodeTile)[tid] = make_uint4(w[0], w[1], w[2], w[3]);
 
         uint32_t x[4];
-        uint32_t was[4] = {0, 0, 0, 0};
+        uint32_t was[4];
         const bool kept = keeps && 64 * s + vkey < begin;
-        if (kept)   // word d: dim vdim + d of this lane's four tokens
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const int vdd = vdim + d, from = (((wave >> 1) * 2 + (vdd >> 5)) * 2 + (wave & 1)) * 32 + (vdd & 31);
-                was[d] = *reinterpret_cast<const uint32_t*>(vc + s * kCodeTile + 16 * from + 4 * (lane & 3));
-            }
+        if (keeps) {   // word d: dim vdim + d of this lane's four tokens
+            was[0] = vwas[s].x; was[1] = vwas[s].y; was[2] = vwas[s].z; was[3] = vwas[s].w;
+            quad_transpose(was);
+        }
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             float z[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = vq.inv > 0.f ? vq.quotient(v[s][i][d]) : 0.f;
+            for (int i = 0; i < 4; ++i) z[i] = vq.quotient(v[s][i][d]);
             if (kept) {
                 const float4 c = codes_f32<FP8>(was[d]);
                 const float old[4] = {c.x, c.y, c.z, c.w};
@@ -275,20 +335,21 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
     }
 
     // the keys' mean: the sixteen sums over the 32 rows of a half wave, each exchange halving what a lane holds
-#pragma unroll
-    for (int d = 16, n = 16; d > 1; d >>= 1, n >>= 1) {
-        const bool upper = lane & d;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (i >= n / 2) break;
-            const float give = upper ? sum[i] : sum[i + n / 2];
-            sum[i] = (upper ? sum[i + n / 2] : sum[i]) + __shfl_xor(give, d);
-        }
-    }
-    sum[0] += __shfl_xor(sum[0], 1);
+    halve_sums<8, 16>(sum, lane & 16);
+    halve_sums<4, 8>(sum, lane & 8);
+    halve_sums<2, 4>(sum, lane & 4);
+    halve_sums<1, 2>(sum, lane & 2);
+    sum[0] += lane_xor<1>(sum[0]);
     // lane bits 4..1 chose the dim: bit 4 the upper eight of sixteen, and so on
     const int dim = kdim + 8 * ((lane >> 4) & 1) + 4 * ((lane >> 3) & 1) + 2 * ((lane >> 2) & 1) + ((lane >> 1) & 1);
     if ((lane & 1) == 0) sums[wave >> 1][dim] = sum[0];
+    // the largest part of 16 dims of a key's square, for each of the four parts
+    norm = fmaxf(norm, lane_xor<1>(norm));
+    norm = fmaxf(norm, lane_xor<2>(norm));
+    norm = fmaxf(norm, lane_xor<4>(norm));
+    norm = fmaxf(norm, lane_xor<8>(norm));
+    norm = fmaxf(norm, lane_xor<16>(norm));
+    if ((lane & 31) == 0) norms[wave >> 1][(wave & 1) * 2 + (lane >> 5)] = norm;
     __syncthreads();
     if (tid < 32) {
         // (the mean of the codes first: their sum times the scale need not fit)
@@ -297,8 +358,12 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
         static_cast<uint32_t*>(p.c.k_mean)[blk * 32 + tid] = pack_bf16x2(a, c);
     }
     if (tid == 0) {
+        float square = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) square += fmaxf(norms[0][i], norms[1][i]);
         p.c.k_scale[blk] = kq.scale;
         p.c.v_scale[blk] = vq.scale;
+        p.c.k_norm[blk] = sqrtf(square) * kq.scale;
     }
 }
 

@@ -45,8 +45,9 @@ class KVCache:
 
     The lengths of the sequences are the program's own (``kv_lens`` of the attention).  ``k_scale`` and
     ``v_scale`` (float32 [batch, num_blocks, kv_heads]), ``k_mean`` (bfloat16 [batch, num_blocks, kv_heads,
-    64], the mean of the keys of each block: ``k_cmp`` of ``query_topk``) and the codes, in an order of the
-    library's own, are tensors of the cache: ``kv_cache_write`` changes them in place.
+    64], the mean of the keys of each block: ``k_cmp`` of ``query_topk``), ``k_norm`` (float32 as the scales, not
+    below the norm of any key of the block, nor above twice the largest) and the codes, in an order of the library's
+    own, are tensors of the cache: ``kv_cache_write`` changes them in place.
     """
 
     def __init__(self, batch: int, capacity: int, kv_heads: int, block_size: int = 64, dtype: torch.dtype = torch.int8,
@@ -66,7 +67,7 @@ class KVCache:
         self._dtype = dtype
         shape = (batch, nb, kv_heads)
         self._k_codes, self._v_codes = (torch.zeros(*shape, block_size * 64, dtype=torch.uint8, device=device) for _ in range(2))
-        self._k_scale, self._v_scale = (torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2))
+        self._k_scale, self._v_scale, self._k_norm = (torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(3))
         self._k_mean = torch.zeros(*shape, 64, dtype=torch.bfloat16, device=device)
 
     batch = property(lambda self: self._sizes[0])
@@ -80,12 +81,13 @@ class KVCache:
     v_codes = property(lambda self: self._v_codes)
     k_scale = property(lambda self: self._k_scale)
     v_scale = property(lambda self: self._v_scale)
+    k_norm = property(lambda self: self._k_norm)
     k_mean = property(lambda self: self._k_mean)
 
     def _as_c(self) -> _lib.Cache:
         B, nb, Hk, bs, capacity = self._sizes
         return _lib.Cache(self._k_codes.data_ptr(), self._v_codes.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr(),
-                          self._k_mean.data_ptr(), B, nb, Hk, bs, _CODES[self._dtype], capacity)
+                          self._k_norm.data_ptr(), self._k_mean.data_ptr(), B, nb, Hk, bs, _CODES[self._dtype], capacity)
 
     def __repr__(self) -> str:
         B, _, Hk, bs, capacity = self._sizes

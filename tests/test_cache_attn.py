@@ -313,7 +313,7 @@ FAKE = 1 << 20
 
 def test_c_entry_refuses_arguments():
     L = _lib.lib()
-    c = ctypes.byref(_lib.Cache(FAKE, FAKE, FAKE, FAKE, FAKE, 2, 4, 3, 64, _lib.CODE_INT8, 250))
+    c = ctypes.byref(_lib.Cache(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 4, 3, 64, _lib.CODE_INT8, 250))
     rows = _lib.Bnhd(FAKE, 1920, 384, 64)
 
     def call(q=rows, idx=None, lens=None, n=5, hq=6, d=64, K=0, scale=0.0, out=FAKE, ws=FAKE, nbytes=1 << 40, cache=c):

@@ -37,6 +37,12 @@ def same(cache, model):
     assert torch.equal(got.isnan(), want.isnan())
     ok = (got - want).abs() <= (2.0 ** -8 + 2.0 ** -20) * want.abs() + 2.0 ** -133
     assert bool((ok | want.isnan()).all())
+    # the norm: four parts' squares of 16 terms, their root and a product in fp32 (24 roundings of 2^-24); parts of different keys
+    # make up at most four times one key's square
+    norm = (model.codes[0] * model.scale[0].repeat_interleave(model.bs, 1)[..., None]).square().sum(-1).sqrt().unflatten(1, (-1, model.bs)).amax(2)
+    got = cache.k_norm.cpu().double()
+    assert torch.equal(got.isnan(), norm.isnan())
+    assert bool(((got >= norm * (1 - 2.0 ** -19)) & (got <= 2 * norm * (1 + 2.0 ** -19)) | norm.isnan() | (norm > 3e38)).all())
 
 
 def made(B, capacity, H, bs, code):
@@ -319,14 +325,14 @@ FAKE = 1 << 20   # aligned host address; the checks fail before anything reads i
 
 
 def c_cache(**kw):
-    c = _lib.Cache(FAKE, FAKE, FAKE, FAKE, FAKE, 2, 4, 3, 64, _lib.CODE_INT8, 250)
+    c = _lib.Cache(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 4, 3, 64, _lib.CODE_INT8, 250)
     for name, x in kw.items():
         setattr(c, name, x)
     return c
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(k_codes=None), 1), (dict(v_codes=None), 1), (dict(k_scale=None), 1), (dict(v_scale=None), 1), (dict(k_mean=None), 1),
+    (dict(k_codes=None), 1), (dict(v_codes=None), 1), (dict(k_scale=None), 1), (dict(v_scale=None), 1), (dict(k_norm=None), 1), (dict(k_mean=None), 1),
     (dict(batch=0), 8), (dict(num_blocks=0), 8), (dict(num_kv_heads=0), 3), (dict(block_size=32), 4), (dict(block_size=192), 4),
     (dict(code_type=2), 11), (dict(capacity=257), 8), (dict(capacity=0), 8), (dict(k_codes=FAKE + 8), 7), (dict(k_scale=FAKE + 2), 7),
     (dict(k_mean=FAKE + 4), 7), (dict(num_blocks=1 << 26, capacity=1), 8), (dict(batch=1 << 30), 8),
