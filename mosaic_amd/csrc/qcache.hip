@@ -371,6 +371,7 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
 // the cache are zeros.
 template <typename T, bool FP8>
 __global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(CacheParams p) {
+    __shared__ uint4 keys[64][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x % p.c.num_kv_heads, rest = blockIdx.x / p.c.num_kv_heads, unit = rest % p.units, b = rest / p.units;
     const int64_t at = p.starts != nullptr ? p.starts[b] : p.start;
@@ -395,22 +396,24 @@ __global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(CacheParams p) 
     };
     auto times = [](float4 c, float s) { return make_float4(c.x * s, c.y * s, c.z * s, c.w * s); };
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int64_t tk = t0 + 32 * (wave >> 1) + key_of_row(lane & 31);
-    if (tk >= at && tk < at + p.n) {
-        T* out = row(p.k_out, tk, 32 * (wave & 1) + 16 * (lane >> 5));
-        const uint32_t w[4] = {k.x, k.y, k.z, k.w};
-        float4 x[4];
+    // keys: by way of LDS, so that a wave stores whole rows (64 bytes a token, its 16-byte chunks moved by token)
+    const int key = 32 * (wave >> 1) + key_of_row(lane & 31);
+    keys[key][(2 * (wave & 1) + (lane >> 5)) ^ (key >> 1 & 3)] = k;
+    __syncthreads();
+    constexpr int kDims = 16 / sizeof(T), kLanes = 64 / kDims;   // of one store, lanes of a row
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = tk >= 0 && tk < end ? times(codes_f32<FP8>(w[i]), ks) : zero;
+    for (int i = 0; i < 64 * kLanes / kThreads; ++i) {
+        const int token = tid / kLanes + i * (kThreads / kLanes), d = tid % kLanes * kDims;
+        const int64_t t = t0 + token;
+        if (t < at || t >= at + p.n) continue;
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(&keys[token][(d >> 4) ^ (token >> 1 & 3)]) + (d & 15);
+        const bool in = t >= 0 && t < end;
+        T* out = row(p.k_out, t, d);
         if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(pack_bf16x2(x[2 * i].x, x[2 * i].y), pack_bf16x2(x[2 * i].z, x[2 * i].w),
-                                                                    pack_bf16x2(x[2 * i + 1].x, x[2 * i + 1].y), pack_bf16x2(x[2 * i + 1].z, x[2 * i + 1].w));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Row4<T>::store(out + 4 * i, x[i]);
-        }
+            const uint2 u = ld8(from);
+            const float4 x = in ? times(codes_f32<FP8>(u.x), ks) : zero, y = in ? times(codes_f32<FP8>(u.y), ks) : zero;
+            *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w), pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+        } else Row4<T>::store(out, in ? times(codes_f32<FP8>(*reinterpret_cast<const uint32_t*>(from)), ks) : zero);
     }
     uint32_t w[4] = {v.x, v.y, v.z, v.w};
     quad_transpose(w);   // word d: dim vdim + d of tokens vkey ..
