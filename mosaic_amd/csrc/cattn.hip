@@ -6,18 +6,20 @@
 //   k_u = ks code, v_u = vs code, ks and vs the scales of u's block and head
 // Codes are whole numbers of at most 8 bits or e4m3, exact in bf16, so the products are of bf16 operands
 // without a rounding of theirs.  ks goes into the factor of the scores and vs into the exponent,
-//   P = exp2(c ks q.code_k + log2(vs / w) - m),  O = sum P code_v,  l = sum P w / vs,  o = w O / l,
-// so that neither costs an instruction per score (w: a scale that a workgroup takes first).  fp32 scores,
-// maxima, sums and accumulators; P is rounded to bf16 for the product with the values (half a step of
-// bf16 per term, as the output's own rounding), and l sums the rounded P.
+//   P = exp2(c ks q.code_k - m + log2 vs),  O = sum P code_v,  l = sum P / vs,  o = O / l,
+// so that neither costs an instruction per score.  fp32 scores, maxima, sums and accumulators; P is rounded to
+// bf16 for the product with the values (half a step of bf16 per term, as the output's own rounding), and l sums
+// the rounded P.
 //
 // A workgroup takes 4 waves x QW = 32 / G tokens of one kv head, a wave the 32 rows (token, head) of
 // its tokens; the codes of 64 keys are converted once, by all four waves, into operand order in LDS.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "bsa_common.h"
 #include "lds_dma.h"
@@ -32,8 +34,11 @@ struct CacheAttnParams : QuerySets {
     mosaic_kv_cache cache;
     const bf16_t* q; int64_t q_sb, q_sn, q_sh;
     bf16_t* out;               // [B, Nq, Hq, 64]
-    float* part_o;             // [splits, rows, 64] (splits > 1): o of a split's keys
-    float2* part_ml;           // [splits, rows] (m, l): 2^m l is the sum of its weights, l in [1, 2), or 0
+    float* part_o;             // [splits, parts, 64] (splits > 1): o of a split's keys
+    float2* part_ml;           // [splits, parts] (m, l): 2^m l is the sum of its weights, l in [0.5, 1), or 0
+    int64_t* part_at;          // [parts] the row that a part belongs to, or -1
+    int64_t parts;             // rows that are joined
+    int whole;                 // tiles of rows that one workgroup takes with all of their keys
     float c;
 };
 
@@ -45,19 +50,21 @@ struct CacheTile {
 struct DenseLds { CacheTile tile[2]; };
 struct SetsLds : UnionLds { CacheTile tile[2]; };
 
-// What a lane holds of the 64 blocks of a list: the block, its members among the wave's tokens, and the factors
-struct BlockLane {
-    int block, members;
-    float ck;        // c ks
-    float lv, iv;    // log2(vs / w) and w / vs; SAFE: vs and 1
-};
-
 struct AttnState {
     f32x16 o[2];      // O^T [dim tile]
-    float m, l;       // reference, and this lane's part of the sum
+    float m, l;       // reference of the scores, and this lane's part of the sum
+    bool has;         // a key above -inf was met
+    bool wide;        // so was a scale of values that kSafe is for
 };
 
-__device__ __forceinline__ int seq_tokens(const CacheAttnParams& p, int b) { return seq_keys(p, b); }
+// How a tile is computed.  kBounded: no score exceeds kBound (|q| and the blocks' norms say so): the reference
+// is 0.  kRunning: it is 0 too unless a score leaves +- kBound, and moves then, so that a row's bits do not
+// depend on the form, nor so on the rows beside it.  kSafe: for rows that end with a value that is not finite,
+// and for scales of values further than kSpread from 1: the reference is the maximum, and a row's
+// accumulators take nothing from a block that it has not, not even 0 * NaN.
+enum Form { kBounded, kRunning, kSafe };
+constexpr float kBound = 56.f;
+constexpr float kSpread = 0x1p30f;   // P stays within 2^86, its sums over 2^31 codes up to 448 within 2^126
 
 // x a + b in two roundings
 __device__ __forceinline__ float times_plus(float x, float a, float b) {
@@ -66,96 +73,124 @@ __device__ __forceinline__ float times_plus(float x, float a, float b) {
     return y + b;
 }
 
+// Scores of tokens at or past `left` of a lane's 16 become -inf
+__device__ __forceinline__ void mask_scores(f32x16& s, int left) {
+    asm volatile("" : "+v"(left));   // (opaque, or the comparisons of all calls are kept at once)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = e < left ? s[e] : -INFINITY;
+}
+
+// P of 8 scores, as an operand
+template <Form F>
+__device__ __forceinline__ bf16x8 weights(const f32x16& s, int s2, float ck, float ref) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = s[8 * s2 + 2 * i], y = s[8 * s2 + 2 * i + 1];
+        // (of scores past 2^30 the fused form leaves more than fp32's exponents beside their rounded maximum)
+        w[i] = F == kSafe ? pack_bf16x2(__builtin_amdgcn_exp2f(times_plus(x, ck, ref)), __builtin_amdgcn_exp2f(times_plus(y, ck, ref)))
+                          : pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(x, ck, ref)), __builtin_amdgcn_exp2f(fmaf(y, ck, ref)));
+    }
+    return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// Factors of a block's scales: scores by ck = c ks; P times 2^lv = vs, and iv = 1 / vs for the sum of P (kSafe:
+// lv = vs itself, iv an addend of the scores that is 0 or NaN).  A scale of 0 stands for zeros only: any
+// positive one does.  A NaN among them goes where only the members of the block meet it.
+struct Factors { float ck, lv, iv; };
 template <bool SAFE>
-__device__ __forceinline__ void attend_tile(const CacheTile& t, const bf16x8 (&qf)[4], bool member, int valid, float ck, float lv, float iv,
-                                            AttnState& a) {
+__device__ __forceinline__ Factors factors(float c, float ks, float vs, bool& wide) {
+    Factors f;
+    f.ck = ks > 0.f ? fminf(fmaxf(c * ks, FLT_MIN), FLT_MAX) : 1.f;
+    const float poison = ks - ks;
+    wide = false;
+    if constexpr (SAFE) {
+        f.lv = vs;
+        f.iv = poison;
+    } else {
+        const bool near = vs <= kSpread && vs >= 1.f / kSpread;
+        wide = !near && vs != 0.f;   // (a NaN too: kSafe leaves it a NaN)
+        const float of = near ? vs : 1.f;
+        f.lv = __builtin_amdgcn_logf(of) + poison;
+        f.iv = 1.f / of;
+    }
+    return f;
+}
+
+struct TileRead {
+    const CacheTile& t;
+    int lane;
+    __device__ __forceinline__ bf16x8 key(int kt, int ds) const { return as_bf16x8(ld16(t.K + ((kt * 4 + ds) * 64 + lane) * 8)); }
+    __device__ __forceinline__ bf16x8 val(int kt, int dt, int s2) const { return as_bf16x8(ld16(t.V + (((kt * 2 + dt) * 2 + s2) * 64 + lane) * 8)); }
+};
+
+// One tile of 64 keys; valid: how many of them exist.
+template <Form F>
+__device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 (&qf)[4], bool member, int valid, const Factors& f, AttnState& a) {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
-    auto keys = [&](int kt, int ds) { return as_bf16x8(ld16(t.K + ((kt * 4 + ds) * 64 + lane) * 8)); };
-    auto vals = [&](int kt, int dt, int s2) { return as_bf16x8(ld16(t.V + (((kt * 2 + dt) * 2 + s2) * 64 + lane) * 8)); };
+    const TileRead t{tile, lane};
     f32x16 s[2] = {splat(0.f), splat(0.f)};
 #pragma unroll
     for (int ds = 0; ds < 4; ++ds)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma32(keys(kt, ds), qf[ds], s[kt]);
+        for (int kt = 0; kt < 2; ++kt) s[kt] = mfma32(t.key(kt, ds), qf[ds], s[kt]);
     if (valid < 64) {
         seldom();
+        mask_scores(s[0], valid - 16 * hh);
+        mask_scores(s[1], valid - 32 - 16 * hh);
+    }
+    if constexpr (F != kBounded) {
+        float mt = s[0][0];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            int left = valid - 32 * kt - 16 * hh;
-            asm volatile("" : "+v"(left));
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[kt][e] = e < left ? s[kt][e] : -INFINITY;
+            for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
+        mt = xor32_max(mt) * f.ck;
+        const bool some = member && mt > -INFINITY;
+        const bool move = some && (F == kSafe ? !a.has || mt > a.m : mt > a.m + kBound || (!a.has && mt < -kBound));
+        if (__builtin_amdgcn_ballot_w64(move)) {
+            const float alpha = move && a.has ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
+            a.m = move ? mt : a.m;
+            a.o[0] *= alpha;
+            a.o[1] *= alpha;
+            a.l *= alpha;
         }
+        a.has = a.has || some;
     }
-    float mt = s[0][0];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
-    const float shift = SAFE ? 0.f : lv;
-    mt = fmaf(xor32_max(mt), ck, shift);
-    const bool move = member && mt > a.m + kTau;
-    if (__builtin_amdgcn_ballot_w64(move)) {
-        const float alpha = move ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
-        a.m = move ? mt : a.m;
-        a.o[0] *= alpha;
-        a.o[1] *= alpha;
-        a.l *= alpha;
-    }
-    const float ref = member ? shift - a.m : -INFINITY;   // P = 0 for the others
-    // (of scores past 2^30 the fused form leaves more than fp32's exponents beside their rounded maximum)
-    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(SAFE ? times_plus(x, ck, ref) : fmaf(x, ck, ref)); };
+    const float ref = member ? (F == kSafe ? f.iv : f.lv) - a.m : -INFINITY;   // P = 0 for the others
     bf16x8 pb[2][2];
-    float lt[2] = {0.f, 0.f};
+    float lt = 0.f;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = pack_bf16x2(weight(s[kt][8 * s2 + 2 * i]), weight(s[kt][8 * s2 + 2 * i + 1]));
-            }
-            pb[kt][s2] = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-            lt[kt] = operand_sum(pb[kt][s2], lt[kt]);
+            pb[kt][s2] = weights<F>(s[kt], s2, f.ck, ref);
+            lt = operand_sum(pb[kt][s2], lt);
         }
-    if constexpr (SAFE) {
-        if (member) a.l += lt[0] + lt[1];
+    if constexpr (F == kSafe) {
+        if (member) a.l += lt;
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) {
             f32x16 y = splat(0.f);
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) y = mfma32(vals(kt, dt, s2), pb[kt][s2], y);
+                for (int s2 = 0; s2 < 2; ++s2) y = mfma32(t.val(kt, dt, s2), pb[kt][s2], y);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) a.o[dt][e] = member ? fmaf(y[e], lv, a.o[dt][e]) : a.o[dt][e];
+            for (int e = 0; e < 16; ++e) a.o[dt][e] = member ? fmaf(y[e], f.lv, a.o[dt][e]) : a.o[dt][e];
         }
     } else {
-        a.l = fmaf(lt[0] + lt[1], iv, a.l);
+        a.l = fmaf(lt, f.iv, a.l);
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(vals(kt, dt, s2), pb[kt][s2], a.o[dt]);
+                for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(t.val(kt, dt, s2), pb[kt][s2], a.o[dt]);
     }
 }
 
-// Factors of a block's scales.  A scale of 0 stands for zeros only: any positive one does.
-__device__ __forceinline__ float score_factor(float c, float ks) {
-    return ks == 0.f ? 1.f : fminf(fmaxf(c * ks, FLT_MIN), FLT_MAX) + (ks - ks);   // (NaN stays)
-}
-
-__device__ __forceinline__ float wave_max_f(float x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
-}
-
-// Scales of values further than 2^60 from w are for the SAFE form.
-constexpr float kSpread = 0x1p60f;
-
+// The loop over the tiles of a workgroup's blocks
 template <bool FP8, bool SAFE, typename Lds>
 struct Walk {
     const CacheAttnParams& p;
@@ -164,43 +199,40 @@ struct Walk {
     const bf16x8 (&qf)[4];
     const Row& row;
     AttnState& a;
-    float w;        // 0: not chosen yet
-    bool narrow;    // all scales of values within kSpread of w so far
+    float qc;       // c |q| of the wave's rows at most
 
-    __device__ __forceinline__ void load(int block, int st, uint4& k, uint4& v) const {
-        const int64_t from = block_at(p.cache, b, block, h) * (p.bs * 64) + st * kCodeTile + 16 * threadIdx.x;
-        k = ld16(static_cast<const uint8_t*>(p.cache.k_codes) + from);
-        v = ld16(static_cast<const uint8_t*>(p.cache.v_codes) + from);
+    struct Staged { uint4 k, v; };   // a thread's 16 codes of either
+    __device__ __forceinline__ void load(int block, int st, Staged& r) const {
+        const uint32_t at = 16u * threadIdx.x;
+        const int64_t from = block_at(p.cache, b, block, h) * (p.bs * 64) + st * kCodeTile;
+        r.k = ld16(static_cast<const uint8_t*>(p.cache.k_codes) + from + at);
+        r.v = ld16(static_cast<const uint8_t*>(p.cache.v_codes) + from + at);
     }
     __device__ __forceinline__ static void expand(bf16_t* at, const uint4& u) {   // 16 codes: two operands of a lane
         const uint2 a = codes_bf16<FP8>(u.x), b = codes_bf16<FP8>(u.y), c = codes_bf16<FP8>(u.z), d = codes_bf16<FP8>(u.w);
         *reinterpret_cast<uint4*>(at) = make_uint4(a.x, a.y, b.x, b.y);
         *reinterpret_cast<uint4*>(at + 64 * 8) = make_uint4(c.x, c.y, d.x, d.y);
     }
-    __device__ __forceinline__ void put(int buf, const uint4& k, const uint4& v) const {
+    __device__ __forceinline__ void put(int buf, const Staged& r) const {
         const int tid = threadIdx.x, at = ((tid >> 6) * 2 * 64 + (tid & 63)) * 8;
-        expand(L.tile[buf].K + at, k);
-        expand(L.tile[buf].V + at, v);
+        expand(L.tile[buf].K + at, r.k);
+        expand(L.tile[buf].V + at, r.v);
     }
-    // up to 64 blocks, lane i < count holding the i-th
+    // up to 64 blocks, lane i < count holding the i-th and its members among the wave's tokens
     __device__ __forceinline__ void blocks(int count, int block, int members) {
-        const int lane = threadIdx.x & 63;
         const int64_t at = block_at(p.cache, b, block, h);
-        const float vs = p.cache.v_scale[at], ck = score_factor(p.c, p.cache.k_scale[at]);
-        float lv, iv;
-        if constexpr (SAFE) {
-            lv = vs;
-            iv = 1.f;
-        } else {
-            if (w == 0.f) {
-                w = wave_max_f(vs > 0.f && vs < INFINITY ? vs : 0.f);
-                if (w == 0.f) w = 1.f;
-            }
-            const float of = vs == 0.f ? w : vs;
-            narrow = narrow && !__builtin_amdgcn_ballot_w64(!(of <= w * kSpread && of >= w * (1.f / kSpread)));
-            iv = w / of;
-            lv = __builtin_amdgcn_logf(of / w);
+        bool wide;
+        const Factors f = factors<SAFE>(p.c, p.cache.k_scale[at], p.cache.v_scale[at], wide);
+        if constexpr (SAFE) tiles<kSafe>(count, block, members, f, 0);
+        else {
+            const uint64_t far = __builtin_amdgcn_ballot_w64(wide);
+            // (a NaN is not bounded; a wave by itself: the forms have the same barriers)
+            if (__builtin_amdgcn_ballot_w64(!(p.cache.k_norm[at] * qc <= kBound) || a.m != 0.f)) tiles<kRunning>(count, block, members, f, far);
+            else tiles<kBounded>(count, block, members, f, far);
         }
+    }
+    template <Form F>
+    __device__ __forceinline__ void tiles(int count, int block, int members, const Factors& f, uint64_t far) {
         auto key0 = [&](int i) { return __builtin_amdgcn_readlane(block, i) * p.bs; };
         auto next = [&](int& i, int& st) {   // the tile after (i, st); i = count: none
             if (st + 1 < sub && key0(i) + 64 * (st + 1) < end) ++st;
@@ -209,24 +241,28 @@ struct Walk {
                 st = 0;
             }
         };
-        uint4 kr, vr;
+        Staged r;
         int i = 0, st = 0, ni = 0, nst = 0;
-        load(__builtin_amdgcn_readlane(block, 0), 0, kr, vr);
-        put(0, kr, vr);
+        load(__builtin_amdgcn_readlane(block, 0), 0, r);
+        put(0, r);
         next(ni, nst);
-        if (ni < count) load(__builtin_amdgcn_readlane(block, ni), nst, kr, vr);
+        if (ni < count) load(__builtin_amdgcn_readlane(block, ni), nst, r);
         for (int buf = 0; i < count; buf ^= 1) {
             lds_barrier();
             int fi = ni, fst = nst;
             if (ni < count) {
-                put(buf ^ 1, kr, vr);
+                put(buf ^ 1, r);
                 next(fi, fst);
-                if (fi < count) load(__builtin_amdgcn_readlane(block, fi), fst, kr, vr);
+                if (fi < count) load(__builtin_amdgcn_readlane(block, fi), fst, r);
             }
             const uint32_t of = (uint32_t)__builtin_amdgcn_readlane(members, i);
             auto lane_f = [&](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), i)); };
-            if (of != 0)
-                attend_tile<SAFE>(L.tile[buf], qf, row.in(of), min(64, end - key0(i) - 64 * st), lane_f(ck), lane_f(lv), lane_f(iv), a);
+            if (of != 0) {
+                const bool member = row.in(of);
+                if (F == kBounded) a.has = a.has || member;
+                if (far >> i & 1) a.wide = a.wide || member;
+                attend_tile<F>(L.tile[buf], qf, member, min(64, end - key0(i) - 64 * st), Factors{lane_f(f.ck), lane_f(f.lv), lane_f(f.iv)}, a);
+            }
             i = ni; st = nst;
             ni = fi; nst = fst;
         }
@@ -234,25 +270,25 @@ struct Walk {
     }
 };
 
-template <bool FP8, bool DENSE, bool SAFE>
-__device__ __forceinline__ bool attend(const CacheAttnParams& p, std::conditional_t<DENSE, DenseLds, SetsLds>& L, int b, int h, int n0, int split,
-                                       const Row& row, const bf16x8 (&qf)[4], AttnState& a, float& w) {
+template <bool FP8, bool DENSE, bool SAFE, typename Lds>
+__device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, int h, int n0, int split, int splits, const Row& row, int wave_live,
+                                       float qc, const bf16x8 (&qf)[4], AttnState& a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     a.o[0] = a.o[1] = splat(0.f);
-    a.m = -FLT_MAX;   // finite, so that keys whose score is -inf are exp2(-inf) = 0 also before any other
-    a.l = 0.f;
-    const int end = seq_tokens(p, b);
-    Walk<FP8, SAFE, std::remove_reference_t<decltype(L)>> walk{p, L, b, h, end, p.bs / 64, qf, row, a, 0.f, true};
+    a.m = a.l = 0.f;
+    a.has = a.wide = false;
+    const int end = seq_keys(p, b);
+    Walk<FP8, SAFE, Lds> walk{p, L, b, h, end, p.bs / 64, qf, row, a, qc};
     const int live = (int)(((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
     if constexpr (DENSE) {
-        const int first = (int)((int64_t)live * split / p.splits), past = (int)((int64_t)live * (split + 1) / p.splits);
-        for (int e0 = first; e0 < past; e0 += 64) walk.blocks(min(64, past - e0), min(e0 + lane, past - 1), -1);
+        const int first = (int)((int64_t)live * split / splits), past = (int)((int64_t)live * (split + 1) / splits);
+        for (int e0 = first; e0 < past; e0 += 64) walk.blocks(min(64, past - e0), min(e0 + lane, past - 1), wave_live);
     } else {
         const bool by_block = p.keys != nullptr;
         for (int c0 = 0; c0 < live; c0 += kUnion) {
-            const int found = unite(p, L, b, h, n0, end, c0, min(kUnion, live - c0), split, by_block ? p.splits : 1);
-            const int first = by_block ? 0 : (int)((uint32_t)(found * split) / (uint32_t)p.splits);
-            const int past = by_block ? found : (int)((uint32_t)(found * (split + 1)) / (uint32_t)p.splits);
+            const int found = unite(p, L, b, h, n0, end, c0, min(kUnion, live - c0), split, by_block ? splits : 1);
+            const int first = by_block ? 0 : (int)((uint32_t)(found * split) / (uint32_t)splits);
+            const int past = by_block ? found : (int)((uint32_t)(found * (split + 1)) / (uint32_t)splits);
             for (int e0 = first; e0 < past; e0 += 64) {
                 const int count = min(64, past - e0), u = L.list[e0 + min(lane, count - 1)];
                 walk.blocks(count, c0 + u, (int)L.members[u][wave]);
@@ -260,18 +296,45 @@ __device__ __forceinline__ bool attend(const CacheAttnParams& p, std::conditiona
             __syncthreads();
         }
     }
-    w = SAFE || walk.w == 0.f ? 1.f : walk.w;
-    return walk.narrow;
+}
+
+// The result of a row, or its part of it
+__device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row, int64_t part, int split, int splits, AttnState& a) {
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
+    const float l = xor32_add(a.l), f = l == 0.f ? 0.f : 1.f / l;   // (a row without a key, or with none above -inf: zeros)
+    if (splits == 1) {
+        store_row(p.out, row.at, lane, a.o, f);
+        return;
+    }
+    float* d = p.part_o + (split * p.parts + part) * 64 + 4 * hh;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+            *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) =
+                make_float4(a.o[dt][4 * g4] * f, a.o[dt][4 * g4 + 1] * f, a.o[dt][4 * g4 + 2] * f, a.o[dt][4 * g4 + 3] * f);
+    if (hh == 0) {
+        int e = 0;
+        const float y = frexpf(l, &e);   // (NaN and infinity stay what they are)
+        p.part_ml[split * p.parts + part] = make_float2(a.m + (float)e, y);
+    }
 }
 
 template <bool FP8, bool DENSE>
-__global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(CacheAttnParams p, int total) {
+__global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(CacheAttnParams p) {
     __shared__ std::conditional_t<DENSE, DenseLds, SetsLds> L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_runs(blockIdx.x, total);
-    const int split = id % p.splits, tile_id = id / p.splits % p.qtiles, rest = id / p.splits / p.qtiles;
-    const int h = rest % p.Hk, b = rest / p.Hk;
+    // whole tiles of rows, then the others, each with its keys in shares
+    int split = 0, splits = 1, tile = blockIdx.x;
+    if ((int)blockIdx.x < p.whole) tile = xcd_runs(blockIdx.x, p.whole);
+    else {
+        const int i = blockIdx.x - p.whole;
+        splits = p.splits;
+        tile = p.whole + i / splits;
+        split = i % splits;
+    }
+    const int tile_id = tile % p.qtiles, rest = tile / p.qtiles, h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * kWaves * p.QW;
     Row row;
     if constexpr (DENSE) row.init(p, [&](int i) { return min(n0 + i, p.Nq - 1); }, b, h, n0, wave, lane & 31);
@@ -284,32 +347,26 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(CacheAttnParams
 #pragma unroll
     for (int ds = 0; ds < 4; ++ds) qf[ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
     arrived(qf);
-    AttnState a;
-    float w;
-    bool ok = attend<FP8, DENSE, false>(p, L, b, h, n0, split, row, qf, a, w);
-    ok = ok && finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f;
-    if (__syncthreads_or(!ok)) attend<FP8, DENSE, true>(p, L, b, h, n0, split, row, qf, a, w);
-    const float l = xor32_add(a.l), f = l == 0.f ? 0.f : 1.f / l;
-    if (!row.live) return;
-    if (p.splits > 1) {
-        const int64_t rows = (int64_t)p.B * p.Nq * p.Hq;
-        float* d = p.part_o + (split * rows + row.at) * 64 + 4 * hh;
+    float qc = 0.f;   // of the norm, a little more than its roundings
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt)
+    for (int ds = 0; ds < 4; ++ds) {
+        const uint4 u = __builtin_bit_cast(uint4, qf[ds]);
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4)
-                *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) = make_float4(a.o[dt][4 * g4] * f * w, a.o[dt][4 * g4 + 1] * f * w,
-                                                                               a.o[dt][4 * g4 + 2] * f * w, a.o[dt][4 * g4 + 3] * f * w);
-        if (hh == 0) {
-            int e = 0;
-            const float part = frexpf(l, &e);   // (NaN and infinity stay what they are)
-            p.part_ml[split * rows + row.at] = make_float2(a.m + (float)e, part);
-        }
-        return;
+        for (int i = 0; i < 4; ++i) qc = fmaf(bf_lo(x[i]), bf_lo(x[i]), fmaf(bf_hi(x[i]), bf_hi(x[i]), qc));
     }
-#pragma unroll
-    for (int dt = 0; dt < 2; ++dt) a.o[dt] *= f;   // (before w: 1 / l and w / l need not fit together)
-    store_row(p.out, row.at, lane, a.o, w);
+    qc = wave_max_nonneg(sqrtf(xor32_add(qc))) * p.c * 1.001f;
+    const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
+    const int64_t part = (int64_t)(tile - p.whole) * (kWaves * kRows) + wave * kRows + (lane & 31);
+    if (splits > 1 && split == 0 && hh == 0) p.part_at[part] = row.live ? row.at : -1;
+    AttnState a;
+    attend<FP8, DENSE, false>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
+    const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
+    const bool ok = fine && __shfl_xor((int)fine, 32);   // (both halves of the row)
+    if (row.live && ok) put_row(p, row, part, split, splits, a);
+    if (!__syncthreads_or(!ok)) return;
+    attend<FP8, DENSE, true>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
+    if (row.live && !ok) put_row(p, row, part, split, splits, a);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -324,6 +381,7 @@ constexpr int kFewRows = 16, kFewEntries = 64;
 struct FewState {
     f32x4 o[4];       // O^T [16 dims]: dims 16 dg + 4 g + i
     float m, l;
+    bool has, wide;   // as AttnState's
 };
 struct Codes { uint4 k[4], v[4]; float ks, vs; };
 
@@ -343,17 +401,11 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
 }
 
 template <bool FP8, bool SAFE>
-__device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2], bool member, int valid, float c, float& w, bool& narrow, FewState& a) {
+__device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2], bool member, int valid, float c, FewState& a) {
     const int g = (threadIdx.x & 63) >> 4;
-    const float ck = score_factor(c, t.ks);
-    float lv = t.vs, iv = 1.f;
-    if constexpr (!SAFE) {
-        if (w == 0.f && t.vs > 0.f && t.vs < INFINITY) w = t.vs;
-        const float base = w == 0.f ? 1.f : w, of = t.vs == 0.f ? base : t.vs;
-        narrow = narrow && of <= base * kSpread && of >= base * (1.f / kSpread);
-        iv = base / of;
-        lv = __builtin_amdgcn_logf(of / base);
-    }
+    bool wide;
+    const Factors f = factors<SAFE>(c, t.ks, t.vs, wide);
+    a.wide = a.wide || (wide && member);
     f32x4 s[4];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
@@ -374,18 +426,18 @@ __device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2]
     for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mt = __builtin_elementwise_maximum(mt, s[m][i]);
-    const float shift = SAFE ? 0.f : lv;
-    mt = fmaf(xor32_max(xor16_max(mt)), ck, shift);
-    const bool move = member && mt > a.m + kTau;
+    mt = xor32_max(xor16_max(mt)) * f.ck;
+    const bool some = member && mt > -INFINITY, move = some && (!a.has || mt > a.m + (SAFE ? 0.f : kTau));
     if (__builtin_amdgcn_ballot_w64(move)) {
-        const float alpha = move ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
+        const float alpha = move && a.has ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
         a.m = move ? mt : a.m;
 #pragma unroll
         for (int dg = 0; dg < 4; ++dg) a.o[dg] *= alpha;
         a.l *= alpha;
     }
-    const float ref = member ? shift - a.m : -INFINITY;   // P = 0 for the others
-    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(SAFE ? times_plus(x, ck, ref) : fmaf(x, ck, ref)); };
+    a.has = a.has || some;
+    const float ref = member ? (SAFE ? f.iv : f.lv) - a.m : -INFINITY;   // P = 0 for the others
+    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(SAFE ? times_plus(x, f.ck, ref) : fmaf(x, f.ck, ref)); };
     bf16x8 pb[2];
     float lt = 0.f;
 #pragma unroll
@@ -398,14 +450,14 @@ __device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2]
     }
     if constexpr (SAFE) {
         if (member) a.l += lt;
-    } else a.l = fmaf(lt, iv, a.l);
+    } else a.l = fmaf(lt, f.iv, a.l);
 #pragma unroll
     for (int dg = 0; dg < 4; ++dg) {
         const bf16x8 v0 = codes8<FP8>(t.v[dg].x, t.v[dg].y), v1 = codes8<FP8>(t.v[dg].z, t.v[dg].w);
         if constexpr (SAFE) {
             const f32x4 y = mfma16(v1, pb[1], mfma16(v0, pb[0], f32x4{0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a.o[dg][i] = member ? fmaf(y[i], lv, a.o[dg][i]) : a.o[dg][i];
+            for (int i = 0; i < 4; ++i) a.o[dg][i] = member ? fmaf(y[i], f.lv, a.o[dg][i]) : a.o[dg][i];
         } else a.o[dg] = mfma16(v1, pb[1], mfma16(v0, pb[0], a.o[dg]));
     }
 }
@@ -476,15 +528,11 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
         t.vs = p.cache.v_scale[at];
     };
     FewState a;
-    float w;
-    bool narrow;
     auto walk = [&](auto safe) {
-        w = 0.f;
-        narrow = true;
 #pragma unroll
         for (int dg = 0; dg < 4; ++dg) a.o[dg] = f32x4{0.f, 0.f, 0.f, 0.f};
-        a.m = -FLT_MAX;
-        a.l = 0.f;
+        a.m = a.l = 0.f;
+        a.has = a.wide = false;
         if (first + wave >= past) return;
         Codes next;
         uint32_t of_next;
@@ -499,12 +547,11 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
                 load(min(key_next, end - 1), next);
             }
             if (key0 < end)
-                attend_few<FP8, decltype(safe)::value>(t, qf, row_live && (DENSE || (of >> token & 1)), min(64, end - key0), p.c, w, narrow, a);
+                attend_few<FP8, decltype(safe)::value>(t, qf, row_live && (DENSE || (of >> token & 1)), min(64, end - key0), p.c, a);
         }
-        if (decltype(safe)::value || w == 0.f) w = 1.f;
     };
     walk(std::false_type{});
-    bool ok = narrow && a.l - a.l == 0.f;
+    bool ok = !a.wide && a.l - a.l == 0.f;
 #pragma unroll
     for (int dg = 0; dg < 4; ++dg)
 #pragma unroll
@@ -514,7 +561,7 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
 #pragma unroll
     for (int dg = 0; dg < 4; ++dg)
         *reinterpret_cast<float4*>(&O[wave][r][(16 * dg + 4 * g) ^ (4 * r)]) =
-            make_float4(a.o[dg][0] * f * w, a.o[dg][1] * f * w, a.o[dg][2] * f * w, a.o[dg][3] * f * w);
+            make_float4(a.o[dg][0] * f, a.o[dg][1] * f, a.o[dg][2] * f, a.o[dg][3] * f);
     if (g == 0) {
         int e = 0;
         const float part = frexpf(l, &e);
@@ -544,12 +591,11 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
         *reinterpret_cast<uint2*>(p.out + at * 64 + d) = make_uint2(pack_bf16x2(o.x * y, o.y * y), pack_bf16x2(o.z * y, o.w * y));
         return;
     }
-    const int64_t all = (int64_t)p.B * p.Nq * p.Hq;
-    *reinterpret_cast<float4*>(p.part_o + (split * all + at) * 64 + d) = make_float4(o.x * y, o.y * y, o.z * y, o.w * y);
+    *reinterpret_cast<float4*>(p.part_o + (split * p.parts + at) * 64 + d) = make_float4(o.x * y, o.y * y, o.z * y, o.w * y);
     if (d == 0) {
         int e = 0;
         const float part = frexpf(sum, &e);
-        p.part_ml[split * all + at] = make_float2(m + (float)e, part);
+        p.part_ml[split * p.parts + at] = make_float2(m + (float)e, part);
     }
 }
 
@@ -558,11 +604,13 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
 // Joins the splits' partials: 16 lanes a row, 4 dims each, and TEAM such groups a row that take its splits
 // in turn (of few splits one, of many all 16 of a workgroup).
 template <int TEAM>
-__global__ __launch_bounds__(kThreads) void cache_attn_join_kernel(CacheAttnParams p, int64_t rows) {
+__global__ __launch_bounds__(kThreads) void cache_attn_join_kernel(CacheAttnParams p) {
     __shared__ __attribute__((aligned(16))) float4 part[16][16];
     __shared__ float ml[16], sums[16];
     const int group = threadIdx.x / 16, j = threadIdx.x % 16, d = 4 * j, of = group % TEAM;
-    const int64_t at = (int64_t)blockIdx.x * (16 / TEAM) + group / TEAM, row = at < rows ? at : rows - 1;
+    const int64_t rows = p.parts, mine = (int64_t)blockIdx.x * (16 / TEAM) + group / TEAM, row = mine < rows ? mine : rows - 1;
+    const int64_t at = p.part_at != nullptr ? p.part_at[row] : row;
+    if (TEAM > 1 && at < 0) return;   // (all of a workgroup)
     float m = -INFINITY;
     for (int s = of + TEAM * j; s < p.splits; s += 16 * TEAM) {
         const float2 x = p.part_ml[s * rows + row];
@@ -600,9 +648,9 @@ __global__ __launch_bounds__(kThreads) void cache_attn_join_kernel(CacheAttnPara
             o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
         }
     }
-    if (at >= rows) return;
+    if (mine >= rows || at < 0) return;
     const float f = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2*>(p.out + row * 64 + d) = make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
+    *reinterpret_cast<uint2*>(p.out + at * 64 + d) = make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
 }
 
 // ------------------------------------------------------------------ host
@@ -624,33 +672,44 @@ int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, 
 
 constexpr int64_t kFewGroups = 1024, kFewTiles = 2;
 
-int64_t groups_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq) {
-    const int64_t per = kWaves * (kRows / (hq / c.num_kv_heads));
-    return (nq + per - 1) / per * c.num_kv_heads * c.batch;
-}
 // Whether the call is one of cache_attn_few_kernel
 bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     const int64_t rows = (int64_t)nq * (hq / c.num_kv_heads);
     return rows <= kFewRows && (int64_t)nq * K <= kFewEntries;
 }
-// Shares of the keys: below one workgroup per CU they are split.
-int choose_split(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
-    const int64_t sub = c.block_size / 64;
+
+// How a call is laid out: tiles of rows, those taken whole, and shares of the others' keys.
+struct Plan {
+    int64_t qtiles, tiles, whole, splits, parts;   // tiles of a (member, kv head), and of all; rows that are joined
+    size_t part_o, part_ml, part_at, bytes;        // places in the workspace, and what the partials take of it
+};
+Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
+    Plan a{};
+    const int G = hq / c.num_kv_heads;
+    const int64_t heads = (int64_t)c.num_kv_heads * c.batch, sub = c.block_size / 64;
     if (few(c, nq, hq, K)) {
-        const int64_t wgs = (int64_t)c.num_kv_heads * c.batch, tiles = K > 0 ? nq * K * sub : c.num_blocks * sub;
-        const int64_t s = kFewGroups / wgs, most = tiles / (kWaves * kFewTiles);
-        const int64_t n = s < most ? s : most;
-        return (int)(n < 1 ? 1 : n);
+        const int64_t tiles = K > 0 ? nq * K * sub : c.num_blocks * sub;
+        a.tiles = heads;
+        a.splits = std::max<int64_t>(1, std::min(kFewGroups / heads, tiles / (kWaves * kFewTiles)));
+        a.parts = (int64_t)c.batch * nq * hq;
+    } else {
+        const int64_t most = K > 0 ? std::min(K, kMaxSplit) : std::max<int64_t>(1, c.num_blocks / 4);
+        const int64_t per = kWaves * (kRows / G), slots = K > 0 ? 512 : 768;
+        a.qtiles = (nq + per - 1) / per;
+        a.tiles = a.qtiles * heads;
+        // full rounds of the chip, and the rest's keys in shares that fill it once more (sets: where there is no full round)
+        a.whole = K > 0 ? (a.tiles >= 256 ? a.tiles : 0) : a.tiles / slots * slots;
+        const int64_t rest = a.tiles - a.whole;
+        a.splits = rest > 0 ? std::max<int64_t>(1, std::min(slots / rest, most)) : 1;
+        if (a.splits == 1) a.whole = a.tiles;
+        a.parts = (a.tiles - a.whole) * kWaves * kRows;
     }
-    const int64_t wgs = groups_of(c, nq, hq), most = K > 0 ? (K < kMaxSplit ? K : kMaxSplit) : c.num_blocks;
-    if (wgs >= 256) return 1;
-    const int64_t s = (K > 0 ? 512 : 768) / wgs;
-    return (int)(s < most ? s : most);
-}
-size_t part_bytes(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
-    const int s = choose_split(c, nq, hq, K);
-    const size_t rows = s == 1 ? 0 : (size_t)c.batch * nq * hq;
-    return up(s * rows * kHeadDim * sizeof(float)) + up(s * rows * sizeof(float2));
+    if (a.splits > 1) {
+        a.part_ml = up(a.splits * a.parts * kHeadDim * sizeof(float));
+        a.part_at = a.part_ml + up(a.splits * a.parts * sizeof(float2));
+        a.bytes = a.part_at + up(a.parts * sizeof(int64_t));
+    }
+    return a;
 }
 
 }  // namespace
@@ -662,7 +721,7 @@ extern "C" {
 
 size_t mosaic_cache_attn_fwd_workspace_size(const mosaic_kv_cache* cache, int32_t num_queries, int32_t num_q_heads, int32_t block_count) {
     if (check_call(cache, num_queries, num_q_heads, kHeadDim, block_count) != MOSAIC_OK) return 0;
-    return part_bytes(*cache, num_queries, num_q_heads, block_count) +
+    return plan_of(*cache, num_queries, num_q_heads, block_count).bytes +
            (block_count > 0 && !few(*cache, num_queries, num_q_heads, block_count) ? order_bytes(cache->batch, num_queries, num_q_heads, cache->num_kv_heads) : 0);
 }
 
@@ -683,36 +742,37 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     p.idx = block_indices; p.lens = kv_lens;
     p.B = cache->batch; p.Nq = num_queries; p.Nk = cache->capacity; p.Hq = num_q_heads; p.Hk = cache->num_kv_heads;
     p.G = p.Hq / p.Hk; p.QW = kRows / p.G; p.bs = cache->block_size; p.K = block_count; p.nb = cache->num_blocks;
-    p.qtiles = (num_queries + kWaves * p.QW - 1) / (kWaves * p.QW);
     p.qw_inverse = (65536 + p.QW - 1) / p.QW;
-    p.splits = choose_split(*cache, num_queries, num_q_heads, block_count);
+    const Plan plan = plan_of(*cache, num_queries, num_q_heads, block_count);
+    p.qtiles = (int)plan.qtiles; p.splits = (int)plan.splits; p.whole = (int)plan.whole; p.parts = plan.parts;
     p.out = static_cast<bf16_t*>(out);
     p.c = (softmax_scale > 0.f ? softmax_scale : 0.125f) * kLog2e;
-    int64_t rows = (int64_t)p.B * num_queries * num_q_heads;
     char* ws = static_cast<char*>(workspace);
+    const bool small = few(*cache, num_queries, num_q_heads, block_count);
     if (p.splits > 1) {
-        p.part_o = reinterpret_cast<float*>(ws);
-        p.part_ml = reinterpret_cast<float2*>(ws + up(p.splits * rows * kHeadDim * sizeof(float)));
+        p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
+        p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
+        if (!small) p.part_at = reinterpret_cast<int64_t*>(ws + plan.part_at);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (block_count > 0 && !few(*cache, num_queries, num_q_heads, block_count)) {
-        place_order(p, ws + part_bytes(*cache, num_queries, num_q_heads, block_count));
+    if (block_count > 0 && !small) {
+        place_order(p, ws + plan.bytes);
         if (int e = launch_order(p, s)) return e;
     }
-    const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, small = few(*cache, num_queries, num_q_heads, block_count);
-    int total = (small ? 1 : p.qtiles) * p.Hk * p.B * p.splits;
-    void* args[] = {&p, &total};
-    const void* fn = block_count > 0 ? (fp8 ? (const void*)&cache_attn_kernel<true, false> : (const void*)&cache_attn_kernel<false, false>)
-                                     : (fp8 ? (const void*)&cache_attn_kernel<true, true> : (const void*)&cache_attn_kernel<false, true>);
-    if (small)
-        fn = block_count > 0 ? (fp8 ? (const void*)&cache_attn_few_kernel<true, false> : (const void*)&cache_attn_few_kernel<false, false>)
-                             : (fp8 ? (const void*)&cache_attn_few_kernel<true, true> : (const void*)&cache_attn_few_kernel<false, true>);
+    int total = (int)(plan.whole + (plan.tiles - plan.whole) * plan.splits);
+    void* args[] = {&p};
+    const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, sets = block_count > 0;
+    const void* fn;
+    if (small) fn = fp8 ? (sets ? (const void*)&cache_attn_few_kernel<true, false> : (const void*)&cache_attn_few_kernel<true, true>)
+                        : (sets ? (const void*)&cache_attn_few_kernel<false, false> : (const void*)&cache_attn_few_kernel<false, true>);
+    else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false> : (const void*)&cache_attn_kernel<false, false>;
+    else fn = fp8 ? (const void*)&cache_attn_kernel<true, true> : (const void*)&cache_attn_kernel<false, true>;
     if (launch(fn, dim3(total), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
-    void* jargs[] = {&p, &rows};
+    void* jargs[] = {&p};
     const bool team = p.splits > 16;
     const void* join = team ? (const void*)&cache_attn_join_kernel<16> : (const void*)&cache_attn_join_kernel<1>;
-    return launch(join, dim3((unsigned)(team ? rows : (rows + 15) / 16)), jargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+    return launch(join, dim3((unsigned)(team ? p.parts : (p.parts + 15) / 16)), jargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
 
 }  // extern "C"
