@@ -541,8 +541,8 @@ typedef enum {
    values: the value of a code is code * scale.  batch sequences of capacity tokens, in num_blocks =
    ceil(capacity / block_size) blocks of block_size (64, 128 or 256).  k_codes, v_codes: bytes
    [batch, num_blocks, num_kv_heads, block_size * 64], 16-byte aligned, in the library's own order (zeros
-   stand for zeros); k_scale, v_scale, k_norm: fp32 [batch, num_blocks, num_kv_heads], k_norm not below the
-   norm of any key of the block; k_mean: bf16 [batch, num_blocks, num_kv_heads, 64], 16-byte aligned, the mean of
+   stand for zeros); k_scale, v_scale, k_norm: fp32 [batch, num_blocks, num_kv_heads], k_norm the largest
+   norm of a key of the block; k_mean: bf16 [batch, num_blocks, num_kv_heads, 64], 16-byte aligned, the mean of
    each block's keys.  All zeros is an empty cache.  It has no counterpart in the reference. */
 typedef struct {
     void* k_codes;

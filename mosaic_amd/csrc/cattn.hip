@@ -63,8 +63,8 @@ struct AttnState {
 // and for scales of values further than kSpread from 1: the reference is the maximum, and a row's
 // accumulators take nothing from a block that it has not, not even 0 * NaN.
 enum Form { kBounded, kRunning, kSafe };
-constexpr float kBound = 56.f;
-constexpr float kSpread = 0x1p30f;   // P stays within 2^86, its sums over 2^31 codes up to 448 within 2^126
+constexpr float kBound = 90.f;       // (with kSpread: P >= 2^-120, and an overflow of its sums ends in kSafe)
+constexpr float kSpread = 0x1p30f;
 
 // x a + b in two roundings
 __device__ __forceinline__ float times_plus(float x, float a, float b) {
@@ -190,23 +190,102 @@ __device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 
     }
 }
 
+// A whole tile of kBounded for the R x 32 rows of a wave, laid out for the matrix pipe and the vector ALU to run
+// side by side within it: the scores of the first 32 keys, under them the staging of the next tile; those of the
+// others, under them the first weights; the products of these, under them the other weights; their products,
+// under what comes next.
+template <int R, typename Stage>
+__device__ __forceinline__ void attend_whole(const CacheTile& tile, const bf16x8 (&qf)[R][4], const bool (&member)[R], const Factors& f,
+                                             AttnState (&a)[R], Stage stage) {
+    const TileRead t{tile, (int)(threadIdx.x & 63)};
+    bf16x8 x[4];   // operands: keys, then values [s2][dt]
+    f32x16 s[R], u[R];
+    bf16x8 p[R][2];
+    float ref[R], lt[R];
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        ref[g] = member[g] ? f.lv : -INFINITY;   // P = 0 for the others
+        lt[g] = 0.f;
+        s[g] = u[g] = splat(0.f);
+    }
+#pragma unroll
+    for (int ds = 0; ds < 4; ++ds) x[ds] = t.key(0, ds);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < R; ++g)
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) s[g] = mfma32(x[ds], qf[g][ds], s[g]);
+    __builtin_amdgcn_sched_barrier(0);
+    stage();
+#pragma unroll
+    for (int ds = 0; ds < 4; ++ds) x[ds] = t.key(1, ds);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < R; ++g)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+            u[g] = mfma32(x[2 * s2], qf[g][2 * s2], u[g]);
+            u[g] = mfma32(x[2 * s2 + 1], qf[g][2 * s2 + 1], u[g]);
+            p[g][s2] = weights<kBounded>(s[g], s2, f.ck, ref[g]);
+            lt[g] = operand_sum(p[g][s2], lt[g]);
+            if (g == R - 1) {   // (the keys are read)
+                x[2 * s2] = t.val(0, 0, s2);
+                x[2 * s2 + 1] = t.val(0, 1, s2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        bf16x8 w[2];
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt) a[g].o[dt] = mfma32(x[2 * s2 + dt], p[g][s2], a[g].o[dt]);
+            w[s2] = weights<kBounded>(u[g], s2, f.ck, ref[g]);
+            lt[g] = operand_sum(w[s2], lt[g]);
+            if (g == R - 1) {
+                x[2 * s2] = t.val(1, 0, s2);
+                x[2 * s2 + 1] = t.val(1, 1, s2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        p[g][0] = w[0];
+        p[g][1] = w[1];
+    }
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt) a[g].o[dt] = mfma32(x[2 * s2 + dt], p[g][s2], a[g].o[dt]);
+        a[g].l = fmaf(lt[g], f.iv, a[g].l);
+    }
+}
+
 // The loop over the tiles of a workgroup's blocks
-template <bool FP8, bool SAFE, typename Lds>
+template <bool FP8, bool DENSE, bool SAFE, int WAVES, int R, typename Lds>
 struct Walk {
     const CacheAttnParams& p;
     Lds& L;
     int b, h, end, sub;
-    const bf16x8 (&qf)[4];
-    const Row& row;
-    AttnState& a;
+    const bf16x8 (&qf)[R][4];
+    const Row (&row)[R];
+    AttnState (&a)[R];
     float qc;       // c |q| of the wave's rows at most
 
-    struct Staged { uint4 k, v; };   // a thread's 16 codes of either
+    // The 512 runs of 16 codes of a tile, those of the keys first: a thread stages kRuns of them
+    static constexpr int kRuns = (512 + 64 * WAVES - 1) / (64 * WAVES);
+    struct Staged { uint4 x[kRuns]; };
+    __device__ __forceinline__ static int run(int k) { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 + 64 * WAVES * k; }   // of lane 0
     __device__ __forceinline__ void load(int block, int st, Staged& r) const {
-        const uint32_t at = 16u * threadIdx.x;
         const int64_t from = block_at(p.cache, b, block, h) * (p.bs * 64) + st * kCodeTile;
-        r.k = ld16(static_cast<const uint8_t*>(p.cache.k_codes) + from + at);
-        r.v = ld16(static_cast<const uint8_t*>(p.cache.v_codes) + from + at);
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+            const int c = run(k);
+            if (c >= 512) continue;
+            const uint8_t* codes = static_cast<const uint8_t*>(c < 256 ? p.cache.k_codes : p.cache.v_codes) + from + 16 * (c & 255);
+            r.x[k] = ld16(codes + 16 * (threadIdx.x & 63));
+        }
     }
     __device__ __forceinline__ static void expand(bf16_t* at, const uint4& u) {   // 16 codes: two operands of a lane
         const uint2 a = codes_bf16<FP8>(u.x), b = codes_bf16<FP8>(u.y), c = codes_bf16<FP8>(u.z), d = codes_bf16<FP8>(u.w);
@@ -214,9 +293,11 @@ struct Walk {
         *reinterpret_cast<uint4*>(at + 64 * 8) = make_uint4(c.x, c.y, d.x, d.y);
     }
     __device__ __forceinline__ void put(int buf, const Staged& r) const {
-        const int tid = threadIdx.x, at = ((tid >> 6) * 2 * 64 + (tid & 63)) * 8;
-        expand(L.tile[buf].K + at, r.k);
-        expand(L.tile[buf].V + at, r.v);
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+            const int c = run(k);   // (the values' tile follows the keys')
+            if (c < 512) expand(L.tile[buf].K + 16 * c + 8 * (threadIdx.x & 63), r.x[k]);
+        }
     }
     // up to 64 blocks, lane i < count holding the i-th and its members among the wave's tokens
     __device__ __forceinline__ void blocks(int count, int block, int members) {
@@ -227,7 +308,10 @@ struct Walk {
         else {
             const uint64_t far = __builtin_amdgcn_ballot_w64(wide);
             // (a NaN is not bounded; a wave by itself: the forms have the same barriers)
-            if (__builtin_amdgcn_ballot_w64(!(p.cache.k_norm[at] * qc <= kBound) || a.m != 0.f)) tiles<kRunning>(count, block, members, f, far);
+            bool moved = false;
+#pragma unroll
+            for (int g = 0; g < R; ++g) moved = moved || a[g].m != 0.f;
+            if (__builtin_amdgcn_ballot_w64(!(p.cache.k_norm[at] * qc <= kBound) || moved)) tiles<kRunning>(count, block, members, f, far);
             else tiles<kBounded>(count, block, members, f, far);
         }
     }
@@ -241,44 +325,79 @@ struct Walk {
                 st = 0;
             }
         };
+        // Only the sequence's last tile may be short.  It is left to the end: with one way through the loop the
+        // accumulators stay where they are.
+        auto whole = [&](int i, int st) { return end - key0(i) - 64 * st >= 64; };
+        auto lane_f = [&](float x, int i) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), i)); };
+        int buf = 0;
+        uint32_t of;
+        bool member[R];
+        Factors ft;
+        auto meet = [&](int i) {
+            of = (uint32_t)__builtin_amdgcn_readlane(members, i);
+            ft = Factors{lane_f(f.ck, i), lane_f(f.lv, i), lane_f(f.iv, i)};
+#pragma unroll
+            for (int g = 0; g < R; ++g) {
+                member[g] = DENSE ? row[g].live : row[g].in(of);
+                if (F == kBounded) a[g].has = a[g].has || member[g];
+                if (far >> i & 1) a[g].wide = a[g].wide || member[g];
+            }
+        };
+        auto each = [&](int valid) {
+#pragma unroll
+            for (int g = 0; g < R; ++g) attend_tile<F>(L.tile[buf], qf[g], member[g], valid, ft, a[g]);
+        };
         Staged r;
         int i = 0, st = 0, ni = 0, nst = 0;
         load(__builtin_amdgcn_readlane(block, 0), 0, r);
         put(0, r);
         next(ni, nst);
-        if (ni < count) load(__builtin_amdgcn_readlane(block, ni), nst, r);
-        for (int buf = 0; i < count; buf ^= 1) {
+        load(__builtin_amdgcn_readlane(block, min(ni, count - 1)), nst, r);
+        for (; i < count && whole(i, st); buf ^= 1) {
             lds_barrier();
             int fi = ni, fst = nst;
-            if (ni < count) {
+            if (ni < count) next(fi, fst);
+            const int src = __builtin_amdgcn_readlane(block, min(fi, count - 1));
+            // (past the last tile the staged one is put and loaded once more, to no effect: no branch in the way)
+            auto stage = [&] {
                 put(buf ^ 1, r);
-                next(fi, fst);
-                if (fi < count) load(__builtin_amdgcn_readlane(block, fi), fst, r);
-            }
-            const uint32_t of = (uint32_t)__builtin_amdgcn_readlane(members, i);
-            auto lane_f = [&](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), i)); };
-            if (of != 0) {
-                const bool member = row.in(of);
-                if (F == kBounded) a.has = a.has || member;
-                if (far >> i & 1) a.wide = a.wide || member;
-                attend_tile<F>(L.tile[buf], qf, member, min(64, end - key0(i) - 64 * st), Factors{lane_f(f.ck), lane_f(f.lv), lane_f(f.iv)}, a);
+                __builtin_amdgcn_sched_barrier(0);   // (r is free before it is loaded again)
+                load(src, fst, r);
+            };
+            meet(i);
+            if constexpr (F == kBounded && DENSE) attend_whole<R>(L.tile[buf], qf, member, ft, a, stage);
+            else {
+                stage();
+                if (of != 0) {
+                    if constexpr (F == kBounded) attend_whole<R>(L.tile[buf], qf, member, ft, a, [] {});
+                    else each(64);
+                }
             }
             i = ni; st = nst;
             ni = fi; nst = fst;
         }
-        lds_barrier();   // the buffers are free for the next blocks
+        lds_barrier();
+        if (i < count) {
+            meet(i);
+            if (of != 0) each(end - key0(i) - 64 * st);
+            lds_barrier();
+        }
+        // (the buffers are free for the next blocks)
     }
 };
 
-template <bool FP8, bool DENSE, bool SAFE, typename Lds>
-__device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, int h, int n0, int split, int splits, const Row& row, int wave_live,
-                                       float qc, const bf16x8 (&qf)[4], AttnState& a) {
+template <bool FP8, bool DENSE, bool SAFE, int WAVES, int R, typename Lds>
+__device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, int h, int n0, int split, int splits, const Row (&row)[R], int wave_live,
+                                       float qc, const bf16x8 (&qf)[R][4], AttnState (&a)[R]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    a.o[0] = a.o[1] = splat(0.f);
-    a.m = a.l = 0.f;
-    a.has = a.wide = false;
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        a[g].o[0] = a[g].o[1] = splat(0.f);
+        a[g].m = a[g].l = 0.f;
+        a[g].has = a[g].wide = false;
+    }
     const int end = seq_keys(p, b);
-    Walk<FP8, SAFE, Lds> walk{p, L, b, h, end, p.bs / 64, qf, row, a, qc};
+    Walk<FP8, DENSE, SAFE, WAVES, R, Lds> walk{p, L, b, h, end, p.bs / 64, qf, row, a, qc};
     const int live = (int)(((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
     if constexpr (DENSE) {
         const int first = (int)((int64_t)live * split / splits), past = (int)((int64_t)live * (split + 1) / splits);
@@ -320,8 +439,11 @@ __device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row
     }
 }
 
-template <bool FP8, bool DENSE>
-__global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(CacheAttnParams p) {
+// R x 32 rows a wave: with 64, at two waves a SIMD, the codes are converted and the operands read for twice as
+// many rows.
+template <bool FP8, bool DENSE, int WAVES, int R>
+__global__ __launch_bounds__(64 * WAVES, R == 1 ? 3 : 2) void cache_attn_kernel(CacheAttnParams p) {
+    static_assert(DENSE || R == 1, "the union's members are those of 32 rows a wave");
     __shared__ std::conditional_t<DENSE, DenseLds, SetsLds> L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -335,38 +457,57 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(CacheAttnParams
         split = i % splits;
     }
     const int tile_id = tile % p.qtiles, rest = tile / p.qtiles, h = rest % p.Hk, b = rest / p.Hk;
-    const int n0 = tile_id * kWaves * p.QW;
-    Row row;
-    if constexpr (DENSE) row.init(p, [&](int i) { return min(n0 + i, p.Nq - 1); }, b, h, n0, wave, lane & 31);
-    else {
-        load_tokens(p, L, b, h, n0);
-        row.init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
+    const int n0 = tile_id * WAVES * R * p.QW;
+    if constexpr (!DENSE) load_tokens(p, L, b, h, n0);
+    Row row[R];
+    bf16x8 qf[R][4];   // step ds: dims 32 (ds / 2) + 16 hh + 8 (ds % 2) .. (see qcache.h)
+    float qc = 0.f;
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        if constexpr (DENSE) row[g].init(p, [&](int i) { return min(n0 + i, p.Nq - 1); }, b, h, n0, wave * R + g, lane & 31);
+        else row[g].init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
+        const bf16_t* qr = p.q + b * p.q_sb + row[g].n * p.q_sn + row[g].head * p.q_sh + 16 * hh;
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) qf[g][ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
     }
-    bf16x8 qf[4];   // step ds: dims 32 (ds / 2) + 16 hh + 8 (ds % 2) .. (see qcache.h)
-    const bf16_t* qr = p.q + b * p.q_sb + row.n * p.q_sn + row.head * p.q_sh + 16 * hh;
 #pragma unroll
-    for (int ds = 0; ds < 4; ++ds) qf[ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
-    arrived(qf);
-    float qc = 0.f;   // of the norm, a little more than its roundings
+    for (int g = 0; g < R; ++g) {
+        arrived(qf[g]);
+        float square = 0.f;
 #pragma unroll
-    for (int ds = 0; ds < 4; ++ds) {
-        const uint4 u = __builtin_bit_cast(uint4, qf[ds]);
-        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        for (int ds = 0; ds < 4; ++ds) {
+            const uint4 u = __builtin_bit_cast(uint4, qf[g][ds]);
+            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qc = fmaf(bf_lo(x[i]), bf_lo(x[i]), fmaf(bf_hi(x[i]), bf_hi(x[i]), qc));
+            for (int i = 0; i < 4; ++i) square = fmaf(bf_lo(x[i]), bf_lo(x[i]), fmaf(bf_hi(x[i]), bf_hi(x[i]), square));
+        }
+        square = wave_max_nonneg(xor32_add(square));
+        qc = square > qc || square != square ? square : qc;   // (a NaN stays)
     }
-    qc = wave_max_nonneg(sqrtf(xor32_add(qc))) * p.c * 1.001f;
-    const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
-    const int64_t part = (int64_t)(tile - p.whole) * (kWaves * kRows) + wave * kRows + (lane & 31);
-    if (splits > 1 && split == 0 && hh == 0) p.part_at[part] = row.live ? row.at : -1;
-    AttnState a;
-    attend<FP8, DENSE, false>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
-    const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
-    const bool ok = fine && __shfl_xor((int)fine, 32);   // (both halves of the row)
-    if (row.live && ok) put_row(p, row, part, split, splits, a);
-    if (!__syncthreads_or(!ok)) return;
-    attend<FP8, DENSE, true>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
-    if (row.live && !ok) put_row(p, row, part, split, splits, a);
+    qc = sqrtf(qc) * p.c * 1.001f;   // a little more than its roundings
+    bool any = false;
+#pragma unroll
+    for (int g = 0; g < R; ++g) any = any || row[g].live;
+    const int wave_live = __builtin_amdgcn_ballot_w64(any) ? -1 : 0;   // (a wave without rows only stages)
+    auto part = [&](int g) { return (int64_t)(tile - p.whole) * (WAVES * R * kRows) + (wave * R + g) * kRows + (lane & 31); };
+    if (splits > 1 && split == 0 && hh == 0)
+#pragma unroll
+        for (int g = 0; g < R; ++g) p.part_at[part(g)] = row[g].live ? row[g].at : -1;
+    AttnState a[R];
+    bool ok[R], all = true;
+    attend<FP8, DENSE, false, WAVES, R>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        const bool fine = finite(a[g].o[0]) && finite(a[g].o[1]) && a[g].l - a[g].l == 0.f && !a[g].wide;
+        ok[g] = fine && __shfl_xor((int)fine, 32);   // (both halves of the row)
+        all = all && ok[g];
+        if (row[g].live && ok[g]) put_row(p, row[g], part(g), split, splits, a[g]);
+    }
+    if (!__syncthreads_or(!all)) return;
+    attend<FP8, DENSE, true, WAVES, R>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
+#pragma unroll
+    for (int g = 0; g < R; ++g)
+        if (row[g].live && !ok[g]) put_row(p, row[g], part(g), split, splits, a[g]);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -670,7 +811,7 @@ int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, 
     return MOSAIC_OK;
 }
 
-constexpr int64_t kFewGroups = 1024, kFewTiles = 2;
+constexpr int64_t kFewGroups = 1024, kFewTiles = 2, kWideRows = 32768;
 
 // Whether the call is one of cache_attn_few_kernel
 bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
@@ -678,13 +819,15 @@ bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     return rows <= kFewRows && (int64_t)nq * K <= kFewEntries;
 }
 
-// How a call is laid out: tiles of rows, those taken whole, and shares of the others' keys.
+// How a call is laid out: waves of a workgroup, tiles of rows, those taken whole, and shares of the others' keys.
 struct Plan {
+    int waves;
     int64_t qtiles, tiles, whole, splits, parts;   // tiles of a (member, kv head), and of all; rows that are joined
     size_t part_o, part_ml, part_at, bytes;        // places in the workspace, and what the partials take of it
 };
 Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     Plan a{};
+    a.waves = kWaves;
     const int G = hq / c.num_kv_heads;
     const int64_t heads = (int64_t)c.num_kv_heads * c.batch, sub = c.block_size / 64;
     if (few(c, nq, hq, K)) {
@@ -694,7 +837,8 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
         a.parts = (int64_t)c.batch * nq * hq;
     } else {
         const int64_t most = K > 0 ? std::min(K, kMaxSplit) : std::max<int64_t>(1, c.num_blocks / 4);
-        const int64_t per = kWaves * (kRows / G), slots = K > 0 ? 512 : 768;
+        if (K == 0 && (int64_t)nq * G * heads >= kWideRows) a.waves = 12;
+        const int64_t per = a.waves * (kRows / G), slots = K > 0 ? 512 : a.waves == 12 ? 256 : 768;
         a.qtiles = (nq + per - 1) / per;
         a.tiles = a.qtiles * heads;
         // full rounds of the chip, and the rest's keys in shares that fill it once more (sets: where there is no full round)
@@ -702,7 +846,7 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
         const int64_t rest = a.tiles - a.whole;
         a.splits = rest > 0 ? std::max<int64_t>(1, std::min(slots / rest, most)) : 1;
         if (a.splits == 1) a.whole = a.tiles;
-        a.parts = (a.tiles - a.whole) * kWaves * kRows;
+        a.parts = (a.tiles - a.whole) * a.waves * kRows;
     }
     if (a.splits > 1) {
         a.part_ml = up(a.splits * a.parts * kHeadDim * sizeof(float));
@@ -765,9 +909,10 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     const void* fn;
     if (small) fn = fp8 ? (sets ? (const void*)&cache_attn_few_kernel<true, false> : (const void*)&cache_attn_few_kernel<true, true>)
                         : (sets ? (const void*)&cache_attn_few_kernel<false, false> : (const void*)&cache_attn_few_kernel<false, true>);
-    else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false> : (const void*)&cache_attn_kernel<false, false>;
-    else fn = fp8 ? (const void*)&cache_attn_kernel<true, true> : (const void*)&cache_attn_kernel<false, true>;
-    if (launch(fn, dim3(total), args, s) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false, 4, 1> : (const void*)&cache_attn_kernel<false, false, 4, 1>;
+    else if (plan.waves == 12) fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 12, 1> : (const void*)&cache_attn_kernel<false, true, 12, 1>;
+    else fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 4, 1> : (const void*)&cache_attn_kernel<false, true, 4, 1>;
+    if (launch(fn, dim3(total), args, s, 64 * plan.waves) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
     void* jargs[] = {&p};
     const bool team = p.splits > 16;

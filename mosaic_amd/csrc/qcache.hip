@@ -8,8 +8,8 @@
 // Tokens of the block behind the end become zeros; other blocks stay as they are.  A value that is not
 // finite makes its block's scale NaN, which everything read from the block then is.  The mean of the
 // block's keys (the sum of the codes times the scale over the number of tokens) goes to k_mean, where
-// query_topk takes it from, and a bound of their norms (the norm of the largest parts of 16 dims, at most
-// twice the largest norm) to k_norm, by which the attention knows that it needs no maxima.
+// query_topk takes it from, and the largest of their norms to k_norm, by which the attention knows where it
+// needs no maxima.
 //
 // The rounding is that of the exact quotient: x * (1 / scale), within 1.5 units of its last place, is taken to
 // the nearest number that could be a tie, and moved off it by the sign of the remainder, which an fma gives.
@@ -199,7 +199,7 @@ __device__ __forceinline__ float new_scale(uint32_t most, bool keeps, float befo
 template <typename T, bool FP8, int SUB>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p) {
     __shared__ uint32_t most[2][kWaves];
-    __shared__ float sums[2][64], norms[2][4];
+    __shared__ float sums[2][64], squares[SUB][kWaves][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x % p.c.num_kv_heads, rest = blockIdx.x / p.c.num_kv_heads, unit = rest % p.units, b = rest / p.units;
     constexpr int kBlock = 64 * SUB;
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[s][i].clear();
 
-    float sum[16], norm = 0.f;
+    float sum[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[i] = 0.f;
 #pragma unroll
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
             sum[4 * i] += c.x; sum[4 * i + 1] += c.y; sum[4 * i + 2] += c.z; sum[4 * i + 3] += c.w;
             square = fmaf(c.x, c.x, fmaf(c.y, c.y, fmaf(c.z, c.z, fmaf(c.w, c.w, square))));
         }
-        norm = fmaxf(norm, square);
+        squares[s][wave][lane & 31] = xor32_add(square);   // (both halves the same)
         reinterpret_cast<uint4*>(kc + s * kCodeTile)[tid] = make_uint4(w[0], w[1], w[2], w[3]);
 
         uint32_t x[4];
@@ -343,13 +343,6 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
     // lane bits 4..1 chose the dim: bit 4 the upper eight of sixteen, and so on
     const int dim = kdim + 8 * ((lane >> 4) & 1) + 4 * ((lane >> 3) & 1) + 2 * ((lane >> 2) & 1) + ((lane >> 1) & 1);
     if ((lane & 1) == 0) sums[wave >> 1][dim] = sum[0];
-    // the largest part of 16 dims of a key's square, for each of the four parts
-    norm = fmaxf(norm, lane_xor<1>(norm));
-    norm = fmaxf(norm, lane_xor<2>(norm));
-    norm = fmaxf(norm, lane_xor<4>(norm));
-    norm = fmaxf(norm, lane_xor<8>(norm));
-    norm = fmaxf(norm, lane_xor<16>(norm));
-    if ((lane & 31) == 0) norms[wave >> 1][(wave & 1) * 2 + (lane >> 5)] = norm;
     __syncthreads();
     if (tid < 32) {
         // (the mean of the codes first: their sum times the scale need not fit)
@@ -357,13 +350,16 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
         const float c = (sums[0][2 * tid + 1] + sums[1][2 * tid + 1]) / (float)end * kq.scale;
         static_cast<uint32_t*>(p.c.k_mean)[blk * 32 + tid] = pack_bf16x2(a, c);
     }
-    if (tid == 0) {
+    if (wave == 1) {   // the largest norm of a key: waves 0 and 1, 2 and 3 have the halves of a token
         float square = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) square += fmaxf(norms[0][i], norms[1][i]);
+        for (int s = 0; s < SUB; ++s) square = fmaxf(square, squares[s][2 * (lane >> 5)][lane & 31] + squares[s][2 * (lane >> 5) + 1][lane & 31]);
+        square = wave_max_nonneg(square);
+        if (lane == 0) p.c.k_norm[blk] = sqrtf(square) * kq.scale;
+    }
+    if (tid == 0) {
         p.c.k_scale[blk] = kq.scale;
         p.c.v_scale[blk] = vq.scale;
-        p.c.k_norm[blk] = sqrtf(square) * kq.scale;
     }
 }
 

@@ -45,8 +45,8 @@ class KVCache:
 
     The lengths of the sequences are the program's own (``kv_lens`` of the attention).  ``k_scale`` and
     ``v_scale`` (float32 [batch, num_blocks, kv_heads]), ``k_mean`` (bfloat16 [batch, num_blocks, kv_heads,
-    64], the mean of the keys of each block: ``k_cmp`` of ``query_topk``), ``k_norm`` (float32 as the scales, not
-    below the norm of any key of the block, nor above twice the largest) and the codes, in an order of the library's
+    64], the mean of the keys of each block: ``k_cmp`` of ``query_topk``), ``k_norm`` (float32 as the scales, the
+    largest norm of a key of the block) and the codes, in an order of the library's
     own, are tensors of the cache: ``kv_cache_write`` changes them in place.
     """
 
