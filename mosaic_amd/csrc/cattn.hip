@@ -190,102 +190,75 @@ __device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 
     }
 }
 
-// A whole tile of kBounded for the R x 32 rows of a wave, laid out for the matrix pipe and the vector ALU to run
-// side by side within it: the scores of the first 32 keys, under them the staging of the next tile; those of the
-// others, under them the first weights; the products of these, under them the other weights; their products,
-// under what comes next.
-template <int R, typename Stage>
-__device__ __forceinline__ void attend_whole(const CacheTile& tile, const bf16x8 (&qf)[R][4], const bool (&member)[R], const Factors& f,
-                                             AttnState (&a)[R], Stage stage) {
+// A whole tile of kBounded, laid out for the matrix pipe and the vector ALU to run side by side within a wave:
+// the scores of the first 32 keys, under them the staging of the next tile; those of the others, under them the
+// first weights; the product of these, under it the other weights; their product, under what comes next.
+template <typename Stage>
+__device__ __forceinline__ void attend_whole(const CacheTile& tile, const bf16x8 (&qf)[4], bool member, const Factors& f, AttnState& a, Stage stage) {
     const TileRead t{tile, (int)(threadIdx.x & 63)};
-    bf16x8 x[4];   // operands: keys, then values [s2][dt]
-    f32x16 s[R], u[R];
-    bf16x8 p[R][2];
-    float ref[R], lt[R];
-#pragma unroll
-    for (int g = 0; g < R; ++g) {
-        ref[g] = member[g] ? f.lv : -INFINITY;   // P = 0 for the others
-        lt[g] = 0.f;
-        s[g] = u[g] = splat(0.f);
-    }
+    const float ref = member ? f.lv : -INFINITY;   // P = 0 for the others
+    bf16x8 x[4], p[2], w[2];                       // x: operands, the keys', then the values' [s2][dt]
+    f32x16 s = splat(0.f), u = splat(0.f);
+    float lt = 0.f;
 #pragma unroll
     for (int ds = 0; ds < 4; ++ds) x[ds] = t.key(0, ds);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int g = 0; g < R; ++g)
-#pragma unroll
-        for (int ds = 0; ds < 4; ++ds) s[g] = mfma32(x[ds], qf[g][ds], s[g]);
+    for (int ds = 0; ds < 4; ++ds) s = mfma32(x[ds], qf[ds], s);
     __builtin_amdgcn_sched_barrier(0);
     stage();
 #pragma unroll
     for (int ds = 0; ds < 4; ++ds) x[ds] = t.key(1, ds);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int g = 0; g < R; ++g)
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-            u[g] = mfma32(x[2 * s2], qf[g][2 * s2], u[g]);
-            u[g] = mfma32(x[2 * s2 + 1], qf[g][2 * s2 + 1], u[g]);
-            p[g][s2] = weights<kBounded>(s[g], s2, f.ck, ref[g]);
-            lt[g] = operand_sum(p[g][s2], lt[g]);
-            if (g == R - 1) {   // (the keys are read)
-                x[2 * s2] = t.val(0, 0, s2);
-                x[2 * s2 + 1] = t.val(0, 1, s2);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-    for (int g = 0; g < R; ++g) {
-        bf16x8 w[2];
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-#pragma unroll
-            for (int dt = 0; dt < 2; ++dt) a[g].o[dt] = mfma32(x[2 * s2 + dt], p[g][s2], a[g].o[dt]);
-            w[s2] = weights<kBounded>(u[g], s2, f.ck, ref[g]);
-            lt[g] = operand_sum(w[s2], lt[g]);
-            if (g == R - 1) {
-                x[2 * s2] = t.val(1, 0, s2);
-                x[2 * s2 + 1] = t.val(1, 1, s2);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        p[g][0] = w[0];
-        p[g][1] = w[1];
+    for (int s2 = 0; s2 < 2; ++s2) {
+        u = mfma32(x[2 * s2], qf[2 * s2], u);
+        u = mfma32(x[2 * s2 + 1], qf[2 * s2 + 1], u);
+        p[s2] = weights<kBounded>(s, s2, f.ck, ref);
+        lt = operand_sum(p[s2], lt);
+        x[2 * s2] = t.val(0, 0, s2);
+        x[2 * s2 + 1] = t.val(0, 1, s2);
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int g = 0; g < R; ++g) {
+    for (int s2 = 0; s2 < 2; ++s2) {
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-            for (int dt = 0; dt < 2; ++dt) a[g].o[dt] = mfma32(x[2 * s2 + dt], p[g][s2], a[g].o[dt]);
-        a[g].l = fmaf(lt[g], f.iv, a[g].l);
+        for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(x[2 * s2 + dt], p[s2], a.o[dt]);
+        w[s2] = weights<kBounded>(u, s2, f.ck, ref);
+        lt = operand_sum(w[s2], lt);
+        x[2 * s2] = t.val(1, 0, s2);
+        x[2 * s2 + 1] = t.val(1, 1, s2);
+        __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(x[2 * s2 + dt], w[s2], a.o[dt]);
+    a.l = fmaf(lt, f.iv, a.l);
 }
 
 // The loop over the tiles of a workgroup's blocks
-template <bool FP8, bool DENSE, bool SAFE, int WAVES, int R, typename Lds>
+template <bool FP8, bool DENSE, bool SAFE, int WAVES, typename Lds>
 struct Walk {
     const CacheAttnParams& p;
     Lds& L;
-    int b, h, end, sub;
-    const bf16x8 (&qf)[R][4];
-    const Row (&row)[R];
-    AttnState (&a)[R];
-    float qc;       // c |q| of the wave's rows at most
+    int b, h, end;
+    const bf16x8 (&qf)[4];
+    const Row& row;
+    AttnState& a;
 
-    // The 512 runs of 16 codes of a tile, those of the keys first: a thread stages kRuns of them
-    static constexpr int kRuns = (512 + 64 * WAVES - 1) / (64 * WAVES);
+    // The 512 runs of 16 codes of a tile, those of the keys first: a thread stages one of either, of more waves one
+    static constexpr int kRuns = WAVES == 4 ? 2 : 1;
     struct Staged { uint4 x[kRuns]; };
-    __device__ __forceinline__ static int run(int k) { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 + 64 * WAVES * k; }   // of lane 0
+    __device__ __forceinline__ static int first_run() { return WAVES == 4 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x) & ~255; }
     __device__ __forceinline__ void load(int block, int st, Staged& r) const {
-        const int64_t from = block_at(p.cache, b, block, h) * (p.bs * 64) + st * kCodeTile;
-#pragma unroll
-        for (int k = 0; k < kRuns; ++k) {
-            const int c = run(k);
-            if (c >= 512) continue;
-            const uint8_t* codes = static_cast<const uint8_t*>(c < 256 ? p.cache.k_codes : p.cache.v_codes) + from + 16 * (c & 255);
-            r.x[k] = ld16(codes + 16 * (threadIdx.x & 63));
-        }
+        if (first_run() >= 512) return;
+        const int64_t from = ((int64_t)b * p.nb * p.Hk + h) * (p.bs * 64) + (uint64_t)(uint32_t)block * (uint32_t)(p.Hk * p.bs * 64) + st * kCodeTile;
+        const uint32_t at = 16 * (threadIdx.x & 255);
+        if constexpr (kRuns == 2) {
+            r.x[0] = ld16(static_cast<const uint8_t*>(p.cache.k_codes) + from + at);
+            r.x[1] = ld16(static_cast<const uint8_t*>(p.cache.v_codes) + from + at);
+        } else r.x[0] = ld16(static_cast<const uint8_t*>(first_run() == 0 ? p.cache.k_codes : p.cache.v_codes) + from + at);
     }
     __device__ __forceinline__ static void expand(bf16_t* at, const uint4& u) {   // 16 codes: two operands of a lane
         const uint2 a = codes_bf16<FP8>(u.x), b = codes_bf16<FP8>(u.y), c = codes_bf16<FP8>(u.z), d = codes_bf16<FP8>(u.w);
@@ -293,111 +266,101 @@ struct Walk {
         *reinterpret_cast<uint4*>(at + 64 * 8) = make_uint4(c.x, c.y, d.x, d.y);
     }
     __device__ __forceinline__ void put(int buf, const Staged& r) const {
+        const int tid = threadIdx.x, at = ((tid >> 6 & 3) * 2 * 64 + (tid & 63)) * 8;
+        if (first_run() >= 512) return;
+        if constexpr (kRuns == 2) {
+            expand(L.tile[buf].K + at, r.x[0]);
+            expand(L.tile[buf].V + at, r.x[1]);
+        } else expand((first_run() == 0 ? L.tile[buf].K : L.tile[buf].V) + at, r.x[0]);
+    }
+    // c |q| of the wave's rows at most, a little more than its roundings (a NaN stays)
+    __device__ __forceinline__ float bound() const {
+        float square = 0.f;
 #pragma unroll
-        for (int k = 0; k < kRuns; ++k) {
-            const int c = run(k);   // (the values' tile follows the keys')
-            if (c < 512) expand(L.tile[buf].K + 16 * c + 8 * (threadIdx.x & 63), r.x[k]);
+        for (int ds = 0; ds < 4; ++ds) {
+            const uint4 u = __builtin_bit_cast(uint4, qf[ds]);
+            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) square = fmaf(bf_lo(x[i]), bf_lo(x[i]), fmaf(bf_hi(x[i]), bf_hi(x[i]), square));
         }
+        return sqrtf(wave_max_nonneg(xor32_add(square))) * p.c * 1.001f;
     }
     // up to 64 blocks, lane i < count holding the i-th and its members among the wave's tokens
     __device__ __forceinline__ void blocks(int count, int block, int members) {
         const int64_t at = block_at(p.cache, b, block, h);
+        const float ks = p.cache.k_scale[at], vs = p.cache.v_scale[at], norm = p.cache.k_norm[at];
+        Staged r;
+        load(__builtin_amdgcn_readlane(block, 0), 0, r);
         bool wide;
-        const Factors f = factors<SAFE>(p.c, p.cache.k_scale[at], p.cache.v_scale[at], wide);
-        if constexpr (SAFE) tiles<kSafe>(count, block, members, f, 0);
+        const Factors f = factors<SAFE>(p.c, ks, vs, wide);
+        if constexpr (SAFE) tiles<kSafe>(count, block, members, f, r);
         else {
-            const uint64_t far = __builtin_amdgcn_ballot_w64(wide);
+            for (uint64_t far = __builtin_amdgcn_ballot_w64(wide); far != 0; far &= far - 1)
+                a.wide = a.wide || DENSE || row.in((uint32_t)__builtin_amdgcn_readlane(members, (int)__builtin_ctzll(far)));
             // (a NaN is not bounded; a wave by itself: the forms have the same barriers)
-            bool moved = false;
-#pragma unroll
-            for (int g = 0; g < R; ++g) moved = moved || a[g].m != 0.f;
-            if (__builtin_amdgcn_ballot_w64(!(p.cache.k_norm[at] * qc <= kBound) || moved)) tiles<kRunning>(count, block, members, f, far);
-            else tiles<kBounded>(count, block, members, f, far);
+            if (__builtin_amdgcn_ballot_w64(!(norm * bound() <= kBound) || a.m != 0.f)) tiles<kRunning>(count, block, members, f, r);
+            else tiles<kBounded>(count, block, members, f, r);
         }
     }
     template <Form F>
-    __device__ __forceinline__ void tiles(int count, int block, int members, const Factors& f, uint64_t far) {
-        auto key0 = [&](int i) { return __builtin_amdgcn_readlane(block, i) * p.bs; };
-        auto next = [&](int& i, int& st) {   // the tile after (i, st); i = count: none
-            if (st + 1 < sub && key0(i) + 64 * (st + 1) < end) ++st;
-            else {
-                ++i;
-                st = 0;
-            }
-        };
-        // Only the sequence's last tile may be short.  It is left to the end: with one way through the loop the
-        // accumulators stay where they are.
-        auto whole = [&](int i, int st) { return end - key0(i) - 64 * st >= 64; };
-        auto lane_f = [&](float x, int i) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), i)); };
-        int buf = 0;
+    __device__ __forceinline__ void tiles(int count, int block, int members, const Factors& f, Staged& r) {
+        count = __builtin_amdgcn_readfirstlane(count);
+        // Tile t is part t % sub of block t / sub.  Only the sequence's last one may be short, and it is left to the
+        // end: with one way through the loop the accumulators stay where they are.
+        const int shift = p.bs == 64 ? 0 : p.bs == 128 ? 1 : 2, sub = 1 << shift;
+        const int rest = end - __builtin_amdgcn_readlane(block, count - 1) * p.bs;   // keys from the last block on
+        const int total = ((count - 1) << shift) + min(sub, (rest + 63) / 64), whole = ((count - 1) << shift) + min(sub, rest / 64);
+        auto fetch = [&](int t) { load(__builtin_amdgcn_readlane(block, t >> shift), t & (sub - 1), r); };
         uint32_t of;
-        bool member[R];
+        bool member;
         Factors ft;
         auto meet = [&](int i) {
+            auto lane_f = [&](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), i)); };
             of = (uint32_t)__builtin_amdgcn_readlane(members, i);
-            ft = Factors{lane_f(f.ck, i), lane_f(f.lv, i), lane_f(f.iv, i)};
-#pragma unroll
-            for (int g = 0; g < R; ++g) {
-                member[g] = DENSE ? row[g].live : row[g].in(of);
-                if (F == kBounded) a[g].has = a[g].has || member[g];
-                if (far >> i & 1) a[g].wide = a[g].wide || member[g];
-            }
+            ft = Factors{lane_f(f.ck), lane_f(f.lv), lane_f(f.iv)};
+            member = DENSE || row.in(of);   // (rows that do not exist are not stored)
+            if (F == kBounded) a.has = a.has || member;
         };
-        auto each = [&](int valid) {
-#pragma unroll
-            for (int g = 0; g < R; ++g) attend_tile<F>(L.tile[buf], qf[g], member[g], valid, ft, a[g]);
-        };
-        Staged r;
-        int i = 0, st = 0, ni = 0, nst = 0;
-        load(__builtin_amdgcn_readlane(block, 0), 0, r);
         put(0, r);
-        next(ni, nst);
-        load(__builtin_amdgcn_readlane(block, min(ni, count - 1)), nst, r);
-        for (; i < count && whole(i, st); buf ^= 1) {
+        fetch(min(1, total - 1));
+        int t = 0;
+        for (; t < whole; ++t) {
             lds_barrier();
-            int fi = ni, fst = nst;
-            if (ni < count) next(fi, fst);
-            const int src = __builtin_amdgcn_readlane(block, min(fi, count - 1));
             // (past the last tile the staged one is put and loaded once more, to no effect: no branch in the way)
             auto stage = [&] {
-                put(buf ^ 1, r);
+                put(~t & 1, r);
                 __builtin_amdgcn_sched_barrier(0);   // (r is free before it is loaded again)
-                load(src, fst, r);
+                fetch(min(t + 2, total - 1));
             };
-            meet(i);
-            if constexpr (F == kBounded && DENSE) attend_whole<R>(L.tile[buf], qf, member, ft, a, stage);
+            meet(t >> shift);
+            if constexpr (F == kBounded && DENSE) attend_whole(L.tile[t & 1], qf, member, ft, a, stage);
             else {
                 stage();
                 if (of != 0) {
-                    if constexpr (F == kBounded) attend_whole<R>(L.tile[buf], qf, member, ft, a, [] {});
-                    else each(64);
+                    if constexpr (F == kBounded) attend_whole(L.tile[t & 1], qf, member, ft, a, [] {});
+                    else attend_tile<F>(L.tile[t & 1], qf, member, 64, ft, a);
                 }
             }
-            i = ni; st = nst;
-            ni = fi; nst = fst;
         }
         lds_barrier();
-        if (i < count) {
-            meet(i);
-            if (of != 0) each(end - key0(i) - 64 * st);
+        if (t < total) {
+            meet(t >> shift);
+            if (of != 0) attend_tile<F>(L.tile[t & 1], qf, member, rest & 63, ft, a);
             lds_barrier();
         }
         // (the buffers are free for the next blocks)
     }
 };
 
-template <bool FP8, bool DENSE, bool SAFE, int WAVES, int R, typename Lds>
-__device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, int h, int n0, int split, int splits, const Row (&row)[R], int wave_live,
-                                       float qc, const bf16x8 (&qf)[R][4], AttnState (&a)[R]) {
+template <bool FP8, bool DENSE, bool SAFE, int WAVES, typename Lds>
+__device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, int h, int n0, int split, int splits, const Row& row, int wave_live,
+                                       const bf16x8 (&qf)[4], AttnState& a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-    for (int g = 0; g < R; ++g) {
-        a[g].o[0] = a[g].o[1] = splat(0.f);
-        a[g].m = a[g].l = 0.f;
-        a[g].has = a[g].wide = false;
-    }
+    a.o[0] = a.o[1] = splat(0.f);
+    a.m = a.l = 0.f;
+    a.has = a.wide = false;
     const int end = seq_keys(p, b);
-    Walk<FP8, DENSE, SAFE, WAVES, R, Lds> walk{p, L, b, h, end, p.bs / 64, qf, row, a, qc};
+    Walk<FP8, DENSE, SAFE, WAVES, Lds> walk{p, L, b, h, end, qf, row, a};
     const int live = (int)(((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
     if constexpr (DENSE) {
         const int first = (int)((int64_t)live * split / splits), past = (int)((int64_t)live * (split + 1) / splits);
@@ -439,11 +402,9 @@ __device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row
     }
 }
 
-// R x 32 rows a wave: with 64, at two waves a SIMD, the codes are converted and the operands read for twice as
-// many rows.
-template <bool FP8, bool DENSE, int WAVES, int R>
-__global__ __launch_bounds__(64 * WAVES, R == 1 ? 3 : 2) void cache_attn_kernel(CacheAttnParams p) {
-    static_assert(DENSE || R == 1, "the union's members are those of 32 rows a wave");
+template <bool FP8, bool DENSE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_kernel(CacheAttnParams p) {
+    static_assert(DENSE || WAVES == kWaves, "the union's members are those of four waves");
     __shared__ std::conditional_t<DENSE, DenseLds, SetsLds> L;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -457,57 +418,29 @@ __global__ __launch_bounds__(64 * WAVES, R == 1 ? 3 : 2) void cache_attn_kernel(
         split = i % splits;
     }
     const int tile_id = tile % p.qtiles, rest = tile / p.qtiles, h = rest % p.Hk, b = rest / p.Hk;
-    const int n0 = tile_id * WAVES * R * p.QW;
-    if constexpr (!DENSE) load_tokens(p, L, b, h, n0);
-    Row row[R];
-    bf16x8 qf[R][4];   // step ds: dims 32 (ds / 2) + 16 hh + 8 (ds % 2) .. (see qcache.h)
-    float qc = 0.f;
-#pragma unroll
-    for (int g = 0; g < R; ++g) {
-        if constexpr (DENSE) row[g].init(p, [&](int i) { return min(n0 + i, p.Nq - 1); }, b, h, n0, wave * R + g, lane & 31);
-        else row[g].init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
-        const bf16_t* qr = p.q + b * p.q_sb + row[g].n * p.q_sn + row[g].head * p.q_sh + 16 * hh;
-#pragma unroll
-        for (int ds = 0; ds < 4; ++ds) qf[g][ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
+    const int n0 = tile_id * WAVES * p.QW;
+    Row row;
+    if constexpr (DENSE) row.init(p, [&](int i) { return min(n0 + i, p.Nq - 1); }, b, h, n0, wave, lane & 31);
+    else {
+        load_tokens(p, L, b, h, n0);
+        row.init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
     }
+    bf16x8 qf[4];   // step ds: dims 32 (ds / 2) + 16 hh + 8 (ds % 2) .. (see qcache.h)
+    const bf16_t* qr = p.q + b * p.q_sb + row.n * p.q_sn + row.head * p.q_sh + 16 * hh;
 #pragma unroll
-    for (int g = 0; g < R; ++g) {
-        arrived(qf[g]);
-        float square = 0.f;
-#pragma unroll
-        for (int ds = 0; ds < 4; ++ds) {
-            const uint4 u = __builtin_bit_cast(uint4, qf[g][ds]);
-            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) square = fmaf(bf_lo(x[i]), bf_lo(x[i]), fmaf(bf_hi(x[i]), bf_hi(x[i]), square));
-        }
-        square = wave_max_nonneg(xor32_add(square));
-        qc = square > qc || square != square ? square : qc;   // (a NaN stays)
-    }
-    qc = sqrtf(qc) * p.c * 1.001f;   // a little more than its roundings
-    bool any = false;
-#pragma unroll
-    for (int g = 0; g < R; ++g) any = any || row[g].live;
-    const int wave_live = __builtin_amdgcn_ballot_w64(any) ? -1 : 0;   // (a wave without rows only stages)
-    auto part = [&](int g) { return (int64_t)(tile - p.whole) * (WAVES * R * kRows) + (wave * R + g) * kRows + (lane & 31); };
-    if (splits > 1 && split == 0 && hh == 0)
-#pragma unroll
-        for (int g = 0; g < R; ++g) p.part_at[part(g)] = row[g].live ? row[g].at : -1;
-    AttnState a[R];
-    bool ok[R], all = true;
-    attend<FP8, DENSE, false, WAVES, R>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
-#pragma unroll
-    for (int g = 0; g < R; ++g) {
-        const bool fine = finite(a[g].o[0]) && finite(a[g].o[1]) && a[g].l - a[g].l == 0.f && !a[g].wide;
-        ok[g] = fine && __shfl_xor((int)fine, 32);   // (both halves of the row)
-        all = all && ok[g];
-        if (row[g].live && ok[g]) put_row(p, row[g], part(g), split, splits, a[g]);
-    }
-    if (!__syncthreads_or(!all)) return;
-    attend<FP8, DENSE, true, WAVES, R>(p, L, b, h, n0, split, splits, row, wave_live, qc, qf, a);
-#pragma unroll
-    for (int g = 0; g < R; ++g)
-        if (row[g].live && !ok[g]) put_row(p, row[g], part(g), split, splits, a[g]);
+    for (int ds = 0; ds < 4; ++ds) qf[ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
+    const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
+    const int64_t part = (int64_t)(tile - p.whole) * (WAVES * kRows) + wave * kRows + (lane & 31);
+    if (splits > 1 && split == 0 && hh == 0) p.part_at[part] = row.live ? row.at : -1;
+    AttnState a;
+    attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, qf, a);
+    const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
+    const int other = __shfl_xor((int)fine, 32);   // (the other half of the row)
+    const bool ok = !row.live || (fine && other);
+    if (row.live && ok) put_row(p, row, part, split, splits, a);
+    if (!__syncthreads_or(!ok)) return;
+    attend<FP8, DENSE, true, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, qf, a);
+    if (row.live && !ok) put_row(p, row, part, split, splits, a);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -838,7 +771,7 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     } else {
         const int64_t most = K > 0 ? std::min(K, kMaxSplit) : std::max<int64_t>(1, c.num_blocks / 4);
         if (K == 0 && (int64_t)nq * G * heads >= kWideRows) a.waves = 12;
-        const int64_t per = a.waves * (kRows / G), slots = K > 0 ? 512 : a.waves == 12 ? 256 : 768;
+        const int64_t per = a.waves * (kRows / G), slots = a.waves == 12 ? 256 : K > 0 ? 512 : 768;
         a.qtiles = (nq + per - 1) / per;
         a.tiles = a.qtiles * heads;
         // full rounds of the chip, and the rest's keys in shares that fill it once more (sets: where there is no full round)
@@ -909,9 +842,9 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     const void* fn;
     if (small) fn = fp8 ? (sets ? (const void*)&cache_attn_few_kernel<true, false> : (const void*)&cache_attn_few_kernel<true, true>)
                         : (sets ? (const void*)&cache_attn_few_kernel<false, false> : (const void*)&cache_attn_few_kernel<false, true>);
-    else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false, 4, 1> : (const void*)&cache_attn_kernel<false, false, 4, 1>;
-    else if (plan.waves == 12) fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 12, 1> : (const void*)&cache_attn_kernel<false, true, 12, 1>;
-    else fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 4, 1> : (const void*)&cache_attn_kernel<false, true, 4, 1>;
+    else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false, 4> : (const void*)&cache_attn_kernel<false, false, 4>;
+    else if (plan.waves == 12) fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 12> : (const void*)&cache_attn_kernel<false, true, 12>;
+    else fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 4> : (const void*)&cache_attn_kernel<false, true, 4>;
     if (launch(fn, dim3(total), args, s, 64 * plan.waves) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
     void* jargs[] = {&p};
