@@ -335,11 +335,11 @@ struct Walk {
             meet(t >> shift);
             if constexpr (F == kBounded && DENSE) attend_whole(L.tile[t & 1], qf, member, ft, a, stage);
             else {
-                stage();
                 if (of != 0) {
                     if constexpr (F == kBounded) attend_whole(L.tile[t & 1], qf, member, ft, a, [] {});
                     else attend_tile<F>(L.tile[t & 1], qf, member, 64, ft, a);
                 }
+                stage();
             }
         }
         lds_barrier();
