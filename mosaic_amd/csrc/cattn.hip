@@ -54,16 +54,15 @@ struct AttnState {
     f32x16 o[2];      // O^T [dim tile]
     float m, l;       // reference of the scores, and this lane's part of the sum
     bool has;         // a key above -inf was met
-    bool wide;        // so was a scale of values that kSafe is for
+    bool wide;        // so was a scale of values that SAFE is for
 };
 
-// How a tile is computed.  kBounded: no score exceeds kBound (|q| and the blocks' norms say so): the reference
-// is 0.  kRunning: it is 0 too unless a score leaves +- kBound, and moves then, so that a row's bits do not
-// depend on the form, nor so on the rows beside it.  kSafe: for rows that end with a value that is not finite,
-// and for scales of values further than kSpread from 1: the reference is the maximum, and a row's
+// How a tile is computed.  attend_whole: no score exceeds kBound (|q| and the blocks' norms say so), and the
+// reference is 0.  attend_tile: it is 0 too unless a score leaves +- kBound, and moves then, so that a row's bits
+// do not depend on the form, nor so on the rows beside it.  SAFE: for rows that end with a value that is not
+// finite, and for scales of values further than kSpread from 1: the reference is the maximum, and a row's
 // accumulators take nothing from a block that it has not, not even 0 * NaN.
-enum Form { kBounded, kRunning, kSafe };
-constexpr float kBound = 90.f;       // (with kSpread: P >= 2^-120, and an overflow of its sums ends in kSafe)
+constexpr float kBound = 90.f;       // (with kSpread: P >= 2^-120, and an overflow of its sums ends in SAFE)
 constexpr float kSpread = 0x1p30f;
 
 // x a + b in two roundings
@@ -81,20 +80,20 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int left) {
 }
 
 // P of 8 scores, as an operand
-template <Form F>
+template <bool SAFE>
 __device__ __forceinline__ bf16x8 weights(const f32x16& s, int s2, float ck, float ref) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float x = s[8 * s2 + 2 * i], y = s[8 * s2 + 2 * i + 1];
         // (of scores past 2^30 the fused form leaves more than fp32's exponents beside their rounded maximum)
-        w[i] = F == kSafe ? pack_bf16x2(__builtin_amdgcn_exp2f(times_plus(x, ck, ref)), __builtin_amdgcn_exp2f(times_plus(y, ck, ref)))
+        w[i] = SAFE ? pack_bf16x2(__builtin_amdgcn_exp2f(times_plus(x, ck, ref)), __builtin_amdgcn_exp2f(times_plus(y, ck, ref)))
                           : pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(x, ck, ref)), __builtin_amdgcn_exp2f(fmaf(y, ck, ref)));
     }
     return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
 }
 
-// Factors of a block's scales: scores by ck = c ks; P times 2^lv = vs, and iv = 1 / vs for the sum of P (kSafe:
+// Factors of a block's scales: scores by ck = c ks; P times 2^lv = vs, and iv = 1 / vs for the sum of P (SAFE:
 // lv = vs itself, iv an addend of the scores that is 0 or NaN).  A scale of 0 stands for zeros only: any
 // positive one does.  A NaN among them goes where only the members of the block meet it.
 struct Factors { float ck, lv, iv; };
@@ -109,7 +108,7 @@ __device__ __forceinline__ Factors factors(float c, float ks, float vs, bool& wi
         f.iv = poison;
     } else {
         const bool near = vs <= kSpread && vs >= 1.f / kSpread;
-        wide = !near && vs != 0.f;   // (a NaN too: kSafe leaves it a NaN)
+        wide = !near && vs != 0.f;   // (a NaN too: SAFE leaves it a NaN)
         const float of = near ? vs : 1.f;
         f.lv = __builtin_amdgcn_logf(of) + poison;
         f.iv = 1.f / of;
@@ -125,7 +124,7 @@ struct TileRead {
 };
 
 // One tile of 64 keys; valid: how many of them exist.
-template <Form F>
+template <bool SAFE>
 __device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 (&qf)[4], bool member, int valid, const Factors& f, AttnState& a) {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const TileRead t{tile, lane};
@@ -139,35 +138,33 @@ __device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 
         mask_scores(s[0], valid - 16 * hh);
         mask_scores(s[1], valid - 32 - 16 * hh);
     }
-    if constexpr (F != kBounded) {
-        float mt = s[0][0];
+    float mt = s[0][0];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
-        mt = xor32_max(mt) * f.ck;
-        const bool some = member && mt > -INFINITY;
-        const bool move = some && (F == kSafe ? !a.has || mt > a.m : mt > a.m + kBound || (!a.has && mt < -kBound));
-        if (__builtin_amdgcn_ballot_w64(move)) {
-            const float alpha = move && a.has ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
-            a.m = move ? mt : a.m;
-            a.o[0] *= alpha;
-            a.o[1] *= alpha;
-            a.l *= alpha;
-        }
-        a.has = a.has || some;
+        for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
+    mt = xor32_max(mt) * f.ck;
+    const bool some = member && mt > -INFINITY;
+    const bool move = some && (SAFE ? !a.has || mt > a.m : mt > a.m + kBound || (!a.has && mt < -kBound));
+    if (__builtin_amdgcn_ballot_w64(move)) {
+        const float alpha = move && a.has ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
+        a.m = move ? mt : a.m;
+        a.o[0] *= alpha;
+        a.o[1] *= alpha;
+        a.l *= alpha;
     }
-    const float ref = member ? (F == kSafe ? f.iv : f.lv) - a.m : -INFINITY;   // P = 0 for the others
+    a.has = a.has || some;
+    const float ref = member ? (SAFE ? f.iv : f.lv) - a.m : -INFINITY;   // P = 0 for the others
     bf16x8 pb[2][2];
     float lt = 0.f;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-            pb[kt][s2] = weights<F>(s[kt], s2, f.ck, ref);
+            pb[kt][s2] = weights<SAFE>(s[kt], s2, f.ck, ref);
             lt = operand_sum(pb[kt][s2], lt);
         }
-    if constexpr (F == kSafe) {
+    if constexpr (SAFE) {
         if (member) a.l += lt;
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) {
@@ -190,7 +187,7 @@ __device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 
     }
 }
 
-// A whole tile of kBounded, laid out for the matrix pipe and the vector ALU to run side by side within a wave:
+// A whole tile of bounded scores, laid out for the matrix pipe and the vector ALU to run side by side within a wave:
 // the scores of the first 32 keys, under them the staging of the next tile; those of the others, under them the
 // first weights; the product of these, under it the other weights; their product, under what comes next.
 template <typename Stage>
@@ -214,7 +211,7 @@ __device__ __forceinline__ void attend_whole(const CacheTile& tile, const bf16x8
     for (int s2 = 0; s2 < 2; ++s2) {
         u = mfma32(x[2 * s2], qf[2 * s2], u);
         u = mfma32(x[2 * s2 + 1], qf[2 * s2 + 1], u);
-        p[s2] = weights<kBounded>(s, s2, f.ck, ref);
+        p[s2] = weights<false>(s, s2, f.ck, ref);
         lt = operand_sum(p[s2], lt);
         x[2 * s2] = t.val(0, 0, s2);
         x[2 * s2 + 1] = t.val(0, 1, s2);
@@ -224,7 +221,7 @@ __device__ __forceinline__ void attend_whole(const CacheTile& tile, const bf16x8
     for (int s2 = 0; s2 < 2; ++s2) {
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) a.o[dt] = mfma32(x[2 * s2 + dt], p[s2], a.o[dt]);
-        w[s2] = weights<kBounded>(u, s2, f.ck, ref);
+        w[s2] = weights<false>(u, s2, f.ck, ref);
         lt = operand_sum(w[s2], lt);
         x[2 * s2] = t.val(1, 0, s2);
         x[2 * s2 + 1] = t.val(1, 1, s2);
@@ -293,20 +290,15 @@ struct Walk {
         load(__builtin_amdgcn_readlane(block, 0), 0, r);
         bool wide;
         const Factors f = factors<SAFE>(p.c, ks, vs, wide);
-        if constexpr (SAFE) tiles<kSafe>(count, block, members, f, r);
-        else {
+        bool bounded = false;
+        if constexpr (!SAFE) {
             for (uint64_t far = __builtin_amdgcn_ballot_w64(wide); far != 0; far &= far - 1)
                 a.wide = a.wide || DENSE || row.in((uint32_t)__builtin_amdgcn_readlane(members, (int)__builtin_ctzll(far)));
-            // (a NaN is not bounded; a wave by itself: the forms have the same barriers)
-            if (__builtin_amdgcn_ballot_w64(!(norm * bound() <= kBound) || a.m != 0.f)) tiles<kRunning>(count, block, members, f, r);
-            else tiles<kBounded>(count, block, members, f, r);
+            // (a NaN is not bounded; a wave by itself: the barriers are the same)
+            bounded = __builtin_amdgcn_ballot_w64(!(norm * bound() <= kBound) || a.m != 0.f) == 0;
         }
-    }
-    template <Form F>
-    __device__ __forceinline__ void tiles(int count, int block, int members, const Factors& f, Staged& r) {
         count = __builtin_amdgcn_readfirstlane(count);
-        // Tile t is part t % sub of block t / sub.  Only the sequence's last one may be short, and it is left to the
-        // end: with one way through the loop the accumulators stay where they are.
+        // Tile t is part t % sub of block t / sub; only the sequence's last one may be short.
         const int shift = p.bs == 64 ? 0 : p.bs == 128 ? 1 : 2, sub = 1 << shift;
         const int rest = end - __builtin_amdgcn_readlane(block, count - 1) * p.bs;   // keys from the last block on
         const int total = ((count - 1) << shift) + min(sub, (rest + 63) / 64), whole = ((count - 1) << shift) + min(sub, rest / 64);
@@ -319,53 +311,60 @@ struct Walk {
             of = (uint32_t)__builtin_amdgcn_readlane(members, i);
             ft = Factors{lane_f(f.ck), lane_f(f.lv), lane_f(f.iv)};
             member = DENSE || row.in(of);   // (rows that do not exist are not stored)
-            if (F == kBounded) a.has = a.has || member;
+        };
+        int t = 0;
+        // (past the last tile the staged one is put and loaded once more, to no effect: no branch in the way)
+        auto stage = [&] {
+            put(~t & 1, r);
+            __builtin_amdgcn_sched_barrier(0);   // (r is free before it is loaded again)
+            fetch(min(t + 2, total - 1));
         };
         put(0, r);
         fetch(min(1, total - 1));
-        int t = 0;
-        for (; t < whole; ++t) {
-            lds_barrier();
-            // (past the last tile the staged one is put and loaded once more, to no effect: no branch in the way)
-            auto stage = [&] {
-                put(~t & 1, r);
-                __builtin_amdgcn_sched_barrier(0);   // (r is free before it is loaded again)
-                fetch(min(t + 2, total - 1));
-            };
-            meet(t >> shift);
-            if constexpr (F == kBounded && DENSE) attend_whole(L.tile[t & 1], qf, member, ft, a, stage);
-            else {
-                if (of != 0) {
-                    if constexpr (F == kBounded) attend_whole(L.tile[t & 1], qf, member, ft, a, [] {});
-                    else attend_tile<F>(L.tile[t & 1], qf, member, 64, ft, a);
+        // Two loops, each with one way through, so that the accumulators stay where they are
+        if (bounded)
+            for (; t < whole; ++t) {
+                lds_barrier();
+                meet(t >> shift);
+                a.has = a.has || member;
+                if constexpr (DENSE) attend_whole(L.tile[t & 1], qf, member, ft, a, stage);
+                else {
+                    if (of != 0) attend_whole(L.tile[t & 1], qf, member, ft, a, [] {});
+                    stage();
                 }
-                stage();
             }
-        }
-        lds_barrier();
-        if (t < total) {
-            meet(t >> shift);
-            if (of != 0) attend_tile<F>(L.tile[t & 1], qf, member, rest & 63, ft, a);
+        for (; t < total; ++t) {
             lds_barrier();
+            meet(t >> shift);
+            stage();
+            if (of != 0) attend_tile<SAFE>(L.tile[t & 1], qf, member, t < whole ? 64 : rest & 63, ft, a);
         }
-        // (the buffers are free for the next blocks)
+        lds_barrier();   // the buffers are free for the next blocks
     }
 };
 
 template <bool FP8, bool DENSE, bool SAFE, int WAVES, typename Lds>
 __device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, int h, int n0, int split, int splits, const Row& row, int wave_live,
-                                       const bf16x8 (&qf)[4], AttnState& a) {
+                                       AttnState& a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     a.o[0] = a.o[1] = splat(0.f);
     a.m = a.l = 0.f;
     a.has = a.wide = false;
     const int end = seq_keys(p, b);
+    bf16x8 qf[4];   // step ds: dims 32 (ds / 2) + 16 hh + 8 (ds % 2) .. (see qcache.h)
+    auto load_q = [&] {
+        const bf16_t* qr = p.q + b * p.q_sb + row.n * p.q_sn + row.head * p.q_sh + 16 * (lane >> 5);
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) qf[ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
+    };
     Walk<FP8, DENSE, SAFE, WAVES, Lds> walk{p, L, b, h, end, qf, row, a};
     const int live = (int)(((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
     if constexpr (DENSE) {
+        load_q();
         const int first = (int)((int64_t)live * split / splits), past = (int)((int64_t)live * (split + 1) / splits);
         for (int e0 = first; e0 < past; e0 += 64) walk.blocks(min(64, past - e0), min(e0 + lane, past - 1), wave_live);
     } else {
+        load_q();
         const bool by_block = p.keys != nullptr;
         for (int c0 = 0; c0 < live; c0 += kUnion) {
             const int found = unite(p, L, b, h, n0, end, c0, min(kUnion, live - c0), split, by_block ? splits : 1);
@@ -425,21 +424,17 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_kernel(CacheAttnPara
         load_tokens(p, L, b, h, n0);
         row.init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
     }
-    bf16x8 qf[4];   // step ds: dims 32 (ds / 2) + 16 hh + 8 (ds % 2) .. (see qcache.h)
-    const bf16_t* qr = p.q + b * p.q_sb + row.n * p.q_sn + row.head * p.q_sh + 16 * hh;
-#pragma unroll
-    for (int ds = 0; ds < 4; ++ds) qf[ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
     const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
     const int64_t part = (int64_t)(tile - p.whole) * (WAVES * kRows) + wave * kRows + (lane & 31);
     if (splits > 1 && split == 0 && hh == 0) p.part_at[part] = row.live ? row.at : -1;
     AttnState a;
-    attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, qf, a);
+    attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, a);
     const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
     const int other = __shfl_xor((int)fine, 32);   // (the other half of the row)
     const bool ok = !row.live || (fine && other);
     if (row.live && ok) put_row(p, row, part, split, splits, a);
     if (!__syncthreads_or(!ok)) return;
-    attend<FP8, DENSE, true, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, qf, a);
+    attend<FP8, DENSE, true, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, a);
     if (row.live && !ok) put_row(p, row, part, split, splits, a);
 }
 
