@@ -670,39 +670,47 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
 
 // ------------------------------------------------------------------ joins
 
-// Joins the splits' partials: 16 lanes a row, 4 dims each, and TEAM such groups a row that take its splits
-// in turn (of few splits one, of many all 16 of a workgroup).
+// Joins the splits' partials: 16 lanes a row, 4 dims each, and TEAM such groups a row that take its splits in
+// turn, up to 16 each: one for up to 16 splits, 16 for up to 64, 64 (a workgroup of 1024 threads) for more.  A
+// lane holds the weight of one split, and the first of the partials are on their way before the weights are known.
+constexpr int kJoinMost = 1024;
 template <int TEAM>
-__global__ __launch_bounds__(kThreads) void cache_attn_join_kernel(CacheAttnParams p) {
-    __shared__ __attribute__((aligned(16))) float4 part[16][16];
-    __shared__ float ml[16], sums[16];
+__global__ __launch_bounds__(TEAM == 64 ? 1024 : kThreads) void cache_attn_join_kernel(CacheAttnParams p) {
+    constexpr int kGroups = TEAM == 64 ? 64 : kThreads / 16, kAhead = 4;
+    __shared__ float4 part[TEAM == 1 ? 1 : kGroups][16];
+    __shared__ float most[kGroups], sums[kGroups];
     const int group = threadIdx.x / 16, j = threadIdx.x % 16, d = 4 * j, of = group % TEAM;
-    const int64_t rows = p.parts, mine = (int64_t)blockIdx.x * (16 / TEAM) + group / TEAM, row = mine < rows ? mine : rows - 1;
+    const int64_t rows = p.parts, mine = (int64_t)blockIdx.x * (kGroups / TEAM) + group / TEAM, row = mine < rows ? mine : rows - 1;
     const int64_t at = p.part_at != nullptr ? p.part_at[row] : row;
-    if (TEAM > 1 && at < 0) return;   // (all of a workgroup)
-    float m = -INFINITY;
-    for (int s = of + TEAM * j; s < p.splits; s += 16 * TEAM) {
-        const float2 x = p.part_ml[s * rows + row];
-        m = x.y == 0.f ? m : fmaxf(m, x.x);   // l = 0: no key in that share
-    }
+    const int n = of < p.splits ? (p.splits - of + TEAM - 1) / TEAM : 0;   // splits of the group: of + TEAM i
+    auto o_of = [&](int i) { return *reinterpret_cast<const float4*>(p.part_o + ((of + TEAM * i) * rows + row) * 64 + d); };
+    const float2 ml = j < n ? p.part_ml[(of + TEAM * j) * rows + row] : make_float2(0.f, 0.f);
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = n > 0 ? o_of(min(i, n - 1)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = ml.y == 0.f ? -INFINITY : ml.x;   // l = 0: no key in that share
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     if constexpr (TEAM > 1) {
-        if (j == 0) ml[group] = m;
+        if (j == 0) most[group] = m;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < TEAM; ++i) m = fmaxf(m, ml[group / TEAM * TEAM + i]);
+        for (int i = 0; i < TEAM; i += 16) m = fmaxf(m, most[group / TEAM * TEAM + i + j]);
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     }
+    const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m) * ml.y;
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int s = of; s < p.splits; s += TEAM) {
-        const float2 x = p.part_ml[s * rows + row];
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * 64 + d);
-        const float f = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - m) * x.y;
+    auto add = [&](int i, const float4& y) {
+        const float f = __shfl(w, (threadIdx.x & 48) + i);
         l += f;
         o.x = fmaf(f, y.x, o.x); o.y = fmaf(f, y.y, o.y); o.z = fmaf(f, y.z, o.z); o.w = fmaf(f, y.w, o.w);
-    }
+    };
+    // (16 steps in all groups of a wave, so that every lane is there for the exchange; beyond n weights are 0)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) add(i, ahead[i]);
+    for (int i = kAhead; i < (p.splits + TEAM - 1) / TEAM; ++i) add(i, n > 0 ? o_of(min(i, n - 1)) : make_float4(0.f, 0.f, 0.f, 0.f));
     if constexpr (TEAM > 1) {
         part[group][j] = o;
         if (j == 0) sums[group] = l;
@@ -710,7 +718,7 @@ __global__ __launch_bounds__(kThreads) void cache_attn_join_kernel(CacheAttnPara
         if (of != 0) return;
         o = make_float4(0.f, 0.f, 0.f, 0.f);
         l = 0.f;
-#pragma unroll
+#pragma unroll 16
         for (int i = 0; i < TEAM; ++i) {
             const float4 y = part[group + i][j];
             l += sums[group + i];
@@ -739,7 +747,12 @@ int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, 
     return MOSAIC_OK;
 }
 
-constexpr int64_t kFewGroups = 1024, kFewTiles = 2, kWideRows = 32768;
+// Shares of the keys of few rows: four workgroups a CU, where a row has no more than kFewShares then, and else one a
+// CU: its join is the longer (one point over 196608 keys, 75 MB in e4m3: 20.5 us in 85 shares of each head, 23.3 in
+// 170 and in 341; 24 tracks of 16 heads, 113 MB in int8: 25 us in 10 shares, 29 in 2).
+constexpr int64_t kFewGroups = 1024, kFewShares = 64, kFewTiles = 8;
+static_assert(kJoinMost >= kFewGroups, "the join takes every share");
+constexpr int64_t kWideRows = 32768;
 
 // Whether the call is one of cache_attn_few_kernel
 bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
@@ -761,7 +774,9 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     if (few(c, nq, hq, K)) {
         const int64_t tiles = K > 0 ? nq * K * sub : c.num_blocks * sub;
         a.tiles = heads;
-        a.splits = std::max<int64_t>(1, std::min(kFewGroups / heads, tiles / (kWaves * kFewTiles)));
+        a.splits = kFewGroups / heads;
+        if (a.splits > kFewShares) a.splits = std::max(kFewShares, 256 / heads);
+        a.splits = std::max<int64_t>(1, std::min(a.splits, tiles / (kWaves * kFewTiles)));
         a.parts = (int64_t)c.batch * nq * hq;
     } else {
         const int64_t most = K > 0 ? std::min(K, kMaxSplit) : std::max<int64_t>(1, c.num_blocks / 4);
@@ -843,9 +858,12 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     if (launch(fn, dim3(total), args, s, 64 * plan.waves) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
     void* jargs[] = {&p};
-    const bool team = p.splits > 16;
-    const void* join = team ? (const void*)&cache_attn_join_kernel<16> : (const void*)&cache_attn_join_kernel<1>;
-    return launch(join, dim3((unsigned)(team ? p.parts : (p.parts + 15) / 16)), jargs, s) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+    const int team = p.splits <= 16 ? 1 : p.splits <= 64 ? 16 : 64;
+    const void* join = team == 1    ? (const void*)&cache_attn_join_kernel<1>
+                       : team == 16 ? (const void*)&cache_attn_join_kernel<16>
+                                    : (const void*)&cache_attn_join_kernel<64>;
+    const unsigned groups = (unsigned)(team == 1 ? (p.parts + 15) / 16 : p.parts);
+    return launch(join, dim3(groups), jargs, s, team == 64 ? 1024 : kThreads) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
 
 }  // extern "C"

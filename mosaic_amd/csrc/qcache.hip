@@ -126,7 +126,6 @@ struct Quant {
     }
     // of a code under another scale: code * before is high + low exactly
     __device__ __forceinline__ float requotient(float code, float before) const {
-        if (inv == 0.f) return 0.f;
         const float high = code * before, low = fmaf(code, before, -high);
         const float y = blunt(high * inv);
         return beside(y, fmaf(-y, scale, high) + low);
@@ -143,6 +142,18 @@ __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float 
         auto round = [](float x) { return __float_as_uint(x + 12582912.f); };
         const uint32_t lo = __builtin_amdgcn_perm(round(b), round(a), 0x0c0c0400), hi = __builtin_amdgcn_perm(round(d), round(c), 0x04000c0c);
         return lo | hi;
+    }
+}
+
+// Sixteen codes under a block's scale before, set to its scale now
+template <bool FP8>
+__device__ __forceinline__ void rescale(uint32_t (&w)[4], const Quant& q, float before) {
+    if (q.scale == before) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 c = codes_f32<FP8>(w[i]);
+        const uint32_t x = pack_codes<FP8>(q.requotient(c.x, before), q.requotient(c.y, before), q.requotient(c.z, before), q.requotient(c.w, before));
+        w[i] = q.inv == 0.f ? 0u : x;
     }
 }
 
@@ -288,20 +299,18 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
         float y[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) y[i] = kq.quotient(k[s][i]);
-        if (keeps && 64 * s + kkey < begin) {
-            const uint32_t w[4] = {kwas[s].x, kwas[s].y, kwas[s].z, kwas[s].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 c = codes_f32<FP8>(w[i]);
-                y[4 * i] = kq.requotient(c.x, kold); y[4 * i + 1] = kq.requotient(c.y, kold);
-                y[4 * i + 2] = kq.requotient(c.z, kold); y[4 * i + 3] = kq.requotient(c.w, kold);
-            }
-        }
         uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_codes<FP8>(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+        if (keeps) {
+            uint32_t was[4] = {kwas[s].x, kwas[s].y, kwas[s].z, kwas[s].w};
+            rescale<FP8>(was, kq, kold);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = 64 * s + kkey < begin ? was[i] : w[i];
+        }
         float square = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = pack_codes<FP8>(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
             const float4 c = codes_f32<FP8>(w[i]);
             sum[4 * i] += c.x; sum[4 * i + 1] += c.y; sum[4 * i + 2] += c.z; sum[4 * i + 3] += c.w;
             square = fmaf(c.x, c.x, fmaf(c.y, c.y, fmaf(c.z, c.z, fmaf(c.w, c.w, square))));
@@ -309,26 +318,18 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CacheParams p)
         squares[s][wave][lane & 31] = xor32_add(square);   // (both halves the same)
         reinterpret_cast<uint4*>(kc + s * kCodeTile)[tid] = make_uint4(w[0], w[1], w[2], w[3]);
 
-        uint32_t x[4];
-        uint32_t was[4];
-        const bool kept = keeps && 64 * s + vkey < begin;
-        if (keeps) {   // word d: dim vdim + d of this lane's four tokens
-            was[0] = vwas[s].x; was[1] = vwas[s].y; was[2] = vwas[s].z; was[3] = vwas[s].w;
+        uint32_t x[4];   // word d: dim vdim + d of this lane's four tokens
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+            x[d] = pack_codes<FP8>(vq.quotient(v[s][0][d]), vq.quotient(v[s][1][d]), vq.quotient(v[s][2][d]), vq.quotient(v[s][3][d]));
+        if (keeps) {
+            uint32_t was[4] = {vwas[s].x, vwas[s].y, vwas[s].z, vwas[s].w};
             quad_transpose(was);
-        }
+            rescale<FP8>(was, vq, vold);
+            const int kept = min(max(begin - (64 * s + vkey), 0), 4);   // of the four
+            const uint32_t mask = kept == 4 ? ~0u : (1u << (8 * kept)) - 1u;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            float z[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = vq.quotient(v[s][i][d]);
-            if (kept) {
-                const float4 c = codes_f32<FP8>(was[d]);
-                const float old[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (64 * s + vkey + i < begin) z[i] = vq.requotient(old[i], vold);
-            }
-            x[d] = pack_codes<FP8>(z[0], z[1], z[2], z[3]);
+            for (int d = 0; d < 4; ++d) x[d] = (x[d] & ~mask) | (was[d] & mask);
         }
         quad_transpose(x);
         reinterpret_cast<uint4*>(vc + s * kCodeTile)[vchunk] = make_uint4(x[0], x[1], x[2], x[3]);

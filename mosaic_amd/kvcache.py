@@ -69,6 +69,21 @@ class KVCache:
         self._k_codes, self._v_codes = (torch.zeros(*shape, block_size * 64, dtype=torch.uint8, device=device) for _ in range(2))
         self._k_scale, self._v_scale, self._k_norm = (torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(3))
         self._k_mean = torch.zeros(*shape, 64, dtype=torch.bfloat16, device=device)
+        self._describe()
+
+    def _describe(self) -> None:
+        """The storage as the library takes it: made once, the tensors being the cache's own for its life."""
+        B, nb, Hk, bs, capacity = self._sizes
+        self._device = self._k_codes.device
+        self._c = _lib.Cache(self._k_codes.data_ptr(), self._v_codes.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr(),
+                             self._k_norm.data_ptr(), self._k_mean.data_ptr(), B, nb, Hk, bs, _CODES[self._dtype], capacity)
+
+    def __getstate__(self) -> dict:   # (copies and pickles: of the tensors, not of where they lie)
+        return {name: x for name, x in self.__dict__.items() if name not in ("_c", "_device")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._describe()
 
     batch = property(lambda self: self._sizes[0])
     num_blocks = property(lambda self: self._sizes[1])
@@ -76,18 +91,13 @@ class KVCache:
     block_size = property(lambda self: self._sizes[3])
     capacity = property(lambda self: self._sizes[4])
     dtype = property(lambda self: self._dtype)
-    device = property(lambda self: self._k_codes.device)
+    device = property(lambda self: self._device)
     k_codes = property(lambda self: self._k_codes)
     v_codes = property(lambda self: self._v_codes)
     k_scale = property(lambda self: self._k_scale)
     v_scale = property(lambda self: self._v_scale)
     k_norm = property(lambda self: self._k_norm)
     k_mean = property(lambda self: self._k_mean)
-
-    def _as_c(self) -> _lib.Cache:
-        B, nb, Hk, bs, capacity = self._sizes
-        return _lib.Cache(self._k_codes.data_ptr(), self._v_codes.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr(),
-                          self._k_norm.data_ptr(), self._k_mean.data_ptr(), B, nb, Hk, bs, _CODES[self._dtype], capacity)
 
     def __repr__(self) -> str:
         B, _, Hk, bs, capacity = self._sizes
@@ -97,7 +107,8 @@ class KVCache:
 
 def _no_gradient(what: str, **tensors) -> None:
     """Refuses inputs that autograd would follow, in either mode."""
-    forward_only(what, *tensors.values())
+    if torch.is_grad_enabled():
+        forward_only(what, *tensors.values())
     if forward_ad._current_level >= 0:
         for name, t in tensors.items():
             if forward_ad.unpack_dual(t).tangent is not None:
@@ -146,15 +157,15 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: int 
     more holds zeros; one with a value that is not finite holds NaN throughout.
     """
     what = "kv_cache_write"
-    B, _, Hk, _, capacity = cache._sizes
-    for name, t in (("k", k), ("v", v)):
-        if t.dim() != 4 or t.shape[0] != B or t.shape[2:] != (Hk, 64):
-            raise ValueError(f"{what}: {name} {tuple(t.shape)} must be [B, n, kv_heads, 64] = {(B, '*', Hk, 64)}")
-        if t.dtype not in _DT:
-            raise TypeError(f"{what}: {name} is {t.dtype}; bfloat16 and float32 are quantised")
-    if k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"{what}: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} disagree")
-    n = k.shape[1]
+    B, _, Hk, _, _ = cache._sizes
+    shape, dtype, device = k.shape, k.dtype, cache._device
+    if len(shape) != 4 or shape[0] != B or shape[2] != Hk or shape[3] != 64:
+        raise ValueError(f"{what}: k {tuple(shape)} must be [B, n, kv_heads, 64] = {(B, '*', Hk, 64)}")
+    if dtype not in _DT:
+        raise TypeError(f"{what}: k is {dtype}; bfloat16 and float32 are quantised")
+    if v.shape != shape or v.dtype != dtype:
+        raise ValueError(f"{what}: k {tuple(shape)} {dtype} and v {tuple(v.shape)} {v.dtype} disagree")
+    n = shape[1]
     if n >= 1 << 31:
         raise ValueError(f"{what}: {n} tokens are 2^31 or more")
     _no_gradient(what, k=k, v=v)
@@ -166,9 +177,8 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: int 
         return
     starts, counts = _int32(starts, -1 << 31, (1 << 31) - 1), _int32(counts, 0, n)
     (k, kb), (v, vb) = _rows(k), _rows(v)
-    with _on(cache.device):
-        st = _lib.lib().mosaic_kv_cache_write(ctypes.byref(cache._as_c()), kb, vb, _DT[k.dtype], 64, n, start, _ptr(starts), _ptr(counts),
-                                              _stream(cache.device))
+    with _on(device):
+        st = _lib.lib().mosaic_kv_cache_write(ctypes.byref(cache._c), kb, vb, _DT[dtype], 64, n, start, _ptr(starts), _ptr(counts), _stream(device))
     _lib.check(st, "mosaic_kv_cache_write")
 
 
@@ -182,6 +192,7 @@ def kv_cache_read(cache: KVCache, start: int | torch.Tensor = 0, count: int | No
     """
     what = "kv_cache_read"
     B, _, Hk, _, capacity = cache._sizes
+    device = cache._device
     if dtype not in _DT:
         raise TypeError(f"{what}: dtype is {dtype}; bfloat16 and float32 are read")
     if count is None:
@@ -193,13 +204,14 @@ def kv_cache_read(cache: KVCache, start: int | torch.Tensor = 0, count: int | No
         raise ValueError(f"{what}: count must be in [0, 2^31), got {count}")
     start, starts = _run(what, cache, start, count)
     _same_device(what, cache._k_codes, start=starts)
-    k, v = (torch.empty(B, count, Hk, 64, dtype=dtype, device=cache.device) for _ in range(2))
+    k = torch.empty(B, count, Hk, 64, dtype=dtype, device=device)
+    v = torch.empty_like(k)
     if count == 0:
         return k, v
     starts = _int32(starts, -1 << 31, (1 << 31) - 1)
-    with _on(cache.device):
-        st = _lib.lib().mosaic_kv_cache_read(ctypes.byref(cache._as_c()), _DT[dtype], 64, count, start, _ptr(starts), k.data_ptr(), v.data_ptr(),
-                                             _stream(cache.device))
+    with _on(device):
+        st = _lib.lib().mosaic_kv_cache_read(ctypes.byref(cache._c), _DT[dtype], 64, count, start, _ptr(starts), k.data_ptr(), v.data_ptr(),
+                                             _stream(device))
     _lib.check(st, "mosaic_kv_cache_read")
     return k, v
 
@@ -252,11 +264,11 @@ def cache_attn(q: torch.Tensor, cache: KVCache, block_indices: torch.Tensor | No
     dtype, device = q.dtype, q.device
     q, qb = _as_bf16(q)
     out = _like(q)
-    L, c = _lib.lib(), cache._as_c()
-    nbytes = L.mosaic_cache_attn_fwd_workspace_size(ctypes.byref(c), Nq, Hq, K)
+    L, c = _lib.lib(), ctypes.byref(cache._c)
+    nbytes = L.mosaic_cache_attn_fwd_workspace_size(c, Nq, Hq, K)
     ws = _scratch(nbytes, device)
     with _on(device):
-        st = L.mosaic_cache_attn_fwd(qb, ctypes.byref(c), _ptr(idx), _ptr(lens), Nq, Hq, d, K, scale, out.data_ptr(), _ptr(ws), nbytes,
+        st = L.mosaic_cache_attn_fwd(qb, c, _ptr(idx), _ptr(lens), Nq, Hq, d, K, scale, out.data_ptr(), _ptr(ws), nbytes,
                                      _stream(device))
     _lib.check(st, "mosaic_cache_attn_fwd")
     return out if dtype is torch.bfloat16 else out.to(dtype)

@@ -324,6 +324,7 @@ def test_c_entry_refuses_arguments():
     assert call(K=-1) == 5 and call(K=3) == 5 and call(idx=FAKE) == 5 and call(idx=FAKE, K=1025) == 11
     assert call(scale=1e-31) == 11 and call(scale=1e31) == 11
     assert call(q=_lib.Bnhd(FAKE + 8, 1920, 384, 64)) == 7 and call(out=FAKE + 4) == 7 and call(idx=FAKE + 4, K=1) == 7 and call(lens=FAKE + 2) == 7
-    need = L.mosaic_cache_attn_fwd_workspace_size(c, 5, 6, 0)
-    assert need > 0 and call(ws=None) == 6 and call(nbytes=need - 1) == 6 and call(ws=FAKE + 16) == 6
+    big = ctypes.byref(_lib.Cache(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 1000, 3, 64, _lib.CODE_INT8, 64000))
+    need = L.mosaic_cache_attn_fwd_workspace_size(big, 5, 6, 0)
+    assert need > 0 and call(ws=None, cache=big) == 6 and call(nbytes=need - 1, cache=big) == 6 and call(ws=FAKE + 16, cache=big) == 6
     assert L.mosaic_cache_attn_fwd_workspace_size(c, 5, 51, 0) == 0

@@ -285,12 +285,23 @@ def test_what_a_cache_says_of_itself():
         c.k_scale = None
 
 
+def test_copies_have_storage_of_their_own():
+    import copy
+    import pickle
+
+    c = cpu_cache()
+    c.k_scale.fill_(2.0)
+    for other in (copy.deepcopy(c), pickle.loads(pickle.dumps(c))):
+        assert torch.equal(other.k_scale, c.k_scale) and other._c.k_scale == other.k_scale.data_ptr() != c.k_scale.data_ptr()
+        assert (other._c.batch, other._c.capacity) == (2, 100) and other.device == c.device
+
+
 K = torch.zeros(2, 5, 3, 64)
 
 
 @pytest.mark.parametrize("k,v,kw,error,match", [
     (K[0], K, {}, ValueError, "k "), (K[:1], K[:1], {}, ValueError, "k "), (K[:, :, :2], K[:, :, :2], {}, ValueError, "k "),
-    (K[..., :32], K[..., :32], {}, ValueError, "k "), (K, K[:, :4], {}, ValueError, "disagree"), (K, K.bfloat16(), {}, ValueError, "disagree"),
+    (K[..., :32], K[..., :32], {}, ValueError, "k "), (K, K[:, :4], {}, ValueError, "disagree"), (K, K[0], {}, ValueError, "disagree"), (K, K.bfloat16(), {}, ValueError, "disagree"),
     (K.half(), K.half(), {}, TypeError, "float16"), (K.double(), K.double(), {}, TypeError, "float64"),
     (K, K, dict(start=-1), ValueError, "cache of 100"), (K, K, dict(start=96), ValueError, "cache of 100"),
     (K, K, dict(start=torch.zeros(3, dtype=torch.int32)), ValueError, "start"), (K, K, dict(start=torch.zeros(2)), TypeError, "start"),
