@@ -295,14 +295,18 @@ struct Walk {
             for (uint64_t far = __builtin_amdgcn_ballot_w64(wide); far != 0; far &= far - 1)
                 a.wide = a.wide || DENSE || row.in((uint32_t)__builtin_amdgcn_readlane(members, (int)__builtin_ctzll(far)));
             // (a NaN is not bounded; a wave by itself: the barriers are the same)
-            bounded = __builtin_amdgcn_ballot_w64(!(norm * bound() <= kBound) || a.m != 0.f) == 0;
+            // (and a wave without rows only stages)
+            bounded = __builtin_amdgcn_ballot_w64(!(norm * bound() <= kBound) || a.m != 0.f || (DENSE && members == 0)) == 0;
         }
         count = __builtin_amdgcn_readfirstlane(count);
         // Tile t is part t % sub of block t / sub; only the sequence's last one may be short.
         const int shift = p.bs == 64 ? 0 : p.bs == 128 ? 1 : 2, sub = 1 << shift;
         const int rest = end - __builtin_amdgcn_readlane(block, count - 1) * p.bs;   // keys from the last block on
         const int total = ((count - 1) << shift) + min(sub, (rest + 63) / 64), whole = ((count - 1) << shift) + min(sub, rest / 64);
-        auto fetch = [&](int t) { load(__builtin_amdgcn_readlane(block, t >> shift), t & (sub - 1), r); };
+        auto fetch = [&](int t, Staged& to) {
+            t = min(t, total - 1);
+            load(__builtin_amdgcn_readlane(block, t >> shift), t & (sub - 1), to);
+        };
         uint32_t of;
         bool member;
         Factors ft;
@@ -314,31 +318,57 @@ struct Walk {
         };
         int t = 0;
         // (past the last tile the staged one is put and loaded once more, to no effect: no branch in the way)
-        auto stage = [&] {
-            put(~t & 1, r);
-            __builtin_amdgcn_sched_barrier(0);   // (r is free before it is loaded again)
-            fetch(min(t + 2, total - 1));
+        // Tiles on their way to registers: two where the accumulators leave room for them
+        constexpr int kAhead = DENSE && !SAFE ? 2 : 1;
+        Staged ahead[kAhead];
+        auto stage = [&](Staged& x) {
+            put(~t & 1, x);
+            __builtin_amdgcn_sched_barrier(0);   // (x is free before it is loaded again)
+            fetch(t + 1 + kAhead, x);
         };
         put(0, r);
-        fetch(min(1, total - 1));
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) fetch(1 + i, ahead[i]);
         // Two loops, each with one way through, so that the accumulators stay where they are
-        if (bounded)
-            for (; t < whole; ++t) {
-                lds_barrier();
-                meet(t >> shift);
-                a.has = a.has || member;
-                if constexpr (DENSE) attend_whole(L.tile[t & 1], qf, member, ft, a, stage);
-                else {
-                    if (of != 0) attend_whole(L.tile[t & 1], qf, member, ft, a, [] {});
-                    stage();
-                }
-            }
-        for (; t < total; ++t) {
+        auto whole_tile = [&](Staged& x) {
             lds_barrier();
             meet(t >> shift);
-            stage();
+            a.has = a.has || member;
+            if constexpr (DENSE) attend_whole(L.tile[t & 1], qf, member, ft, a, [&] { stage(x); });
+            else {
+                if (of != 0) attend_whole(L.tile[t & 1], qf, member, ft, a, [] {});
+                stage(x);
+            }
+            ++t;
+        };
+        auto any_tile = [&](Staged& x) {
+            lds_barrier();
+            meet(t >> shift);
+            stage(x);
             if (of != 0) attend_tile<SAFE>(L.tile[t & 1], qf, member, t < whole ? 64 : rest & 63, ft, a);
+            ++t;
+        };
+        if (bounded) {
+            if constexpr (kAhead == 1)
+                while (t < whole) whole_tile(ahead[0]);
+            else {
+                while (t + 1 < whole) {
+                    whole_tile(ahead[0]);
+                    whole_tile(ahead[1]);
+                }
+                if (t < whole) {
+                    whole_tile(ahead[0]);
+                    ahead[0] = ahead[1];   // (for the last tile, if it is short)
+                }
+            }
         }
+        if constexpr (kAhead == 1)
+            while (t < total) any_tile(ahead[0]);
+        else
+            while (t < total) {
+                any_tile(ahead[0]);
+                if (t < total) any_tile(ahead[1]);
+            }
         lds_barrier();   // the buffers are free for the next blocks
     }
 };
@@ -682,6 +712,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 1024 : kThreads) void cache_attn_join_
     const int group = threadIdx.x / 16, j = threadIdx.x % 16, d = 4 * j, of = group % TEAM;
     const int64_t rows = p.parts, mine = (int64_t)blockIdx.x * (kGroups / TEAM) + group / TEAM, row = mine < rows ? mine : rows - 1;
     const int64_t at = p.part_at != nullptr ? p.part_at[row] : row;
+    if (TEAM > 1 && at < 0) return;   // (all of a workgroup: no such row)
     const int n = of < p.splits ? (p.splits - of + TEAM - 1) / TEAM : 0;   // splits of the group: of + TEAM i
     auto o_of = [&](int i) { return *reinterpret_cast<const float4*>(p.part_o + ((of + TEAM * i) * rows + row) * 64 + d); };
     const float2 ml = j < n ? p.part_ml[(of + TEAM * j) * rows + row] : make_float2(0.f, 0.f);
@@ -752,7 +783,7 @@ int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, 
 // 170 and in 341; 24 tracks of 16 heads, 113 MB in int8: 25 us in 10 shares, 29 in 2).
 constexpr int64_t kFewGroups = 1024, kFewShares = 64, kFewTiles = 8;
 static_assert(kJoinMost >= kFewGroups, "the join takes every share");
-constexpr int64_t kWideRows = 32768;
+constexpr int64_t kWideRows = 1536;   // of a kv head, from which dense workgroups have twelve waves
 
 // Whether the call is one of cache_attn_few_kernel
 bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
@@ -780,7 +811,7 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
         a.parts = (int64_t)c.batch * nq * hq;
     } else {
         const int64_t most = K > 0 ? std::min(K, kMaxSplit) : std::max<int64_t>(1, c.num_blocks / 4);
-        if (K == 0 && (int64_t)nq * G * heads >= kWideRows) a.waves = 12;
+        if (K == 0 && (int64_t)nq * G >= kWideRows) a.waves = 12;
         const int64_t per = a.waves * (kRows / G), slots = a.waves == 12 ? 256 : K > 0 ? 512 : 768;
         a.qtiles = (nq + per - 1) / per;
         a.tiles = a.qtiles * heads;
