@@ -6,8 +6,8 @@
 //   k_u = ks code, v_u = vs code, ks and vs the scales of u's block and head
 // Codes are whole numbers of at most 8 bits or e4m3, exact in bf16, so the products are of bf16 operands
 // without a rounding of theirs.  ks goes into the factor of the scores and vs into the exponent,
-//   P = exp2(c ks q.code_k - m + log2 vs),  O = sum P code_v,  l = sum P / vs,  o = O / l,
-// so that neither costs an instruction per score.  fp32 scores, maxima, sums and accumulators; P is rounded to
+//   P = exp2(c ks q.code_k - m + log2(vs / w)),  O = sum P code_v,  l = sum P w / vs,  o = w O / l,
+// so that neither costs an instruction per score (w: the scale of the sequence's first block).  fp32 scores, maxima, sums and accumulators; P is rounded to
 // bf16 for the product with the values (half a step of bf16 per term, as the output's own rounding), and l sums
 // the rounded P.
 //
@@ -60,10 +60,11 @@ struct AttnState {
 // How a tile is computed.  attend_whole: no score exceeds kBound (|q| and the blocks' norms say so), and the
 // reference is 0.  attend_tile: it is 0 too unless a score leaves +- kBound, and moves then, so that a row's bits
 // do not depend on the form, nor so on the rows beside it.  SAFE: for rows that end with a value that is not
-// finite, and for scales of values further than kSpread from 1: the reference is the maximum, and a row's
+// finite, and for scales of values further than kSpread from w: the reference is the maximum, and a row's
 // accumulators take nothing from a block that it has not, not even 0 * NaN.
-constexpr float kBound = 90.f;       // (with kSpread: P >= 2^-120, and an overflow of its sums ends in SAFE)
-constexpr float kSpread = 0x1p30f;
+// With these P is 2^-100 at least, 26 bits above the smallest normal number; an overflow of its sums ends in SAFE.
+constexpr float kBound = 80.f;
+constexpr float kSpread = 0x1p20f;
 
 // x a + b in two roundings
 __device__ __forceinline__ float times_plus(float x, float a, float b) {
@@ -93,12 +94,19 @@ __device__ __forceinline__ bf16x8 weights(const f32x16& s, int s2, float ck, flo
     return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
 }
 
-// Factors of a block's scales: scores by ck = c ks; P times 2^lv = vs, and iv = 1 / vs for the sum of P (SAFE:
+// What the scales of values are taken relative to: that of the sequence's first block (1 where that is zeros or
+// not finite), so that it does not depend on what else a workgroup computes.
+__device__ __forceinline__ float value_unit(const mosaic_kv_cache& c, int b, int h) {
+    const float vs = c.v_scale[block_at(c, b, 0, h)];
+    return vs > 0.f && vs < INFINITY ? vs : 1.f;
+}
+
+// Factors of a block's scales: scores by ck = c ks; P times 2^lv = vs / w, and iv = w / vs for the sum of P (SAFE:
 // lv = vs itself, iv an addend of the scores that is 0 or NaN).  A scale of 0 stands for zeros only: any
 // positive one does.  A NaN among them goes where only the members of the block meet it.
 struct Factors { float ck, lv, iv; };
 template <bool SAFE>
-__device__ __forceinline__ Factors factors(float c, float ks, float vs, bool& wide) {
+__device__ __forceinline__ Factors factors(float c, float ks, float vs, float w, bool& wide) {
     Factors f;
     f.ck = ks > 0.f ? fminf(fmaxf(c * ks, FLT_MIN), FLT_MAX) : 1.f;
     const float poison = ks - ks;
@@ -107,9 +115,10 @@ __device__ __forceinline__ Factors factors(float c, float ks, float vs, bool& wi
         f.lv = vs;
         f.iv = poison;
     } else {
-        const bool near = vs <= kSpread && vs >= 1.f / kSpread;
+        const float ratio = vs / w;
+        const bool near = ratio <= kSpread && ratio >= 1.f / kSpread;
         wide = !near && vs != 0.f;   // (a NaN too: SAFE leaves it a NaN)
-        const float of = near ? vs : 1.f;
+        const float of = near ? ratio : 1.f;
         f.lv = __builtin_amdgcn_logf(of) + poison;
         f.iv = 1.f / of;
     }
@@ -240,6 +249,7 @@ struct Walk {
     const CacheAttnParams& p;
     Lds& L;
     int b, h, end;
+    float w;        // value_unit
     const bf16x8 (&qf)[4];
     const Row& row;
     AttnState& a;
@@ -289,7 +299,7 @@ struct Walk {
         Staged r;
         load(__builtin_amdgcn_readlane(block, 0), 0, r);
         bool wide;
-        const Factors f = factors<SAFE>(p.c, ks, vs, wide);
+        const Factors f = factors<SAFE>(p.c, ks, vs, w, wide);
         bool bounded = false;
         if constexpr (!SAFE) {
             for (uint64_t far = __builtin_amdgcn_ballot_w64(wide); far != 0; far &= far - 1)
@@ -375,7 +385,7 @@ struct Walk {
 
 template <bool FP8, bool DENSE, bool SAFE, int WAVES, typename Lds>
 __device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, int h, int n0, int split, int splits, const Row& row, int wave_live,
-                                       AttnState& a) {
+                                       float w, AttnState& a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     a.o[0] = a.o[1] = splat(0.f);
     a.m = a.l = 0.f;
@@ -387,7 +397,7 @@ __device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, 
 #pragma unroll
         for (int ds = 0; ds < 4; ++ds) qf[ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
     };
-    Walk<FP8, DENSE, SAFE, WAVES, Lds> walk{p, L, b, h, end, qf, row, a};
+    Walk<FP8, DENSE, SAFE, WAVES, Lds> walk{p, L, b, h, end, w, qf, row, a};
     const int live = (int)(((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
     if constexpr (DENSE) {
         load_q();
@@ -410,11 +420,13 @@ __device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, 
 }
 
 // The result of a row, or its part of it
-__device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row, int64_t part, int split, int splits, AttnState& a) {
+__device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row, int64_t part, int split, int splits, float w, AttnState& a) {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const float l = xor32_add(a.l), f = l == 0.f ? 0.f : 1.f / l;   // (a row without a key, or with none above -inf: zeros)
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) a.o[dt] *= f;   // (before w: 1 / l and w need not fit together)
     if (splits == 1) {
-        store_row(p.out, row.at, lane, a.o, f);
+        store_row(p.out, row.at, lane, a.o, w);
         return;
     }
     float* d = p.part_o + (split * p.parts + part) * 64 + 4 * hh;
@@ -423,7 +435,7 @@ __device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4)
             *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) =
-                make_float4(a.o[dt][4 * g4] * f, a.o[dt][4 * g4 + 1] * f, a.o[dt][4 * g4 + 2] * f, a.o[dt][4 * g4 + 3] * f);
+                make_float4(a.o[dt][4 * g4] * w, a.o[dt][4 * g4 + 1] * w, a.o[dt][4 * g4 + 2] * w, a.o[dt][4 * g4 + 3] * w);
     if (hh == 0) {
         int e = 0;
         const float y = frexpf(l, &e);   // (NaN and infinity stay what they are)
@@ -457,15 +469,16 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_kernel(CacheAttnPara
     const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
     const int64_t part = (int64_t)(tile - p.whole) * (WAVES * kRows) + wave * kRows + (lane & 31);
     if (splits > 1 && split == 0 && hh == 0) p.part_at[part] = row.live ? row.at : -1;
+    const float w = value_unit(p.cache, b, h);
     AttnState a;
-    attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, a);
+    attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, w, a);
     const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
     const int other = __shfl_xor((int)fine, 32);   // (the other half of the row)
     const bool ok = !row.live || (fine && other);
-    if (row.live && ok) put_row(p, row, part, split, splits, a);
+    if (row.live && ok) put_row(p, row, part, split, splits, w, a);
     if (!__syncthreads_or(!ok)) return;
-    attend<FP8, DENSE, true, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, a);
-    if (row.live && !ok) put_row(p, row, part, split, splits, a);
+    attend<FP8, DENSE, true, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, 1.f, a);
+    if (row.live && !ok) put_row(p, row, part, split, splits, 1.f, a);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -500,10 +513,10 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
 }
 
 template <bool FP8, bool SAFE>
-__device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2], bool member, int valid, float c, FewState& a) {
+__device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2], bool member, int valid, float c, float w, FewState& a) {
     const int g = (threadIdx.x & 63) >> 4;
     bool wide;
-    const Factors f = factors<SAFE>(c, t.ks, t.vs, wide);
+    const Factors f = factors<SAFE>(c, t.ks, t.vs, w, wide);
     a.wide = a.wide || (wide && member);
     f32x4 s[4];
 #pragma unroll
@@ -627,6 +640,7 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
         t.vs = p.cache.v_scale[at];
     };
     FewState a;
+    float w = value_unit(p.cache, b, h);
     auto walk = [&](auto safe) {
 #pragma unroll
         for (int dg = 0; dg < 4; ++dg) a.o[dg] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -646,7 +660,7 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
                 load(min(key_next, end - 1), next);
             }
             if (key0 < end)
-                attend_few<FP8, decltype(safe)::value>(t, qf, row_live && (DENSE || (of >> token & 1)), min(64, end - key0), p.c, a);
+                attend_few<FP8, decltype(safe)::value>(t, qf, row_live && (DENSE || (of >> token & 1)), min(64, end - key0), p.c, w, a);
         }
     };
     walk(std::false_type{});
@@ -655,12 +669,15 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
     for (int dg = 0; dg < 4; ++dg)
 #pragma unroll
         for (int i = 0; i < 4; ++i) ok = ok && a.o[dg][i] - a.o[dg][i] == 0.f;
-    if (__builtin_amdgcn_ballot_w64(!ok)) walk(std::true_type{});   // (a wave by itself)
+    if (__builtin_amdgcn_ballot_w64(!ok)) {   // (a wave by itself)
+        w = 1.f;
+        walk(std::true_type{});
+    }
     const float l = xor32_add(xor16_add(a.l)), f = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int dg = 0; dg < 4; ++dg)
         *reinterpret_cast<float4*>(&O[wave][r][(16 * dg + 4 * g) ^ (4 * r)]) =
-            make_float4(a.o[dg][0] * f, a.o[dg][1] * f, a.o[dg][2] * f, a.o[dg][3] * f);
+            make_float4(a.o[dg][0] * f * w, a.o[dg][1] * f * w, a.o[dg][2] * f * w, a.o[dg][3] * f * w);
     if (g == 0) {
         int e = 0;
         const float part = frexpf(l, &e);

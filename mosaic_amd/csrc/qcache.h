@@ -62,7 +62,7 @@ inline int check_cache(const mosaic_kv_cache* c) {
         c->k_norm == nullptr || c->k_mean == nullptr)
         return MOSAIC_ERR_NULL_POINTER;
     if (c->batch <= 0 || c->num_blocks <= 0 || c->capacity <= 0) return MOSAIC_ERR_SHAPE;
-    if (c->num_kv_heads <= 0) return MOSAIC_ERR_HEADS;
+    if (c->num_kv_heads <= 0 || c->num_kv_heads > 65535) return MOSAIC_ERR_HEADS;   // (a block of all heads is below 2^31 bytes)
     if (c->block_size != 64 && c->block_size != 128 && c->block_size != 256) return MOSAIC_ERR_BLOCK_SIZE;
     if (c->code_type != MOSAIC_CODE_INT8 && c->code_type != MOSAIC_CODE_E4M3) return MOSAIC_ERR_UNSUPPORTED;
     // positions of tokens, and tiles of 64 of all heads and members, are counted in 31 bits

@@ -53,8 +53,8 @@ class KVCache:
     def __init__(self, batch: int, capacity: int, kv_heads: int, block_size: int = 64, dtype: torch.dtype = torch.int8,
                  device="cuda"):
         batch, capacity, kv_heads, block_size = int(batch), int(capacity), int(kv_heads), int(block_size)
-        if batch < 1 or capacity < 1 or kv_heads < 1:
-            raise ValueError(f"KVCache: batch, capacity and kv_heads must be positive, got {batch}, {capacity}, {kv_heads}")
+        if batch < 1 or capacity < 1 or not 1 <= kv_heads <= 65535:
+            raise ValueError(f"KVCache: batch, capacity and kv_heads must be positive, kv_heads at most 65535, got {batch}, {capacity}, {kv_heads}")
         if block_size not in (64, 128, 256):
             raise ValueError(f"KVCache: block_size must be 64, 128 or 256, got {block_size}")
         if dtype not in _CODES:

@@ -73,7 +73,9 @@ def attention(q, k, v, scale, lens=None, idx=None, bs=64):
     shared by numerator and denominator (2^-8 of sum w |v - o|, and 2^-8 of that again); scores in fp32, each
     off by e (64 products, their sum and the factors: 72 roundings of 2^-24 of sum |q k| scale, and 2^-22 of
     |score| for its place in the exponent) which weigh 2 e sum w |v - o|; fp32 sums over the keys, 2^-24 each of
-    sum w |v|, and 8 more for products with the scales, exponentials and joins.
+    sum w |v|, and 8 more for products with the scales, exponentials and joins; and weights
+    that leave fp32 (and bf16): the reference of the scores, in powers of two, is 0 or up to 80 above the row's largest, and
+    scales of values may take 20 more, so that what lies 2^-106 below the reference may be zeros.
     """
     q, k, v = (t.to(F64) for t in (q, k, v))
     B, Nq, Hq, d = q.shape
@@ -104,7 +106,9 @@ def attention(q, k, v, scale, lens=None, idx=None, bs=64):
                 size = p @ vv.abs()
                 e = 72 * 2.0 ** -24 * scale * (q[b, :, g].abs() @ kk.abs().t()) + 2.0 ** -22 * x.abs()
                 e = torch.where(okk, e, 0.0).amax(-1, keepdim=True) if kk.numel() else torch.zeros(Nq, 1, dtype=F64)
+                most = (x.masked_fill(~okk, -math.inf).amax(-1, keepdim=True) / math.log(2.0) if kk.numel() else x.new_zeros(Nq, 1)).clamp(-80, 0)
+                lost = okk.sum(-1, keepdim=True) * 2.0 ** (-106 - most) * (vv.abs().amax() if vv.numel() else 0.0)
                 out[b, :, g] = o
                 tol[b, :, g] = (2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -16 + 2 * e) * off
-                                + (okk.sum(-1, keepdim=True) + 8) * 2.0 ** -24 * size)
+                                + (okk.sum(-1, keepdim=True) + 8) * 2.0 ** -24 * size + lost)
     return out, tol

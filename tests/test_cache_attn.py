@@ -228,6 +228,44 @@ def test_the_same_bits_each_time_and_on_another_stream():
 
 
 @gpu
+@pytest.mark.parametrize("code", [I8, E4M3], ids=["int8", "e4m3"])
+def test_a_token_s_bits_do_not_depend_on_the_tokens_beside_it(code):
+    """In calls that fill the chip: tokens in another order, and beside ones whose scores leave the bounds."""
+    n, H = 4200, 2
+    cache = filled(1, 64 * 70, H, 64, code, seed=21)
+    g = torch.Generator().manual_seed(22)
+    idx = torch.randint(0, 70, (1, n, H, 5), generator=g).cuda()
+    q = queries(1, n, 8, 23).cuda()
+    want = M.cache_attn(q, cache, idx)
+    order = torch.randperm(n, generator=g).cuda()
+    assert torch.equal(M.cache_attn(q[:, order], cache, idx[:, order]), want[:, order])
+    large = torch.rand(n, generator=g).cuda() < 0.1
+    got = M.cache_attn(torch.where(large[None, :, None, None], 64 * q, q), cache, idx)
+    assert torch.equal(got[:, ~large], want[:, ~large]) and not torch.equal(got[:, large], want[:, large])
+
+
+@gpu
+@pytest.mark.parametrize("nq", [1, 40, 900])
+def test_scores_past_the_bounds(nq):
+    """Rows whose references move, up and down, from the first block or a later one, and rows at the bound."""
+    n = 64 * 12
+    g = torch.Generator().manual_seed(24)
+    k, v = torch.randn(2, 1, n, 1, 64, generator=g)
+    size = torch.tensor([1.0, 1, 8, 1, 30, 1, 1, 60, 1, 2, 1, 100]).repeat_interleave(64)
+    k = k * size[None, :, None, None]
+    k[0, :, 0, 0] = torch.where(size > 20, -size, k[0, :, 0, 0])
+    cache = M.KVCache(1, n, 1)
+    M.kv_cache_write(cache, k.cuda(), v.cuda())
+    q = queries(1, nq, 4, 25)
+    q[0, ::3, :, 0] = 30.0
+    q[0, 1::3, :, 0] = -30.0
+    check(cache, q, scale=0.5)
+    check(cache, q, sets(1, nq, 1, 4, 12), scale=0.5)
+    only = torch.tensor([11, 7]).expand(1, nq, 1, 2)     # nothing but scores far below zero, for a third of the rows
+    check(cache, q, only, scale=1.0)
+
+
+@gpu
 def test_a_captured_step():
     """A token written and attended to, replayed over changing inputs; every replay against the eager call."""
     B, H, n = 2, 2, 300

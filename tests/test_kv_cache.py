@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mosaic_amd as M
-from kv_cache_model import Model, nearest_code
+from kv_cache_model import Model, attention, nearest_code
 from mosaic_amd import _lib
 
 gpu = pytest.mark.gpu
@@ -219,6 +219,36 @@ def test_windows_of_each_sequence(code):
 
 
 @gpu
+@CODES
+def test_offsets_past_32_bits(code):
+    """A cache of 5.4 GB of codes for each of k and v: its last tokens, written, read and attended to."""
+    n, H = 1 << 20, 80
+    cache = M.KVCache(1, n, H, block_size=128, dtype=code)
+    at = n - 150
+    k, v = tokens(1, 150, H, seed=19)
+    M.kv_cache_write(cache, k.cuda(), v.cuda(), at)
+    M.kv_cache_write(cache, k[:, :3].cuda(), v[:, :3].cuda(), torch.tensor([5], device="cuda"))
+    small = Model(1, 256, H, 128, code)               # the last two blocks
+    small.write(k, v, 256 - 150)
+    got = M.kv_cache_read(cache, at, 150, F32)
+    for i in range(2):
+        assert torch.equal(got[i].cpu(), small.values(i)[:, 106:])
+    assert torch.equal(M.kv_cache_read(cache, torch.tensor([at], device="cuda"), 200, F32)[0][:, :150], got[0])
+    q = torch.randn(1, 40, H, 64, generator=torch.Generator().manual_seed(20)).to(BF16)
+    idx = torch.tensor([n // 128 - 1, n // 128 - 2]).expand(1, 40, H, 2)
+    want, tol = attention(q, small.values(0), small.values(1), 0.125)
+    for rows in (slice(0, 1), slice(0, 40)):          # one row, and many
+        out = M.cache_attn(q[:, rows].cuda(), cache, idx[:, rows].cuda()).cpu().double()
+        assert ((out - want[:, rows]).abs() <= tol[:, rows]).all()
+    # the whole of it: keys of zeros all but the last, and the first few
+    one = M.cache_attn(q[:, :1].cuda() * 0, cache).cpu().double()[0, 0]
+    total = (small.values(1).double().sum(1)[0] + M.kv_cache_read(cache, 5, 3, F32)[1].cpu().double().sum(1)[0]) / n
+    # equal scores: weights of 1, or of a block's scale each, off by 2^-8 at most
+    size = (small.values(1).double().abs().sum(1)[0] + M.kv_cache_read(cache, 5, 3, F32)[1].cpu().double().abs().sum(1)[0]) / n
+    assert ((one - total).abs() <= (2.0 ** -7 + 2.0 ** -12) * size + 2.0 ** -8 * total.abs()).all()
+
+
+@gpu
 def test_empty_writes_leave_the_cache():
     cache, model = made(2, 100, 1, 64, I8)
     write(cache, model, *tokens(2, 100, 1, seed=17))
@@ -267,7 +297,7 @@ def cpu_cache(**kw):
 
 
 @pytest.mark.parametrize("kw,error", [
-    (dict(batch=0), ValueError), (dict(capacity=0), ValueError), (dict(kv_heads=0), ValueError), (dict(block_size=32), ValueError),
+    (dict(batch=0), ValueError), (dict(capacity=0), ValueError), (dict(kv_heads=0), ValueError), (dict(kv_heads=65536), ValueError), (dict(block_size=32), ValueError),
     (dict(block_size=512), ValueError), (dict(dtype=torch.uint8), TypeError), (dict(dtype=torch.float8_e5m2), TypeError),
     (dict(capacity=1 << 31), ValueError), (dict(batch=1 << 20, capacity=1 << 20), ValueError),
 ])
@@ -343,7 +373,7 @@ def c_cache(**kw):
 
 @pytest.mark.parametrize("kw,status", [
     (dict(k_codes=None), 1), (dict(v_codes=None), 1), (dict(k_scale=None), 1), (dict(v_scale=None), 1), (dict(k_norm=None), 1), (dict(k_mean=None), 1),
-    (dict(batch=0), 8), (dict(num_blocks=0), 8), (dict(num_kv_heads=0), 3), (dict(block_size=32), 4), (dict(block_size=192), 4),
+    (dict(batch=0), 8), (dict(num_blocks=0), 8), (dict(num_kv_heads=0), 3), (dict(num_kv_heads=65536), 3), (dict(block_size=32), 4), (dict(block_size=192), 4),
     (dict(code_type=2), 11), (dict(capacity=257), 8), (dict(capacity=0), 8), (dict(k_codes=FAKE + 8), 7), (dict(k_scale=FAKE + 2), 7),
     (dict(k_mean=FAKE + 4), 7), (dict(num_blocks=1 << 26, capacity=1), 8), (dict(batch=1 << 30), 8),
 ])
