@@ -460,25 +460,38 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_kernel(CacheAttnPara
     }
     const int tile_id = tile % p.qtiles, rest = tile / p.qtiles, h = rest % p.Hk, b = rest / p.Hk;
     const int n0 = tile_id * WAVES * p.QW;
-    Row row;
-    if constexpr (DENSE) row.init(p, [&](int i) { return min(n0 + i, p.Nq - 1); }, b, h, n0, wave, lane & 31);
-    else {
-        load_tokens(p, L, b, h, n0);
-        row.init(p, [&](int i) { return L.tokens[i]; }, b, h, n0, wave, lane & 31);
-    }
-    const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
-    const int64_t part = (int64_t)(tile - p.whole) * (WAVES * kRows) + wave * kRows + (lane & 31);
-    if (splits > 1 && split == 0 && hh == 0) p.part_at[part] = row.live ? row.at : -1;
+    if constexpr (!DENSE) load_tokens(p, L, b, h, n0);
+    // (formed anew where it is needed again: the loops between have no register for it)
+    auto my_row = [&] {
+        int first = n0;
+        asm volatile("" : "+s"(first));
+        Row row;
+        if constexpr (DENSE) row.init(p, [&](int i) { return min(first + i, p.Nq - 1); }, b, h, first, wave, lane & 31);
+        else row.init(p, [&](int i) { return L.tokens[i]; }, b, h, first, wave, lane & 31);
+        return row;
+    };
+    auto put = [&](AttnState& a, float w, bool ok) {
+        const Row row = my_row();
+        const int64_t part = (int64_t)(tile - p.whole) * (WAVES * kRows) + wave * kRows + (lane & 31);
+        if (splits > 1 && split == 0 && hh == 0) p.part_at[part] = row.live ? row.at : -1;
+        if (row.live && ok) put_row(p, row, part, split, splits, w, a);
+    };
     const float w = value_unit(p.cache, b, h);
     AttnState a;
-    attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, w, a);
-    const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
-    const int other = __shfl_xor((int)fine, 32);   // (the other half of the row)
-    const bool ok = !row.live || (fine && other);
-    if (row.live && ok) put_row(p, row, part, split, splits, w, a);
+    bool ok;
+    {
+        const Row row = my_row();
+        const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
+        attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, w, a);
+        const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
+        const int other = __shfl_xor((int)fine, 32);   // (the other half of the row)
+        ok = !row.live || (fine && other);
+    }
+    put(a, w, ok);
     if (!__syncthreads_or(!ok)) return;
-    attend<FP8, DENSE, true, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, 1.f, a);
-    if (row.live && !ok) put_row(p, row, part, split, splits, 1.f, a);
+    const Row row = my_row();
+    attend<FP8, DENSE, true, WAVES>(p, L, b, h, n0, split, splits, row, __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0, 1.f, a);
+    put(a, 1.f, !ok);
 }
 
 // ------------------------------------------------------------------ few rows
