@@ -7,12 +7,21 @@
 // Codes are whole numbers of at most 8 bits or e4m3, exact in bf16, so the products are of bf16 operands
 // without a rounding of theirs.  ks goes into the factor of the scores and vs into the exponent,
 //   P = exp2(c ks q.code_k - m + log2(vs / w)),  O = sum P code_v,  l = sum P w / vs,  o = w O / l,
-// so that neither costs an instruction per score (w: the scale of the sequence's first block).  fp32 scores, maxima, sums and accumulators; P is rounded to
-// bf16 for the product with the values (half a step of bf16 per term, as the output's own rounding), and l sums
-// the rounded P.
+// so that neither costs an instruction per score (w: the scale of the sequence's first block).  fp32 scores,
+// maxima, sums and accumulators.  P is rounded to bf16 for the product with the values and l sums the rounded P:
+// an error as the output's own rounding (together 2.2e-3 of the result, the output's alone 1.7e-3); a second term of
+// P would be half as many products again where they are the bound.  Of few rows it is taken: see there.
 //
-// A workgroup takes 4 waves x QW = 32 / G tokens of one kv head, a wave the 32 rows (token, head) of
-// its tokens; the codes of 64 keys are converted once, by all four waves, into operand order in LDS.
+// Two kernels.  Many rows: a workgroup takes 4 or 12 waves x QW = 32 / G tokens of one kv head, a wave the 32 rows
+// (token, head) of its tokens; the codes of 64 keys are converted once, by all of its waves, into operand order in
+// LDS, which each of them reads.  The matrix pipe bounds it: 12 heads of 12288 tokens over 49152 keys, 1.86 TFLOP,
+// in 1.65 ms or 1130 TF/s, where a bf16 library product of 8192^3 reaches 1230.  With blocks for each token (49152
+// tokens, 8 blocks of 64, 12 heads: 0.21 ms, 730 TF/s) a workgroup walks the union of its tokens' blocks: a quarter
+// of its 67000 cycles goes before the first tile, into the union and its scales, and the tiles of tokens that do not
+// share them are computed for all rows.
+// Few rows (up to 16 of a kv head, one token above all): memory bounds a long cache (one token over 196608 keys of 3
+// heads in e4m3, 75 MB: 15.5 us, 4.9 TB/s), the vector ALU's conversions and the launch a short one.
+// In both, the keys of a call with few workgroups are split into shares, and a third kernel joins their parts.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -500,7 +509,10 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_kernel(CacheAttnPara
 // of 64 keys of its share in turn, straight from memory into the operands of v_mfma_f32_16x16x32_bf16
 // (lane group g = lane / 16): in step m the keys' rows 4 g + i are tokens 16 g + 4 m + i, so that a lane
 // ends with the scores of the 16 tokens that its chunk of the values holds.  A tile is requested while
-// the one before is computed.
+// the one before is computed (two ahead need 196 registers: 32 us for 21 over 196608 keys).
+// Eight waves where one workgroup takes a head's keys: a wave alone issues a vector instruction in four cycles, about
+// 1 us a tile, and two of a SIMD hide each other's waits (one token, 16 blocks of 128: 14.4 us of a call, of 4 waves
+// 16.1, of 16 waves 15.5).
 constexpr int kFewRows = 16, kFewEntries = 64;
 
 struct FewState {
@@ -563,15 +575,21 @@ __device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2]
     a.has = a.has || some;
     const float ref = member ? (SAFE ? f.iv : f.lv) - a.m : -INFINITY;   // P = 0 for the others
     auto weight = [&](float x) { return __builtin_amdgcn_exp2f(SAFE ? times_plus(x, f.ck, ref) : fmaf(x, f.ck, ref)); };
-    bf16x8 pb[2];
+    // P in two terms, 16 bits of it: the products wait for the codes, and a single row does not average the rounding
+    bf16x8 pb[2], rest[2];
     float lt = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        uint32_t u[4];
+        uint32_t u[4], y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = pack_bf16x2(weight(s[2 * j + (i >> 1)][2 * (i & 1)]), weight(s[2 * j + (i >> 1)][2 * (i & 1) + 1]));
+        for (int i = 0; i < 4; ++i) {
+            const float x0 = weight(s[2 * j + (i >> 1)][2 * (i & 1)]), x1 = weight(s[2 * j + (i >> 1)][2 * (i & 1) + 1]);
+            lt += x0 + x1;
+            u[i] = pack_bf16x2(x0, x1);
+            y[i] = pack_bf16x2(x0 - bf_lo(u[i]), x1 - bf_hi(u[i]));
+        }
         pb[j] = as_bf16x8(make_uint4(u[0], u[1], u[2], u[3]));
-        lt = operand_sum(pb[j], lt);
+        rest[j] = as_bf16x8(make_uint4(y[0], y[1], y[2], y[3]));
     }
     if constexpr (SAFE) {
         if (member) a.l += lt;
@@ -579,18 +597,19 @@ __device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2]
 #pragma unroll
     for (int dg = 0; dg < 4; ++dg) {
         const bf16x8 v0 = codes8<FP8>(t.v[dg].x, t.v[dg].y), v1 = codes8<FP8>(t.v[dg].z, t.v[dg].w);
+        auto product = [&](f32x4 y) { return mfma16(v1, pb[1], mfma16(v0, pb[0], mfma16(v1, rest[1], mfma16(v0, rest[0], y)))); };
         if constexpr (SAFE) {
-            const f32x4 y = mfma16(v1, pb[1], mfma16(v0, pb[0], f32x4{0.f, 0.f, 0.f, 0.f}));
+            const f32x4 y = product(f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int i = 0; i < 4; ++i) a.o[dg][i] = member ? fmaf(y[i], f.lv, a.o[dg][i]) : a.o[dg][i];
-        } else a.o[dg] = mfma16(v1, pb[1], mfma16(v0, pb[0], a.o[dg]));
+        } else a.o[dg] = product(a.o[dg]);
     }
 }
 
-template <bool FP8, bool DENSE>
-__global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnParams p) {
-    __shared__ __attribute__((aligned(16))) float O[kWaves][kFewRows][64];
-    __shared__ float2 ml[kWaves][kFewRows];
+template <bool FP8, bool DENSE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few_kernel(CacheAttnParams p) {
+    __shared__ __attribute__((aligned(16))) float O[WAVES][kFewRows][64];
+    __shared__ float2 ml[WAVES][kFewRows];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits, h = rest % p.Hk, b = rest / p.Hk;
@@ -664,12 +683,12 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
         uint32_t of_next;
         int key_next = where(first + wave, of_next);
         load(min(key_next, end - 1), next);   // (a block's later tiles may lie behind the end)
-        for (int u = first + wave; u < past; u += kWaves) {
+        for (int u = first + wave; u < past; u += WAVES) {
             const Codes t = next;
             const uint32_t of = of_next;
             const int key0 = key_next;
-            if (u + kWaves < past) {
-                key_next = where(u + kWaves, of_next);
+            if (u + WAVES < past) {
+                key_next = where(u + WAVES, of_next);
                 load(min(key_next, end - 1), next);
             }
             if (key0 < end)
@@ -702,11 +721,11 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_few_kernel(CacheAttnPa
     if (row >= rows) return;
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) m = ml[i][row].y == 0.f ? m : fmaxf(m, ml[i][row].x);
+    for (int i = 0; i < WAVES; ++i) m = ml[i][row].y == 0.f ? m : fmaxf(m, ml[i][row].x);
     float sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < WAVES; ++i) {
         const float2 part = ml[i][row];
         const float4 x = *reinterpret_cast<const float4*>(&O[i][row][d ^ (4 * row)]);
         const float y = part.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(part.x - m) * part.y;   // 0: no key
@@ -812,13 +831,23 @@ int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, 
 // CU: its join is the longer (one point over 196608 keys, 75 MB in e4m3: 20.5 us in 85 shares of each head, 23.3 in
 // 170 and in 341; 24 tracks of 16 heads, 113 MB in int8: 25 us in 10 shares, 29 in 2).
 constexpr int64_t kFewGroups = 1024, kFewShares = 64, kFewTiles = 8;
+constexpr int kManyWaves = 8;   // of a workgroup that takes all keys of a head of few rows
 static_assert(kJoinMost >= kFewGroups, "the join takes every share");
-constexpr int64_t kWideRows = 1536;   // of a kv head, from which dense workgroups have twelve waves
+// Dense workgroups of twelve waves, one a CU, convert a tile once for 384 rows instead of three times, but leave CUs
+// idle where rows are few: from kWideRows rows of a kv head on (12288 tokens over 49152 keys: 1735 us of 4 waves,
+// 1640 of 12; 1024 rows: 4 waves are the faster).
+constexpr int64_t kWideRows = 1536;
 
 // Whether the call is one of cache_attn_few_kernel
 bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     const int64_t rows = (int64_t)nq * (hq / c.num_kv_heads);
     return rows <= kFewRows && (int64_t)nq * K <= kFewEntries;
+}
+
+template <int WAVES>
+const void* few_kernel(bool fp8, bool sets) {
+    return fp8 ? (sets ? (const void*)&cache_attn_few_kernel<true, false, WAVES> : (const void*)&cache_attn_few_kernel<true, true, WAVES>)
+               : (sets ? (const void*)&cache_attn_few_kernel<false, false, WAVES> : (const void*)&cache_attn_few_kernel<false, true, WAVES>);
 }
 
 // How a call is laid out: waves of a workgroup, tiles of rows, those taken whole, and shares of the others' keys.
@@ -838,6 +867,7 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
         a.splits = kFewGroups / heads;
         if (a.splits > kFewShares) a.splits = std::max(kFewShares, 256 / heads);
         a.splits = std::max<int64_t>(1, std::min(a.splits, tiles / (kWaves * kFewTiles)));
+        if (a.splits == 1 && tiles > kWaves) a.waves = kManyWaves;
         a.parts = (int64_t)c.batch * nq * hq;
     } else {
         const int64_t most = K > 0 ? std::min(K, kMaxSplit) : std::max<int64_t>(1, c.num_blocks / 4);
@@ -911,8 +941,8 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     void* args[] = {&p};
     const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, sets = block_count > 0;
     const void* fn;
-    if (small) fn = fp8 ? (sets ? (const void*)&cache_attn_few_kernel<true, false> : (const void*)&cache_attn_few_kernel<true, true>)
-                        : (sets ? (const void*)&cache_attn_few_kernel<false, false> : (const void*)&cache_attn_few_kernel<false, true>);
+    if (small && plan.waves == kManyWaves) fn = few_kernel<kManyWaves>(fp8, sets);
+    else if (small) fn = few_kernel<kWaves>(fp8, sets);
     else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false, 4> : (const void*)&cache_attn_kernel<false, false, 4>;
     else if (plan.waves == 12) fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 12> : (const void*)&cache_attn_kernel<false, true, 12>;
     else fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 4> : (const void*)&cache_attn_kernel<false, true, 4>;
