@@ -829,14 +829,18 @@ int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, 
 
 // Shares of the keys of few rows: four workgroups a CU, where a row has no more than kFewShares then, and else one a
 // CU: its join is the longer (one point over 196608 keys, 75 MB in e4m3: 20.5 us in 85 shares of each head, 23.3 in
-// 170 and in 341; 24 tracks of 16 heads, 113 MB in int8: 25 us in 10 shares, 29 in 2).
-constexpr int64_t kFewGroups = 1024, kFewShares = 64, kFewTiles = 8;
+// 170 and in 341; 24 tracks of 16 heads, 113 MB in int8: 25 us in 10 shares, 29 in 2).  One share and no join up to
+// kFewWhole tiles (2048 keys: 13 us, 17 in four shares), and no fewer than kFewTiles in a share, two a wave (4096 keys:
+// 16 us in eight shares, 17 in two, 21 in one).
+constexpr int64_t kFewGroups = 1024, kFewShares = 64, kFewWhole = 40, kFewTiles = 8;
 constexpr int kManyWaves = 8;   // of a workgroup that takes all keys of a head of few rows
 static_assert(kJoinMost >= kFewGroups, "the join takes every share");
-// Dense workgroups of twelve waves, one a CU, convert a tile once for 384 rows instead of three times, but leave CUs
-// idle where rows are few: from kWideRows rows of a kv head on (12288 tokens over 49152 keys: 1735 us of 4 waves,
-// 1640 of 12; 1024 rows: 4 waves are the faster).
-constexpr int64_t kWideRows = 1536;
+// A dense call's layout is the one of the least time by these, in microseconds: a tile of 64 keys of a chip full of
+// rows, in workgroups of 4 waves, three a CU, or of 12, one a CU, which convert a tile once for 384 rows; a join, and a
+// row's part of it.  (12 heads on 3 over 49152 keys, 4 | 12 waves | the choice: 128 tokens 44 | 46 | 44 us, 1000 tokens
+// 192 | 183 | 182, 12288 tokens 1875 | 1660 | 1660; 6000 tokens, whose last round is
+// nearly empty, 1021 without shares of it, 850 with; 12288 tokens over 12288 keys of 4 members 1845 | 1677 | 1677.)
+constexpr double kTile = 1.7, kWideTile = 1.45, kJoinTime = 4., kPartTime = 6e-5;
 
 // Whether the call is one of cache_attn_few_kernel
 bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
@@ -866,21 +870,38 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
         a.tiles = heads;
         a.splits = kFewGroups / heads;
         if (a.splits > kFewShares) a.splits = std::max(kFewShares, 256 / heads);
-        a.splits = std::max<int64_t>(1, std::min(a.splits, tiles / (kWaves * kFewTiles)));
+        a.splits = tiles <= kFewWhole ? 1 : std::max<int64_t>(1, std::min(a.splits, tiles / kFewTiles));
         if (a.splits == 1 && tiles > kWaves) a.waves = kManyWaves;
         a.parts = (int64_t)c.batch * nq * hq;
-    } else {
-        const int64_t most = K > 0 ? std::min(K, kMaxSplit) : std::max<int64_t>(1, c.num_blocks / 4);
-        if (K == 0 && (int64_t)nq * G >= kWideRows) a.waves = 12;
-        const int64_t per = a.waves * (kRows / G), slots = a.waves == 12 ? 256 : K > 0 ? 512 : 768;
-        a.qtiles = (nq + per - 1) / per;
+    } else if (K > 0) {   // shares where there are few tiles (16 blocks of 64: 1000 tokens 39 us, 73 in one share; 3500 tokens 57 in either)
+        a.qtiles = (nq + kWaves * (kRows / G) - 1) / (kWaves * (kRows / G));
         a.tiles = a.qtiles * heads;
-        // full rounds of the chip, and the rest's keys in shares that fill it once more (sets: where there is no full round)
-        a.whole = K > 0 ? (a.tiles >= 256 ? a.tiles : 0) : a.tiles / slots * slots;
-        const int64_t rest = a.tiles - a.whole;
-        a.splits = rest > 0 ? std::max<int64_t>(1, std::min(slots / rest, most)) : 1;
+        a.splits = a.tiles >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / a.tiles, std::min(K, kMaxSplit)));
+        a.whole = a.splits == 1 ? a.tiles : 0;
+        a.parts = (a.tiles - a.whole) * kWaves * kRows;
+    } else {   // full rounds of the chip, and the rest's keys in shares
+        double best = INFINITY;
+        for (int waves : {4, 12}) {
+            const int64_t per = waves * (kRows / G), qtiles = (nq + per - 1) / per, tiles = qtiles * heads, slots = waves == 4 ? 768 : 256;
+            const int64_t whole = tiles / slots * slots, rest = tiles - whole;
+            const double round = c.num_blocks * sub * (waves == 4 ? kTile : kWideTile);
+            auto take = [&](int64_t unsplit, int64_t splits) {
+                const int64_t groups = (tiles - unsplit) * splits, left = groups % slots, parts = splits > 1 ? rest * waves * kRows : 0;
+                // (a last round of one or two workgroups a CU takes less time than one of three)
+                const double rounds = groups / slots + (left == 0 ? 0. : waves == 12 || left > 512 ? 1. : left > 256 ? .75 : .5);
+                const double time = (unsplit / slots + rounds / splits) * round + (splits > 1 ? kJoinTime + splits * parts * kPartTime : 0.);
+                if (time >= best) return;
+                best = time;
+                a.waves = waves; a.qtiles = qtiles; a.tiles = tiles; a.whole = unsplit; a.splits = splits; a.parts = parts;
+            };
+            take(0, 1);
+            if (rest > 0)
+                for (int64_t fill : {256, 512, 768, 1024, 1536, 2304}) {
+                    const int64_t splits = std::min<int64_t>({fill / rest, std::max<int64_t>(1, c.num_blocks / 4), kJoinMost});
+                    if (splits > 1) take(whole, splits);
+                }
+        }
         if (a.splits == 1) a.whole = a.tiles;
-        a.parts = (a.tiles - a.whole) * a.waves * kRows;
     }
     if (a.splits > 1) {
         a.part_ml = up(a.splits * a.parts * kHeadDim * sizeof(float));
