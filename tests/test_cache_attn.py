@@ -73,6 +73,36 @@ def test_blocks_of_each_token(code, K, B, Nq, Nk, Hq, Hk, bs):
 
 
 @gpu
+@pytest.mark.parametrize("grow", [1.0, 20.0], ids=["bounded", "past the bounds"])
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hk,bs,code", [
+    (1, 6500, 500, 16, 1, 64, I8), (3, 2100, 700, 16, 1, 128, E4M3), (1, 1000, 3100, 4, 4, 64, E4M3), (2, 400, 2000, 6, 2, 256, I8),
+    (1, 1, 40000, 4, 1, 64, I8), (1, 16, 2600, 1, 1, 64, E4M3), (1, 17, 40000, 1, 1, 64, I8),
+])
+def test_layouts_of_whole_sequences(B, Nq, Nk, Hq, Hk, bs, code, grow):
+    """Full rounds of workgroups with the rest in shares, shares alone, many of them; lengths that leave shares empty."""
+    cache = filled(B, Nk, Hk, bs, code, seed=Nk + 1, grow=grow)
+    q = queries(B, Nq, Hq, 26)
+    check(cache, q)
+    check(cache, q, lens=torch.tensor([Nk - 70, 0, 65][:B]))
+    check(cache, q, lens=torch.tensor([1, Nk, 130][:B]))
+
+
+@gpu
+@pytest.mark.parametrize("code", [I8, E4M3], ids=["int8", "e4m3"])
+def test_a_full_round_and_a_rest_in_shares(code):
+    """Many tokens over a long sequence; every 61st of them, and the last, against float64."""
+    n = 6500
+    cache = filled(1, 2000, 1, 64, code, seed=27)
+    q = queries(1, n, 16, 28)
+    k, v = (t.cpu() for t in M.kv_cache_read(cache, dtype=F32))
+    rows = torch.cat([torch.arange(0, n, 61), torch.arange(n - 40, n)])
+    for lens in (None, torch.tensor([1801])):
+        got = M.cache_attn(q.cuda(), cache, kv_lens=None if lens is None else lens.cuda())[:, rows.cuda()]
+        want, tol = attention(q[:, rows], k, v, 0.125, lens, None, 64)
+        assert bool(((got.cpu().double() - want).abs() <= tol).all())
+
+
+@gpu
 @pytest.mark.parametrize("lens", [0, 1, 63, 64, 65, 127, 128, 129, 255, 256])
 @pytest.mark.parametrize("bs", [64, 128, 256])
 def test_lengths_at_the_edges(bs, lens):
