@@ -943,6 +943,8 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     p.G = p.Hq / p.Hk; p.QW = kRows / p.G; p.bs = cache->block_size; p.K = block_count; p.nb = cache->num_blocks;
     p.qw_inverse = (65536 + p.QW - 1) / p.QW;
     const Plan plan = plan_of(*cache, num_queries, num_q_heads, block_count);
+    const int64_t groups = plan.whole + (plan.tiles - plan.whole) * plan.splits;
+    if (!grid_fits(groups, 64 * plan.waves)) return MOSAIC_ERR_SHAPE;
     p.qtiles = (int)plan.qtiles; p.splits = (int)plan.splits; p.whole = (int)plan.whole; p.parts = plan.parts;
     p.out = static_cast<bf16_t*>(out);
     p.c = (softmax_scale > 0.f ? softmax_scale : 0.125f) * kLog2e;
@@ -958,7 +960,6 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
         place_order(p, ws + plan.bytes);
         if (int e = launch_order(p, s)) return e;
     }
-    int total = (int)(plan.whole + (plan.tiles - plan.whole) * plan.splits);
     void* args[] = {&p};
     const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, sets = block_count > 0;
     const void* fn;
@@ -967,15 +968,15 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false, 4> : (const void*)&cache_attn_kernel<false, false, 4>;
     else if (plan.waves == 12) fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 12> : (const void*)&cache_attn_kernel<false, true, 12>;
     else fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 4> : (const void*)&cache_attn_kernel<false, true, 4>;
-    if (launch(fn, dim3(total), args, s, 64 * plan.waves) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    if (launch(fn, dim3((unsigned)groups), args, s, 64 * plan.waves) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
     void* jargs[] = {&p};
     const int team = p.splits <= 16 ? 1 : p.splits <= 64 ? 16 : 64;
     const void* join = team == 1    ? (const void*)&cache_attn_join_kernel<1>
                        : team == 16 ? (const void*)&cache_attn_join_kernel<16>
                                     : (const void*)&cache_attn_join_kernel<64>;
-    const unsigned groups = (unsigned)(team == 1 ? (p.parts + 15) / 16 : p.parts);
-    return launch(join, dim3(groups), jargs, s, team == 64 ? 1024 : kThreads) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
+    const unsigned joins = (unsigned)(team == 1 ? (p.parts + 15) / 16 : p.parts);
+    return launch(join, dim3(joins), jargs, s, team == 64 ? 1024 : kThreads) == hipSuccess ? MOSAIC_OK : MOSAIC_ERR_LAUNCH;
 }
 
 }  // extern "C"

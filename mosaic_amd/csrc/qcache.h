@@ -55,6 +55,9 @@ __device__ __forceinline__ float4 codes_f32(uint32_t w) {
     }
 }
 
+// Whether a launch's threads can be counted: in 32 bits.
+inline bool grid_fits(int64_t groups, int threads) { return groups < (1LL << 32) / threads; }
+
 // Whether a cache's description can be addressed.
 inline int check_cache(const mosaic_kv_cache* c) {
     if (c == nullptr) return MOSAIC_ERR_NULL_POINTER;

@@ -486,6 +486,7 @@ int mosaic_kv_cache_write(const mosaic_kv_cache* cache, mosaic_bnhd k, mosaic_bn
     p.starts = starts; p.counts = counts; p.start = start; p.n = num_tokens;
     int64_t units = units_of(num_tokens, cache->block_size, start, starts != nullptr);
     if (units > cache->num_blocks) units = cache->num_blocks;
+    if (!grid_fits(units * cache->num_kv_heads * cache->batch, kThreads)) return MOSAIC_ERR_SHAPE;
     p.units = (int)units;
     const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, half = dtype == MOSAIC_DTYPE_BF16;
     const void* fn = half ? (fp8 ? write_kernel<bf16_t, true>(cache->block_size) : write_kernel<bf16_t, false>(cache->block_size))
@@ -505,8 +506,8 @@ int mosaic_kv_cache_read(const mosaic_kv_cache* cache, int32_t dtype, int32_t he
     p.k_out = k_out; p.v_out = v_out;
     p.starts = starts; p.start = start; p.n = num_tokens;
     const int64_t units = units_of(num_tokens, 64, start, starts != nullptr);
+    if ((double)units * cache->num_kv_heads * cache->batch > 2147483647.0 || !grid_fits(units * cache->num_kv_heads * cache->batch, kThreads)) return MOSAIC_ERR_SHAPE;
     p.units = (int)units;
-    if ((double)units * cache->num_kv_heads * cache->batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
     const bool fp8 = cache->code_type == MOSAIC_CODE_E4M3, half = dtype == MOSAIC_DTYPE_BF16;
     const void* fn = half ? (fp8 ? (const void*)&kv_cache_read_kernel<bf16_t, true> : (const void*)&kv_cache_read_kernel<bf16_t, false>)
                           : (fp8 ? (const void*)&kv_cache_read_kernel<float, true> : (const void*)&kv_cache_read_kernel<float, false>);

@@ -396,3 +396,5 @@ def test_c_entry_refuses_arguments():
     need = L.mosaic_cache_attn_fwd_workspace_size(big, 5, 6, 0)
     assert need > 0 and call(ws=None, cache=big) == 6 and call(nbytes=need - 1, cache=big) == 6 and call(ws=FAKE + 16, cache=big) == 6
     assert L.mosaic_cache_attn_fwd_workspace_size(c, 5, 51, 0) == 0
+    many = ctypes.byref(_lib.Cache(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 20, 1, 16, 64, _lib.CODE_INT8, 64))   # 2^24 workgroups of 256 threads
+    assert call(n=1, hq=16, cache=many) == 8 and call(n=40, hq=16, cache=many) == 8

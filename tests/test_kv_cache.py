@@ -393,5 +393,7 @@ def test_c_entries_refuse_arguments():
     assert put(d=128) == 2 and put(dt=5) == 11 and put(n=0) == 8 and put(start=246) == 8 and put(start=-1) == 8
     assert put(k=_lib.Bnhd(FAKE + 8, 960, 192, 64)) == 7 and put(k=_lib.Bnhd(FAKE, 960, 190, 64)) == 7
     assert put(starts=FAKE + 2) == 7 and put(counts=FAKE + 1) == 7
+    huge = ctypes.byref(c_cache(batch=1, num_blocks=1 << 24, num_kv_heads=1, capacity=1 << 30))   # 2^24 workgroups of 256 threads
+    assert put(n=1 << 30, cache=huge) == 8 and L.mosaic_kv_cache_read(huge, 1, 64, 1 << 30, 0, None, FAKE, FAKE, None) == 8
     get = lambda n=5, start=0, k=FAKE, v=FAKE: L.mosaic_kv_cache_read(c, 1, 64, n, start, None, k, v, None)
     assert get(k=None) == 1 and get(v=FAKE + 8) == 7 and get(n=251) == 8 and get(start=1 << 40) == 8
