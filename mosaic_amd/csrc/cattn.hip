@@ -124,14 +124,20 @@ __device__ __forceinline__ Factors factors(float c, float ks, float vs, float w,
         f.lv = vs;
         f.iv = poison;
     } else {
-        const float ratio = vs / w;
+        const float ratio = vs * __builtin_amdgcn_rcpf(w);   // (reciprocals to a unit of the last place)
         const bool near = ratio <= kSpread && ratio >= 1.f / kSpread;
         wide = !near && vs != 0.f;   // (a NaN too: SAFE leaves it a NaN)
         const float of = near ? ratio : 1.f;
         f.lv = __builtin_amdgcn_logf(of) + poison;
-        f.iv = 1.f / of;
+        f.iv = __builtin_amdgcn_rcpf(of);
     }
     return f;
+}
+
+// The first of a share's units, where the first shares take one more
+__device__ __forceinline__ int share_begin(int units, int share, int shares) {
+    const int each = (int)((uint32_t)units / (uint32_t)shares);
+    return each * share + min(share, units - each * shares);
 }
 
 struct TileRead {
@@ -410,7 +416,7 @@ __device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, 
     const int live = (int)(((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
     if constexpr (DENSE) {
         load_q();
-        const int first = (int)((int64_t)live * split / splits), past = (int)((int64_t)live * (split + 1) / splits);
+        const int first = share_begin(live, split, splits), past = share_begin(live, split + 1, splits);
         for (int e0 = first; e0 < past; e0 += 64) walk.blocks(min(64, past - e0), min(e0 + lane, past - 1), wave_live);
     } else {
         load_q();
@@ -613,7 +619,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits, h = rest % p.Hk, b = rest / p.Hk;
-    const int end = seq_keys(p, b), sub = p.bs / 64, rows = p.Nq * p.G;
+    const int end = seq_keys(p, b), shift = p.bs == 64 ? 6 : p.bs == 128 ? 7 : 8, sub = 1 << (shift - 6), rows = p.Nq * p.G;   // bs = 2^shift
     const bool row_live = r < rows;
     const int token = row_live ? r / p.G : 0, head = h * p.G + (row_live ? r - token * p.G : 0);
     const bf16_t* qr = p.q + b * p.q_sb + token * p.q_sn + head * p.q_sh + 16 * g;
@@ -644,7 +650,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
         rank = (int)__builtin_popcountll(leads & ((1ull << lane) - 1ull));
         units = (int)__builtin_popcountll(leads) * sub;
     }
-    const int first = (int)((int64_t)units * split / p.splits), past = (int)((int64_t)units * (split + 1) / p.splits);
+    const int first = share_begin(units, split, p.splits), past = share_begin(units, split + 1, p.splits);
     const int kt = r >> 3, ko = kt * 2048 + (g >> 1) * 1024 + (g & 1) * 512 + (r & 7) * 16;
     const int vo = (g >> 1) * 2048 + (g & 1) * 512 + r * 16;
     // unit u: its first key, and the tokens that have it
@@ -652,15 +658,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
         of = ~0u;
         if constexpr (DENSE) return u * 64;
         else {
-            const int which = (int)((uint32_t)u / (uint32_t)sub);
+            const int which = u >> (shift - 6);
             const int src = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(lead && rank == which));
             of = (uint32_t)__builtin_amdgcn_readlane((int)tokens, src);
             return __builtin_amdgcn_readlane(blk, src) * p.bs + (u - which * sub) * 64;
         }
     };
     auto load = [&](int key0, Codes& t) {
-        const int j = (int)((uint32_t)key0 / (uint32_t)p.bs);
-        const int64_t at = block_at(p.cache, b, j, h), from = at * (p.bs * 64) + (key0 - j * p.bs) * 64;
+        const int j = key0 >> shift;
+        const int64_t at = block_at(p.cache, b, j, h), from = (at << (shift + 6)) + (key0 - (j << shift)) * 64;
         const uint8_t* kc = static_cast<const uint8_t*>(p.cache.k_codes) + from;
         const uint8_t* vc = static_cast<const uint8_t*>(p.cache.v_codes) + from;
 #pragma unroll
@@ -719,18 +725,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
     // 16 threads a row
     const int row = tid / 16, d = 4 * (tid % 16);
     if (row >= rows) return;
+    float2 part[WAVES];
+    float4 x[WAVES];
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+        part[i] = ml[i][row];
+        x[i] = *reinterpret_cast<const float4*>(&O[i][row][d ^ (4 * row)]);
+    }
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) m = ml[i][row].y == 0.f ? m : fmaxf(m, ml[i][row].x);
+    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, part[i].y == 0.f ? -INFINITY : part[i].x);   // l = 0: no key
     float sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-        const float2 part = ml[i][row];
-        const float4 x = *reinterpret_cast<const float4*>(&O[i][row][d ^ (4 * row)]);
-        const float y = part.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(part.x - m) * part.y;   // 0: no key
+        const float e = __builtin_amdgcn_exp2f(part[i].x - m) * part[i].y, y = part[i].y == 0.f ? 0.f : e;
         sum += y;
-        o.x = fmaf(y, x.x, o.x); o.y = fmaf(y, x.y, o.y); o.z = fmaf(y, x.z, o.z); o.w = fmaf(y, x.w, o.w);
+        o.x = fmaf(y, x[i].x, o.x); o.y = fmaf(y, x[i].y, o.y); o.z = fmaf(y, x[i].z, o.z); o.w = fmaf(y, x[i].w, o.w);
     }
     const float y = sum == 0.f ? 0.f : 1.f / sum;
     const int t = row / p.G;
@@ -742,8 +753,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
     *reinterpret_cast<float4*>(p.part_o + (split * p.parts + at) * 64 + d) = make_float4(o.x * y, o.y * y, o.z * y, o.w * y);
     if (d == 0) {
         int e = 0;
-        const float part = frexpf(sum, &e);
-        p.part_ml[split * p.parts + at] = make_float2(m + (float)e, part);
+        const float f = frexpf(sum, &e);
+        p.part_ml[split * p.parts + at] = make_float2(m + (float)e, f);
     }
 }
 
