@@ -517,8 +517,8 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_kernel(CacheAttnPara
 // ends with the scores of the 16 tokens that its chunk of the values holds.  A tile is requested while
 // the one before is computed (two ahead need 196 registers: 32 us for 21 over 196608 keys).
 // Eight waves where one workgroup takes a head's keys: a wave alone issues a vector instruction in four cycles, about
-// 1 us a tile, and two of a SIMD hide each other's waits (one token, 16 blocks of 128, a call of the first such
-// form: 14.4 us, of 4 waves 16.1, of 16 waves 15.5; 13.7 now).
+// 1 us a tile, and two of a SIMD hide each other's waits (one token, 16 blocks of 128, a call: 14.4 us,
+// of 4 waves 16.1, of 16 waves 15.5; 13.7 since the shares and the join became shorter).
 constexpr int kFewRows = 16, kFewEntries = 64;
 
 struct FewState {
