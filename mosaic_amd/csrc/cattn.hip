@@ -884,10 +884,14 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
         a.splits = tiles <= kFewWhole ? 1 : std::max<int64_t>(1, std::min(a.splits, tiles / kFewTiles));
         if (a.splits == 1 && tiles > kWaves) a.waves = kManyWaves;
         a.parts = (int64_t)c.batch * nq * hq;
-    } else if (K > 0) {   // shares where there are few tiles (16 blocks of 64: 1000 tokens 39 us, 73 in one share; 3500 tokens 57 in either)
-        a.qtiles = (nq + kWaves * (kRows / G) - 1) / (kWaves * (kRows / G));
+    } else if (K > 0) {
+        // Shares where there are few tiles: of a union that may be as many blocks as the tile's tokens have entries, three
+        // workgroups a CU, two where the join is one of teams (16 blocks of 64 a token: 17 scattered tokens 17 us,
+        // 26 in 16 shares; 40 32, 41 in 16; 200 33, 35 in 36; 1000 39, 73 in one; 3500 57 in one or two)
+        const int64_t per = kWaves * (kRows / G), tokens = std::min<int64_t>(nq, per);
+        a.qtiles = (nq + per - 1) / per;
         a.tiles = a.qtiles * heads;
-        a.splits = a.tiles >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / a.tiles, std::min(K, kMaxSplit)));
+        a.splits = a.tiles >= 256 ? 1 : std::min<int64_t>({768 / a.tiles, std::max<int64_t>(16, 512 / a.tiles), tokens * K, 64});
         a.whole = a.splits == 1 ? a.tiles : 0;
         a.parts = (a.tiles - a.whole) * kWaves * kRows;
     } else {   // full rounds of the chip, and the rest's keys in shares
