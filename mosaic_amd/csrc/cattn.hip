@@ -859,6 +859,13 @@ bool few(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     return rows <= kFewRows && (int64_t)nq * K <= kFewEntries;
 }
 
+// Whether the tokens' order is looked for: its two launches cost 7 us and more, and unions of tokens in no order cost
+// less up to about 8192 entries of all heads (scattered tokens, 3 kv heads: 40 of 16 blocks 24 us, 31 with the launches;
+// 500 of 4 blocks 30 and 35; 200 of 16 blocks, 9600 entries, 37 and 37; 500 of 16 blocks 54 and 37).
+bool ordered(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
+    return K > 0 && !few(c, nq, hq, K) && (double)c.num_kv_heads * c.batch * nq * K > 8192.;
+}
+
 template <int WAVES>
 const void* few_kernel(bool fp8, bool sets) {
     return fp8 ? (sets ? (const void*)&cache_attn_few_kernel<true, false, WAVES> : (const void*)&cache_attn_few_kernel<true, true, WAVES>)
@@ -887,7 +894,8 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     } else if (K > 0) {
         // Shares where there are few tiles: of a union that may be as many blocks as the tile's tokens have entries, three
         // workgroups a CU, two where the join is one of teams (16 blocks of 64 a token: 17 scattered tokens 17 us,
-        // 26 in 16 shares; 40 32, 41 in 16; 200 33, 35 in 36; 1000 39, 73 in one; 3500 57 in one or two)
+        // 26 in 16 shares; 40, their order looked for, 32 and 41 in 16; 200 33 and 35 in 36; 1000 39 and 73 in one; 3500 57
+        // in one or two)
         const int64_t per = kWaves * (kRows / G), tokens = std::min<int64_t>(nq, per);
         a.qtiles = (nq + per - 1) / per;
         a.tiles = a.qtiles * heads;
@@ -936,7 +944,7 @@ extern "C" {
 size_t mosaic_cache_attn_fwd_workspace_size(const mosaic_kv_cache* cache, int32_t num_queries, int32_t num_q_heads, int32_t block_count) {
     if (check_call(cache, num_queries, num_q_heads, kHeadDim, block_count) != MOSAIC_OK) return 0;
     return plan_of(*cache, num_queries, num_q_heads, block_count).bytes +
-           (block_count > 0 && !few(*cache, num_queries, num_q_heads, block_count) ? order_bytes(cache->batch, num_queries, num_q_heads, cache->num_kv_heads) : 0);
+           (ordered(*cache, num_queries, num_q_heads, block_count) ? order_bytes(cache->batch, num_queries, num_q_heads, cache->num_kv_heads) : 0);
 }
 
 int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int64_t* block_indices, const int32_t* kv_lens,
@@ -971,7 +979,7 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
         if (!small) p.part_at = reinterpret_cast<int64_t*>(ws + plan.part_at);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (block_count > 0 && !small) {
+    if (ordered(*cache, num_queries, num_q_heads, block_count)) {
         place_order(p, ws + plan.bytes);
         if (int e = launch_order(p, s)) return e;
     }
