@@ -14,7 +14,7 @@
 //
 // Two kernels.  Many rows: a workgroup takes 4 or 12 waves x QW = 32 / G tokens of one kv head, a wave the 32 rows
 // (token, head) of its tokens; the codes of 64 keys are converted once, by all of its waves, into operand order in
-// LDS, which each of them reads.  12 heads of 12288 tokens over 49152 keys, 1.86 TFLOP: 1.65 to 1.72 ms, 1080 to 1130
+// LDS, which each of them reads.  12 heads of 12288 tokens over 49152 keys, 1.86 TFLOP: 1.65 to 1.77 ms, 1050 to 1130
 // TF/s, where a bf16 library product of 8192^3 reaches 1200 to 1230 under the same power limit (1.9 GHz: vector ALU 66 %
 // of the cycles, matrix pipe 48 %).  With blocks for each token (49152 tokens, 16 blocks of 64, 12 heads: 0.21 to 0.23
 // ms, 660 to 730 TF/s; 65 % and 32 %) a workgroup walks the union of its tokens' blocks: a quarter of its 67000 cycles
