@@ -69,11 +69,15 @@ struct AttnState {
 // How a tile is computed.  attend_whole: no score exceeds kBound (|q| and the blocks' norms say so), and the
 // reference is 0.  attend_tile: it is 0 too unless a score leaves +- kBound, and moves then, so that a row's bits
 // do not depend on the form, nor so on the rows beside it.  SAFE: for rows that end with a value that is not
-// finite, and for scales of values further than kSpread from w: the reference is the maximum, and a row's
-// accumulators take nothing from a block that it has not, not even 0 * NaN.
+// finite or with a reference past kFar, and for scales of values further than kSpread from w: the reference is the
+// maximum, and a row's accumulators take nothing from a block that it has not, not even 0 * NaN.
 // With these P is 2^-100 at least, 26 bits above the smallest normal number; an overflow of its sums ends in SAFE.
+// An underflow does not show, so it is kept away: a fused score differs from its maximum, a rounded product, by half a
+// unit of the reference, and lv - m is rounded to one; up to kFar that is 2^-9, what P's own rounding is, but of scores past
+// 2^30 it leaves the largest P anywhere from 0 to infinity.
 constexpr float kBound = 80.f;
 constexpr float kSpread = 0x1p20f;
+constexpr float kFar = 0x1p15f;
 
 // x a + b in two roundings
 __device__ __forceinline__ float times_plus(float x, float a, float b) {
@@ -96,7 +100,7 @@ __device__ __forceinline__ bf16x8 weights(const f32x16& s, int s2, float ck, flo
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float x = s[8 * s2 + 2 * i], y = s[8 * s2 + 2 * i + 1];
-        // (of scores past 2^30 the fused form leaves more than fp32's exponents beside their rounded maximum)
+        // (in SAFE the score at the maximum is the maximum, whatever its unit: P is 1 there)
         w[i] = SAFE ? pack_bf16x2(__builtin_amdgcn_exp2f(times_plus(x, ck, ref)), __builtin_amdgcn_exp2f(times_plus(y, ck, ref)))
                           : pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(x, ck, ref)), __builtin_amdgcn_exp2f(fmaf(y, ck, ref)));
     }
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_kernel(CacheAttnPara
         const Row row = my_row();
         const int wave_live = __builtin_amdgcn_ballot_w64(row.live) ? -1 : 0;   // (a wave without rows only stages)
         attend<FP8, DENSE, false, WAVES>(p, L, b, h, n0, split, splits, row, wave_live, w, a);
-        const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide;
+        const bool fine = finite(a.o[0]) && finite(a.o[1]) && a.l - a.l == 0.f && !a.wide && fabsf(a.m) <= kFar;
         const int other = __shfl_xor((int)fine, 32);   // (the other half of the row)
         ok = !row.live || (fine && other);
     }
@@ -702,7 +706,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
         }
     };
     walk(std::false_type{});
-    bool ok = !a.wide && a.l - a.l == 0.f;
+    bool ok = !a.wide && a.l - a.l == 0.f && fabsf(a.m) <= kFar;
 #pragma unroll
     for (int dg = 0; dg < 4; ++dg)
 #pragma unroll

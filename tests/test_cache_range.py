@@ -1,0 +1,72 @@
+"""Attention over the cache where scores, queries and scales are far from ordinary, and what writes leave for autograd."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import mosaic_amd as M
+from kv_cache_model import attention
+from mosaic_amd import _lib
+from test_cache_attn import BF16, E4M3, F32, I8, check, filled, queries, sets
+
+gpu = pytest.mark.gpu
+CODES = pytest.mark.parametrize("code", [I8, E4M3], ids=["int8", "e4m3"])
+F64 = torch.float64
+
+# nq, tokens, query heads, kv heads, block size, entries of a token (0: whole sequences): few rows of one workgroup a head, of
+# shares; many rows whole, in shares, in workgroups of either size; blocks of few rows, in shares, of a chip full of rows
+LAYOUTS = [
+    (1, 200, 4, 1, 64, 0), (3, 64 * 9, 4, 4, 128, 0), (1, 64 * 61, 16, 1, 64, 0), (40, 64 * 12, 4, 1, 64, 0), (37, 64 * 70 + 9, 12, 3, 64, 0),
+    (6500, 500, 16, 1, 64, 0), (3, 64 * 9, 4, 2, 64, 5), (1, 64 * 200, 4, 1, 256, 20), (17, 64 * 40, 4, 2, 64, 16), (4200, 64 * 70, 8, 2, 64, 3),
+]
+
+
+def one_hot(cache, q, scale, idx=None, lens=None):
+    """Rows whose largest score is further above the others than fp32 can be off by hold the value of its key.
+
+    A score of fp32: 72 roundings of 2^-24 of sum |q k|, and 2^-22 of |score| (see ``attention``); beyond twice that, in scores
+    of 2^20 and more, no other key has a weight.  The value: its output's rounding, 2^-8, and 16 of fp32.
+    """
+    got = M.cache_attn(q.cuda(), cache, None if idx is None else idx.cuda(), scale, None if lens is None else lens.cuda())
+    assert got.isfinite().all()
+    got = got.cpu().to(F64)
+    k, v = (t.cpu().to(F64) for t in M.kv_cache_read(cache, dtype=F32))
+    B, Nq, Hq, _ = q.shape
+    Nk, Hk = k.shape[1:3]
+    G, bs, nb = Hq // Hk, cache.block_size, cache.num_blocks
+    sure = 0
+    for b in range(B):
+        end = Nk if lens is None else int(lens[b])
+        for h in range(Hk):
+            ok = (torch.arange(Nk) < end).expand(Nq, Nk)
+            if idx is not None:
+                i, member = idx[b, :, h], torch.zeros(Nq, nb + 1, dtype=torch.bool)
+                member.scatter_(1, torch.where((i < 0) | (i >= nb), nb, i), True)
+                ok = ok & member[:, :nb].repeat_interleave(bs, 1)[:, :Nk]
+            for g in range(h * G, h * G + G):
+                qq = q[b, :, g].to(F64)
+                x = (qq @ k[b, :, h].t()).masked_fill(~ok, -math.inf)
+                top, at = x.topk(2, dim=-1)
+                e = 72 * 2.0 ** -24 * (qq.abs() @ k[b, :, h].abs().t()).masked_fill(~ok, 0.0).amax(-1) + 2.0 ** -22 * top[:, 0].abs()
+                rows = ok.any(-1) & (top[:, 0] - top[:, 1] > 2 * e + 200 / scale)
+                want = v[b, at[:, 0], h]
+                assert bool(((got[b, :, g] - want).abs() <= (2.0 ** -8 + 2.0 ** -20) * want.abs())[rows].all()), (b, h, g)
+                assert not got[b, ~ok.any(-1), g].any()
+                sure += int(rows.sum())
+    assert sure > 0.8 * B * Nq * Hq * (1.0 if idx is None else 0.8)
+
+
+@gpu
+@CODES
+@pytest.mark.parametrize("scale", [3e8, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("nq,n,Hq,Hk,bs,K", LAYOUTS)
+def test_scores_past_fp32_s_units_choose_one_key(nq, n, Hq, Hk, bs, K, scale, code):
+    cache = filled(1, n, Hk, bs, code, seed=nq + n)
+    idx = sets(1, nq, Hk, K, cache.num_blocks) if K else None
+    if nq == 1 and K:
+        idx = idx.clamp(min=0).add(1) % cache.num_blocks
+    one_hot(cache, queries(1, nq, Hq, 31), scale, idx)
+    if nq < 1000:
+        one_hot(cache, queries(1, nq, Hq, 32), scale, idx, torch.tensor([n - n // 4]))
