@@ -44,7 +44,7 @@ struct CacheAttnParams : QuerySets {
     const bf16_t* q; int64_t q_sb, q_sn, q_sh;
     bf16_t* out;               // [B, Nq, Hq, 64]
     float* part_o;             // [splits, parts, 64] (splits > 1): o of a split's keys
-    float2* part_ml;           // [splits, parts] (m, l): 2^m l is the sum of its weights, l in [0.5, 1), or 0
+    float2* part_ml;           // [splits, parts] (m, l): 2^m l is the sum of its weights
     int64_t* part_at;          // [parts] the row that a part belongs to, or -1
     int64_t parts;             // rows that are joined
     int whole;                 // tiles of rows that one workgroup takes with all of their keys
@@ -438,6 +438,17 @@ __device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, 
     }
 }
 
+// A part's sum of weights 2^m l in joins: no weight overflows, whatever m and l are, and parts of one m weigh as their l,
+// also where m's unit is more than the exponent of l (which therefore stays beside m, not in it).
+struct Sum {
+    float m, y;   // l = 2^e y
+    int e;
+    __device__ __forceinline__ explicit Sum(float2 ml) : m(ml.x), y(__builtin_amdgcn_frexp_mantf(ml.y)), e(__builtin_amdgcn_frexp_expf(ml.y)) {}
+    __device__ __forceinline__ float top() const { return y == 0.f ? -INFINITY : m + (float)e; }   // (l = 0: no key)
+    // relative to the largest top
+    __device__ __forceinline__ float weight(float most) const { return y == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - most + (float)e) * y; }
+};
+
 // The result of a row, or its part of it
 __device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row, int64_t part, int split, int splits, float w, AttnState& a) {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
@@ -455,11 +466,7 @@ __device__ __forceinline__ void put_row(const CacheAttnParams& p, const Row& row
         for (int g4 = 0; g4 < 4; ++g4)
             *reinterpret_cast<float4*>(d + 32 * dt + 8 * g4) =
                 make_float4(a.o[dt][4 * g4] * w, a.o[dt][4 * g4 + 1] * w, a.o[dt][4 * g4 + 2] * w, a.o[dt][4 * g4 + 3] * w);
-    if (hh == 0) {
-        int e = 0;
-        const float y = frexpf(l, &e);   // (NaN and infinity stay what they are)
-        p.part_ml[split * p.parts + part] = make_float2(a.m + (float)e, y);
-    }
+    if (hh == 0) p.part_ml[split * p.parts + part] = make_float2(a.m, l);
 }
 
 template <bool FP8, bool DENSE, int WAVES>
@@ -720,11 +727,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
     for (int dg = 0; dg < 4; ++dg)
         *reinterpret_cast<float4*>(&O[wave][r][(16 * dg + 4 * g) ^ (4 * r)]) =
             make_float4(a.o[dg][0] * f * w, a.o[dg][1] * f * w, a.o[dg][2] * f * w, a.o[dg][3] * f * w);
-    if (g == 0) {
-        int e = 0;
-        const float part = frexpf(l, &e);
-        ml[wave][r] = make_float2(a.m + (float)e, part);
-    }
+    if (g == 0) ml[wave][r] = make_float2(a.m, l);
     __syncthreads();
     // 16 threads a row
     const int row = tid / 16, d = 4 * (tid % 16);
@@ -738,12 +741,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
     }
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, part[i].y == 0.f ? -INFINITY : part[i].x);   // l = 0: no key
+    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, Sum(part[i]).top());
     float sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-        const float e = __builtin_amdgcn_exp2f(part[i].x - m) * part[i].y, y = part[i].y == 0.f ? 0.f : e;
+        const float y = Sum(part[i]).weight(m);
         sum += y;
         o.x = fmaf(y, x[i].x, o.x); o.y = fmaf(y, x[i].y, o.y); o.z = fmaf(y, x[i].z, o.z); o.w = fmaf(y, x[i].w, o.w);
     }
@@ -755,11 +758,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
         return;
     }
     *reinterpret_cast<float4*>(p.part_o + (split * p.parts + at) * 64 + d) = make_float4(o.x * y, o.y * y, o.z * y, o.w * y);
-    if (d == 0) {
-        int e = 0;
-        const float f = frexpf(sum, &e);
-        p.part_ml[split * p.parts + at] = make_float2(m + (float)e, f);
-    }
+    if (d == 0) p.part_ml[split * p.parts + at] = make_float2(m, sum);
 }
 
 // ------------------------------------------------------------------ joins
@@ -783,7 +782,8 @@ __global__ __launch_bounds__(TEAM == 64 ? 1024 : kThreads) void cache_attn_join_
     float4 ahead[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) ahead[i] = n > 0 ? o_of(min(i, n - 1)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = ml.y == 0.f ? -INFINITY : ml.x;   // l = 0: no key in that share
+    const Sum share(ml);
+    float m = share.top();
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     if constexpr (TEAM > 1) {
@@ -794,7 +794,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 1024 : kThreads) void cache_attn_join_
 #pragma unroll
         for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     }
-    const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m) * ml.y;
+    const float w = share.weight(m);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](int i, const float4& y) {

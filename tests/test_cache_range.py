@@ -70,3 +70,25 @@ def test_scores_past_fp32_s_units_choose_one_key(nq, n, Hq, Hk, bs, K, scale, co
     one_hot(cache, queries(1, nq, Hq, 31), scale, idx)
     if nq < 1000:
         one_hot(cache, queries(1, nq, Hq, 32), scale, idx, torch.tensor([n - n // 4]))
+
+
+@gpu
+@CODES
+@pytest.mark.parametrize("scale", [1.0, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("nq,n,Hq,Hk,bs,K", LAYOUTS)
+def test_equal_keys_weigh_the_same_in_every_share(nq, n, Hq, Hk, bs, K, scale, code):
+    """Values of keys that are all one key: their mean, however many of them a share or a wave has."""
+    g = torch.Generator().manual_seed(nq + n)
+    k, v = torch.randn(1, 1, Hk, 64, generator=g).expand(1, n, Hk, 64), torch.randn(1, n, Hk, 64, generator=g) + 1
+    cache = M.KVCache(1, n, Hk, block_size=bs, dtype=code)
+    M.kv_cache_write(cache, k.cuda(), v.cuda())
+    idx = sets(1, nq, Hk, K, cache.num_blocks) if K else None
+    if nq == 1 and K:
+        idx = idx.clamp(min=0).add(1) % cache.num_blocks
+    q, values = queries(1, nq, Hq, 33), M.kv_cache_read(cache, dtype=F32)[1].cpu()
+    for lens in (n, n - n // 3 - 1):
+        lens = torch.tensor([lens])
+        got = M.cache_attn(q.cuda(), cache, None if idx is None else idx.cuda(), scale, lens.cuda()).cpu().to(F64)
+        # scores of 0 are the same softmax; equal scores are equal in fp32 too, so their errors do not enter
+        want, tol = attention(torch.zeros_like(q), torch.zeros(1, n, Hk, 64), values, scale, lens, idx, bs)
+        assert bool(((got - want).abs() <= tol).all()), ((got - want).abs() / tol.clamp(min=1e-300)).max().item()
