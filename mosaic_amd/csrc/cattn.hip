@@ -299,7 +299,8 @@ struct Walk {
             expand(L.tile[buf].V + at, r.x[1]);
         } else expand((first_run() == 0 ? L.tile[buf].K : L.tile[buf].V) + at, r.x[0]);
     }
-    // c |q| of the wave's rows at most, a little more than its roundings (a NaN stays)
+    // c |q| of the wave's rows at most, a little more than its roundings (a NaN stays).  Elements below 2^-63, whose squares
+    // leave fp32, add 8 * 2^-63 to |q| at most: nothing beside 80 but where c is large.
     __device__ __forceinline__ float bound() const {
         float square = 0.f;
 #pragma unroll
@@ -309,7 +310,7 @@ struct Walk {
 #pragma unroll
             for (int i = 0; i < 4; ++i) square = fmaf(bf_lo(x[i]), bf_lo(x[i]), fmaf(bf_hi(x[i]), bf_hi(x[i]), square));
         }
-        return sqrtf(wave_max_nonneg(xor32_add(square))) * p.c * 1.001f;
+        return (sqrtf(wave_max_nonneg(xor32_add(square))) + 0x1p-60f) * p.c * 1.001f;
     }
     // up to 64 blocks, lane i < count holding the i-th and its members among the wave's tokens
     __device__ __forceinline__ void blocks(int count, int block, int members) {

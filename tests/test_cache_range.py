@@ -92,3 +92,22 @@ def test_equal_keys_weigh_the_same_in_every_share(nq, n, Hq, Hk, bs, K, scale, c
         # scores of 0 are the same softmax; equal scores are equal in fp32 too, so their errors do not enter
         want, tol = attention(torch.zeros_like(q), torch.zeros(1, n, Hk, 64), values, scale, lens, idx, bs)
         assert bool(((got - want).abs() <= tol).all()), ((got - want).abs() / tol.clamp(min=1e-300)).max().item()
+
+
+@gpu
+@CODES
+@pytest.mark.parametrize("size", [2.0 ** -64, 2.0 ** -76, 2.0 ** -90], ids=["2^-64", "2^-76", "2^-90"])
+@pytest.mark.parametrize("K", [0, 3])
+@pytest.mark.parametrize("nq", [1, 40, 700])
+def test_queries_near_nothing_with_large_scales(nq, K, size, code):
+    """Scores of hundreds, all of them below zero for half of the rows, from queries whose squares leave fp32."""
+    n = 64 * 12
+    g = torch.Generator().manual_seed(34)
+    k, v = torch.randn(2, 1, n, 1, 64, generator=g)
+    k[..., 0] = 30.0
+    cache = M.KVCache(1, n, 1, dtype=code)
+    M.kv_cache_write(cache, k.cuda(), v.cuda())
+    q = queries(1, nq, 4, 35).float()
+    q[..., 0] = torch.tensor([-8.0, 8.0, -16.0, -3.0])
+    idx = sets(1, nq, 1, K, 12).clamp(min=0) if K else None
+    check(cache, (q * size).to(BF16), idx, scale=1.0 / size)
