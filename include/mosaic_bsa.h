@@ -578,8 +578,8 @@ MOSAIC_API int mosaic_kv_cache_read(const mosaic_kv_cache* cache, int32_t dtype,
    What a row has not chosen does not reach it, whatever it holds.  q: bf16 [B, Nq, Hq, 64]; block_indices: int64
    [B, Nq, Hk, block_count] contiguous, or NULL (block_count 0); out: bf16 [B, Nq, Hq, 64] contiguous.  At most
    16 query heads per kv head, block_count at most 1024.  workspace: mosaic_cache_attn_fwd_workspace_size()
-   bytes, 256-byte aligned (0: none).  softmax_scale <= 0 selects 64^-0.5; others lie within 1e-30 .. 1e30.  It
-   has no counterpart in the reference. */
+   bytes, 256-byte aligned (0: none).  softmax_scale <= 0 selects 64^-0.5; others lie within 1e-30 .. 1e30.  Scores
+   are fp32: a row with some past its range (2e38) is not defined.  It has no counterpart in the reference. */
 MOSAIC_API size_t mosaic_cache_attn_fwd_workspace_size(const mosaic_kv_cache* cache, int32_t num_queries,
                                                        int32_t num_q_heads, int32_t block_count);
 MOSAIC_API int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int64_t* block_indices,

@@ -62,15 +62,18 @@ struct SetsLds : UnionLds { CacheTile tile[2]; };
 struct AttnState {
     f32x16 o[2];      // O^T [dim tile]
     float m, l;       // reference of the scores, and this lane's part of the sum
+    float c;          // SAFE: the factor of the row's scores
     bool has;         // a key above -inf was met
-    bool wide;        // so was a scale of values that SAFE is for
+    bool wide;        // so was a scale of values, or a query, that SAFE is for
 };
 
 // How a tile is computed.  attend_whole: no score exceeds kBound (|q| and the blocks' norms say so), and the
 // reference is 0.  attend_tile: it is 0 too unless a score leaves +- kBound, and moves then, so that a row's bits
 // do not depend on the form, nor so on the rows beside it.  SAFE: for rows that end with a value that is not
-// finite or with a reference past kFar, and for scales of values further than kSpread from w: the reference is the
-// maximum, and a row's accumulators take nothing from a block that it has not, not even 0 * NaN.
+// finite or with a reference past kFar, for scales of values further than kSpread from w, and for queries of a norm of 2^63 or
+// more: the reference is the maximum, and a row's accumulators take nothing from a block that it has not, not even 0 * NaN.
+// A query with an element of 2^80 or more goes into it times 2^-32, and its scores' factor times 2^32: with codes in the
+// place of keys its products would leave fp32 where the scores do not.
 // With these P is 2^-100 at least, 26 bits above the smallest normal number; an overflow of its sums ends in SAFE.
 // An underflow does not show, so it is kept away: a fused score differs from its maximum, a rounded product, by half a
 // unit of the reference, and lv - m is rounded to one; up to kFar that is 2^-9, what P's own rounding is, but of scores past
@@ -78,6 +81,8 @@ struct AttnState {
 constexpr float kBound = 80.f;
 constexpr float kSpread = 0x1p20f;
 constexpr float kFar = 0x1p15f;
+constexpr float kLargeQuery = 0x1p126f;                  // (the norm's square)
+constexpr uint16_t kLargeElement = (127 + 80) << 7;      // (bf16's bits)
 
 // x a + b in two roundings
 __device__ __forceinline__ float times_plus(float x, float a, float b) {
@@ -114,14 +119,17 @@ __device__ __forceinline__ float value_unit(const mosaic_kv_cache& c, int b, int
     return vs > 0.f && vs < INFINITY ? vs : 1.f;
 }
 
+// c ks as an fp32 number above 0
+__device__ __forceinline__ float score_factor(float c, float ks) { return fminf(fmaxf(c * ks, FLT_MIN), FLT_MAX); }
+
 // Factors of a block's scales: scores by ck = c ks; P times 2^lv = vs / w, and iv = w / vs for the sum of P (SAFE:
-// lv = vs itself, iv an addend of the scores that is 0 or NaN).  A scale of 0 stands for zeros only: any
-// positive one does.  A NaN among them goes where only the members of the block meet it.
+// ck = ks, as c is a row's own, lv = vs itself, iv an addend of the scores that is 0 or NaN).  A scale of 0 stands for
+// zeros only: any positive one does.  A NaN among them goes where only the members of the block meet it.
 struct Factors { float ck, lv, iv; };
 template <bool SAFE>
 __device__ __forceinline__ Factors factors(float c, float ks, float vs, float w, bool& wide) {
     Factors f;
-    f.ck = ks > 0.f ? fminf(fmaxf(c * ks, FLT_MIN), FLT_MAX) : 1.f;
+    f.ck = ks > 0.f ? (SAFE ? ks : score_factor(c, ks)) : 1.f;
     const float poison = ks - ks;
     wide = false;
     if constexpr (SAFE) {
@@ -136,6 +144,24 @@ __device__ __forceinline__ Factors factors(float c, float ks, float vs, float w,
         f.iv = __builtin_amdgcn_rcpf(of);
     }
     return f;
+}
+
+// Whether an element of a query's operand is kLargeElement or more (infinities and NaN too), the factor of the scores of a
+// row where one is, and its operands then.  (A factor past fp32, c above 2^96, stays in it: products of 2^48 and more
+// are then one key's all the same.)
+__device__ __forceinline__ bool large_query(const bf16x8& f) {
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    const u16x8 x = __builtin_bit_cast(u16x8, f) & (uint16_t)0x7fff;
+    const auto y = __builtin_elementwise_max(x.lo, x.hi);
+    const auto z = __builtin_elementwise_max(y.lo, y.hi);
+    return max(z.x, z.y) >= kLargeElement;
+}
+__device__ __forceinline__ float row_factor(float c, bool large) { return large ? fminf(c * 0x1p32f, FLT_MAX) : c; }
+__device__ __forceinline__ bf16x8 within(const bf16x8& f, bool large) {
+    const uint4 u = __builtin_bit_cast(uint4, f);
+    const float by = large ? 0x1p-32f : 1.f;
+    auto times = [&](uint32_t x) { return pack_bf16x2(bf_lo(x) * by, bf_hi(x) * by); };
+    return as_bf16x8(make_uint4(times(u.x), times(u.y), times(u.z), times(u.w)));
 }
 
 // The first of a share's units, where the first shares take one more
@@ -171,7 +197,8 @@ __device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mt = __builtin_elementwise_maximum(mt, s[kt][e]);
-    mt = xor32_max(mt) * f.ck;
+    const float ck = SAFE ? score_factor(a.c, f.ck) : f.ck;
+    mt = xor32_max(mt) * ck;
     const bool some = member && mt > -INFINITY;
     const bool move = some && (SAFE ? !a.has || mt > a.m : mt > a.m + kBound || (!a.has && mt < -kBound));
     if (__builtin_amdgcn_ballot_w64(move)) {
@@ -189,7 +216,7 @@ __device__ __forceinline__ void attend_tile(const CacheTile& tile, const bf16x8 
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-            pb[kt][s2] = weights<SAFE>(s[kt], s2, f.ck, ref);
+            pb[kt][s2] = weights<SAFE>(s[kt], s2, ck, ref);
             lt = operand_sum(pb[kt][s2], lt);
         }
     if constexpr (SAFE) {
@@ -299,9 +326,8 @@ struct Walk {
             expand(L.tile[buf].V + at, r.x[1]);
         } else expand((first_run() == 0 ? L.tile[buf].K : L.tile[buf].V) + at, r.x[0]);
     }
-    // c |q| of the wave's rows at most, a little more than its roundings (a NaN stays).  Elements below 2^-63, whose squares
-    // leave fp32, add 8 * 2^-63 to |q| at most: nothing beside 80 but where c is large.
-    __device__ __forceinline__ float bound() const {
+    // |q|^2 of the lane's row
+    __device__ __forceinline__ float norm_square() const {
         float square = 0.f;
 #pragma unroll
         for (int ds = 0; ds < 4; ++ds) {
@@ -310,8 +336,11 @@ struct Walk {
 #pragma unroll
             for (int i = 0; i < 4; ++i) square = fmaf(bf_lo(x[i]), bf_lo(x[i]), fmaf(bf_hi(x[i]), bf_hi(x[i]), square));
         }
-        return (sqrtf(wave_max_nonneg(xor32_add(square))) + 0x1p-60f) * p.c * 1.001f;
+        return xor32_add(square);
     }
+    // c |q| of the wave's rows at most, a little more than its roundings (a NaN stays).  Elements below 2^-63, whose squares
+    // leave fp32, add 8 * 2^-63 to |q| at most: nothing beside 80 but where c is large.
+    __device__ __forceinline__ float bound(float square) const { return (sqrtf(wave_max_nonneg(square)) + 0x1p-60f) * p.c * 1.001f; }
     // up to 64 blocks, lane i < count holding the i-th and its members among the wave's tokens
     __device__ __forceinline__ void blocks(int count, int block, int members) {
         const int64_t at = block_at(p.cache, b, block, h);
@@ -324,9 +353,11 @@ struct Walk {
         if constexpr (!SAFE) {
             for (uint64_t far = __builtin_amdgcn_ballot_w64(wide); far != 0; far &= far - 1)
                 a.wide = a.wide || DENSE || row.in((uint32_t)__builtin_amdgcn_readlane(members, (int)__builtin_ctzll(far)));
+            const float square = norm_square();
+            a.wide = a.wide || !(square < kLargeQuery);
             // (a NaN is not bounded; a wave by itself: the barriers are the same)
             // (and a wave without rows only stages)
-            bounded = __builtin_amdgcn_ballot_w64(!(norm * bound() <= kBound) || a.m != 0.f || (DENSE && members == 0)) == 0;
+            bounded = __builtin_amdgcn_ballot_w64(!(norm * bound(square) <= kBound) || a.m != 0.f || (DENSE && members == 0)) == 0;
         }
         count = __builtin_amdgcn_readfirstlane(count);
         // Tile t is part t % sub of block t / sub; only the sequence's last one may be short.
@@ -416,6 +447,15 @@ __device__ __forceinline__ void attend(const CacheAttnParams& p, Lds& L, int b, 
         const bf16_t* qr = p.q + b * p.q_sb + row.n * p.q_sn + row.head * p.q_sh + 16 * (lane >> 5);
 #pragma unroll
         for (int ds = 0; ds < 4; ++ds) qf[ds] = as_bf16x8(ld16(qr + 32 * (ds >> 1) + 8 * (ds & 1)));
+        if constexpr (SAFE) {
+            bool large = false;
+#pragma unroll
+            for (int ds = 0; ds < 4; ++ds) large = large || large_query(qf[ds]);
+            large = __builtin_amdgcn_ballot_w64(large) >> (lane & 31) & 0x100000001ull;   // (either half of the row)
+            a.c = row_factor(p.c, large);
+#pragma unroll
+            for (int ds = 0; ds < 4; ++ds) qf[ds] = within(qf[ds], large);
+        }
     };
     Walk<FP8, DENSE, SAFE, WAVES, Lds> walk{p, L, b, h, end, w, qf, row, a};
     const int live = (int)(((int64_t)end + p.bs - 1) / p.bs);   // blocks with a key
@@ -581,7 +621,8 @@ __device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2]
     for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mt = __builtin_elementwise_maximum(mt, s[m][i]);
-    mt = xor32_max(xor16_max(mt)) * f.ck;
+    const float ck = SAFE ? score_factor(c, f.ck) : f.ck;
+    mt = xor32_max(xor16_max(mt)) * ck;
     const bool some = member && mt > -INFINITY, move = some && (!a.has || mt > a.m + (SAFE ? 0.f : kTau));
     if (__builtin_amdgcn_ballot_w64(move)) {
         const float alpha = move && a.has ? __builtin_amdgcn_exp2f(a.m - mt) : 1.f;
@@ -592,7 +633,7 @@ __device__ __forceinline__ void attend_few(const Codes& t, const bf16x8 (&qf)[2]
     }
     a.has = a.has || some;
     const float ref = member ? (SAFE ? f.iv : f.lv) - a.m : -INFINITY;   // P = 0 for the others
-    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(SAFE ? times_plus(x, f.ck, ref) : fmaf(x, f.ck, ref)); };
+    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(SAFE ? times_plus(x, ck, ref) : fmaf(x, ck, ref)); };
     // P in two terms, 16 bits of it: the products wait for the codes, and a single row does not average the rounding
     bf16x8 pb[2], rest[2];
     float lt = 0.f;
@@ -690,7 +731,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
         t.vs = p.cache.v_scale[at];
     };
     FewState a;
-    float w = value_unit(p.cache, b, h);
+    float w = value_unit(p.cache, b, h), c = p.c;
     auto walk = [&](auto safe) {
 #pragma unroll
         for (int dg = 0; dg < 4; ++dg) a.o[dg] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -710,17 +751,22 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
                 load(min(key_next, end - 1), next);
             }
             if (key0 < end)
-                attend_few<FP8, decltype(safe)::value>(t, qf, row_live && (DENSE || (of >> token & 1)), min(64, end - key0), p.c, w, a);
+                attend_few<FP8, decltype(safe)::value>(t, qf, row_live && (DENSE || (of >> token & 1)), min(64, end - key0), c, w, a);
         }
     };
     walk(std::false_type{});
-    bool ok = !a.wide && a.l - a.l == 0.f && fabsf(a.m) <= kFar;
+    bool large = large_query(qf[0]) || large_query(qf[1]);
+    bool ok = !a.wide && !large && a.l - a.l == 0.f && fabsf(a.m) <= kFar;
 #pragma unroll
     for (int dg = 0; dg < 4; ++dg)
 #pragma unroll
         for (int i = 0; i < 4; ++i) ok = ok && a.o[dg][i] - a.o[dg][i] == 0.f;
     if (__builtin_amdgcn_ballot_w64(!ok)) {   // (a wave by itself)
         w = 1.f;
+        large = __builtin_amdgcn_ballot_w64(large) >> r & 0x1000100010001ull;   // (any part of the row)
+        c = row_factor(p.c, large);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qf[i] = within(qf[i], large);
         walk(std::true_type{});
     }
     const float l = xor32_add(xor16_add(a.l)), f = l == 0.f ? 0.f : 1.f / l;

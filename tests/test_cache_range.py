@@ -111,3 +111,21 @@ def test_queries_near_nothing_with_large_scales(nq, K, size, code):
     q[..., 0] = torch.tensor([-8.0, 8.0, -16.0, -3.0])
     idx = sets(1, nq, 1, K, 12).clamp(min=0) if K else None
     check(cache, (q * size).to(BF16), idx, scale=1.0 / size)
+
+
+@gpu
+@CODES
+@pytest.mark.parametrize("large,small,scale", [(1e36, 1e-28, 1e-9), (2e37, 1e-26, 1e-12), (1e33, 1e-29, 1e-30), (3e34, 1e-29, 1e-30), (1e30, 1.0, 1e-30), (1e36, 1e4, 1e-30), (1e25, 1.0, 1e-25)])
+@pytest.mark.parametrize("K", [0, 3])
+@pytest.mark.parametrize("nq", [1, 40, 700])
+def test_queries_whose_products_with_codes_leave_fp32(nq, K, large, small, scale, code):
+    """Ordinary scores of large queries with small keys or scales, beside rows of ordinary queries (scores of nothing)."""
+    n = 64 * 12
+    g = torch.Generator().manual_seed(36)
+    k, v = torch.randn(2, 1, n, 1, 64, generator=g)
+    cache = M.KVCache(1, n, 1, dtype=code)
+    M.kv_cache_write(cache, (k * small).cuda(), v.cuda())
+    q = queries(1, nq, 4, 37).float()
+    q[:, :, :3] *= large
+    q[:, 1::3] = queries(1, nq, 4, 38)[:, 1::3].float()
+    check(cache, q.to(BF16), sets(1, nq, 1, K, 12).clamp(min=0) if K else None, scale=scale)
