@@ -874,21 +874,6 @@ __global__ __launch_bounds__(TEAM == 64 ? 1024 : kThreads) void cache_attn_join_
 
 // ------------------------------------------------------------------ host
 
-int check_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, int32_t K) {
-    if (int e = check_cache(cache)) return e;
-    if (nq <= 0) return MOSAIC_ERR_SHAPE;
-    if (d != kHeadDim) return MOSAIC_ERR_HEAD_DIM;
-    if (hq <= 0 || hq % cache->num_kv_heads) return MOSAIC_ERR_HEADS;
-    const int G = hq / cache->num_kv_heads;
-    if (G > 16 || K > kMaxSelected) return MOSAIC_ERR_UNSUPPORTED;
-    if (K < 0) return MOSAIC_ERR_BLOCK_COUNT;
-    // ids of workgroups stay in 31 bits
-    const int64_t per = kWaves * (kRows / G), tiles = ((int64_t)nq + per - 1) / per;
-    if ((double)tiles * cache->num_kv_heads * cache->batch * kMaxSplit > 2147483647.0 || nq > 0x7fffffff - 1024) return MOSAIC_ERR_SHAPE;
-    if (((double)nq / kKeyTokens + 1) * cache->num_kv_heads * cache->batch > 2147483647.0) return MOSAIC_ERR_SHAPE;
-    return MOSAIC_OK;
-}
-
 // Shares of the keys of few rows: four workgroups a CU, where a row has no more than kFewShares then, and else one a
 // CU: its join is the longer (one point over 196608 keys, 75 MB in e4m3: 20.5 us in 85 shares of each head, 23.3 in
 // 170 and in 341; 24 tracks of 16 heads, 113 MB in int8: 25 us in 10 shares, 29 in 2).  One share and no join up to
@@ -927,7 +912,9 @@ const void* few_kernel(bool fp8, bool sets) {
 struct Plan {
     int waves;
     int64_t qtiles, tiles, whole, splits, parts;   // tiles of a (member, kv head), and of all; rows that are joined
-    size_t part_o, part_ml, part_at, bytes;        // places in the workspace, and what the partials take of it
+    size_t part_o, part_ml, part_at, bytes;        // places in the workspace, and what the partials take of it; then
+    size_t order;                                  // bytes of the tokens' order (0: they stay in their own)
+    int64_t groups() const { return whole + (tiles - whole) * splits; }
 };
 Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     Plan a{};
@@ -985,6 +972,24 @@ Plan plan_of(const mosaic_kv_cache& c, int32_t nq, int32_t hq, int32_t K) {
     return a;
 }
 
+// A call's checks that need no pointer, and its plan
+int plan_call(const mosaic_kv_cache* cache, int32_t nq, int32_t hq, int32_t d, int32_t K, Plan& plan) {
+    if (int e = check_cache(cache)) return e;
+    if (nq <= 0) return MOSAIC_ERR_SHAPE;
+    if (d != kHeadDim) return MOSAIC_ERR_HEAD_DIM;
+    const int hk = cache->num_kv_heads;
+    if (hq <= 0 || hq % hk) return MOSAIC_ERR_HEADS;
+    if (hq / hk > 16 || K > kMaxSelected) return MOSAIC_ERR_UNSUPPORTED;
+    if (K < 0) return MOSAIC_ERR_BLOCK_COUNT;
+    if (nq > 0x7fffffff - 1024) return MOSAIC_ERR_SHAPE;   // (tokens past the last stay in 31 bits)
+    plan = plan_of(*cache, nq, hq, K);
+    if (!grid_fits(plan.groups(), 64 * plan.waves)) return MOSAIC_ERR_SHAPE;
+    plan.order = ordered(*cache, nq, hq, K) ? order_bytes(cache->batch, nq, hq, hk) : 0;
+    const int64_t heads = (int64_t)cache->batch * hk;
+    if (plan.order > 0 && (!grid_fits(heads * key_chunks(nq), kThreads) || !grid_fits(heads, kOrderThreads))) return MOSAIC_ERR_SHAPE;
+    return MOSAIC_OK;
+}
+
 }  // namespace
 }  // namespace mosaic
 
@@ -993,21 +998,22 @@ using namespace mosaic;
 extern "C" {
 
 size_t mosaic_cache_attn_fwd_workspace_size(const mosaic_kv_cache* cache, int32_t num_queries, int32_t num_q_heads, int32_t block_count) {
-    if (check_call(cache, num_queries, num_q_heads, kHeadDim, block_count) != MOSAIC_OK) return 0;
-    return plan_of(*cache, num_queries, num_q_heads, block_count).bytes +
-           (ordered(*cache, num_queries, num_q_heads, block_count) ? order_bytes(cache->batch, num_queries, num_q_heads, cache->num_kv_heads) : 0);
+    Plan plan;
+    if (plan_call(cache, num_queries, num_q_heads, kHeadDim, block_count, plan) != MOSAIC_OK) return 0;
+    return plan.bytes + plan.order;
 }
 
 int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int64_t* block_indices, const int32_t* kv_lens,
                           int32_t num_queries, int32_t num_q_heads, int32_t head_dim, int32_t block_count, float softmax_scale,
                           void* out, void* workspace, size_t workspace_bytes, void* stream) {
-    if (int e = check_call(cache, num_queries, num_q_heads, head_dim, block_count)) return e;
+    Plan plan;
+    if (int e = plan_call(cache, num_queries, num_q_heads, head_dim, block_count, plan)) return e;
     if (!scale_ok(softmax_scale)) return MOSAIC_ERR_UNSUPPORTED;
     if (q.ptr == nullptr || out == nullptr) return MOSAIC_ERR_NULL_POINTER;
     if ((block_indices == nullptr) != (block_count == 0)) return MOSAIC_ERR_BLOCK_COUNT;
     if (!aligned(q.ptr, 16) || q.stride_b % 8 || q.stride_n % 8 || q.stride_h % 8) return MOSAIC_ERR_ALIGNMENT;
     if (!aligned(block_indices, 8) || !aligned(out, 16) || !aligned(kv_lens, 4)) return MOSAIC_ERR_ALIGNMENT;
-    const size_t need = mosaic_cache_attn_fwd_workspace_size(cache, num_queries, num_q_heads, block_count);
+    const size_t need = plan.bytes + plan.order;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256))) return MOSAIC_ERR_WORKSPACE;
     CacheAttnParams p{};
     p.cache = *cache;
@@ -1016,9 +1022,6 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     p.B = cache->batch; p.Nq = num_queries; p.Nk = cache->capacity; p.Hq = num_q_heads; p.Hk = cache->num_kv_heads;
     p.G = p.Hq / p.Hk; p.QW = kRows / p.G; p.bs = cache->block_size; p.K = block_count; p.nb = cache->num_blocks;
     p.qw_inverse = (65536 + p.QW - 1) / p.QW;
-    const Plan plan = plan_of(*cache, num_queries, num_q_heads, block_count);
-    const int64_t groups = plan.whole + (plan.tiles - plan.whole) * plan.splits;
-    if (!grid_fits(groups, 64 * plan.waves)) return MOSAIC_ERR_SHAPE;
     p.qtiles = (int)plan.qtiles; p.splits = (int)plan.splits; p.whole = (int)plan.whole; p.parts = plan.parts;
     p.out = static_cast<bf16_t*>(out);
     p.c = (softmax_scale > 0.f ? softmax_scale : 0.125f) * kLog2e;
@@ -1030,7 +1033,7 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
         if (!small) p.part_at = reinterpret_cast<int64_t*>(ws + plan.part_at);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (ordered(*cache, num_queries, num_q_heads, block_count)) {
+    if (plan.order > 0) {
         place_order(p, ws + plan.bytes);
         if (int e = launch_order(p, s)) return e;
     }
@@ -1042,7 +1045,7 @@ int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int
     else if (sets) fn = fp8 ? (const void*)&cache_attn_kernel<true, false, 4> : (const void*)&cache_attn_kernel<false, false, 4>;
     else if (plan.waves == 12) fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 12> : (const void*)&cache_attn_kernel<false, true, 12>;
     else fn = fp8 ? (const void*)&cache_attn_kernel<true, true, 4> : (const void*)&cache_attn_kernel<false, true, 4>;
-    if (launch(fn, dim3((unsigned)groups), args, s, 64 * plan.waves) != hipSuccess) return MOSAIC_ERR_LAUNCH;
+    if (launch(fn, dim3((unsigned)plan.groups()), args, s, 64 * plan.waves) != hipSuccess) return MOSAIC_ERR_LAUNCH;
     if (p.splits == 1) return MOSAIC_OK;
     void* jargs[] = {&p};
     const int team = p.splits <= 16 ? 1 : p.splits <= 64 ? 16 : 64;

@@ -129,3 +129,21 @@ def test_queries_whose_products_with_codes_leave_fp32(nq, K, large, small, scale
     q[:, :, :3] *= large
     q[:, 1::3] = queries(1, nq, 4, 38)[:, 1::3].float()
     check(cache, q.to(BF16), sets(1, nq, 1, K, 12).clamp(min=0) if K else None, scale=scale)
+
+
+FAKE = 1 << 20
+
+
+def c_cache(batch, num_blocks, heads, capacity):
+    return ctypes.byref(_lib.Cache(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, batch, num_blocks, heads, 64, _lib.CODE_INT8, capacity))
+
+
+@pytest.mark.parametrize("batch,heads,nq,hq,K", [
+    (1, 64, 1 << 23, 64, 4),            # 2^24 workgroups of 256 threads would look for the tokens' order, 2^22 attend
+    (1 << 18, 16, 9, 256, 1),           # 2^22 workgroups of 1024 threads would make it, 2^23 of 256 attend
+])
+def test_launches_of_the_order_that_cannot_be_counted_are_refused(batch, heads, nq, hq, K):
+    L, c = _lib.lib(), c_cache(batch, 4, heads, 250)
+    assert L.mosaic_cache_attn_fwd_workspace_size(c, nq, hq, K) == 0
+    rows = _lib.Bnhd(FAKE, nq * hq * 64, hq * 64, 64)
+    assert L.mosaic_cache_attn_fwd(rows, c, FAKE, None, nq, hq, 64, K, 0.0, FAKE, FAKE, 1 << 62, None) == 8
