@@ -462,7 +462,7 @@ int check_run(const mosaic_kv_cache* cache, int32_t dtype, int32_t head_dim, int
     if (head_dim != kHeadDim) return MOSAIC_ERR_HEAD_DIM;
     if (dtype != MOSAIC_DTYPE_BF16 && dtype != MOSAIC_DTYPE_F32) return MOSAIC_ERR_UNSUPPORTED;
     if (n <= 0) return MOSAIC_ERR_SHAPE;
-    if (starts == nullptr && (start < 0 || start + n > cache->capacity)) return MOSAIC_ERR_SHAPE;
+    if (starts == nullptr && (start < 0 || start > (int64_t)cache->capacity - n)) return MOSAIC_ERR_SHAPE;
     if (!aligned(starts, 4) || !aligned(counts, 4)) return MOSAIC_ERR_ALIGNMENT;
     return MOSAIC_OK;
 }

@@ -147,3 +147,10 @@ def test_launches_of_the_order_that_cannot_be_counted_are_refused(batch, heads, 
     assert L.mosaic_cache_attn_fwd_workspace_size(c, nq, hq, K) == 0
     rows = _lib.Bnhd(FAKE, nq * hq * 64, hq * 64, 64)
     assert L.mosaic_cache_attn_fwd(rows, c, FAKE, None, nq, hq, 64, K, 0.0, FAKE, FAKE, 1 << 62, None) == 8
+
+
+@pytest.mark.parametrize("start", [(1 << 63) - 1, (1 << 63) - 5, 246, -1, -1 << 63])
+def test_starts_whose_end_leaves_64_bits_are_refused(start):
+    L, c, rows = _lib.lib(), c_cache(2, 4, 3, 250), _lib.Bnhd(FAKE, 960, 192, 64)
+    assert L.mosaic_kv_cache_write(c, rows, rows, 1, 64, 5, start, None, None, None) == 8
+    assert L.mosaic_kv_cache_read(c, 1, 64, 5, start, None, FAKE, FAKE, None) == 8
