@@ -47,7 +47,7 @@ class KVCache:
     ``v_scale`` (float32 [batch, num_blocks, kv_heads]), ``k_mean`` (bfloat16 [batch, num_blocks, kv_heads,
     64], the mean of the keys of each block: ``k_cmp`` of ``query_topk``), ``k_norm`` (float32 as the scales, the
     largest norm of a key of the block) and the codes, in an order of the library's
-    own, are tensors of the cache: ``kv_cache_write`` changes them in place.
+    own, are tensors of the cache: ``kv_cache_write`` changes them in place, as autograd sees.
     """
 
     def __init__(self, batch: int, capacity: int, kv_heads: int, block_size: int = 64, dtype: torch.dtype = torch.int8,
@@ -75,11 +75,12 @@ class KVCache:
         """The storage as the library takes it: made once, the tensors being the cache's own for its life."""
         B, nb, Hk, bs, capacity = self._sizes
         self._device = self._k_codes.device
+        self._tensors = (self._k_codes, self._v_codes, self._k_scale, self._v_scale, self._k_norm, self._k_mean)
         self._c = _lib.Cache(self._k_codes.data_ptr(), self._v_codes.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr(),
                              self._k_norm.data_ptr(), self._k_mean.data_ptr(), B, nb, Hk, bs, _CODES[self._dtype], capacity)
 
     def __getstate__(self) -> dict:   # (copies and pickles: of the tensors, not of where they lie)
-        return {name: x for name, x in self.__dict__.items() if name not in ("_c", "_device")}
+        return {name: x for name, x in self.__dict__.items() if name not in ("_c", "_device", "_tensors")}
 
     def __setstate__(self, state: dict) -> None:
         self.__dict__.update(state)
@@ -180,6 +181,7 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: int 
     with _on(device):
         st = _lib.lib().mosaic_kv_cache_write(ctypes.byref(cache._c), kb, vb, _DT[dtype], 64, n, start, _ptr(starts), _ptr(counts), _stream(device))
     _lib.check(st, "mosaic_kv_cache_write")
+    torch.autograd.graph.increment_version(cache._tensors)   # (what was saved of them for a backward is no longer there)
 
 
 def kv_cache_read(cache: KVCache, start: int | torch.Tensor = 0, count: int | None = None,

@@ -154,3 +154,38 @@ def test_starts_whose_end_leaves_64_bits_are_refused(start):
     L, c, rows = _lib.lib(), c_cache(2, 4, 3, 250), _lib.Bnhd(FAKE, 960, 192, 64)
     assert L.mosaic_kv_cache_write(c, rows, rows, 1, 64, 5, start, None, None, None) == 8
     assert L.mosaic_kv_cache_read(c, 1, 64, 5, start, None, FAKE, FAKE, None) == 8
+
+
+def held(cache):
+    return [cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale, cache.k_norm, cache.k_mean]
+
+
+@gpu
+def test_writes_are_seen_by_autograd():
+    cache = filled(1, 200, 2, seed=39)
+    w = torch.ones(64, dtype=BF16, device="cuda", requires_grad=True)
+    versions = [t._version for t in held(cache)]
+    y = (w * cache.k_mean).sum()
+    M.kv_cache_read(cache)
+    M.cache_query_attn(queries(1, 3, 2).cuda(), cache, 2)
+    none = torch.zeros(1, 0, 2, 64, dtype=BF16, device="cuda")
+    M.kv_cache_write(cache, none, none)
+    assert [t._version for t in held(cache)] == versions
+    y.backward()                                        # nothing was written
+    y = (w * cache.k_mean).sum()
+    one = torch.ones(1, 1, 2, 64, dtype=BF16, device="cuda")
+    M.kv_cache_write(cache, one, one, 70)
+    assert all(t._version > x for t, x in zip(held(cache), versions))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@gpu
+def test_writes_in_inference_mode():
+    with torch.inference_mode():
+        cache = filled(1, 100, 1, seed=40)
+        k, _ = M.kv_cache_read(cache)
+        M.kv_cache_write(cache, k[:, :64] * 2, k[:, :64], 0)
+    one = torch.ones(1, 1, 1, 64, dtype=BF16, device="cuda")
+    M.kv_cache_write(cache, one, one, 64)
+    assert torch.equal(M.kv_cache_read(cache, 64, 1)[0], one)
