@@ -283,7 +283,9 @@ def cache_query_attn(q: torch.Tensor, cache: KVCache, block_count: int, *, softm
 
     ``mosaic_query_attn`` on a cache: ``query_topk`` against ``cache.k_mean``, which ``kv_cache_write`` keeps,
     then ``cache_attn``.  Blocks that begin at or past ``kv_lens[b]``, and those that ``block_mask`` (bool [B,
-    num_blocks]) leaves out, are not chosen.  With ``return_block_indices`` the choice (int64 [B, Nq,
+    num_blocks]) leaves out, are not chosen.  The mean of the block that a length ends in is that of every token
+    written to it, those past the length too, though the attention leaves them out: lengths are best where the last
+    write ended, which sets that block's mean.  With ``return_block_indices`` the choice (int64 [B, Nq,
     kv_heads, block_count], -1 past the last) is returned too.
     """
     what = "cache_query_attn"

@@ -189,3 +189,25 @@ def test_writes_in_inference_mode():
     one = torch.ones(1, 1, 1, 64, dtype=BF16, device="cuda")
     M.kv_cache_write(cache, one, one, 64)
     assert torch.equal(M.kv_cache_read(cache, 64, 1)[0], one)
+
+
+@gpu
+def test_a_choice_takes_the_means_of_all_that_is_written():
+    """Lengths below what is written: the attention leaves the later tokens out, the last block's mean does not, until it is cut."""
+    g = torch.Generator().manual_seed(41)
+    k, v = torch.randn(2, 1, 192, 1, 64, generator=g)
+    k[0, 70:128] += 4.0                                     # past the length, in the block that it ends in
+    k[0, 128:] += 8.0                                       # a block past the length
+    cache = M.KVCache(1, 192, 1)
+    M.kv_cache_write(cache, k.cuda(), v.cuda())
+    q, lens = torch.ones(1, 2, 1, 64, dtype=BF16).cuda(), torch.tensor([70]).cuda()
+    out, idx = M.cache_query_attn(q, cache, 1, kv_lens=lens, return_block_indices=True)
+    assert torch.equal(idx, M.query_topk(q, cache.k_mean, 1, torch.tensor([[True, True, False]]).cuda())) and bool((idx == 1).all())
+    check(cache, q.cpu(), idx.cpu(), lens.cpu())            # ... over tokens 64 .. 69
+    k[0, :64] += 0.5
+    k[0, 64:70] -= 4.0
+    M.kv_cache_write(cache, k[:, :64].cuda(), v[:, :64].cuda())
+    M.kv_cache_write(cache, k[:, 64:70].cuda(), v[:, 64:70].cuda(), 64)      # the sequence ends there
+    out, idx = M.cache_query_attn(q, cache, 1, kv_lens=lens, return_block_indices=True)
+    assert bool((idx == 0).all())
+    assert torch.equal(out, M.cache_attn(q, cache, idx, kv_lens=lens))
