@@ -173,7 +173,7 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: int 
     start, starts = _run(what, cache, start, n)
     if counts is not None:
         _per_sequence(what, "counts", counts, B)
-    _same_device(what, cache._k_codes, k=k, v=v, start=starts, counts=counts)
+    _same_device(what, cache._k_codes, of="the cache", k=k, v=v, start=starts, counts=counts)
     if n == 0:
         return
     starts, counts = _int32(starts, -1 << 31, (1 << 31) - 1), _int32(counts, 0, n)
@@ -205,7 +205,7 @@ def kv_cache_read(cache: KVCache, start: int | torch.Tensor = 0, count: int | No
     if not 0 <= count < 1 << 31:
         raise ValueError(f"{what}: count must be in [0, 2^31), got {count}")
     start, starts = _run(what, cache, start, count)
-    _same_device(what, cache._k_codes, start=starts)
+    _same_device(what, cache._k_codes, of="the cache", start=starts)
     k = torch.empty(B, count, Hk, 64, dtype=dtype, device=device)
     v = torch.empty_like(k)
     if count == 0:

@@ -60,13 +60,13 @@ def _no_grad_through(what: str, **tensors) -> None:
             raise RuntimeError(f"{what} has no gradient in {name}: pass it detached")
 
 
-def _same_device(what: str, q: torch.Tensor, **tensors) -> None:
+def _same_device(what: str, q: torch.Tensor, *, of: str = "q", **tensors) -> None:
     if not q.is_cuda:
-        raise ValueError(f"{what}: q must be on a ROCm device, got {q.device}")
+        raise ValueError(f"{what}: {of} must be on a ROCm device, got {q.device}")
     index = q.get_device()
     for name, t in tensors.items():
         if t is not None and (t.get_device() != index or not t.is_cuda):
-            raise ValueError(f"{what}: {name} is on {t.device}, q on {q.device}")
+            raise ValueError(f"{what}: {name} is on {t.device}, {of} on {q.device}")
 
 
 _here = contextlib.nullcontext()

@@ -211,3 +211,22 @@ def test_a_choice_takes_the_means_of_all_that_is_written():
     out, idx = M.cache_query_attn(q, cache, 1, kv_lens=lens, return_block_indices=True)
     assert bool((idx == 0).all())
     assert torch.equal(out, M.cache_attn(q, cache, idx, kv_lens=lens))
+
+
+def test_a_cache_in_host_memory_is_named_by_the_refusal():
+    cache, x = M.KVCache(1, 64, 1, device="cpu"), torch.zeros(1, 1, 1, 64)
+    with pytest.raises(ValueError, match="kv_cache_write: the cache must be on a ROCm device, got cpu"):
+        M.kv_cache_write(cache, x, x)
+    with pytest.raises(ValueError, match="kv_cache_read: the cache must be on a ROCm device, got cpu"):
+        M.kv_cache_read(cache)
+
+
+@gpu
+def test_tensors_elsewhere_are_named_by_the_refusal():
+    cache, x = M.KVCache(2, 64, 1), torch.zeros(2, 1, 1, 64)
+    with pytest.raises(ValueError, match="kv_cache_write: k is on cpu, the cache on cuda"):
+        M.kv_cache_write(cache, x, x.cuda())
+    with pytest.raises(ValueError, match="kv_cache_write: counts is on cpu, the cache on cuda"):
+        M.kv_cache_write(cache, x.cuda(), x.cuda(), counts=torch.tensor([1, 1]))
+    with pytest.raises(ValueError, match="kv_cache_read: start is on cpu, the cache on cuda"):
+        M.kv_cache_read(cache, torch.tensor([1, 1]), 1)
