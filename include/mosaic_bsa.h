@@ -575,11 +575,12 @@ MOSAIC_API int mosaic_kv_cache_read(const mosaic_kv_cache* cache, int32_t dtype,
 /* Attention of q over a cache.  Row (b, n, g): the softmax over the keys of sequence b below its length
    kv_lens[b] (optional, clamped to [0, capacity]; NULL: capacity), with block_indices only over those of the
    blocks named in block_indices[b, n, h, :], a set as in mosaic_query_attn_fwd; a row without a key is zeros.
-   What a row has not chosen does not reach it, whatever it holds.  q: bf16 [B, Nq, Hq, 64]; block_indices: int64
+   What a row has not chosen does not reach it, whatever it holds (but for roundings: the scale of the values of the
+   sequence's first block is the unit of the others').  q: bf16 [B, Nq, Hq, 64]; block_indices: int64
    [B, Nq, Hk, block_count] contiguous, or NULL (block_count 0); out: bf16 [B, Nq, Hq, 64] contiguous.  At most
    16 query heads per kv head, block_count at most 1024.  workspace: mosaic_cache_attn_fwd_workspace_size()
    bytes, 256-byte aligned (0: none).  softmax_scale <= 0 selects 64^-0.5; others lie within 1e-30 .. 1e30.  Scores
-   are fp32: a row with some past its range (2e38) is not defined.  It has no counterpart in the reference. */
+   are fp32: a row with some past its range (2e38), or with sums of values past it, is not defined.  It has no counterpart in the reference. */
 MOSAIC_API size_t mosaic_cache_attn_fwd_workspace_size(const mosaic_kv_cache* cache, int32_t num_queries,
                                                        int32_t num_q_heads, int32_t block_count);
 MOSAIC_API int mosaic_cache_attn_fwd(mosaic_bnhd q, const mosaic_kv_cache* cache, const int64_t* block_indices,

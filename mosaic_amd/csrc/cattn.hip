@@ -69,7 +69,10 @@ struct AttnState {
 
 // How a tile is computed.  attend_whole: no score exceeds kBound (|q| and the blocks' norms say so), and the
 // reference is 0.  attend_tile: it is 0 too unless a score leaves +- kBound, and moves then, so that a row's bits
-// do not depend on the form, nor so on the rows beside it.  SAFE: for rows that end with a value that is not
+// do not depend on the form, and on the rows beside it only where a union without an order is cut into shares, by its size.
+// Which form is one decision for a wave's rows and up to 64 blocks (12288 tokens over 49152 keys: 1720 us, 1780 where one
+// token of 100 leaves the bound, 1910 to 1960 where all or a block of each 64 do; the tokens of nside 64 with blocks of
+// their own 213, 211 and 222 to 227).  SAFE: for rows that end with a value that is not
 // finite or with a reference past kFar, for scales of values further than kSpread from w, and for queries of a norm of 2^63 or
 // more: the reference is the maximum, and a row's accumulators take nothing from a block that it has not, not even 0 * NaN.
 // A query with an element of 2^80 or more goes into it times 2^-32, and its scores' factor times 2^32: with codes in the
@@ -113,7 +116,8 @@ __device__ __forceinline__ bf16x8 weights(const f32x16& s, int s2, float ck, flo
 }
 
 // What the scales of values are taken relative to: that of the sequence's first block (1 where that is zeros or
-// not finite), so that it does not depend on what else a workgroup computes.
+// not finite), so that it does not depend on what else a workgroup computes.  Rows without that block follow it by their
+// roundings in fp32, and beyond kSpread by the second pass.
 __device__ __forceinline__ float value_unit(const mosaic_kv_cache& c, int b, int h) {
     const float vs = c.v_scale[block_at(c, b, 0, h)];
     return vs > 0.f && vs < INFINITY ? vs : 1.f;
@@ -761,7 +765,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void cache_attn_few
     for (int dg = 0; dg < 4; ++dg)
 #pragma unroll
         for (int i = 0; i < 4; ++i) ok = ok && a.o[dg][i] - a.o[dg][i] == 0.f;
-    if (__builtin_amdgcn_ballot_w64(!ok)) {   // (a wave by itself)
+    if (__builtin_amdgcn_ballot_w64(!ok)) {   // (a wave by itself, with all of its rows)
         w = 1.f;
         large = __builtin_amdgcn_ballot_w64(large) >> r & 0x1000100010001ull;   // (any part of the row)
         c = row_factor(p.c, large);

@@ -242,7 +242,8 @@ def cache_attn(q: torch.Tensor, cache: KVCache, block_indices: torch.Tensor | No
     1024), to those of the blocks of ``cache.block_size`` tokens named there: a set, as in
     ``query_sparse_attn``.  A token without a key gets zeros.  ``softmax_scale`` defaults to 1/8 and lies
     within 1e-30 .. 1e30.  Scores, sums and accumulators are fp32, the weights rounded to bfloat16, as
-    float32 q is; a row with scores past fp32's range (2e38) is not defined.  There is no gradient.
+    float32 q is; a row with scores, or sums of values over its keys, past fp32's range (2e38) is not
+    defined.  There is no gradient.
     """
     what = "cache_attn"
     _check_queries(what, q, cache, kv_lens)
